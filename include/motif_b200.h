@@ -518,6 +518,66 @@ MB_API int motif_b200_testing_force(int knob, int value);
 MB_API int motif_b200_embed(const int64_t* ids, const void* table, void* out, int64_t rows, int64_t D,
                      int64_t V, int dtype, void* stream);
 
+/* ------------------------------------------------------------------ paged 4-bit cache
+ * A pool [num_pages][Hkv][page_size / 16][unit] of bytes (16-byte aligned; page_size a multiple of
+ * 16 up to 1024; num_pages * page_size < 2^31) holds keys and values in 4 bits.  A unit is 16
+ * consecutive tokens of one kv head, motif_b200_kv4_unit_bytes(D) bytes:
+ *   K codes [16][D/2] | V codes [16][D/2] | K pairs [D/DG][16] | V pairs [D/DG][16], DG = min(D, 64).
+ * Dim 2i of a row is the low nibble of byte i; a group of DG dims of one token has a pair (scale s,
+ * centre m) in bf16, s in the low half of its 32-bit word; code c stands for m + s (c - 8).
+ * block_table [B, max_pages] int32 (row stride table_stride) names each request's pages; slot
+ * numbers are page * page_size + offset.  D in {32, 64, 128}.  No counterpart in the reference. */
+
+/* Slots for new_lens[b] more tokens of each request (lens[b] cached): fresh pages are taken from
+ * the end of free_pages[:*free_count] (capacity free_capacity) in request order and written to
+ * block_table; slots[total_new] gets every new token's slot, request after request, -1 past the
+ * last token and for requests that were not served.  A request is served if its pages fit
+ * max_pages, its tokens fit total_new and the pages asked for up to and including it do not exceed
+ * the free ones (one that needs no page always passes the last test).  lens_out[b] = lens[b] +
+ * new_lens[b] where served, else lens[b]; lens_out / free_count_out may be lens / free_count. */
+MB_API int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_lens, int32_t* block_table,
+                             int64_t table_stride, const int32_t* free_pages,
+                             const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out,
+                             int32_t* slots, int64_t total_new, int64_t B, int64_t max_pages,
+                             int64_t free_capacity, int64_t page_size, void* stream);
+/* The pages of requests with done[b] != 0 go back onto the end of the free list in request order;
+ * their table entries become -1 and their lengths 0. */
+MB_API int motif_b200_paged_release(const uint8_t* done, int32_t* lens, int32_t* block_table,
+                             int64_t table_stride, int32_t* free_pages, int32_t* free_count, int64_t B,
+                             int64_t max_pages, int64_t free_capacity, int64_t page_size, void* stream);
+/* Bytes of one unit for head dim D (0 if there is no kernel for D). */
+MB_API int64_t motif_b200_kv4_unit_bytes(int64_t D);
+/* Quantise the rows of k, v (B x T tokens in (b, t) order, slot slots[b*T + t]; a slot outside the
+ * pool is skipped) and store them: s = bf16((max - min) / 15), m = bf16(min + 8 s), c = 8 + the
+ * nearest whole number (ties to even) to (x - m) / s within -8 .. 7.  k_out / v_out (both or
+ * neither NULL) receive the stored values.  `strides` (elements), [12]: (b, h, t) of k, v, k_out,
+ * v_out; rows 16-byte aligned. */
+MB_API int motif_b200_kv4_append(const void* k, const void* v, const int32_t* slots, void* pool,
+                          void* k_out, void* v_out, const int64_t* strides, int64_t B, int64_t T,
+                          int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size, int dtype,
+                          void* stream);
+/* The first S cached keys and values of every request as contiguous [B, Hkv, S, D] dtype arrays,
+ * zeros at and past lens[b] and where a table entry is no page of the pool. */
+MB_API int motif_b200_kv4_gather(const void* pool, const int32_t* block_table, int64_t table_stride,
+                          const int32_t* lens, void* k_out, void* v_out, int64_t B, int64_t Hkv,
+                          int64_t S, int64_t D, int64_t num_pages, int64_t page_size,
+                          int64_t max_pages, int dtype, void* stream);
+/* Chord attention (motif_b200_chord_attention's logits with log_n = log(position + 1)) of the T
+ * newest tokens of every request over its cache: token t of request b is at position
+ * lens[b] - T + t, or lens[b] - q_lens[b] + t where q_lens != NULL (rows t >= q_lens[b] are
+ * padding).  Rows that see no key are zeros; keys on table entries outside the pool are left out.
+ * `strides` (elements), [6]: (b, h, t) of q, out.  `workspace` (16-byte aligned) holds
+ * motif_b200_kv4_attention_workspace_bytes bytes. */
+MB_API int64_t motif_b200_kv4_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t T,
+                                                 int64_t D);
+MB_API int motif_b200_kv4_chord_attention(const void* q, const void* pool, const int32_t* block_table,
+                                   int64_t table_stride, const int32_t* lens, const int32_t* q_lens,
+                                   const float* alpha, const float* beta, const float* mu,
+                                   const float* ssmax, void* out, const int64_t* strides, int64_t B,
+                                   int64_t H, int64_t Hkv, int64_t T, int64_t D, int64_t num_pages,
+                                   int64_t page_size, int64_t max_pages, float scale, float eps,
+                                   void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

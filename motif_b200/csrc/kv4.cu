@@ -1,0 +1,526 @@
+// Chord attention over a paged key / value cache held in 4 bits, and what a serving loop needs
+// beside it: the reservation of cache slots from request lengths, the quantising append, and the
+// read-back of cached prefixes.  Layout and value of a stored code: kv4.cuh.
+#include <math.h>
+
+#include "common.cuh"
+#include "kv4.cuh"
+
+namespace mb {
+namespace {
+
+using kv4::kUnit;
+using kv4::Layout;
+
+// ------------------------------------------------------------------ slot reservation
+// need_b = ceil((len_b + new_b) / P) - ceil(len_b / P) fresh pages.  Requests are served in order:
+// request b gets its pages when they fit its table row, its tokens fit the slot map, and the pages
+// asked for up to and including it do not exceed the free count; the i-th fresh page is the i-th
+// from the top of the free list.  One CTA: a block scan over the requests (tokens and pages), then
+// one warp per request writes its table entries and slots.
+constexpr int kReserveThreads = 1024;
+
+__device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+__device__ __forceinline__ int64_t warp_scan(int64_t v) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v += u;
+  }
+  return v;
+}
+
+// Inclusive scan over the block's threads; `part` holds one value per warp.
+__device__ int64_t block_scan(int64_t v, int64_t* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_scan(v);
+  __syncthreads();
+  if (lane == 31) part[warp] = v;
+  __syncthreads();
+  if (warp == 0) part[lane] = warp_scan(part[lane]);
+  __syncthreads();
+  return warp ? v + part[warp - 1] : v;
+}
+
+__global__ void __launch_bounds__(kReserveThreads) paged_reserve_kernel(
+    const int32_t* lens, const int32_t* __restrict__ new_lens, int32_t* table, int64_t ts,
+    const int32_t* __restrict__ free_pages, const int32_t* free_count, int32_t* lens_out, int32_t* free_out,
+    int32_t* __restrict__ slots, int64_t total, int B, int columns, int64_t cap, int P) {
+  __shared__ int64_t part[32];
+  __shared__ int64_t s_start[kReserveThreads], s_pages[kReserveThreads];
+  __shared__ int s_len[kReserveThreads], s_new[kReserveThreads];
+  __shared__ bool s_ok[kReserveThreads];
+  __shared__ int64_t s_tokens, s_used, s_taken;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t avail = min((int64_t)max(*free_count, 0), cap);
+  if (tid == 0) s_tokens = s_used = s_taken = 0;
+  __syncthreads();
+  for (int b0 = 0; b0 < B; b0 += kReserveThreads) {
+    const int b = b0 + tid;
+    int64_t len = 0, fresh = 0;
+    if (b < B) {
+      len = max(lens[b], 0);
+      fresh = max(new_lens[b], 0);
+    }
+    const int64_t tok_end = s_tokens + block_scan(fresh, part);
+    const int64_t all = ceil_div(len + fresh, P);
+    const bool possible = b < B && all <= columns && tok_end <= total;
+    const int64_t need = possible ? all - ceil_div(len, P) : 0;
+    const int64_t upto = s_used + block_scan(need, part);
+    const bool ok = possible && (need == 0 || upto <= avail);
+    s_start[tid] = tok_end - fresh;
+    s_pages[tid] = upto - need;
+    s_len[tid] = (int)len;
+    s_new[tid] = (int)fresh;
+    s_ok[tid] = ok;
+    if (b < B) lens_out[b] = (int32_t)(ok ? len + fresh : len);
+    const int64_t taken = block_scan(ok ? need : 0, part);
+    __syncthreads();
+    if (tid == kReserveThreads - 1) {
+      s_tokens = tok_end;
+      s_used = upto;
+      s_taken += taken;
+    }
+    for (int r = warp; r < min(kReserveThreads, B - b0); r += kReserveThreads / 32) {
+      const int64_t n = s_new[r], at = s_len[r];
+      int32_t* row = table + (int64_t)(b0 + r) * ts;
+      if (s_ok[r]) {
+        const int64_t have = ceil_div(at, P), want = ceil_div(at + n, P) - have;
+        for (int64_t j = lane; j < want; j += 32) row[have + j] = free_pages[avail - 1 - (s_pages[r] + j)];
+        __syncwarp();
+      }
+      for (int64_t t = lane; t < n; t += 32) {
+        if (s_start[r] + t >= total) break;
+        const int64_t pos = at + t;
+        slots[s_start[r] + t] = s_ok[r] ? row[pos / P] * P + (int32_t)(pos % P) : -1;
+      }
+    }
+    __syncthreads();
+  }
+  for (int64_t i = s_tokens + tid; i < total; i += kReserveThreads) slots[i] = -1;
+  if (tid == 0) *free_out = (int32_t)(avail - s_taken);
+}
+
+// Finished requests give their pages back: onto the top of the free list in request order, their
+// table rows become -1 and their lengths 0.
+__global__ void __launch_bounds__(kReserveThreads) paged_release_kernel(
+    const uint8_t* __restrict__ done, int32_t* __restrict__ lens, int32_t* __restrict__ table, int64_t ts,
+    int32_t* __restrict__ free_pages, int32_t* __restrict__ free_count, int B, int columns, int64_t cap, int P) {
+  __shared__ int64_t part[32];
+  __shared__ int64_t s_at[kReserveThreads];
+  __shared__ int s_held[kReserveThreads];
+  __shared__ int64_t s_top;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) s_top = max(*free_count, 0);
+  __syncthreads();
+  for (int b0 = 0; b0 < B; b0 += kReserveThreads) {
+    const int b = b0 + tid;
+    int64_t held = 0;
+    if (b < B && done[b]) {
+      held = min(ceil_div(max(lens[b], 0), P), (int64_t)columns);
+      lens[b] = 0;
+    }
+    const int64_t upto = s_top + block_scan(held, part);
+    s_at[tid] = upto - held;
+    s_held[tid] = (int)held;
+    __syncthreads();
+    if (tid == kReserveThreads - 1) s_top = upto;
+    for (int r = warp; r < min(kReserveThreads, B - b0); r += kReserveThreads / 32) {
+      int32_t* row = table + (int64_t)(b0 + r) * ts;
+      for (int j = lane; j < s_held[r]; j += 32) {
+        if (s_at[r] + j < cap) free_pages[s_at[r] + j] = row[j];
+        row[j] = -1;
+      }
+    }
+    __syncthreads();
+  }
+  if (tid == 0) *free_count = (int32_t)min(s_top, cap);
+}
+
+// ------------------------------------------------------------------ append
+struct Strides12 {
+  int64_t s[12];  // k(b,h,t) v(b,h,t) k_out(b,h,t) v_out(b,h,t)
+};
+
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float fmin_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Eight consecutive elements at a 16-byte aligned address.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* x) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const T* h = reinterpret_cast<const T*>(&a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f(h[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+  }
+}
+
+// A thread takes eight dims of one row (one 32-bit word of codes); the DG / 8 neighbouring lanes of
+// a group find its extremes by xor-shuffles.  The quotient is the IEEE one and ties go to the even
+// code, so the stored bits are a function of the input alone.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
+                                                         const int32_t* __restrict__ slots,
+                                                         uint8_t* __restrict__ pool, T* __restrict__ k_out,
+                                                         T* __restrict__ v_out, Strides12 st, int64_t rows, int T_,
+                                                         int Hkv, int64_t nslots, int P) {
+  using L = Layout<D>;
+  constexpr int W = D / 8;  // threads of one row
+  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int w = (int)(idx % W);
+  int64_t row = idx / W;
+  const bool live = row < 2 * rows;  // whole groups of lanes: W divides the warp
+  const bool isv = row >= rows;
+  if (isv) row -= rows;
+  if (!live) row = 0;
+  const int h = (int)(row % Hkv);
+  const int64_t n = row / Hkv, b = n / T_, t = n % T_;
+  float x[8];
+  const int o = isv ? 3 : 0;
+  load8((isv ? v : k) + b * st.s[o] + h * st.s[o + 1] + t * st.s[o + 2] + 8 * w, x);
+  float hi = x[0], lo = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) hi = fmax_nan(hi, x[i]), lo = fmin_nan(lo, x[i]);
+#pragma unroll
+  for (int d = 1; d < L::DG / 8; d <<= 1) {
+    hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+    lo = fmin_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+  }
+  const float range = __fsub_rn(hi, lo);
+  float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(range, 15.0f)));
+  float m = __bfloat162float(__float2bfloat16_rn(__fadd_rn(lo, 8.0f * s)));
+  if (!(range <= 3.4028234e38f)) s = m = __uint_as_float(0x7fc00000u);  // a NaN or an infinity: all NaN
+  uint32_t word = 0;
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[i], m), s)) : 0.f;
+    const float c = fminf(fmaxf(q, -8.f), 7.f);
+    word |= (uint32_t)((int)c + 8) << (4 * i);
+    y[i] = fmaf(s, c, m);
+  }
+  if (!live) return;
+  const int64_t slot = slots[n];
+  if (slot >= 0 && slot < nslots) {
+    const int64_t unit = (slot / P * Hkv + h) * (P / kUnit) + slot % P / kUnit;
+    const int r = (int)(slot % kUnit);
+    uint8_t* u = pool + unit * L::kBytes;
+    *reinterpret_cast<uint32_t*>(u + (isv ? L::kV : 0) + r * L::kRow + 4 * w) = word;
+    if (w % (L::DG / 8) == 0)
+      *reinterpret_cast<uint32_t*>(u + (isv ? L::kVp : L::kKp) + (w / (L::DG / 8) * kUnit + r) * 4) =
+          (__float_as_uint(m) & 0xffff0000u) | (__float_as_uint(s) >> 16);
+  }
+  T* out = isv ? v_out : k_out;
+  if (out) store8(out + b * st.s[6 + o] + h * st.s[7 + o] + t * st.s[8 + o] + 8 * w, y);
+}
+
+// ------------------------------------------------------------------ gather
+// A thread reads one word of codes of K and of V and writes eight values of each; tokens at or past
+// the request's length, and those of pages outside the pool, become zeros.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_gather_kernel(const uint8_t* __restrict__ pool,
+                                                         const int32_t* __restrict__ table, int64_t ts,
+                                                         const int32_t* __restrict__ lens, T* __restrict__ k_out,
+                                                         T* __restrict__ v_out, int64_t words, int Hkv, int S,
+                                                         int64_t pages, int P, int columns) {
+  using L = Layout<D>;
+  constexpr int W = D / 8;
+  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (idx >= words) return;
+  const int w = (int)(idx % W);
+  const int64_t bhs = idx / W;
+  const int j = (int)(bhs % S);
+  const int64_t bh = bhs / S;
+  const int h = (int)(bh % Hkv);
+  const int64_t b = bh / Hkv;
+  const int64_t len = min((int64_t)lens[b], (int64_t)columns * P);
+  float kx[8], vx[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) kx[i] = vx[i] = 0.f;
+  if (j < len) {
+    const int64_t page = table[b * ts + j / P];
+    if (page >= 0 && page < pages) {
+      const uint8_t* u = pool + ((page * Hkv + h) * (P / kUnit) + j % P / kUnit) * (int64_t)L::kBytes;
+      const int r = j % kUnit, g = w / (L::DG / 8);
+      const uint32_t kc = *reinterpret_cast<const uint32_t*>(u + r * L::kRow + 4 * w);
+      const uint32_t vc = *reinterpret_cast<const uint32_t*>(u + L::kV + r * L::kRow + 4 * w);
+      const uint32_t kp = *reinterpret_cast<const uint32_t*>(u + L::kKp + (g * kUnit + r) * 4);
+      const uint32_t vp = *reinterpret_cast<const uint32_t*>(u + L::kVp + (g * kUnit + r) * 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        kx[i] = fmaf(kv4::pair_scale(kp), (float)(int)((kc >> (4 * i)) & 15u) - 8.f, kv4::pair_centre(kp));
+        vx[i] = fmaf(kv4::pair_scale(vp), (float)(int)((vc >> (4 * i)) & 15u) - 8.f, kv4::pair_centre(vp));
+      }
+    }
+  }
+  store8(k_out + bhs * D + 8 * w, kx);
+  store8(v_out + bhs * D + 8 * w, vx);
+}
+
+// ------------------------------------------------------------------ attention
+struct Strides6 {
+  int64_t s[6];  // q(b,h,t) out(b,h,t)
+};
+
+// One CTA per query row, a warp takes every fourth key, a lane D / 32 dims.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv4_attention_kernel(
+    const T* __restrict__ q, const uint8_t* __restrict__ pool, const int32_t* __restrict__ table, int64_t ts,
+    const int32_t* __restrict__ lens, const int32_t* __restrict__ q_lens, const float* __restrict__ alpha,
+    const float* __restrict__ beta, const float* __restrict__ mu, const float* __restrict__ ssmax,
+    T* __restrict__ out, Strides6 st, int H, int Hkv, int T_, int64_t pages, int P, int columns, float scale,
+    float eps) {
+  using L = Layout<D>;
+  constexpr int E = D / 32;
+  __shared__ float s_m[4], s_l[4], s_o[4][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t = blockIdx.x % T_, h = blockIdx.x / T_ % H, b = blockIdx.x / T_ / H;
+  const int hk = h / (H / Hkv);
+  const int64_t len = max((int64_t)0, min((int64_t)lens[b], (int64_t)columns * P));
+  const int nq = q_lens ? min(max(q_lens[b], 0), T_) : T_;
+  const int64_t pos = len - nq + t;
+  float qx[E], o[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    qx[e] = to_f(q[b * st.s[0] + h * st.s[1] + t * st.s[2] + lane * E + e]);
+    o[e] = 0.f;
+  }
+  if (t < nq && pos >= 0) {
+    const float al = alpha[h], be = beta[h], mh = mu[h], mul = ssmax[h] * logf((float)(pos + 1));
+    for (int64_t j = warp; j <= pos; j += 4) {
+      const int64_t page = table[b * ts + j / P];
+      if (page < 0 || page >= pages) continue;
+      const uint8_t* u = pool + ((page * Hkv + hk) * (P / kUnit) + j % P / kUnit) * (int64_t)L::kBytes;
+      const int r = (int)(j % kUnit), g = lane * E / L::DG;
+      const uint32_t kp = *reinterpret_cast<const uint32_t*>(u + L::kKp + (g * kUnit + r) * 4);
+      const uint32_t vp = *reinterpret_cast<const uint32_t*>(u + L::kVp + (g * kUnit + r) * 4);
+      float dot = 0.f, vx[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int d = lane * E + e;
+        const int kc = (u[r * L::kRow + d / 2] >> (4 * (d & 1))) & 15;
+        const int vc = (u[L::kV + r * L::kRow + d / 2] >> (4 * (d & 1))) & 15;
+        dot = fmaf(qx[e], fmaf(kv4::pair_scale(kp), (float)(kc - 8), kv4::pair_centre(kp)), dot);
+        vx[e] = fmaf(kv4::pair_scale(vp), (float)(vc - 8), kv4::pair_centre(vp));
+      }
+      dot = warp_sum(dot);
+      const float bias = -al * powf(fabsf((float)(j - pos) - mh) + eps, be);
+      const float x = (dot * scale + bias) * mul;
+      const float mn = fmaxf(m, x);
+      const float f = expf(m - mn), p = expf(x - mn);
+      l = l * f + p;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(p, vx[e], o[e] * f);
+      m = mn;
+    }
+  }
+  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
+  __syncthreads();
+  const float mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  for (int d = threadIdx.x; d < D; d += 128) {
+    float num = 0.f, den = 0.f;
+    for (int w = 0; w < 4; ++w) {
+      if (s_m[w] == -INFINITY) continue;
+      const float f = expf(s_m[w] - mx);
+      num = fmaf(f, s_o[w][d], num);
+      den = fmaf(f, s_l[w], den);
+    }
+    out[b * st.s[3] + h * st.s[4] + t * st.s[5] + d] = from_f<T>(den > 0.f ? num / den : 0.f);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+template <typename F>
+int dispatch_dim(int64_t D, F&& f) {
+  switch (D) {
+    case 32: return f(std::integral_constant<int, 32>());
+    case 64: return f(std::integral_constant<int, 64>());
+    case 128: return f(std::integral_constant<int, 128>());
+  }
+  return set_error(MB_ERR_UNSUPPORTED, "kv4: head dim %lld (32, 64 or 128)", (long long)D);
+}
+template <typename F>
+int dispatch(int dtype, int64_t D, F&& f) {
+  switch (dtype) {
+    case MB_F32: return dispatch_dim(D, [&](auto d) { return f(float(), d); });
+    case MB_F16: return dispatch_dim(D, [&](auto d) { return f(__half(), d); });
+    case MB_BF16: return dispatch_dim(D, [&](auto d) { return f(__nv_bfloat16(), d); });
+  }
+  return set_error(MB_ERR_DTYPE, "kv4: unsupported dtype %d", dtype);
+}
+
+int check_paging(const char* who, int64_t B, int64_t columns, int64_t ts, int64_t P) {
+  MB_REQUIRE(B >= 0 && B <= (1 << 20), MB_ERR_SHAPE, "%s: %lld requests (0 .. 2^20)", who, (long long)B);
+  MB_REQUIRE(columns >= 1 && ts >= columns, MB_ERR_SHAPE, "%s: block table of %lld columns, row stride %lld", who,
+             (long long)columns, (long long)ts);
+  MB_REQUIRE(P >= kUnit && P <= 1024 && P % kUnit == 0, MB_ERR_ARG, "%s: page size %lld (a multiple of 16, at most 1024)",
+             who, (long long)P);
+  MB_REQUIRE(columns * P < (1ll << 31), MB_ERR_SHAPE, "%s: a request could hold %lld tokens (fewer than 2^31)", who,
+             (long long)(columns * P));
+  return MB_OK;
+}
+int check_pool(const char* who, const void* pool, int64_t pages, int64_t Hkv, int64_t P) {
+  MB_REQUIRE(pool, MB_ERR_ARG, "%s: null pointer", who);
+  MB_REQUIRE(reinterpret_cast<uintptr_t>(pool) % 16 == 0, MB_ERR_ALIGN, "%s: the pool must be 16-byte aligned", who);
+  MB_REQUIRE(pages >= 1 && Hkv >= 1 && Hkv <= 65535, MB_ERR_SHAPE, "%s: %lld pages, %lld kv heads", who,
+             (long long)pages, (long long)Hkv);
+  MB_REQUIRE(pages * P < (1ll << 31), MB_ERR_SHAPE, "%s: %lld slots (fewer than 2^31)", who, (long long)(pages * P));
+  return MB_OK;
+}
+int check_rows16(const char* who, const void* p, const int64_t* s, int64_t esize) {
+  bool ok = reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && s[i] * esize % 16 == 0;
+  MB_REQUIRE(ok, MB_ERR_ALIGN, "%s: rows must start on 16-byte boundaries", who);
+  return MB_OK;
+}
+
+}  // namespace
+}  // namespace mb
+
+using namespace mb;
+
+extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_lens, int32_t* block_table,
+                                        int64_t table_stride, const int32_t* free_pages, const int32_t* free_count,
+                                        int32_t* lens_out, int32_t* free_count_out, int32_t* slots, int64_t total_new,
+                                        int64_t B, int64_t max_pages, int64_t free_capacity, int64_t page_size,
+                                        void* stream) {
+  MB_REQUIRE(lens && new_lens && block_table && free_pages && free_count && lens_out && free_count_out &&
+                 (slots || total_new == 0),
+             MB_ERR_ARG, "paged_reserve: null pointer");
+  if (int rc = check_paging("paged_reserve", B, max_pages, table_stride, page_size)) return rc;
+  MB_REQUIRE(total_new >= 0 && total_new < (1ll << 31), MB_ERR_SHAPE, "paged_reserve: %lld new tokens",
+             (long long)total_new);
+  MB_REQUIRE(free_capacity >= 1 && free_capacity * page_size < (1ll << 31), MB_ERR_SHAPE,
+             "paged_reserve: free list of %lld pages", (long long)free_capacity);
+  paged_reserve_kernel<<<1, kReserveThreads, 0, (cudaStream_t)stream>>>(
+      lens, new_lens, block_table, table_stride, free_pages, free_count, lens_out, free_count_out, slots, total_new,
+      (int)B, (int)max_pages, free_capacity, (int)page_size);
+  return check_launch("paged_reserve");
+}
+
+extern "C" int motif_b200_paged_release(const uint8_t* done, int32_t* lens, int32_t* block_table, int64_t table_stride,
+                                        int32_t* free_pages, int32_t* free_count, int64_t B, int64_t max_pages,
+                                        int64_t free_capacity, int64_t page_size, void* stream) {
+  MB_REQUIRE(done && lens && block_table && free_pages && free_count, MB_ERR_ARG, "paged_release: null pointer");
+  if (int rc = check_paging("paged_release", B, max_pages, table_stride, page_size)) return rc;
+  MB_REQUIRE(free_capacity >= 1 && free_capacity * page_size < (1ll << 31), MB_ERR_SHAPE,
+             "paged_release: free list of %lld pages", (long long)free_capacity);
+  paged_release_kernel<<<1, kReserveThreads, 0, (cudaStream_t)stream>>>(done, lens, block_table, table_stride,
+                                                                         free_pages, free_count, (int)B,
+                                                                         (int)max_pages, free_capacity,
+                                                                         (int)page_size);
+  return check_launch("paged_release");
+}
+
+extern "C" int64_t motif_b200_kv4_unit_bytes(int64_t D) { return D == 32 || D == 64 || D == 128 ? kv4::unit_bytes(D) : 0; }
+
+extern "C" int motif_b200_kv4_append(const void* k, const void* v, const int32_t* slots, void* pool, void* k_out,
+                                     void* v_out, const int64_t* strides, int64_t B, int64_t T, int64_t Hkv, int64_t D,
+                                     int64_t num_pages, int64_t page_size, int dtype, void* stream) {
+  MB_REQUIRE(strides && ((k && v && slots) || B * T == 0), MB_ERR_ARG, "kv4_append: null pointer");
+  MB_REQUIRE((k_out == nullptr) == (v_out == nullptr), MB_ERR_ARG, "kv4_append: k_out and v_out go together");
+  MB_REQUIRE(B >= 0 && T >= 0 && B * T < (1ll << 31), MB_ERR_SHAPE, "kv4_append: B %lld, T %lld", (long long)B,
+             (long long)T);
+  if (int rc = check_paging("kv4_append", B, 1, 1, page_size)) return rc;
+  if (int rc = check_pool("kv4_append", pool, num_pages, Hkv, page_size)) return rc;
+  return dispatch(dtype, D, [&](auto t, auto d) -> int {
+    using E = decltype(t);
+    constexpr int DD = decltype(d)::value;
+    if (B * T == 0) return MB_OK;
+    const void* ptrs[4] = {k, v, k_out, v_out};
+    Strides12 st;
+    for (int i = 0; i < 12; ++i) st.s[i] = strides[i];
+    for (int i = 0; i < 4; ++i)
+      if (ptrs[i])
+        if (int rc = check_rows16("kv4_append", ptrs[i], strides + 3 * i, sizeof(E))) return rc;
+    const int64_t rows = B * T * Hkv, threads = 2 * rows * (DD / 8);
+    MB_REQUIRE((threads + 255) / 256 < (1ll << 31), MB_ERR_SHAPE, "kv4_append: %lld rows", (long long)rows);
+    kv4_append_kernel<E, DD><<<(unsigned)((threads + 255) / 256), 256, 0, (cudaStream_t)stream>>>(
+        (const E*)k, (const E*)v, slots, (uint8_t*)pool, (E*)k_out, (E*)v_out, st, rows, (int)T, (int)Hkv,
+        num_pages * page_size, (int)page_size);
+    return check_launch("kv4_append");
+  });
+}
+
+extern "C" int motif_b200_kv4_gather(const void* pool, const int32_t* block_table, int64_t table_stride,
+                                     const int32_t* lens, void* k_out, void* v_out, int64_t B, int64_t Hkv, int64_t S,
+                                     int64_t D, int64_t num_pages, int64_t page_size, int64_t max_pages, int dtype,
+                                     void* stream) {
+  MB_REQUIRE((block_table && lens && k_out && v_out) || B * S == 0, MB_ERR_ARG, "kv4_gather: null pointer");
+  if (int rc = check_paging("kv4_gather", B, max_pages, table_stride, page_size)) return rc;
+  if (int rc = check_pool("kv4_gather", pool, num_pages, Hkv, page_size)) return rc;
+  MB_REQUIRE(S >= 0 && S < (1ll << 31), MB_ERR_SHAPE, "kv4_gather: length %lld", (long long)S);
+  return dispatch(dtype, D, [&](auto t, auto d) -> int {
+    using E = decltype(t);
+    constexpr int DD = decltype(d)::value;
+    if (B * S == 0) return MB_OK;
+    const int64_t none[3] = {0, 0, 0};
+    if (int rc = check_rows16("kv4_gather", k_out, none, 1)) return rc;
+    if (int rc = check_rows16("kv4_gather", v_out, none, 1)) return rc;
+    const int64_t words = B * Hkv * S * (DD / 8);
+    MB_REQUIRE((words + 255) / 256 < (1ll << 31), MB_ERR_SHAPE, "kv4_gather: %lld rows", (long long)(B * Hkv * S));
+    kv4_gather_kernel<E, DD><<<(unsigned)((words + 255) / 256), 256, 0, (cudaStream_t)stream>>>(
+        (const uint8_t*)pool, block_table, table_stride, lens, (E*)k_out, (E*)v_out, words, (int)Hkv, (int)S,
+        num_pages, (int)page_size, (int)max_pages);
+    return check_launch("kv4_gather");
+  });
+}
+
+extern "C" int64_t motif_b200_kv4_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t D) {
+  (void)B, (void)H, (void)Hkv, (void)T, (void)D;
+  return 0;
+}
+
+extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, const int32_t* block_table,
+                                              int64_t table_stride, const int32_t* lens, const int32_t* q_lens,
+                                              const float* alpha, const float* beta, const float* mu,
+                                              const float* ssmax, void* out, const int64_t* strides, int64_t B,
+                                              int64_t H, int64_t Hkv, int64_t T, int64_t D, int64_t num_pages,
+                                              int64_t page_size, int64_t max_pages, float scale, float eps,
+                                              void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+  (void)workspace, (void)workspace_bytes;
+  MB_REQUIRE(strides && alpha && beta && mu && ssmax && ((q && out && block_table && lens) || B * T == 0), MB_ERR_ARG,
+             "kv4_chord_attention: null pointer");
+  if (int rc = check_paging("kv4_chord_attention", B, max_pages, table_stride, page_size)) return rc;
+  if (int rc = check_pool("kv4_chord_attention", pool, num_pages, Hkv, page_size)) return rc;
+  MB_REQUIRE(H >= 1 && H % Hkv == 0, MB_ERR_SHAPE, "kv4_chord_attention: %lld heads not divisible by %lld kv heads",
+             (long long)H, (long long)Hkv);
+  MB_REQUIRE(T >= 0 && B * H * T < (1ll << 31), MB_ERR_SHAPE, "kv4_chord_attention: B %lld, H %lld, T %lld",
+             (long long)B, (long long)H, (long long)T);
+  return dispatch(dtype, D, [&](auto t, auto d) -> int {
+    using E = decltype(t);
+    constexpr int DD = decltype(d)::value;
+    if (B * T == 0) return MB_OK;
+    Strides6 st;
+    for (int i = 0; i < 6; ++i) st.s[i] = strides[i];
+    kv4_attention_kernel<E, DD><<<(unsigned)(B * H * T), 128, 0, (cudaStream_t)stream>>>(
+        (const E*)q, (const uint8_t*)pool, block_table, table_stride, lens, q_lens, alpha, beta, mu, ssmax, (E*)out,
+        st, (int)H, (int)Hkv, (int)T, num_pages, (int)page_size, (int)max_pages, scale, eps);
+    return check_launch("kv4_chord_attention");
+  });
+}

@@ -16,12 +16,14 @@ import torch.nn as nn
 
 from . import _lib
 from .autograd import AttnResFunction, ChordAttentionFunction, GatedDeltaRuleFunction, needs_grad
+from .paged import kv4_append, kv4_chord_attention, kv4_gather, kv4_pool, paged_release, paged_reserve
 from .sampler import Sampler, make_sampler  # noqa: F401  (install targets)
 
 __all__ = [
     'RMSNorm', 'GatedRMSNorm', 'SwiGLU', 'apply_chord_attention', 'HAS_TRITON',
     'recurrent_gated_delta_rule', 'chunk_gated_delta_rule', 'chunk_gated_delta_rule_triton',
     'attn_res_block', 'can_use_triton_attn_res', 'apply_block_attn_res', 'MAX_SRC',
+    'kv4_pool', 'paged_reserve', 'paged_release', 'kv4_append', 'kv4_gather', 'kv4_chord_attention',
 ]
 
 # The reference's switch for its fused-kernel path.  Here the fused path is always the
