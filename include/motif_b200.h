@@ -567,9 +567,8 @@ MB_API int motif_b200_kv4_gather(const void* pool, const int32_t* block_table, i
  * lens[b] - T + t, or lens[b] - q_lens[b] + t where q_lens != NULL (rows t >= q_lens[b] are
  * padding).  Rows that see no key are zeros; keys on table entries outside the pool are left out.
  * `strides` (elements), [6]: (b, h, t) of q, out.  `workspace` (16-byte aligned) holds
- * motif_b200_kv4_attention_workspace_bytes bytes. */
-MB_API int64_t motif_b200_kv4_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t T,
-                                                 int64_t D);
+ * motif_b200_kv4_attention_workspace_bytes bytes of the current device. */
+MB_API int64_t motif_b200_kv4_attention_workspace_bytes(int64_t H, int64_t Hkv, int64_t T, int64_t D);
 MB_API int motif_b200_kv4_chord_attention(const void* q, const void* pool, const int32_t* block_table,
                                    int64_t table_stride, const int32_t* lens, const int32_t* q_lens,
                                    const float* alpha, const float* beta, const float* mu,

@@ -100,7 +100,7 @@ SIGNATURES = {
     'motif_b200_kv4_unit_bytes': (_I64, [_I64]),
     'motif_b200_kv4_append': (_I, [_P] * 7 + [_I64] * 6 + [_I, _P]),
     'motif_b200_kv4_gather': (_I, [_P, _P, _I64, _P, _P, _P] + [_I64] * 7 + [_I, _P]),
-    'motif_b200_kv4_attention_workspace_bytes': (_I64, [_I64] * 5),
+    'motif_b200_kv4_attention_workspace_bytes': (_I64, [_I64] * 4),
     'motif_b200_kv4_chord_attention': (_I, [_P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P] + [_I64] * 8
                                        + [_F, _F, _P, _I64, _I, _P]),
 }
@@ -166,7 +166,7 @@ KERNELS_PER_CALL.update({'motif_b200_last_error': 0, 'motif_b200_abi_version': 0
                          'motif_b200_chord_workspace_bytes': 0, 'motif_b200_chord_decode_workspace_bytes': 0,
                          'motif_b200_skinny_packed_bytes': 0, 'motif_b200_gdn_chunk_workspace_bytes': 0,
                          'motif_b200_chord_backward_workspace_bytes': 0, 'motif_b200_gdn_backward_workspace_bytes': 0,
-                         'motif_b200_chord_backward': 2,
+                         'motif_b200_chord_backward': 2, 'motif_b200_kv4_chord_attention': 2,
                          'motif_b200_kv4_unit_bytes': 0, 'motif_b200_kv4_attention_workspace_bytes': 0,
                          'motif_b200_wait_timeouts': 0, 'motif_b200_testing_force': 0,
                          'motif_b200_chord_decode': 2, 'motif_b200_chord_decode_noalloc': 2,

@@ -1,6 +1,6 @@
-// Chord attention over a paged key / value cache held in 4 bits, and what a serving loop needs
-// beside it: the reservation of cache slots from request lengths, the quantising append, and the
-// read-back of cached prefixes.  Layout and value of a stored code: kv4.cuh.
+// What a serving loop needs beside the attention over its paged 4-bit cache (kv4_attention.cu): the
+// reservation of cache slots from request lengths, the quantising append, and the read-back of
+// cached prefixes.  Layout and value of a stored code: kv4.cuh.
 #include <math.h>
 
 #include "common.cuh"
@@ -280,129 +280,11 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const uint8_t* __restri
   store8(v_out + bhs * D + 8 * w, vx);
 }
 
-// ------------------------------------------------------------------ attention
-struct Strides6 {
-  int64_t s[6];  // q(b,h,t) out(b,h,t)
-};
-
-// One CTA per query row, a warp takes every fourth key, a lane D / 32 dims.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_attention_kernel(
-    const T* __restrict__ q, const uint8_t* __restrict__ pool, const int32_t* __restrict__ table, int64_t ts,
-    const int32_t* __restrict__ lens, const int32_t* __restrict__ q_lens, const float* __restrict__ alpha,
-    const float* __restrict__ beta, const float* __restrict__ mu, const float* __restrict__ ssmax,
-    T* __restrict__ out, Strides6 st, int H, int Hkv, int T_, int64_t pages, int P, int columns, float scale,
-    float eps) {
-  using L = Layout<D>;
-  constexpr int E = D / 32;
-  __shared__ float s_m[4], s_l[4], s_o[4][D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t = blockIdx.x % T_, h = blockIdx.x / T_ % H, b = blockIdx.x / T_ / H;
-  const int hk = h / (H / Hkv);
-  const int64_t len = max((int64_t)0, min((int64_t)lens[b], (int64_t)columns * P));
-  const int nq = q_lens ? min(max(q_lens[b], 0), T_) : T_;
-  const int64_t pos = len - nq + t;
-  float qx[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qx[e] = to_f(q[b * st.s[0] + h * st.s[1] + t * st.s[2] + lane * E + e]);
-    o[e] = 0.f;
-  }
-  if (t < nq && pos >= 0) {
-    const float al = alpha[h], be = beta[h], mh = mu[h], mul = ssmax[h] * logf((float)(pos + 1));
-    for (int64_t j = warp; j <= pos; j += 4) {
-      const int64_t page = table[b * ts + j / P];
-      if (page < 0 || page >= pages) continue;
-      const uint8_t* u = pool + ((page * Hkv + hk) * (P / kUnit) + j % P / kUnit) * (int64_t)L::kBytes;
-      const int r = (int)(j % kUnit), g = lane * E / L::DG;
-      const uint32_t kp = *reinterpret_cast<const uint32_t*>(u + L::kKp + (g * kUnit + r) * 4);
-      const uint32_t vp = *reinterpret_cast<const uint32_t*>(u + L::kVp + (g * kUnit + r) * 4);
-      float dot = 0.f, vx[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int d = lane * E + e;
-        const int kc = (u[r * L::kRow + d / 2] >> (4 * (d & 1))) & 15;
-        const int vc = (u[L::kV + r * L::kRow + d / 2] >> (4 * (d & 1))) & 15;
-        dot = fmaf(qx[e], fmaf(kv4::pair_scale(kp), (float)(kc - 8), kv4::pair_centre(kp)), dot);
-        vx[e] = fmaf(kv4::pair_scale(vp), (float)(vc - 8), kv4::pair_centre(vp));
-      }
-      dot = warp_sum(dot);
-      const float bias = -al * powf(fabsf((float)(j - pos) - mh) + eps, be);
-      const float x = (dot * scale + bias) * mul;
-      const float mn = fmaxf(m, x);
-      const float f = expf(m - mn), p = expf(x - mn);
-      l = l * f + p;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(p, vx[e], o[e] * f);
-      m = mn;
-    }
-  }
-  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-#pragma unroll
-  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-  __syncthreads();
-  const float mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float num = 0.f, den = 0.f;
-    for (int w = 0; w < 4; ++w) {
-      if (s_m[w] == -INFINITY) continue;
-      const float f = expf(s_m[w] - mx);
-      num = fmaf(f, s_o[w][d], num);
-      den = fmaf(f, s_l[w], den);
-    }
-    out[b * st.s[3] + h * st.s[4] + t * st.s[5] + d] = from_f<T>(den > 0.f ? num / den : 0.f);
-  }
-}
-
-// ------------------------------------------------------------------ host side
-template <typename F>
-int dispatch_dim(int64_t D, F&& f) {
-  switch (D) {
-    case 32: return f(std::integral_constant<int, 32>());
-    case 64: return f(std::integral_constant<int, 64>());
-    case 128: return f(std::integral_constant<int, 128>());
-  }
-  return set_error(MB_ERR_UNSUPPORTED, "kv4: head dim %lld (32, 64 or 128)", (long long)D);
-}
-template <typename F>
-int dispatch(int dtype, int64_t D, F&& f) {
-  switch (dtype) {
-    case MB_F32: return dispatch_dim(D, [&](auto d) { return f(float(), d); });
-    case MB_F16: return dispatch_dim(D, [&](auto d) { return f(__half(), d); });
-    case MB_BF16: return dispatch_dim(D, [&](auto d) { return f(__nv_bfloat16(), d); });
-  }
-  return set_error(MB_ERR_DTYPE, "kv4: unsupported dtype %d", dtype);
-}
-
-int check_paging(const char* who, int64_t B, int64_t columns, int64_t ts, int64_t P) {
-  MB_REQUIRE(B >= 0 && B <= (1 << 20), MB_ERR_SHAPE, "%s: %lld requests (0 .. 2^20)", who, (long long)B);
-  MB_REQUIRE(columns >= 1 && ts >= columns, MB_ERR_SHAPE, "%s: block table of %lld columns, row stride %lld", who,
-             (long long)columns, (long long)ts);
-  MB_REQUIRE(P >= kUnit && P <= 1024 && P % kUnit == 0, MB_ERR_ARG, "%s: page size %lld (a multiple of 16, at most 1024)",
-             who, (long long)P);
-  MB_REQUIRE(columns * P < (1ll << 31), MB_ERR_SHAPE, "%s: a request could hold %lld tokens (fewer than 2^31)", who,
-             (long long)(columns * P));
-  return MB_OK;
-}
-int check_pool(const char* who, const void* pool, int64_t pages, int64_t Hkv, int64_t P) {
-  MB_REQUIRE(pool, MB_ERR_ARG, "%s: null pointer", who);
-  MB_REQUIRE(reinterpret_cast<uintptr_t>(pool) % 16 == 0, MB_ERR_ALIGN, "%s: the pool must be 16-byte aligned", who);
-  MB_REQUIRE(pages >= 1 && Hkv >= 1 && Hkv <= 65535, MB_ERR_SHAPE, "%s: %lld pages, %lld kv heads", who,
-             (long long)pages, (long long)Hkv);
-  MB_REQUIRE(pages * P < (1ll << 31), MB_ERR_SHAPE, "%s: %lld slots (fewer than 2^31)", who, (long long)(pages * P));
-  return MB_OK;
-}
-int check_rows16(const char* who, const void* p, const int64_t* s, int64_t esize) {
-  bool ok = reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  for (int i = 0; i < 3; ++i) ok = ok && s[i] * esize % 16 == 0;
-  MB_REQUIRE(ok, MB_ERR_ALIGN, "%s: rows must start on 16-byte boundaries", who);
-  return MB_OK;
-}
-
 }  // namespace
 }  // namespace mb
 
 using namespace mb;
+using namespace mb::kv4;
 
 extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_lens, int32_t* block_table,
                                         int64_t table_stride, const int32_t* free_pages, const int32_t* free_count,
@@ -488,39 +370,5 @@ extern "C" int motif_b200_kv4_gather(const void* pool, const int32_t* block_tabl
         (const uint8_t*)pool, block_table, table_stride, lens, (E*)k_out, (E*)v_out, words, (int)Hkv, (int)S,
         num_pages, (int)page_size, (int)max_pages);
     return check_launch("kv4_gather");
-  });
-}
-
-extern "C" int64_t motif_b200_kv4_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t D) {
-  (void)B, (void)H, (void)Hkv, (void)T, (void)D;
-  return 0;
-}
-
-extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, const int32_t* block_table,
-                                              int64_t table_stride, const int32_t* lens, const int32_t* q_lens,
-                                              const float* alpha, const float* beta, const float* mu,
-                                              const float* ssmax, void* out, const int64_t* strides, int64_t B,
-                                              int64_t H, int64_t Hkv, int64_t T, int64_t D, int64_t num_pages,
-                                              int64_t page_size, int64_t max_pages, float scale, float eps,
-                                              void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
-  (void)workspace, (void)workspace_bytes;
-  MB_REQUIRE(strides && alpha && beta && mu && ssmax && ((q && out && block_table && lens) || B * T == 0), MB_ERR_ARG,
-             "kv4_chord_attention: null pointer");
-  if (int rc = check_paging("kv4_chord_attention", B, max_pages, table_stride, page_size)) return rc;
-  if (int rc = check_pool("kv4_chord_attention", pool, num_pages, Hkv, page_size)) return rc;
-  MB_REQUIRE(H >= 1 && H % Hkv == 0, MB_ERR_SHAPE, "kv4_chord_attention: %lld heads not divisible by %lld kv heads",
-             (long long)H, (long long)Hkv);
-  MB_REQUIRE(T >= 0 && B * H * T < (1ll << 31), MB_ERR_SHAPE, "kv4_chord_attention: B %lld, H %lld, T %lld",
-             (long long)B, (long long)H, (long long)T);
-  return dispatch(dtype, D, [&](auto t, auto d) -> int {
-    using E = decltype(t);
-    constexpr int DD = decltype(d)::value;
-    if (B * T == 0) return MB_OK;
-    Strides6 st;
-    for (int i = 0; i < 6; ++i) st.s[i] = strides[i];
-    kv4_attention_kernel<E, DD><<<(unsigned)(B * H * T), 128, 0, (cudaStream_t)stream>>>(
-        (const E*)q, (const uint8_t*)pool, block_table, table_stride, lens, q_lens, alpha, beta, mu, ssmax, (E*)out,
-        st, (int)H, (int)Hkv, (int)T, num_pages, (int)page_size, (int)max_pages, scale, eps);
-    return check_launch("kv4_chord_attention");
   });
 }

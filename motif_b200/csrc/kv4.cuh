@@ -13,6 +13,8 @@
 // and every unit starts on a 128-byte boundary.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mb {
@@ -36,6 +38,52 @@ __host__ __device__ constexpr int64_t unit_bytes(int64_t D) { return kUnit * D +
 
 __device__ __forceinline__ float pair_scale(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float pair_centre(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// ------------------------------------------------------------------ host side
+template <typename F>
+int dispatch_dim(int64_t D, F&& f) {
+  switch (D) {
+    case 32: return f(std::integral_constant<int, 32>());
+    case 64: return f(std::integral_constant<int, 64>());
+    case 128: return f(std::integral_constant<int, 128>());
+  }
+  return set_error(MB_ERR_UNSUPPORTED, "kv4: head dim %lld (32, 64 or 128)", (long long)D);
+}
+template <typename F>
+int dispatch(int dtype, int64_t D, F&& f) {
+  switch (dtype) {
+    case MB_F32: return dispatch_dim(D, [&](auto d) { return f(float(), d); });
+    case MB_F16: return dispatch_dim(D, [&](auto d) { return f(__half(), d); });
+    case MB_BF16: return dispatch_dim(D, [&](auto d) { return f(__nv_bfloat16(), d); });
+  }
+  return set_error(MB_ERR_DTYPE, "kv4: unsupported dtype %d", dtype);
+}
+
+inline int check_paging(const char* who, int64_t B, int64_t columns, int64_t ts, int64_t P) {
+  MB_REQUIRE(B >= 0 && B <= (1 << 20), MB_ERR_SHAPE, "%s: %lld requests (0 .. 2^20)", who, (long long)B);
+  MB_REQUIRE(columns >= 1 && ts >= columns, MB_ERR_SHAPE, "%s: block table of %lld columns, row stride %lld", who,
+             (long long)columns, (long long)ts);
+  MB_REQUIRE(P >= kUnit && P <= 1024 && P % kUnit == 0, MB_ERR_ARG, "%s: page size %lld (a multiple of 16, at most 1024)",
+             who, (long long)P);
+  MB_REQUIRE(columns * P < (1ll << 31), MB_ERR_SHAPE, "%s: a request could hold %lld tokens (fewer than 2^31)", who,
+             (long long)(columns * P));
+  return MB_OK;
+}
+inline int check_pool(const char* who, const void* pool, int64_t pages, int64_t Hkv, int64_t P) {
+  MB_REQUIRE(pool, MB_ERR_ARG, "%s: null pointer", who);
+  MB_REQUIRE(reinterpret_cast<uintptr_t>(pool) % 16 == 0, MB_ERR_ALIGN, "%s: the pool must be 16-byte aligned", who);
+  MB_REQUIRE(pages >= 1 && Hkv >= 1 && Hkv <= 65535, MB_ERR_SHAPE, "%s: %lld pages, %lld kv heads", who,
+             (long long)pages, (long long)Hkv);
+  MB_REQUIRE(pages * P < (1ll << 31), MB_ERR_SHAPE, "%s: %lld slots (fewer than 2^31)", who, (long long)(pages * P));
+  return MB_OK;
+}
+inline int check_rows16(const char* who, const void* p, const int64_t* s, int64_t esize) {
+  bool ok = reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && s[i] * esize % 16 == 0;
+  MB_REQUIRE(ok, MB_ERR_ALIGN, "%s: rows must start on 16-byte boundaries", who);
+  return MB_OK;
+}
+
 
 }  // namespace kv4
 }  // namespace mb

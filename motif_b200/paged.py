@@ -233,7 +233,7 @@ def kv4_chord_attention(q, pool, block_table, lens, alpha, beta, mu, ssmax, q_le
     if q.stride(3) != 1:
         q = q.contiguous()
     out = torch.empty((B, H, T, D), dtype=q.dtype, device=dev)
-    ws_bytes = _lib.load().motif_b200_kv4_attention_workspace_bytes(B, H, kv, T, D)
+    ws_bytes = _lib.load().motif_b200_kv4_attention_workspace_bytes(H, kv, T, D)
     ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
     strides = _lib.i64_array([*q.stride()[:3], *out.stride()[:3]])
     _lib.call('motif_b200_kv4_chord_attention', q.data_ptr(), pool.data_ptr(), block_table.data_ptr(),
