@@ -82,59 +82,84 @@ __device__ __forceinline__ int tiles_of(const Args& a, int b) {
   return queries_of(a, b) > 0 ? (length_of(a, b) + KT - 1) / KT : 0;
 }
 
-// Exclusive prefix of the requests' tiles at each thread's run of requests (pre[0 .. threads]).
-template <int KT, int THREADS>
-__device__ __forceinline__ void scan_requests(const Args& a, int64_t* pre) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int run = (a.B + THREADS - 1) / THREADS;
-  __shared__ int64_t part[THREADS / 32];
-  int64_t v = 0;
-  for (int b = tid * run; b < min(a.B, (tid + 1) * run); ++b) v += tiles_of<KT>(a, b);
+// The requests' tiles, by one warp: lane i counts those of the i-th run of `run` requests.
+struct Requests {
+  int run;
+  int upto;   // tiles of this lane's run and the ones before it
+  int mine;
+  int total;  // tiles of all segments (the host keeps this below 2^31)
+};
+__device__ __forceinline__ int warp_scan(int v) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v += u;
   }
-  if (lane == 31) part[warp] = v;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) v += part[w];
-  pre[tid + 1] = v;
-  if (tid == 0) pre[0] = 0;
-  __syncthreads();
+  return v;
+}
+template <int KT>
+__device__ __forceinline__ Requests scan_requests(const Args& a) {
+  Requests q;
+  const int lane = threadIdx.x & 31;
+  q.run = (a.B + 31) / 32;
+  q.mine = 0;
+#pragma unroll 4
+  for (int i = 0; i < q.run; ++i) {
+    const int b = lane * q.run + i;
+    if (b < a.B) q.mine += tiles_of<KT>(a, b);
+  }
+  q.upto = warp_scan(q.mine);
+  q.total = __shfl_sync(0xffffffffu, q.upto, 31) * a.Z * a.Hkv;
+  return q;
 }
 
-// `total` tiles over at most `n` CTAs, at least one tile per warp: the number of CTAs that work, the
-// first tile of CTA c of `m` working ones, and the CTA of tile x.
-__device__ __forceinline__ int64_t working_ctas(int64_t total, int n) {
-  return min((int64_t)n, (total + kWarps - 1) / kWarps);
-}
-__device__ __forceinline__ int64_t cta_start(int64_t total, int64_t m, int64_t c) { return total * c / m; }
-__device__ __forceinline__ int64_t cta_of(int64_t total, int64_t m, int64_t x) { return ((x + 1) * m - 1) / total; }
+// `total` tiles over at most `n` CTAs, at least one tile per warp: the first CTAs take one more than
+// the others.
+struct Cut {
+  int working, each, more;
+  __device__ __forceinline__ Cut(int total, int n) {
+    working = min(n, (total + kWarps - 1) / kWarps);
+    each = working ? total / working : 0;
+    more = total - each * working;
+  }
+  __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
+  __device__ __forceinline__ int cta_of(int x) const {
+    const int wide = more * (each + 1);
+    return x < wide ? x / (each + 1) : more + (x - wide) / each;
+  }
+};
 
 // A place in the order of tiles: request, segment of it (z * Hkv + kv head), tile of the segment.
 struct Cursor {
   int b, seg, k, nt;
 };
 
-template <int KT, int THREADS>
-__device__ __forceinline__ Cursor locate(const Args& a, const int64_t* pre, int64_t x) {
+template <int KT>
+__device__ __forceinline__ Cursor locate(const Args& a, const Requests& q, int x) {
   const int zh = a.Z * a.Hkv, lane = threadIdx.x & 31;
-  const int run = (a.B + THREADS - 1) / THREADS;
-  int c = 0;  // last run of requests that starts at or before x (empty ones share a start)
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i)
-    c += __popc(__ballot_sync(0xffffffffu, pre[i * 32 + lane + 1] * zh <= x));
-  int64_t left = x - pre[c] * zh;
+  // the first run whose tiles reach past x
+  const int c = __popc(__ballot_sync(0xffffffffu, q.upto * zh <= x));
+  int left = x - __shfl_sync(0xffffffffu, q.upto - q.mine, c) * zh;
   Cursor u;
-  u.b = c * run;
-  while (true) {
-    u.nt = tiles_of<KT>(a, u.b);
-    if (left < (int64_t)u.nt * zh || u.b + 1 >= a.B) break;
-    left -= (int64_t)u.nt * zh;
-    ++u.b;
+  u.b = c;
+  u.nt = __shfl_sync(0xffffffffu, q.mine, c);
+  if (q.run > 1) {
+    for (int i0 = 0; i0 < q.run; i0 += 32) {
+      const int b = c * q.run + i0 + lane;
+      const int t = i0 + lane < q.run && b < a.B ? tiles_of<KT>(a, b) : 0;
+      const int upto = warp_scan(t);
+      const int n = __popc(__ballot_sync(0xffffffffu, upto * zh <= left));
+      if (n < 32) {
+        left -= __shfl_sync(0xffffffffu, upto - t, n) * zh;
+        u.b = c * q.run + i0 + n;
+        u.nt = __shfl_sync(0xffffffffu, t, n);
+        break;
+      }
+      left -= __shfl_sync(0xffffffffu, upto, 31) * zh;
+    }
   }
-  u.seg = (int)(left / max(u.nt, 1));
-  u.k = (int)(left % max(u.nt, 1));
+  u.seg = left / u.nt;
+  u.k = left - u.seg * u.nt;
   return u;
 }
 template <int KT>
@@ -148,6 +173,17 @@ __device__ __forceinline__ bool advance(const Args& a, Cursor& u) {  // true: an
     u.nt = tiles_of<KT>(a, u.b);
   } while (u.nt == 0);
   return true;
+}
+
+// The row tile and kv head of a segment, and the new token and head (within the kv head's group) of
+// query row r.
+__device__ __forceinline__ void split_segment(const Args& a, int seg, int& z, int& hk) {
+  z = a.Z == 1 ? 0 : seg / a.Hkv;
+  hk = seg - z * a.Hkv;
+}
+__device__ __forceinline__ void split_row(const Args& a, int r, int& t, int& gi) {
+  t = a.T == 1 ? 0 : r / a.G;
+  gi = r - t * a.G;
 }
 
 // ------------------------------------------------------------------ small device helpers
@@ -182,15 +218,37 @@ __device__ __forceinline__ void codes(uint32_t w, uint32_t* h) {
   h[3] = v & 0x00f000f0u;
 }
 
+// Eight consecutive elements at a 16-byte aligned address.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* x) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const T* h = reinterpret_cast<const T*>(&a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f(h[i]);
+  }
+}
+// Four neighbouring outputs y f (zeros where the row sees no key); the host asks for rows of out on
+// 16-byte boundaries.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 y, float f, bool sees) {
+  const float4 v = sees ? make_float4(y.x * f, y.y * f, y.z * f, y.w * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = v;
+  else *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+}
+
 // Place of row r of a group of 8 keys: rows 2t, 2t + 1 are keys t, t + 4, so that the four lanes of a
 // V load take neighbouring keys (128 consecutive bytes of shared memory per load).
 __device__ __forceinline__ int key_of_row(int r) { return (r >> 1) + 4 * (r & 1); }
 
 // ------------------------------------------------------------------ the worker kernel
 // An unfinished piece of a segment at the end of a warp's run: [RT rows][D + 4] floats (o, m, l), its
-// segment (request * Z * Hkv + seg, -1: none) and whether it holds the segment's first / last tile.
+// segment and whether it holds the segment's first / last tile.
 struct Piece {
-  int64_t segment;
+  int b, seg;  // b < 0: none
   int begins, ends;
 };
 template <int D, int NT>
@@ -219,7 +277,6 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
   constexpr int RT = 4 * NT;         // query rows of a row tile
   constexpr int THREADS = 32 * kWarps;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t pre[THREADS + 1];
   __shared__ __align__(8) uint64_t bars[kWarps][kStages];
   __shared__ Piece pieces[kWarps][2];
 
@@ -234,23 +291,19 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&bar[s], 1);
     mbar_init_fence();
-    pieces[warp][0].segment = pieces[warp][1].segment = -1;
+    pieces[warp][0].b = pieces[warp][1].b = -1;
   }
-  scan_requests<KT, THREADS>(a, pre);
   allow_dependent_launch();  // the merge may take its place; it waits for this grid to end
-
-  const int zh = a.Z * a.Hkv;
-  const int64_t total = pre[THREADS] * zh;
-  const int64_t working = working_ctas(total, gridDim.x);
-  if (blockIdx.x >= working) return;
-  const int64_t cta_first = cta_start(total, working, blockIdx.x);
-  const int cta_count = (int)(cta_start(total, working, blockIdx.x + 1) - cta_first);
+  const Requests reqs = scan_requests<KT>(a);
+  const Cut cut(reqs.total, gridDim.x);
+  if ((int)blockIdx.x >= cut.working) return;
+  const int cta_first = cut.start(blockIdx.x), cta_count = cut.each + ((int)blockIdx.x < cut.more ? 1 : 0);
   const int run0 = (int)((int64_t)cta_count * warp / kWarps);
   const int count = (int)((int64_t)cta_count * (warp + 1) / kWarps) - run0;
 
   bool failed = false;
   if (count > 0) {
-    Cursor cur = locate<KT, THREADS>(a, pre, cta_first + run0);
+    Cursor cur = locate<KT>(a, reqs, cta_first + run0);
 
     // The tile to be copied next: its page of this lane's unit (lanes 0 .. TU - 1) is looked up one
     // tile before the copy is issued.
@@ -258,17 +311,21 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
     const bool one_copy = UP % TU == 0;  // a tile's units lie in one page, next to each other
     const int step_page = TU / UP, step_sub = TU % UP, page0 = lane / UP, sub0 = lane % UP;
     Cursor ahead = cur;
-    int a_len = length_of(a, ahead.b), a_head = ahead.seg % a.Hkv;
+    int a_len = length_of(a, ahead.b), a_z, a_head;
+    split_segment(a, ahead.seg, a_z, a_head);
     int a_page = (ahead.k * TU + lane) / UP, a_sub = (ahead.k * TU + lane) % UP;
     const int32_t* a_row = a.table + (int64_t)ahead.b * a.ts;
-    int pid = -1;
+    struct Look {
+      int pid, head, sub;  // pid -1: no such unit
+    };
     auto look = [&]() {
-      pid = -1;
-      if (lane < TU && (ahead.k * TU + lane) * kUnit < a_len) pid = a_row[a_page];
+      Look f = {-1, a_head, a_sub};
+      if (lane < TU && (ahead.k * TU + lane) * kUnit < a_len) f.pid = a_row[a_page];
+      return f;
     };
     auto step = [&]() {
       if (advance<KT>(a, ahead)) {
-        a_head = ahead.seg % a.Hkv;
+        split_segment(a, ahead.seg, a_z, a_head);
         a_len = length_of(a, ahead.b);
         a_row = a.table + (int64_t)ahead.b * a.ts;
         a_page = page0, a_sub = sub0;
@@ -276,11 +333,11 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
         a_page += step_page, a_sub += step_sub;
         if (a_sub >= UP) a_sub -= UP, ++a_page;
       }
-      look();
+      return look();
     };
     uint32_t valid = 0;  // units that are there, TU bits per stage
-    auto issue = [&](int s) {
-      const bool ok = pid >= 0 && pid < a.pages;
+    auto issue = [&](int s, const Look& f) {
+      const bool ok = f.pid >= 0 && f.pid < a.pages;
       const uint32_t mask = __ballot_sync(0xffffffffu, ok);
       valid = (valid & ~(((1u << TU) - 1) << (TU * s))) | (mask << (TU * s));
       const uint32_t bytes = __popc(mask) * L::kBytes;
@@ -288,16 +345,21 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
       __syncwarp();
       if (ok && (lane == 0 || !one_copy))
         bulk_load(ring + s * Tile<D>::kBytes + lane * L::kBytes,
-                  a.pool + (((int64_t)pid * a.Hkv + a_head) * UP + a_sub) * (int64_t)L::kBytes,
+                  a.pool + (((int64_t)f.pid * a.Hkv + f.head) * UP + f.sub) * (int64_t)L::kBytes,
                   one_copy ? bytes : L::kBytes, &bar[s]);
     };
-    look();
-    int looked = 0;  // tiles issued
-    while (true) {
-      issue(looked);
-      ++looked;
-      if (looked < count) step();
-      if (looked >= min(kStages, count)) break;
+    static_assert(kStages == 2, "two look-ups start the ring");
+    Look next = look();
+    int looked = 1;  // tiles issued
+    if (count > 1) {
+      const Look zeroth = next;
+      next = step();
+      issue(0, zeroth);
+      issue(1, next);
+      looked = 2;
+      if (count > 2) next = step();
+    } else {
+      issue(0, next);
     }
 
     // state of the current segment
@@ -316,26 +378,30 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
       if (fresh) {
         fresh = false;
         from_start = cur.k == 0;
-        const int hk = cur.seg % a.Hkv, z = cur.seg / a.Hkv;
+        int z, hk;
+        split_segment(a, cur.seg, z, hk);
         len = length_of(a, cur.b);
         nq = queries_of(a, cur.b);
         base = len - nq;
         ve = -110;
         const int rows = a.G * a.T;
-        lo_pos = max(0, base + z * RT / a.G);
+        int t, gi;
+        split_row(a, z * RT, t, gi);
+        lo_pos = max(0, base + t);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           // the query row of this thread's B fragments: column g8 = (row g8 / 2, part g8 & 1)
-          const int r2 = min(z * RT + n * 4 + (g8 >> 1), rows - 1);
-          const T* qp = q + cur.b * a.st.s[0] + (hk * a.G + r2 % a.G) * a.st.s[1] + (r2 / a.G) * a.st.s[2];
+          split_row(a, min(z * RT + n * 4 + (g8 >> 1), rows - 1), t, gi);
+          const T* qp = q + cur.b * a.st.s[0] + (hk * a.G + gi) * a.st.s[1] + t * a.st.s[2];
           float x[NG][8 * KW], top = 0.f;
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int e = 0; e < 8 * KW; ++e) {
-              x[g][e] = to_f(qp[g * DG + t4 * 8 * KW + e]);
-              top = fmaxf(top, fabsf(x[g][e]));
-            }
+            for (int w = 0; w < KW; ++w) load8(qp + g * DG + t4 * 8 * KW + 8 * w, x[g] + 8 * w);
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int e = 0; e < 8 * KW; e += 2) top = fmax3(top, fabsf(x[g][e]), fabsf(x[g][e + 1]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           // power of two that brings the row's largest value to 2^13 .. 2^14 (fp16 ends at 2^16)
@@ -343,31 +409,32 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
           const float up = pow2(13 - ex);
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            float sum = 0.f, part[8 * KW];
-#pragma unroll
-            for (int e = 0; e < 8 * KW; ++e) {
-              const float y = x[g][e] * up, hi = __half2float(__float2half_rn(y));
-              part[e] = (g8 & 1) ? __half2float(__float2half_rn(y - hi)) : hi;
-              sum += part[e];
-            }
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < KW; ++w)
 #pragma unroll
-              for (int p = 0; p < 2; ++p) {
-                qf[n][g][2 * w + p][0] = pack2<__half>(part[8 * w + 2 * p], part[8 * w + 2 * p + 4]);
-                // the codes of these dims are 16 times as large
-                qf[n][g][2 * w + p][1] = pack2<__half>(part[8 * w + 2 * p + 1] * 0.0625f, part[8 * w + 2 * p + 5] * 0.0625f);
+              for (int p = 0; p < 4; ++p) {
+                const float2 y = fmul2(make_float2(x[g][8 * w + p], x[g][8 * w + p + 4]), make_float2(up, up));
+                sum = fadd2(sum, y);
+                // the codes of the odd pairs are 16 times as large
+                const float2 v = p & 1 ? fmul2(y, make_float2(0.0625f, 0.0625f)) : y;
+                uint32_t f = pack2<__half>(v.x, v.y);
+                if (g8 & 1) {  // the low part; values of 16 bits have none
+                  const float2 hi = __half22float2(*reinterpret_cast<__half2*>(&f));
+                  f = sizeof(T) == 4 ? pack2<__half>(v.x - hi.x, v.y - hi.y) : 0u;
+                }
+                qf[n][g][2 * w + (p >> 1)][p & 1] = f;
               }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-            sq[n][g] = __shfl_sync(0xffffffffu, sum, 8 * t4) * pow2(-24);
+            float all = sum.x + sum.y;
+            all += __shfl_xor_sync(0xffffffffu, all, 1);
+            all += __shfl_xor_sync(0xffffffffu, all, 2);
+            sq[n][g] = __shfl_sync(0xffffffffu, all, 8 * t4) * pow2(-24);
           }
           const int exr = __shfl_sync(0xffffffffu, ex, 8 * t4);
           // the query row whose scores this thread holds; logits in units of log 2
-          const int r = min(z * RT + n * 4 + t4, rows - 1);
-          const int h = hk * a.G + r % a.G;
-          pos[n] = max(0, base + min(r / a.G, nq - 1));
+          split_row(a, min(z * RT + n * 4 + t4, rows - 1), t, gi);
+          const int h = hk * a.G + gi;
+          pos[n] = max(0, base + min(t, nq - 1));
           const float rc = a.ssmax[h] * logf((float)pos[n] + 1.f) * kLog2e;
           qr[n] = a.scale * rc * 2048.f * pow2(exr);
           ar[n] = -a.alpha[h] * rc;
@@ -396,19 +463,13 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
       const uint32_t units = (valid >> (TU * s)) & ((1u << TU) - 1);
       const int k0 = cur.k * KT;
 
-      // W: every key of the tile is there and visible to every row
-      auto attend = [&](auto whole) {
-        constexpr bool W = decltype(whole)::value;
+      {
         const int r0 = key_of_row(g8);
         float2 x[NT][TU];
         float top[NT], dk[NT];
         uint32_t vp[TU][NG][2];
-        float big = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          top[n] = -INFINITY;
-          dk[n] = (float)(k0 - pos[n]) + kf;
-        }
+        for (int n = 0; n < NT; ++n) dk[n] = (float)(k0 - pos[n]) + kf;
 #pragma unroll
         for (int u = 0; u < TU; ++u) {
           const uint8_t* unit = tile + u * L::kBytes;
@@ -444,13 +505,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
             const uint32_t* kp = reinterpret_cast<const uint32_t*>(unit + L::kKp) + g * kUnit + r0;
             const uint32_t p0 = kp[0], p1 = kp[8];
             const uint32_t* vq = reinterpret_cast<const uint32_t*>(unit + L::kVp) + g * kUnit + r0;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              vp[u][g][e] = vq[8 * e];
-              // what lies in a slot that holds no token may be any pair
-              if (!W && (!((units >> u) & 1u) || k0 + u * kUnit + r0 + 8 * e >= len)) vp[u][g][e] = 0u;
-              big = fmaxf(big, kv4::pair_scale(vp[u][g][e]));
-            }
+            vp[u][g][0] = vq[0], vp[u][g][1] = vq[8];
             const float2 ks = make_float2(kv4::pair_scale(p0), kv4::pair_scale(p1));
             const float2 km = make_float2(kv4::pair_centre(p0), kv4::pair_centre(p1));
 #pragma unroll
@@ -473,15 +528,36 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
               const float2 ln = fmul2(make_float2(lg2_(dist.x), lg2_(dist.y)), make_float2(be[n], be[n]));
               pw = make_float2(ex2f_(ln.x), ex2f_(ln.y));
             }
-            float2 y = ffma2(dot[n], make_float2(qr[n], qr[n]), fmul2(pw, make_float2(ar[n], ar[n])));
-            if (!W) {
-              const bool there = (units >> u) & 1u;
-              if (!there || gap.x > 0.f) y.x = -INFINITY;
-              if (!there || gap.y > 0.f) y.y = -INFINITY;
-            }
-            x[n][u] = y;
-            top[n] = fmax3(top[n], y.x, y.y);
+            x[n][u] = ffma2(dot[n], make_float2(qr[n], qr[n]), fmul2(pw, make_float2(ar[n], ar[n])));
           }
+        }
+        if (units != (1u << TU) - 1 || k0 + KT - 1 > lo_pos) {
+          // keys that a row does not see weigh nothing; a slot that holds no token may hold any pair,
+          // which must not meet the weight 0
+#pragma unroll
+          for (int u = 0; u < TU; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int key = k0 + u * kUnit + r0 + 8 * e;
+              const bool there = (units >> u) & 1u;
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                if (!there || key > pos[n]) (e ? x[n][u].y : x[n][u].x) = -INFINITY;
+#pragma unroll
+              for (int g = 0; g < NG; ++g)
+                if (!there || key >= len) vp[u][g][e] = 0u;
+            }
+        }
+        float big = 0.f;
+#pragma unroll
+        for (int u = 0; u < TU; ++u)
+#pragma unroll
+          for (int g = 0; g < NG; ++g) big = fmax3(big, kv4::pair_scale(vp[u][g][0]), kv4::pair_scale(vp[u][g][1]));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          top[n] = m[n];
+#pragma unroll
+          for (int u = 0; u < TU; ++u) top[n] = fmax3(top[n], x[n][u].x, x[n][u].y);
         }
 
         // o is kept against the largest V scale so far: p s 2^(14 - ve) stays below fp16's end
@@ -493,10 +569,9 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], d));
-          const float mn = fmaxf(m[n], top[n]);
-          const float shift = mn == -INFINITY ? 0.f : mn;
+          const float shift = top[n] == -INFINITY ? 0.f : top[n];
           const float f = exp2f(m[n] - shift);
-          m[n] = mn;
+          m[n] = top[n];
           if (__any_sync(0xffffffffu, f * vdown != 1.f)) {
             l[n] *= f;
 #pragma unroll
@@ -528,12 +603,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
             uint32_t bf[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              float2 ps = fmul2(x[n][u], vn2);
-              float2 pc = fmul2(x[n][u], vm);
-              if (!W) {  // a weight of 0 leaves out even a NaN (a later token of the same request)
-                if (x[n][u].x == 0.f) ps.x = pc.x = 0.f;
-                if (x[n][u].y == 0.f) ps.y = pc.y = 0.f;
-              }
+              const float2 ps = fmul2(x[n][u], vn2);
+              const float2 pc = fmul2(x[n][u], vm);
               pm[n][g] += pc.x + pc.y;
               // 11 bits each: the high part is cut off, exactly a number of fp16
               const float2 hi = make_float2(__uint_as_float(__float_as_uint(ps.x) & 0xffffe000u),
@@ -560,27 +631,27 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
             }
           }
         }
-      };
-      if (units == (1u << TU) - 1 && k0 + KT - 1 <= lo_pos) attend(std::true_type());
-      else attend(std::false_type());
+      }
 
       __syncwarp();  // every lane is done with the stage
       if (looked < count) {
         fence_proxy_async_smem();
-        issue(s);
-        if (++looked < count) step();
+        issue(s, next);
+        if (++looked < count) next = step();
       }
       if (++s == kStages) s = 0, phase ^= 1;
 
       const bool ends = cur.k + 1 == cur.nt;
       if (ends || i + 1 == count) {
-        const int hk = cur.seg % a.Hkv, z = cur.seg / a.Hkv;
+        int z, hk;
+        split_segment(a, cur.seg, z, hk);
         const bool direct = ends && from_start;
         // the run's last piece goes where the ring was
         const int which = i + 1 == count ? 1 : 0;
         float* part = piece_at(warp, which);
         if (!direct && lane == 0) {
-          pieces[warp][which].segment = (int64_t)cur.b * zh + cur.seg;
+          pieces[warp][which].b = cur.b;
+          pieces[warp][which].seg = cur.seg;
           pieces[warp][which].begins = from_start;
           pieces[warp][which].ends = ends;
         }
@@ -594,7 +665,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
             for (int g = 0; g < NG; ++g) pm[n][g] += __shfl_xor_sync(0xffffffffu, pm[n][g], d);
           }
           const int r = z * RT + n * 4 + t4;
-          const int t = r / a.G;
+          int t, gi;
+          split_row(a, r, t, gi);
           const bool sees = t < nq && base + t >= 0;
           const float inv = direct ? (sees && l[n] != 0.f ? 1.f / l[n] : 0.f) : 1.f;
 #pragma unroll
@@ -608,9 +680,10 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
             const int d0 = g * DG + g8 * 2 * MT;
             if (direct) {
               if (r < a.G * a.T) {
-                T* dst = out + cur.b * a.st.s[3] + (hk * a.G + r % a.G) * a.st.s[4] + t * a.st.s[5] + d0;
+                T* dst = out + cur.b * a.st.s[3] + (hk * a.G + gi) * a.st.s[4] + t * a.st.s[5] + d0;
 #pragma unroll
-                for (int j = 0; j < 2 * MT; ++j) dst[j] = from_f<T>(sees ? y[j] : 0.f);
+                for (int j = 0; j < 2 * MT; j += 4)
+                  store4(dst + j, make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]), 1.f, sees);
               }
             } else {
               float* dst = part + (n * 4 + t4) * (D + 4) + d0;
@@ -634,53 +707,55 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
   // CTA holds all of the segment, else left to the merge (slot 0 where the segment began before this
   // CTA's run, 1 where it began in it).
   if (__syncthreads_or(failed)) return;
-  for (int first = 0; first < 2 * kWarps;) {
+  constexpr int SLOTS = 2 * kWarps;
+  for (int first = 0; first < SLOTS;) {
     const Piece head = pieces[first >> 1][first & 1];
-    if (head.segment < 0) {
+    if (head.b < 0) {
       ++first;
       continue;
     }
     uint32_t members = 1u << first;
     int ends = head.ends, next = first + 1;
-    for (; next < 2 * kWarps; ++next) {
+    for (; next < SLOTS; ++next) {
       const Piece& p = pieces[next >> 1][next & 1];
-      if (p.segment < 0) continue;
-      if (p.segment != head.segment) break;
+      if (p.b < 0) continue;
+      if (p.b != head.b || p.seg != head.seg) break;
       members |= 1u << next;
       ends = p.ends;
     }
     const bool direct = head.begins && ends;
-    const int b = (int)(head.segment / zh), seg = (int)(head.segment % zh);
-    const int hk = seg % a.Hkv, z = seg / a.Hkv;
+    const int b = head.b;
+    int z, hk;
+    split_segment(a, head.seg, z, hk);
     const int nq = queries_of(a, b), base = length_of(a, b) - nq;
     float* part = a.ws + ((int64_t)blockIdx.x * 2 + (head.begins ? 1 : 0)) * piece_floats<D, NT>();
     for (int v = threadIdx.x; v < RT * (D / 4); v += THREADS) {
       const int rr = v / (D / 4), d = v % (D / 4) * 4;
-      float mx = -INFINITY;
-      for (uint32_t w = members; w; w &= w - 1) {
-        const int i = __ffs(w) - 1;
-        mx = fmaxf(mx, piece_at(i >> 1, i & 1)[rr * (D + 4) + D]);
+      float mi[SLOTS], mx = -INFINITY, den = 0.f;
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i) {
+        mi[i] = (members >> i) & 1u ? piece_at(i >> 1, i & 1)[rr * (D + 4) + D] : -INFINITY;
+        mx = fmaxf(mx, mi[i]);
       }
       const float shift = mx == -INFINITY ? 0.f : mx;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float den = 0.f;
-      for (uint32_t w = members; w; w &= w - 1) {
-        const int i = __ffs(w) - 1;
-        const float* src = piece_at(i >> 1, i & 1) + rr * (D + 4);
-        const float f = exp2f(src[D] - shift);
-        const float4 y = *reinterpret_cast<const float4*>(src + d);
-        acc.x = fmaf(f, y.x, acc.x), acc.y = fmaf(f, y.y, acc.y);
-        acc.z = fmaf(f, y.z, acc.z), acc.w = fmaf(f, y.w, acc.w);
-        den = fmaf(f, src[D + 1], den);
-      }
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i)
+        if ((members >> i) & 1u) {
+          const float* src = piece_at(i >> 1, i & 1) + rr * (D + 4);
+          const float f = exp2f(mi[i] - shift);
+          const float4 y = *reinterpret_cast<const float4*>(src + d);
+          acc.x = fmaf(f, y.x, acc.x), acc.y = fmaf(f, y.y, acc.y);
+          acc.z = fmaf(f, y.z, acc.z), acc.w = fmaf(f, y.w, acc.w);
+          den = fmaf(f, src[D + 1], den);
+        }
       if (direct) {
-        const int r = z * RT + rr, t = r / a.G;
+        const int r = z * RT + rr;
+        int t, gi;
+        split_row(a, r, t, gi);
         if (r < a.G * a.T) {
-          const float inv = t < nq && base + t >= 0 && den != 0.f ? 1.f / den : 0.f;
-          T* dst = out + b * a.st.s[3] + (hk * a.G + r % a.G) * a.st.s[4] + t * a.st.s[5] + d;
-          const bool sees = t < nq && base + t >= 0;
-          dst[0] = from_f<T>(sees ? acc.x * inv : 0.f), dst[1] = from_f<T>(sees ? acc.y * inv : 0.f);
-          dst[2] = from_f<T>(sees ? acc.z * inv : 0.f), dst[3] = from_f<T>(sees ? acc.w * inv : 0.f);
+          const bool sees = t < nq && base + t >= 0 && den != 0.f;
+          store4(out + b * a.st.s[3] + (hk * a.G + gi) * a.st.s[4] + t * a.st.s[5] + d, acc, sees ? 1.f / den : 0.f, sees);
         }
       } else {
         *reinterpret_cast<float4*>(part + rr * (D + 4) + d) = acc;
@@ -695,81 +770,78 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
 }
 
 // ------------------------------------------------------------------ merge
-// One CTA per segment: joins the CTAs' partials of a segment that spans several, in a fixed order
-// (each group of D RT / 4 threads takes every n-th partial, the groups are summed in order), and
-// zeroes the rows of a segment without tiles.
-constexpr int kMergeThreads = 512;
+// One CTA per segment: joins the CTAs' partials of a segment that spans several, and zeroes the rows
+// of a segment without tiles.  Thread group i of D RT / 4 threads takes partials i, i + PL, ... in one
+// pass with a running maximum; the groups are joined in order.  256 threads of 32 registers find
+// room beside the worker CTAs, so the search for the segment's CTAs runs before they end.
+constexpr int kMergeThreads = 256;
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(T* __restrict__ out, const Args a) {
   constexpr int KT = Tile<D>::kKeys, RT = 4 * NT, NV = RT * D / 4, PL = kMergeThreads / NV;
   static_assert(NV <= kMergeThreads && kMergeThreads % NV == 0, "whole groups of threads");
-  __shared__ int64_t pre[kMergeThreads + 1];
-  __shared__ float s_shift[RT], s_den[RT];
+  __shared__ float s_m[PL][RT], s_l[PL][RT];
   __shared__ float4 s_acc[PL][NV];
-  scan_requests<KT, kMergeThreads>(a, pre);
-  const int zh = a.Z * a.Hkv, run = (a.B + kMergeThreads - 1) / kMergeThreads;
-  const int b = blockIdx.x / zh, seg = blockIdx.x % zh;
-  const int hk = seg % a.Hkv, z = seg / a.Hkv;
-  int64_t before = pre[b / run];
-  for (int i = b / run * run; i < b; ++i) before += tiles_of<KT>(a, i);
-  const int64_t total = pre[kMergeThreads] * zh;
-  const int nt = tiles_of<KT>(a, b);
-  const int64_t x0 = before * zh + (int64_t)seg * nt;
-  int64_t c0 = 0;
-  int n = 0;  // partials
+  const int tid = threadIdx.x;
+  const Requests reqs = scan_requests<KT>(a);
+  const int zh = a.Z * a.Hkv;
+  const int b = blockIdx.x / zh, seg = blockIdx.x - b * zh;
+  // tiles before request b: the runs before its own, then the requests before it in its run
+  const int c = b / reqs.run;
+  int before = __shfl_sync(0xffffffffu, reqs.upto - reqs.mine, c);
+  for (int i = c * reqs.run; i < b; ++i) before += tiles_of<KT>(a, i);
+  const int nt = tiles_of<KT>(a, b), x0 = before * zh + seg * nt;
+  int c0 = 0, n = 0;  // first CTA, partials
   if (nt > 0) {
-    const int64_t working = working_ctas(total, a.ctas);
-    c0 = cta_of(total, working, x0);
-    n = (int)(cta_of(total, working, x0 + nt - 1) - c0) + 1;
+    const Cut cut(reqs.total, a.ctas);
+    c0 = cut.cta_of(x0);
+    n = cut.cta_of(x0 + nt - 1) - c0 + 1;
   }
+  const int v = tid % NV, pl = tid / NV, rr = v / (D / 4), d = v % (D / 4) * 4;
+  const int nq = queries_of(a, b), base = length_of(a, b) - nq;
+  int z, hk, t, gi;
+  split_segment(a, seg, z, hk);
+  const int r = z * RT + rr;
+  split_row(a, r, t, gi);
   // every CTA waits, also those without work: what follows this grid must find the workers' done
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (n == 1) return;  // written by its CTA
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // the first CTA's slot 1 (the segment began in its run), every other one's slot 0
-  auto slot = [&](int i) { return a.ws + ((c0 + i) * 2 + (i == 0 ? 1 : 0)) * piece_floats<D, NT>(); };
-  if (n > 0) {
-    for (int rr = warp; rr < RT; rr += kMergeThreads / 32) {
-      float mx = -INFINITY, den = 0.f;
-      for (int i = lane; i < n; i += 32) mx = fmaxf(mx, slot(i)[rr * (D + 4) + D]);
-      mx = warp_max(mx);
-      if (mx == -INFINITY) mx = 0.f;
-      for (int i = lane; i < n; i += 32)
-        den = fmaf(exp2f(slot(i)[rr * (D + 4) + D] - mx), slot(i)[rr * (D + 4) + D + 1], den);
-      den = warp_sum(den);
-      if (lane == 0) s_shift[rr] = mx, s_den[rr] = den;
-    }
-  }
-  __syncthreads();
-  const int v = tid % NV, pl = tid / NV, rr = v / (D / 4), d = v % (D / 4) * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (n > 0) {
-    const float shift = s_shift[rr];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll 4
-    for (int i = pl; i < n; i += PL) {
-      const float* src = slot(i) + rr * (D + 4);
-      const float f = exp2f(src[D] - shift);
-      const float4 y = *reinterpret_cast<const float4*>(src + d);
-      acc.x = fmaf(f, y.x, acc.x), acc.y = fmaf(f, y.y, acc.y);
-      acc.z = fmaf(f, y.z, acc.z), acc.w = fmaf(f, y.w, acc.w);
-    }
+  for (int i = pl; i < n; i += PL) {
+    // the first CTA's slot 1 (the segment began in its run), every other one's slot 0
+    const float* src = a.ws + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * piece_floats<D, NT>() + rr * (D + 4);
+    const float4 y = *reinterpret_cast<const float4*>(src + d);
+    const float2 ml = *reinterpret_cast<const float2*>(src + D);
+    const float mn = fmaxf(m, ml.x), shift = mn == -INFINITY ? 0.f : mn;
+    const float f = exp2f(m - shift), fi = exp2f(ml.x - shift);
+    acc.x = fmaf(fi, y.x, acc.x * f), acc.y = fmaf(fi, y.y, acc.y * f);
+    acc.z = fmaf(fi, y.z, acc.z * f), acc.w = fmaf(fi, y.w, acc.w * f);
+    l = fmaf(fi, ml.y, l * f);
+    m = mn;
   }
   s_acc[pl][v] = acc;
+  if (d == 0) s_m[pl][rr] = m, s_l[pl][rr] = l;
   __syncthreads();
   if (pl) return;
-  for (int i = 1; i < PL; ++i) {
+  m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) m = fmaxf(m, s_m[i][rr]);
+  const float shift = m == -INFINITY ? 0.f : m;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) {
+    const float f = exp2f(s_m[i][rr] - shift);
     const float4 y = s_acc[i][v];
-    acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
+    acc.x = fmaf(f, y.x, acc.x), acc.y = fmaf(f, y.y, acc.y);
+    acc.z = fmaf(f, y.z, acc.z), acc.w = fmaf(f, y.w, acc.w);
+    l = fmaf(f, s_l[i][rr], l);
   }
-  const int nq = queries_of(a, b), base = length_of(a, b) - nq;
-  const int r = z * RT + rr, t = r / a.G;
   if (r >= a.G * a.T) return;
-  const bool sees = n > 0 && t < nq && base + t >= 0 && s_den[rr] != 0.f;
-  const float inv = sees ? 1.f / s_den[rr] : 0.f;
-  T* dst = out + b * a.st.s[3] + (hk * a.G + r % a.G) * a.st.s[4] + t * a.st.s[5] + d;
-  dst[0] = from_f<T>(sees ? acc.x * inv : 0.f), dst[1] = from_f<T>(sees ? acc.y * inv : 0.f);
-  dst[2] = from_f<T>(sees ? acc.z * inv : 0.f), dst[3] = from_f<T>(sees ? acc.w * inv : 0.f);
+  const bool sees = t < nq && base + t >= 0 && l != 0.f;
+  store4(out + b * a.st.s[3] + (hk * a.G + gi) * a.st.s[4] + t * a.st.s[5] + d, acc, sees ? 1.f / l : 0.f, sees);
 }
 
 // ------------------------------------------------------------------ host side
@@ -866,10 +938,15 @@ extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, c
     a.B = (int)B, a.H = (int)H, a.Hkv = (int)Hkv, a.T = (int)T, a.G = (int)(H / Hkv);
     a.P = (int)page_size, a.columns = (int)max_pages, a.pages = num_pages;
     a.scale = scale, a.eps = eps;
+    if (int rc = check_rows16("kv4_chord_attention", q, strides, sizeof(E))) return rc;
+    if (int rc = check_rows16("kv4_chord_attention", out, strides + 3, sizeof(E))) return rc;
     const int nt = row_tile((int64_t)a.G * T, D);
     a.Z = (int)(((int64_t)a.G * T + 4 * nt - 1) / (4 * nt));
     a.ctas = sm_count() * ctas_per_sm(nt, (int)D);
-    MB_REQUIRE((int64_t)a.B * a.Z * a.Hkv < (1ll << 31), MB_ERR_SHAPE, "kv4_chord_attention: too many rows");
+    const int64_t tiles = (max_pages * page_size + Tile<DD>::kKeys - 1) / Tile<DD>::kKeys;
+    MB_REQUIRE((int64_t)a.B * a.Z * a.Hkv * tiles < (1ll << 31), MB_ERR_SHAPE,
+               "kv4_chord_attention: B * Hkv * row tiles * key tiles = %lld (fewer than 2^31)",
+               (long long)((int64_t)a.B * a.Z * a.Hkv * tiles));
     if (nt == 1) return launch<E, DD, 1>(q, out, a, (cudaStream_t)stream);
     if constexpr (DD < 128)
       if (nt == 4) return launch<E, DD, 4>(q, out, a, (cudaStream_t)stream);

@@ -230,8 +230,7 @@ def kv4_chord_attention(q, pool, block_table, lens, alpha, beta, mu, ssmax, q_le
         _int32('q_lens', q_lens, (B,), dev)
     for name, t in (('alpha', alpha), ('beta', beta), ('mu', mu), ('ssmax', ssmax)):
         _int32(name, t, (H,), dev, torch.float32)
-    if q.stride(3) != 1:
-        q = q.contiguous()
+    q = _rows16(q)
     out = torch.empty((B, H, T, D), dtype=q.dtype, device=dev)
     ws_bytes = _lib.load().motif_b200_kv4_attention_workspace_bytes(H, kv, T, D)
     ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
