@@ -366,7 +366,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
     uint32_t qf[NT][NG][2 * KW][2];
     float sq[NT][NG], qr[NT], ar[NT], be[NT], mh[NT];
     int pos[NT];
-    float o[NT][NG][MT][4], m[NT], l[NT], pm[NT][NG];
+    float o[NT][NG][MT][4], m[NT];
+    float2 l[NT], pm[NT][NG];  // of the thread's keys of rows 0 .. 7 and 8 .. 15 of the units
     int ve = 0;        // o holds p s 2^(14 - ve): the exponent of the largest V scale so far
     int lo_pos = 0;    // smallest position of a row that sees keys
     int nq = 0, base = 0, len = 0;
@@ -441,24 +442,18 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
           be[n] = a.beta[h];
           mh[n] = -a.mu[h];
           m[n] = -INFINITY;
-          l[n] = 0.f;
+          l[n] = make_float2(0.f, 0.f);
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            pm[n][g] = 0.f;
+            pm[n][g] = make_float2(0.f, 0.f);
 #pragma unroll
             for (int t = 0; t < MT; ++t) o[n][g][t][0] = o[n][g][t][1] = o[n][g][t][2] = o[n][g][t][3] = 0.f;
           }
         }
       }
 
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bar[s], (uint32_t)phase, kWaitLimit))) {
-        // never expected: the error is counted, copies in flight are waited for, the rows stay unwritten
-        if (lane == 0) atomicAdd(&g_kv4_wait_timeouts, 1u);
-        for (int j = i + 1; j < looked; ++j)
-          mbar_wait_bounded(&bar[j % kStages], (uint32_t)((j / kStages) & 1), kWaitLimit);
-        failed = true;
-        break;
-      }
+      // never expected to run out: the rows then stay unwritten
+      failed |= !mbar_wait_bounded(&bar[s], (uint32_t)phase, kWaitLimit);
       const uint8_t* tile = ring + s * Tile<D>::kBytes;
       const uint32_t units = (valid >> (TU * s)) & ((1u << TU) - 1);
       const int k0 = cur.k * KT;
@@ -466,10 +461,14 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
       {
         const int r0 = key_of_row(g8);
         float2 x[NT][TU];
-        float top[NT], dk[NT];
+        float2 gap[NT];  // key - pos: a whole number, exact
+        float top[NT];
         uint32_t vp[TU][NG][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) dk[n] = (float)(k0 - pos[n]) + kf;
+        for (int n = 0; n < NT; ++n) {
+          const float d = (float)(k0 - pos[n]) + kf;
+          gap[n] = make_float2(d, d + 8.f);
+        }
 #pragma unroll
         for (int u = 0; u < TU; ++u) {
           const uint8_t* unit = tile + u * L::kBytes;
@@ -511,15 +510,14 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const float2 s2 = make_float2(sq[n][g], sq[n][g]);
-              const float2 both = fadd2(make_float2(acc[n][0], acc[n][2]), make_float2(acc[n][1], acc[n][3]));
+              const float2 both = make_float2(acc[n][0] + acc[n][1], acc[n][2] + acc[n][3]);
               dot[n] = g ? ffma2(ks, both, ffma2(km, s2, dot[n])) : ffma2(ks, both, fmul2(km, s2));
             }
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            // key - pos is a whole number: exact; -mu, |.| + eps round as in the formula
-            const float2 gap = fadd2(make_float2(dk[n], dk[n]), make_float2(u * 16.f, u * 16.f + 8.f));
-            const float2 off = fadd2(gap, make_float2(mh[n], mh[n]));
+            const float2 off = fadd2(gap[n], make_float2(mh[n], mh[n]));
+            if (u + 1 < TU) gap[n] = fadd2(gap[n], make_float2(16.f, 16.f));
             const float2 dist = make_float2(fabsf(off.x) + a.eps, fabsf(off.y) + a.eps);
             float2 pw;
             if constexpr (sizeof(T) == 4) {
@@ -570,24 +568,28 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], d));
           const float shift = top[n] == -INFINITY ? 0.f : top[n];
-          const float f = exp2f(m[n] - shift);
+          const float f = sizeof(T) == 4 ? exp2f(m[n] - shift) : ex2f_(m[n] - shift);
           m[n] = top[n];
           if (__any_sync(0xffffffffu, f * vdown != 1.f)) {
-            l[n] *= f;
+            const float2 f2 = make_float2(f, f), fo = make_float2(f * vdown, f * vdown);
+            l[n] = fmul2(l[n], f2);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-              pm[n][g] *= f;
+              pm[n][g] = fmul2(pm[n][g], f2);
 #pragma unroll
               for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[n][g][t][e] *= f * vdown;
+                for (int e = 0; e < 4; e += 2) {
+                  const float2 y = fmul2(make_float2(o[n][g][t][e], o[n][g][t][e + 1]), fo);
+                  o[n][g][t][e] = y.x, o[n][g][t][e + 1] = y.y;
+                }
             }
           }
 #pragma unroll
           for (int u = 0; u < TU; ++u) {
             const float2 y = fadd2(x[n][u], make_float2(-shift, -shift));
             x[n][u] = sizeof(T) == 4 ? make_float2(exp2f(y.x), exp2f(y.y)) : make_float2(ex2f_(y.x), ex2f_(y.y));
-            l[n] += x[n][u].x + x[n][u].y;
+            l[n] = fadd2(l[n], x[n][u]);
           }
         }
 
@@ -604,13 +606,13 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const float2 ps = fmul2(x[n][u], vn2);
-              const float2 pc = fmul2(x[n][u], vm);
-              pm[n][g] += pc.x + pc.y;
+              pm[n][g] = ffma2(x[n][u], vm, pm[n][g]);
               // 11 bits each: the high part is cut off, exactly a number of fp16
               const float2 hi = make_float2(__uint_as_float(__float_as_uint(ps.x) & 0xffffe000u),
                                             __uint_as_float(__float_as_uint(ps.y) & 0xffffe000u));
-              bf[n][0] = transpose8x8(pack2<__half>(hi.x, ps.x - hi.x));
-              bf[n][1] = transpose8x8(pack2<__half>(hi.y, ps.y - hi.y));
+              const float2 lo = ffma2(hi, make_float2(-1.f, -1.f), ps);
+              bf[n][0] = transpose8x8(pack2<__half>(hi.x, lo.x));
+              bf[n][1] = transpose8x8(pack2<__half>(hi.y, lo.y));
             }
             const uint8_t* at = unit + L::kV + t4 * L::kRow + g * (DG / 2) + (KW == 2 ? 4 * g8 : 4 * (g8 >> 1));
             uint32_t w[4];
@@ -658,24 +660,27 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
         const float back = pow2(min(ve, 127));  // and 2^10
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+          float ln = l[n].x + l[n].y, pn[NG];
+#pragma unroll
+          for (int g = 0; g < NG; ++g) pn[g] = pm[n][g].x + pm[n][g].y;
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
-            l[n] += __shfl_xor_sync(0xffffffffu, l[n], d);
+            ln += __shfl_xor_sync(0xffffffffu, ln, d);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) pm[n][g] += __shfl_xor_sync(0xffffffffu, pm[n][g], d);
+            for (int g = 0; g < NG; ++g) pn[g] += __shfl_xor_sync(0xffffffffu, pn[g], d);
           }
           const int r = z * RT + n * 4 + t4;
           int t, gi;
           split_row(a, r, t, gi);
           const bool sees = t < nq && base + t >= 0;
-          const float inv = direct ? (sees && l[n] != 0.f ? 1.f / l[n] : 0.f) : 1.f;
+          const float inv = direct ? (sees && ln != 0.f ? 1.f / ln : 0.f) : 1.f;
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             float y[2 * MT];
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
-              y[2 * j] = fmaf((o[n][g][j][0] + o[n][g][j][1]) * 1024.f, back, pm[n][g]) * inv;
-              y[2 * j + 1] = fmaf((o[n][g][j][2] + o[n][g][j][3]) * 64.f, back, pm[n][g]) * inv;
+              y[2 * j] = fmaf((o[n][g][j][0] + o[n][g][j][1]) * 1024.f, back, pn[g]) * inv;
+              y[2 * j + 1] = fmaf((o[n][g][j][2] + o[n][g][j][3]) * 64.f, back, pn[g]) * inv;
             }
             const int d0 = g * DG + g8 * 2 * MT;
             if (direct) {
@@ -694,7 +699,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
           }
           if (!direct && g8 == 0) {
             part[(n * 4 + t4) * (D + 4) + D] = m[n];
-            part[(n * 4 + t4) * (D + 4) + D + 1] = l[n];
+            part[(n * 4 + t4) * (D + 4) + D + 1] = ln;
           }
         }
         fresh = true;
@@ -706,7 +711,10 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
   // The CTA's pieces in tile order: neighbours of one segment are joined, and written out where the
   // CTA holds all of the segment, else left to the merge (slot 0 where the segment began before this
   // CTA's run, 1 where it began in it).
-  if (__syncthreads_or(failed)) return;
+  if (__syncthreads_or(failed)) {  // each copy was waited for, so none is in flight
+    if (threadIdx.x == 0) atomicAdd(&g_kv4_wait_timeouts, 1u);
+    return;
+  }
   constexpr int SLOTS = 2 * kWarps;
   for (int first = 0; first < SLOTS;) {
     const Piece head = pieces[first >> 1][first & 1];
