@@ -37,10 +37,10 @@ using kv4::Layout;
 
 __device__ unsigned int g_kv4_wait_timeouts = 0;
 
-constexpr int kWarps = 4;
 constexpr int kStages = 2;
 constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 4.f;  // log 2 units
 
 struct Strides6 {
   int64_t s[6];  // q(b,h,t) out(b,h,t)
@@ -113,12 +113,12 @@ __device__ __forceinline__ Requests scan_requests(const Args& a) {
   return q;
 }
 
-// `total` tiles over at most `n` CTAs, at least one tile per warp: the first CTAs take one more than
-// the others.
+// `total` tiles over at most `n` CTAs, at least four each (one for a warp of every scheduler): the
+// first CTAs take one more than the others.
 struct Cut {
   int working, each, more;
   __device__ __forceinline__ Cut(int total, int n) {
-    working = min(n, (total + kWarps - 1) / kWarps);
+    working = min(n, (total + 3) / 4);
     each = working ? total / working : 0;
     more = total - each * working;
   }
@@ -245,6 +245,9 @@ __device__ __forceinline__ void store4(T* p, float4 y, float f, bool sees) {
 __device__ __forceinline__ int key_of_row(int r) { return (r >> 1) + 4 * (r & 1); }
 
 // ------------------------------------------------------------------ the worker kernel
+// Warps of the one CTA an SM runs, by the registers that the output tile takes.
+__host__ __device__ constexpr int warps_of(int nt, int D) { return nt == 1 || (nt == 2 && D <= 64) ? 12 : 8; }
+
 // An unfinished piece of a segment at the end of a warp's run: [RT rows][D + 4] floats (o, m, l), its
 // segment and whether it holds the segment's first / last tile.
 struct Piece {
@@ -260,15 +263,20 @@ constexpr int piece_floats() {
 template <int D, int NT>
 constexpr int attention_smem() {
   static_assert(piece_floats<D, NT>() * 4 <= kStages * Tile<D>::kBytes, "a piece fits the ring");
-  return kWarps * (kStages * Tile<D>::kBytes + piece_floats<D, NT>() * 4);
+  return warps_of(NT, D) * (kStages * Tile<D>::kBytes + piece_floats<D, NT>() * 4);
 }
 
-// CTAs per SM of the worker kernel, by the registers its output tile leaves.
-__host__ __device__ constexpr int ctas_per_sm(int nt, int D) { return nt == 1 ? (D <= 64 ? 4 : 3) : nt == 2 && D <= 64 ? 3 : 2; }
+// A CTA's `count` tiles over its W warps: warp w's run starts at tile run_start(count, w).  Fewer
+// tiles than warps go to the first ones, one of each scheduler in turn.
+template <int W>
+__device__ __forceinline__ int run_start(int count, int w) {
+  return count <= W ? min(w, count) : (int)((int64_t)count * w / W);
+}
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention_kernel(const T* __restrict__ q, T* __restrict__ out,
-                                                                    const Args a) {
+__global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(const T* __restrict__ q, T* __restrict__ out,
+                                                                       const Args a) {
+  constexpr int kWarps = warps_of(NT, D);
   using L = Layout<D>;
   constexpr int TU = Tile<D>::kUnits, KT = Tile<D>::kKeys;
   constexpr int NG = L::NG, DG = L::DG;
@@ -298,8 +306,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
   const Cut cut(reqs.total, gridDim.x);
   if ((int)blockIdx.x >= cut.working) return;
   const int cta_first = cut.start(blockIdx.x), cta_count = cut.each + ((int)blockIdx.x < cut.more ? 1 : 0);
-  const int run0 = (int)((int64_t)cta_count * warp / kWarps);
-  const int count = (int)((int64_t)cta_count * (warp + 1) / kWarps) - run0;
+  const int run0 = run_start<kWarps>(cta_count, warp);
+  const int count = run_start<kWarps>(cta_count, warp + 1) - run0;
 
   bool failed = false;
   if (count > 0) {
@@ -348,27 +356,19 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
                   a.pool + (((int64_t)f.pid * a.Hkv + f.head) * UP + f.sub) * (int64_t)L::kBytes,
                   one_copy ? bytes : L::kBytes, &bar[s]);
     };
-    static_assert(kStages == 2, "two look-ups start the ring");
     Look next = look();
-    int looked = 1;  // tiles issued
-    if (count > 1) {
-      const Look zeroth = next;
-      next = step();
-      issue(0, zeroth);
-      issue(1, next);
-      looked = 2;
-      if (count > 2) next = step();
-    } else {
-      issue(0, next);
-    }
+    int looked = 0;  // tiles issued
 
     // state of the current segment
     uint32_t qf[NT][NG][2 * KW][2];
     float sq[NT][NG], qr[NT], ar[NT], be[NT], mh[NT];
     int pos[NT];
-    float o[NT][NG][MT][4], m[NT];
+    // weights are taken against a reference that a row's logits exceed by 2^kSlack at most: it moves
+    // when a tile goes beyond that (limit[n] above it, relative), not with every new maximum
+    float o[NT][NG][MT][4], ref[NT], limit[NT];
     float2 l[NT], pm[NT][NG];  // of the thread's keys of rows 0 .. 7 and 8 .. 15 of the units
-    int ve = 0;        // o holds p s 2^(14 - ve): the exponent of the largest V scale so far
+    int ve = 0;        // o holds p s 2^(10 - ve): the exponent of the largest V scale so far
+    float vup = 0.f, vtop = 0.f;  // 2^(10 - ve), 2^(ve + 1) (0: no tile yet)
     int lo_pos = 0;    // smallest position of a row that sees keys
     int nq = 0, base = 0, len = 0;
     const float kf = (float)key_of_row(g8);
@@ -385,24 +385,44 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
         nq = queries_of(a, cur.b);
         base = len - nq;
         ve = -110;
+        vup = pow2(120);
+        vtop = 0.f;
         const int rows = a.G * a.T;
         int t, gi;
         split_row(a, z * RT, t, gi);
         lo_pos = max(0, base + t);
+        float x[NT][NG][8 * KW];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           // the query row of this thread's B fragments: column g8 = (row g8 / 2, part g8 & 1)
           split_row(a, min(z * RT + n * 4 + (g8 >> 1), rows - 1), t, gi);
           const T* qp = q + cur.b * a.st.s[0] + (hk * a.G + gi) * a.st.s[1] + t * a.st.s[2];
-          float x[NG][8 * KW], top = 0.f;
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int w = 0; w < KW; ++w) load8(qp + g * DG + t4 * 8 * KW + 8 * w, x[g] + 8 * w);
+            for (int w = 0; w < KW; ++w) load8(qp + g * DG + t4 * 8 * KW + 8 * w, x[n][g] + 8 * w);
+          // the query row whose scores this thread holds; logits in units of log 2
+          split_row(a, min(z * RT + n * 4 + t4, rows - 1), t, gi);
+          const int h = hk * a.G + gi;
+          pos[n] = max(0, base + min(t, nq - 1));
+          qr[n] = a.ssmax[h];
+          ar[n] = a.alpha[h];
+          be[n] = a.beta[h];
+          mh[n] = -a.mu[h];
+        }
+        if (i == 0) {
+          // the first copies go out after the loads above, which would wait behind every warp's copies
+          issue(0, next);
+          looked = 1;
+          if (count > 1) next = step();
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float top = 0.f;
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int e = 0; e < 8 * KW; e += 2) top = fmax3(top, fabsf(x[g][e]), fabsf(x[g][e + 1]));
+            for (int e = 0; e < 8 * KW; e += 2) top = fmax3(top, fabsf(x[n][g][e]), fabsf(x[n][g][e + 1]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           // power of two that brings the row's largest value to 2^13 .. 2^14 (fp16 ends at 2^16)
@@ -415,7 +435,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
             for (int w = 0; w < KW; ++w)
 #pragma unroll
               for (int p = 0; p < 4; ++p) {
-                const float2 y = fmul2(make_float2(x[g][8 * w + p], x[g][8 * w + p + 4]), make_float2(up, up));
+                const float2 y = fmul2(make_float2(x[n][g][8 * w + p], x[n][g][8 * w + p + 4]), make_float2(up, up));
                 sum = fadd2(sum, y);
                 // the codes of the odd pairs are 16 times as large
                 const float2 v = p & 1 ? fmul2(y, make_float2(0.0625f, 0.0625f)) : y;
@@ -432,16 +452,11 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
             sq[n][g] = __shfl_sync(0xffffffffu, all, 8 * t4) * pow2(-24);
           }
           const int exr = __shfl_sync(0xffffffffu, ex, 8 * t4);
-          // the query row whose scores this thread holds; logits in units of log 2
-          split_row(a, min(z * RT + n * 4 + t4, rows - 1), t, gi);
-          const int h = hk * a.G + gi;
-          pos[n] = max(0, base + min(t, nq - 1));
-          const float rc = a.ssmax[h] * logf((float)pos[n] + 1.f) * kLog2e;
+          const float rc = qr[n] * logf((float)pos[n] + 1.f) * kLog2e;
           qr[n] = a.scale * rc * 2048.f * pow2(exr);
-          ar[n] = -a.alpha[h] * rc;
-          be[n] = a.beta[h];
-          mh[n] = -a.mu[h];
-          m[n] = -INFINITY;
+          ar[n] *= -rc;
+          ref[n] = 0.f;
+          limit[n] = -INFINITY;
           l[n] = make_float2(0.f, 0.f);
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
@@ -452,6 +467,11 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
         }
       }
 
+      if (i == 0 && count > 1) {
+        issue(1, next);
+        looked = 2;
+        if (count > 2) next = step();
+      }
       // never expected to run out: the rows then stay unwritten
       failed |= !mbar_wait_bounded(&bar[s], (uint32_t)phase, kWaitLimit);
       const uint8_t* tile = ring + s * Tile<D>::kBytes;
@@ -526,7 +546,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
               const float2 ln = fmul2(make_float2(lg2_(dist.x), lg2_(dist.y)), make_float2(be[n], be[n]));
               pw = make_float2(ex2f_(ln.x), ex2f_(ln.y));
             }
-            x[n][u] = ffma2(dot[n], make_float2(qr[n], qr[n]), fmul2(pw, make_float2(ar[n], ar[n])));
+            x[n][u] = ffma2(dot[n], make_float2(qr[n], qr[n]), ffma2(pw, make_float2(ar[n], ar[n]), make_float2(-ref[n], -ref[n])));
           }
         }
         if (units != (1u << TU) - 1 || k0 + KT - 1 > lo_pos) {
@@ -551,26 +571,30 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
         for (int u = 0; u < TU; ++u)
 #pragma unroll
           for (int g = 0; g < NG; ++g) big = fmax3(big, kv4::pair_scale(vp[u][g][0]), kv4::pair_scale(vp[u][g][1]));
+        bool beyond = big >= vtop;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          top[n] = m[n];
+          top[n] = -INFINITY;
 #pragma unroll
           for (int u = 0; u < TU; ++u) top[n] = fmax3(top[n], x[n][u].x, x[n][u].y);
+          beyond = beyond || top[n] > limit[n];
         }
-
-        // o is kept against the largest V scale so far: p s 2^(14 - ve) stays below fp16's end
-        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-        const int vn = max(ve, (int)(bits >> 23) - 127);
-        const float vdown = pow2(max(ve - vn, -126)), vup = pow2(14 - vn);
-        ve = vn;
+        if (__any_sync(0xffffffffu, beyond)) {
+          // o is kept against the largest V scale so far: p s 2^(10 - ve) < 2^(kSlack + 11)
+          const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+          const int vn = max(ve, (int)(bits >> 23) - 127);
+          const float vdown = pow2(max(ve - vn, -126));
+          ve = vn;
+          vup = pow2(10 - vn);
+          vtop = pow2(min(vn, 126) + 1);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+          for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], d));
-          const float shift = top[n] == -INFINITY ? 0.f : top[n];
-          const float f = sizeof(T) == 4 ? exp2f(m[n] - shift) : ex2f_(m[n] - shift);
-          m[n] = top[n];
-          if (__any_sync(0xffffffffu, f * vdown != 1.f)) {
+            for (int d = 4; d < 32; d <<= 1) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], d));
+            const float up = top[n] > limit[n] ? top[n] : 0.f;
+            const float f = limit[n] == -INFINITY ? 1.f : exp2f(-up);  // the first keys: the sums are still 0
+            if (top[n] > limit[n]) limit[n] = kSlack;
+            ref[n] += up;
             const float2 f2 = make_float2(f, f), fo = make_float2(f * vdown, f * vdown);
             l[n] = fmul2(l[n], f2);
 #pragma unroll
@@ -584,14 +608,18 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
                   o[n][g][t][e] = y.x, o[n][g][t][e + 1] = y.y;
                 }
             }
+#pragma unroll
+            for (int u = 0; u < TU; ++u) x[n][u] = fadd2(x[n][u], make_float2(-up, -up));
           }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int u = 0; u < TU; ++u) {
-            const float2 y = fadd2(x[n][u], make_float2(-shift, -shift));
+            const float2 y = x[n][u];
             x[n][u] = sizeof(T) == 4 ? make_float2(exp2f(y.x), exp2f(y.y)) : make_float2(ex2f_(y.x), ex2f_(y.y));
             l[n] = fadd2(l[n], x[n][u]);
           }
-        }
 
 #pragma unroll
         for (int u = 0; u < TU; ++u) {
@@ -657,7 +685,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
           pieces[warp][which].begins = from_start;
           pieces[warp][which].ends = ends;
         }
-        const float back = pow2(min(ve, 127));  // and 2^10
+        const float back = pow2(min(ve, 127));  // and 2^14
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float ln = l[n].x + l[n].y, pn[NG];
@@ -679,8 +707,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
             float y[2 * MT];
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
-              y[2 * j] = fmaf((o[n][g][j][0] + o[n][g][j][1]) * 1024.f, back, pn[g]) * inv;
-              y[2 * j + 1] = fmaf((o[n][g][j][2] + o[n][g][j][3]) * 64.f, back, pn[g]) * inv;
+              y[2 * j] = fmaf((o[n][g][j][0] + o[n][g][j][1]) * 16384.f, back, pn[g]) * inv;
+              y[2 * j + 1] = fmaf((o[n][g][j][2] + o[n][g][j][3]) * 1024.f, back, pn[g]) * inv;
             }
             const int d0 = g * DG + g8 * 2 * MT;
             if (direct) {
@@ -698,7 +726,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
             }
           }
           if (!direct && g8 == 0) {
-            part[(n * 4 + t4) * (D + 4) + D] = m[n];
+            part[(n * 4 + t4) * (D + 4) + D] = limit[n] == -INFINITY ? -INFINITY : ref[n];
             part[(n * 4 + t4) * (D + 4) + D + 1] = ln;
           }
         }
@@ -715,65 +743,65 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT, D)) kv4_attention
     if (threadIdx.x == 0) atomicAdd(&g_kv4_wait_timeouts, 1u);
     return;
   }
-  constexpr int SLOTS = 2 * kWarps;
-  for (int first = 0; first < SLOTS;) {
-    const Piece head = pieces[first >> 1][first & 1];
-    if (head.b < 0) {
-      ++first;
-      continue;
-    }
-    uint32_t members = 1u << first;
-    int ends = head.ends, next = first + 1;
-    for (; next < SLOTS; ++next) {
-      const Piece& p = pieces[next >> 1][next & 1];
-      if (p.b < 0) continue;
-      if (p.b != head.b || p.seg != head.seg) break;
-      members |= 1u << next;
-      ends = p.ends;
-    }
-    const bool direct = head.begins && ends;
-    const int b = head.b;
-    int z, hk;
-    split_segment(a, head.seg, z, hk);
-    const int nq = queries_of(a, b), base = length_of(a, b) - nq;
-    float* part = a.ws + ((int64_t)blockIdx.x * 2 + (head.begins ? 1 : 0)) * piece_floats<D, NT>();
-    for (int v = threadIdx.x; v < RT * (D / 4); v += THREADS) {
-      const int rr = v / (D / 4), d = v % (D / 4) * 4;
-      float mi[SLOTS], mx = -INFINITY, den = 0.f;
+  constexpr int SLOTS = 2 * kWarps, LV = D / 4, H = 32 / LV;
+  static_assert(SLOTS <= 32, "a lane per slot");
+  Piece mine = {-1, 0, 0, 0};
+  if (lane < SLOTS) mine = pieces[lane >> 1][lane & 1];
+  const uint32_t present = __ballot_sync(0xffffffffu, mine.b >= 0);
+  uint32_t group = __match_any_sync(0xffffffffu, ((uint64_t)(uint32_t)mine.b << 32) | (uint32_t)mine.seg) & present;
+  const uint32_t heads = __ballot_sync(0xffffffffu, mine.b >= 0 && lane == __ffs(group) - 1);
+  const uint32_t ending = __ballot_sync(0xffffffffu, mine.b >= 0 && mine.ends);
+  // an item is one row of one group; H members at a time, D / 4 lanes each
+  for (int item = warp; item < __popc(heads) * RT; item += kWarps) {
+    const int rr = item % RT;
+    uint32_t rest = heads;
+    for (int i = item / RT; i > 0; --i) rest &= rest - 1;
+    const int head = __ffs(rest) - 1;
+    uint32_t members = __shfl_sync(0xffffffffu, group, head);
+    const bool begins = __shfl_sync(0xffffffffu, mine.begins, head), direct = begins && (members & ending);
+    const int b = __shfl_sync(0xffffffffu, mine.b, head), seg = __shfl_sync(0xffffffffu, mine.seg, head);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if ((members >> lane) & 1u) ml = *reinterpret_cast<const float2*>(piece_at(lane >> 1, lane & 1) + rr * (D + 4) + D);
+    const float mx = warp_max(ml.x), shift = mx == -INFINITY ? 0.f : mx;
+    const float f = exp2f(ml.x - shift);
+    const float den = warp_sum(f * ml.y);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    while (members) {
+      int i = -1;
 #pragma unroll
-      for (int i = 0; i < SLOTS; ++i) {
-        mi[i] = (members >> i) & 1u ? piece_at(i >> 1, i & 1)[rr * (D + 4) + D] : -INFINITY;
-        mx = fmaxf(mx, mi[i]);
+      for (int h = 0; h < H; ++h) {
+        if (h == lane / LV) i = __ffs(members) - 1;
+        members &= members - 1;
       }
-      const float shift = mx == -INFINITY ? 0.f : mx;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < SLOTS; ++i)
-        if ((members >> i) & 1u) {
-          const float* src = piece_at(i >> 1, i & 1) + rr * (D + 4);
-          const float f = exp2f(mi[i] - shift);
-          const float4 y = *reinterpret_cast<const float4*>(src + d);
-          acc.x = fmaf(f, y.x, acc.x), acc.y = fmaf(f, y.y, acc.y);
-          acc.z = fmaf(f, y.z, acc.z), acc.w = fmaf(f, y.w, acc.w);
-          den = fmaf(f, src[D + 1], den);
-        }
-      if (direct) {
-        const int r = z * RT + rr;
-        int t, gi;
-        split_row(a, r, t, gi);
-        if (r < a.G * a.T) {
-          const bool sees = t < nq && base + t >= 0 && den != 0.f;
-          store4(out + b * a.st.s[3] + (hk * a.G + gi) * a.st.s[4] + t * a.st.s[5] + d, acc, sees ? 1.f / den : 0.f, sees);
-        }
-      } else {
-        *reinterpret_cast<float4*>(part + rr * (D + 4) + d) = acc;
-        if (d == 0) {
-          part[rr * (D + 4) + D] = mx;
-          part[rr * (D + 4) + D + 1] = den;
-        }
+      const float fi = __shfl_sync(0xffffffffu, f, max(i, 0));
+      if (i >= 0) {
+        const float4 y = *reinterpret_cast<const float4*>(piece_at(i >> 1, i & 1) + rr * (D + 4) + lane % LV * 4);
+        acc.x = fmaf(fi, y.x, acc.x), acc.y = fmaf(fi, y.y, acc.y);
+        acc.z = fmaf(fi, y.z, acc.z), acc.w = fmaf(fi, y.w, acc.w);
       }
     }
-    first = next;
+#pragma unroll
+    for (int h = LV; h < 32; h <<= 1) {
+      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, h), acc.y += __shfl_xor_sync(0xffffffffu, acc.y, h);
+      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, h), acc.w += __shfl_xor_sync(0xffffffffu, acc.w, h);
+    }
+    if (lane >= LV) continue;
+    const int d = lane * 4;
+    if (direct) {
+      int z, hk, t, gi;
+      split_segment(a, seg, z, hk);
+      const int r = z * RT + rr;
+      split_row(a, r, t, gi);
+      if (r < a.G * a.T) {
+        const int nq = queries_of(a, b), base = length_of(a, b) - nq;
+        const bool sees = t < nq && base + t >= 0 && den != 0.f;
+        store4(out + b * a.st.s[3] + (hk * a.G + gi) * a.st.s[4] + t * a.st.s[5] + d, acc, sees ? 1.f / den : 0.f, sees);
+      }
+    } else {
+      float* part = a.ws + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * piece_floats<D, NT>() + rr * (D + 4);
+      *reinterpret_cast<float4*>(part + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(part + D) = make_float2(mx, den);
+    }
   }
 }
 
@@ -872,7 +900,7 @@ int launch(const void* q, void* out, Args a, cudaStream_t stream) {
   constexpr int smem = attention_smem<D, NT>();
   const void* fn = reinterpret_cast<const void*>(&kv4_attention_kernel<T, D, NT>);
   if (int rc = ensure_smem_attr(fn, smem)) return rc;
-  kv4_attention_kernel<T, D, NT><<<a.ctas, 32 * kWarps, smem, stream>>>((const T*)q, (T*)out, a);
+  kv4_attention_kernel<T, D, NT><<<a.ctas, 32 * warps_of(NT, D), smem, stream>>>((const T*)q, (T*)out, a);
   if (int rc = check_launch("kv4_chord_attention")) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.Z * a.Hkv));
@@ -906,7 +934,7 @@ using namespace mb::kv4;
 extern "C" int64_t motif_b200_kv4_attention_workspace_bytes(int64_t H, int64_t Hkv, int64_t T, int64_t D) {
   if (Hkv < 1 || H < Hkv || T < 1) return 0;
   const int nt = row_tile(H / Hkv * T, D);
-  return (int64_t)sm_count() * ctas_per_sm(nt, (int)D) * 2 * 4 * nt * (D + 4) * 4;
+  return (int64_t)sm_count() * 2 * 4 * nt * (D + 4) * 4;
 }
 
 extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, const int32_t* block_table,
@@ -950,7 +978,7 @@ extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, c
     if (int rc = check_rows16("kv4_chord_attention", out, strides + 3, sizeof(E))) return rc;
     const int nt = row_tile((int64_t)a.G * T, D);
     a.Z = (int)(((int64_t)a.G * T + 4 * nt - 1) / (4 * nt));
-    a.ctas = sm_count() * ctas_per_sm(nt, (int)D);
+    a.ctas = sm_count();
     const int64_t tiles = (max_pages * page_size + Tile<DD>::kKeys - 1) / Tile<DD>::kKeys;
     MB_REQUIRE((int64_t)a.B * a.Z * a.Hkv * tiles < (1ll << 31), MB_ERR_SHAPE,
                "kv4_chord_attention: B * Hkv * row tiles * key tiles = %lld (fewer than 2^31)",
