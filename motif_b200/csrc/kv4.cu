@@ -16,126 +16,178 @@ using kv4::Layout;
 // need_b = ceil((len_b + new_b) / P) - ceil(len_b / P) fresh pages.  Requests are served in order:
 // request b gets its pages when they fit its table row, its tokens fit the slot map, and the pages
 // asked for up to and including it do not exceed the free count; the i-th fresh page is the i-th
-// from the top of the free list.  One CTA: a block scan over the requests (tokens and pages), then
-// one warp per request writes its table entries and slots.
-constexpr int kReserveThreads = 1024;
+// from the top of the free list.
+//
+// One cluster of CTAs, a block of THREADS requests at a time: every CTA scans the block's tokens and
+// pages by itself, then (after a cluster barrier, since lens_out may be lens) the cluster's threads
+// share the writing.  A new token's page is an old table entry or comes straight from the free list,
+// so nobody waits for the fresh entries to be written.  Bound by latency: one scan and two dependent
+// loads; few tokens go to one CTA, which a barrier with others would only slow down.
+constexpr int kReserveCtas = 8;
 
 __device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-__device__ __forceinline__ int64_t warp_scan(int64_t v) {  // inclusive
+// Sums of whole numbers 0 .. 2^31 - 1 that stop at 2^31 - 1 (which is past every limit compared with).
+__device__ __forceinline__ int add_to_most(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, 0x7fffffffu); }
+
+__device__ __forceinline__ int warp_scan(int v) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-    if ((int)(threadIdx.x & 31) >= o) v += u;
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v = add_to_most(v, u);
   }
   return v;
 }
 
 // Inclusive scan over the block's threads; `part` holds one value per warp.
-__device__ int64_t block_scan(int64_t v, int64_t* part) {
+template <int THREADS>
+__device__ __forceinline__ int block_scan(int v, int* part) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v = warp_scan(v);
-  __syncthreads();
   if (lane == 31) part[warp] = v;
   __syncthreads();
-  if (warp == 0) part[lane] = warp_scan(part[lane]);
-  __syncthreads();
-  return warp ? v + part[warp - 1] : v;
+  // every warp scans the warps' sums for itself
+  const int sums = warp_scan(lane < THREADS / 32 ? part[lane] : 0);
+  const int before = __shfl_sync(0xffffffffu, sums, max(warp - 1, 0));
+  return warp ? add_to_most(v, before) : v;
 }
 
-__global__ void __launch_bounds__(kReserveThreads) paged_reserve_kernel(
+// x / P for 0 <= x < 2^31 and P = 16 UP, UP <= 64: (x / 16) ceil(2^33 / UP) / 2^33 is exact.
+struct PageDiv {
+  uint64_t m;
+  int P;
+  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)((uint32_t)x >> 4) * m) >> 33); }
+};
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_reserve_kernel(
     const int32_t* lens, const int32_t* __restrict__ new_lens, int32_t* table, int64_t ts,
     const int32_t* __restrict__ free_pages, const int32_t* free_count, int32_t* lens_out, int32_t* free_out,
-    int32_t* __restrict__ slots, int64_t total, int B, int columns, int64_t cap, int P) {
-  __shared__ int64_t part[32];
-  __shared__ int64_t s_start[kReserveThreads], s_pages[kReserveThreads];
-  __shared__ int s_len[kReserveThreads], s_new[kReserveThreads];
-  __shared__ bool s_ok[kReserveThreads];
-  __shared__ int64_t s_tokens, s_used, s_taken;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t avail = min((int64_t)max(*free_count, 0), cap);
-  if (tid == 0) s_tokens = s_used = s_taken = 0;
-  __syncthreads();
-  for (int b0 = 0; b0 < B; b0 += kReserveThreads) {
-    const int b = b0 + tid;
-    int64_t len = 0, fresh = 0;
+    int32_t* __restrict__ slots, bool vector, int total, int B, int columns, int cap, PageDiv by) {
+  // of each request of the block: end of its tokens and of its fresh pages, both counted over all
+  __shared__ int s_end[THREADS], s_pages[THREADS];
+  __shared__ int s_len[THREADS], s_new[THREADS];  // new: -1 - new where it is not served
+  __shared__ int part[2][32];
+  __shared__ int s_taken;
+  const int tid = threadIdx.x, lane = tid & 31, P = by.P;
+  const int ranks = gridDim.x, rank = blockIdx.x;  // one cluster
+  const int me = rank * THREADS + tid, all_threads = ranks * THREADS;
+  auto pages = [&](int n) { return by(n) + (by(n) * P < n ? 1 : 0); };
+  const int avail = min(max(*free_count, 0), cap);
+  if (tid == 0) s_taken = 0;
+  int tokens = 0, used = 0;  // of the blocks before
+  for (int b0 = 0; b0 < B; b0 += THREADS) {
+    const int b = b0 + tid, n = min(THREADS, B - b0);
+    int half = THREADS / 2;
+    while (half >= n && half > 1) half >>= 1;
+    int len = 0, fresh = 0;
     if (b < B) {
       len = max(lens[b], 0);
       fresh = max(new_lens[b], 0);
     }
-    const int64_t tok_end = s_tokens + block_scan(fresh, part);
-    const int64_t all = ceil_div(len + fresh, P);
-    const bool possible = b < B && all <= columns && tok_end <= total;
-    const int64_t need = possible ? all - ceil_div(len, P) : 0;
-    const int64_t upto = s_used + block_scan(need, part);
+    const int end = add_to_most(tokens, block_scan<THREADS>(fresh, part[0]));
+    const int full = add_to_most(len, fresh);
+    const bool possible = b < B && full <= columns * P && end <= total;
+    const int need = possible ? pages(full) - pages(len) : 0;
+    const int upto = add_to_most(used, block_scan<THREADS>(need, part[1]));
     const bool ok = possible && (need == 0 || upto <= avail);
-    s_start[tid] = tok_end - fresh;
-    s_pages[tid] = upto - need;
-    s_len[tid] = (int)len;
-    s_new[tid] = (int)fresh;
-    s_ok[tid] = ok;
-    if (b < B) lens_out[b] = (int32_t)(ok ? len + fresh : len);
-    const int64_t taken = block_scan(ok ? need : 0, part);
-    __syncthreads();
-    if (tid == kReserveThreads - 1) {
-      s_tokens = tok_end;
-      s_used = upto;
-      s_taken += taken;
+    s_end[tid] = end;
+    s_pages[tid] = upto;
+    s_len[tid] = len;
+    s_new[tid] = ok ? fresh : -1 - fresh;
+    // those that were served and took pages come first: the last of them says how many were taken
+    const int taken = __reduce_max_sync(0xffffffffu, ok && need ? upto : 0);
+    if (lane == 0 && taken) atomicMax(&s_taken, taken);
+    if (ranks > 1) asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+    else __syncthreads();
+    if (rank == 0 && b < B) lens_out[b] = ok ? full : len;
+    // the first request of the block whose running sum (tokens or pages) passes x
+    auto find = [&](const int* sums, int x) {
+      int r = 0;
+      for (int step = half; step; step >>= 1)
+        if (r + step < n && sums[r + step - 1] <= x) r += step;
+      return r;
+    };
+    // fresh table entries: the i-th from the top of the free list (past `avail` nobody is served)
+    for (int i = used + me; i < min(s_pages[n - 1], avail); i += all_threads) {
+      const int r = find(s_pages, i);
+      if (s_new[r] < 0) continue;
+      const int want = pages(s_len[r] + s_new[r]);
+      table[(int64_t)(b0 + r) * ts + want - (s_pages[r] - i)] = free_pages[avail - 1 - i];
     }
-    for (int r = warp; r < min(kReserveThreads, B - b0); r += kReserveThreads / 32) {
-      const int64_t n = s_new[r], at = s_len[r];
-      int32_t* row = table + (int64_t)(b0 + r) * ts;
-      if (s_ok[r]) {
-        const int64_t have = ceil_div(at, P), want = ceil_div(at + n, P) - have;
-        for (int64_t j = lane; j < want; j += 32) row[have + j] = free_pages[avail - 1 - (s_pages[r] + j)];
-        __syncwarp();
-      }
-      for (int64_t t = lane; t < n; t += 32) {
-        if (s_start[r] + t >= total) break;
-        const int64_t pos = at + t;
-        slots[s_start[r] + t] = s_ok[r] ? row[pos / P] * P + (int32_t)(pos % P) : -1;
+    // slots: a run of neighbouring tokens per thread, whole groups of four where there are many; a
+    // page is looked up once for the tokens of the run that lie in it
+    const int stop = min(s_end[n - 1], total);
+    const int run = stop - tokens <= all_threads ? 1 : ((stop - tokens + 3) / all_threads + 4) / 4 * 4;
+    const int from = (run == 1 ? tokens : tokens & ~3) + me * run;  // groups of four start at multiples of 4
+    int token = max(from, tokens);
+    const int last = min(from + run, stop);
+    if (from < stop && token < last) {
+      int r = find(s_end, token);
+      while (token < last) {
+        while (s_end[r] <= token) ++r;
+        int until = min(last, s_end[r]), v = -1, up = 0;
+        if (s_new[r] >= 0) {
+          const int pos = s_len[r] + token - (s_end[r] - s_new[r]), at = by(pos), off = pos - at * P;
+          const int have = pages(s_len[r]), want = pages(s_len[r] + s_new[r]);
+          const int page = at < have ? table[(int64_t)(b0 + r) * ts + at]
+                                     : free_pages[avail - 1 - (s_pages[r] - (want - at))];
+          v = page * P + off;
+          up = 1;
+          until = min(until, token + P - off);
+        }
+        while (token < until) {
+          if ((token & 3) == 0 && token + 4 <= until && vector) {
+            *reinterpret_cast<int4*>(slots + token) = make_int4(v, v + up, v + 2 * up, v + 3 * up);
+            token += 4, v += 4 * up;
+          } else {
+            slots[token] = v;
+            ++token, v += up;
+          }
+        }
       }
     }
+    tokens = s_end[THREADS - 1];
+    used = s_pages[THREADS - 1];
     __syncthreads();
   }
-  for (int64_t i = s_tokens + tid; i < total; i += kReserveThreads) slots[i] = -1;
-  if (tid == 0) *free_out = (int32_t)(avail - s_taken);
+  for (int64_t i = (int64_t)tokens + me; i < total; i += all_threads) slots[i] = -1;
+  if (rank == 0 && tid == 0) *free_out = avail - s_taken;
 }
 
 // Finished requests give their pages back: onto the top of the free list in request order, their
 // table rows become -1 and their lengths 0.
-__global__ void __launch_bounds__(kReserveThreads) paged_release_kernel(
+constexpr int kReleaseThreads = 1024;
+
+__global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
     const uint8_t* __restrict__ done, int32_t* __restrict__ lens, int32_t* __restrict__ table, int64_t ts,
     int32_t* __restrict__ free_pages, int32_t* __restrict__ free_count, int B, int columns, int64_t cap, int P) {
-  __shared__ int64_t part[32];
-  __shared__ int64_t s_at[kReserveThreads];
-  __shared__ int s_held[kReserveThreads];
-  __shared__ int64_t s_top;
+  __shared__ int part[32];
+  __shared__ int s_at[kReleaseThreads], s_held[kReleaseThreads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) s_top = max(*free_count, 0);
-  __syncthreads();
-  for (int b0 = 0; b0 < B; b0 += kReserveThreads) {
+  int top = max(*free_count, 0);
+  for (int b0 = 0; b0 < B; b0 += kReleaseThreads) {
     const int b = b0 + tid;
-    int64_t held = 0;
+    int held = 0;
     if (b < B && done[b]) {
-      held = min(ceil_div(max(lens[b], 0), P), (int64_t)columns);
+      held = (int)min(ceil_div(max(lens[b], 0), P), (int64_t)columns);
       lens[b] = 0;
     }
-    const int64_t upto = s_top + block_scan(held, part);
+    const int upto = add_to_most(top, block_scan<kReleaseThreads>(held, part));
     s_at[tid] = upto - held;
-    s_held[tid] = (int)held;
+    s_held[tid] = held;
     __syncthreads();
-    if (tid == kReserveThreads - 1) s_top = upto;
-    for (int r = warp; r < min(kReserveThreads, B - b0); r += kReserveThreads / 32) {
+    for (int r = warp; r < min(kReleaseThreads, B - b0); r += kReleaseThreads / 32) {
       int32_t* row = table + (int64_t)(b0 + r) * ts;
       for (int j = lane; j < s_held[r]; j += 32) {
         if (s_at[r] + j < cap) free_pages[s_at[r] + j] = row[j];
         row[j] = -1;
       }
     }
+    top = s_at[kReleaseThreads - 1] + s_held[kReleaseThreads - 1];
     __syncthreads();
   }
-  if (tid == 0) *free_count = (int32_t)min(s_top, cap);
+  if (tid == 0) *free_count = (int32_t)min((int64_t)top, cap);
 }
 
 // ------------------------------------------------------------------ append
@@ -299,9 +351,30 @@ extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_
              (long long)total_new);
   MB_REQUIRE(free_capacity >= 1 && free_capacity * page_size < (1ll << 31), MB_ERR_SHAPE,
              "paged_reserve: free list of %lld pages", (long long)free_capacity);
-  paged_reserve_kernel<<<1, kReserveThreads, 0, (cudaStream_t)stream>>>(
-      lens, new_lens, block_table, table_stride, free_pages, free_count, lens_out, free_count_out, slots, total_new,
-      (int)B, (int)max_pages, free_capacity, (int)page_size);
+  PageDiv by;
+  by.P = (int)page_size;
+  const uint64_t up = (uint64_t)page_size / kUnit;
+  by.m = ((1ull << 33) + up - 1) / up;
+  const bool vector = reinterpret_cast<uintptr_t>(slots) % 16 == 0;
+  auto go = [&](auto kernel, int threads, int ctas) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ctas;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, lens, new_lens, block_table, table_stride, free_pages, free_count, lens_out,
+                       free_count_out, slots, vector, (int)total_new, (int)B, (int)max_pages, (int)free_capacity, by);
+  };
+  // a decode step's worth of requests and tokens: four warps scan faster than 16; many tokens: the
+  // cluster shares the writing
+  if (B <= 128 && total_new <= 1024) go(paged_reserve_kernel<128>, 128, 1);
+  else if (B <= 512) go(paged_reserve_kernel<512>, 512, total_new <= 4096 ? 1 : kReserveCtas);
+  else go(paged_reserve_kernel<1024>, 1024, total_new <= 4096 ? 1 : kReserveCtas);
   return check_launch("paged_reserve");
 }
 
@@ -312,7 +385,7 @@ extern "C" int motif_b200_paged_release(const uint8_t* done, int32_t* lens, int3
   if (int rc = check_paging("paged_release", B, max_pages, table_stride, page_size)) return rc;
   MB_REQUIRE(free_capacity >= 1 && free_capacity * page_size < (1ll << 31), MB_ERR_SHAPE,
              "paged_release: free list of %lld pages", (long long)free_capacity);
-  paged_release_kernel<<<1, kReserveThreads, 0, (cudaStream_t)stream>>>(done, lens, block_table, table_stride,
+  paged_release_kernel<<<1, kReleaseThreads, 0, (cudaStream_t)stream>>>(done, lens, block_table, table_stride,
                                                                          free_pages, free_count, (int)B,
                                                                          (int)max_pages, free_capacity,
                                                                          (int)page_size);
