@@ -12,6 +12,17 @@ namespace {
 using kv4::kUnit;
 using kv4::Layout;
 
+// x / P for 0 <= x < 2^31 and P = 16 UP, UP <= 64: (x / 16) ceil(2^33 / UP) / 2^33 is exact.
+struct PageDiv {
+  uint64_t m;
+  int P;
+  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)((uint32_t)x >> 4) * m) >> 33); }
+};
+PageDiv page_div(int64_t P) {
+  const uint64_t up = (uint64_t)P / kUnit;
+  return {((1ull << 33) + up - 1) / up, (int)P};
+}
+
 // ------------------------------------------------------------------ slot reservation
 // need_b = ceil((len_b + new_b) / P) - ceil(len_b / P) fresh pages.  Requests are served in order:
 // request b gets its pages when they fit its table row, its tokens fit the slot map, and the pages
@@ -51,13 +62,6 @@ __device__ __forceinline__ int block_scan(int v, int* part) {
   const int before = __shfl_sync(0xffffffffu, sums, max(warp - 1, 0));
   return warp ? add_to_most(v, before) : v;
 }
-
-// x / P for 0 <= x < 2^31 and P = 16 UP, UP <= 64: (x / 16) ceil(2^33 / UP) / 2^33 is exact.
-struct PageDiv {
-  uint64_t m;
-  int P;
-  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)((uint32_t)x >> 4) * m) >> 33); }
-};
 
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) paged_reserve_kernel(
@@ -230,34 +234,22 @@ __device__ __forceinline__ void store8(T* p, const float* x) {
   }
 }
 
-// A thread takes eight dims of one row (one 32-bit word of codes); the DG / 8 neighbouring lanes of
-// a group find its extremes by xor-shuffles.  The quotient is the IEEE one and ties go to the even
-// code, so the stored bits are a function of the input alone.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
-                                                         const int32_t* __restrict__ slots,
-                                                         uint8_t* __restrict__ pool, T* __restrict__ k_out,
-                                                         T* __restrict__ v_out, Strides12 st, int64_t rows, int T_,
-                                                         int Hkv, int64_t nslots, int P) {
-  using L = Layout<D>;
-  constexpr int W = D / 8;  // threads of one row
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int w = (int)(idx % W);
-  int64_t row = idx / W;
-  const bool live = row < 2 * rows;  // whole groups of lanes: W divides the warp
-  const bool isv = row >= rows;
-  if (isv) row -= rows;
-  if (!live) row = 0;
-  const int h = (int)(row % Hkv);
-  const int64_t n = row / Hkv, b = n / T_, t = n % T_;
-  float x[8];
-  const int o = isv ? 3 : 0;
-  load8((isv ? v : k) + b * st.s[o] + h * st.s[o + 1] + t * st.s[o + 2] + 8 * w, x);
+// The group's pair and this thread's eight codes; y becomes the values they stand for.  LANES
+// neighbouring lanes hold the group.
+//
+// The code is the nearest whole number to RN(d / s), d = RN(x - m), ties to even.  With r = RN(1 / s),
+// q = RN(d r) and the exact residual e = d - q s (one fma), RN(q + e r) is RN(d / s) (Markstein 1990:
+// a correctly rounded reciprocal and a quotient within one unit give the correctly rounded quotient),
+// at a multiplication and two fmas a value; scales below 2^-100, where r or e could leave the range,
+// divide.  Adding 1.5 2^23 + 8 rounds to a whole number, ties to even, and leaves c + 8 in the low
+// bits, so the word is a sum of shifted sums less a constant.
+template <int LANES>
+__device__ __forceinline__ void quantise8(const float* x, float* y, uint32_t& word, uint32_t& pair) {
   float hi = x[0], lo = x[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) hi = fmax_nan(hi, x[i]), lo = fmin_nan(lo, x[i]);
 #pragma unroll
-  for (int d = 1; d < L::DG / 8; d <<= 1) {
+  for (int d = 1; d < LANES; d <<= 1) {
     hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
     lo = fmin_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
   }
@@ -265,28 +257,63 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k
   float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(range, 15.0f)));
   float m = __bfloat162float(__float2bfloat16_rn(__fadd_rn(lo, 8.0f * s)));
   if (!(range <= 3.4028234e38f)) s = m = __uint_as_float(0x7fc00000u);  // a NaN or an infinity: all NaN
-  uint32_t word = 0;
-  float y[8];
+  const float r = __frcp_rn(s);
+  constexpr float kRound = 12582912.f + 8.f;
+  uint32_t sum = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float q = s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[i], m), s)) : 0.f;
-    const float c = fminf(fmaxf(q, -8.f), 7.f);
-    word |= (uint32_t)((int)c + 8) << (4 * i);
-    y[i] = fmaf(s, c, m);
+    const float d = __fsub_rn(x[i], m);
+    float q = __fmul_rn(d, r);
+    q = __fmaf_rn(__fmaf_rn(-q, s, d), r, q);
+    if (!(s >= 7.8886091e-31f)) q = s > 0.f ? __fdiv_rn(d, s) : 0.f;
+    const float t = __fadd_rn(fminf(fmaxf(q, -8.f), 7.f), kRound);
+    sum += __float_as_uint(t) << (4 * i);
+    y[i] = fmaf(s, __fsub_rn(t, kRound), m);
   }
+  // the bits of 1.5 2^23 in every term
+  word = sum - 0x4b400000u * 0x11111111u;
+  pair = (__float_as_uint(m) & 0xffff0000u) | (__float_as_uint(s) >> 16);
+}
+
+// A thread takes the same eight dims of K and V of one token and head: D / 8 neighbouring lanes make a
+// row, the rows of a warp are neighbouring tokens of one head (blockIdx.y), whose codes and pairs lie
+// next to each other.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
+                                                         const int32_t* __restrict__ slots,
+                                                         uint8_t* __restrict__ pool, T* __restrict__ k_out,
+                                                         T* __restrict__ v_out, Strides12 st, int N, int T_, int Hkv,
+                                                         int nslots, PageDiv by) {
+  using L = Layout<D>;
+  constexpr int W = D / 8;  // threads of one row
+  const int w = threadIdx.x % W, h = blockIdx.y;
+  const int64_t at = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
+  const bool live = at < N;  // whole groups of lanes: W divides the warp
+  const int n = live ? (int)at : 0;
+  const int b = T_ == N ? 0 : n / T_, t = n - b * T_;
+  const int slot = live ? slots[n] : -1;
+  float x[2][8], y[2][8];
+  load8(k + b * st.s[0] + h * st.s[1] + t * st.s[2] + 8 * w, x[0]);
+  load8(v + b * st.s[3] + h * st.s[4] + t * st.s[5] + 8 * w, x[1]);
+  uint32_t word[2], pair[2];
+  quantise8<L::DG / 8>(x[0], y[0], word[0], pair[0]);
+  quantise8<L::DG / 8>(x[1], y[1], word[1], pair[1]);
   if (!live) return;
-  const int64_t slot = slots[n];
   if (slot >= 0 && slot < nslots) {
-    const int64_t unit = (slot / P * Hkv + h) * (P / kUnit) + slot % P / kUnit;
-    const int r = (int)(slot % kUnit);
-    uint8_t* u = pool + unit * L::kBytes;
-    *reinterpret_cast<uint32_t*>(u + (isv ? L::kV : 0) + r * L::kRow + 4 * w) = word;
-    if (w % (L::DG / 8) == 0)
-      *reinterpret_cast<uint32_t*>(u + (isv ? L::kVp : L::kKp) + (w / (L::DG / 8) * kUnit + r) * 4) =
-          (__float_as_uint(m) & 0xffff0000u) | (__float_as_uint(s) >> 16);
+    const int page = by(slot), off = slot - page * by.P, r = off % kUnit;
+    uint8_t* u = pool + (((int64_t)page * Hkv + h) * (by.P / kUnit) + off / kUnit) * L::kBytes;
+    *reinterpret_cast<uint32_t*>(u + r * L::kRow + 4 * w) = word[0];
+    *reinterpret_cast<uint32_t*>(u + L::kV + r * L::kRow + 4 * w) = word[1];
+    if (w % (L::DG / 8) == 0) {
+      const int g = w / (L::DG / 8);
+      *reinterpret_cast<uint32_t*>(u + L::kKp + (g * kUnit + r) * 4) = pair[0];
+      *reinterpret_cast<uint32_t*>(u + L::kVp + (g * kUnit + r) * 4) = pair[1];
+    }
   }
-  T* out = isv ? v_out : k_out;
-  if (out) store8(out + b * st.s[6 + o] + h * st.s[7 + o] + t * st.s[8 + o] + 8 * w, y);
+  if (k_out) {
+    store8(k_out + b * st.s[6] + h * st.s[7] + t * st.s[8] + 8 * w, y[0]);
+    store8(v_out + b * st.s[9] + h * st.s[10] + t * st.s[11] + 8 * w, y[1]);
+  }
 }
 
 // ------------------------------------------------------------------ gather
@@ -351,10 +378,7 @@ extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_
              (long long)total_new);
   MB_REQUIRE(free_capacity >= 1 && free_capacity * page_size < (1ll << 31), MB_ERR_SHAPE,
              "paged_reserve: free list of %lld pages", (long long)free_capacity);
-  PageDiv by;
-  by.P = (int)page_size;
-  const uint64_t up = (uint64_t)page_size / kUnit;
-  by.m = ((1ull << 33) + up - 1) / up;
+  const PageDiv by = page_div(page_size);
   const bool vector = reinterpret_cast<uintptr_t>(slots) % 16 == 0;
   auto go = [&](auto kernel, int threads, int ctas) {
     cudaLaunchConfig_t cfg = {};
@@ -413,11 +437,11 @@ extern "C" int motif_b200_kv4_append(const void* k, const void* v, const int32_t
     for (int i = 0; i < 4; ++i)
       if (ptrs[i])
         if (int rc = check_rows16("kv4_append", ptrs[i], strides + 3 * i, sizeof(E))) return rc;
-    const int64_t rows = B * T * Hkv, threads = 2 * rows * (DD / 8);
-    MB_REQUIRE((threads + 255) / 256 < (1ll << 31), MB_ERR_SHAPE, "kv4_append: %lld rows", (long long)rows);
-    kv4_append_kernel<E, DD><<<(unsigned)((threads + 255) / 256), 256, 0, (cudaStream_t)stream>>>(
-        (const E*)k, (const E*)v, slots, (uint8_t*)pool, (E*)k_out, (E*)v_out, st, rows, (int)T, (int)Hkv,
-        num_pages * page_size, (int)page_size);
+    const int64_t per_cta = 256 / (DD / 8);
+    kv4_append_kernel<E, DD><<<dim3((unsigned)((B * T + per_cta - 1) / per_cta), (unsigned)Hkv), 256, 0,
+                               (cudaStream_t)stream>>>((const E*)k, (const E*)v, slots, (uint8_t*)pool, (E*)k_out,
+                                                       (E*)v_out, st, (int)(B * T), (int)T, (int)Hkv,
+                                                       (int)(num_pages * page_size), page_div(page_size));
     return check_launch("kv4_append");
   });
 }
