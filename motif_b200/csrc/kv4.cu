@@ -210,15 +210,19 @@ __device__ __forceinline__ float fmin_nan(float a, float b) {
   return r;
 }
 
-// Eight consecutive elements at a 16-byte aligned address.
+template <typename T> struct Pair;
+template <> struct Pair<__half> { using type = __half2; };
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+
+// Eight consecutive elements at a 16-byte aligned address, and for 16-bit types as they lie there.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* x) {
+__device__ __forceinline__ void load8(const T* p, float* x, uint4& raw) {
   if constexpr (sizeof(T) == 4) {
     const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
   } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&a);
+    raw = *reinterpret_cast<const uint4*>(p);
+    const T* h = reinterpret_cast<const T*>(&raw);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = to_f(h[i]);
   }
@@ -234,41 +238,91 @@ __device__ __forceinline__ void store8(T* p, const float* x) {
   }
 }
 
-// The group's pair and this thread's eight codes; y becomes the values they stand for.  LANES
-// neighbouring lanes hold the group.
+__device__ __forceinline__ __half2 lows(__half2 a, __half2 b) { return __lows2half2(a, b); }
+__device__ __forceinline__ __half2 highs(__half2 a, __half2 b) { return __highs2half2(a, b); }
+__device__ __forceinline__ __nv_bfloat162 lows(__nv_bfloat162 a, __nv_bfloat162 b) { return __lows2bfloat162(a, b); }
+__device__ __forceinline__ __nv_bfloat162 highs(__nv_bfloat162 a, __nv_bfloat162 b) { return __highs2bfloat162(a, b); }
+
+// Largest and smallest of the group that LANES neighbouring lanes hold, eight values each (a NaN
+// anywhere: both NaN).  16-bit values keep (max, -min) as a packed pair of their own type, so one
+// packed maximum per step reduces both.
+template <typename T, int LANES>
+__device__ __forceinline__ void extremes(const uint4* raw, const float* x, float& hi, float& lo) {
+  if constexpr (sizeof(T) == 4) {
+    hi = lo = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) hi = fmax_nan(hi, x[i]), lo = fmin_nan(lo, x[i]);
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) {
+      hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+      lo = fmin_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+    }
+  } else {
+    using T2 = typename Pair<T>::type;
+    const T2* v = reinterpret_cast<const T2*>(raw);
+    T2 a = __hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3]));
+    const T2 c = __hmin2_nan(__hmin2_nan(v[0], v[1]), __hmin2_nan(v[2], v[3]));
+    const T2 n = __hneg2(c);
+    // (largest, -smallest) of the two halves
+    T2 both = __hmax2_nan(lows(a, n), highs(a, n));
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) {
+      const uint32_t u = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&both), d);
+      both = __hmax2_nan(both, *reinterpret_cast<const T2*>(&u));
+    }
+    hi = to_f(both.x);
+    lo = -to_f(both.y);
+  }
+}
+
+// The group's pair and this thread's eight codes; y becomes the values they stand for.
 //
 // The code is the nearest whole number to RN(d / s), d = RN(x - m), ties to even.  With r = RN(1 / s),
 // q = RN(d r) and the exact residual e = d - q s (one fma), RN(q + e r) is RN(d / s) (Markstein 1990:
 // a correctly rounded reciprocal and a quotient within one unit give the correctly rounded quotient),
-// at a multiplication and two fmas a value; scales below 2^-100, where r or e could leave the range,
-// divide.  Adding 1.5 2^23 + 8 rounds to a whole number, ties to even, and leaves c + 8 in the low
-// bits, so the word is a sum of shifted sums less a constant.
-template <int LANES>
-__device__ __forceinline__ void quantise8(const float* x, float* y, uint32_t& word, uint32_t& pair) {
-  float hi = x[0], lo = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) hi = fmax_nan(hi, x[i]), lo = fmin_nan(lo, x[i]);
-#pragma unroll
-  for (int d = 1; d < LANES; d <<= 1) {
-    hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-    lo = fmin_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-  }
+// at a multiplication and two fmas a value, in packed pairs; so is range / 15.  Scales below 2^-100,
+// where r or e could leave the range, divide.  Adding 1.5 2^23 + 8 rounds to a whole number, ties to
+// even, and leaves c + 8 in the low bits, so the word is a sum of shifted sums less a constant.
+__device__ __forceinline__ void quantise8(const float* x, float hi, float lo, float* y, uint32_t& word, uint32_t& pair) {
   const float range = __fsub_rn(hi, lo);
-  float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(range, 15.0f)));
-  float m = __bfloat162float(__float2bfloat16_rn(__fadd_rn(lo, 8.0f * s)));
+  constexpr float r15 = 1.0f / 15.0f;
+  const float q15 = __fmul_rn(range, r15);
+  float step = __fmaf_rn(__fmaf_rn(-q15, 15.0f, range), r15, q15);
+  const bool tiny = !(range >= 1.2e-29f);  // 15 times 2^-100 and a little: also 0 and NaN
+  if (tiny) step = __fdiv_rn(range, 15.0f);
+  float s = __bfloat162float(__float2bfloat16_rn(step));
+  float m = __bfloat162float(__float2bfloat16_rn(__fmaf_rn(8.0f, s, lo)));  // 8 s is exact: one rounding
   if (!(range <= 3.4028234e38f)) s = m = __uint_as_float(0x7fc00000u);  // a NaN or an infinity: all NaN
   const float r = __frcp_rn(s);
   constexpr float kRound = 12582912.f + 8.f;
+  const float2 m2 = make_float2(-m, -m), r2 = make_float2(r, r), s2 = make_float2(s, s), n2 = make_float2(-s, -s);
+  float2 q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 d = fadd2(make_float2(x[2 * i], x[2 * i + 1]), m2), q0 = fmul2(d, r2);
+    q[i] = ffma2(ffma2(n2, q0, d), r2, q0);
+  }
+  if (tiny) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      float z = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e == i) z = __fsub_rn(x[e], m);
+      z = s > 0.f ? __fdiv_rn(z, s) : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e == i) (e & 1 ? q[e / 2].y : q[e / 2].x) = z;
+    }
+  }
   uint32_t sum = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float d = __fsub_rn(x[i], m);
-    float q = __fmul_rn(d, r);
-    q = __fmaf_rn(__fmaf_rn(-q, s, d), r, q);
-    if (!(s >= 7.8886091e-31f)) q = s > 0.f ? __fdiv_rn(d, s) : 0.f;
-    const float t = __fadd_rn(fminf(fmaxf(q, -8.f), 7.f), kRound);
-    sum += __float_as_uint(t) << (4 * i);
-    y[i] = fmaf(s, __fsub_rn(t, kRound), m);
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = fadd2(make_float2(fminf(fmaxf(q[i].x, -8.f), 7.f), fminf(fmaxf(q[i].y, -8.f), 7.f)),
+                           make_float2(kRound, kRound));
+    sum += __float_as_uint(t.x) * (1u << (8 * i)) + __float_as_uint(t.y) * (16u << (8 * i));
+    const float2 v = ffma2(s2, fadd2(t, make_float2(-kRound, -kRound)), make_float2(m, m));
+    y[2 * i] = v.x, y[2 * i + 1] = v.y;
   }
   // the bits of 1.5 2^23 in every term
   word = sum - 0x4b400000u * 0x11111111u;
@@ -292,12 +346,16 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k
   const int n = live ? (int)at : 0;
   const int b = T_ == N ? 0 : n / T_, t = n - b * T_;
   const int slot = live ? slots[n] : -1;
-  float x[2][8], y[2][8];
-  load8(k + b * st.s[0] + h * st.s[1] + t * st.s[2] + 8 * w, x[0]);
-  load8(v + b * st.s[3] + h * st.s[4] + t * st.s[5] + 8 * w, x[1]);
+  float x[2][8], y[2][8], hi, lo;
+  uint4 raw[2];
+  load8(k + b * st.s[0] + h * st.s[1] + t * st.s[2] + 8 * w, x[0], raw[0]);
+  load8(v + b * st.s[3] + h * st.s[4] + t * st.s[5] + 8 * w, x[1], raw[1]);
   uint32_t word[2], pair[2];
-  quantise8<L::DG / 8>(x[0], y[0], word[0], pair[0]);
-  quantise8<L::DG / 8>(x[1], y[1], word[1], pair[1]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    extremes<T, L::DG / 8>(&raw[i], x[i], hi, lo);
+    quantise8(x[i], hi, lo, y[i], word[i], pair[i]);
+  }
   if (!live) return;
   if (slot >= 0 && slot < nslots) {
     const int page = by(slot), off = slot - page * by.P, r = off % kUnit;
