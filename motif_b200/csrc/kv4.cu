@@ -195,8 +195,12 @@ __global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
 }
 
 // ------------------------------------------------------------------ append
+template <typename I>
 struct Strides12 {
-  int64_t s[12];  // k(b,h,t) v(b,h,t) k_out(b,h,t) v_out(b,h,t)
+  I s[12];  // k(b,h,t) v(b,h,t) k_out(b,h,t) v_out(b,h,t); 32-bit ones make each product one instruction
+  __device__ __forceinline__ int64_t at(int i, int b, int h, int t) const {
+    return (int64_t)b * s[i] + (int64_t)h * s[i + 1] + (int64_t)t * s[i + 2];
+  }
 };
 
 __device__ __forceinline__ float fmax_nan(float a, float b) {
@@ -281,48 +285,43 @@ __device__ __forceinline__ void extremes(const uint4* raw, const float* x, float
 // q = RN(d r) and the exact residual e = d - q s (one fma), RN(q + e r) is RN(d / s) (Markstein 1990:
 // a correctly rounded reciprocal and a quotient within one unit give the correctly rounded quotient),
 // at a multiplication and two fmas a value, in packed pairs; so is range / 15.  Scales below 2^-100,
-// where r or e could leave the range, divide.  Adding 1.5 2^23 + 8 rounds to a whole number, ties to
+// where r or e could leave the range, divide, as do groups whose codes could.  Adding 1.5 2^23 + 8 rounds to a whole number, ties to
 // even, and leaves c + 8 in the low bits, so the word is a sum of shifted sums less a constant.
 __device__ __forceinline__ void quantise8(const float* x, float hi, float lo, float* y, uint32_t& word, uint32_t& pair) {
   const float range = __fsub_rn(hi, lo);
   constexpr float r15 = 1.0f / 15.0f;
   const float q15 = __fmul_rn(range, r15);
   float step = __fmaf_rn(__fmaf_rn(-q15, 15.0f, range), r15, q15);
-  const bool tiny = !(range >= 1.2e-29f);  // 15 times 2^-100 and a little: also 0 and NaN
-  if (tiny) step = __fdiv_rn(range, 15.0f);
+  // ranges whose scale is below 2^-100 divide; 0 and NaN are among them
+  bool odd = !(range >= 1.2e-29f);
+  if (odd) step = __fdiv_rn(range, 15.0f);
   float s = __bfloat162float(__float2bfloat16_rn(step));
   float m = __bfloat162float(__float2bfloat16_rn(__fmaf_rn(8.0f, s, lo)));  // 8 s is exact: one rounding
   if (!(range <= 3.4028234e38f)) s = m = __uint_as_float(0x7fc00000u);  // a NaN or an infinity: all NaN
-  const float r = __frcp_rn(s);
+  // the extremes lie on -8 and 7 but for the rounding of s and m: only where that is large (a centre
+  // far from 0) can a code leave the range
+  odd = odd || lo - m < -8.49f * s || hi - m > 7.49f * s;
   constexpr float kRound = 12582912.f + 8.f;
-  const float2 m2 = make_float2(-m, -m), r2 = make_float2(r, r), s2 = make_float2(s, s), n2 = make_float2(-s, -s);
-  float2 q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 d = fadd2(make_float2(x[2 * i], x[2 * i + 1]), m2), q0 = fmul2(d, r2);
-    q[i] = ffma2(ffma2(n2, q0, d), r2, q0);
-  }
-  if (tiny) {
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      float z = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e == i) z = __fsub_rn(x[e], m);
-      z = s > 0.f ? __fdiv_rn(z, s) : 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e == i) (e & 1 ? q[e / 2].y : q[e / 2].x) = z;
-    }
-  }
   uint32_t sum = 0;
+  if (!odd) {
+    const float r = __frcp_rn(s);
+    const float2 m2 = make_float2(-m, -m), r2 = make_float2(r, r), s2 = make_float2(s, s), n2 = make_float2(-s, -s);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = fadd2(make_float2(fminf(fmaxf(q[i].x, -8.f), 7.f), fminf(fmaxf(q[i].y, -8.f), 7.f)),
-                           make_float2(kRound, kRound));
-    sum += __float_as_uint(t.x) * (1u << (8 * i)) + __float_as_uint(t.y) * (16u << (8 * i));
-    const float2 v = ffma2(s2, fadd2(t, make_float2(-kRound, -kRound)), make_float2(m, m));
-    y[2 * i] = v.x, y[2 * i + 1] = v.y;
+    for (int i = 0; i < 4; ++i) {
+      const float2 d = fadd2(make_float2(x[2 * i], x[2 * i + 1]), m2), q0 = fmul2(d, r2);
+      const float2 t = fadd2(ffma2(ffma2(n2, q0, d), r2, q0), make_float2(kRound, kRound));
+      sum += __float_as_uint(t.x) * (1u << (8 * i)) + __float_as_uint(t.y) * (16u << (8 * i));
+      const float2 v = ffma2(s2, fadd2(t, make_float2(-kRound, -kRound)), make_float2(m, m));
+      y[2 * i] = v.x, y[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float q = s > 0.f ? __fdiv_rn(__fsub_rn(x[i], m), s) : 0.f;
+      const float t = __fadd_rn(fminf(fmaxf(q, -8.f), 7.f), kRound);
+      sum += __float_as_uint(t) << (4 * i);
+      y[i] = fmaf(s, __fsub_rn(t, kRound), m);
+    }
   }
   // the bits of 1.5 2^23 in every term
   word = sum - 0x4b400000u * 0x11111111u;
@@ -332,11 +331,11 @@ __device__ __forceinline__ void quantise8(const float* x, float hi, float lo, fl
 // A thread takes the same eight dims of K and V of one token and head: D / 8 neighbouring lanes make a
 // row, the rows of a warp are neighbouring tokens of one head (blockIdx.y), whose codes and pairs lie
 // next to each other.
-template <typename T, int D>
+template <typename T, int D, typename I>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                          const int32_t* __restrict__ slots,
                                                          uint8_t* __restrict__ pool, T* __restrict__ k_out,
-                                                         T* __restrict__ v_out, Strides12 st, int N, int T_, int Hkv,
+                                                         T* __restrict__ v_out, Strides12<I> st, int N, int T_, int Hkv,
                                                          int nslots, PageDiv by) {
   using L = Layout<D>;
   constexpr int W = D / 8;  // threads of one row
@@ -348,8 +347,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k
   const int slot = live ? slots[n] : -1;
   float x[2][8], y[2][8], hi, lo;
   uint4 raw[2];
-  load8(k + b * st.s[0] + h * st.s[1] + t * st.s[2] + 8 * w, x[0], raw[0]);
-  load8(v + b * st.s[3] + h * st.s[4] + t * st.s[5] + 8 * w, x[1], raw[1]);
+  load8(k + st.at(0, b, h, t) + 8 * w, x[0], raw[0]);
+  load8(v + st.at(3, b, h, t) + 8 * w, x[1], raw[1]);
   uint32_t word[2], pair[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -369,8 +368,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k
     }
   }
   if (k_out) {
-    store8(k_out + b * st.s[6] + h * st.s[7] + t * st.s[8] + 8 * w, y[0]);
-    store8(v_out + b * st.s[9] + h * st.s[10] + t * st.s[11] + 8 * w, y[1]);
+    store8(k_out + st.at(6, b, h, t) + 8 * w, y[0]);
+    store8(v_out + st.at(9, b, h, t) + 8 * w, y[1]);
   }
 }
 
@@ -490,16 +489,23 @@ extern "C" int motif_b200_kv4_append(const void* k, const void* v, const int32_t
     constexpr int DD = decltype(d)::value;
     if (B * T == 0) return MB_OK;
     const void* ptrs[4] = {k, v, k_out, v_out};
-    Strides12 st;
-    for (int i = 0; i < 12; ++i) st.s[i] = strides[i];
     for (int i = 0; i < 4; ++i)
       if (ptrs[i])
         if (int rc = check_rows16("kv4_append", ptrs[i], strides + 3 * i, sizeof(E))) return rc;
     const int64_t per_cta = 256 / (DD / 8);
-    kv4_append_kernel<E, DD><<<dim3((unsigned)((B * T + per_cta - 1) / per_cta), (unsigned)Hkv), 256, 0,
-                               (cudaStream_t)stream>>>((const E*)k, (const E*)v, slots, (uint8_t*)pool, (E*)k_out,
-                                                       (E*)v_out, st, (int)(B * T), (int)T, (int)Hkv,
-                                                       (int)(num_pages * page_size), page_div(page_size));
+    auto go = [&](auto width) {
+      using I = decltype(width);
+      Strides12<I> st;
+      for (int i = 0; i < 12; ++i) st.s[i] = (I)strides[i];
+      kv4_append_kernel<E, DD, I><<<dim3((unsigned)((B * T + per_cta - 1) / per_cta), (unsigned)Hkv), 256, 0,
+                                    (cudaStream_t)stream>>>((const E*)k, (const E*)v, slots, (uint8_t*)pool, (E*)k_out,
+                                                            (E*)v_out, st, (int)(B * T), (int)T, (int)Hkv,
+                                                            (int)(num_pages * page_size), page_div(page_size));
+    };
+    bool fits = true;
+    for (int i = 0; i < 12; ++i) fits = fits && strides[i] >= 0 && strides[i] < (1ll << 31);
+    if (fits) go(int32_t());
+    else go(int64_t());
     return check_launch("kv4_append");
   });
 }
