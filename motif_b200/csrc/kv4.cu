@@ -374,46 +374,52 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k
 }
 
 // ------------------------------------------------------------------ gather
-// A thread reads one word of codes of K and of V and writes eight values of each; tokens at or past
-// the request's length, and those of pages outside the pool, become zeros.
+// Eight values of one word: a code in the last bits of 2^23 is a float 2^23 + c; taking 2^23 + 8 off is
+// exact, and s (c - 8) + m is rounded once.
+__device__ __forceinline__ void values8(uint32_t word, uint32_t pair, float* x) {
+  const float2 s = make_float2(kv4::pair_scale(pair), kv4::pair_scale(pair));
+  const float2 m = make_float2(kv4::pair_centre(pair), kv4::pair_centre(pair));
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float2 c = make_float2(__uint_as_float(((word >> (4 * i)) & 15u) | 0x4b000000u),
+                                 __uint_as_float(((word >> (4 * i + 4)) & 15u) | 0x4b000000u));
+    const float2 v = ffma2(fadd2(c, make_float2(-8388616.f, -8388616.f)), s, m);
+    x[i] = v.x, x[i + 1] = v.y;
+  }
+}
+
+// A thread reads one word of codes of K and of V and writes eight values of each; D / 8 neighbouring
+// lanes make a row, a warp neighbouring tokens of one head.  Tokens at or past the request's length,
+// and those of pages outside the pool, become zeros.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(const uint8_t* __restrict__ pool,
                                                          const int32_t* __restrict__ table, int64_t ts,
                                                          const int32_t* __restrict__ lens, T* __restrict__ k_out,
-                                                         T* __restrict__ v_out, int64_t words, int Hkv, int S,
-                                                         int64_t pages, int P, int columns) {
+                                                         T* __restrict__ v_out, int blocks, int Hkv, int S, int pages,
+                                                         int columns, PageDiv by) {
   using L = Layout<D>;
   constexpr int W = D / 8;
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (idx >= words) return;
-  const int w = (int)(idx % W);
-  const int64_t bhs = idx / W;
-  const int j = (int)(bhs % S);
-  const int64_t bh = bhs / S;
-  const int h = (int)(bh % Hkv);
-  const int64_t b = bh / Hkv;
-  const int64_t len = min((int64_t)lens[b], (int64_t)columns * P);
+  const int b = blockIdx.x / blocks, h = blockIdx.y, w = threadIdx.x % W;
+  const int64_t token = (int64_t)(blockIdx.x - b * blocks) * (256 / W) + threadIdx.x / W;
+  if (token >= S) return;
+  const int j = (int)token;
   float kx[8], vx[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) kx[i] = vx[i] = 0.f;
-  if (j < len) {
-    const int64_t page = table[b * ts + j / P];
+  if (j < min(lens[b], columns * by.P)) {
+    const int column = by(j), off = j - column * by.P, page = table[b * ts + column];
     if (page >= 0 && page < pages) {
-      const uint8_t* u = pool + ((page * Hkv + h) * (P / kUnit) + j % P / kUnit) * (int64_t)L::kBytes;
-      const int r = j % kUnit, g = w / (L::DG / 8);
+      const uint8_t* u = pool + (((int64_t)page * Hkv + h) * (by.P / kUnit) + off / kUnit) * L::kBytes;
+      const int r = off % kUnit, g = w / (L::DG / 8);
       const uint32_t kc = *reinterpret_cast<const uint32_t*>(u + r * L::kRow + 4 * w);
       const uint32_t vc = *reinterpret_cast<const uint32_t*>(u + L::kV + r * L::kRow + 4 * w);
-      const uint32_t kp = *reinterpret_cast<const uint32_t*>(u + L::kKp + (g * kUnit + r) * 4);
-      const uint32_t vp = *reinterpret_cast<const uint32_t*>(u + L::kVp + (g * kUnit + r) * 4);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        kx[i] = fmaf(kv4::pair_scale(kp), (float)(int)((kc >> (4 * i)) & 15u) - 8.f, kv4::pair_centre(kp));
-        vx[i] = fmaf(kv4::pair_scale(vp), (float)(int)((vc >> (4 * i)) & 15u) - 8.f, kv4::pair_centre(vp));
-      }
+      values8(kc, *reinterpret_cast<const uint32_t*>(u + L::kKp + (g * kUnit + r) * 4), kx);
+      values8(vc, *reinterpret_cast<const uint32_t*>(u + L::kVp + (g * kUnit + r) * 4), vx);
     }
   }
-  store8(k_out + bhs * D + 8 * w, kx);
-  store8(v_out + bhs * D + 8 * w, vx);
+  const int64_t to = (((int64_t)b * Hkv + h) * S + j) * D + 8 * w;
+  store8(k_out + to, kx);
+  store8(v_out + to, vx);
 }
 
 }  // namespace
@@ -525,11 +531,11 @@ extern "C" int motif_b200_kv4_gather(const void* pool, const int32_t* block_tabl
     const int64_t none[3] = {0, 0, 0};
     if (int rc = check_rows16("kv4_gather", k_out, none, 1)) return rc;
     if (int rc = check_rows16("kv4_gather", v_out, none, 1)) return rc;
-    const int64_t words = B * Hkv * S * (DD / 8);
-    MB_REQUIRE((words + 255) / 256 < (1ll << 31), MB_ERR_SHAPE, "kv4_gather: %lld rows", (long long)(B * Hkv * S));
-    kv4_gather_kernel<E, DD><<<(unsigned)((words + 255) / 256), 256, 0, (cudaStream_t)stream>>>(
-        (const uint8_t*)pool, block_table, table_stride, lens, (E*)k_out, (E*)v_out, words, (int)Hkv, (int)S,
-        num_pages, (int)page_size, (int)max_pages);
+    const int64_t blocks = (S + 256 / (DD / 8) - 1) / (256 / (DD / 8));
+    MB_REQUIRE(B * blocks < (1ll << 31), MB_ERR_SHAPE, "kv4_gather: %lld rows", (long long)(B * Hkv * S));
+    kv4_gather_kernel<E, DD><<<dim3((unsigned)(B * blocks), (unsigned)Hkv), 256, 0, (cudaStream_t)stream>>>(
+        (const uint8_t*)pool, block_table, table_stride, lens, (E*)k_out, (E*)v_out, (int)blocks, (int)Hkv, (int)S,
+        (int)num_pages, (int)max_pages, page_div(page_size));
     return check_launch("kv4_gather");
   });
 }
