@@ -20,6 +20,7 @@ of one token, s = bf16((max - min) / 15), m = bf16(min + 8 s), c - 8 = the neare
 exceeds the largest float) is stored as NaN.
 """
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -46,33 +47,42 @@ def kv4_pool(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 
                        device=device)
 
 
+@functools.lru_cache(maxsize=256)
+def _shape_dims(shape):
+    pages, kv, units, nbytes = shape
+    return pages, kv, units * UNIT, _DIMS[nbytes]
+
+
 def _pool_dims(pool) -> Tuple[int, int, int, int]:
     """(pages, kv heads, page size, head dim) of a pool."""
     if not isinstance(pool, torch.Tensor) or not pool.is_cuda:
         raise ValueError('pool must live on CUDA')
-    if pool.dtype != torch.uint8 or pool.dim() != 4 or pool.shape[3] not in _DIMS or not pool.is_contiguous():
-        raise ValueError(f'pool must be a contiguous uint8 tensor from kv4_pool, got {pool.dtype} '
-                         f'{tuple(pool.shape)}')
-    pages, kv, units, nbytes = pool.shape
-    return pages, kv, units * UNIT, _DIMS[nbytes]
+    shape = pool.shape
+    if pool.dtype is not torch.uint8 or len(shape) != 4 or shape[3] not in _DIMS or not pool.is_contiguous():
+        raise ValueError(f'pool must be a contiguous uint8 tensor from kv4_pool, got {pool.dtype} {tuple(shape)}')
+    return _shape_dims(shape)
 
 
-def _int32(name, t, shape, dev, dtype=torch.int32):
+def _vector(name, t, n, dev, dtype=torch.int32):
+    """t is a contiguous [n] tensor of dtype on dev."""
     if not isinstance(t, torch.Tensor) or t.device != dev:
         raise ValueError(f'{name} must live on {dev}')
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f'{name} must be a contiguous {dtype} tensor of shape {shape}, got {t.dtype} '
-                         f'{tuple(t.shape)}')
-    return t
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f'{name} must be a contiguous {dtype} tensor [{n}], got {t.dtype} {tuple(t.shape)}')
 
 
 def _table(t, dev, batch=None):
     if not isinstance(t, torch.Tensor) or t.device != dev:
         raise ValueError(f'block_table must live on {dev}')
-    if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or (batch is not None and t.shape[0] != batch):
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.stride(1) != 1 or (batch is not None and t.shape[0] != batch):
         raise ValueError(f'block_table must be an int32 [B, max_pages] tensor with contiguous rows, got {t.dtype} '
                          f'{tuple(t.shape)}')
-    return t
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(index, H, kv, T, D) -> int:
+    with torch.cuda.device(index):
+        return _lib.load().motif_b200_kv4_attention_workspace_bytes(H, kv, T, D)
 
 
 def paged_reserve(lens, new_lens, block_table, free_pages, free_count, page_size: int, total_new: int,
@@ -94,20 +104,25 @@ def paged_reserve(lens, new_lens, block_table, free_pages, free_count, page_size
     if not isinstance(lens, torch.Tensor) or not lens.is_cuda or lens.dim() != 1:
         raise ValueError('lens must be a CUDA tensor [B]')
     dev, B = lens.device, lens.shape[0]
-    _int32('lens', lens, (B,), dev)
-    _int32('new_lens', new_lens, (B,), dev)
+    _vector('lens', lens, B, dev)
+    _vector('new_lens', new_lens, B, dev)
     _table(block_table, dev, B)
-    _int32('free_pages', free_pages, (free_pages.numel(),), dev)
-    _int32('free_count', free_count, (1,), dev)
+    _vector('free_pages', free_pages, free_pages.numel(), dev)
+    _vector('free_count', free_count, 1, dev)
     if total_new < 0:
         raise ValueError(f'total_new must not be negative, got {total_new}')
-    lens_out = torch.empty_like(lens) if lens_out is None else _int32('lens_out', lens_out, (B,), dev)
-    free_count_out = (torch.empty_like(free_count) if free_count_out is None
-                      else _int32('free_count_out', free_count_out, (1,), dev))
-    if slots is None:
-        slots = torch.empty((total_new,), dtype=torch.int32, device=dev)
+    if lens_out is None:
+        lens_out = torch.empty_like(lens)
     else:
-        _int32('slots', slots, (total_new,), dev)
+        _vector('lens_out', lens_out, B, dev)
+    if free_count_out is None:
+        free_count_out = torch.empty_like(free_count)
+    else:
+        _vector('free_count_out', free_count_out, 1, dev)
+    if slots is None:
+        slots = lens.new_empty((total_new,))
+    else:
+        _vector('slots', slots, total_new, dev)
     _lib.call('motif_b200_paged_reserve', lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
               block_table.stride(0), free_pages.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(),
               free_count_out.data_ptr(), slots.data_ptr(), total_new, B, block_table.shape[1], free_pages.numel(),
@@ -122,11 +137,11 @@ def paged_release(done, lens, block_table, free_pages, free_count, page_size: in
     if not isinstance(lens, torch.Tensor) or not lens.is_cuda or lens.dim() != 1:
         raise ValueError('lens must be a CUDA tensor [B]')
     dev, B = lens.device, lens.shape[0]
-    _int32('lens', lens, (B,), dev)
-    _int32('done', done, (B,), dev, torch.bool)
+    _vector('lens', lens, B, dev)
+    _vector('done', done, B, dev, torch.bool)
     _table(block_table, dev, B)
-    _int32('free_pages', free_pages, (free_pages.numel(),), dev)
-    _int32('free_count', free_count, (1,), dev)
+    _vector('free_pages', free_pages, free_pages.numel(), dev)
+    _vector('free_count', free_count, 1, dev)
     _lib.call('motif_b200_paged_release', done.data_ptr(), lens.data_ptr(), block_table.data_ptr(),
               block_table.stride(0), free_pages.data_ptr(), free_count.data_ptr(), B, block_table.shape[1],
               free_pages.numel(), page_size, _lib.stream_ptr(dev))
@@ -134,8 +149,9 @@ def paged_release(done, lens, block_table, free_pages, free_count, page_size: in
 
 def _rows16(t):
     """t with rows that the kernel can read as 16-byte vectors (a copy where they are not)."""
-    e = t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in t.stride()[:-1]):
+    *outer, last = t.stride()
+    step = 16 // t.element_size()
+    if last == 1 and t.data_ptr() % 16 == 0 and not any(s % step for s in outer):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -163,22 +179,24 @@ def kv4_append(k, v, slots, pool, values: bool = False):
         raise ValueError(f'k / v must be [N, {kv}, {D}] or [B, {kv}, T, {D}], got {tuple(k.shape)}, {tuple(v.shape)}')
     if k.dtype != v.dtype:
         raise ValueError('k / v must share one dtype')
-    if k.requires_grad or v.requires_grad:
-        if torch.is_grad_enabled():
-            raise NotImplementedError('the 4-bit cache is forward-only (no autograd)')
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        raise NotImplementedError('the 4-bit cache is forward-only (no autograd)')
     B, T = (1, k.shape[0]) if k.dim() == 3 else (k.shape[0], k.shape[2])
-    _int32('slots', slots, (B * T,), dev)
+    _vector('slots', slots, B * T, dev)
     dc = _lib.dtype_code(k.dtype)
     k, v = _rows16(k), _rows16(v)
-    ko = vo = None
-    strides = [*_token_strides(k), *_token_strides(v), 0, 0, 0, 0, 0, 0]
-    if values:
-        ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        vo = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        strides[6:] = [*_token_strides(ko), *_token_strides(vo)]
-    _lib.call('motif_b200_kv4_append', k.data_ptr(), v.data_ptr(), slots.data_ptr(), pool.data_ptr(), _lib.ptr(ko),
-              _lib.ptr(vo), _lib.i64_array(strides), B, T, kv, D, pages, page_size, dc, _lib.stream_ptr(dev))
-    return (ko, vo) if values else None
+    if not values:
+        strides = _lib.i64_const(*_token_strides(k), *_token_strides(v), 0, 0, 0, 0, 0, 0)
+        _lib.call('motif_b200_kv4_append', k.data_ptr(), v.data_ptr(), slots.data_ptr(), pool.data_ptr(), None, None,
+                  strides, B, T, kv, D, pages, page_size, dc, _lib.stream_ptr(dev))
+        return None
+    ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+    vo = torch.empty_like(ko)
+    to = _token_strides(ko)
+    strides = _lib.i64_const(*_token_strides(k), *_token_strides(v), *to, *to)
+    _lib.call('motif_b200_kv4_append', k.data_ptr(), v.data_ptr(), slots.data_ptr(), pool.data_ptr(), ko.data_ptr(),
+              vo.data_ptr(), strides, B, T, kv, D, pages, page_size, dc, _lib.stream_ptr(dev))
+    return ko, vo
 
 
 def kv4_gather(pool, block_table, lens, max_len: int, dtype=torch.bfloat16):
@@ -188,12 +206,12 @@ def kv4_gather(pool, block_table, lens, max_len: int, dtype=torch.bfloat16):
     dev = pool.device
     _table(block_table, dev)
     B = block_table.shape[0]
-    _int32('lens', lens, (B,), dev)
+    _vector('lens', lens, B, dev)
     if max_len < 0:
         raise ValueError(f'max_len must not be negative, got {max_len}')
     dc = _lib.dtype_code(dtype)
     k = torch.empty((B, kv, max_len, D), dtype=dtype, device=dev)
-    v = torch.empty((B, kv, max_len, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     _lib.call('motif_b200_kv4_gather', pool.data_ptr(), block_table.data_ptr(), block_table.stride(0), lens.data_ptr(),
               k.data_ptr(), v.data_ptr(), B, kv, max_len, D, pages, page_size, block_table.shape[1], dc,
               _lib.stream_ptr(dev))
@@ -225,19 +243,21 @@ def kv4_chord_attention(q, pool, block_table, lens, alpha, beta, mu, ssmax, q_le
         raise NotImplementedError('the 4-bit cache is forward-only (no autograd)')
     dc = _lib.dtype_code(q.dtype)
     _table(block_table, dev, B)
-    _int32('lens', lens, (B,), dev)
+    _vector('lens', lens, B, dev)
     if q_lens is not None:
-        _int32('q_lens', q_lens, (B,), dev)
-    for name, t in (('alpha', alpha), ('beta', beta), ('mu', mu), ('ssmax', ssmax)):
-        _int32(name, t, (H,), dev, torch.float32)
+        _vector('q_lens', q_lens, B, dev)
+    _vector('alpha', alpha, H, dev, torch.float32)
+    _vector('beta', beta, H, dev, torch.float32)
+    _vector('mu', mu, H, dev, torch.float32)
+    _vector('ssmax', ssmax, H, dev, torch.float32)
     q = _rows16(q)
-    out = torch.empty((B, H, T, D), dtype=q.dtype, device=dev)
-    ws_bytes = _lib.load().motif_b200_kv4_attention_workspace_bytes(H, kv, T, D)
-    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
-    strides = _lib.i64_array([*q.stride()[:3], *out.stride()[:3]])
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ws_bytes = _attention_workspace(dev.index, H, kv, T, D)
+    ws = pool.new_empty((ws_bytes,))
+    strides = _lib.i64_const(*q.stride()[:3], *out.stride()[:3])
     _lib.call('motif_b200_kv4_chord_attention', q.data_ptr(), pool.data_ptr(), block_table.data_ptr(),
               block_table.stride(0), lens.data_ptr(), _lib.ptr(q_lens), alpha.data_ptr(), beta.data_ptr(),
               mu.data_ptr(), ssmax.data_ptr(), out.data_ptr(), strides, B, H, kv, T, D, pages, page_size,
               block_table.shape[1], D ** -0.5 if softmax_scale is None else float(softmax_scale), float(eps),
-              _lib.ptr(ws), ws_bytes, dc, _lib.stream_ptr(dev))
+              ws.data_ptr(), ws_bytes, dc, _lib.stream_ptr(dev))
     return out

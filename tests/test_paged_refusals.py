@@ -110,8 +110,8 @@ def test_device_checks():
     with pytest.raises(ValueError, match='block_table'):
         paged._table(torch.zeros(2, 2, dtype=torch.int32).t()[:, ::2], torch.device('cpu'), 3)
     with pytest.raises(ValueError, match='lens'):
-        paged._int32('lens', torch.zeros(3, dtype=torch.int64), (3,), torch.device('cpu'))
+        paged._vector('lens', torch.zeros(3, dtype=torch.int64), 3, torch.device('cpu'))
     with pytest.raises(ValueError, match='lens'):
-        paged._int32('lens', torch.zeros(3, dtype=torch.int32), (2,), torch.device('cpu'))
+        paged._vector('lens', torch.zeros(3, dtype=torch.int32), 2, torch.device('cpu'))
     with pytest.raises(ValueError, match='pool'):
         paged._pool_dims(pool[:, :, :, :100])
