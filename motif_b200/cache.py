@@ -7,6 +7,9 @@
 * `GatedDeltaAttentionLayerCache` keeps the recurrent state `[B, H, Dk, Dv]` in fp32 and
   the three conv states in one time-major `[B, 3, C]` buffer (C = q | k | v channels), the
   layout the decode kernel reads; `conv_state` exposes the reference's `[B, D, 3]` views.
+* `KV4LayerCache` keeps the keys / values in 4 bits in a pool of pages (`motif_b200.paged`); the
+  layers of one model cache share the block table, lengths and free list of a `KV4Pages`.  No
+  counterpart in the reference.
 * `AttnResCache`, `DecoderBlockCache`, `ModelCache`, `build_cache` follow
   `cache.py:397-847` line for line.
 """
@@ -15,6 +18,8 @@ from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+
+from .paged import kv4_append, kv4_gather, kv4_pool, paged_reserve
 
 
 class BasicLayerCache:
@@ -133,6 +138,128 @@ class FunctionalKVLayerCache(KVLayerCache):
             self._vbuf = torch.cat([self.v, v_new.detach()], dim=2)
         self.length = self._kbuf.shape[2]
         return self.k, self.v
+
+
+class KV4Pages:
+    """Pages of the 4-bit Chord caches of one model cache: every layer has a pool of its own, all
+    layers share the block table, the cached lengths and the free list (a token has the same slot
+    in every layer).  Room for `capacity` tokens of every request is set aside at the first use."""
+
+    def __init__(self, capacity: int, page_size: int = 64):
+        if capacity < 1:
+            raise ValueError(f'capacity must be positive, got {capacity}')
+        self.capacity_asked = int(capacity)
+        self.page_size = int(page_size)
+        self.columns = -(-self.capacity_asked // self.page_size)
+        self.reset()
+
+    def reset(self):
+        self.length = 0       # tokens of every request that have slots
+        self.batch = 0
+        self.table = self.lens = self.free = self.count = None
+        self.slots = None     # of the newest tokens
+        self._new = None
+
+    @property
+    def capacity(self) -> int:
+        return self.columns * self.page_size
+
+    def bind(self, batch: int, device):
+        if self.batch == 0:
+            self.batch = batch
+            pages = batch * self.columns
+            self.table = torch.full((batch, self.columns), -1, dtype=torch.int32, device=device)
+            self.lens = torch.zeros((batch,), dtype=torch.int32, device=device)
+            self.free = torch.arange(pages, dtype=torch.int32, device=device)
+            self.count = torch.full((1,), pages, dtype=torch.int32, device=device)
+        elif batch != self.batch or self.lens.device != device:
+            raise ValueError(f'the cache holds {self.batch} requests on {self.lens.device}, got {batch} on {device}')
+
+    def take(self, start: int, tokens: int) -> torch.Tensor:
+        """Slots of `tokens` more tokens of every request behind the first `start`; the first layer
+        that asks reserves them, the others get the same ones."""
+        if start == self.length:
+            if start + tokens > self.capacity:
+                raise ValueError(f'{start + tokens} tokens exceed the cache capacity of {self.capacity}')
+            if self._new is None or self._new[0] != tokens:
+                self._new = (tokens, torch.full_like(self.lens, tokens))
+            self.slots, _, _ = paged_reserve(self.lens, self._new[1], self.table, self.free, self.count,
+                                             self.page_size, self.batch * tokens, lens_out=self.lens,
+                                             free_count_out=self.count)
+            self.length += tokens
+        elif start + tokens != self.length or self.slots.numel() != self.batch * tokens:
+            raise ValueError(f'the Chord layers disagree on length: {start} + {tokens} against {self.length}')
+        return self.slots
+
+    def to(self, device):
+        for n in ('table', 'lens', 'free', 'count', 'slots'):
+            t = getattr(self, n)
+            if t is not None:
+                setattr(self, n, t.to(device))
+        self._new = None
+
+
+class KV4LayerCache(KVLayerCache):
+    """Key / value cache of a chord layer in 4 bits, on the pages of a shared `KV4Pages`."""
+
+    def __init__(self, pages: KV4Pages):
+        super().__init__()
+        self.pages = pages
+        self.pool: Optional[torch.Tensor] = None
+        self.dtype: Optional[torch.dtype] = None
+
+    @property
+    def capacity(self) -> int:
+        return self.pages.capacity
+
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor, values: bool = False):
+        """Store `[B, H_kv, T, D]` keys / values; with `values`, return what the stored bits stand for."""
+        B, Hkv, T, D = k_new.shape
+        self.pages.bind(B, k_new.device)
+        if self.pool is None:
+            self.pool = kv4_pool(B * self.pages.columns, Hkv, D, self.pages.page_size, k_new.device)
+            self.dtype = k_new.dtype
+        out = kv4_append(k_new.detach(), v_new.detach(), self.pages.take(self.length, T), self.pool, values=values)
+        self.length += T
+        return out
+
+    def gather(self):
+        """The cached keys and values, `[B, H_kv, length, D]` in the dtype they came in."""
+        return kv4_gather(self.pool, self.pages.table, self.pages.lens, self.length, dtype=self.dtype)
+
+    @property
+    def k(self) -> Optional[torch.Tensor]:
+        return None if self.pool is None else self.gather()[0]
+
+    @property
+    def v(self) -> Optional[torch.Tensor]:
+        return None if self.pool is None else self.gather()[1]
+
+    def reserve(self, need: int, like: torch.Tensor = None, shape=None):
+        if need > self.capacity:
+            raise ValueError(f'{need} tokens exceed the cache capacity of {self.capacity}')
+
+    def update(self, k_new, v_new, dim: int = 2):
+        if dim not in (2, -2):
+            raise ValueError('KVLayerCache stores the sequence on dim 2')
+        self.append(k_new, v_new)
+        return self.gather()
+
+    def reset(self):
+        super().reset()
+        self.pool = None
+        self.pages.reset()
+
+    def to(self, device=None, dtype=None):
+        if dtype is not None:
+            self.dtype = dtype
+        if device is not None and self.pool is not None:
+            self.pool = self.pool.to(device)
+            self.pages.to(device)
+        return self
+
+    def __repr__(self):
+        return f'KV4LayerCache(seq_length={self.length}, capacity={self.capacity})'
 
 
 class GatedDeltaAttentionLayerCache(BasicLayerCache):
@@ -338,8 +465,19 @@ class ModelCache:
 
 
 def build_cache(model, use_attn: Optional[bool] = None, functional: bool = False,
-                wide_kv: bool = False) -> ModelCache:
-    """`build_cache` (`motif/model/cache.py:802-847`)."""
+                wide_kv: bool = False, kv_bits: Optional[int] = None, kv_capacity: Optional[int] = None,
+                page_size: int = 64) -> ModelCache:
+    """`build_cache` (`motif/model/cache.py:802-847`).  `kv_bits=4` keeps the Chord layers' keys and
+    values in 4 bits, with room for `kv_capacity` tokens of every request on pages of `page_size`."""
+    pages = None
+    if kv_bits is not None:
+        if kv_bits != 4:
+            raise NotImplementedError(f'kv_bits must be 4 (or None: the model dtype), got {kv_bits}')
+        if kv_capacity is None:
+            raise ValueError('kv_bits=4 needs kv_capacity, the most tokens a request may cache')
+        if functional or wide_kv or use_attn is False:
+            raise ValueError('kv_bits=4 goes with neither functional, wide_kv nor use_attn=False')
+        pages, use_attn = KV4Pages(kv_capacity, page_size), True
     if use_attn is None:
         use_attn = not getattr(model, 'training', False)
     if not use_attn:
@@ -349,6 +487,9 @@ def build_cache(model, use_attn: Optional[bool] = None, functional: bool = False
         attn = []
         for decoder in block.features:
             t = decoder.cache_type
+            if pages is not None and issubclass(t, KVLayerCache):
+                attn.append(KV4LayerCache(pages))
+                continue
             if functional and issubclass(t, KVLayerCache):
                 t = FunctionalKVLayerCache
             if wide_kv and issubclass(t, KVLayerCache):

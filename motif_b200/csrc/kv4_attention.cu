@@ -818,6 +818,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(T* __restrict_
   static_assert(NV <= kMergeThreads && kMergeThreads % NV == 0, "whole groups of threads");
   __shared__ float s_m[PL][RT], s_l[PL][RT];
   __shared__ float4 s_acc[PL][NV];
+  allow_dependent_launch();  // a projection that follows may start fetching its weights
   const int tid = threadIdx.x;
   const Requests reqs = scan_requests<KT>(a);
   const int zh = a.Z * a.Hkv;

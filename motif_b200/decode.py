@@ -18,6 +18,11 @@ The math is the eager T = 1 path's: the same kernels in the same order, except t
 split-KV count is fixed at capture (from the cache capacity) instead of chosen per length;
 with `model.decode_splits` set, graph and eager decode give identical tokens.
 
+A cache built with `kv_bits=4` keeps the Chord layers' keys and values in 4 bits on shared pages:
+the step then reserves one slot per request (`motif_b200_paged_reserve`), and each Chord layer
+appends to its pool and attends over it (`motif_b200_kv4_append` / `_kv4_chord_attention`); the
+lengths that the attention reads are the pages' own, one per request.
+
 With a `motif_b200.sampler.Sampler` (no grammar constraint: its hooks run on the host), the
 argmax is replaced by `motif_b200_sample`: the Philox offset is the sampler's offset plus the
 device step counter, and the repetition-penalty history is a device buffer [B, start + 1 +
@@ -31,8 +36,9 @@ from typing import List, Optional, Tuple
 import torch
 
 from . import _lib
-from .cache import GatedDeltaAttentionLayerCache, KVLayerCache, ModelCache
+from .cache import GatedDeltaAttentionLayerCache, KV4LayerCache, KVLayerCache, ModelCache
 from .config import GGD_EPS, NORM_EPS
+from .paged import kv4_append, kv4_chord_attention, paged_reserve
 from .model import _chord_tail, _decode_splits, _down_add_gated, _mm, _norm_read
 
 __all__ = ['GraphDecoder', 'fill_cache_random']
@@ -57,6 +63,12 @@ def _check_layer_caches(model, cache: ModelCache, B: int, need: int):
         for i, dec in enumerate(block.features):
             lc = bc.attn[i]
             if dec.attn_type == 'chord':
+                if isinstance(lc, KV4LayerCache) and lc.pool is not None:
+                    if lc.pages.batch != B:
+                        raise ValueError(f'block {b} decoder {i}: KV cache batch mismatch')
+                    lc.reserve(need)
+                    kv.append(lc)
+                    continue
                 if not isinstance(lc, KVLayerCache) or lc._kbuf is None:
                     raise ValueError(f'block {b} decoder {i}: an allocated KVLayerCache is required')
                 if lc.wide:
@@ -73,6 +85,8 @@ def _check_layer_caches(model, cache: ModelCache, B: int, need: int):
                 if lc._conv.dtype != dt or not lc._conv.is_contiguous():
                     lc._conv = lc._conv.to(dt).contiguous()
                 gdn.append(_GDNSlot(lc))
+    if len({isinstance(lc, KV4LayerCache) for lc in kv}) > 1:
+        raise ValueError('the Chord layers must all keep their cache in 4 bits, or none of them')
     lengths = {lc.length for lc in kv}
     if len(lengths) > 1:
         raise ValueError(f'Chord layer caches disagree on length: {sorted(lengths)}')
@@ -105,6 +119,9 @@ class GraphDecoder:
         kv0 = None
         for bc in cache:
             for lc in bc.attn:
+                if isinstance(lc, KV4LayerCache) and lc.pool is not None:
+                    kv0 = lc
+                    break
                 if isinstance(lc, KVLayerCache) and lc._kbuf is not None:
                     kv0 = lc
                     break
@@ -112,7 +129,9 @@ class GraphDecoder:
                 break
         if kv0 is None:
             raise ValueError('no allocated KV cache: prefill the cache before building the graph')
-        self.B = kv0._kbuf.shape[0]
+        # a 4-bit cache: its pages, whose lengths and free list the captured step advances in place
+        self.pages = kv0.pages if isinstance(kv0, KV4LayerCache) else None
+        self.B = kv0._kbuf.shape[0] if self.pages is None else self.pages.batch
         self.start = kv0.length
         self.seq_start = cache.seq_len  # the block histories' token count (`ModelCache.seq_len`)
         self.max_steps = int(max_steps)
@@ -155,6 +174,9 @@ class GraphDecoder:
             if finished is not None:
                 self.finished.copy_(finished.reshape(-1).to(self.dev, torch.bool))
             self.all_done = torch.zeros((self.max_steps,), dtype=torch.bool, device=self.dev)
+        if self.pages is not None:
+            self.one_new = torch.ones((self.B,), dtype=torch.int32, device=self.dev)
+            self.slots = torch.empty((self.B,), dtype=torch.int32, device=self.dev)
         self.launches_per_step = 0
         self.graph = None
         self._capture()
@@ -171,6 +193,10 @@ class GraphDecoder:
         _lib.call('motif_b200_embed', _lib.ptr(self.ids), _lib.ptr(w), _lib.ptr(x), B, d, cfg.vocab_size, dc, st)
         hn = torch.empty((B, d), dtype=dt, device=dev)
         _norm_read([x], None, None, None, hn)
+        pg = self.pages
+        if pg is not None:  # one slot per request for this step's token, the same in every layer
+            paged_reserve(pg.lens, self.one_new, pg.table, pg.free, pg.count, pg.page_size, B, lens_out=pg.lens,
+                          free_count_out=pg.count, slots=self.slots)
         kv_i = gdn_i = 0
         for b, block in enumerate(model.blocks):
             fs: List[torch.Tensor] = []
@@ -237,9 +263,12 @@ class GraphDecoder:
         H, Hkv, D, hid = pk.H, pk.Hkv, pk.D, pk.hid
         d = H * D
         N_in = proj.shape[1]
-        cap = lc._kbuf.shape[2]
         qb = torch.empty((B, d), dtype=dt, device=dev)
         act = torch.empty((B, hid), dtype=dt, device=dev)
+        if self.pages is not None:
+            attn = self._attend_kv4(pk, proj, lc, qb, act, dc, st)
+            return self._chord_rest(pk, proj, attn, act, dc, st)
+        cap = lc._kbuf.shape[2]
         lens_ptr = self.lens.data_ptr()
         # q/k norms + cache append and the MLP activation in one launch
         _lib.call('motif_b200_chord_prep_swiglu', _lib.ptr(proj), N_in, _lib.ptr(pk.qn_w), _lib.ptr(pk.kn_w),
@@ -251,6 +280,26 @@ class GraphDecoder:
         _lib.call('motif_b200_chord_decode', _lib.ptr(qb), _lib.ptr(lc._kbuf), _lib.ptr(lc._vbuf), cap,
                   lens_ptr + 4, 0, _lib.ptr(pk.alpha), _lib.ptr(pk.beta), _lib.ptr(pk.mu), _lib.ptr(pk.ssmax),
                   _lib.ptr(attn), d, B, H, Hkv, 1, D, D ** -0.5, GGD_EPS, self.splits, _lib.ptr(ws), ws_bytes, dc, st)
+        return self._chord_rest(pk, proj, attn, act, dc, st)
+
+    def _attend_kv4(self, pk, proj, lc: KV4LayerCache, qb, act, dc, st):
+        """q / k norms and the MLP activation, the 4-bit append, and attention over the pages."""
+        B, dt, dev = self.B, self.dt, self.dev
+        H, Hkv, D, hid = pk.H, pk.Hkv, pk.D, pk.hid
+        N_in = proj.shape[1]
+        kt = torch.empty((B, Hkv, 1, D), dtype=dt, device=dev)
+        vt = torch.empty_like(kt)
+        _lib.call('motif_b200_chord_prep_swiglu', _lib.ptr(proj), N_in, _lib.ptr(pk.qn_w), _lib.ptr(pk.kn_w),
+                  _lib.ptr(qb), _lib.ptr(kt), _lib.ptr(vt), 1, None, 0, B, 1, H, Hkv, D, NORM_EPS,
+                  proj.data_ptr() + pk.off_gu * proj.element_size(), N_in, _lib.ptr(act), hid, hid, dc, st)
+        kv4_append(kt, vt, self.slots, lc.pool)
+        pg = self.pages
+        return kv4_chord_attention(qb.view(B, H, 1, D), lc.pool, pg.table, pg.lens, pk.alpha, pk.beta, pk.mu, pk.ssmax,
+                                   softmax_scale=D ** -0.5, eps=GGD_EPS).view(B, H * D)
+
+    def _chord_rest(self, pk, proj, attn, act, dc, st):
+        """o_proj, down_proj and the gated residual."""
+        B, d, N_in = self.B, pk.H * pk.D, proj.shape[1]
         gate = proj[:, pk.off_g:pk.off_g + d]
         f = _chord_tail(attn, pk.w_o, act, pk.w_down, gate)
         if f is not None:  # o_proj, down_proj and the gated residual in one launch
@@ -268,7 +317,8 @@ class GraphDecoder:
     def _snapshot(self):
         hist = None if self.hist is None else (self.hist.clone(), self.hist_col.clone())
         fin = None if self.eos is None else self.finished.clone()
-        return [s.state.clone() for s in self.gdn], [s.conv.clone() for s in self.gdn], hist, fin
+        pages = None if self.pages is None else (self.pages.lens.clone(), self.pages.count.clone())
+        return [s.state.clone() for s in self.gdn], [s.conv.clone() for s in self.gdn], hist, fin, pages
 
     def _restore(self, snap):
         for s, st_, cv in zip(self.gdn, snap[0], snap[1]):
@@ -279,6 +329,9 @@ class GraphDecoder:
             self.hist_col.copy_(snap[2][1])
         if snap[3] is not None:
             self.finished.copy_(snap[3])
+        if snap[4] is not None:  # table entries past the restored lengths are written again
+            self.pages.lens.copy_(snap[4][0])
+            self.pages.count.copy_(snap[4][1])
 
     def set_history(self, history: torch.Tensor):
         """Seed the repetition-penalty history with the sequence so far ([B, start + 1], ending
@@ -362,6 +415,8 @@ class GraphDecoder:
         histories' `seq_len` (each step feeds one token)."""
         for lc in self.kv:
             lc.length = self.start + self.taken
+        if self.pages is not None:
+            self.pages.length = self.start + self.taken
         for s in self.gdn:
             s.cache.length = self.start + self.taken
         for bc in self.cache:
@@ -416,6 +471,13 @@ def fill_cache_random(model, cache: ModelCache, batch: int, length: int, capacit
             lc = bc.attn[i]
             if dec.attn_type == 'chord':
                 Hkv, D = cfg.kv_heads, cfg.head_dim
+                if isinstance(lc, KV4LayerCache):
+                    lc.reserve(capacity)
+                    for t0 in range(0, length, 1024):
+                        shape = (batch, Hkv, min(1024, length - t0), D)
+                        lc.append(torch.empty(shape, dtype=dt, device=dev).normal_(0.0, 1.0, generator=g),
+                                  torch.empty(shape, dtype=dt, device=dev).normal_(0.0, 0.5, generator=g))
+                    continue
                 lc._kbuf = torch.empty((batch, Hkv, capacity, D), dtype=dt, device=dev)
                 lc._vbuf = torch.empty_like(lc._kbuf)
                 lc._kbuf.normal_(0.0, 1.0, generator=g)

@@ -39,9 +39,10 @@ import torch.nn.functional as F
 
 from . import _lib
 from .cache import (AttnResCache, BasicLayerCache, DecoderBlockCache, GatedDeltaAttentionLayerCache,
-                    KVLayerCache, ModelCache, build_cache)
+                    KV4LayerCache, KVLayerCache, ModelCache, build_cache)
 from .config import CHUNK_SIZE, CONV_SIZE, EXPAND_V, GGD_EPS, NORM_EPS, MotifChordConfig
 from .ops import GatedRMSNorm, RMSNorm, SwiGLU as SwiGLUOp
+from .paged import kv4_chord_attention
 from .sampler import Sampler, make_sampler
 
 
@@ -484,10 +485,13 @@ class MotifChordModel(nn.Module):
     def cache_types(self):
         return [[d.cache_type for d in blk.features] for blk in self.blocks]
 
-    def create_cache(self, use_attn: Optional[bool] = None, functional: bool = False,
-                     wide_kv: bool = False) -> ModelCache:
-        """`create_cache` (`model/motif.py:413-455`)."""
-        return build_cache(self, use_attn=use_attn, functional=functional, wide_kv=wide_kv)
+    def create_cache(self, use_attn: Optional[bool] = None, functional: bool = False, wide_kv: bool = False,
+                     kv_bits: Optional[int] = None, kv_capacity: Optional[int] = None,
+                     page_size: int = 64) -> ModelCache:
+        """`create_cache` (`model/motif.py:413-455`); `kv_bits=4` with `kv_capacity` keeps the Chord
+        layers' keys and values in 4 bits (`motif_b200.paged`)."""
+        return build_cache(self, use_attn=use_attn, functional=functional, wide_kv=wide_kv, kv_bits=kv_bits,
+                           kv_capacity=kv_capacity, page_size=page_size)
 
     def set_sampler(self, sampler=None, **kwargs):
         """Model-level sampler carried by every later `ModelOutput` (`motif.py:457-482`)."""
@@ -846,6 +850,11 @@ def _decode_splits(model, B, Hkv, S):
     return int(max(1, min(want, 64, (S + 255) // 256)))
 
 
+# Most query rows of a kv head (query heads of its group x new tokens) that attend to a 4-bit cache
+# directly; longer chunks read it back and use the prefill kernel.
+KV4_DIRECT_ROWS = 64
+
+
 def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache], position, dt, dev, dc, st,
                    key_bias: Optional[torch.Tensor] = None):
     """`ChordAttention.forward` (fused path) + SwiGLU MLP + parallel residual.  `key_bias`
@@ -868,7 +877,33 @@ def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache
     cached = cache.length
     q_start = position if position != 0 else cached
     qb = torch.empty((M, d), dtype=dt, device=dev)
-    if cache.wide:
+    scale = D ** -0.5
+    G = H // Hkv
+    attn = None
+    kv = None  # contiguous keys and values [B, Hkv, S, D] of a cache that does not hold them so
+    if isinstance(cache, KV4LayerCache):
+        kt = torch.empty((B, Hkv, T, D), dtype=dt, device=dev)
+        vt = torch.empty_like(kt)
+        if act_done:
+            _lib.call('motif_b200_chord_prep', _lib.ptr(proj), N_in, _lib.ptr(pk.qn_w), _lib.ptr(pk.kn_w),
+                      _lib.ptr(qb), _lib.ptr(kt), _lib.ptr(vt), T, None, 0, B, T, H, Hkv, D, NORM_EPS, dc, st)
+        else:
+            _lib.call('motif_b200_chord_prep_swiglu', _lib.ptr(proj), N_in, _lib.ptr(pk.qn_w), _lib.ptr(pk.kn_w),
+                      _lib.ptr(qb), _lib.ptr(kt), _lib.ptr(vt), T, None, 0, B, T, H, Hkv, D, NORM_EPS,
+                      proj.data_ptr() + pk.off_gu * proj.element_size(), N_in, _lib.ptr(act), hid, hid, dc, st)
+            act_done = True
+        if cached == 0 and T > 1:
+            # a first chunk attends to the values that its stored bits stand for, as later tokens will
+            kv = cache.append(kt, vt, values=True)
+        else:
+            cache.append(kt, vt)
+            if key_bias is None and q_start == cached and G * T <= KV4_DIRECT_ROWS:
+                attn = kv4_chord_attention(qb.view(B, T, H, D).transpose(1, 2), cache.pool, cache.pages.table,
+                                           cache.pages.lens, pk.alpha, pk.beta, pk.mu, pk.ssmax, softmax_scale=scale,
+                                           eps=GGD_EPS).transpose(1, 2).reshape(M, d)
+            else:
+                kv = cache.gather()
+    elif cache.wide:
         # a wide cache (`cache.py:42-70`) stores every key / value head once per query head: the
         # new keys / values are prepared narrow, widened by the cache's own update, and the
         # attention then reads one kv head per query head (the same arithmetic as grouped)
@@ -895,35 +930,38 @@ def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache
                   hid, hid, dc, st)
         act_done = True
         cache.length = cached + T
-    cap = cache._kbuf.shape[2]
     S = cache.length
-    attn = torch.empty((M, d), dtype=dt, device=dev)
-    scale = D ** -0.5
+    kbuf, vbuf = (cache._kbuf, cache._vbuf) if kv is None else kv
+    cap = 0 if attn is not None else kbuf.shape[2]
     G = H // Hkv
-    if q_start == S - T and G * T <= 16 and D in (32, 64):
+    if attn is not None:
+        pass
+    elif q_start == S - T and G * T <= 16 and D in (32, 64):
+        attn = torch.empty((M, d), dtype=dt, device=dev)
         splits = _decode_splits(model, B, Hkv, S)
         ws_bytes = _lib.load().motif_b200_chord_decode_workspace_bytes(B, H, T, D, splits)
         ws = torch.empty((ws_bytes // 4,), dtype=torch.float32, device=dev)
         if key_bias is None:
-            _lib.call('motif_b200_chord_decode', _lib.ptr(qb), _lib.ptr(cache._kbuf), _lib.ptr(cache._vbuf), cap,
+            _lib.call('motif_b200_chord_decode', _lib.ptr(qb), _lib.ptr(kbuf), _lib.ptr(vbuf), cap,
                       None, S, _lib.ptr(pk.alpha), _lib.ptr(pk.beta), _lib.ptr(pk.mu), _lib.ptr(pk.ssmax),
                       _lib.ptr(attn), d, B, H, Hkv, T, D, scale, GGD_EPS, splits, _lib.ptr(ws), ws_bytes, dc, st)
         else:
-            _lib.call('motif_b200_chord_decode_masked', _lib.ptr(qb), _lib.ptr(cache._kbuf), _lib.ptr(cache._vbuf),
+            _lib.call('motif_b200_chord_decode_masked', _lib.ptr(qb), _lib.ptr(kbuf), _lib.ptr(vbuf),
                       cap, None, S, _lib.ptr(pk.alpha), _lib.ptr(pk.beta), _lib.ptr(pk.mu), _lib.ptr(pk.ssmax),
                       _lib.ptr(attn), d, B, H, Hkv, T, D, scale, GGD_EPS, splits, _lib.ptr(key_bias),
                       key_bias.stride(0), _lib.ptr(ws), ws_bytes, dc, st)
     else:
+        attn = torch.empty((M, d), dtype=dt, device=dev)
         log_n = _log_n(q_start, T, dev)
         strides = [T * d, D, d, Hkv * cap * D, cap * D, D, Hkv * cap * D, cap * D, D, T * d, D, d, 0, 1]
         if key_bias is None:
-            _lib.call('motif_b200_chord_attention', _lib.ptr(qb), _lib.ptr(cache._kbuf), _lib.ptr(cache._vbuf),
+            _lib.call('motif_b200_chord_attention', _lib.ptr(qb), _lib.ptr(kbuf), _lib.ptr(vbuf),
                       _lib.ptr(pk.alpha), _lib.ptr(pk.beta), _lib.ptr(pk.mu), _lib.ptr(pk.ssmax), _lib.ptr(log_n),
                       _lib.ptr(attn), B, H, Hkv, T, S, D, q_start, scale, GGD_EPS, _lib.i64_array(strides), dc, None,
                       0, st)
         else:
-            _lib.call('motif_b200_chord_attention_masked', _lib.ptr(qb), _lib.ptr(cache._kbuf),
-                      _lib.ptr(cache._vbuf), _lib.ptr(pk.alpha), _lib.ptr(pk.beta), _lib.ptr(pk.mu),
+            _lib.call('motif_b200_chord_attention_masked', _lib.ptr(qb), _lib.ptr(kbuf),
+                      _lib.ptr(vbuf), _lib.ptr(pk.alpha), _lib.ptr(pk.beta), _lib.ptr(pk.mu),
                       _lib.ptr(pk.ssmax), _lib.ptr(log_n), _lib.ptr(attn), B, H, Hkv, T, S, D, q_start, scale,
                       GGD_EPS, _lib.i64_array(strides), _lib.ptr(key_bias), key_bias.stride(0), dc, st)
     if not act_done:
