@@ -157,7 +157,8 @@ class KV4Pages:
         self.length = 0       # tokens of every request that have slots
         self.batch = 0
         self.table = self.lens = self.free = self.count = None
-        self.slots = None     # of the newest tokens
+        self.slots = None     # of the newest tokens, `_at` = (first, number)
+        self._at = None
         self._new = None
 
     @property
@@ -187,8 +188,12 @@ class KV4Pages:
                                              self.page_size, self.batch * tokens, lens_out=self.lens,
                                              free_count_out=self.count)
             self.length += tokens
-        elif start + tokens != self.length or self.slots.numel() != self.batch * tokens:
+            self._at = (start, tokens)
+        elif start + tokens > self.length:
             raise ValueError(f'the Chord layers disagree on length: {start} + {tokens} against {self.length}')
+        elif self._at != (start, tokens):  # a layer that lags by more than the newest tokens
+            pos = torch.arange(start, start + tokens, device=self.table.device)
+            return (self.table[:, pos // self.page_size] * self.page_size + (pos % self.page_size).int()).view(-1)
         return self.slots
 
     def to(self, device):

@@ -851,7 +851,9 @@ def _decode_splits(model, B, Hkv, S):
 
 
 # Most query rows of a kv head (query heads of its group x new tokens) that attend to a 4-bit cache
-# directly; longer chunks read it back and use the prefill kernel.
+# directly; longer chunks read it back and use the prefill kernel.  Measured at 12 / 3 heads of 64,
+# direct against read back: 64 requests of 2048 tokens 94 / 111 us at 64 rows, 170 / 111 at 128; of
+# 8192 tokens 283 / 402 and 547 / 404; 8 requests of 8192 53 / 165 and 85 / 165.
 KV4_DIRECT_ROWS = 64
 
 

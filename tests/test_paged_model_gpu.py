@@ -148,8 +148,10 @@ def test_refusals_and_reset():
 
 
 def test_random_fill_stands_for_a_prefill():
-    m = model_of(torch.bfloat16)
+    m = model_of(torch.bfloat16, block=('chord', 'gdn', 'chord'))
     cache = fill_cache_random(m, m.create_cache(kv_bits=4, kv_capacity=1200), 2, 1100, 1200)
     dec = GraphDecoder(m, cache, max_steps=8)
     toks = dec.run(torch.zeros(2, 1, dtype=torch.int64, device='cuda'), 8)
+    a, b = cache[0].attn[0], cache[0].attn[2]
+    assert a.k.shape == b.v.shape == (2, 2, 1108, 64) and not torch.equal(a.k, b.k)
     assert toks.shape == (2, 8) and dec.pages.lens.tolist() == [1108, 1108] and torch.isfinite(dec.logits).all()
