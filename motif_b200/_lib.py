@@ -8,7 +8,6 @@ dtype / alignment errors, `NotImplementedError` for shapes this build has no ker
 """
 
 import ctypes
-import functools
 import os
 import threading
 
@@ -155,12 +154,6 @@ def stream_ptr(device=None) -> int:
 
 def i64_array(vals):
     vals = [int(v) for v in vals]
-    return (ctypes.c_int64 * len(vals))(*vals)
-
-
-@functools.lru_cache(maxsize=1024)
-def i64_const(*vals):
-    """i64_array of ints for entry points that only read it: one array per value list."""
     return (ctypes.c_int64 * len(vals))(*vals)
 
 

@@ -209,13 +209,25 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, const uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-// The nibbles of w as four fp16 pairs: nibbles (0, 4) and (2, 6) times 2^-24, (1, 5) and (3, 7) times 2^-20.
+// The nibbles of w as four fp16 pairs: nibbles (0, 4) and (2, 6) times U, (1, 5) and (3, 7) times 16 U.
+// For 16-bit tensors they stay the subnormal numbers that the masked bits are (U = 2^-24).  The tensor
+// cores align the products of a step by their operands' exponent fields, which for a subnormal say up
+// to 10 bits more than it has, and cut below 24 bits: sums keep about 17 bits (the results of 300 keys
+// were 3e-5 off where 16 bits round at 4e-4 to 4e-3).  fp32 tensors make them normal numbers c - 8
+// (U = 1: the bits of 1024 or-ed in, 1024 + 8 U taken off) at one more instruction a pair, and need
+// the sums less 8 no more.
+template <bool EXACT>
 __device__ __forceinline__ void codes(uint32_t w, uint32_t* h) {
   const uint32_t v = w >> 8;
   h[0] = w & 0x000f000fu;
   h[1] = w & 0x00f000f0u;
   h[2] = v & 0x000f000fu;
   h[3] = v & 0x00f000f0u;
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(h[i]) : "r"(h[i] | 0x64006400u), "r"(i & 1 ? 0xe480e480u : 0xe408e408u));
+  }
 }
 
 // Eight consecutive elements at a 16-byte aligned address.
@@ -283,6 +295,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
   constexpr int KW = DG / 32;        // 32-bit words of K codes of a thread per row and group
   constexpr int MT = DG / 16;        // 16-dim output tiles of a group
   constexpr int RT = 4 * NT;         // query rows of a row tile
+  constexpr bool EXACT = sizeof(T) == 4;
+  constexpr int kUnitBits = EXACT ? 0 : 24;  // codes enter the products times 2^-kUnitBits
   constexpr int THREADS = 32 * kWarps;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kWarps][kStages];
@@ -449,11 +463,11 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
             float all = sum.x + sum.y;
             all += __shfl_xor_sync(0xffffffffu, all, 1);
             all += __shfl_xor_sync(0xffffffffu, all, 2);
-            sq[n][g] = __shfl_sync(0xffffffffu, all, 8 * t4) * pow2(-24);
+            sq[n][g] = __shfl_sync(0xffffffffu, all, 8 * t4) * pow2(-kUnitBits);
           }
           const int exr = __shfl_sync(0xffffffffu, ex, 8 * t4);
           const float rc = qr[n] * logf((float)pos[n] + 1.f) * kLog2e;
-          qr[n] = a.scale * rc * 2048.f * pow2(exr);
+          qr[n] = a.scale * rc * pow2(kUnitBits - 13) * pow2(exr);
           ar[n] *= -rc;
           ref[n] = 0.f;
           limit[n] = -INFINITY;
@@ -508,14 +522,14 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
               uint32_t c0[4], c1[4];
-              codes(w0[w], c0);
-              codes(w1[w], c1);
+              codes<EXACT>(w0[w], c0);
+              codes<EXACT>(w1[w], c1);
 #pragma unroll
               for (int p = 0; p < 2; ++p) {
                 const uint32_t af[4] = {c0[2 * p], c1[2 * p], c0[2 * p + 1], c1[2 * p + 1]};
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                  const float start = -8.f * sq[n][g];
+                  const float start = EXACT ? 0.f : -8.f * sq[n][g];
                   if (w == 0 && p == 0) mma_f16(acc[n], af, qf[n][g][0], start, 0.f, start, 0.f);
                   else mma_16816<__half>(acc[n], af, qf[n][g][2 * w + p]);
                 }
@@ -627,8 +641,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             const float2 vs = make_float2(kv4::pair_scale(vp[u][g][0]), kv4::pair_scale(vp[u][g][1]));
-            const float2 vm = ffma2(vs, make_float2(-8.f, -8.f),
-                                    make_float2(kv4::pair_centre(vp[u][g][0]), kv4::pair_centre(vp[u][g][1])));
+            const float2 vc = make_float2(kv4::pair_centre(vp[u][g][0]), kv4::pair_centre(vp[u][g][1]));
+            const float2 vm = EXACT ? vc : ffma2(vs, make_float2(-8.f, -8.f), vc);
             const float2 vn2 = fmul2(vs, make_float2(vup, vup));
             uint32_t bf[NT][2];
 #pragma unroll
@@ -650,8 +664,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
             for (int hf = 0; hf < KW; ++hf) {  // halves of a word: four dims each
               const uint32_t sel = KW == 2 ? (hf ? 0x7632u : 0x5410u) : ((g8 & 1) ? 0x7632u : 0x5410u);
               uint32_t c0[4], c1[4];
-              codes(__byte_perm(w[0], w[1], sel), c0);
-              codes(__byte_perm(w[2], w[3], sel), c1);
+              codes<EXACT>(__byte_perm(w[0], w[1], sel), c0);
+              codes<EXACT>(__byte_perm(w[2], w[3], sel), c1);
 #pragma unroll
               for (int p = 0; p < 2; ++p) {
                 const uint32_t af[4] = {c0[2 * p], c0[2 * p + 1], c1[2 * p], c1[2 * p + 1]};
@@ -685,7 +699,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
           pieces[warp][which].begins = from_start;
           pieces[warp][which].ends = ends;
         }
-        const float back = pow2(min(ve, 127));  // and 2^14
+        const float back = pow2(min(ve, 127));  // and 2^(kUnitBits - 10)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float ln = l[n].x + l[n].y, pn[NG];
@@ -707,8 +721,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
             float y[2 * MT];
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
-              y[2 * j] = fmaf((o[n][g][j][0] + o[n][g][j][1]) * 16384.f, back, pn[g]) * inv;
-              y[2 * j + 1] = fmaf((o[n][g][j][2] + o[n][g][j][3]) * 1024.f, back, pn[g]) * inv;
+              y[2 * j] = fmaf((o[n][g][j][0] + o[n][g][j][1]) * pow2(kUnitBits - 10), back, pn[g]) * inv;
+              y[2 * j + 1] = fmaf((o[n][g][j][2] + o[n][g][j][3]) * pow2(kUnitBits - 14), back, pn[g]) * inv;
             }
             const int d0 = g * DG + g8 * 2 * MT;
             if (direct) {

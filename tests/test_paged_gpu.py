@@ -16,9 +16,11 @@ import pytest
 import torch
 
 from motif_b200 import ops
-from motif_b200.paged import _DIMS, UNIT
+from motif_b200.paged import UNIT, _UNIT_BYTES
 
 pytestmark = pytest.mark.gpu
+
+_DIMS = {v: k for k, v in _UNIT_BYTES.items()}
 
 ROUND = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 LOGIT = 3e-5
@@ -539,3 +541,46 @@ def test_step_in_a_cuda_graph_follows_the_lengths():
     ko, _ = ops.kv4_append(ks[:, 0, :, 0].contiguous(), vs[:, 0, :, 0].contiguous(),
                            torch.arange(steps, dtype=torch.int32, device='cuda'), fake, values=True)
     assert torch.equal(gk[0].transpose(0, 1), ko)
+
+
+def test_refusals_on_device_tensors():
+    """Shapes, types and places that the calls refuse before anything is launched."""
+    pool, table, ln = random_cache([20, 3], 2, 64, 16, 30)
+    q, p = torch.zeros(2, 4, 1, 64, device='cuda'), torch.zeros(4, device='cuda')
+    x, slots = torch.zeros(3, 2, 64, device='cuda'), torch.zeros(3, dtype=torch.int32, device='cuda')
+    free, one = torch.zeros(4, dtype=torch.int32, device='cuda'), torch.zeros(1, dtype=torch.int32, device='cuda')
+
+    def bad(match, call, *a, error=ValueError, **kw):
+        with pytest.raises(error, match=match):
+            call(*a, **kw)
+
+    att = ops.kv4_chord_attention
+    bad('q must be', att, q[..., :32], pool, table, ln, p, p, p, p)
+    bad('divisible', att, q[:, :3], pool, table, ln, p[:3], p[:3], p[:3], p[:3])
+    bad('alpha must be', att, q, pool, table, ln, p.double(), p, p, p)
+    bad('mu must be', att, q, pool, table, ln, p, p, p[:3], p)
+    bad('beta must live', att, q, pool, table, ln, p, p.cpu(), p, p)
+    bad('lens must be', att, q, pool, table, ln.long(), p, p, p, p)
+    bad('q_lens must be', att, q, pool, table, ln, p, p, p, p, q_lens=ln[:1])
+    bad('block_table', att, q, pool, table[:1], ln, p, p, p, p)
+    bad('block_table', att, q, pool, table.t(), ln, p, p, p, p)
+    bad('dtype', att, q.double(), pool, table, ln, p, p, p, p)
+    bad('pool must be', att, q, pool[..., :100], table, ln, p, p, p, p)
+    bad('forward-only', att, q.clone().requires_grad_(), pool, table, ln, p, p, p, p, error=NotImplementedError)
+    bad('k / v must be', ops.kv4_append, x[:, :1], x[:, :1], slots, pool)
+    bad('k / v must be', ops.kv4_append, x, x[:2], slots, pool)
+    bad('share one dtype', ops.kv4_append, x, x.half(), slots, pool)
+    bad('slots must be', ops.kv4_append, x, x, slots[:2], pool)
+    bad('slots must be', ops.kv4_append, x, x, slots.long(), pool)
+    bad('forward-only', ops.kv4_append, x.clone().requires_grad_(), x, slots, pool, error=NotImplementedError)
+    bad('max_len', ops.kv4_gather, pool, table, ln, -1)
+    bad('dtype', ops.kv4_gather, pool, table, ln, 3, dtype=torch.int32)
+    bad('new_lens', ops.paged_reserve, ln, ln[:1], table, free, one, 16, 3)
+    bad('free_count', ops.paged_reserve, ln, ln, table, free, free, 16, 3)
+    bad('total_new', ops.paged_reserve, ln, ln, table, free, one, 16, -3)
+    bad('page size', ops.paged_reserve, ln, ln, table, free, one, 20, 3)
+    bad('slots must be', ops.paged_reserve, ln, ln, table, free, one, 16, 3, slots=slots[:2])
+    bad('lens_out', ops.paged_reserve, ln, ln, table, free, one, 16, 3, lens_out=slots)
+    bad('done must be', ops.paged_release, ln, ln, table, free, one, 16)
+    with torch.no_grad():
+        ops.kv4_append(x.clone().requires_grad_(), x, torch.full_like(slots, -1), pool)

@@ -102,16 +102,11 @@ def test_empty_calls_launch_nothing():
     attention(T=0)
 
 
-def test_device_checks():
-    """Shapes, types and devices that the Python calls refuse (checked on meta-free host objects)."""
-    pool = ops.kv4_pool(3, 2, 64, 32, device='cpu')
-    with pytest.raises(ValueError, match='block_table'):
-        paged._table(torch.zeros(2, 2), torch.device('cpu'))
-    with pytest.raises(ValueError, match='block_table'):
-        paged._table(torch.zeros(2, 2, dtype=torch.int32).t()[:, ::2], torch.device('cpu'), 3)
-    with pytest.raises(ValueError, match='lens'):
-        paged._vector('lens', torch.zeros(3, dtype=torch.int64), 3, torch.device('cpu'))
-    with pytest.raises(ValueError, match='lens'):
-        paged._vector('lens', torch.zeros(3, dtype=torch.int32), 2, torch.device('cpu'))
-    with pytest.raises(ValueError, match='pool'):
-        paged._pool_dims(pool[:, :, :, :100])
+def test_host_entries_check_their_arguments():
+    host = paged._host()
+    with pytest.raises(TypeError, match='10 arguments'):
+        host.paged_reserve(1, 2)
+    with pytest.raises(ValueError, match='must be a tensor'):
+        host.kv4_gather(1, 2, 3, 4, 5)
+    with pytest.raises(ValueError, match='must be a tensor'):
+        ops.kv4_append(None, None, None, None)
