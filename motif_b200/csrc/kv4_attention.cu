@@ -297,13 +297,17 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
   constexpr int RT = 4 * NT;         // query rows of a row tile
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int kUnitBits = EXACT ? 0 : 24;  // codes enter the products times 2^-kUnitBits
-  constexpr int THREADS = 32 * kWarps;
+  // 16-bit queries have no low part: with 8 rows or more every column of the first product is a row,
+  // a thread holding rows 2 t4 and 2 t4 + 1 of each 8; else row t4 of each 4, its parts in two columns
+  constexpr bool WIDE = !EXACT && NT > 1;
+  constexpr int QT = WIDE ? NT / 2 : NT;  // column tiles of the first product
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kWarps][kStages];
   __shared__ Piece pieces[kWarps][2];
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g8 = lane >> 2, t4 = lane & 3;
+  auto row_of = [&](int n) { return WIDE ? (n >> 1) * 8 + 2 * t4 + (n & 1) : n * 4 + t4; };  // in the row tile
   uint8_t* ring = smem + warp * (kStages * Tile<D>::kBytes);
   auto piece_at = [&](int w, int which) {
     return reinterpret_cast<float*>(which ? smem + w * (kStages * Tile<D>::kBytes)
@@ -374,7 +378,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
     int looked = 0;  // tiles issued
 
     // state of the current segment
-    uint32_t qf[NT][NG][2 * KW][2];
+    uint32_t qf[QT][NG][2 * KW][2];
     float sq[NT][NG], qr[NT], ar[NT], be[NT], mh[NT];
     int pos[NT];
     // weights are taken against a reference that a row's logits exceed by 2^kSlack at most: it moves
@@ -405,18 +409,21 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
         int t, gi;
         split_row(a, z * RT, t, gi);
         lo_pos = max(0, base + t);
-        float x[NT][NG][8 * KW];
+        float x[QT][NG][8 * KW];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          // the query row of this thread's B fragments: column g8 = (row g8 / 2, part g8 & 1)
-          split_row(a, min(z * RT + n * 4 + (g8 >> 1), rows - 1), t, gi);
+        for (int n = 0; n < QT; ++n) {
+          // the query row of this thread's B fragments: column g8 = row g8, or (row g8 / 2, part g8 & 1)
+          split_row(a, min(z * RT + (WIDE ? n * 8 + g8 : n * 4 + (g8 >> 1)), rows - 1), t, gi);
           const T* qp = q + cur.b * a.st.s[0] + (hk * a.G + gi) * a.st.s[1] + t * a.st.s[2];
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int w = 0; w < KW; ++w) load8(qp + g * DG + t4 * 8 * KW + 8 * w, x[n][g] + 8 * w);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
           // the query row whose scores this thread holds; logits in units of log 2
-          split_row(a, min(z * RT + n * 4 + t4, rows - 1), t, gi);
+          split_row(a, min(z * RT + row_of(n), rows - 1), t, gi);
           const int h = hk * a.G + gi;
           pos[n] = max(0, base + min(t, nq - 1));
           qr[n] = a.ssmax[h];
@@ -430,8 +437,10 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
           looked = 1;
           if (count > 1) next = step();
         }
+        float sums[QT][NG];
+        int exps[QT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int n = 0; n < QT; ++n) {
           float top = 0.f;
 #pragma unroll
           for (int g = 0; g < NG; ++g)
@@ -440,8 +449,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           // power of two that brings the row's largest value to 2^13 .. 2^14 (fp16 ends at 2^16)
-          const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -112), 127);
-          const float up = pow2(13 - ex);
+          exps[n] = min(max((int)(__float_as_uint(top) >> 23) - 127, -112), 127);
+          const float up = pow2(13 - exps[n]);
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             float2 sum = make_float2(0.f, 0.f);
@@ -454,18 +463,23 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
                 // the codes of the odd pairs are 16 times as large
                 const float2 v = p & 1 ? fmul2(y, make_float2(0.0625f, 0.0625f)) : y;
                 uint32_t f = pack2<__half>(v.x, v.y);
-                if (g8 & 1) {  // the low part; values of 16 bits have none
+                if (!WIDE && (g8 & 1)) {  // the low part; values of 16 bits have none
                   const float2 hi = __half22float2(*reinterpret_cast<__half2*>(&f));
-                  f = sizeof(T) == 4 ? pack2<__half>(v.x - hi.x, v.y - hi.y) : 0u;
+                  f = EXACT ? pack2<__half>(v.x - hi.x, v.y - hi.y) : 0u;
                 }
                 qf[n][g][2 * w + (p >> 1)][p & 1] = f;
               }
-            float all = sum.x + sum.y;
-            all += __shfl_xor_sync(0xffffffffu, all, 1);
-            all += __shfl_xor_sync(0xffffffffu, all, 2);
-            sq[n][g] = __shfl_sync(0xffffffffu, all, 8 * t4) * pow2(-kUnitBits);
+            sums[n][g] = sum.x + sum.y;
+            sums[n][g] += __shfl_xor_sync(0xffffffffu, sums[n][g], 1);
+            sums[n][g] += __shfl_xor_sync(0xffffffffu, sums[n][g], 2);
           }
-          const int exr = __shfl_sync(0xffffffffu, ex, 8 * t4);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int qt = WIDE ? n >> 1 : n, from = WIDE ? 4 * (2 * t4 + (n & 1)) : 8 * t4;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) sq[n][g] = __shfl_sync(0xffffffffu, sums[qt][g], from) * pow2(-kUnitBits);
+          const int exr = __shfl_sync(0xffffffffu, exps[qt], from);
           const float rc = qr[n] * logf((float)pos[n] + 1.f) * kLog2e;
           qr[n] = a.scale * rc * pow2(kUnitBits - 13) * pow2(exr);
           ar[n] *= -rc;
@@ -518,7 +532,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
               w0[0] = *reinterpret_cast<const uint32_t*>(at);
               w1[0] = *reinterpret_cast<const uint32_t*>(at + 8 * L::kRow);
             }
-            float acc[NT][4];
+            float acc[QT][4];
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
               uint32_t c0[4], c1[4];
@@ -528,10 +542,14 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
               for (int p = 0; p < 2; ++p) {
                 const uint32_t af[4] = {c0[2 * p], c1[2 * p], c0[2 * p + 1], c1[2 * p + 1]};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  const float start = EXACT ? 0.f : -8.f * sq[n][g];
-                  if (w == 0 && p == 0) mma_f16(acc[n], af, qf[n][g][0], start, 0.f, start, 0.f);
-                  else mma_16816<__half>(acc[n], af, qf[n][g][2 * w + p]);
+                for (int n = 0; n < QT; ++n) {
+                  if (w == 0 && p == 0) {
+                    const float s0 = EXACT ? 0.f : -8.f * sq[WIDE ? 2 * n : n][g];
+                    const float s1 = WIDE ? -8.f * sq[WIDE ? 2 * n + 1 : n][g] : 0.f;
+                    mma_f16(acc[n], af, qf[n][g][0], s0, s1, s0, s1);
+                  } else {
+                    mma_16816<__half>(acc[n], af, qf[n][g][2 * w + p]);
+                  }
                 }
               }
             }
@@ -544,7 +562,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const float2 s2 = make_float2(sq[n][g], sq[n][g]);
-              const float2 both = make_float2(acc[n][0] + acc[n][1], acc[n][2] + acc[n][3]);
+              const float* c = acc[WIDE ? n >> 1 : n];
+              const float2 both = WIDE ? make_float2(c[n & 1], c[2 + (n & 1)]) : make_float2(c[0] + c[1], c[2] + c[3]);
               dot[n] = g ? ffma2(ks, both, ffma2(km, s2, dot[n])) : ffma2(ks, both, fmul2(km, s2));
             }
           }
@@ -711,7 +730,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
 #pragma unroll
             for (int g = 0; g < NG; ++g) pn[g] += __shfl_xor_sync(0xffffffffu, pn[g], d);
           }
-          const int r = z * RT + n * 4 + t4;
+          const int r = z * RT + row_of(n);
           int t, gi;
           split_row(a, r, t, gi);
           const bool sees = t < nq && base + t >= 0;
@@ -733,15 +752,15 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
                   store4(dst + j, make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]), 1.f, sees);
               }
             } else {
-              float* dst = part + (n * 4 + t4) * (D + 4) + d0;
+              float* dst = part + row_of(n) * (D + 4) + d0;
 #pragma unroll
               for (int j = 0; j < 2 * MT; j += 4)
                 *reinterpret_cast<float4*>(dst + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
             }
           }
           if (!direct && g8 == 0) {
-            part[(n * 4 + t4) * (D + 4) + D] = limit[n] == -INFINITY ? -INFINITY : ref[n];
-            part[(n * 4 + t4) * (D + 4) + D + 1] = ln;
+            part[row_of(n) * (D + 4) + D] = limit[n] == -INFINITY ? -INFINITY : ref[n];
+            part[row_of(n) * (D + 4) + D + 1] = ln;
           }
         }
         fresh = true;
@@ -824,6 +843,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
 // of a segment without tiles.  Thread group i of D RT / 4 threads takes partials i, i + PL, ... in one
 // pass with a running maximum; the groups are joined in order.  256 threads of 32 registers find
 // room beside the worker CTAs, so the search for the segment's CTAs runs before they end.
+
 constexpr int kMergeThreads = 256;
 
 template <typename T, int D, int NT>
@@ -896,8 +916,9 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(T* __restrict_
 }
 
 // ------------------------------------------------------------------ host side
-// Rows of one row tile: 4, 8 or 16 query rows (NT score columns per thread); 8 at most for D = 128,
-// whose output tile is twice as wide.
+// Score columns per thread of a row tile: tiles of 4, 8 or 16 query rows.  D = 128 stops at 8: with 16
+// the output tile alone takes half the registers, and the spills cost more than the second pass over
+// the cache saves (48 ragged requests of up to 5000 tokens, 16 rows: 53.9 us against 45.1).
 int row_tile(int64_t rows, int64_t D) {
   if (rows <= 4) return 1;
   return rows <= 8 || D == 128 ? 2 : 4;
