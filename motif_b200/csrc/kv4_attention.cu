@@ -56,7 +56,7 @@ struct Args {
   float* ws;
   Strides6 st;
   int B, H, Hkv, T, G, Z;   // Z: row tiles of the G T query rows of one (request, kv head)
-  int P, columns;
+  int P, most;              // most: tokens that a row of the table can name
   int64_t pages;
   int ctas;
   float scale, eps;
@@ -71,15 +71,13 @@ struct Tile {
 
 // ------------------------------------------------------------------ the cut into workers
 // Lengths are clamped to what the table can name; a request without query rows has no tiles.
-__device__ __forceinline__ int length_of(const Args& a, int b) {
-  return (int)max((int64_t)0, min((int64_t)a.lens[b], (int64_t)a.columns * a.P));
-}
+__device__ __forceinline__ int length_of(const Args& a, int b) { return max(0, min(a.lens[b], a.most)); }
 __device__ __forceinline__ int queries_of(const Args& a, int b) {
   return a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
 }
 template <int KT>
 __device__ __forceinline__ int tiles_of(const Args& a, int b) {
-  return queries_of(a, b) > 0 ? (length_of(a, b) + KT - 1) / KT : 0;
+  return queries_of(a, b) > 0 ? (int)((uint32_t)(length_of(a, b) + KT - 1) / KT) : 0;
 }
 
 // The requests' tiles, by one warp: lane i counts those of the i-th run of `run` requests.
@@ -101,12 +99,34 @@ template <int KT>
 __device__ __forceinline__ Requests scan_requests(const Args& a) {
   Requests q;
   const int lane = threadIdx.x & 31;
-  q.run = (a.B + 31) / 32;
   q.mine = 0;
-#pragma unroll 4
-  for (int i = 0; i < q.run; ++i) {
-    const int b = lane * q.run + i;
-    if (b < a.B) q.mine += tiles_of<KT>(a, b);
+  if (a.B <= 128) {
+    q.run = (a.B + 31) / 32;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = lane * q.run + i;
+      if (i < q.run && b < a.B) q.mine += tiles_of<KT>(a, b);
+    }
+  } else {
+    // 32 neighbouring requests at a time (a lane reading a run of its own would spread every load over
+    // as many lines): the sum of a group goes to the lane whose run it lies in
+    const int groups = (a.B + 31) / 32, each = (groups + 31) / 32;
+    q.run = 32 * each;
+    for (int i0 = 0; i0 < groups; i0 += 8) {
+      int len[8], nq[8];  // asked for together
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int b = 32 * (i0 + i) + lane;
+        len[i] = b < a.B ? a.lens[b] : 0;
+        nq[i] = a.q_lens && b < a.B ? a.q_lens[b] : a.T;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t t = nq[i] > 0 ? (uint32_t)(max(0, min(len[i], a.most)) + KT - 1) / KT : 0u;
+        const int sum = (int)__reduce_add_sync(0xffffffffu, t);
+        if ((i0 + i) / each == lane) q.mine += sum;
+      }
+    }
   }
   q.upto = warp_scan(q.mine);
   q.total = __shfl_sync(0xffffffffu, q.upto, 31) * a.Z * a.Hkv;
@@ -839,15 +859,15 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
 }
 
 // ------------------------------------------------------------------ merge
-// One CTA per segment: joins the CTAs' partials of a segment that spans several, and zeroes the rows
-// of a segment without tiles.  Thread group i of D RT / 4 threads takes partials i, i + PL, ... in one
-// pass with a running maximum; the groups are joined in order.  256 threads of 32 registers find
-// room beside the worker CTAs, so the search for the segment's CTAs runs before they end.
-
+// Merge CTA c joins the partials of the segment that begins in worker CTA c's run and goes on in the
+// next one's, if there is one, and zeroes the rows of every n-th request without tiles.  Thread group
+// i of D RT / 4 threads takes partials i, i + PL, ... in one pass with a running maximum; the groups
+// are joined in order.  256 threads of 32 registers find room beside the worker CTAs, so the search
+// for the segment runs before they end.
 constexpr int kMergeThreads = 256;
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(T* __restrict__ out, const Args a) {
+__global__ void __launch_bounds__(kMergeThreads, 6) kv4_merge_kernel(T* __restrict__ out, const Args a) {
   constexpr int KT = Tile<D>::kKeys, RT = 4 * NT, NV = RT * D / 4, PL = kMergeThreads / NV;
   static_assert(NV <= kMergeThreads && kMergeThreads % NV == 0, "whole groups of threads");
   __shared__ float s_m[PL][RT], s_l[PL][RT];
@@ -855,28 +875,33 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(T* __restrict_
   allow_dependent_launch();  // a projection that follows may start fetching its weights
   const int tid = threadIdx.x;
   const Requests reqs = scan_requests<KT>(a);
-  const int zh = a.Z * a.Hkv;
-  const int b = blockIdx.x / zh, seg = blockIdx.x - b * zh;
-  // tiles before request b: the runs before its own, then the requests before it in its run
-  const int c = b / reqs.run;
-  int before = __shfl_sync(0xffffffffu, reqs.upto - reqs.mine, c);
-  for (int i = c * reqs.run; i < b; ++i) before += tiles_of<KT>(a, i);
-  const int nt = tiles_of<KT>(a, b), x0 = before * zh + seg * nt;
-  int c0 = 0, n = 0;  // first CTA, partials
-  if (nt > 0) {
-    const Cut cut(reqs.total, a.ctas);
-    c0 = cut.cta_of(x0);
-    n = cut.cta_of(x0 + nt - 1) - c0 + 1;
+  const Cut cut(reqs.total, a.ctas);
+  const int c0 = blockIdx.x;
+  Cursor u = {0, 0, 0, 1};
+  int n = 0;  // partials
+  if (c0 + 1 < cut.working) {
+    const int x = cut.start(c0 + 1);  // the next CTA's first tile
+    u = locate<KT>(a, reqs, x);
+    if (u.k > 0 && x - u.k >= cut.start(c0)) n = cut.cta_of(x - u.k + u.nt - 1) - c0 + 1;
   }
   const int v = tid % NV, pl = tid / NV, rr = v / (D / 4), d = v % (D / 4) * 4;
-  const int nq = queries_of(a, b), base = length_of(a, b) - nq;
+  const int b = u.b, nq = queries_of(a, b), base = length_of(a, b) - nq;
   int z, hk, t, gi;
-  split_segment(a, seg, z, hk);
+  split_segment(a, u.seg, z, hk);
   const int r = z * RT + rr;
   split_row(a, r, t, gi);
+  // the workers write other rows
+  for (int e = blockIdx.x; e < a.B; e += gridDim.x) {
+    if (tiles_of<KT>(a, e) > 0) continue;
+    for (int i = tid; i < a.H * a.T * (D / 4); i += kMergeThreads) {
+      const int row = i / (D / 4), h = row / a.T;
+      store4(out + e * a.st.s[3] + h * a.st.s[4] + (row - h * a.T) * a.st.s[5] + i % (D / 4) * 4,
+             make_float4(0.f, 0.f, 0.f, 0.f), 0.f, false);
+    }
+  }
   // every CTA waits, also those without work: what follows this grid must find the workers' done
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (n == 1) return;  // written by its CTA
+  if (n == 0) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float m = -INFINITY, l = 0.f;
 #pragma unroll 4
@@ -931,15 +956,27 @@ int sm_count() {
   return n;
 }
 
+// Both kernels ask for the same split of an SM's memory, so that merge CTAs may start beside workers.
+int prepare_kernel(const void* fn, int smem) {
+  if (smem && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return check_launch("cudaFuncSetAttribute (dynamic shared memory)");
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) !=
+      cudaSuccess)
+    return check_launch("cudaFuncSetAttribute (carveout)");
+  return MB_OK;
+}
+
 template <typename T, int D, int NT>
 int launch(const void* q, void* out, Args a, cudaStream_t stream) {
   constexpr int smem = attention_smem<D, NT>();
   const void* fn = reinterpret_cast<const void*>(&kv4_attention_kernel<T, D, NT>);
-  if (int rc = ensure_smem_attr(fn, smem)) return rc;
+  if (int rc = once_per_device(fn, prepare_kernel, smem)) return rc;
+  const void* merge = reinterpret_cast<const void*>(&kv4_merge_kernel<T, D, NT>);
+  if (int rc = once_per_device(merge, prepare_kernel, 0)) return rc;
   kv4_attention_kernel<T, D, NT><<<a.ctas, 32 * warps_of(NT, D), smem, stream>>>((const T*)q, (T*)out, a);
   if (int rc = check_launch("kv4_chord_attention")) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.Z * a.Hkv));
+  cfg.gridDim = dim3((unsigned)a.ctas);
   cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
@@ -1008,7 +1045,7 @@ extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, c
     a.ws = (float*)workspace;
     for (int i = 0; i < 6; ++i) a.st.s[i] = strides[i];
     a.B = (int)B, a.H = (int)H, a.Hkv = (int)Hkv, a.T = (int)T, a.G = (int)(H / Hkv);
-    a.P = (int)page_size, a.columns = (int)max_pages, a.pages = num_pages;
+    a.P = (int)page_size, a.most = (int)(max_pages * page_size), a.pages = num_pages;
     a.scale = scale, a.eps = eps;
     if (int rc = check_rows16("kv4_chord_attention", q, strides, sizeof(E))) return rc;
     if (int rc = check_rows16("kv4_chord_attention", out, strides + 3, sizeof(E))) return rc;
