@@ -13,17 +13,25 @@
 // two neighbouring columns of one MMA: with the keys on the M side a tile of 4 query rows fills
 // N = 8, a thread's two accumulator columns are the two parts of ONE query row, and their sum is the
 // product to 22 bits at no further instruction.  The score tile [keys x (row, part)] is the transpose
-// of what the second product wants: one movmatrix per 8 keys.
+// of what the second product wants: one movmatrix per 8 keys.  mma.sync and not tcgen05: a kv head has
+// 4 to 16 query rows, the operand that comes from memory must be unpacked in registers, and the tensor
+// pipe is busy for a fifth of the time as it is.
 //
 // Work is cut by tiles of 64 keys (32 for D = 128), not by requests: the tiles of all (request, row
-// tile, kv head) segments in order are dealt out in equal runs to the CTAs and within them to the
-// warps, so requests of any lengths load the GPU evenly, and the lengths may change on the device
-// between replays of a CUDA graph.  A segment inside one warp's run is written out by it; one that
-// spans warps is joined in shared memory, one that spans CTAs leaves a partial (o, m, l) per CTA,
-// which the merge kernel joins in CTA order.
+// tile, kv head) segments in order are dealt out in equal runs to the CTAs (one per SM) and within
+// them to the warps, so requests of any lengths load the GPU evenly, and the lengths may change on the
+// device between replays of a CUDA graph.  A segment inside one warp's run is written out by it; one
+// that spans warps is joined in shared memory, one that spans CTAs leaves a partial (o, m, l) per CTA,
+// which the merge kernel joins in CTA order.  Each warp owns a ring of two tiles in shared memory that
+// its first lanes fill with bulk copies (one per tile where a tile lies in one page).
 //
-// Each warp owns a ring of tiles in shared memory that its first lanes fill with bulk copies (one per
-// tile where a tile lies in one page).
+// What bounds it: the instructions that unpack and weigh, not the memory.  A unit of 16 keys takes 150
+// instructions of a warp, 70 of them on the half-rate integer pipe (44 isolate the codes), which is
+// busy for two thirds of the main loop.  64 requests of 8192 tokens (12 / 3 heads of 64, 113 MB):
+// 32.6 us on the GPU, 3.5 TB/s, where the bytes alone would take 17.4; of it 4 us pass before the
+// first tile has arrived (lengths, page table, copy: three dependent loads) and 3 in joining.  12 warps
+// of 144 registers measured best there: 8 warps 37.3 us, 16 warps 33.4 (and 13.2 against 10.8 for 8
+// requests), three stages 33.4 and 128-key tiles on 8 warps 34.2.
 #include <math.h>
 
 #include "common.cuh"
@@ -277,7 +285,8 @@ __device__ __forceinline__ void store4(T* p, float4 y, float f, bool sees) {
 __device__ __forceinline__ int key_of_row(int r) { return (r >> 1) + 4 * (r & 1); }
 
 // ------------------------------------------------------------------ the worker kernel
-// Warps of the one CTA an SM runs, by the registers that the output tile takes.
+// Warps of the one CTA an SM runs, by the registers that the output tile takes (more warps spill: 8 query
+// rows of D = 128 on 12 warps 51.0 us against 44.1, 16 rows of D = 64 on 12 warps 109 against 73).
 __host__ __device__ constexpr int warps_of(int nt, int D) { return nt == 1 || (nt == 2 && D <= 64) ? 12 : 8; }
 
 // An unfinished piece of a segment at the end of a warp's run: [RT rows][D + 4] floats (o, m, l), its
@@ -306,8 +315,8 @@ __device__ __forceinline__ int run_start(int count, int w) {
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(const T* __restrict__ q, T* __restrict__ out,
-                                                                       const Args a) {
+__global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
+    kv4_attention_kernel(const T* __restrict__ q, T* __restrict__ out, const Args a) {
   constexpr int kWarps = warps_of(NT, D);
   using L = Layout<D>;
   constexpr int TU = Tile<D>::kUnits, KT = Tile<D>::kKeys;
@@ -599,7 +608,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
               const float2 ln = fmul2(make_float2(lg2_(dist.x), lg2_(dist.y)), make_float2(be[n], be[n]));
               pw = make_float2(ex2f_(ln.x), ex2f_(ln.y));
             }
-            x[n][u] = ffma2(dot[n], make_float2(qr[n], qr[n]), ffma2(pw, make_float2(ar[n], ar[n]), make_float2(-ref[n], -ref[n])));
+            x[n][u] = ffma2(dot[n], make_float2(qr[n], qr[n]),
+                            ffma2(pw, make_float2(ar[n], ar[n]), make_float2(-ref[n], -ref[n])));
           }
         }
         if (units != (1u << TU) - 1 || k0 + KT - 1 > lo_pos) {
@@ -862,7 +872,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1) kv4_attention_kernel(
 // Merge CTA c joins the partials of the segment that begins in worker CTA c's run and goes on in the
 // next one's, if there is one, and zeroes the rows of every n-th request without tiles.  Thread group
 // i of D RT / 4 threads takes partials i, i + PL, ... in one pass with a running maximum; the groups
-// are joined in order.  256 threads of 32 registers find room beside the worker CTAs, so the search
+// are joined in order.  256 threads of 40 registers find room beside the worker CTAs, so the search
 // for the segment runs before they end.
 constexpr int kMergeThreads = 256;
 
