@@ -74,7 +74,7 @@ def _build_host(force: bool) -> None:
     cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', *[f'-I{p}' for p in include], HOST_SRC,
            '-o', tmp, f'-L{HERE}', '-l:libmotif_b200.so', '-Wl,-rpath,$ORIGIN', f'-L{os.path.join(root, "lib")}',
-           '-ltorch_python', '-ltorch', '-ltorch_cpu', '-lc10', '-lc10_cuda']
+           '-ltorch_python', '-ltorch', '-ltorch_cpu', '-ltorch_cuda', '-lc10', '-lc10_cuda']
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f'{cmd[0]} failed on {HOST_SRC}:\n{r.stderr}')

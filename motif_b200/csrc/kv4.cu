@@ -29,14 +29,15 @@ PageDiv page_div(int64_t P) {
 // asked for up to and including it do not exceed the free count; the i-th fresh page is the i-th
 // from the top of the free list.
 //
-// One cluster of CTAs, a block of THREADS requests at a time: every CTA scans the block's tokens and
-// pages by itself, then (after a cluster barrier, since lens_out may be lens) the cluster's threads
-// share the writing.  A new token's page is an old table entry or comes straight from the free list,
+// A block of THREADS requests at a time: every CTA scans the block's tokens and pages by itself, then
+// the threads of all CTAs share the writing.  Where lens_out is lens (or the free counts are one) the
+// CTAs are a cluster, whose barrier keeps the writes behind everybody's reads.  A new token's page is an old table entry or comes straight from the free list,
 // so nobody waits for the fresh entries to be written.  Bound by latency (the bytes take 0.1 us): one
-// scan and two dependent loads.  3.6 us for one token of each of 64 requests (one CTA of four warps),
-// 7.5 for 32 prompts of 4096 tokens, 9.1 for 517 ragged chunks; on one CTA the latter two took 43.9
-// and 35.2.
-constexpr int kReserveCtas = 8;
+// scan and two dependent loads.  3.4 us for one token of each of 64 requests (one CTA of four warps),
+// 4.6 for 32 prompts of 4096 tokens, 5.7 for 517 ragged chunks (7.1 and 8.7 on a cluster of 8); on one
+// CTA the latter two took 43.9 and 35.2.
+constexpr int kClusterCtas = 8;  // the most a cluster holds everywhere
+constexpr int kReserveCtas = 64;
 
 __device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -69,14 +70,14 @@ template <int THREADS>
 __global__ void __launch_bounds__(THREADS) paged_reserve_kernel(
     const int32_t* lens, const int32_t* __restrict__ new_lens, int32_t* table, int64_t ts,
     const int32_t* __restrict__ free_pages, const int32_t* free_count, int32_t* lens_out, int32_t* free_out,
-    int32_t* __restrict__ slots, bool vector, int total, int B, int columns, int cap, PageDiv by) {
+    int32_t* __restrict__ slots, bool vector, bool in_place, int total, int B, int columns, int cap, PageDiv by) {
   // of each request of the block: end of its tokens and of its fresh pages, both counted over all
   __shared__ int s_end[THREADS], s_pages[THREADS];
   __shared__ int s_len[THREADS], s_new[THREADS];  // new: -1 - new where it is not served
   __shared__ int part[2][32];
   __shared__ int s_taken;
   const int tid = threadIdx.x, lane = tid & 31, P = by.P;
-  const int ranks = gridDim.x, rank = blockIdx.x;  // one cluster
+  const int ranks = gridDim.x, rank = blockIdx.x;
   const int me = rank * THREADS + tid, all_threads = ranks * THREADS;
   auto pages = [&](int n) { return by(n) + (by(n) * P < n ? 1 : 0); };
   const int avail = min(max(*free_count, 0), cap);
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(THREADS) paged_reserve_kernel(
     // those that were served and took pages come first: the last of them says how many were taken
     const int taken = __reduce_max_sync(0xffffffffu, ok && need ? upto : 0);
     if (lane == 0 && taken) atomicMax(&s_taken, taken);
-    if (ranks > 1) asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+    if (in_place && ranks > 1) asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
     else __syncthreads();
     if (rank == 0 && b < B) lens_out[b] = ok ? full : len;
     // the first request of the block whose running sum (tokens or pages) passes x
@@ -452,7 +453,9 @@ extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_
              "paged_reserve: free list of %lld pages", (long long)free_capacity);
   const PageDiv by = page_div(page_size);
   const bool vector = reinterpret_cast<uintptr_t>(slots) % 16 == 0;
-  auto go = [&](auto kernel, int threads, int ctas) {
+  const bool in_place = lens_out == lens || free_count_out == free_count;
+  auto go = [&](auto kernel, int threads, bool many) {
+    const int ctas = !many ? 1 : in_place ? kClusterCtas : kReserveCtas;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(threads);
@@ -462,15 +465,18 @@ extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_
     at[0].val.clusterDim.x = ctas;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = in_place && ctas > 1 ? 1 : 0;
     cudaLaunchKernelEx(&cfg, kernel, lens, new_lens, block_table, table_stride, free_pages, free_count, lens_out,
-                       free_count_out, slots, vector, (int)total_new, (int)B, (int)max_pages, (int)free_capacity, by);
+                       free_count_out, slots, vector, in_place, (int)total_new, (int)B, (int)max_pages,
+                       (int)free_capacity, by);
   };
-  // a decode step's worth of requests and tokens: four warps scan faster than 16; many tokens: the
-  // cluster shares the writing
-  if (B <= 128 && total_new <= 1024) go(paged_reserve_kernel<128>, 128, 1);
-  else if (B <= 512) go(paged_reserve_kernel<512>, 512, total_new <= 4096 ? 1 : kReserveCtas);
-  else go(paged_reserve_kernel<1024>, 1024, total_new <= 4096 ? 1 : kReserveCtas);
+  // a decode step's worth of requests and tokens: four warps scan faster than 16; many tokens: many
+  // CTAs share the writing, from where their cost (nothing, or a cluster's barrier) is made up for:
+  // 16384 tokens take 3.8 us on 64 CTAs, 4.4 on a cluster of 8, 4096 tokens 4.7 on one
+  const bool many = total_new > (in_place ? 4096 : 1024);
+  if (B <= 128 && total_new <= 1024) go(paged_reserve_kernel<128>, 128, false);
+  else if (B <= 512) go(paged_reserve_kernel<512>, 512, many);
+  else go(paged_reserve_kernel<1024>, 1024, many);
   return check_launch("paged_reserve");
 }
 

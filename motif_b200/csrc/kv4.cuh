@@ -13,6 +13,7 @@
 // and every unit starts on a 128-byte boundary.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -57,6 +58,17 @@ int dispatch(int dtype, int64_t D, F&& f) {
     case MB_BF16: return dispatch_dim(D, [&](auto d) { return f(__nv_bfloat16(), d); });
   }
   return set_error(MB_ERR_DTYPE, "kv4: unsupported dtype %d", dtype);
+}
+
+// SMs of the current device (0: the query failed).
+inline int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 inline int check_paging(const char* who, int64_t B, int64_t columns, int64_t ts, int64_t P) {

@@ -959,13 +959,6 @@ int row_tile(int64_t rows, int64_t D) {
   return rows <= 8 || D == 128 ? 2 : 4;
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return n;
-}
-
 // Both kernels ask for the same split of an SM's memory, so that merge CTAs may start beside workers.
 int prepare_kernel(const void* fn, int smem) {
   if (smem && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
@@ -1061,7 +1054,7 @@ extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, c
     if (int rc = check_rows16("kv4_chord_attention", out, strides + 3, sizeof(E))) return rc;
     const int nt = row_tile((int64_t)a.G * T, D);
     a.Z = (int)(((int64_t)a.G * T + 4 * nt - 1) / (4 * nt));
-    a.ctas = sm_count();
+    a.ctas = kv4::sm_count();
     const int64_t tiles = (max_pages * page_size + Tile<DD>::kKeys - 1) / Tile<DD>::kKeys;
     MB_REQUIRE((int64_t)a.B * a.Z * a.Hkv * tiles < (1ll << 31), MB_ERR_SHAPE,
                "kv4_chord_attention: B * Hkv * row tiles * key tiles = %lld (fewer than 2^31)",

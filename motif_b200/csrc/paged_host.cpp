@@ -5,6 +5,7 @@
 // themselves are 2 to 5.
 #include <Python.h>
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -129,13 +130,19 @@ void no_grad(const at::Tensor& t) {
     throw Refusal{PyExc_NotImplementedError, "the 4-bit cache is forward-only (no autograd)"};
 }
 
+// A contiguous output.  Straight from the allocator: the dispatcher would take as long again, and there
+// is nothing for it to do for a tensor without a gradient on a known device.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
+  return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
+}
+
 // ------------------------------------------------------------------ the calls
 PyObject* reserve(PyObject* const* a) {
   const at::Tensor& lens = lengths(a[0]);
   const c10::Device dev = lens.device();
   const int64_t B = lens.size(0);
   vector("lens", a[0], B, dev);
-  const at::Tensor& fresh = vector("new_lens", a[1], B, dev);
+  const at::Tensor& added = vector("new_lens", a[1], B, dev);
   const at::Tensor& tab = table(a[2], dev, B);
   const at::Tensor& free = on("free_pages", a[3], dev);
   vector("free_pages", a[3], free.numel(), dev);
@@ -143,11 +150,11 @@ PyObject* reserve(PyObject* const* a) {
   const int64_t page_size = whole(a[5]), total = whole(a[6]);
   if (total < 0) refuse("total_new must not be negative, got " + std::to_string(total));
   const c10::cuda::CUDAGuard guard(dev);
-  const at::Tensor lens_out = a[7] == Py_None ? at::empty({B}, lens.options()) : vector("lens_out", a[7], B, dev);
-  const at::Tensor count_out = a[8] == Py_None ? at::empty({1}, lens.options()) : vector("free_count_out", a[8], 1, dev);
-  const at::Tensor slots = a[9] == Py_None ? at::empty({total}, lens.options()) : vector("slots", a[9], total, dev);
+  const at::Tensor lens_out = a[7] == Py_None ? fresh({B}, at::kInt, dev) : vector("lens_out", a[7], B, dev);
+  const at::Tensor count_out = a[8] == Py_None ? fresh({1}, at::kInt, dev) : vector("free_count_out", a[8], 1, dev);
+  const at::Tensor slots = a[9] == Py_None ? fresh({total}, at::kInt, dev) : vector("slots", a[9], total, dev);
   check("motif_b200_paged_reserve",
-        motif_b200_paged_reserve(lens.data_ptr<int>(), fresh.data_ptr<int>(), tab.data_ptr<int>(), tab.stride(0),
+        motif_b200_paged_reserve(lens.data_ptr<int>(), added.data_ptr<int>(), tab.data_ptr<int>(), tab.stride(0),
                                  free.data_ptr<int>(), count.data_ptr<int>(), lens_out.data_ptr<int>(),
                                  count_out.data_ptr<int>(), slots.data_ptr<int>(), total, B, tab.size(1), free.numel(),
                                  page_size, stream_of(dev)));
@@ -194,8 +201,8 @@ PyObject* append(PyObject* const* a) {
   const at::Tensor k = rows16(k0), v = rows16(v0);
   at::Tensor ko, vo;
   if (values) {
-    ko = at::empty(k.sizes(), k.options());
-    vo = at::empty(k.sizes(), k.options());
+    ko = fresh(k.sizes(), k.scalar_type(), dev);
+    vo = fresh(k.sizes(), k.scalar_type(), dev);
   }
   int64_t strides[12] = {0};
   const at::Tensor* ts[4] = {&k, &v, &ko, &vo};
@@ -224,8 +231,7 @@ PyObject* gather(PyObject* const* a) {
   const at::ScalarType type = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
   const int dc = dtype_code(type);
   const c10::cuda::CUDAGuard guard(dev);
-  const auto options = p.t.options().dtype(type);
-  const at::Tensor k = at::empty({B, p.kv, S, p.dim}, options), v = at::empty({B, p.kv, S, p.dim}, options);
+  const at::Tensor k = fresh({B, p.kv, S, p.dim}, type, dev), v = fresh({B, p.kv, S, p.dim}, type, dev);
   check("motif_b200_kv4_gather",
         motif_b200_kv4_gather(p.t.data_ptr(), tab.data_ptr<int>(), tab.stride(0), lens.data_ptr<int>(), k.data_ptr(),
                               v.data_ptr(), B, p.kv, S, p.dim, p.pages, p.page_size, tab.size(1), dc, stream_of(dev)));
@@ -251,7 +257,7 @@ PyObject* attention(PyObject* const* a) {
   const int* q_lens = a[8] == Py_None ? nullptr : vector("q_lens", a[8], B, dev).data_ptr<int>();
   const double scale = a[9] == Py_None ? 1.0 / std::sqrt((double)p.dim) : number(a[9]), eps = number(a[10]);
   const c10::cuda::CUDAGuard guard(dev);
-  const at::Tensor q = rows16(q0), out = at::empty(q.sizes(), q.options());
+  const at::Tensor q = rows16(q0), out = fresh(q.sizes(), q.scalar_type(), dev);
   const int64_t bytes = motif_b200_kv4_attention_workspace_bytes(H, p.kv, T, p.dim);
   const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes);
   const int64_t strides[6] = {q.stride(0), q.stride(1), q.stride(2), out.stride(0), out.stride(1), out.stride(2)};
