@@ -227,6 +227,18 @@ __device__ __forceinline__ float lg2_(float x) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 .. 127
 
+// x^b of a positive x for fp32 tensors: log2 x as a whole number e and log2 f of f = x 2^-e in 0.75 ..
+// 1.5, b e with its rounding error kept, and 2^(b log2 x) from the fraction of b e, so that the fast
+// logarithm's and power's errors (2^-22 absolute and relative) are all there is, however large log2 x.
+__device__ __forceinline__ float power(float x, float b) {
+  const int e = (int)(__float_as_uint(x) - 0x3f400000u) >> 23;
+  const float f = __uint_as_float(__float_as_uint(x) - ((uint32_t)e << 23)), fe = (float)e;
+  const float t = b * fe, lost = fmaf(b, fe, -t);
+  const float n = rintf(t);
+  const float y = ex2f_((t - n) + fmaf(b, lg2_(f), lost));
+  return y * pow2((int)fminf(fmaxf(n, -126.f), 127.f));
+}
+
 // D = A B + C on fp16 operands with C in registers of its own.
 __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, const uint32_t* b, float c0, float c1, float c2,
                                         float c3) {
@@ -458,7 +470,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
           qr[n] = a.ssmax[h];
           ar[n] = a.alpha[h];
           be[n] = a.beta[h];
-          mh[n] = -a.mu[h];
+          mh[n] = be[n] == 0.f ? 0.5f : -a.mu[h];  // x^0 is 1 for x = 0 too (no eps): any other place will do
         }
         if (i == 0) {
           // the first copies go out after the loads above, which would wait behind every warp's copies
@@ -603,7 +615,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
             const float2 dist = make_float2(fabsf(off.x) + a.eps, fabsf(off.y) + a.eps);
             float2 pw;
             if constexpr (sizeof(T) == 4) {
-              pw = make_float2(powf(dist.x, be[n]), powf(dist.y, be[n]));
+              pw = make_float2(power(dist.x, be[n]), power(dist.y, be[n]));
             } else {
               const float2 ln = fmul2(make_float2(lg2_(dist.x), lg2_(dist.y)), make_float2(be[n], be[n]));
               pw = make_float2(ex2f_(ln.x), ex2f_(ln.y));

@@ -473,6 +473,22 @@ def test_attention_of_large_and_tiny_values():
           torch.float32)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_attention_decay_at_its_edges(dtype):
+    """No decay (beta = 0: x^0 is 1 at x = 0 too), eps = 0 at a key that lies at mu, a steep decay whose
+    far keys weigh nothing, and a negative exponent."""
+    H, kv, D, P = 8, 2, 32, 16
+    pool, table, ln = random_cache([300, 40, 1], kv, D, P, 13)
+    q = torch.randn(3, H, 1, D, device='cuda', generator=gen(7)).to(dtype)
+    alpha = torch.tensor([1.0, 0.5, 1.0, 2.0, 0.3, 40.0, 0.5, 0.0], device='cuda')
+    beta = torch.tensor([0.0, 0.7, 1.0, 0.0, 2.5, 3.0, -0.5, 1.0], device='cuda')
+    mu = torch.tensor([0.0, -3.0, 0.0, -5.0, -1.0, 0.0, 0.5, 0.0], device='cuda')
+    ssmax = torch.full((H,), 0.7, device='cuda')
+    for eps in (0.0, 1e-5):
+        out = ops.kv4_chord_attention(q, pool, table, ln, alpha, beta, mu, ssmax, eps=eps)
+        close(out, attention_64(q, pool, table, ln, alpha, beta, mu, ssmax, eps=eps), dtype)
+
+
 def test_offsets_past_32_bits():
     """Pages whose bytes lie past 4 GiB."""
     kv, D, P = 4, 128, 128
