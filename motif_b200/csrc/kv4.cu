@@ -76,6 +76,8 @@ __global__ void __launch_bounds__(THREADS) paged_reserve_kernel(
   __shared__ int s_len[THREADS], s_new[THREADS];  // new: -1 - new where it is not served
   __shared__ int part[2][32];
   __shared__ int s_taken;
+  allow_dependent_launch();
+  kv4::wait_for_previous();
   const int tid = threadIdx.x, lane = tid & 31, P = by.P;
   const int ranks = gridDim.x, rank = blockIdx.x;
   const int me = rank * THREADS + tid, all_threads = ranks * THREADS;
@@ -171,6 +173,8 @@ __global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
     int32_t* __restrict__ free_pages, int32_t* __restrict__ free_count, int B, int columns, int64_t cap, int P) {
   __shared__ int part[32];
   __shared__ int s_at[kReleaseThreads], s_held[kReleaseThreads];
+  allow_dependent_launch();
+  kv4::wait_for_previous();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int top = max(*free_count, 0);
   for (int b0 = 0; b0 < B; b0 += kReleaseThreads) {
@@ -352,6 +356,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k
   const bool live = at < N;  // whole groups of lanes: W divides the warp
   const int n = live ? (int)at : 0;
   const int b = T_ == N ? 0 : n / T_, t = n - b * T_;
+  allow_dependent_launch();
+  kv4::wait_for_previous();
   const int slot = live ? slots[n] : -1;
   float x[2][8], y[2][8], hi, lo;
   uint4 raw[2];
@@ -411,6 +417,8 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const uint8_t* __restri
   constexpr int W = D / 8;
   const int b = blockIdx.x / blocks, h = blockIdx.y, w = threadIdx.x % W;
   const int64_t token = (int64_t)(blockIdx.x - b * blocks) * (256 / W) + threadIdx.x / W;
+  allow_dependent_launch();
+  kv4::wait_for_previous();
   if (token >= S) return;
   const int j = (int)token;
   float kx[8], vx[8];
@@ -460,12 +468,14 @@ extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(threads);
     cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ctas;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = ctas;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = in_place && ctas > 1 ? 1 : 0;
+    cfg.numAttrs = in_place && ctas > 1 ? 2 : 1;
     cudaLaunchKernelEx(&cfg, kernel, lens, new_lens, block_table, table_stride, free_pages, free_count, lens_out,
                        free_count_out, slots, vector, in_place, (int)total_new, (int)B, (int)max_pages,
                        (int)free_capacity, by);
@@ -487,10 +497,8 @@ extern "C" int motif_b200_paged_release(const uint8_t* done, int32_t* lens, int3
   if (int rc = check_paging("paged_release", B, max_pages, table_stride, page_size)) return rc;
   MB_REQUIRE(free_capacity >= 1 && free_capacity * page_size < (1ll << 31), MB_ERR_SHAPE,
              "paged_release: free list of %lld pages", (long long)free_capacity);
-  paged_release_kernel<<<1, kReleaseThreads, 0, (cudaStream_t)stream>>>(done, lens, block_table, table_stride,
-                                                                         free_pages, free_count, (int)B,
-                                                                         (int)max_pages, free_capacity,
-                                                                         (int)page_size);
+  launch(paged_release_kernel, dim3(1), kReleaseThreads, 0, stream, done, lens, block_table, table_stride, free_pages,
+         free_count, (int)B, (int)max_pages, free_capacity, (int)page_size);
   return check_launch("paged_release");
 }
 
@@ -518,10 +526,9 @@ extern "C" int motif_b200_kv4_append(const void* k, const void* v, const int32_t
       using I = decltype(width);
       Strides12<I> st;
       for (int i = 0; i < 12; ++i) st.s[i] = (I)strides[i];
-      kv4_append_kernel<E, DD, I><<<dim3((unsigned)((B * T + per_cta - 1) / per_cta), (unsigned)Hkv), 256, 0,
-                                    (cudaStream_t)stream>>>((const E*)k, (const E*)v, slots, (uint8_t*)pool, (E*)k_out,
-                                                            (E*)v_out, st, (int)(B * T), (int)T, (int)Hkv,
-                                                            (int)(num_pages * page_size), page_div(page_size));
+      launch(kv4_append_kernel<E, DD, I>, dim3((unsigned)((B * T + per_cta - 1) / per_cta), (unsigned)Hkv), 256, 0, stream,
+             (const E*)k, (const E*)v, slots, (uint8_t*)pool, (E*)k_out, (E*)v_out, st, (int)(B * T), (int)T, (int)Hkv,
+             (int)(num_pages * page_size), page_div(page_size));
     };
     bool fits = true;
     for (int i = 0; i < 12; ++i) fits = fits && strides[i] >= 0 && strides[i] < (1ll << 31);
@@ -548,7 +555,7 @@ extern "C" int motif_b200_kv4_gather(const void* pool, const int32_t* block_tabl
     if (int rc = check_rows16("kv4_gather", v_out, none, 1)) return rc;
     const int64_t blocks = (S + 256 / (DD / 8) - 1) / (256 / (DD / 8));
     MB_REQUIRE(B * blocks < (1ll << 31), MB_ERR_SHAPE, "kv4_gather: %lld rows", (long long)(B * Hkv * S));
-    kv4_gather_kernel<E, DD><<<dim3((unsigned)(B * blocks), (unsigned)Hkv), 256, 0, (cudaStream_t)stream>>>(
+    launch(kv4_gather_kernel<E, DD>, dim3((unsigned)(B * blocks), (unsigned)Hkv), 256, 0, stream,
         (const uint8_t*)pool, block_table, table_stride, lens, (E*)k_out, (E*)v_out, (int)blocks, (int)Hkv, (int)S,
         (int)num_pages, (int)max_pages, page_div(page_size));
     return check_launch("kv4_gather");

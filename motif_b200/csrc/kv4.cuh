@@ -15,6 +15,7 @@
 
 #include <atomic>
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 
@@ -37,6 +38,9 @@ struct Layout {
 
 __host__ __device__ constexpr int64_t unit_bytes(int64_t D) { return kUnit * D + 8 * kUnit * (D < 64 ? 1 : D / 64); }
 
+// Everything before this kernel in the stream has ended and its writes are there.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float pair_scale(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float pair_centre(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
@@ -58,6 +62,23 @@ int dispatch(int dtype, int64_t D, F&& f) {
     case MB_BF16: return dispatch_dim(D, [&](auto d) { return f(__nv_bfloat16(), d); });
   }
   return set_error(MB_ERR_DTYPE, "kv4: unsupported dtype %d", dtype);
+}
+
+// Launch that may begin while the kernel before it in the stream ends: every kernel launched so starts
+// with wait_for_previous(), before it touches memory, and lets the next one begin early in turn.
+template <typename... P, typename... A>
+void launch(void (*kernel)(P...), dim3 grid, int threads, int smem, void* stream, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
 }
 
 // SMs of the current device (0: the query failed).

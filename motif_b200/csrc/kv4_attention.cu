@@ -360,7 +360,10 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
     mbar_init_fence();
     pieces[warp][0].b = pieces[warp][1].b = -1;
   }
-  allow_dependent_launch();  // the merge may take its place; it waits for this grid to end
+  kv4::wait_for_previous();
+  // only now may the merge take its place: it reads the lengths before it waits for this grid to end,
+  // and what came before this grid may have written them
+  allow_dependent_launch();
   const Requests reqs = scan_requests<KT>(a);
   const Cut cut(reqs.total, gridDim.x);
   if ((int)blockIdx.x >= cut.working) return;
@@ -922,7 +925,7 @@ __global__ void __launch_bounds__(kMergeThreads, 6) kv4_merge_kernel(T* __restri
     }
   }
   // every CTA waits, also those without work: what follows this grid must find the workers' done
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  kv4::wait_for_previous();
   if (n == 0) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float m = -INFINITY, l = 0.f;
@@ -988,18 +991,10 @@ int launch(const void* q, void* out, Args a, cudaStream_t stream) {
   if (int rc = once_per_device(fn, prepare_kernel, smem)) return rc;
   const void* merge = reinterpret_cast<const void*>(&kv4_merge_kernel<T, D, NT>);
   if (int rc = once_per_device(merge, prepare_kernel, 0)) return rc;
-  kv4_attention_kernel<T, D, NT><<<a.ctas, 32 * warps_of(NT, D), smem, stream>>>((const T*)q, (T*)out, a);
+  kv4::launch(kv4_attention_kernel<T, D, NT>, dim3(a.ctas), 32 * warps_of(NT, D), smem, stream, (const T*)q, (T*)out,
+              (const Args)a);
   if (int rc = check_launch("kv4_chord_attention")) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.ctas);
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kv4_merge_kernel<T, D, NT>, (T*)out, (const Args)a);
+  kv4::launch(kv4_merge_kernel<T, D, NT>, dim3(a.ctas), kMergeThreads, 0, stream, (T*)out, (const Args)a);
   return check_launch("kv4_chord_attention (merge)");
 }
 

@@ -600,3 +600,68 @@ def test_refusals_on_device_tensors():
     bad('done must be', ops.paged_release, ln, ln, table, free, one, 16)
     with torch.no_grad():
         ops.kv4_append(x.clone().requires_grad_(), x, torch.full_like(slots, -1), pool)
+
+
+def test_a_chain_of_calls_sees_what_was_just_written():
+    """Every call of a step starts while the one before it ends: lengths, slots, pool and queries are all
+    written by the kernels right before.  The chain without waits equals the one with a wait after
+    every call."""
+    B, H, kv, D, P = 40, 12, 3, 64, 16
+    g = gen(40)
+    base = torch.randint(0, 400, (B,), generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda()
+    pr = params(H, 8)
+    ks, vs = (torch.randn(8, B * 16, kv, D, device='cuda', generator=g).bfloat16() for _ in range(2))
+    qs = torch.randn(8, B, H, 1, D, device='cuda', generator=g).bfloat16()
+
+    def chain(wait):
+        pause = torch.cuda.synchronize if wait else (lambda: None)
+        pool = ops.kv4_pool(2200, kv, D, P)
+        table = torch.full((B, 64), -1, dtype=torch.int32, device='cuda')
+        free = torch.arange(2200, dtype=torch.int32, device='cuda')
+        count = torch.full((1,), 2200, dtype=torch.int32, device='cuda')
+        lens = torch.zeros(B, dtype=torch.int32, device='cuda')
+        new = torch.empty_like(lens)
+        outs = []
+        pause()
+        for i in range(8):
+            new.copy_((base * (i + 3)) % 16 + (0 if i else 1))
+            pause()
+            slots, lens, count = ops.paged_reserve(lens, new, table, free, count, P, B * 16)
+            pause()
+            ops.kv4_append(ks[i], vs[i], slots, pool)
+            pause()
+            q = qs[i] * 1.0
+            pause()
+            outs.append(ops.kv4_chord_attention(q, pool, table, lens, *pr))
+            pause()
+            outs += list(ops.kv4_gather(pool, table, lens, 130))
+            pause()
+            done = lens > 100
+            pause()
+            ops.paged_release(done, lens, table, free, count, P)
+            pause()
+        return outs + [lens, count, table]
+
+    want = chain(True)
+    for _ in range(5):
+        got = chain(False)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_streams_at_once():
+    """Calls on two streams share nothing but what they read."""
+    H, kv, D, P = 8, 2, 64, 32
+    pool, table, ln = random_cache([3000, 17, 900], kv, D, P, 41)
+    pr = params(H, 9)
+    qs = [torch.randn(3, H, 2, D, device='cuda', generator=gen(50 + i)).half() for i in range(2)]
+    want = [ops.kv4_chord_attention(q, pool, table, ln, *pr) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(20):
+        got = []
+        for s, q in zip(streams, qs):
+            with torch.cuda.stream(s):
+                got.append(ops.kv4_chord_attention(q, pool, table, ln, *pr))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
