@@ -33,8 +33,8 @@ PageDiv page_div(int64_t P) {
 // the threads of all CTAs share the writing.  Where lens_out is lens (or the free counts are one) the
 // CTAs are a cluster, whose barrier keeps the writes behind everybody's reads.  A new token's page is an old table entry or comes straight from the free list,
 // so nobody waits for the fresh entries to be written.  Bound by latency (the bytes take 0.1 us): one
-// scan and two dependent loads.  3.4 us for one token of each of 64 requests (one CTA of four warps),
-// 4.6 for 32 prompts of 4096 tokens, 5.7 for 517 ragged chunks (7.1 and 8.7 on a cluster of 8); on one
+// scan and two dependent loads.  3.3 us for one token of each of 64 requests (one CTA of four warps),
+// 4.4 for 32 prompts of 4096 tokens, 5.6 for 517 ragged chunks (7.1 and 8.7 on a cluster of 8); on one
 // CTA the latter two took 43.9 and 35.2.
 constexpr int kClusterCtas = 8;  // the most a cluster holds everywhere
 constexpr int kReserveCtas = 64;
@@ -338,10 +338,10 @@ __device__ __forceinline__ void quantise8(const float* x, float hi, float lo, fl
 
 // A thread takes the same eight dims of K and V of one token and head: D / 8 neighbouring lanes make a
 // row, the rows of a warp are neighbouring tokens of one head (blockIdx.y), whose codes and pairs lie
-// next to each other.  131072 tokens of 3 bf16 heads of 64 with the stored values given back: 51.0 us,
+// next to each other.  131072 tokens of 3 bf16 heads of 64 with the stored values given back: 50.7 us,
 // 4.5 TB/s, bound by the instructions of the quantisation (362 a warp for 16 values a lane, two thirds
 // of the issue slots; the bytes take 35.2); IEEE divisions took 128.6.  5003 tokens of 8 fp32 heads of
-// 128: 12.2 us, at the copy rate.  CTAs that stay and fetch their next rows early measured slower (60.5:
+// 128: 11.6 us, at the copy rate.  CTAs that stay and fetch their next rows early measured slower (60.5:
 // the registers cost more warps than the early loads hide).
 template <typename T, int D, typename I>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
@@ -405,7 +405,7 @@ __device__ __forceinline__ void values8(uint32_t word, uint32_t pair, float* x) 
 // A thread reads one word of codes of K and of V and writes eight values of each; D / 8 neighbouring
 // lanes make a row, a warp neighbouring tokens of one head.  Tokens at or past the request's length,
 // and those of pages outside the pool, become zeros.  32 prefixes of up to 4096 tokens, 3 bf16 heads
-// of 64 (115 MB, most of it written): 21.3 us, where the bytes take 17.6; 64-bit indexes and
+// of 64 (115 MB, most of it written): 20.4 us, where the bytes take 17.6; 64-bit indexes and
 // conversions from integers took 26.6.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(const uint8_t* __restrict__ pool,

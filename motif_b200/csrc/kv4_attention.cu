@@ -17,7 +17,7 @@
 // 4 to 16 query rows, the operand that comes from memory must be unpacked in registers, and the tensor
 // pipe is busy for a fifth of the time as it is.
 //
-// Work is cut by tiles of 64 keys (32 for D = 128), not by requests: the tiles of all (request, row
+// Work is cut by tiles of 64 keys (128 for D = 32), not by requests: the tiles of all (request, row
 // tile, kv head) segments in order are dealt out in equal runs to the CTAs (one per SM) and within
 // them to the warps, so requests of any lengths load the GPU evenly, and the lengths may change on the
 // device between replays of a CUDA graph.  A segment inside one warp's run is written out by it; one
@@ -28,10 +28,11 @@
 // What bounds it: the instructions that unpack and weigh, not the memory.  A unit of 16 keys takes 150
 // instructions of a warp, 70 of them on the half-rate integer pipe (44 isolate the codes), which is
 // busy for two thirds of the main loop.  64 requests of 8192 tokens (12 / 3 heads of 64, 113 MB):
-// 32.6 us on the GPU, 3.5 TB/s, where the bytes alone would take 17.4; of it 4 us pass before the
+// 32.9 us on the GPU, 3.4 TB/s, where the bytes alone would take 17.4; of it 4 us pass before the
 // first tile has arrived (lengths, page table, copy: three dependent loads) and 3 in joining.  12 warps
 // of 144 registers measured best there: 8 warps 37.3 us, 16 warps 33.4 (and 13.2 against 10.8 for 8
-// requests), three stages 33.4 and 128-key tiles on 8 warps 34.2.
+// requests), 128-key tiles on 8 warps 34.2.  48 ragged requests of up to 5000 tokens, 4 new ones each,
+// 16 query rows on 4 fp16 kv heads of 128 (54 MB): 40.3 us, in two passes of 8 rows.
 #include <math.h>
 
 #include "common.cuh"
@@ -70,9 +71,12 @@ struct Args {
   float scale, eps;
 };
 
+// 64 keys: a tile's independent chains are what hides latency beside two or three warps a scheduler.
+// D = 128 on 32 keys and 12 warps 41.1 us against 38.3 on 64 keys and 8 (32 requests of 8192 tokens, 4 kv
+// heads); D = 32 on 64 keys 27.3 against 25.2 on 128 (64 requests of 8192, 3 kv heads).
 template <int D>
 struct Tile {
-  static constexpr int kUnits = D == 128 ? 2 : 4;
+  static constexpr int kUnits = D == 32 ? 8 : 4;
   static constexpr int kKeys = kUnits * kUnit;
   static constexpr int kBytes = kUnits * Layout<D>::kBytes;
 };
@@ -297,9 +301,9 @@ __device__ __forceinline__ void store4(T* p, float4 y, float f, bool sees) {
 __device__ __forceinline__ int key_of_row(int r) { return (r >> 1) + 4 * (r & 1); }
 
 // ------------------------------------------------------------------ the worker kernel
-// Warps of the one CTA an SM runs, by the registers that the output tile takes (more warps spill: 8 query
-// rows of D = 128 on 12 warps 51.0 us against 44.1, 16 rows of D = 64 on 12 warps 109 against 73).
-__host__ __device__ constexpr int warps_of(int nt, int D) { return nt == 1 || (nt == 2 && D <= 64) ? 12 : 8; }
+// Warps of the one CTA an SM runs, by the registers and the ring that the output tile leaves them (8 query
+// rows of D = 128 on 12 warps spill: 51.0 us against 44.1; so do 16 rows of D = 64: 109 against 73).
+__host__ __device__ constexpr int warps_of(int nt, int D) { return nt <= 2 && D <= 64 ? 12 : 8; }
 
 // An unfinished piece of a segment at the end of a warp's run: [RT rows][D + 4] floats (o, m, l), its
 // segment and whether it holds the segment's first / last tile.
@@ -968,7 +972,7 @@ __global__ void __launch_bounds__(kMergeThreads, 6) kv4_merge_kernel(T* __restri
 // ------------------------------------------------------------------ host side
 // Score columns per thread of a row tile: tiles of 4, 8 or 16 query rows.  D = 128 stops at 8: with 16
 // the output tile alone takes half the registers, and the spills cost more than the second pass over
-// the cache saves (48 ragged requests of up to 5000 tokens, 16 rows: 53.9 us against 45.1).
+// the cache saves (48 ragged requests of up to 5000 tokens, 16 rows, 32-key tiles: 53.9 us against 45.1).
 int row_tile(int64_t rows, int64_t D) {
   if (rows <= 4) return 1;
   return rows <= 8 || D == 128 ? 2 : 4;
