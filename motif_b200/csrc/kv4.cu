@@ -254,15 +254,15 @@ __device__ __forceinline__ __half2 highs(__half2 a, __half2 b) { return __highs2
 __device__ __forceinline__ __nv_bfloat162 lows(__nv_bfloat162 a, __nv_bfloat162 b) { return __lows2bfloat162(a, b); }
 __device__ __forceinline__ __nv_bfloat162 highs(__nv_bfloat162 a, __nv_bfloat162 b) { return __highs2bfloat162(a, b); }
 
-// Largest and smallest of the group that LANES neighbouring lanes hold, eight values each (a NaN
+// Largest and smallest of the group that LANES neighbouring lanes hold, 8 E values each (a NaN
 // anywhere: both NaN).  16-bit values keep (max, -min) as a packed pair of their own type, so one
 // packed maximum per step reduces both.
-template <typename T, int LANES>
+template <typename T, int LANES, int E>
 __device__ __forceinline__ void extremes(const uint4* raw, const float* x, float& hi, float& lo) {
   if constexpr (sizeof(T) == 4) {
     hi = lo = x[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) hi = fmax_nan(hi, x[i]), lo = fmin_nan(lo, x[i]);
+    for (int i = 1; i < 8 * E; ++i) hi = fmax_nan(hi, x[i]), lo = fmin_nan(lo, x[i]);
 #pragma unroll
     for (int d = 1; d < LANES; d <<= 1) {
       hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
@@ -271,8 +271,9 @@ __device__ __forceinline__ void extremes(const uint4* raw, const float* x, float
   } else {
     using T2 = typename Pair<T>::type;
     const T2* v = reinterpret_cast<const T2*>(raw);
-    T2 a = __hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3]));
-    const T2 c = __hmin2_nan(__hmin2_nan(v[0], v[1]), __hmin2_nan(v[2], v[3]));
+    T2 a = v[0], c = v[0];
+#pragma unroll
+    for (int i = 1; i < 4 * E; ++i) a = __hmax2_nan(a, v[i]), c = __hmin2_nan(c, v[i]);
     const T2 n = __hneg2(c);
     // (largest, -smallest) of the two halves
     T2 both = __hmax2_nan(lows(a, n), highs(a, n));
@@ -286,7 +287,7 @@ __device__ __forceinline__ void extremes(const uint4* raw, const float* x, float
   }
 }
 
-// The group's pair and this thread's eight codes; y becomes the values they stand for.
+// The group's pair and this thread's 8 E codes, a word for eight; y becomes the values they stand for.
 //
 // The code is the nearest whole number to RN(d / s), d = RN(x - m), ties to even.  With r = RN(1 / s),
 // q = RN(d r) and the exact residual e = d - q s (one fma), RN(q + e r) is RN(d / s) (Markstein 1990:
@@ -295,7 +296,8 @@ __device__ __forceinline__ void extremes(const uint4* raw, const float* x, float
 // where r or e could leave the range, divide, as do groups whose codes could.  Adding 1.5 2^23 + 8
 // rounds to a whole number, ties to even, and leaves c + 8 in the low bits, so the word is a sum of
 // shifted sums less a constant.
-__device__ __forceinline__ void quantise8(const float* x, float hi, float lo, float* y, uint32_t& word, uint32_t& pair) {
+template <int E>
+__device__ __forceinline__ void quantise(const float* x, float hi, float lo, float* y, uint32_t* word, uint32_t& pair) {
   const float range = __fsub_rn(hi, lo);
   constexpr float r15 = 1.0f / 15.0f;
   const float q15 = __fmul_rn(range, r15);
@@ -310,47 +312,51 @@ __device__ __forceinline__ void quantise8(const float* x, float hi, float lo, fl
   // far from 0) can a code leave the range
   odd = odd || lo - m < -8.49f * s || hi - m > 7.49f * s;
   constexpr float kRound = 12582912.f + 8.f;
-  uint32_t sum = 0;
+  uint32_t sum[E] = {};
   if (!odd) {
     const float r = __frcp_rn(s);
     const float2 m2 = make_float2(-m, -m), r2 = make_float2(r, r), s2 = make_float2(s, s), n2 = make_float2(-s, -s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4 * E; ++i) {
       const float2 d = fadd2(make_float2(x[2 * i], x[2 * i + 1]), m2), q0 = fmul2(d, r2);
       const float2 t = fadd2(ffma2(ffma2(n2, q0, d), r2, q0), make_float2(kRound, kRound));
-      sum += __float_as_uint(t.x) * (1u << (8 * i)) + __float_as_uint(t.y) * (16u << (8 * i));
+      sum[i / 4] += __float_as_uint(t.x) * (1u << (8 * (i % 4))) + __float_as_uint(t.y) * (16u << (8 * (i % 4)));
       const float2 v = ffma2(s2, fadd2(t, make_float2(-kRound, -kRound)), make_float2(m, m));
       y[2 * i] = v.x, y[2 * i + 1] = v.y;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8 * E; ++i) {
       const float q = s > 0.f ? __fdiv_rn(__fsub_rn(x[i], m), s) : 0.f;
       const float t = __fadd_rn(fminf(fmaxf(q, -8.f), 7.f), kRound);
-      sum += __float_as_uint(t) << (4 * i);
+      sum[i / 8] += __float_as_uint(t) << (4 * (i % 8));
       y[i] = fmaf(s, __fsub_rn(t, kRound), m);
     }
   }
   // the bits of 1.5 2^23 in every term
-  word = sum - 0x4b400000u * 0x11111111u;
+#pragma unroll
+  for (int e = 0; e < E; ++e) word[e] = sum[e] - 0x4b400000u * 0x11111111u;
   pair = (__float_as_uint(m) & 0xffff0000u) | (__float_as_uint(s) >> 16);
 }
 
-// A thread takes the same eight dims of K and V of one token and head: D / 8 neighbouring lanes make a
-// row, the rows of a warp are neighbouring tokens of one head (blockIdx.y), whose codes and pairs lie
-// next to each other.  131072 tokens of 3 bf16 heads of 64 with the stored values given back: 50.7 us,
-// 4.5 TB/s, bound by the instructions of the quantisation (362 a warp for 16 values a lane, two thirds
-// of the issue slots; the bytes take 35.2); IEEE divisions took 128.6.  5003 tokens of 8 fp32 heads of
-// 128: 11.6 us, at the copy rate.  CTAs that stay and fetch their next rows early measured slower (60.5:
-// the registers cost more warps than the early loads hide).
-template <typename T, int D, typename I>
+// A thread takes E chunks of eight dims of one group, the same ones of K and V of one token and head:
+// DG / 8 E neighbouring lanes make a group, the rows of a warp are neighbouring tokens of one head
+// (blockIdx.y), whose codes and pairs lie next to each other.  What a group needs once (its pair, the
+// reciprocal, the addresses: more than half of the instructions at E = 1) is shared by 8 E values a
+// lane.  131072 tokens of 3 bf16 heads of 64 with the stored values given back: 40.4 us at E = 2, 5.7
+// TB/s or 87 % of the copy rate (E = 1 50.7; E = 4 as slow, of too few warps; IEEE divisions at E = 1
+// 128.6).  A call that does not fill the GPU is a chain of latencies, which E = 1 makes shorter: one
+// token of 64 requests 1.8 us against 2.1.  fp32 is at the copy rate at E = 1: 5003 tokens of 8 heads
+// of 128 11.6 us.  CTAs that stay and fetch their next rows early measured slower (60.5 us where E = 1
+// took 51.0: the registers cost more warps than the early loads hide).
+template <typename T, int D, int E, typename I>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                          const int32_t* __restrict__ slots,
                                                          uint8_t* __restrict__ pool, T* __restrict__ k_out,
                                                          T* __restrict__ v_out, Strides12<I> st, int N, int T_, int Hkv,
                                                          int nslots, PageDiv by) {
   using L = Layout<D>;
-  constexpr int W = D / 8;  // threads of one row
+  constexpr int LANES = L::DG / (8 * E), W = D / (8 * E);  // threads of a group, of a row
   const int w = threadIdx.x % W, h = blockIdx.y;
   const int64_t at = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
   const bool live = at < N;  // whole groups of lanes: W divides the warp
@@ -359,31 +365,40 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k
   allow_dependent_launch();
   kv4::wait_for_previous();
   const int slot = live ? slots[n] : -1;
-  float x[2][8], y[2][8], hi, lo;
-  uint4 raw[2];
-  load8(k + st.at(0, b, h, t) + 8 * w, x[0], raw[0]);
-  load8(v + st.at(3, b, h, t) + 8 * w, x[1], raw[1]);
-  uint32_t word[2], pair[2];
+  const int g = w / LANES, c0 = g * (L::DG / 8) + w % LANES;  // chunks c0, c0 + LANES, ... of eight dims
+  float x[2][8 * E], y[2][8 * E], hi, lo;
+  uint4 raw[2][E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    load8(k + st.at(0, b, h, t) + 8 * (c0 + LANES * e), x[0] + 8 * e, raw[0][e]);
+    load8(v + st.at(3, b, h, t) + 8 * (c0 + LANES * e), x[1] + 8 * e, raw[1][e]);
+  }
+  uint32_t word[2][E], pair[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    extremes<T, L::DG / 8>(&raw[i], x[i], hi, lo);
-    quantise8(x[i], hi, lo, y[i], word[i], pair[i]);
+    extremes<T, LANES, E>(raw[i], x[i], hi, lo);
+    quantise<E>(x[i], hi, lo, y[i], word[i], pair[i]);
   }
   if (!live) return;
   if (slot >= 0 && slot < nslots) {
     const int page = by(slot), off = slot - page * by.P, r = off % kUnit;
     uint8_t* u = pool + (((int64_t)page * Hkv + h) * (by.P / kUnit) + off / kUnit) * L::kBytes;
-    *reinterpret_cast<uint32_t*>(u + r * L::kRow + 4 * w) = word[0];
-    *reinterpret_cast<uint32_t*>(u + L::kV + r * L::kRow + 4 * w) = word[1];
-    if (w % (L::DG / 8) == 0) {
-      const int g = w / (L::DG / 8);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      *reinterpret_cast<uint32_t*>(u + r * L::kRow + 4 * (c0 + LANES * e)) = word[0][e];
+      *reinterpret_cast<uint32_t*>(u + L::kV + r * L::kRow + 4 * (c0 + LANES * e)) = word[1][e];
+    }
+    if (w % LANES == 0) {
       *reinterpret_cast<uint32_t*>(u + L::kKp + (g * kUnit + r) * 4) = pair[0];
       *reinterpret_cast<uint32_t*>(u + L::kVp + (g * kUnit + r) * 4) = pair[1];
     }
   }
   if (k_out) {
-    store8(k_out + st.at(6, b, h, t) + 8 * w, y[0]);
-    store8(v_out + st.at(9, b, h, t) + 8 * w, y[1]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      store8(k_out + st.at(6, b, h, t) + 8 * (c0 + LANES * e), y[0] + 8 * e);
+      store8(v_out + st.at(9, b, h, t) + 8 * (c0 + LANES * e), y[1] + 8 * e);
+    }
   }
 }
 
@@ -521,19 +536,34 @@ extern "C" int motif_b200_kv4_append(const void* k, const void* v, const int32_t
     for (int i = 0; i < 4; ++i)
       if (ptrs[i])
         if (int rc = check_rows16("kv4_append", ptrs[i], strides + 3 * i, sizeof(E))) return rc;
-    const int64_t per_cta = 256 / (DD / 8);
-    auto go = [&](auto width) {
+    // 16-bit rows: two chunks a thread unless one makes at most two CTAs an SM.  Measured in CTAs of the
+    // one-chunk form, one against two: 96 CTAs 2.05 us / 2.21, 192 2.91 / 2.77, 256 3.00 / 3.22 (4 heads
+    // of 32) and 3.07 / 3.32 (8 of 128), 384 3.31 / 2.78, 512 3.29 / 3.49 and 3.32 / 3.45, 1024 5.90 / 4.68
+    // and 5.93 / 4.71.  fp32 (one): 12.34 us / 12.54 for 4096 tokens of 8 heads of 128.
+    auto go = [&](auto width, auto chunks) {
       using I = decltype(width);
+      constexpr int C = decltype(chunks)::value;
+      constexpr int64_t per_cta = 256 / (DD / (8 * C));
       Strides12<I> st;
       for (int i = 0; i < 12; ++i) st.s[i] = (I)strides[i];
-      launch(kv4_append_kernel<E, DD, I>, dim3((unsigned)((B * T + per_cta - 1) / per_cta), (unsigned)Hkv), 256, 0, stream,
+      launch(kv4_append_kernel<E, DD, C, I>, dim3((unsigned)((B * T + per_cta - 1) / per_cta), (unsigned)Hkv), 256, 0, stream,
              (const E*)k, (const E*)v, slots, (uint8_t*)pool, (E*)k_out, (E*)v_out, st, (int)(B * T), (int)T, (int)Hkv,
              (int)(num_pages * page_size), page_div(page_size));
     };
     bool fits = true;
     for (int i = 0; i < 12; ++i) fits = fits && strides[i] >= 0 && strides[i] < (1ll << 31);
-    if (fits) go(int32_t());
-    else go(int64_t());
+    auto go_width = [&](auto chunks) {
+      if (fits) go(int32_t(), chunks);
+      else go(int64_t(), chunks);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if constexpr (sizeof(E) == 2) {
+      if ((B * T + 2048 / DD - 1) / (2048 / DD) * Hkv > 2 * sm_count()) go_width(Two());
+      else go_width(One());
+    } else {
+      go_width(One());
+    }
     return check_launch("kv4_append");
   });
 }

@@ -362,6 +362,34 @@ def test_append_layouts_strides_and_skipped_slots(dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('N,kv,D,P', [(10007, 4, 32, 64), (5001, 3, 64, 48), (1027, 8, 128, 16)])
+def test_append_of_many_tokens_equals_small_calls(dtype, N, kv, D, P):
+    g = gen(N + D)
+    base = torch.randn(N, 2, kv, D, device='cuda', generator=g) * torch.rand(N, 2, kv, 1, device='cuda', generator=g)
+    base = base + torch.randint(-3, 4, (N, 2, kv, 1), device='cuda', generator=g)
+    base[5, 0, 0, D - 1], base[N - 1, 1, kv - 1, 8], base[7, 0, 0, 0] = float('nan'), float('inf'), float('-inf')
+    base[11, 0, 0], base[12, 1, 0] = 1e-6 * base[11, 0, 0], 0.0
+    base = base.to(dtype)
+    k, v = base[:, 0], base[:, 1]
+    pages = -(-N // P)
+    slots = torch.randperm(pages * P, device='cuda', generator=g)[:N].to(torch.int32)
+    slots[3], slots[N - 2] = -1, pages * P
+    pool, parts = ops.kv4_pool(pages, kv, D, P), ops.kv4_pool(pages, kv, D, P)
+    ko, vo = ops.kv4_append(k, v, slots, pool, values=True)
+    for i in range(0, N, 128):
+        pk, pv = ops.kv4_append(k[i:i + 128], v[i:i + 128], slots[i:i + 128].contiguous(), parts, values=True)
+        assert torch.equal(ko[i:i + 128].isnan(), pk.isnan()) and torch.equal(vo[i:i + 128].isnan(), pv.isnan())
+        assert torch.equal(ko[i:i + 128].nan_to_num(), pk.nan_to_num())
+        assert torch.equal(vo[i:i + 128].nan_to_num(), pv.nan_to_num())
+    assert torch.equal(pool, parts)
+    # [1, Hkv, N, D] views whose batch stride needs 64 bits (it is never taken a step of)
+    far = [x.transpose(0, 1).as_strided((1, kv, N, D), (2 ** 33, D, 2 * kv * D, 1), x.storage_offset()) for x in (k, v)]
+    again = ops.kv4_pool(pages, kv, D, P)
+    ops.kv4_append(*far, slots, again)
+    assert torch.equal(pool, again)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize('kv,D,P', [(1, 32, 16), (3, 64, 64), (2, 128, 48)])
 def test_gather_is_exact(dtype, kv, D, P):
     lens = [0, 1, 47, 48, 49, 200]
