@@ -417,42 +417,52 @@ __device__ __forceinline__ void values8(uint32_t word, uint32_t pair, float* x) 
   }
 }
 
-// A thread reads one word of codes of K and of V and writes eight values of each; D / 8 neighbouring
-// lanes make a row, a warp neighbouring tokens of one head.  Tokens at or past the request's length,
-// and those of pages outside the pool, become zeros.  32 prefixes of up to 4096 tokens, 3 bf16 heads
-// of 64 (115 MB, most of it written): 20.4 us, where the bytes take 17.6; 64-bit indexes and
-// conversions from integers took 26.6.
-template <typename T, int D>
+// A thread reads E words of codes of K and of V of one token and group and writes eight values of each;
+// D / 8 E neighbouring lanes make a row, a warp neighbouring tokens of one head.  Tokens at or past the
+// request's length, and those of pages outside the pool, become zeros.  32 prefixes of up to 4096 tokens,
+// 3 bf16 heads of 64 (115 MB, most of it written): 19.3 us at E = 2, where the bytes take 17.6; 20.4 at
+// E = 1, whose length, page and pair serve half as many values (64-bit indexes and conversions from
+// integers: 26.6).
+template <typename T, int D, int E>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(const uint8_t* __restrict__ pool,
                                                          const int32_t* __restrict__ table, int64_t ts,
                                                          const int32_t* __restrict__ lens, T* __restrict__ k_out,
                                                          T* __restrict__ v_out, int blocks, int Hkv, int S, int pages,
                                                          int columns, PageDiv by) {
   using L = Layout<D>;
-  constexpr int W = D / 8;
+  constexpr int LANES = L::DG / (8 * E), W = D / (8 * E);  // threads of a group, of a row
   const int b = blockIdx.x / blocks, h = blockIdx.y, w = threadIdx.x % W;
   const int64_t token = (int64_t)(blockIdx.x - b * blocks) * (256 / W) + threadIdx.x / W;
   allow_dependent_launch();
   kv4::wait_for_previous();
   if (token >= S) return;
   const int j = (int)token;
-  float kx[8], vx[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) kx[i] = vx[i] = 0.f;
+  const int g = w / LANES, c0 = g * (L::DG / 8) + w % LANES;  // chunks c0, c0 + LANES, ... of eight dims
+  const int64_t to = (((int64_t)b * Hkv + h) * S + j) * D + 8 * c0;
+  bool there = false;
+  uint32_t kc[E], vc[E], kp, vp;
   if (j < min(lens[b], columns * by.P)) {
     const int column = by(j), off = j - column * by.P, page = table[b * ts + column];
     if (page >= 0 && page < pages) {
       const uint8_t* u = pool + (((int64_t)page * Hkv + h) * (by.P / kUnit) + off / kUnit) * L::kBytes;
-      const int r = off % kUnit, g = w / (L::DG / 8);
-      const uint32_t kc = *reinterpret_cast<const uint32_t*>(u + r * L::kRow + 4 * w);
-      const uint32_t vc = *reinterpret_cast<const uint32_t*>(u + L::kV + r * L::kRow + 4 * w);
-      values8(kc, *reinterpret_cast<const uint32_t*>(u + L::kKp + (g * kUnit + r) * 4), kx);
-      values8(vc, *reinterpret_cast<const uint32_t*>(u + L::kVp + (g * kUnit + r) * 4), vx);
+      const int r = off % kUnit;
+      there = true;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        kc[e] = *reinterpret_cast<const uint32_t*>(u + r * L::kRow + 4 * (c0 + LANES * e));
+        vc[e] = *reinterpret_cast<const uint32_t*>(u + L::kV + r * L::kRow + 4 * (c0 + LANES * e));
+      }
+      kp = *reinterpret_cast<const uint32_t*>(u + L::kKp + (g * kUnit + r) * 4);
+      vp = *reinterpret_cast<const uint32_t*>(u + L::kVp + (g * kUnit + r) * 4);
     }
   }
-  const int64_t to = (((int64_t)b * Hkv + h) * S + j) * D + 8 * w;
-  store8(k_out + to, kx);
-  store8(v_out + to, vx);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    float kx[8] = {}, vx[8] = {};
+    if (there) values8(kc[e], kp, kx), values8(vc[e], vp, vx);
+    store8(k_out + to + 8 * LANES * e, kx);
+    store8(v_out + to + 8 * LANES * e, vx);
+  }
 }
 
 }  // namespace
@@ -583,11 +593,22 @@ extern "C" int motif_b200_kv4_gather(const void* pool, const int32_t* block_tabl
     const int64_t none[3] = {0, 0, 0};
     if (int rc = check_rows16("kv4_gather", k_out, none, 1)) return rc;
     if (int rc = check_rows16("kv4_gather", v_out, none, 1)) return rc;
-    const int64_t blocks = (S + 256 / (DD / 8) - 1) / (256 / (DD / 8));
-    MB_REQUIRE(B * blocks < (1ll << 31), MB_ERR_SHAPE, "kv4_gather: %lld rows", (long long)(B * Hkv * S));
-    launch(kv4_gather_kernel<E, DD>, dim3((unsigned)(B * blocks), (unsigned)Hkv), 256, 0, stream,
-        (const uint8_t*)pool, block_table, table_stride, lens, (E*)k_out, (E*)v_out, (int)blocks, (int)Hkv, (int)S,
-        (int)num_pages, (int)max_pages, page_div(page_size));
+    MB_REQUIRE(B * ((S + 2048 / DD - 1) / (2048 / DD)) < (1ll << 31), MB_ERR_SHAPE, "kv4_gather: %lld rows",
+               (long long)(B * Hkv * S));
+    auto go = [&](auto chunks) {
+      constexpr int C = decltype(chunks)::value;
+      constexpr int64_t per_cta = 256 / (DD / (8 * C));
+      const int64_t blocks = (S + per_cta - 1) / per_cta;
+      launch(kv4_gather_kernel<E, DD, C>, dim3((unsigned)(B * blocks), (unsigned)Hkv), 256, 0, stream,
+             (const uint8_t*)pool, block_table, table_stride, lens, (E*)k_out, (E*)v_out, (int)blocks, (int)Hkv,
+             (int)S, (int)num_pages, (int)max_pages, page_div(page_size));
+    };
+    // Two chunks a thread unless one would have all of its CTAs running at once (eight an SM).  Measured
+    // in CTAs of the one-chunk form, one against two: 512 2.51 us / 3.63 (fp16, 8 heads of 128) and 2.60 /
+    // 3.71 (bf16, 4 of 32), 768 3.22 / 2.74 (bf16, 3 of 64), 1024 3.87 / 4.24 and 3.89 / 4.23, 2048 6.45 /
+    // 5.19, 32768 69.8 / 54.2; fp32, 8 heads of 128: 1024 7.50 / 9.17, 4096 20.6 / 19.7, 32768 144.6 / 133.1.
+    if (B * ((S + 2048 / DD - 1) / (2048 / DD)) * Hkv > 8 * sm_count()) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 1>());
     return check_launch("kv4_gather");
   });
 }

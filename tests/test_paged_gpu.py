@@ -409,6 +409,24 @@ def test_gather_is_exact(dtype, kv, D, P):
     assert ops.kv4_gather(pool, table, ln, 0, dtype=dtype)[0].shape == (6, kv, 0, D)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('kv,D,P', [(4, 32, 16), (3, 64, 48), (8, 128, 64)])
+def test_gather_of_many_tokens_equals_small_calls(dtype, kv, D, P):
+    lens = [3001, 0, 2600, 1, 1777, 3000, 2999, 16]
+    pool, table, ln = random_cache(lens, kv, D, P, D)
+    table[2, 5] = -1
+    step = 10 * P
+    k, v = ops.kv4_gather(pool, table, ln, 3001, dtype=dtype)
+    for b in range(len(lens)):
+        for i in range(0, 3001, step):
+            row, left = table[b:b + 1, i // P:], (ln[b:b + 1] - i).clamp_min(0)
+            if row.shape[1] == 0:
+                continue
+            sk, sv = ops.kv4_gather(pool, row, left, min(step, 3001 - i), dtype=dtype)
+            assert torch.equal(k[b, :, i:i + step], sk[0]) and torch.equal(v[b, :, i:i + step], sv[0])
+    assert not k[2, :, 5 * P:6 * P].any() and k[2, :, 6 * P:2600].any() and not k[2, :, 2600:].any()
+
+
 # ------------------------------------------------------------------ attention
 @pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize('H,kv,D,P,T', [(12, 3, 64, 64, 1), (4, 4, 64, 16, 1), (6, 2, 32, 32, 3), (8, 1, 128, 128, 1),
