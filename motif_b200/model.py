@@ -850,11 +850,14 @@ def _decode_splits(model, B, Hkv, S):
     return int(max(1, min(want, 64, (S + 255) // 256)))
 
 
-# Most query rows of a kv head (query heads of its group x new tokens) that attend to a 4-bit cache
-# directly; longer chunks read it back and use the prefill kernel.  Measured at 12 / 3 heads of 64,
-# direct against read back: 64 requests of 2048 tokens 94 / 111 us at 64 rows, 170 / 111 at 128; of
-# 8192 tokens 283 / 402 and 547 / 404; 8 requests of 8192 53 / 165 and 85 / 165.
+# Most query rows of a kv head (query heads of its group x new tokens) of one request, and of all requests
+# together, that attend to a 4-bit cache directly; other chunks read it back and use the prefill kernel,
+# which is as slow for few tiles of queries as for many.  Measured at 12 / 3 heads of 64, direct against
+# read back: 64 rows: 64 requests of 2048 tokens 81 / 102 us, of 8192 251 / 373; 128 rows 146 / 103 and
+# 484 / 373.  2048 rows in all: 1 request of 8192 132 / 195 us, 8 133 / 203, 32 133 / 189, 1 of 2048 48 /
+# 56, 16 49 / 48, 1 of 32768 472 / 748; 4096: 4 requests of 8192 248 / 198, 8 of 2048 81 / 58.
 KV4_DIRECT_ROWS = 64
+KV4_DIRECT_ROWS_IN_ALL = 2048
 
 
 def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache], position, dt, dev, dc, st,
@@ -899,7 +902,8 @@ def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache
             kv = cache.append(kt, vt, values=True)
         else:
             cache.append(kt, vt)
-            if key_bias is None and q_start == cached and G * T <= KV4_DIRECT_ROWS:
+            direct = G * T <= KV4_DIRECT_ROWS or B * G * T <= KV4_DIRECT_ROWS_IN_ALL
+            if direct and key_bias is None and q_start == cached:
                 attn = kv4_chord_attention(qb.view(B, T, H, D).transpose(1, 2), cache.pool, cache.pages.table,
                                            cache.pages.lens, pk.alpha, pk.beta, pk.mu, pk.ssmax, softmax_scale=scale,
                                            eps=GGD_EPS).transpose(1, 2).reshape(M, d)

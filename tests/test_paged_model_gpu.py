@@ -57,7 +57,7 @@ def close(a, b, rel=1e-4):
     assert (a.double() - b.double()).abs().max() <= rel * b.double().abs().max()
 
 
-@pytest.mark.parametrize('chunks', [[70, 1, 1, 1], [1, 1, 5], [40, 33, 1, 90, 2], [130, 1]])
+@pytest.mark.parametrize('chunks', [[70, 1, 1, 1], [1, 1, 5], [40, 33, 1, 90, 2], [130, 1], [30, 350, 2]])
 def test_logits_match_a_cache_of_rounded_values(chunks):
     m = model_of(torch.float32)
     B, total = 3, sum(chunks)
