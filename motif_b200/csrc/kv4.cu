@@ -11,17 +11,7 @@ namespace {
 
 using kv4::kUnit;
 using kv4::Layout;
-
-// x / P for 0 <= x < 2^31 and P = 16 UP, UP <= 64: (x / 16) ceil(2^33 / UP) / 2^33 is exact.
-struct PageDiv {
-  uint64_t m;
-  int P;
-  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)((uint32_t)x >> 4) * m) >> 33); }
-};
-PageDiv page_div(int64_t P) {
-  const uint64_t up = (uint64_t)P / kUnit;
-  return {((1ull << 33) + up - 1) / up, (int)P};
-}
+using kv4::PageDiv;
 
 // ------------------------------------------------------------------ slot reservation
 // need_b = ceil((len_b + new_b) / P) - ceil(len_b / P) fresh pages.  Requests are served in order:
@@ -31,11 +21,11 @@ PageDiv page_div(int64_t P) {
 //
 // A block of THREADS requests at a time: every CTA scans the block's tokens and pages by itself, then
 // the threads of all CTAs share the writing.  Where lens_out is lens (or the free counts are one) the
-// CTAs are a cluster, whose barrier keeps the writes behind everybody's reads.  A new token's page is an old table entry or comes straight from the free list,
-// so nobody waits for the fresh entries to be written.  Bound by latency (the bytes take 0.1 us): one
-// scan and two dependent loads.  3.3 us for one token of each of 64 requests (one CTA of four warps),
-// 4.4 for 32 prompts of 4096 tokens, 5.6 for 517 ragged chunks (7.1 and 8.7 on a cluster of 8); on one
-// CTA the latter two took 43.9 and 35.2.
+// CTAs are a cluster, whose barrier keeps the writes behind everybody's reads.  A new token's page is an
+// old table entry or comes straight from the free list, so nobody waits for the fresh entries to be
+// written.  Bound by latency (the bytes take 0.1 us): one scan and two dependent loads.  3.3 us for one
+// token of each of 64 requests (one CTA of four warps), 4.4 for 32 prompts of 4096 tokens, 5.7 for 517
+// ragged chunks (7.1 and 8.7 on a cluster of 8); on one CTA the latter two took 43.9 and 35.2.
 constexpr int kClusterCtas = 8;  // the most a cluster holds everywhere
 constexpr int kReserveCtas = 64;
 

@@ -44,6 +44,17 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 __device__ __forceinline__ float pair_scale(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float pair_centre(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
+// x / P for 0 <= x < 2^31 and P = 16 UP, UP <= 64: (x / 16) ceil(2^33 / UP) / 2^33 is exact.
+struct PageDiv {
+  uint64_t m;
+  int P;
+  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)((uint32_t)x >> 4) * m) >> 33); }
+};
+inline PageDiv page_div(int64_t P) {
+  const uint64_t up = (uint64_t)P / kUnit;
+  return {((1ull << 33) + up - 1) / up, (int)P};
+}
+
 // ------------------------------------------------------------------ host side
 template <typename F>
 int dispatch_dim(int64_t D, F&& f) {

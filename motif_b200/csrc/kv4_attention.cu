@@ -65,7 +65,8 @@ struct Args {
   float* ws;
   Strides6 st;
   int B, H, Hkv, T, G, Z;   // Z: row tiles of the G T query rows of one (request, kv head)
-  int P, most;              // most: tokens that a row of the table can name
+  kv4::PageDiv by;
+  int most;                 // tokens that a row of the table can name
   int64_t pages;
   int ctas;
   float scale, eps;
@@ -381,13 +382,14 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
 
     // The tile to be copied next: its page of this lane's unit (lanes 0 .. TU - 1) is looked up one
     // tile before the copy is issued.
-    const int UP = a.P / kUnit;
+    const int UP = a.by.P / kUnit;
     const bool one_copy = UP % TU == 0;  // a tile's units lie in one page, next to each other
-    const int step_page = TU / UP, step_sub = TU % UP, page0 = lane / UP, sub0 = lane % UP;
+    const int step_page = a.by(KT), step_sub = TU - step_page * UP;
+    const int page0 = a.by(lane * kUnit), sub0 = lane - page0 * UP;
     Cursor ahead = cur;
     int a_len = length_of(a, ahead.b), a_z, a_head;
     split_segment(a, ahead.seg, a_z, a_head);
-    int a_page = (ahead.k * TU + lane) / UP, a_sub = (ahead.k * TU + lane) % UP;
+    int a_page = a.by((ahead.k * TU + lane) * kUnit), a_sub = ahead.k * TU + lane - a_page * UP;
     const int32_t* a_row = a.table + (int64_t)ahead.b * a.ts;
     struct Look {
       int pid, head, sub;  // pid -1: no such unit
@@ -1059,7 +1061,7 @@ extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, c
     a.ws = (float*)workspace;
     for (int i = 0; i < 6; ++i) a.st.s[i] = strides[i];
     a.B = (int)B, a.H = (int)H, a.Hkv = (int)Hkv, a.T = (int)T, a.G = (int)(H / Hkv);
-    a.P = (int)page_size, a.most = (int)(max_pages * page_size), a.pages = num_pages;
+    a.by = page_div(page_size), a.most = (int)(max_pages * page_size), a.pages = num_pages;
     a.scale = scale, a.eps = eps;
     if (int rc = check_rows16("kv4_chord_attention", q, strides, sizeof(E))) return rc;
     if (int rc = check_rows16("kv4_chord_attention", out, strides + 3, sizeof(E))) return rc;
