@@ -5,10 +5,9 @@
 // with k_j = m_j + s_j (c_j - 8) per group of dims, so
 //   q . k_j          = sum_groups  s_j (q . c_j - 8 sum(q)) + m_j sum(q)
 //   sum_j p_j v_j    = sum_j (p_j s_j) c_j                  + sum_j p_j (m_j - 8 s_j)
-// and both products run on the codes themselves.  A code in bits 0..3 of an fp16 IS the number
-// c 2^-24, in bits 4..7 c 2^-20 (subnormal, exact, and the tensor cores take them as they are), so a
-// packed word becomes matrix operands with one AND per pair and no conversion; the powers of two are
-// undone in fp32.  The other operand is split into two fp16 parts of 11 bits each (q after a
+// and both products run on the codes themselves.  A code in bits 6..9 of an fp16 IS the number c 2^-18
+// (subnormal, exact, and the tensor cores take it as it is), so a packed word becomes matrix operands
+// with a shift and an AND per pair and no conversion; the power of two is undone in fp32.  The other operand is split into two fp16 parts of 11 bits each (q after a
 // power-of-two normalisation of its row, p s against the largest scale so far), and the parts are
 // two neighbouring columns of one MMA: with the keys on the M side a tile of 4 query rows fills
 // N = 8, a thread's two accumulator columns are the two parts of ONE query row, and their sum is the
@@ -254,24 +253,30 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, const uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-// The nibbles of w as four fp16 pairs: nibbles (0, 4) and (2, 6) times U, (1, 5) and (3, 7) times 16 U.
-// For 16-bit tensors they stay the subnormal numbers that the masked bits are (U = 2^-24).  The tensor
-// cores align the products of a step by their operands' exponent fields, which for a subnormal say up
-// to 10 bits more than it has, and cut below 24 bits: sums keep about 17 bits (the results of 300 keys
-// were 3e-5 off where 16 bits round at 4e-4 to 4e-3).  fp32 tensors make them normal numbers c - 8
-// (U = 1: the bits of 1024 or-ed in, 1024 + 8 U taken off) at one more instruction a pair, and need
-// the sums less 8 no more.
+// The nibbles of w as four fp16 pairs, nibbles (0, 4), (1, 5), (2, 6) and (3, 7) times U (or kOdd U).  For 16-bit
+// tensors they stay the subnormal numbers that the masked bits are (U = 2^-18).  The tensor cores align
+// the products of a step by their operands' exponent fields and cut below 24 bits; a subnormal's field
+// stands for its bit 9, so the codes are shifted to end there, which leaves the sums all but the bits of
+// 8 sum(q) against q . c.  In bits 0..3 and 4..7, without most of the shifts, the sums kept 17 bits and 64
+// requests of 8192 took 33.0 us where they take 35.2; distance from 64 bits before the last rounding (16
+// requests of 8192, fp16) 2.0e-5 there, 9.5e-7 here, and 1.1e-6 for elementary operations in fp32.  fp32
+// tensors make them normal numbers c - 8 (U = 1: the bits of 1024 or-ed in, 1024 + 8 U taken off; where
+// they lie in the word does not matter then, and the odd nibbles come out 16 times as large) at one more
+// instruction a pair, and need the sums less 8 no more; for 16-bit ones that took 39.5 us.
 template <bool EXACT>
 __device__ __forceinline__ void codes(uint32_t w, uint32_t* h) {
-  const uint32_t v = w >> 8;
-  h[0] = w & 0x000f000fu;
-  h[1] = w & 0x00f000f0u;
-  h[2] = v & 0x000f000fu;
-  h[3] = v & 0x00f000f0u;
   if constexpr (EXACT) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(h[i]) : "r"(h[i] | 0x64006400u), "r"(i & 1 ? 0xe480e480u : 0xe408e408u));
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = (i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(h[i]) : "r"(v | 0x64006400u), "r"(i & 1 ? 0xe480e480u : 0xe408e408u));
+    }
+  } else {
+    constexpr uint32_t kBits = 0x03c003c0u;
+    h[0] = (w << 6) & kBits;
+    h[1] = (w << 2) & kBits;
+    h[2] = (w >> 2) & kBits;
+    h[3] = (w >> 6) & kBits;
   }
 }
 
@@ -342,7 +347,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
   constexpr int MT = DG / 16;        // 16-dim output tiles of a group
   constexpr int RT = 4 * NT;         // query rows of a row tile
   constexpr bool EXACT = sizeof(T) == 4;
-  constexpr int kUnitBits = EXACT ? 0 : 24;  // codes enter the products times 2^-kUnitBits
+  constexpr int kUnitBits = EXACT ? 0 : 18;  // codes enter the products times 2^-kUnitBits,
+  constexpr float kOdd = EXACT ? 16.f : 1.f;  // those of odd nibbles times kOdd as well
   // 16-bit queries have no low part: with 8 rows or more every column of the first product is a row,
   // a thread holding rows 2 t4 and 2 t4 + 1 of each 8; else row t4 of each 4, its parts in two columns
   constexpr bool WIDE = !EXACT && NT > 1;
@@ -510,8 +516,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
               for (int p = 0; p < 4; ++p) {
                 const float2 y = fmul2(make_float2(x[n][g][8 * w + p], x[n][g][8 * w + p + 4]), make_float2(up, up));
                 sum = fadd2(sum, y);
-                // the codes of the odd pairs are 16 times as large
-                const float2 v = p & 1 ? fmul2(y, make_float2(0.0625f, 0.0625f)) : y;
+                const float2 v = p & 1 ? fmul2(y, make_float2(1.f / kOdd, 1.f / kOdd)) : y;
                 uint32_t f = pack2<__half>(v.x, v.y);
                 if (!WIDE && (g8 & 1)) {  // the low part; values of 16 bits have none
                   const float2 hi = __half22float2(*reinterpret_cast<__half2*>(&f));
@@ -792,7 +797,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
               y[2 * j] = fmaf((o[n][g][j][0] + o[n][g][j][1]) * pow2(kUnitBits - 10), back, pn[g]) * inv;
-              y[2 * j + 1] = fmaf((o[n][g][j][2] + o[n][g][j][3]) * pow2(kUnitBits - 14), back, pn[g]) * inv;
+              y[2 * j + 1] = fmaf((o[n][g][j][2] + o[n][g][j][3]) * (pow2(kUnitBits - 10) / kOdd), back, pn[g]) * inv;
             }
             const int d0 = g * DG + g8 * 2 * MT;
             if (direct) {
