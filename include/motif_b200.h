@@ -503,14 +503,17 @@ MB_API int motif_b200_sample(const void* logits, int64_t ld, int64_t B, int64_t 
  *   MB_FORCE_GDN_FUSED       16-bit chunked delta rule with a workspace on the single fused
  *                            kernel (the no-workspace path)
  *   MB_FORCE_GDN_WIDE        the split path's state scan on 64-column value slices even for small
- *                            batches (which take 32-column slices; the results are identical) */
+ *                            batches (which take 32-column slices; the results are identical)
+ *   MB_FORCE_KV4_WAIT_FAILS  the copy waits of every third CTA of motif_b200_kv4_chord_attention run
+ *                            out at once: its rows become NaN and motif_b200_wait_timeouts counts it */
 enum {
   MB_FORCE_CHORD_MMA_SYNC = 0,
   MB_FORCE_DECODE_SCALAR = 1,
   MB_FORCE_GDN_PRECISE = 2,
   MB_FORCE_GDN_FUSED = 3,
   MB_FORCE_GDN_WIDE = 4,
-  MB_FORCE_COUNT = 5
+  MB_FORCE_KV4_WAIT_FAILS = 5,
+  MB_FORCE_COUNT = 6
 };
 MB_API int motif_b200_testing_force(int knob, int value);
 
@@ -566,6 +569,7 @@ MB_API int motif_b200_kv4_gather(const void* pool, const int32_t* block_table, i
  * newest tokens of every request over its cache: token t of request b is at position
  * lens[b] - T + t, or lens[b] - q_lens[b] + t where q_lens != NULL (rows t >= q_lens[b] are
  * padding).  Rows that see no key are zeros; keys on table entries outside the pool are left out.
+ * Rows of a CTA whose copy wait ran out (never expected; motif_b200_wait_timeouts) are NaN.
  * `strides` (elements), [6]: (b, h, t) of q, out.  `workspace` (16-byte aligned) holds
  * motif_b200_kv4_attention_workspace_bytes bytes of the current device. */
 MB_API int64_t motif_b200_kv4_attention_workspace_bytes(int64_t H, int64_t Hkv, int64_t T, int64_t D);

@@ -68,6 +68,7 @@ struct Args {
   int most;                 // tokens that a row of the table can name
   int64_t pages;
   int ctas;
+  bool fail;                // a test: the waits of every third CTA run out at once
   float scale, eps;
 };
 
@@ -383,6 +384,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
   const int count = run_start<kWarps>(cta_count, warp + 1) - run0;
 
   bool failed = false;
+  const uint32_t polls = a.fail && blockIdx.x % 3 == 1 ? 0 : kWaitLimit;
   if (count > 0) {
     Cursor cur = locate<KT>(a, reqs, cta_first + run0);
 
@@ -555,8 +557,13 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
         looked = 2;
         if (count > 2) next = step();
       }
-      // never expected to run out: the rows then stay unwritten
-      failed |= !mbar_wait_bounded(&bar[s], (uint32_t)phase, kWaitLimit);
+      // never expected to run out: nothing more is asked for then, and what is on its way may still land
+      if (__any_sync(0xffffffffu, !mbar_wait_bounded(&bar[s], (uint32_t)phase, polls))) {
+        failed = true;
+        mbar_wait_bounded(&bar[s], (uint32_t)phase, kWaitLimit);
+        if (looked > i + 1) mbar_wait_bounded(&bar[s ^ 1], (uint32_t)(phase ^ s), kWaitLimit);
+        break;
+      }
       const uint8_t* tile = ring + s * Tile<D>::kBytes;
       const uint32_t units = (valid >> (TU * s)) & ((1u << TU) - 1);
       const int k0 = cur.k * KT;
@@ -828,8 +835,31 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
   // The CTA's pieces in tile order: neighbours of one segment are joined, and written out where the
   // CTA holds all of the segment, else left to the merge (slot 0 where the segment began before this
   // CTA's run, 1 where it began in it).
-  if (__syncthreads_or(failed)) {  // each copy was waited for, so none is in flight
+  if (__syncthreads_or(failed)) {
+    // the copies that were on their way had a second wait; what depends on this CTA's tiles becomes NaN,
+    // here for the segments within its run and by the merge for those that reach beyond
     if (threadIdx.x == 0) atomicAdd(&g_kv4_wait_timeouts, 1u);
+    float* part = a.ws + (int64_t)blockIdx.x * 2 * piece_floats<D, NT>();
+    for (int i = threadIdx.x; i < 2 * piece_floats<D, NT>(); i += 32 * kWarps) part[i] = NAN;
+    const Requests all = scan_requests<KT>(a);
+    const Cut again(all.total, gridDim.x);
+    const int first = again.start(blockIdx.x), last = again.start(blockIdx.x + 1);
+    Cursor u = locate<KT>(a, all, first);
+    for (int x = first - u.k; x < last;) {
+      const int nq = queries_of(a, u.b), base = length_of(a, u.b) - nq;
+      int z, hk, t, gi;
+      split_segment(a, u.seg, z, hk);
+      for (int i = threadIdx.x; i < RT * (D / 4) && x >= first && x + u.nt <= last; i += 32 * kWarps) {
+        const int r = z * RT + i / (D / 4);
+        split_row(a, r, t, gi);
+        if (r < a.G * a.T)
+          store4(out + u.b * a.st.s[3] + (hk * a.G + gi) * a.st.s[4] + t * a.st.s[5] + i % (D / 4) * 4,
+                 make_float4(NAN, NAN, NAN, NAN), 1.f, t < nq && base + t >= 0);
+      }
+      x += u.nt;
+      u.k = u.nt - 1;
+      advance<KT>(a, u);
+    }
     return;
   }
   constexpr int SLOTS = 2 * kWarps, LV = D / 4, H = 32 / LV;
@@ -1068,6 +1098,7 @@ extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, c
     a.B = (int)B, a.H = (int)H, a.Hkv = (int)Hkv, a.T = (int)T, a.G = (int)(H / Hkv);
     a.by = page_div(page_size), a.most = (int)(max_pages * page_size), a.pages = num_pages;
     a.scale = scale, a.eps = eps;
+    a.fail = forced(MB_FORCE_KV4_WAIT_FAILS);
     if (int rc = check_rows16("kv4_chord_attention", q, strides, sizeof(E))) return rc;
     if (int rc = check_rows16("kv4_chord_attention", out, strides + 3, sizeof(E))) return rc;
     const int nt = row_tile((int64_t)a.G * T, D);

@@ -7,8 +7,8 @@ Bars are those of `test_paged_gpu.py` unless a test derives its own.
 import pytest
 import torch
 
-from motif_b200 import ops
-from test_paged_gpu import attention_64, gen, random_cache
+from motif_b200 import _lib, ops
+from test_paged_gpu import attention_64, close, gen, params, random_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,26 @@ def test_sums_of_16_bit_tensors_keep_their_bits(H, kv, D, T):
     want = attention_64(q, pool, table, ln, *p).half()
     wrong = (ops.kv4_chord_attention(q, pool, table, ln, *p) != want).sum()
     assert wrong <= 8 * (attention_32(q, pool, table, ln, *p) != want).sum()
+
+
+# ------------------------------------------------------------------ waits that run out
+@pytest.mark.parametrize('H,kv,D,T', [(12, 3, 64, 1), (16, 1, 64, 3), (8, 2, 128, 2), (4, 4, 32, 1)])
+def test_rows_of_a_failed_wait_are_nan_and_counted(H, kv, D, T):
+    """A CTA whose copy wait runs out (here at once, in every third CTA) leaves NaN in the rows that
+    needed it, the right values in all others, and is counted; the next call is as ever."""
+    lens = [(91 * i) % 700 + 1 for i in range(90)] + [9000, 0, 2, 4001]
+    pool, table, ln = random_cache(lens, kv, D, 64, 62)
+    q = torch.randn(len(lens), H, T, D, device='cuda', generator=gen(63)).bfloat16()
+    pr = params(H, 10)
+    want = ops.kv4_chord_attention(q, pool, table, ln, *pr)
+    assert _lib.wait_timeouts() == 0 and not want.isnan().any()
+    with _lib.forced(_lib.FORCE_KV4_WAIT_FAILS):
+        got = ops.kv4_chord_attention(q, pool, table, ln, *pr)
+    ctas = torch.cuda.get_device_properties(0).multi_processor_count
+    assert _lib.wait_timeouts() == len(range(1, ctas, 3))
+    lost = got.isnan()
+    assert torch.equal(lost.any(-1), lost.all(-1))             # whole rows
+    assert torch.equal(got[~lost], want[~lost])
+    assert lost[90].all() and not lost[91].any()               # over many CTAs; without keys
+    assert 0.2 < lost.double().mean() < 0.8
+    assert torch.equal(ops.kv4_chord_attention(q, pool, table, ln, *pr), want) and _lib.wait_timeouts() == 0
