@@ -307,20 +307,46 @@ __device__ __forceinline__ void store4(T* p, float4 y, float f, bool sees) {
 // V load take neighbouring keys (128 consecutive bytes of shared memory per load).
 __device__ __forceinline__ int key_of_row(int r) { return (r >> 1) + 4 * (r & 1); }
 
+// Zeroes the rows of every n-th request without tiles.
+template <typename T, int D>
+__device__ __forceinline__ void zero_rows(T* out, const Args& a) {
+  for (int e = blockIdx.x; e < a.B; e += gridDim.x) {
+    if (tiles_of<Tile<D>::kKeys>(a, e) > 0) continue;
+    for (int i = threadIdx.x; i < a.H * a.T * (D / 4); i += blockDim.x) {
+      const int row = i / (D / 4), h = row / a.T;
+      store4(out + e * a.st.s[3] + h * a.st.s[4] + (row - h * a.T) * a.st.s[5] + i % (D / 4) * 4,
+             make_float4(0.f, 0.f, 0.f, 0.f), 0.f, false);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ the worker kernel
 // Warps of the one CTA an SM runs, by the registers and the ring that the output tile leaves them (8 query
 // rows of D = 128 on 12 warps spill: 51.0 us against 44.1; so do 16 rows of D = 64: 109 against 73).
 __host__ __device__ constexpr int warps_of(int nt, int D) { return nt <= 2 && D <= 64 ? 12 : 8; }
 
 // An unfinished piece of a segment at the end of a warp's run: [RT rows][D + 4] floats (o, m, l), its
-// segment and whether it holds the segment's first / last tile.
+// segment, whether it holds the segment's first / last tile, the tiles that follow it in the segment, and
+// the new tokens and first position of the request.
 struct Piece {
   int b, seg;  // b < 0: none
-  int begins, ends;
+  int begins, ends, more, nq, base;
 };
+// What a worker CTA leaves to the merge beside its partials: the segment that begins in its run and goes
+// on in the next ones, in how many CTAs it lies, and the new tokens and first position of its request.
+struct alignas(16) Open {
+  int parts, b, seg, nq, base;  // parts 0: none
+  int pad[3];
+};
+__host__ __device__ constexpr int piece_floats(int nt, int64_t D) { return 4 * nt * ((int)D + 4); }
 template <int D, int NT>
-constexpr int piece_floats() {
-  return 4 * NT * (D + 4);
+__host__ __device__ constexpr int piece_floats() {
+  return piece_floats(NT, D);
+}
+// The workspace: two partials of every CTA, then an Open of each.
+template <int D, int NT>
+__device__ __forceinline__ Open* open_of(const Args& a, int cta) {
+  return reinterpret_cast<Open*>(a.ws + (int64_t)a.ctas * 2 * piece_floats<D, NT>()) + cta;
 }
 // A warp's last piece takes its ring's place, which is free by then; one that a segment from before
 // the run leaves on the way needs its own.
@@ -357,6 +383,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kWarps][kStages];
   __shared__ Piece pieces[kWarps][2];
+  __shared__ int s_total;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g8 = lane >> 2, t4 = lane & 3;
@@ -373,12 +400,15 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
     pieces[warp][0].b = pieces[warp][1].b = -1;
   }
   kv4::wait_for_previous();
-  // only now may the merge take its place: it reads the lengths before it waits for this grid to end,
-  // and what came before this grid may have written them
-  allow_dependent_launch();
+  allow_dependent_launch();  // the merge, which waits for the end of this grid before it touches memory
   const Requests reqs = scan_requests<KT>(a);
   const Cut cut(reqs.total, gridDim.x);
-  if ((int)blockIdx.x >= cut.working) return;
+  if ((int)blockIdx.x >= cut.working) {
+    if (threadIdx.x == 0) open_of<D, NT>(a, blockIdx.x)->parts = 0;
+    zero_rows<T, D>(out, a);
+    return;
+  }
+  if (threadIdx.x == 0) s_total = reqs.total;
   const int cta_first = cut.start(blockIdx.x), cta_count = cut.each + ((int)blockIdx.x < cut.more ? 1 : 0);
   const int run0 = run_start<kWarps>(cta_count, warp);
   const int count = run_start<kWarps>(cta_count, warp + 1) - run0;
@@ -780,6 +810,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
           pieces[warp][which].seg = cur.seg;
           pieces[warp][which].begins = from_start;
           pieces[warp][which].ends = ends;
+          pieces[warp][which].more = cur.nt - 1 - cur.k;
+          pieces[warp][which].nq = nq;
+          pieces[warp][which].base = base;
         }
         const float back = pow2(min(ve, 127));  // and 2^(kUnitBits - 10)
 #pragma unroll
@@ -832,6 +865,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
     }
   }
 
+  zero_rows<T, D>(out, a);  // while other warps are still at work
+
   // The CTA's pieces in tile order: neighbours of one segment are joined, and written out where the
   // CTA holds all of the segment, else left to the merge (slot 0 where the segment began before this
   // CTA's run, 1 where it began in it).
@@ -845,6 +880,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
     const Cut again(all.total, gridDim.x);
     const int first = again.start(blockIdx.x), last = again.start(blockIdx.x + 1);
     Cursor u = locate<KT>(a, all, first);
+    if (threadIdx.x == 0) open_of<D, NT>(a, blockIdx.x)->parts = 0;
     for (int x = first - u.k; x < last;) {
       const int nq = queries_of(a, u.b), base = length_of(a, u.b) - nq;
       int z, hk, t, gi;
@@ -856,6 +892,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
           store4(out + u.b * a.st.s[3] + (hk * a.G + gi) * a.st.s[4] + t * a.st.s[5] + i % (D / 4) * 4,
                  make_float4(NAN, NAN, NAN, NAN), 1.f, t < nq && base + t >= 0);
       }
+      if (threadIdx.x == 0 && x >= first && x + u.nt > last)
+        *open_of<D, NT>(a, blockIdx.x) = {again.cta_of(x + u.nt - 1) - (int)blockIdx.x + 1, u.b, u.seg, nq, base, {}};
       x += u.nt;
       u.k = u.nt - 1;
       advance<KT>(a, u);
@@ -864,12 +902,19 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
   }
   constexpr int SLOTS = 2 * kWarps, LV = D / 4, H = 32 / LV;
   static_assert(SLOTS <= 32, "a lane per slot");
-  Piece mine = {-1, 0, 0, 0};
+  Piece mine = {-1, 0, 0, 0, 0, 0, 0};
   if (lane < SLOTS) mine = pieces[lane >> 1][lane & 1];
   const uint32_t present = __ballot_sync(0xffffffffu, mine.b >= 0);
   uint32_t group = __match_any_sync(0xffffffffu, ((uint64_t)(uint32_t)mine.b << 32) | (uint32_t)mine.seg) & present;
   const uint32_t heads = __ballot_sync(0xffffffffu, mine.b >= 0 && lane == __ffs(group) - 1);
   const uint32_t ending = __ballot_sync(0xffffffffu, mine.b >= 0 && mine.ends);
+  const uint32_t open = __ballot_sync(0xffffffffu, ((heads >> lane) & 1u) && mine.begins && !(group & ending));
+  const int more = __shfl_sync(0xffffffffu, mine.more, 31 - __clz(group | 1u));  // of the group's last piece
+  if (warp == kWarps - 1 && lane == max(__ffs(open) - 1, 0)) {  // at most one; the last warp has the fewest items
+    const Cut all(s_total, gridDim.x);  // the open segment holds the CTA's last tile
+    const int parts = open ? all.cta_of(all.start(blockIdx.x + 1) - 1 + more) - (int)blockIdx.x + 1 : 0;
+    *open_of<D, NT>(a, blockIdx.x) = {parts, mine.b, mine.seg, mine.nq, mine.base, {}};
+  }
   // an item is one row of one group; H members at a time, D / 4 lanes each
   for (int item = warp; item < __popc(heads) * RT; item += kWarps) {
     const int rr = item % RT;
@@ -926,10 +971,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
 
 // ------------------------------------------------------------------ merge
 // Merge CTA c joins the partials of the segment that begins in worker CTA c's run and goes on in the
-// next one's, if there is one, and zeroes the rows of every n-th request without tiles.  Thread group
-// i of D RT / 4 threads takes partials i, i + PL, ... in one pass with a running maximum; the groups
-// are joined in order.  256 threads of 40 registers find room beside the worker CTAs, so the search
-// for the segment runs before they end.
+// next one's, if there is one (the worker has left beside them which).  Thread group i of D RT / 4 threads takes partials i, i + PL, ... in one pass
+// with a running maximum; the groups are joined in order.  256 threads of 40 registers find room beside
+// the worker CTAs, so the merge is there when they end.
 constexpr int kMergeThreads = 256;
 
 template <typename T, int D, int NT>
@@ -939,43 +983,30 @@ __global__ void __launch_bounds__(kMergeThreads, 6) kv4_merge_kernel(T* __restri
   __shared__ float s_m[PL][RT], s_l[PL][RT];
   __shared__ float4 s_acc[PL][NV];
   allow_dependent_launch();  // a projection that follows may start fetching its weights
-  const int tid = threadIdx.x;
-  const Requests reqs = scan_requests<KT>(a);
-  const Cut cut(reqs.total, a.ctas);
-  const int c0 = blockIdx.x;
-  Cursor u = {0, 0, 0, 1};
-  int n = 0;  // partials
-  if (c0 + 1 < cut.working) {
-    const int x = cut.start(c0 + 1);  // the next CTA's first tile
-    u = locate<KT>(a, reqs, x);
-    if (u.k > 0 && x - u.k >= cut.start(c0)) n = cut.cta_of(x - u.k + u.nt - 1) - c0 + 1;
-  }
+  // no memory is touched before; every CTA waits, also those without work: what follows this grid must
+  // find the workers' done
+  kv4::wait_for_previous();
+  const int tid = threadIdx.x, c0 = blockIdx.x;
   const int v = tid % NV, pl = tid / NV, rr = v / (D / 4), d = v % (D / 4) * 4;
-  const int b = u.b, nq = queries_of(a, b), base = length_of(a, b) - nq;
+  const Open u = *open_of<D, NT>(a, c0);
+  const int n = min(u.parts, a.ctas - c0);
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f), acc = y;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  float m = -INFINITY, l = 0.f;
+  auto fetch = [&](int i) {
+    // the first CTA's slot 1 (the segment began in its run), every other one's slot 0
+    const float* src = a.ws + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * piece_floats<D, NT>() + rr * (D + 4);
+    y = *reinterpret_cast<const float4*>(src + d);
+    ml = *reinterpret_cast<const float2*>(src + D);
+  };
+  if (c0 + pl < a.ctas) fetch(pl);  // together with the number of them
   int z, hk, t, gi;
   split_segment(a, u.seg, z, hk);
   const int r = z * RT + rr;
   split_row(a, r, t, gi);
-  // the workers write other rows
-  for (int e = blockIdx.x; e < a.B; e += gridDim.x) {
-    if (tiles_of<KT>(a, e) > 0) continue;
-    for (int i = tid; i < a.H * a.T * (D / 4); i += kMergeThreads) {
-      const int row = i / (D / 4), h = row / a.T;
-      store4(out + e * a.st.s[3] + h * a.st.s[4] + (row - h * a.T) * a.st.s[5] + i % (D / 4) * 4,
-             make_float4(0.f, 0.f, 0.f, 0.f), 0.f, false);
-    }
-  }
-  // every CTA waits, also those without work: what follows this grid must find the workers' done
-  kv4::wait_for_previous();
-  if (n == 0) return;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float m = -INFINITY, l = 0.f;
 #pragma unroll 4
   for (int i = pl; i < n; i += PL) {
-    // the first CTA's slot 1 (the segment began in its run), every other one's slot 0
-    const float* src = a.ws + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * piece_floats<D, NT>() + rr * (D + 4);
-    const float4 y = *reinterpret_cast<const float4*>(src + d);
-    const float2 ml = *reinterpret_cast<const float2*>(src + D);
+    if (i > pl) fetch(i);
     const float mn = fmaxf(m, ml.x), shift = mn == -INFINITY ? 0.f : mn;
     const float f = exp2f(m - shift), fi = exp2f(ml.x - shift);
     acc.x = fmaf(fi, y.x, acc.x * f), acc.y = fmaf(fi, y.y, acc.y * f);
@@ -983,27 +1014,29 @@ __global__ void __launch_bounds__(kMergeThreads, 6) kv4_merge_kernel(T* __restri
     l = fmaf(fi, ml.y, l * f);
     m = mn;
   }
-  s_acc[pl][v] = acc;
-  if (d == 0) s_m[pl][rr] = m, s_l[pl][rr] = l;
-  __syncthreads();
-  if (pl) return;
-  m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < PL; ++i) m = fmaxf(m, s_m[i][rr]);
-  const float shift = m == -INFINITY ? 0.f : m;
-  acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < PL; ++i) {
-    const float f = exp2f(s_m[i][rr] - shift);
-    const float4 y = s_acc[i][v];
-    acc.x = fmaf(f, y.x, acc.x), acc.y = fmaf(f, y.y, acc.y);
-    acc.z = fmaf(f, y.z, acc.z), acc.w = fmaf(f, y.w, acc.w);
-    l = fmaf(f, s_l[i][rr], l);
+  if (n) {  // the same for all threads
+    s_acc[pl][v] = acc;
+    if (d == 0) s_m[pl][rr] = m, s_l[pl][rr] = l;
+    __syncthreads();
   }
-  if (r >= a.G * a.T) return;
-  const bool sees = t < nq && base + t >= 0 && l != 0.f;
-  store4(out + b * a.st.s[3] + (hk * a.G + gi) * a.st.s[4] + t * a.st.s[5] + d, acc, sees ? 1.f / l : 0.f, sees);
+  if (n && pl == 0 && r < a.G * a.T) {
+    m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) m = fmaxf(m, s_m[i][rr]);
+    const float shift = m == -INFINITY ? 0.f : m;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      const float f = exp2f(s_m[i][rr] - shift);
+      y = s_acc[i][v];
+      acc.x = fmaf(f, y.x, acc.x), acc.y = fmaf(f, y.y, acc.y);
+      acc.z = fmaf(f, y.z, acc.z), acc.w = fmaf(f, y.w, acc.w);
+      l = fmaf(f, s_l[i][rr], l);
+    }
+    const bool sees = t < u.nq && u.base + t >= 0 && l != 0.f;
+    store4(out + u.b * a.st.s[3] + (hk * a.G + gi) * a.st.s[4] + t * a.st.s[5] + d, acc, sees ? 1.f / l : 0.f, sees);
+  }
 }
 
 // ------------------------------------------------------------------ host side
@@ -1057,8 +1090,7 @@ using namespace mb::kv4;
 
 extern "C" int64_t motif_b200_kv4_attention_workspace_bytes(int64_t H, int64_t Hkv, int64_t T, int64_t D) {
   if (Hkv < 1 || H < Hkv || T < 1) return 0;
-  const int nt = row_tile(H / Hkv * T, D);
-  return (int64_t)sm_count() * 2 * 4 * nt * (D + 4) * 4;
+  return (int64_t)sm_count() * (2 * piece_floats(row_tile(H / Hkv * T, D), D) * (int64_t)sizeof(float) + sizeof(Open));
 }
 
 extern "C" int motif_b200_kv4_chord_attention(const void* q, const void* pool, const int32_t* block_table,
