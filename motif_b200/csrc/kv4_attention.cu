@@ -49,6 +49,7 @@ constexpr int kStages = 2;
 constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 4.f;  // log 2 units
+constexpr int kLift = 60;
 
 struct Strides6 {
   int64_t s[6];  // q(b,h,t) out(b,h,t)
@@ -469,12 +470,15 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
     uint32_t qf[QT][NG][2 * KW][2];
     float sq[NT][NG], qr[NT], ar[NT], be[NT], mh[NT];
     int pos[NT];
-    // weights are taken against a reference that a row's logits exceed by 2^kSlack at most: it moves
-    // when a tile goes beyond that (limit[n] above it, relative), not with every new maximum
+    // weights are taken against a reference that a row's logits exceed by limit[n] at most, kSlack more
+    // than the row's lift: it moves when a tile goes beyond that, not with every new maximum
     float o[NT][NG][MT][4], ref[NT], limit[NT];
     float2 l[NT], pm[NT][NG];  // of the thread's keys of rows 0 .. 7 and 8 .. 15 of the units
-    int ve = 0;        // o holds p s 2^(10 - ve): the exponent of the largest V scale so far
-    float vup = 0.f, vtop = 0.f;  // 2^(10 - ve), 2^(ve + 1) (0: no tile yet)
+    // o holds p s 2^(10 - ve), ve the exponent of the largest V scale so far.  Where the keys that have
+    // weight have scales more than 2^12 below it, the row's weights are all 2^lift larger, so that the
+    // fp16 parts of p s keep their 22 bits; a tile whose scales reach vtop looks again
+    int ve = 0;
+    float vup = 0.f, vtop = 0.f;  // 2^(10 - ve), the least 2^(ve + 1 - lift) (0: no tile yet)
     int lo_pos = 0;    // smallest position of a row that sees keys
     int nq = 0, base = 0, len = 0;
     const float kf = (float)key_of_row(g8);
@@ -706,20 +710,24 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
           beyond = beyond || top[n] > limit[n];
         }
         if (__any_sync(0xffffffffu, beyond)) {
-          // o is kept against the largest V scale so far: p s 2^(10 - ve) < 2^(kSlack + 11)
-          const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-          const int vn = max(ve, (int)(bits >> 23) - 127);
+          // p s 2^(10 - ve) stays below 2^(kSlack + 11), weights and what they are multiplied with in range
+          const int most = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23) - 127;
+          const int vn = max(ve, most);
           const float vdown = pow2(max(ve - vn, -126));
-          ve = vn;
-          vup = pow2(10 - vn);
-          vtop = pow2(min(vn, 126) + 1);
+          float small = INFINITY, lifted = kSlack;
+#pragma unroll
+          for (int u = 0; u < TU; ++u)
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+              small = fminf(small, fminf(kv4::pair_scale(vp[u][g][0]), kv4::pair_scale(vp[u][g][1])));
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
+            lifted = fmaxf(lifted, limit[n]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], d));
-            const float up = top[n] > limit[n] ? top[n] : 0.f;
+          }
+          auto move = [&](int n, float up) {
             const float f = limit[n] == -INFINITY ? 1.f : exp2f(-up);  // the first keys: the sums are still 0
-            if (top[n] > limit[n]) limit[n] = kSlack;
             ref[n] += up;
             const float2 f2 = make_float2(f, f), fo = make_float2(f * vdown, f * vdown);
             l[n] = fmul2(l[n], f2);
@@ -736,7 +744,42 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
             }
 #pragma unroll
             for (int u = 0; u < TU; ++u) x[n][u] = fadd2(x[n][u], make_float2(-up, -up));
+          };
+          // scales within 2^12 of each other need no lift, whatever the weights
+          if (!__any_sync(0xffffffffu, small * 4096.f < pow2(min(vn, 127)) || lifted > kSlack || (vn > ve && vtop > 0.f))) {
+            vtop = pow2(min(vn, 126) + 1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              move(n, top[n] > limit[n] ? top[n] : 0.f);
+              if (top[n] > limit[n]) limit[n] = kSlack;
+            }
+          } else {
+            vtop = pow2(min(vn, 126) + 1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const bool first = limit[n] == -INFINITY, moves = top[n] > limit[n];
+              const float was = first ? 0.f : limit[n] - kSlack, at = moves ? top[n] : was;
+              float heavy = 0.f;  // the largest weighted scale of this tile
+#pragma unroll
+              for (int u = 0; u < TU; ++u) {
+                float2 vs = make_float2(kv4::pair_scale(vp[u][0][0]), kv4::pair_scale(vp[u][0][1]));
+                if constexpr (NG == 2)
+                  vs = make_float2(fmaxf(vs.x, kv4::pair_scale(vp[u][1][0])), fmaxf(vs.y, kv4::pair_scale(vp[u][1][1])));
+                heavy = fmax3(heavy, ex2f_(x[n][u].x - at) * vs.x, ex2f_(x[n][u].y - at) * vs.y);
+              }
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) heavy = fmaxf(heavy, __shfl_xor_sync(0xffffffffu, heavy, d));
+              // the exponent that the row needs, which falls no faster than its sums do
+              int need = heavy > 0.f ? min(most, (int)(__float_as_uint(heavy) >> 23) - 127 + 12) : first ? vn : -127;
+              if (!first) need = max(need, ve - (int)was - (int)fminf(at - was, 256.f));
+              const int lift = vn > 100 || (first && !moves) ? 0 : min(max(vn - need, 0), kLift);
+              vtop = fminf(vtop, pow2(min(vn - lift, 126) + 1));
+              move(n, first && !moves ? 0.f : at - (float)lift);
+              if (!first || moves) limit[n] = kSlack + (float)lift;
+            }
           }
+          ve = vn;
+          vup = pow2(10 - vn);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)

@@ -67,3 +67,86 @@ def test_rows_of_a_failed_wait_are_nan_and_counted(H, kv, D, T):
     assert lost[90].all() and not lost[91].any()               # over many CTAs; without keys
     assert 0.2 < lost.double().mean() < 0.8
     assert torch.equal(ops.kv4_chord_attention(q, pool, table, ln, *pr), want) and _lib.wait_timeouts() == 0
+
+
+# ------------------------------------------------------------------ values far larger than those of weight
+def slots_of(table, lens, P):
+    """Slot of every cached token, request after request."""
+    out = []
+    for b, n in enumerate(lens):
+        pos = torch.arange(n, device='cuda')
+        out.append(table[b, (pos // P).long()] * P + pos % P)
+    return torch.cat(out).to(torch.int32)
+
+
+LAYOUTS = [(2, 2, 64, 2), (8, 2, 64, 2), (16, 2, 64, 2), (4, 2, 128, 2), (8, 4, 32, 2)]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('H,kv,D,T', LAYOUTS)
+@pytest.mark.parametrize('exponent', [14, 30, 60])
+def test_large_values_that_a_row_does_not_see(dtype, H, kv, D, T, exponent):
+    """The newest token's values are 2^exponent times as large as the others: the rows before it do not
+    see them, and keep the bar against their own largest output."""
+    lens, P = [80, 200, 64, 3], 16
+    pool, table, ln = random_cache(lens, kv, D, P, 19)
+    newest = slots_of(table, lens, P)[torch.tensor(lens, device='cuda').cumsum(0) - 1].contiguous()
+    g = gen(20)
+    k, v = (torch.randn(4, kv, D, device='cuda', generator=g) for _ in range(2))
+    ops.kv4_append(k, 2.0 ** exponent * v, newest, pool)
+    q = torch.randn(4, H, T, D, device='cuda', generator=g).to(dtype)
+    pr = params(H, 9)
+    out, ref = ops.kv4_chord_attention(q, pool, table, ln, *pr), attention_64(q, pool, table, ln, *pr)
+    for b in range(4):
+        for t in range(T - 1):
+            for h in range(H):
+                close(out[b, h, t], ref[b, h, t], dtype)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('H,kv,D,T', LAYOUTS)
+@pytest.mark.parametrize('at', ['first', 'middle'])
+def test_large_values_without_weight(dtype, H, kv, D, T, at):
+    """One key per request has values 2^30 times as large and, by the decay, a weight of 2^-200 at most.
+    Its neighbours (and their weights) change by steps of 2^-40 a key, so the reference moves on with
+    every tile."""
+    lens, P = [300, 200, 90, 131], 16
+    pool, table, ln = random_cache(lens, kv, D, P, 19)
+    starts = torch.tensor([0] + lens[:-1], device='cuda').cumsum(0)
+    which = slots_of(table, lens, P)[starts + (0 if at == 'first' else 70)].contiguous()
+    g = gen(21)
+    k, v = (torch.randn(4, kv, D, device='cuda', generator=g) for _ in range(2))
+    ops.kv4_append(k, 2.0 ** 30 * v, which, pool)
+    q = torch.randn(4, H, T, D, device='cuda', generator=g).to(dtype)
+    alpha, beta, mu, ssmax = (torch.full((H,), c, device='cuda') for c in (10.0, 1.0, 0.0, 0.7))
+    out = ops.kv4_chord_attention(q, pool, table, ln, alpha, beta, mu, ssmax)
+    ref = attention_64(q, pool, table, ln, alpha, beta, mu, ssmax)
+    for b in range(4):
+        for t in range(T):
+            for h in range(H):
+                close(out[b, h, t], ref[b, h, t], dtype)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('H,kv,D,T', LAYOUTS)
+def test_values_that_shrink_and_grow_along_the_cache(dtype, H, kv, D, T):
+    """Values of 2^-60 to 2^60 in turn, tile by tile, under no decay and under one that leaves the last keys
+    alone with a weight: every row keeps the bar against its own largest output."""
+    lens, P = [640, 300], 16
+    pool, table, ln = random_cache(lens, kv, D, P, 22)
+    g = gen(23)
+    n = sum(lens)
+    size = 2.0 ** (60.0 * torch.tensor([1.0, -1.0, 0.0, 0.9, -0.3, 0.4], device='cuda'))
+    where = torch.cat([torch.arange(x, device='cuda') for x in lens])
+    v = torch.randn(n, kv, D, device='cuda', generator=g) * size[(where // 50) % 6].view(n, 1, 1)
+    k = torch.randn(n, kv, D, device='cuda', generator=g)
+    ops.kv4_append(k, v, slots_of(table, lens, P), pool)
+    q = torch.randn(2, H, T, D, device='cuda', generator=g).to(dtype)
+    for a in (0.0, 20.0):
+        alpha, beta, mu, ssmax = (torch.full((H,), c, device='cuda') for c in (a, 1.0, 0.0, 0.5))
+        out = ops.kv4_chord_attention(q, pool, table, ln, alpha, beta, mu, ssmax)
+        ref = attention_64(q, pool, table, ln, alpha, beta, mu, ssmax)
+        for b in range(2):
+            for t in range(T):
+                for h in range(H):
+                    close(out[b, h, t], ref[b, h, t], dtype)
