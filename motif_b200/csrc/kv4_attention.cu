@@ -682,6 +682,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
         if (units != (1u << TU) - 1 || k0 + KT - 1 > lo_pos) {
           // keys that a row does not see weigh nothing; a slot that holds no token may hold any pair,
           // which must not meet the weight 0
+          float all = 0.f;
 #pragma unroll
           for (int u = 0; u < TU; ++u)
 #pragma unroll
@@ -692,9 +693,28 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
               for (int n = 0; n < NT; ++n)
                 if (!there || key > pos[n]) (e ? x[n][u].y : x[n][u].x) = -INFINITY;
 #pragma unroll
-              for (int g = 0; g < NG; ++g)
+              for (int g = 0; g < NG; ++g) {
                 if (!there || key >= len) vp[u][g][e] = 0u;
+                all += kv4::pair_scale(vp[u][g][e]) + kv4::pair_centre(vp[u][g][e]);
+              }
             }
+          if (!(fabsf(all) < INFINITY)) {
+            // nor may the pair of a group that is no number: it goes by itself to the sums of the rows that
+            // see its key
+#pragma unroll
+            for (int u = 0; u < TU; ++u)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                  const float any = kv4::pair_scale(vp[u][g][e]) + kv4::pair_centre(vp[u][g][e]);
+                  if (fabsf(any) < INFINITY) continue;
+                  vp[u][g][e] = 0u;
+#pragma unroll
+                  for (int n = 0; n < NT; ++n)
+                    if (k0 + u * kUnit + r0 + 8 * e <= pos[n]) (e ? pm[n][g].y : pm[n][g].x) += any;
+                }
+          }
         }
         float big = 0.f;
 #pragma unroll

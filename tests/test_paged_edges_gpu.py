@@ -150,3 +150,34 @@ def test_values_that_shrink_and_grow_along_the_cache(dtype, H, kv, D, T):
             for t in range(T):
                 for h in range(H):
                     close(out[b, h, t], ref[b, h, t], dtype)
+
+
+# ------------------------------------------------------------------ values that are no numbers
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('H,kv,D,T', [(2, 2, 64, 3), (8, 2, 64, 3), (16, 2, 64, 3), (4, 2, 128, 3), (8, 4, 32, 3)])
+@pytest.mark.parametrize('what', [float('nan'), float('inf')])
+def test_values_that_are_no_numbers_reach_the_rows_that_see_them(dtype, H, kv, D, T, what):
+    """The newest token holds a NaN or an infinity in its first group of dims: NaN in that group's outputs of
+    its own row, nothing in its other group's values, nothing in the rows before it."""
+    lens, P = [80, 17, 64, 3], 16
+    pool, table, ln = random_cache(lens, kv, D, P, 16)
+    clean = pool.clone()
+    newest = slots_of(table, lens, P)[torch.tensor(lens, device='cuda').cumsum(0) - 1].contiguous()
+    k, v = (torch.randn(4, kv, D, device='cuda', generator=gen(17)) for _ in range(2))
+    ops.kv4_append(k, v, newest, clean)
+    v[..., 5] = what
+    ops.kv4_append(k, v, newest, pool)
+    q = torch.randn(4, H, T, D, device='cuda', generator=gen(18)).to(dtype)
+    pr = params(H, 9)
+    out, ref = ops.kv4_chord_attention(q, pool, table, ln, *pr), attention_64(q, clean, table, ln, *pr)
+    first = min(D, 64)
+    close(out[:, :, :T - 1], ref[:, :, :T - 1], dtype)
+    assert out[:, :, T - 1, :first].isnan().all()
+    if D > first:
+        close(out[:, :, T - 1, first:], ref[:, :, T - 1, first:], dtype)
+    # a key that is no number is NaN in the row that sees it, and in no other
+    k[..., 5] = what
+    ops.kv4_append(k, torch.ones_like(k), newest, pool)
+    out = ops.kv4_chord_attention(q, pool, table, ln, *pr)
+    close(out[:, :, :T - 1], ref[:, :, :T - 1], dtype)
+    assert out[:, :, T - 1].isnan().all()
