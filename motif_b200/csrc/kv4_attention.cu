@@ -233,16 +233,17 @@ __device__ __forceinline__ float lg2_(float x) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 .. 127
 
-// x^b of a positive x for fp32 tensors: log2 x as a whole number e and log2 f of f = x 2^-e in 0.75 ..
-// 1.5, b e with its rounding error kept, and 2^(b log2 x) from the fraction of b e, so that the fast
-// logarithm's and power's errors (2^-22 absolute and relative) are all there is, however large log2 x.
+// x^b, b != 0, for fp32 tensors: log2 x as a whole number e and log2 f of f = x 2^-e in 0.75 .. 1.5, b e
+// with its rounding error kept, and 2^(b log2 x) from the fraction of b e, so that the fast logarithm's
+// and power's errors (2^-22 absolute and relative) are all there is, however large log2 x.  At x = 0 (no
+// eps, a key at mu) it is 0 or, for b < 0, infinite.
 __device__ __forceinline__ float power(float x, float b) {
   const int e = (int)(__float_as_uint(x) - 0x3f400000u) >> 23;
   const float f = __uint_as_float(__float_as_uint(x) - ((uint32_t)e << 23)), fe = (float)e;
   const float t = b * fe, lost = fmaf(b, fe, -t);
   const float n = rintf(t);
   const float y = ex2f_((t - n) + fmaf(b, lg2_(f), lost));
-  return y * pow2((int)fminf(fmaxf(n, -126.f), 127.f));
+  return x == 0.f ? (b > 0.f ? 0.f : INFINITY) : y * pow2((int)fminf(fmaxf(n, -126.f), 127.f));
 }
 
 // D = A B + C on fp16 operands with C in registers of its own.

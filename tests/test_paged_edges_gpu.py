@@ -181,3 +181,19 @@ def test_values_that_are_no_numbers_reach_the_rows_that_see_them(dtype, H, kv, D
     out = ops.kv4_chord_attention(q, pool, table, ln, *pr)
     close(out[:, :, :T - 1], ref[:, :, :T - 1], dtype)
     assert out[:, :, T - 1].isnan().all()
+
+
+# ------------------------------------------------------------------ the decay at distance 0
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('D', [32, 64, 128])
+def test_decay_of_a_key_at_distance_0(dtype, D):
+    """No eps and a whole mu: 0^beta is 0 however small beta is, and infinite for a negative one (its key
+    then weighs nothing)."""
+    H, kv, P = 8, 2, 16
+    pool, table, ln = random_cache([300, 40, 2], kv, D, P, 14)
+    q = torch.randn(3, H, 1, D, device='cuda', generator=gen(15)).to(dtype)
+    beta = torch.tensor([0.01, 0.02, 0.05, 0.1, 0.01, 0.05, -0.05, -0.5], device='cuda')
+    mu = torch.tensor([0.0, 0.0, 0.0, 0.0, -1.0, -3.0, 0.0, -1.0], device='cuda')
+    alpha, ssmax = torch.full((H,), 1.5, device='cuda'), torch.full((H,), 0.7, device='cuda')
+    out = ops.kv4_chord_attention(q, pool, table, ln, alpha, beta, mu, ssmax, eps=0.0)
+    close(out, attention_64(q, pool, table, ln, alpha, beta, mu, ssmax, eps=0.0), dtype)
