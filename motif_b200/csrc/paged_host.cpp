@@ -74,7 +74,7 @@ Pool pool(PyObject* o) {
   if (t.dim() == 4)
     for (int64_t d : {32, 64, 128})
       if (motif_b200_kv4_unit_bytes(d) == t.size(3)) dim = d;
-  if (t.scalar_type() != at::kByte || !dim || !t.is_contiguous())
+  if (t.scalar_type() != at::kByte || !dim || !t.numel() || !t.is_contiguous())
     refuse("pool must be a contiguous uint8 tensor from kv4_pool, got " + kind_of(t));
   return {t, t.size(0), t.size(1), t.size(2) * kUnit, dim};
 }

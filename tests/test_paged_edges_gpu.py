@@ -197,3 +197,17 @@ def test_decay_of_a_key_at_distance_0(dtype, D):
     alpha, ssmax = torch.full((H,), 1.5, device='cuda'), torch.full((H,), 0.7, device='cuda')
     out = ops.kv4_chord_attention(q, pool, table, ln, alpha, beta, mu, ssmax, eps=0.0)
     close(out, attention_64(q, pool, table, ln, alpha, beta, mu, ssmax, eps=0.0), dtype)
+
+
+# ------------------------------------------------------------------ refusals
+def test_pools_without_pages_heads_or_units_are_refused():
+    pool, table, ln = random_cache([20, 3], 2, 64, 16, 30)
+    q, p = torch.zeros(2, 4, 1, 64, device='cuda'), torch.zeros(4, device='cuda')
+    x, slots = torch.zeros(3, 2, 64, device='cuda'), torch.zeros(3, dtype=torch.int32, device='cuda')
+    for bad in (pool[:0], pool[:, :0], pool[:, :, :0]):
+        with pytest.raises(ValueError, match='pool must be'):
+            ops.kv4_chord_attention(q, bad, table, ln, p, p, p, p)
+        with pytest.raises(ValueError, match='pool must be'):
+            ops.kv4_append(x, x, slots, bad)
+        with pytest.raises(ValueError, match='pool must be'):
+            ops.kv4_gather(bad, table, ln, 20)
