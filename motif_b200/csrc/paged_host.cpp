@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -125,8 +126,10 @@ PyObject* tuple(std::initializer_list<at::Tensor> ts) {
   return out;
 }
 
+// No gradient is dropped without a word: neither a backward one nor a forward-mode tangent.
 void no_grad(const at::Tensor& t) {
-  if (t.requires_grad() && at::GradMode::is_enabled())
+  if ((t.requires_grad() && at::GradMode::is_enabled()) ||
+      (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()))
     throw Refusal{PyExc_NotImplementedError, "the 4-bit cache is forward-only (no autograd)"};
 }
 
@@ -253,7 +256,11 @@ PyObject* attention(PyObject* const* a) {
   const at::Tensor& lens = vector("lens", a[3], B, dev);
   const float* per_head[4];
   const char* names[4] = {"alpha", "beta", "mu", "ssmax"};
-  for (int i = 0; i < 4; ++i) per_head[i] = vector(names[i], a[4 + i], H, dev, at::kFloat).data_ptr<float>();
+  for (int i = 0; i < 4; ++i) {
+    const at::Tensor& t = vector(names[i], a[4 + i], H, dev, at::kFloat);
+    no_grad(t);
+    per_head[i] = t.data_ptr<float>();
+  }
   const int* q_lens = a[8] == Py_None ? nullptr : vector("q_lens", a[8], B, dev).data_ptr<int>();
   const double scale = a[9] == Py_None ? 1.0 / std::sqrt((double)p.dim) : number(a[9]), eps = number(a[10]);
   const c10::cuda::CUDAGuard guard(dev);

@@ -341,7 +341,7 @@ def _pack_decoder(dec: Decoder):
         w_down = dec.mlp.down_proj.weight.detach().contiguous()
         return _ChordPack(w_in=w_in, qn_w=a.q_norm.weight.detach().contiguous(),
                           kn_w=a.k_norm.weight.detach().contiguous(), w_o=w_o, w_down=w_down, alpha=al.contiguous(),
-                          beta=be.contiguous(), mu=mu.contiguous(), ssmax=a.ssmax_s.detach().float().contiguous(),
+                          beta=be.detach().contiguous(), mu=mu.contiguous(), ssmax=a.ssmax_s.detach().float().contiguous(),
                           H=a.num_heads, Hkv=a.num_kv_heads, D=a.head_dim, hid=hid, off_g=off_g,
                           off_gu=off_g + a.hidden_size, w_in_il=w_in_il, w_in_sk=_skinny_packed(w_in),
                           w_o_sk=_skinny_packed(w_o), w_down_sk=_skinny_packed(w_down))

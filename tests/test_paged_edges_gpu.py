@@ -211,3 +211,27 @@ def test_pools_without_pages_heads_or_units_are_refused():
             ops.kv4_append(x, x, slots, bad)
         with pytest.raises(ValueError, match='pool must be'):
             ops.kv4_gather(bad, table, ln, 20)
+
+
+def test_gradients_are_refused_and_not_dropped():
+    """Forward-only: an argument that asks for a gradient, or carries a forward-mode tangent, raises."""
+    pool, table, ln = random_cache([20, 3], 2, 64, 16, 30)
+    q, p = torch.zeros(2, 4, 1, 64, device='cuda'), torch.zeros(4, device='cuda')
+    x, slots = torch.zeros(3, 2, 64, device='cuda'), torch.full((3,), -1, dtype=torch.int32, device='cuda')
+    fwd = torch.autograd.forward_ad
+    for i in range(5):
+        a = [q, p, p, p, p]
+        a[i] = a[i].clone().requires_grad_()
+        with pytest.raises(NotImplementedError, match='forward-only'):
+            ops.kv4_chord_attention(a[0], pool, table, ln, *a[1:])
+        with torch.no_grad():
+            assert not ops.kv4_chord_attention(a[0], pool, table, ln, *a[1:]).requires_grad
+        with fwd.dual_level():
+            a[i] = fwd.make_dual(a[i].detach(), torch.ones_like(a[i]))
+            with pytest.raises(NotImplementedError, match='forward-only'):
+                ops.kv4_chord_attention(a[0], pool, table, ln, *a[1:])
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for k, v in ((dual, x), (x, dual)):
+            with pytest.raises(NotImplementedError, match='forward-only'):
+                ops.kv4_append(k, v, slots, pool)
