@@ -466,8 +466,8 @@ extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_
                                         int32_t* lens_out, int32_t* free_count_out, int32_t* slots, int64_t total_new,
                                         int64_t B, int64_t max_pages, int64_t free_capacity, int64_t page_size,
                                         void* stream) {
-  MB_REQUIRE(lens && new_lens && block_table && free_pages && free_count && lens_out && free_count_out &&
-                 (slots || total_new == 0),
+  MB_REQUIRE(((lens && new_lens && block_table && lens_out) || B == 0) && free_pages && free_count &&
+                 free_count_out && (slots || total_new == 0),
              MB_ERR_ARG, "paged_reserve: null pointer");
   if (int rc = check_paging("paged_reserve", B, max_pages, table_stride, page_size)) return rc;
   MB_REQUIRE(total_new >= 0 && total_new < (1ll << 31), MB_ERR_SHAPE, "paged_reserve: %lld new tokens",
@@ -508,10 +508,12 @@ extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_
 extern "C" int motif_b200_paged_release(const uint8_t* done, int32_t* lens, int32_t* block_table, int64_t table_stride,
                                         int32_t* free_pages, int32_t* free_count, int64_t B, int64_t max_pages,
                                         int64_t free_capacity, int64_t page_size, void* stream) {
-  MB_REQUIRE(done && lens && block_table && free_pages && free_count, MB_ERR_ARG, "paged_release: null pointer");
+  MB_REQUIRE(((done && lens && block_table) || B == 0) && free_pages && free_count, MB_ERR_ARG,
+             "paged_release: null pointer");
   if (int rc = check_paging("paged_release", B, max_pages, table_stride, page_size)) return rc;
   MB_REQUIRE(free_capacity >= 1 && free_capacity * page_size < (1ll << 31), MB_ERR_SHAPE,
              "paged_release: free list of %lld pages", (long long)free_capacity);
+  if (B == 0) return MB_OK;
   launch(paged_release_kernel, dim3(1), kReleaseThreads, 0, stream, done, lens, block_table, table_stride, free_pages,
          free_count, (int)B, (int)max_pages, free_capacity, (int)page_size);
   return check_launch("paged_release");

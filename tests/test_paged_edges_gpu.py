@@ -235,3 +235,18 @@ def test_gradients_are_refused_and_not_dropped():
         for k, v in ((dual, x), (x, dual)):
             with pytest.raises(NotImplementedError, match='forward-only'):
                 ops.kv4_append(k, v, slots, pool)
+
+
+# ------------------------------------------------------------------ batches without requests
+def test_a_batch_of_no_requests():
+    i32 = dict(dtype=torch.int32, device='cuda')
+    none, table = torch.empty(0, **i32), torch.empty((0, 4), **i32)
+    free, count = torch.arange(5, **i32), torch.tensor([5], **i32)
+    for total in (0, 3, 5000):
+        slots, lens, left = ops.paged_reserve(none, none, table, free, count, 16, total)
+        assert slots.tolist() == [-1] * total and lens.shape == (0,) and left.tolist() == [5]
+        slots, lens, left = ops.paged_reserve(none, none, table, free, count, 16, total, lens_out=none,
+                                              free_count_out=count)
+        assert slots.tolist() == [-1] * total and count.tolist() == [5]
+    ops.paged_release(torch.empty(0, dtype=torch.bool, device='cuda'), none, table, free, count, 16)
+    assert count.tolist() == [5] and free.tolist() == list(range(5))
