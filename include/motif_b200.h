@@ -533,8 +533,8 @@ MB_API int motif_b200_embed(const int64_t* ids, const void* table, void* out, in
 
 /* Slots for new_lens[b] more tokens of each request (lens[b] cached): fresh pages are taken from
  * the end of free_pages[:*free_count] (capacity free_capacity) in request order and written to
- * block_table; slots[total_new] gets every new token's slot, request after request, -1 past the
- * last token and for requests that were not served.  A request is served if its pages fit
+ * block_table; slots[total_new] (at most 2^31 - 2^20) gets every new token's slot, request after
+ * request, -1 past the last token and for requests that were not served.  A request is served if its pages fit
  * max_pages, its tokens fit total_new and the pages asked for up to and including it do not exceed
  * the free ones (one that needs no page always passes the last test).  lens_out[b] = lens[b] +
  * new_lens[b] where served, else lens[b]; lens_out / free_count_out may be lens / free_count. */

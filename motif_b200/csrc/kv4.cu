@@ -470,8 +470,9 @@ extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_
                  free_count_out && (slots || total_new == 0),
              MB_ERR_ARG, "paged_reserve: null pointer");
   if (int rc = check_paging("paged_reserve", B, max_pages, table_stride, page_size)) return rc;
-  MB_REQUIRE(total_new >= 0 && total_new < (1ll << 31), MB_ERR_SHAPE, "paged_reserve: %lld new tokens",
-             (long long)total_new);
+  // the kernel counts tokens in 32 bits and looks up to a page, and up to eight tokens a thread, ahead
+  MB_REQUIRE(total_new >= 0 && total_new <= (1ll << 31) - (1 << 20), MB_ERR_SHAPE,
+             "paged_reserve: %lld new tokens (0 .. 2^31 - 2^20)", (long long)total_new);
   MB_REQUIRE(free_capacity >= 1 && free_capacity * page_size < (1ll << 31), MB_ERR_SHAPE,
              "paged_reserve: free list of %lld pages", (long long)free_capacity);
   const PageDiv by = page_div(page_size);
