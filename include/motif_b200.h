@@ -528,8 +528,8 @@ MB_API int motif_b200_embed(const int64_t* ids, const void* table, void* out, in
  *   K codes [16][D/2] | V codes [16][D/2] | K pairs [D/DG][16] | V pairs [D/DG][16], DG = min(D, 64).
  * Dim 2i of a row is the low nibble of byte i; a group of DG dims of one token has a pair (scale s,
  * centre m) in bf16, s in the low half of its 32-bit word; code c stands for m + s (c - 8).
- * block_table [B, max_pages] int32 (row stride table_stride) names each request's pages; slot
- * numbers are page * page_size + offset.  D in {32, 64, 128}.  No counterpart in the reference. */
+ * block_table [B, max_pages] int32 (row stride table_stride; max_pages * page_size at most 2^31 - 1024)
+ * names each request's pages; slot numbers are page * page_size + offset.  D in {32, 64, 128}.  No counterpart in the reference. */
 
 /* Slots for new_lens[b] more tokens of each request (lens[b] cached): fresh pages are taken from
  * the end of free_pages[:*free_count] (capacity free_capacity) in request order and written to

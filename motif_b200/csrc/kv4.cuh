@@ -109,8 +109,10 @@ inline int check_paging(const char* who, int64_t B, int64_t columns, int64_t ts,
              (long long)columns, (long long)ts);
   MB_REQUIRE(P >= kUnit && P <= 1024 && P % kUnit == 0, MB_ERR_ARG, "%s: page size %lld (a multiple of 16, at most 1024)",
              who, (long long)P);
-  MB_REQUIRE(columns * P < (1ll << 31), MB_ERR_SHAPE, "%s: a request could hold %lld tokens (fewer than 2^31)", who,
-             (long long)(columns * P));
+  // the attention's 32-bit token numbers run up to a tile past the last one
+  MB_REQUIRE(columns <= (1 << 27) && columns * P <= (1ll << 31) - 1024, MB_ERR_SHAPE,
+             "%s: a request could hold %lld pages of %lld tokens (fewer than 2^31 - 1023 tokens)", who, (long long)columns,
+             (long long)P);
   return MB_OK;
 }
 inline int check_pool(const char* who, const void* pool, int64_t pages, int64_t Hkv, int64_t P) {
