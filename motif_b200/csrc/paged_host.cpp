@@ -139,6 +139,12 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
   return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
 }
 
+// Other Python threads run while a call allocates and launches (a launch waits where the queue is full).
+struct NoGil {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~NoGil() { PyEval_RestoreThread(state); }
+};
+
 // ------------------------------------------------------------------ the calls
 PyObject* reserve(PyObject* const* a) {
   const at::Tensor& lens = lengths(a[0]);
@@ -152,15 +158,22 @@ PyObject* reserve(PyObject* const* a) {
   const at::Tensor& count = vector("free_count", a[4], 1, dev);
   const int64_t page_size = whole(a[5]), total = whole(a[6]);
   if (total < 0) refuse("total_new must not be negative, got " + std::to_string(total));
-  const c10::cuda::CUDAGuard guard(dev);
-  const at::Tensor lens_out = a[7] == Py_None ? fresh({B}, at::kInt, dev) : vector("lens_out", a[7], B, dev);
-  const at::Tensor count_out = a[8] == Py_None ? fresh({1}, at::kInt, dev) : vector("free_count_out", a[8], 1, dev);
-  const at::Tensor slots = a[9] == Py_None ? fresh({total}, at::kInt, dev) : vector("slots", a[9], total, dev);
-  check("motif_b200_paged_reserve",
-        motif_b200_paged_reserve(lens.data_ptr<int>(), added.data_ptr<int>(), tab.data_ptr<int>(), tab.stride(0),
-                                 free.data_ptr<int>(), count.data_ptr<int>(), lens_out.data_ptr<int>(),
-                                 count_out.data_ptr<int>(), slots.data_ptr<int>(), total, B, tab.size(1), free.numel(),
-                                 page_size, stream_of(dev)));
+  at::Tensor lens_out, count_out, slots;
+  if (a[7] != Py_None) lens_out = vector("lens_out", a[7], B, dev);
+  if (a[8] != Py_None) count_out = vector("free_count_out", a[8], 1, dev);
+  if (a[9] != Py_None) slots = vector("slots", a[9], total, dev);
+  {
+    const NoGil others;
+    const c10::cuda::CUDAGuard guard(dev);
+    if (!lens_out.defined()) lens_out = fresh({B}, at::kInt, dev);
+    if (!count_out.defined()) count_out = fresh({1}, at::kInt, dev);
+    if (!slots.defined()) slots = fresh({total}, at::kInt, dev);
+    check("motif_b200_paged_reserve",
+          motif_b200_paged_reserve(lens.data_ptr<int>(), added.data_ptr<int>(), tab.data_ptr<int>(), tab.stride(0),
+                                   free.data_ptr<int>(), count.data_ptr<int>(), lens_out.data_ptr<int>(),
+                                   count_out.data_ptr<int>(), slots.data_ptr<int>(), total, B, tab.size(1),
+                                   free.numel(), page_size, stream_of(dev)));
+  }
   return tuple({slots, lens_out, count_out});
 }
 
@@ -174,11 +187,15 @@ PyObject* release(PyObject* const* a) {
   const at::Tensor& free = on("free_pages", a[3], dev);
   vector("free_pages", a[3], free.numel(), dev);
   const at::Tensor& count = vector("free_count", a[4], 1, dev);
-  const c10::cuda::CUDAGuard guard(dev);
-  check("motif_b200_paged_release",
-        motif_b200_paged_release(static_cast<const uint8_t*>(done.data_ptr()), lens.data_ptr<int>(),
-                                 tab.data_ptr<int>(), tab.stride(0), free.data_ptr<int>(), count.data_ptr<int>(), B,
-                                 tab.size(1), free.numel(), whole(a[5]), stream_of(dev)));
+  const int64_t page_size = whole(a[5]);
+  {
+    const NoGil others;
+    const c10::cuda::CUDAGuard guard(dev);
+    check("motif_b200_paged_release",
+          motif_b200_paged_release(static_cast<const uint8_t*>(done.data_ptr()), lens.data_ptr<int>(),
+                                   tab.data_ptr<int>(), tab.stride(0), free.data_ptr<int>(), count.data_ptr<int>(), B,
+                                   tab.size(1), free.numel(), page_size, stream_of(dev)));
+  }
   Py_RETURN_NONE;
 }
 
@@ -200,24 +217,27 @@ PyObject* append(PyObject* const* a) {
   const int dc = dtype_code(k0.scalar_type());
   const int values = PyObject_IsTrue(a[4]);
   if (values < 0) throw Refusal{nullptr, ""};
-  const c10::cuda::CUDAGuard guard(dev);
-  const at::Tensor k = rows16(k0), v = rows16(v0);
   at::Tensor ko, vo;
-  if (values) {
-    ko = fresh(k.sizes(), k.scalar_type(), dev);
-    vo = fresh(k.sizes(), k.scalar_type(), dev);
+  {
+    const NoGil others;
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor k = rows16(k0), v = rows16(v0);
+    if (values) {
+      ko = fresh(k.sizes(), k.scalar_type(), dev);
+      vo = fresh(k.sizes(), k.scalar_type(), dev);
+    }
+    int64_t strides[12] = {0};
+    const at::Tensor* ts[4] = {&k, &v, &ko, &vo};
+    for (int i = 0; i < (values ? 4 : 2); ++i) {
+      strides[3 * i] = flat ? 0 : ts[i]->stride(0);
+      strides[3 * i + 1] = ts[i]->stride(1);
+      strides[3 * i + 2] = ts[i]->stride(flat ? 0 : 2);
+    }
+    check("motif_b200_kv4_append",
+          motif_b200_kv4_append(k.data_ptr(), v.data_ptr(), slots.data_ptr<int>(), p.t.data_ptr(),
+                                values ? ko.data_ptr() : nullptr, values ? vo.data_ptr() : nullptr, strides, B, T, p.kv,
+                                p.dim, p.pages, p.page_size, dc, stream_of(dev)));
   }
-  int64_t strides[12] = {0};
-  const at::Tensor* ts[4] = {&k, &v, &ko, &vo};
-  for (int i = 0; i < (values ? 4 : 2); ++i) {
-    strides[3 * i] = flat ? 0 : ts[i]->stride(0);
-    strides[3 * i + 1] = ts[i]->stride(1);
-    strides[3 * i + 2] = ts[i]->stride(flat ? 0 : 2);
-  }
-  check("motif_b200_kv4_append",
-        motif_b200_kv4_append(k.data_ptr(), v.data_ptr(), slots.data_ptr<int>(), p.t.data_ptr(),
-                              values ? ko.data_ptr() : nullptr, values ? vo.data_ptr() : nullptr, strides, B, T, p.kv,
-                              p.dim, p.pages, p.page_size, dc, stream_of(dev)));
   if (!values) Py_RETURN_NONE;
   return tuple({ko, vo});
 }
@@ -233,11 +253,16 @@ PyObject* gather(PyObject* const* a) {
   if (!THPDtype_Check(a[4])) refuse("dtype must be a torch.dtype");
   const at::ScalarType type = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
   const int dc = dtype_code(type);
-  const c10::cuda::CUDAGuard guard(dev);
-  const at::Tensor k = fresh({B, p.kv, S, p.dim}, type, dev), v = fresh({B, p.kv, S, p.dim}, type, dev);
-  check("motif_b200_kv4_gather",
-        motif_b200_kv4_gather(p.t.data_ptr(), tab.data_ptr<int>(), tab.stride(0), lens.data_ptr<int>(), k.data_ptr(),
-                              v.data_ptr(), B, p.kv, S, p.dim, p.pages, p.page_size, tab.size(1), dc, stream_of(dev)));
+  at::Tensor k, v;
+  {
+    const NoGil others;
+    const c10::cuda::CUDAGuard guard(dev);
+    k = fresh({B, p.kv, S, p.dim}, type, dev), v = fresh({B, p.kv, S, p.dim}, type, dev);
+    check("motif_b200_kv4_gather",
+          motif_b200_kv4_gather(p.t.data_ptr(), tab.data_ptr<int>(), tab.stride(0), lens.data_ptr<int>(), k.data_ptr(),
+                                v.data_ptr(), B, p.kv, S, p.dim, p.pages, p.page_size, tab.size(1), dc,
+                                stream_of(dev)));
+  }
   return tuple({k, v});
 }
 
@@ -263,17 +288,22 @@ PyObject* attention(PyObject* const* a) {
   }
   const int* q_lens = a[8] == Py_None ? nullptr : vector("q_lens", a[8], B, dev).data_ptr<int>();
   const double scale = a[9] == Py_None ? 1.0 / std::sqrt((double)p.dim) : number(a[9]), eps = number(a[10]);
-  const c10::cuda::CUDAGuard guard(dev);
-  const at::Tensor q = rows16(q0), out = fresh(q.sizes(), q.scalar_type(), dev);
-  const int64_t bytes = motif_b200_kv4_attention_workspace_bytes(H, p.kv, T, p.dim);
-  const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes);
-  const int64_t strides[6] = {q.stride(0), q.stride(1), q.stride(2), out.stride(0), out.stride(1), out.stride(2)};
-  check("motif_b200_kv4_chord_attention",
-        motif_b200_kv4_chord_attention(q.data_ptr(), p.t.data_ptr(), tab.data_ptr<int>(), tab.stride(0),
-                                       lens.data_ptr<int>(), q_lens, per_head[0], per_head[1], per_head[2],
-                                       per_head[3], out.data_ptr(), strides, B, H, p.kv, T, p.dim, p.pages,
-                                       p.page_size, tab.size(1), (float)scale, (float)eps, ws.get(), bytes, dc,
-                                       stream_of(dev)));
+  at::Tensor out;
+  {
+    const NoGil others;
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor q = rows16(q0);
+    out = fresh(q.sizes(), q.scalar_type(), dev);
+    const int64_t bytes = motif_b200_kv4_attention_workspace_bytes(H, p.kv, T, p.dim);
+    const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes);
+    const int64_t strides[6] = {q.stride(0), q.stride(1), q.stride(2), out.stride(0), out.stride(1), out.stride(2)};
+    check("motif_b200_kv4_chord_attention",
+          motif_b200_kv4_chord_attention(q.data_ptr(), p.t.data_ptr(), tab.data_ptr<int>(), tab.stride(0),
+                                         lens.data_ptr<int>(), q_lens, per_head[0], per_head[1], per_head[2],
+                                         per_head[3], out.data_ptr(), strides, B, H, p.kv, T, p.dim, p.pages,
+                                         p.page_size, tab.size(1), (float)scale, (float)eps, ws.get(), bytes, dc,
+                                         stream_of(dev)));
+  }
   return wrap(out);
 }
 

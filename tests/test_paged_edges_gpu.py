@@ -4,6 +4,9 @@ calls take, each against the definition in 64 bits (or a plain loop).
 Bars are those of `test_paged_gpu.py` unless a test derives its own.
 """
 
+import threading
+import time
+
 import pytest
 import torch
 
@@ -250,3 +253,37 @@ def test_a_batch_of_no_requests():
         assert slots.tolist() == [-1] * total and count.tolist() == [5]
     ops.paged_release(torch.empty(0, dtype=torch.bool, device='cuda'), none, table, free, count, 16)
     assert count.tolist() == [5] and free.tolist() == list(range(5))
+
+
+# ------------------------------------------------------------------ other threads
+def test_other_python_threads_run_while_a_launch_waits():
+    """The GPU is kept busy for about a second and the launch queue (some thousand launches) filled
+    behind it: a call then waits in its launch, and meanwhile another Python thread goes on."""
+    pool, table, ln = random_cache([20, 3], 2, 64, 16, 30)
+    x = torch.randn(3, 2, 64, device='cuda', generator=gen(31))
+    slots = torch.full((3,), -1, dtype=torch.int32, device='cuda')
+    ops.kv4_append(x, x, slots, pool)
+    torch.cuda.synchronize()
+    longest, stop = [0.0], threading.Event()
+
+    def watch():
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            longest[0], last = max(longest[0], now - last), now
+
+    thread = threading.Thread(target=watch)
+    thread.start()
+    try:
+        torch.cuda._sleep(2_000_000_000)  # cycles of at most 1.965 GHz
+        begin = time.perf_counter()
+        for _ in range(6000):
+            ops.kv4_append(x, x, slots, pool)
+        waited = time.perf_counter() - begin
+    finally:
+        stop.set()
+        thread.join()
+        torch.cuda.synchronize()
+    assert waited > 0.7, 'the launches did not fill the queue'
+    assert longest[0] < 0.35
