@@ -1,12 +1,13 @@
 """Build `libmotif_b200.so` (all CUDA kernels + the C ABI) in-tree for sm_100a, and `_paged_host.so`
 (the compiled Python entry points of the paged cache, on the same C ABI) beside it.
 
-    python -m motif_b200.build [--force] [--jobs N]
+    python -m motif_b200.build [--force] [--jobs N] [--lib-only]
 
 Each `csrc/*.cu` is compiled to an object in `_build/` with
 `-gencode arch=compute_100a,code=sm_100a`, then linked into
 `motif_b200/libmotif_b200.so` next to this file.  Rebuilds only when a source or
-header is newer than the library (the host module: its source or the C header).
+header is newer than the library (the host module: its source or the C header).  A user of the C ABI
+alone needs neither Python's headers nor a C++ compiler for torch's: `--lib-only` leaves the module out.
 """
 
 import argparse
@@ -81,13 +82,15 @@ def _build_host(force: bool) -> None:
     os.replace(tmp, HOST)
 
 
-def build(force: bool = False, jobs: int = 0, verbose: bool = False) -> str:
-    """Compile every kernel and link the shared library and the host module; returns the library's path."""
+def build(force: bool = False, jobs: int = 0, verbose: bool = False, host: bool = True) -> str:
+    """Compile every kernel and link the shared library and (with `host`) the host module; returns the
+    library's path."""
     if force or _stale():
         _build_lib(jobs)
         if verbose:
             print(f'built {LIB}')
-    _build_host(force)
+    if host:
+        _build_host(force)
     return LIB
 
 
@@ -109,8 +112,9 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument('--force', action='store_true')
     ap.add_argument('--jobs', type=int, default=0)
+    ap.add_argument('--lib-only', action='store_true')
     a = ap.parse_args()
-    build(force=a.force, jobs=a.jobs, verbose=True)
+    build(force=a.force, jobs=a.jobs, verbose=True, host=not a.lib_only)
 
 
 if __name__ == '__main__':
