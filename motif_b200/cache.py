@@ -228,9 +228,11 @@ class KV4LayerCache(KVLayerCache):
         self.length += T
         return out
 
-    def gather(self):
-        """The cached keys and values, `[B, H_kv, length, D]` in the dtype they came in."""
-        return kv4_gather(self.pool, self.pages.table, self.pages.lens, self.length, dtype=self.dtype)
+    def gather(self, dtype: Optional[torch.dtype] = None):
+        """The cached keys and values, `[B, H_kv, length, D]` in `dtype` (the one they came in, or that
+        `to` has set)."""
+        return kv4_gather(self.pool, self.pages.table, self.pages.lens, self.length,
+                          dtype=self.dtype if dtype is None else dtype)
 
     @property
     def k(self) -> Optional[torch.Tensor]:

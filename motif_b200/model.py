@@ -908,7 +908,7 @@ def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache
                                            cache.pages.lens, pk.alpha, pk.beta, pk.mu, pk.ssmax, softmax_scale=scale,
                                            eps=GGD_EPS).transpose(1, 2).reshape(M, d)
             else:
-                kv = cache.gather()
+                kv = cache.gather(dt)  # the layer's own dtype may be another one (`to`)
     elif cache.wide:
         # a wide cache (`cache.py:42-70`) stores every key / value head once per query head: the
         # new keys / values are prepared narrow, widened by the cache's own update, and the
