@@ -177,24 +177,23 @@ class KV4Pages:
             raise ValueError(f'the cache holds {self.batch} requests on {self.lens.device}, got {batch} on {device}')
 
     def take(self, start: int, tokens: int) -> torch.Tensor:
-        """Slots of `tokens` more tokens of every request behind the first `start`; the first layer
-        that asks reserves them, the others get the same ones."""
-        if start == self.length:
+        """Slots of `tokens` more tokens of every request behind the first `start`.  Those past the shared
+        length are reserved by the first layer that asks, the others find them in the table."""
+        more = start + tokens - self.length
+        if more > 0:
             if start + tokens > self.capacity:
                 raise ValueError(f'{start + tokens} tokens exceed the cache capacity of {self.capacity}')
-            if self._new is None or self._new[0] != tokens:
-                self._new = (tokens, torch.full_like(self.lens, tokens))
+            if self._new is None or self._new[0] != more:
+                self._new = (more, torch.full_like(self.lens, more))
             self.slots, _, _ = paged_reserve(self.lens, self._new[1], self.table, self.free, self.count,
-                                             self.page_size, self.batch * tokens, lens_out=self.lens,
+                                             self.page_size, self.batch * more, lens_out=self.lens,
                                              free_count_out=self.count)
-            self.length += tokens
-            self._at = (start, tokens)
-        elif start + tokens > self.length:
-            raise ValueError(f'the Chord layers disagree on length: {start} + {tokens} against {self.length}')
-        elif self._at != (start, tokens):  # a layer that lags by more than the newest tokens
-            pos = torch.arange(start, start + tokens, device=self.table.device)
-            return (self.table[:, pos // self.page_size] * self.page_size + (pos % self.page_size).int()).view(-1)
-        return self.slots
+            self._at = (self.length, more)
+            self.length += more
+        if self._at == (start, tokens):
+            return self.slots
+        pos = torch.arange(start, start + tokens, device=self.table.device)
+        return (self.table[:, pos // self.page_size] * self.page_size + (pos % self.page_size).int()).view(-1)
 
     def to(self, device):
         for n in ('table', 'lens', 'free', 'count', 'slots'):

@@ -66,6 +66,9 @@ def _check_layer_caches(model, cache: ModelCache, B: int, need: int):
                 if isinstance(lc, KV4LayerCache) and lc.pool is not None:
                     if lc.pages.batch != B:
                         raise ValueError(f'block {b} decoder {i}: KV cache batch mismatch')
+                    if lc.length != lc.pages.length:
+                        raise ValueError(f'block {b} decoder {i}: the layer holds {lc.length} tokens of the '
+                                         f'{lc.pages.length} that the shared pages have')
                     lc.reserve(need)
                     kv.append(lc)
                     continue

@@ -903,7 +903,8 @@ def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache
         else:
             cache.append(kt, vt)
             direct = G * T <= KV4_DIRECT_ROWS or B * G * T <= KV4_DIRECT_ROWS_IN_ALL
-            if direct and key_bias is None and q_start == cached:
+            # a layer behind the shared lengths (a forward that stopped between two layers) reads its own
+            if direct and key_bias is None and q_start == cached and cache.length == cache.pages.length:
                 attn = kv4_chord_attention(qb.view(B, T, H, D).transpose(1, 2), cache.pool, cache.pages.table,
                                            cache.pages.lens, pk.alpha, pk.beta, pk.mu, pk.ssmax, softmax_scale=scale,
                                            eps=GGD_EPS).transpose(1, 2).reshape(M, d)

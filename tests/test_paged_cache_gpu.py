@@ -7,6 +7,8 @@ Models, the cache of rounded values and the bar are those of `test_paged_model_g
 import pytest
 import torch
 
+from motif_b200 import model as engine
+from motif_b200.decode import GraphDecoder
 from test_paged_model_gpu import close, model_of, rounded_cache
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +34,31 @@ def test_cache_of_another_dtype_is_read_back_in_the_models(other):
             if hasattr(lc, 'pages'):
                 lc.to(dtype=other)
     close(m(ids[:, 20:], cache=cache, mask=mask).logits, m(ids[:, 20:], cache=ref, mask=mask).logits)
+
+
+@pytest.mark.parametrize('stopped,chunks', [(2, [1, 1, 1]), (1, [2, 1, 3]), (5, [1, 1, 8, 1]), (3, [3, 1])])
+def test_layers_of_unequal_length_attend_to_their_own_tokens(monkeypatch, stopped, chunks):
+    """A forward that stops between two Chord layers leaves the first one ahead; what follows is what two
+    layers of separate caches give."""
+    m = model_of(torch.float32, block=('chord', 'gdn', 'chord'))
+    ids = ids_of(2, 60, 5)
+    cache, ref = m.create_cache(kv_bits=4, kv_capacity=64, page_size=16), rounded_cache(m)
+
+    def stop(*a):
+        raise RuntimeError('stopped')
+
+    for c in (cache, ref):
+        m(ids[:, :20], cache=c)
+        with monkeypatch.context() as p, pytest.raises(RuntimeError, match='stopped'):
+            p.setattr(engine, '_gdn_decoder', stop)
+            m(ids[:, 20:20 + stopped], cache=c)
+        c[0].attn_res.seq_len = 20
+    first, last = cache[0].attn[0], cache[0].attn[2]
+    assert (first.length, last.length, first.pages.length) == (20 + stopped, 20, 20 + stopped)
+    with pytest.raises(ValueError, match='shared pages|disagree'):
+        GraphDecoder(m, cache, max_steps=2)
+    at = 20
+    for n in chunks:
+        close(m(ids[:, at:at + n], cache=cache).logits, m(ids[:, at:at + n], cache=ref).logits)
+        at += n
+    assert (first.length, last.length) == (at + stopped, at) and torch.equal(last.k, ref[0].attn[2].k[:, ::2])
