@@ -19,7 +19,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from .paged import kv4_append, kv4_gather, kv4_pool, paged_reserve
+from .paged import check_head_dim, check_page_size, kv4_append, kv4_gather, kv4_pool, paged_reserve
 
 
 class BasicLayerCache:
@@ -148,6 +148,7 @@ class KV4Pages:
     def __init__(self, capacity: int, page_size: int = 64):
         if capacity < 1:
             raise ValueError(f'capacity must be positive, got {capacity}')
+        check_page_size(page_size)
         self.capacity_asked = int(capacity)
         self.page_size = int(page_size)
         self.columns = -(-self.capacity_asked // self.page_size)
@@ -215,6 +216,12 @@ class KV4LayerCache(KVLayerCache):
     @property
     def capacity(self) -> int:
         return self.pages.capacity
+
+    def expect(self, batch: int, tokens: int, device):
+        """Refuse what `append` would refuse of `tokens` more tokens of `batch` requests, before anything of
+        a forward has run."""
+        self.reserve(self.length + tokens)
+        self.pages.bind(batch, device)
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, values: bool = False):
         """Store `[B, H_kv, T, D]` keys / values; with `values`, return what the stored bits stand for."""
@@ -483,6 +490,7 @@ def build_cache(model, use_attn: Optional[bool] = None, functional: bool = False
             raise ValueError('kv_bits=4 needs kv_capacity, the most tokens a request may cache')
         if functional or wide_kv or use_attn is False:
             raise ValueError('kv_bits=4 goes with neither functional, wide_kv nor use_attn=False')
+        check_head_dim(model.config.head_dim)
         pages, use_attn = KV4Pages(kv_capacity, page_size), True
     if use_attn is None:
         use_attn = not getattr(model, 'training', False)

@@ -713,6 +713,10 @@ def _forward(model: MotifChordModel, ids: torch.Tensor, cache: ModelCache, posit
     dc = _lib.dtype_code(dt)
     st = _lib.stream_ptr(dev)
     ids = ids.contiguous()
+    for bc in cache:  # a cache of fixed capacity refuses before any layer has advanced
+        for lc in bc.attn:
+            if isinstance(lc, KV4LayerCache):
+                lc.expect(B, T, dev)
 
     x = torch.empty((M, d), dtype=dt, device=dev)
     _lib.call('motif_b200_embed', _lib.ptr(ids), _lib.ptr(w), _lib.ptr(x), M, d, cfg.vocab_size, dc, st)

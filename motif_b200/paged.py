@@ -32,13 +32,21 @@ UNIT = 16  # tokens of one storage unit: page sizes are multiples of it
 _UNIT_BYTES = {32: 640, 64: 1152, 128: 2304}  # motif_b200_kv4_unit_bytes
 
 
+def check_head_dim(head_dim: int) -> None:
+    if head_dim not in _UNIT_BYTES:
+        raise NotImplementedError(f'head_dim must be 32, 64 or 128, got {head_dim}')
+
+
+def check_page_size(page_size: int) -> None:
+    if page_size < UNIT or page_size % UNIT or page_size > 1024:
+        raise ValueError(f'page_size must be a multiple of {UNIT} up to 1024, got {page_size}')
+
+
 def kv4_pool(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 64, device='cuda') -> torch.Tensor:
     """An empty pool `[num_pages, num_kv_heads, page_size / 16, unit bytes]` (uint8): its shape
     carries the page size and the head dim (32, 64 or 128) for the calls below."""
-    if head_dim not in _UNIT_BYTES:
-        raise NotImplementedError(f'head_dim must be 32, 64 or 128, got {head_dim}')
-    if page_size < UNIT or page_size % UNIT or page_size > 1024:
-        raise ValueError(f'page_size must be a multiple of {UNIT} up to 1024, got {page_size}')
+    check_head_dim(head_dim)
+    check_page_size(page_size)
     if num_pages < 1 or num_kv_heads < 1:
         raise ValueError(f'num_pages and num_kv_heads must be positive, got {num_pages}, {num_kv_heads}')
     return torch.zeros((num_pages, num_kv_heads, page_size // UNIT, _UNIT_BYTES[head_dim]), dtype=torch.uint8,

@@ -62,3 +62,21 @@ def test_layers_of_unequal_length_attend_to_their_own_tokens(monkeypatch, stoppe
         close(m(ids[:, at:at + n], cache=cache).logits, m(ids[:, at:at + n], cache=ref).logits)
         at += n
     assert (first.length, last.length) == (at + stopped, at) and torch.equal(last.k, ref[0].attn[2].k[:, ::2])
+
+
+def test_a_refused_forward_leaves_the_cache_as_it_was():
+    """Capacity and batch are checked before any layer advances (the recurrent layers before the first
+    Chord layer could not be taken back)."""
+    m = model_of(torch.float32, block=('gdn', 'chord'), block_n=2)
+    ids = ids_of(2, 40, 6)
+    cache, whole = (m.create_cache(kv_bits=4, kv_capacity=n, page_size=16) for n in (32, 64))
+    for c in (cache, whole):
+        m(ids[:, :30], cache=c)
+    for bad, match in ((ids[:, 30:33], 'capacity'), (ids[:1, 30:31], '2 requests'), (ids[:, :33], 'capacity')):
+        with pytest.raises(ValueError, match=match):
+            m(bad, cache=cache)
+    assert cache.seq_len == 30
+    assert torch.equal(m(ids[:, 30:32], cache=cache).logits, m(ids[:, 30:32], cache=whole).logits)
+    with pytest.raises(ValueError, match='capacity'):
+        m(ids[:, 32:33], cache=cache)
+    assert cache.seq_len == 32 and all(lc.length == 32 for bc in cache for lc in bc.attn)

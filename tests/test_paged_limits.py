@@ -3,6 +3,8 @@
 import pytest
 
 from motif_b200 import _lib
+from motif_b200.config import MotifChordConfig
+from motif_b200.model import MotifChordModel
 
 ADDR = 4096  # a non-null, aligned stand-in: these calls fail before any use of it
 
@@ -23,3 +25,20 @@ def test_tables_whose_tokens_pass_32_bits_are_refused(page, columns):
                        ('motif_b200_paged_release', (ADDR, ADDR, ADDR, columns, ADDR, ADDR, 2, columns, 8, page, None))):
         with pytest.raises(ValueError, match='fewer than 2'):
             _lib.call(name, *args)
+
+
+def test_a_cache_that_cannot_be_kept_is_refused_when_it_is_made():
+    """Page size, capacity and head dim, not at the first Chord layer of a forward."""
+    def model(heads):
+        return MotifChordModel(MotifChordConfig(vocab_size=64, model_dim=128, num_heads=heads, num_kv_heads=1, head_k_dim=64,
+                                                block=('gdn', 'chord'), block_n=1))
+
+    m = model(2)
+    for page in (0, 8, 24, 40, 2048, -16):
+        with pytest.raises(ValueError, match='page_size'):
+            m.create_cache(kv_bits=4, kv_capacity=100, page_size=page)
+    with pytest.raises(ValueError, match='capacity'):
+        m.create_cache(kv_bits=4, kv_capacity=0)
+    with pytest.raises(NotImplementedError, match='head_dim'):
+        model(8).create_cache(kv_bits=4, kv_capacity=100)
+    assert m.create_cache(kv_bits=4, kv_capacity=100, page_size=48)[0].attn[1].capacity == 144
