@@ -152,6 +152,7 @@ class KV4Pages:
         self.capacity_asked = int(capacity)
         self.page_size = int(page_size)
         self.columns = -(-self.capacity_asked // self.page_size)
+        self.layers: List['KV4LayerCache'] = []
         self.reset()
 
     def reset(self):
@@ -210,6 +211,7 @@ class KV4LayerCache(KVLayerCache):
     def __init__(self, pages: KV4Pages):
         super().__init__()
         self.pages = pages
+        pages.layers.append(self)
         self.pool: Optional[torch.Tensor] = None
         self.dtype: Optional[torch.dtype] = None
 
@@ -259,9 +261,11 @@ class KV4LayerCache(KVLayerCache):
         return self.gather()
 
     def reset(self):
+        """Empty this layer; the pages are given back with the last layer that holds any."""
         super().reset()
         self.pool = None
-        self.pages.reset()
+        if all(lc.pool is None for lc in self.pages.layers):
+            self.pages.reset()
 
     def to(self, device=None, dtype=None):
         if dtype is not None:

@@ -80,3 +80,19 @@ def test_a_refused_forward_leaves_the_cache_as_it_was():
     with pytest.raises(ValueError, match='capacity'):
         m(ids[:, 32:33], cache=cache)
     assert cache.seq_len == 32 and all(lc.length == 32 for bc in cache for lc in bc.attn)
+
+
+def test_reset_of_one_layer_leaves_the_others():
+    m = model_of(torch.float32, block=('chord', 'gdn', 'chord'))
+    cache = m.create_cache(kv_bits=4, kv_capacity=64, page_size=16)
+    m(ids_of(2, 40, 5), cache=cache)
+    a, b = cache[0].attn[0], cache[0].attn[2]
+    k, v = b.k, b.v
+    a.reset()
+    assert (a.length, b.length, a.k) == (0, 40, None) and torch.equal(b.k, k) and torch.equal(b.v, v)
+    x = torch.randn(2, 2, 50, 64, device='cuda')
+    ka, va = a.append(x, x + 1, values=True)   # ahead of the other layer, on its pages and ten more tokens
+    assert torch.equal(a.k, ka) and torch.equal(a.v, va) and torch.equal(b.k, k) and torch.equal(b.v, v)
+    a.reset()
+    b.reset()
+    assert a.pages.batch == 0 and a.pages.table is None
