@@ -427,7 +427,13 @@ class DecoderBlockCache:
 
     def reset(self):
         self.attn_res.reset()
-        self.attn.clear()
+        if any(isinstance(c, KV4LayerCache) for c in self.attn):
+            # their kind and capacity come from `build_cache`, not from the decoders' cache types
+            for c in self.attn:
+                if c is not None:
+                    c.reset()
+        else:
+            self.attn.clear()
 
     def is_empty(self) -> bool:
         return self.attn_res.is_empty and len(self.attn) == 0

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from motif_b200 import model as engine
+from motif_b200.cache import KV4LayerCache
 from motif_b200.decode import GraphDecoder
 from test_paged_model_gpu import close, model_of, rounded_cache
 
@@ -80,6 +81,32 @@ def test_a_refused_forward_leaves_the_cache_as_it_was():
     with pytest.raises(ValueError, match='capacity'):
         m(ids[:, 32:33], cache=cache)
     assert cache.seq_len == 32 and all(lc.length == 32 for bc in cache for lc in bc.attn)
+
+
+def test_reset_keeps_the_cache_in_4_bits():
+    """After `ModelCache.reset` the layers are 4-bit ones of the same capacity, and empty."""
+    m = model_of(torch.float32, block=('gdn', 'chord', 'chord'), block_n=2)
+    ids = ids_of(2, 40, 5)
+    cache = m.create_cache(kv_bits=4, kv_capacity=40, page_size=16)
+    want = m(ids, cache=cache).logits
+    for other in (ids, ids_of(3, 40, 5)):      # the batch may change
+        cache.reset()
+        assert cache.seq_len == 0 and cache[0].attn[1].pages.batch == 0
+        out = m(other, cache=cache)
+        for bc, block in zip(cache, m.blocks):
+            assert [isinstance(lc, KV4LayerCache) for lc in bc.attn] == [d.attn_type == 'chord' for d in block.features]
+        assert torch.equal(out.logits, m(other, cache=m.create_cache(kv_bits=4, kv_capacity=40, page_size=16)).logits)
+        with pytest.raises(ValueError, match='capacity'):
+            m(other[:, :9], cache=cache)
+        if other is ids:
+            assert torch.equal(out.logits, want)
+    out.reset_caches()
+    assert torch.equal(m(ids, cache=cache).logits, want)
+    # caches of the model dtype are rebuilt from the decoders' types, as ever
+    plain = m.create_cache()
+    m(ids, cache=plain)
+    plain.reset()
+    assert all(len(bc.attn) == 0 for bc in plain)
 
 
 def test_reset_of_one_layer_leaves_the_others():
