@@ -142,7 +142,7 @@ class GraphDecoder:
         self.cap = min(lc.capacity for lc in self.kv)
         cfg = model.config
         Hkv = cfg.kv_heads
-        if self.kv and cfg.head_dim not in (32, 64):
+        if self.kv and self.pages is None and cfg.head_dim not in (32, 64):
             raise NotImplementedError(f'the decode graph uses the split-KV kernel (head dim 32 or 64), '
                                       f'got head dim {cfg.head_dim}')
         self.splits = int(splits) if splits else _decode_splits(model, self.B, Hkv, self.cap)

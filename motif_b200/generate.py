@@ -112,6 +112,7 @@ class Generation:
         return self
 
     def _graph_ok(self) -> bool:
+        from .cache import KV4LayerCache
         from .model import MotifChordModel
         from .sampler import Sampler
         if not isinstance(self.model, MotifChordModel) or self._key_mask is not None or self.cache is None:
@@ -121,7 +122,8 @@ class Generation:
             return False
         cfg = self.model.config
         has_chord = any(d.attn_type == 'chord' for blk in self.model.blocks for d in blk.features)
-        return has_chord and cfg.head_dim in (32, 64)
+        in_4_bits = any(isinstance(lc, KV4LayerCache) for bc in self.cache for lc in bc.attn)
+        return has_chord and (in_4_bits or cfg.head_dim in (32, 64))
 
     def _run_graph(self):
         from .decode import GraphDecoder

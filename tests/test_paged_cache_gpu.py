@@ -9,7 +9,9 @@ import torch
 
 from motif_b200 import model as engine
 from motif_b200.cache import KV4LayerCache
+from motif_b200.config import MotifChordConfig
 from motif_b200.decode import GraphDecoder
+from motif_b200.model import MotifChordModel
 from test_paged_model_gpu import close, model_of, rounded_cache
 
 pytestmark = pytest.mark.gpu
@@ -123,3 +125,26 @@ def test_reset_of_one_layer_leaves_the_others():
     a.reset()
     b.reset()
     assert a.pages.batch == 0 and a.pages.table is None
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('D', [32, 64, 128])
+def test_every_head_dim_decodes_as_a_graph(dtype, D):
+    """The captured step runs the 4-bit attention alone, which takes head dims of 128 too; prefill and
+    decode in fp32 are held against a cache of rounded values."""
+    torch.manual_seed(1)
+    cfg = MotifChordConfig(vocab_size=512, model_dim=4 * D, num_heads=4, num_kv_heads=2, head_k_dim=64,
+                           block=('gdn', 'chord'), block_n=1)
+    m = MotifChordModel(cfg).to('cuda', dtype).eval()
+    ids = ids_of(2, 40, 7)
+    runs = []
+    for graph in (False, True):
+        cache = m.create_cache(kv_bits=4, kv_capacity=64, page_size=16)
+        g = m.generate(ids[:, :30], max_new_tokens=20, cache=cache, graph=graph).run()
+        assert g.graph_steps == (19 if graph else 0)
+        runs.append(g.generated)
+    assert torch.equal(*runs)
+    if dtype == torch.float32:
+        cache, ref = m.create_cache(kv_bits=4, kv_capacity=64, page_size=16), rounded_cache(m)
+        for a, b in ((0, 25), (25, 26), (26, 40)):
+            close(m(ids[:, a:b], cache=cache).logits, m(ids[:, a:b], cache=ref).logits)
