@@ -148,3 +148,24 @@ def test_every_head_dim_decodes_as_a_graph(dtype, D):
         cache, ref = m.create_cache(kv_bits=4, kv_capacity=64, page_size=16), rounded_cache(m)
         for a, b in ((0, 25), (25, 26), (26, 40)):
             close(m(ids[:, a:b], cache=cache).logits, m(ids[:, a:b], cache=ref).logits)
+
+
+def test_captured_step_follows_lengths_that_differ_on_the_device():
+    """Two requests of 24 and 10 tokens on one cache, crossing page boundaries at different steps: each decodes
+    as it does alone."""
+    m = model_of(torch.float32, block=('chord', 'chord'), seed=8)
+    ids, lens = ids_of(2, 24, 9), (24, 10)
+    cache = m.create_cache(kv_bits=4, kv_capacity=64, page_size=16)
+    m(ids, cache=cache)
+    pages = cache[0].attn[0].pages
+    pages.lens.copy_(torch.tensor(lens))   # the second request's later tokens are forgotten
+    fed = torch.tensor([[7], [11]], device='cuda')
+    dec = GraphDecoder(m, cache, max_steps=12)
+    got = dec.run(fed, 12)
+    assert pages.lens.tolist() == [n + 12 for n in lens]
+    for b, n in enumerate(lens):
+        alone = m.create_cache(kv_bits=4, kv_capacity=64, page_size=16)
+        m(ids[b:b + 1, :n], cache=alone)
+        one = GraphDecoder(m, alone, max_steps=12)
+        assert torch.equal(one.run(fed[b:b + 1], 12)[0], got[b])
+        close(dec.logits[b:b + 1], one.logits)
