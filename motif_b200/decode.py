@@ -177,12 +177,25 @@ class GraphDecoder:
             if finished is not None:
                 self.finished.copy_(finished.reshape(-1).to(self.dev, torch.bool))
             self.all_done = torch.zeros((self.max_steps,), dtype=torch.bool, device=self.dev)
+        self.held = None
         if self.pages is not None:
+            # the graph writes to these however long it is kept
+            self.held = [lc.pool for lc in self.kv], self._shared()
             self.one_new = torch.ones((self.B,), dtype=torch.int32, device=self.dev)
             self.slots = torch.empty((self.B,), dtype=torch.int32, device=self.dev)
         self.launches_per_step = 0
         self.graph = None
         self._capture()
+
+    def _shared(self):
+        return [self.pages.table, self.pages.lens, self.pages.free, self.pages.count]
+
+    def _check_held(self):
+        """The cache still consists of what the graph was captured on."""
+        if self.held is not None:
+            pools, shared = self.held
+            if any(a is not b for a, b in zip(pools + shared, [lc.pool for lc in self.kv] + self._shared())):
+                raise RuntimeError('the cache was reset or moved since this decoder was built')
 
     # ------------------------------------------------------------------ one step
     def _step(self):
@@ -354,6 +367,7 @@ class GraphDecoder:
         return (self._snapshot(), self.lens.clone(), self.step_idx.clone(), self.ids.clone(), self.taken)
 
     def load(self, saved):
+        self._check_held()
         snap, lens, step_idx, ids, taken = saved
         self._restore(snap)
         self.lens.copy_(lens)
@@ -395,6 +409,7 @@ class GraphDecoder:
         With a sampler that applies a repetition penalty, `history` ([B, start + 1], the
         sequence so far ending with `first_ids`, as `Generation.sequences`) seeds the penalty
         on the first run; without it the penalty sees only the tokens fed by the graph."""
+        self._check_held()
         steps = int(steps)
         if steps < 0 or self.taken + steps > self.max_steps:
             raise ValueError(f'{steps} steps after {self.taken} exceed max_steps={self.max_steps}')
@@ -432,6 +447,7 @@ class GraphDecoder:
         counter are put back afterwards, so the decoder is unchanged.  Eager launches leave
         gaps the graph does not have, so these times explain the graph step's SHARES; their
         sum exceeds the graph step."""
+        self._check_held()
         snap = self._snapshot()
         lens = self.lens.clone()
         step_idx = self.step_idx.clone()
@@ -455,6 +471,7 @@ class GraphDecoder:
     def release(self):
         """Free the graph (and its memory pool)."""
         self.graph = None
+        self.held = None
 
 
 def fill_cache_random(model, cache: ModelCache, batch: int, length: int, capacity: int, seed: int = 0):

@@ -169,3 +169,24 @@ def test_captured_step_follows_lengths_that_differ_on_the_device():
         one = GraphDecoder(m, alone, max_steps=12)
         assert torch.equal(one.run(fed[b:b + 1], 12)[0], got[b])
         close(dec.logits[b:b + 1], one.logits)
+
+
+@pytest.mark.parametrize('how', ['model cache', 'one layer', 'moved'])
+def test_a_decoder_whose_cache_was_reset_refuses_to_run(how):
+    """The graph writes to the pool and the lengths it was captured on; they stay its own."""
+    m = model_of(torch.float32)
+    ids = ids_of(2, 20, 10)
+    cache = m.create_cache(kv_bits=4, kv_capacity=64, page_size=16)
+    first = m(ids, cache=cache).next_token()
+    dec = GraphDecoder(m, cache, max_steps=8)
+    dec.run(first, 2)
+    saved = dec.save()
+    if how == 'moved':
+        lc = cache[0].attn[1]
+        lc.pool = lc.pool.clone()
+    else:
+        (cache if how == 'model cache' else cache[0].attn[1]).reset()
+    for call in (lambda: dec.run(first, 2), lambda: dec.load(saved), lambda: dec.breakdown(first, 1)):
+        with pytest.raises(RuntimeError, match='reset or moved'):
+            call()
+    dec.release()
