@@ -854,14 +854,26 @@ def _decode_splits(model, B, Hkv, S):
     return int(max(1, min(want, 64, (S + 255) // 256)))
 
 
-# Most query rows of a kv head (query heads of its group x new tokens) of one request, and of all requests
-# together, that attend to a 4-bit cache directly; other chunks read it back and use the prefill kernel,
-# which is as slow for few tiles of queries as for many.  Measured at 12 / 3 heads of 64, direct against
-# read back: 64 rows: 64 requests of 2048 tokens 81 / 102 us, of 8192 251 / 373; 128 rows 146 / 103 and
-# 484 / 373.  2048 rows in all: 1 request of 8192 132 / 195 us, 8 133 / 203, 32 133 / 189, 1 of 2048 48 /
-# 56, 16 49 / 48, 1 of 32768 472 / 748; 4096: 4 requests of 8192 248 / 198, 8 of 2048 81 / 58.
-KV4_DIRECT_ROWS = 64
-KV4_DIRECT_ROWS_IN_ALL = 2048
+# By head dim: the most query rows of one kv head (query heads of its group x new tokens) of a request, and
+# the most query rows of all requests and heads together, that attend to a 4-bit cache directly; larger
+# 16-bit chunks read it back and use the prefill kernel.  The direct kernel passes over the cache once for
+# 16 rows of a kv head (41e-6 us a cached token and pass at D = 64, 31e-6 at 32, all SMs at work), the
+# prefill kernel once for 128, but it is as slow for a few tiles of queries as for a wave of them.
+# Measured, direct against read back: D = 64, 8 kv heads of 4, 8192 tokens: 8192 rows 183 / 200 us, 16384
+# 348 / 200; 2048 tokens: 66 / 59 and 112 / 59; 32768: 665 / 767 and 1308 / 766; 64 requests of 2048 with
+# 64 rows a kv head 198 / 213, with 128 366 / 214.  3 kv heads of 4, 8192 tokens: 6144 rows 141 / 198,
+# 12288 265 / 201.  D = 32, 3 kv heads of 4, 8192 tokens: 12288 rows 198 / 260, 24576 386 / 300; 8 kv heads,
+# 64 requests of 2048 with 32 rows 99 / 77 (16 requests), with 64 172 / 125.
+# fp32 and head dim 128 have no tensor-core prefill kernel: 4 requests of 8192 tokens, 256 new ones, 4 kv
+# heads of 4 and D = 128 take 0.67 ms directly and 65 ms read back (fp32 0.94 and 68).
+KV4_DIRECT_ROWS = {64: (64, 8192), 32: (48, 12288)}
+
+
+def _kv4_direct(B: int, H: int, Hkv: int, T: int, D: int, dt: torch.dtype) -> bool:
+    if dt == torch.float32 or D not in KV4_DIRECT_ROWS:
+        return True
+    of_one, of_all = KV4_DIRECT_ROWS[D]
+    return H // Hkv * T <= of_one or B * H * T <= of_all
 
 
 def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache], position, dt, dev, dc, st,
@@ -906,7 +918,7 @@ def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache
             kv = cache.append(kt, vt, values=True)
         else:
             cache.append(kt, vt)
-            direct = G * T <= KV4_DIRECT_ROWS or B * G * T <= KV4_DIRECT_ROWS_IN_ALL
+            direct = _kv4_direct(B, H, Hkv, T, D, dt)
             # a layer behind the shared lengths (a forward that stopped between two layers) reads its own
             if direct and key_bias is None and q_start == cached and cache.length == cache.pages.length:
                 attn = kv4_chord_attention(qb.view(B, T, H, D).transpose(1, 2), cache.pool, cache.pages.table,
