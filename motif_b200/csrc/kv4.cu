@@ -475,6 +475,14 @@ extern "C" int motif_b200_paged_reserve(const int32_t* lens, const int32_t* new_
              "paged_reserve: %lld new tokens (0 .. 2^31 - 2^20)", (long long)total_new);
   MB_REQUIRE(free_capacity >= 1 && free_capacity * page_size < (1ll << 31), MB_ERR_SHAPE,
              "paged_reserve: free list of %lld pages", (long long)free_capacity);
+  // every CTA reads the lengths, and some write: where the outputs are not the inputs themselves, whose
+  // writes wait for all reads, they share nothing with them
+  auto meet = [](const int32_t* p, int64_t n, const int32_t* q, int64_t m) { return p < q + m && q < p + n; };
+  MB_REQUIRE((lens_out == lens || !meet(lens_out, B, lens, B)) && !meet(lens_out, B, new_lens, B) &&
+                 !meet(slots, total_new, lens, B) && !meet(slots, total_new, new_lens, B) &&
+                 !meet(slots, total_new, lens_out, B) && !meet(free_count_out, 1, new_lens, B) &&
+                 !meet(free_count_out, 1, lens, B) && !meet(free_count_out, 1, lens_out, B),
+             MB_ERR_ARG, "paged_reserve: lens_out, slots and free_count_out overlap each other or the lengths");
   const PageDiv by = page_div(page_size);
   const bool vector = reinterpret_cast<uintptr_t>(slots) % 16 == 0;
   const bool in_place = lens_out == lens || free_count_out == free_count;

@@ -287,3 +287,24 @@ def test_other_python_threads_run_while_a_launch_waits():
         torch.cuda.synchronize()
     assert waited > 0.7, 'the launches did not fill the queue'
     assert longest[0] < 0.35
+
+
+def test_reservations_into_their_own_inputs_are_refused():
+    """lens_out may be lens, free_count_out free_count; anything else that overlaps would be read by one CTA
+    after another has written it."""
+    i32 = dict(dtype=torch.int32, device='cuda')
+    both = torch.tensor([3, 4, 5, 1, 1, 1], **i32)
+    lens, new = both[:3], both[3:]
+    free, count = torch.arange(20, **i32), torch.tensor([20], **i32)
+    table = torch.tensor([[15, -1], [16, -1], [17, -1]], **i32)
+
+    def reserve(**kw):
+        return ops.paged_reserve(lens, new, table, free, count, 16, 3, **kw)
+
+    for kw in (dict(lens_out=new), dict(lens_out=both[1:4]), dict(lens_out=both[2:5]), dict(slots=lens), dict(slots=new),
+               dict(slots=both[2:5]), dict(free_count_out=both[:1]), dict(free_count_out=both[5:])):
+        with pytest.raises(ValueError, match='overlap'):
+            reserve(**kw)
+    assert both.tolist() == [3, 4, 5, 1, 1, 1] and count.tolist() == [20]
+    slots, out, left = reserve(lens_out=lens, free_count_out=count)
+    assert slots.tolist() == [15 * 16 + 3, 16 * 16 + 4, 17 * 16 + 5] and out.tolist() == [4, 5, 6] and left is count
