@@ -17,12 +17,12 @@ pytestmark = pytest.mark.gpu
 
 
 # ------------------------------------------------------------------ sums of 16-bit tensors
-def attention_32(q, pool, table, lens, alpha, beta, mu, ssmax):
+def attention_32(q, pool, table, lens, alpha, beta, mu, ssmax, scale=None):
     """Elementary operations in 32 bits, rounded once at the end."""
     most = int(lens.max())
     k, v = ops.kv4_gather(pool, table, lens, most, dtype=torch.float32)
     B, H, T, D = q.shape
-    x = (q.float().view(B, k.shape[1], -1, D) @ k.transpose(-1, -2) * D ** -0.5).view(B, H, T, most)
+    x = (q.float().view(B, k.shape[1], -1, D) @ k.transpose(-1, -2) * (scale or D ** -0.5)).view(B, H, T, most)
     pos = (lens[:, None] - T + torch.arange(T, device='cuda')).view(B, 1, T, 1)
     key = torch.arange(most, device='cuda')
     alpha, beta, mu, ssmax = (p.view(1, H, 1, 1) for p in (alpha, beta, mu, ssmax))
@@ -47,6 +47,11 @@ def test_sums_of_16_bit_tensors_keep_their_bits(H, kv, D, T):
     want = attention_64(q, pool, table, ln, *p).half()
     wrong = (ops.kv4_chord_attention(q, pool, table, ln, *p) != want).sum()
     assert wrong <= 8 * (attention_32(q, pool, table, ln, *p) != want).sum()
+    # logits ten times as large: an error of the first product's sums grows with them
+    scale = 10 * D ** -0.5
+    want = attention_64(q, pool, table, ln, *p, scale=scale).half()
+    wrong = (ops.kv4_chord_attention(q, pool, table, ln, *p, softmax_scale=scale) != want).sum()
+    assert wrong <= 8 * (attention_32(q, pool, table, ln, *p, scale) != want).sum()
 
 
 # ------------------------------------------------------------------ waits that run out
