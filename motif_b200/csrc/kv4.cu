@@ -25,7 +25,7 @@ using kv4::PageDiv;
 // old table entry or comes straight from the free list, so nobody waits for the fresh entries to be
 // written.  Bound by latency (the bytes take 0.1 us): one scan and two dependent loads.  3.3 us for one
 // token of each of 64 requests (one CTA of four warps), 4.4 for 32 prompts of 4096 tokens, 5.7 for 517
-// ragged chunks (7.1 and 8.7 on a cluster of 8); on one CTA the latter two took 43.9 and 35.2.
+// ragged chunks (in place, on a cluster of 8, 7.6 and 9.0); on one CTA the latter two took 43.9 and 35.2.
 constexpr int kClusterCtas = 8;  // the most a cluster holds everywhere
 constexpr int kReserveCtas = 64;
 
@@ -155,7 +155,8 @@ __global__ void __launch_bounds__(THREADS) paged_reserve_kernel(
 }
 
 // Finished requests give their pages back: onto the top of the free list in request order, their
-// table rows become -1 and their lengths 0.
+// table rows become -1 and their lengths 0.  One CTA, whose warps copy rows: 64 requests of 128 pages 4.9
+// us, 512 of 128 19.8, 512 of 512 67 (the bytes take 0.02 to 0.5); once in a request's life.
 constexpr int kReleaseThreads = 1024;
 
 __global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
@@ -337,7 +338,7 @@ __device__ __forceinline__ void quantise(const float* x, float hi, float lo, flo
 // TB/s or 87 % of the copy rate (E = 1 50.7; E = 4 as slow, of too few warps; IEEE divisions at E = 1
 // 128.6).  A call that does not fill the GPU is a chain of latencies, which E = 1 makes shorter: one
 // token of 64 requests 1.8 us against 2.1.  fp32 is at the copy rate at E = 1: 5003 tokens of 8 heads
-// of 128 11.6 us.  CTAs that stay and fetch their next rows early measured slower (60.5 us where E = 1
+// of 128 11.7 us (15.1 with inputs that were not in L2 before).  CTAs that stay and fetch their next rows early measured slower (60.5 us where E = 1
 // took 51.0: the registers cost more warps than the early loads hide).
 template <typename T, int D, int E, typename I>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v,

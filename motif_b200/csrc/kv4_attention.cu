@@ -6,32 +6,34 @@
 //   q . k_j          = sum_groups  s_j (q . c_j - 8 sum(q)) + m_j sum(q)
 //   sum_j p_j v_j    = sum_j (p_j s_j) c_j                  + sum_j p_j (m_j - 8 s_j)
 // and both products run on the codes themselves.  A code in bits 6..9 of an fp16 IS the number c 2^-18
-// (subnormal, exact, and the tensor cores take it as it is), so a packed word becomes matrix operands
-// with a shift and an AND per pair and no conversion; the power of two is undone in fp32.  The other operand is split into two fp16 parts of 11 bits each (q after a
-// power-of-two normalisation of its row, p s against the largest scale so far), and the parts are
-// two neighbouring columns of one MMA: with the keys on the M side a tile of 4 query rows fills
-// N = 8, a thread's two accumulator columns are the two parts of ONE query row, and their sum is the
-// product to 22 bits at no further instruction.  The score tile [keys x (row, part)] is the transpose
-// of what the second product wants: one movmatrix per 8 keys.  mma.sync and not tcgen05: a kv head has
-// 4 to 16 query rows, the operand that comes from memory must be unpacked in registers, and the tensor
-// pipe is busy for a fifth of the time as it is.
+// (subnormal, exact, and the tensor cores take it as it is), so a packed word becomes matrix operands with
+// a shift and an AND per pair and no conversion; the power of two is undone in fp32.  The other operand is
+// split into two fp16 parts of 11 bits each (q after a power-of-two normalisation of its row, p s against
+// the largest scales that have weight), and the parts are two neighbouring columns of one MMA: with the
+// keys on the M side a tile of 4 query rows fills N = 8, a thread's two accumulator columns are the two
+// parts of ONE query row, and their sum is the product to 22 bits at no further instruction.  (16-bit
+// queries are one part; the sums of the products are the tensor cores', which cut below 24 bits of the
+// largest term: see codes().)  The score tile [keys x (row, part)] is the transpose of what the second
+// product wants: one movmatrix per 8 keys.  mma.sync and not tcgen05: a kv head has 4 to 16 query rows,
+// the operand that comes from memory must be unpacked in registers, and the tensor pipe is busy for a
+// fifth of the time as it is.
 //
-// Work is cut by tiles of 64 keys (128 for D = 32), not by requests: the tiles of all (request, row
-// tile, kv head) segments in order are dealt out in equal runs to the CTAs (one per SM) and within
-// them to the warps, so requests of any lengths load the GPU evenly, and the lengths may change on the
-// device between replays of a CUDA graph.  A segment inside one warp's run is written out by it; one
-// that spans warps is joined in shared memory, one that spans CTAs leaves a partial (o, m, l) per CTA,
-// which the merge kernel joins in CTA order.  Each warp owns a ring of two tiles in shared memory that
-// its first lanes fill with bulk copies (one per tile where a tile lies in one page).
+// Work is cut by tiles of 64 keys (128 for D = 32), not by requests: the tiles of all (request, row tile,
+// kv head) segments in order are dealt out in equal runs to the CTAs (one per SM) and within them to the
+// warps, so requests of any lengths load the GPU evenly, and the lengths may change on the device between
+// replays of a CUDA graph.  A segment inside one warp's run is written out by it; one that spans warps is
+// joined in shared memory, one that spans CTAs leaves a partial (o, m, l) per CTA, which the merge kernel
+// joins in CTA order once it has waited for the workers.  Each warp owns a ring of two tiles in shared
+// memory that its first lanes fill with bulk copies (one per tile where a tile lies in one page).
 //
-// What bounds it: the instructions that unpack and weigh, not the memory.  A unit of 16 keys takes 150
-// instructions of a warp, 70 of them on the half-rate integer pipe (44 isolate the codes), which is
-// busy for two thirds of the main loop.  64 requests of 8192 tokens (12 / 3 heads of 64, 113 MB):
-// 32.9 us on the GPU, 3.4 TB/s, where the bytes alone would take 17.4; of it 4 us pass before the
-// first tile has arrived (lengths, page table, copy: three dependent loads) and 3 in joining.  12 warps
-// of 144 registers measured best there: 8 warps 37.3 us, 16 warps 33.4 (and 13.2 against 10.8 for 8
-// requests), 128-key tiles on 8 warps 34.2.  48 ragged requests of up to 5000 tokens, 4 new ones each,
-// 16 query rows on 4 fp16 kv heads of 128 (54 MB): 40.3 us, in two passes of 8 rows.
+// What bounds it: neither the memory nor a pipe, but latency that three warps a scheduler do not hide, each
+// of which waits for a tile, scores it, weighs it and takes the second product one after the other.  64
+// requests of 8192 tokens (12 / 3 heads of 64, 113 MB): 36.2 us on the GPU, 3.1 TB/s, where the bytes alone
+// would take 17.4; 197 warp instructions a unit of 16 keys in all, issue slots 54 % busy, the half-rate
+// integer pipe that isolates the codes 51 %, the tensor pipe 18 %.  8 requests, where a warp has one or two
+// tiles: 11.5 us.  12 warps of 147 registers: 8 warps 40.5 us; 16 warps 35.7, but 12.5 against 11.5 for 8
+// requests; 128-key tiles on 8 warps 38.7.  48 ragged requests of up to 5000 tokens, 4 new ones each, 16
+// query rows on 4 fp16 kv heads of 128 (54 MB): 46.1 us, in two passes of 8 rows.
 #include <math.h>
 
 #include "common.cuh"
@@ -49,7 +51,7 @@ constexpr int kStages = 2;
 constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 4.f;  // log 2 units
-constexpr int kLift = 60;
+constexpr int kLift = 60;       // the most that a row's weights are lifted by, log 2
 
 struct Strides6 {
   int64_t s[6];  // q(b,h,t) out(b,h,t)
@@ -74,8 +76,8 @@ struct Args {
 };
 
 // 64 keys: a tile's independent chains are what hides latency beside two or three warps a scheduler.
-// D = 128 on 32 keys and 12 warps 41.1 us against 38.3 on 64 keys and 8 (32 requests of 8192 tokens, 4 kv
-// heads); D = 32 on 64 keys 27.3 against 25.2 on 128 (64 requests of 8192, 3 kv heads).
+// D = 128 on 32 keys and 12 warps 46.2 us against 42.3 on 64 keys and 8 (32 requests of 8192 tokens, 4 kv
+// heads); D = 32 on 64 keys 29.1 against 27.0 on 128 (64 requests of 8192, 3 kv heads).
 template <int D>
 struct Tile {
   static constexpr int kUnits = D == 32 ? 8 : 4;
@@ -261,11 +263,13 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, const uint3
 // the products of a step by their operands' exponent fields and cut below 24 bits; a subnormal's field
 // stands for its bit 9, so the codes are shifted to end there, which leaves the sums all but the bits of
 // 8 sum(q) against q . c.  In bits 0..3 and 4..7, without most of the shifts, the sums kept 17 bits and 64
-// requests of 8192 took 33.0 us where they take 35.2; distance from 64 bits before the last rounding (16
+// requests of 8192 took 33.0 us where they took 35.2; distance from 64 bits before the last rounding (16
 // requests of 8192, fp16) 2.0e-5 there, 9.5e-7 here, and 1.1e-6 for elementary operations in fp32.  fp32
 // tensors make them normal numbers c - 8 (U = 1: the bits of 1024 or-ed in, 1024 + 8 U taken off; where
 // they lie in the word does not matter then, and the odd nibbles come out 16 times as large) at one more
-// instruction a pair, and need the sums less 8 no more; for 16-bit ones that took 39.5 us.
+// instruction a pair, and need the sums less 8 no more; for 16-bit ones that took 39.5 us.  Nearly all of
+// the distance is the second product's; the first one's shows where logits are sharp (ten times as large, D
+// = 32: 8.7e-6 against 5.6e-7 with its codes in bits 0..3 and 4..7, at 35.3 us; fp32 operations 4.8e-7).
 template <bool EXACT>
 __device__ __forceinline__ void codes(uint32_t w, uint32_t* h) {
   if constexpr (EXACT) {
@@ -324,7 +328,8 @@ __device__ __forceinline__ void zero_rows(T* out, const Args& a) {
 
 // ------------------------------------------------------------------ the worker kernel
 // Warps of the one CTA an SM runs, by the registers and the ring that the output tile leaves them (8 query
-// rows of D = 128 on 12 warps spill: 51.0 us against 44.1; so do 16 rows of D = 64: 109 against 73).
+// rows of D = 128 on 12 warps and 32 keys spill: 53.3 us against 46.1; so do 16 rows of D = 64: 113
+// against 77).
 __host__ __device__ constexpr int warps_of(int nt, int D) { return nt <= 2 && D <= 64 ? 12 : 8; }
 
 // An unfinished piece of a segment at the end of a warp's run: [RT rows][D + 4] floats (o, m, l), its
@@ -767,7 +772,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
             for (int u = 0; u < TU; ++u) x[n][u] = fadd2(x[n][u], make_float2(-up, -up));
           };
           // scales within 2^12 of each other need no lift, whatever the weights
-          if (!__any_sync(0xffffffffu, small * 4096.f < pow2(min(vn, 127)) || lifted > kSlack || (vn > ve && vtop > 0.f))) {
+          const bool apart = small * 4096.f < pow2(min(vn, 127)) || lifted > kSlack || (vn > ve && vtop > 0.f);
+          if (!__any_sync(0xffffffffu, apart)) {
             vtop = pow2(min(vn, 126) + 1);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -785,7 +791,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
               for (int u = 0; u < TU; ++u) {
                 float2 vs = make_float2(kv4::pair_scale(vp[u][0][0]), kv4::pair_scale(vp[u][0][1]));
                 if constexpr (NG == 2)
-                  vs = make_float2(fmaxf(vs.x, kv4::pair_scale(vp[u][1][0])), fmaxf(vs.y, kv4::pair_scale(vp[u][1][1])));
+                  vs = make_float2(fmaxf(vs.x, kv4::pair_scale(vp[u][1][0])),
+                                   fmaxf(vs.y, kv4::pair_scale(vp[u][1][1])));
                 heavy = fmax3(heavy, ex2f_(x[n][u].x - at) * vs.x, ex2f_(x[n][u].y - at) * vs.y);
               }
 #pragma unroll
@@ -1034,10 +1041,10 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
 }
 
 // ------------------------------------------------------------------ merge
-// Merge CTA c joins the partials of the segment that begins in worker CTA c's run and goes on in the
-// next one's, if there is one (the worker has left beside them which).  Thread group i of D RT / 4 threads takes partials i, i + PL, ... in one pass
-// with a running maximum; the groups are joined in order.  256 threads of 40 registers find room beside
-// the worker CTAs, so the merge is there when they end.
+// Merge CTA c joins the partials of the segment that begins in worker CTA c's run and goes on in the next
+// one's, if there is one (the worker has left beside them which).  Thread group i of D RT / 4 threads
+// takes partials i, i + PL, ... in one pass with a running maximum; the groups are joined in order.  256
+// threads of 40 registers find room beside the worker CTAs, so the merge is there when they end.
 constexpr int kMergeThreads = 256;
 
 template <typename T, int D, int NT>
@@ -1106,7 +1113,7 @@ __global__ void __launch_bounds__(kMergeThreads, 6) kv4_merge_kernel(T* __restri
 // ------------------------------------------------------------------ host side
 // Score columns per thread of a row tile: tiles of 4, 8 or 16 query rows.  D = 128 stops at 8: with 16
 // the output tile alone takes half the registers, and the spills cost more than the second pass over
-// the cache saves (48 ragged requests of up to 5000 tokens, 16 rows, 32-key tiles: 53.9 us against 45.1).
+// the cache saves (48 ragged requests of up to 5000 tokens, 16 rows: a fifth slower).
 int row_tile(int64_t rows, int64_t D) {
   if (rows <= 4) return 1;
   return rows <= 8 || D == 128 ? 2 : 4;

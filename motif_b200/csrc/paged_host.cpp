@@ -2,7 +2,7 @@
 // the outputs and the call of the C ABI in one compiled step.  A decode step's calls are bound by the
 // host (each kernel runs for a few microseconds): through ctypes and Python-level checks an attention
 // call took 20.3 us, an append 14.6, a gather 12.3 and a reservation 14.3 on the host; here they take
-// 7.5, 4.8, 4.2 and 5.3, of which the launches themselves are 2 to 5.
+// 7.4, 5.3 (3.5 without the stored values), 4.6 and 5.7, of which the launches themselves are 2 to 5.
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
