@@ -500,7 +500,8 @@ def build_cache(model, use_attn: Optional[bool] = None, functional: bool = False
             raise ValueError('kv_bits=4 needs kv_capacity, the most tokens a request may cache')
         if functional or wide_kv or use_attn is False:
             raise ValueError('kv_bits=4 goes with neither functional, wide_kv nor use_attn=False')
-        check_head_dim(model.config.head_dim)
+        if any(issubclass(d.cache_type, KVLayerCache) for b in model.blocks for d in b.features):
+            check_head_dim(model.config.head_dim)
         pages, use_attn = KV4Pages(kv_capacity, page_size), True
     if use_attn is None:
         use_attn = not getattr(model, 'training', False)

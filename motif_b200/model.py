@@ -869,7 +869,11 @@ def _decode_splits(model, B, Hkv, S):
 KV4_DIRECT_ROWS = {64: (64, 8192), 32: (48, 12288)}
 
 
-def _kv4_direct(B: int, H: int, Hkv: int, T: int, D: int, dt: torch.dtype) -> bool:
+def _kv4_direct(B: int, H: int, Hkv: int, T: int, D: int, dt: torch.dtype, capacity: int = 0) -> bool:
+    # the kernel counts its work in 32 bits, at least 4 rows and 64 of the keys that a request could hold at
+    # a time
+    if H * T >= 1 << 24 or B * Hkv * -(-(H // Hkv * T) // 4) * -(-capacity // 64) >= 1 << 31:
+        return False
     if dt == torch.float32 or D not in KV4_DIRECT_ROWS:
         return True
     of_one, of_all = KV4_DIRECT_ROWS[D]
@@ -918,7 +922,7 @@ def _chord_decoder(model, pk: _ChordPack, hn, B, T, cache: Optional[KVLayerCache
             kv = cache.append(kt, vt, values=True)
         else:
             cache.append(kt, vt)
-            direct = _kv4_direct(B, H, Hkv, T, D, dt)
+            direct = _kv4_direct(B, H, Hkv, T, D, dt, cache.capacity)
             # a layer behind the shared lengths (a forward that stopped between two layers) reads its own
             if direct and key_bias is None and q_start == cached and cache.length == cache.pages.length:
                 attn = kv4_chord_attention(qb.view(B, T, H, D).transpose(1, 2), cache.pool, cache.pages.table,

@@ -29,9 +29,9 @@ def test_tables_whose_tokens_pass_32_bits_are_refused(page, columns):
 
 def test_a_cache_that_cannot_be_kept_is_refused_when_it_is_made():
     """Page size, capacity and head dim, not at the first Chord layer of a forward."""
-    def model(heads):
+    def model(heads, block=('gdn', 'chord')):
         return MotifChordModel(MotifChordConfig(vocab_size=64, model_dim=128, num_heads=heads, num_kv_heads=1, head_k_dim=64,
-                                                block=('gdn', 'chord'), block_n=1))
+                                                block=block, block_n=1))
 
     m = model(2)
     for page in (0, 8, 24, 40, 2048, -16):
@@ -41,4 +41,5 @@ def test_a_cache_that_cannot_be_kept_is_refused_when_it_is_made():
         m.create_cache(kv_bits=4, kv_capacity=0)
     with pytest.raises(NotImplementedError, match='head_dim'):
         model(8).create_cache(kv_bits=4, kv_capacity=100)
+    model(8, ('gdn',)).create_cache(kv_bits=4, kv_capacity=100)   # no Chord layer, nothing to keep
     assert m.create_cache(kv_bits=4, kv_capacity=100, page_size=48)[0].attn[1].capacity == 144

@@ -24,3 +24,9 @@ def test_chunks_without_a_tensor_core_prefill_kernel_are_never_read_back(T):
     for D in (32, 64, 128):
         assert _kv4_direct(64, 32, 8, T, D, torch.float32)
     assert _kv4_direct(64, 32, 8, T, 128, torch.bfloat16)
+
+
+def test_chunks_that_the_direct_kernel_cannot_count_are_read_back():
+    assert _kv4_direct(64, 32, 8, 4096, 128, torch.bfloat16, 32768)
+    assert not _kv4_direct(64, 32, 8, 4096, 128, torch.bfloat16, 131072)
+    assert not _kv4_direct(1, 32, 8, 1 << 19, 64, torch.float32, 1 << 20)
