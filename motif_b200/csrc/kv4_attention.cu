@@ -601,6 +601,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT, D), 1)
       if (__any_sync(0xffffffffu, !mbar_wait_bounded(&bar[s], (uint32_t)phase, polls))) {
         failed = true;
         mbar_wait_bounded(&bar[s], (uint32_t)phase, kWaitLimit);
+        static_assert(kStages == 2, "one other stage");
         if (looked > i + 1) mbar_wait_bounded(&bar[s ^ 1], (uint32_t)(phase ^ s), kWaitLimit);
         break;
       }
