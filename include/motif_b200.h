@@ -160,6 +160,29 @@ MB_API int motif_b200_gated_rms_norm(const void* x, const void* w, void* y, int6
 MB_API int motif_b200_swiglu(const void* x, void* y, int64_t M, int64_t N, int64_t x_stride,
                       int64_t y_stride, int dtype, void* stream);
 
+/* ------------------------------------------------------------------ norms and SwiGLU for training
+ * Forward of RMSNorm (gated = 0: rows of N) or GatedRMSNorm (gated = 1: rows of N values, then N gates)
+ * in fp32 with one rounding at the end; w [N] of w_dtype, or NULL.  Rows of x, y, dy and dx are
+ * xs, ys, ds and os elements apart, their elements next to each other. */
+MB_API int motif_b200_rms_norm_train(const void* x, const void* w, int w_dtype, void* y, int64_t M, int64_t N,
+                              int64_t xs, int64_t ys, int gated, float eps, int dtype, void* stream);
+
+/* Its gradients: dx (laid out as x: N, or 2 N with the gates' gradient behind) and, unless dw is
+ * NULL, dw [N] of w_dtype, summed in fp32 in an order that depends on the sizes alone.  `workspace`
+ * (needed for dw) holds motif_b200_rms_norm_backward_workspace_bytes(...) bytes (-1: bad sizes).
+ * Replaces the backward of RMSNorm / GatedRMSNorm, motif/ops/rms_norm.py:63-112,162-229. */
+MB_API int64_t motif_b200_rms_norm_backward_workspace_bytes(int64_t M, int64_t N, int dtype);
+MB_API int motif_b200_rms_norm_backward(const void* x, const void* w, int w_dtype, const void* dy, void* dx, void* dw,
+                                 int64_t M, int64_t N, int64_t xs, int64_t ds, int64_t os, int gated, float eps,
+                                 void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/* SwiGLU of x [M, 2 N] in fp32 with one rounding, and its gradient: x, dy [M, N] -> dx [M, 2 N].
+ * Replaces SwiGLU's forward and backward under autograd, motif/ops/swiglu.py:62-117,239-253. */
+MB_API int motif_b200_swiglu_train(const void* x, void* y, int64_t M, int64_t N, int64_t xs, int64_t ys, int dtype,
+                            void* stream);
+MB_API int motif_b200_swiglu_backward(const void* x, const void* dy, void* dx, int64_t M, int64_t N, int64_t xs,
+                               int64_t ds, int64_t os, int dtype, void* stream);
+
 /* ------------------------------------------------------------------ fused model kernels
  * These replace sequences of reference statements inside one layer; each cites them.
  * Token-major activations: row r = b*T + t, element stride 1 within a row.

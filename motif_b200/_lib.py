@@ -42,6 +42,11 @@ SIGNATURES = {
     'motif_b200_rms_norm': (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _F, _I, _P]),
     'motif_b200_gated_rms_norm': (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _F, _I, _P]),
     'motif_b200_swiglu': (_I, [_P, _P, _I64, _I64, _I64, _I64, _I, _P]),
+    'motif_b200_rms_norm_train': (_I, [_P, _P, _I, _P] + [_I64] * 4 + [_I, _F, _I, _P]),
+    'motif_b200_rms_norm_backward_workspace_bytes': (_I64, [_I64, _I64, _I]),
+    'motif_b200_rms_norm_backward': (_I, [_P, _P, _I, _P, _P, _P] + [_I64] * 5 + [_I, _F, _P, _I64, _I, _P]),
+    'motif_b200_swiglu_train': (_I, [_P, _P] + [_I64] * 4 + [_I, _P]),
+    'motif_b200_swiglu_backward': (_I, [_P, _P, _P] + [_I64] * 5 + [_I, _P]),
     'motif_b200_attn_res_norm': (_I, [_P, _I, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F, _F, _I, _P]),
     'motif_b200_gdn_prep': (_I, [_P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                                  _I64, _I, _P]),
@@ -153,6 +158,25 @@ def stream_ptr(device=None) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+class _Here:
+    """A context that changes nothing."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Context in which launches go to `device` (its index must be set): the library launches on the
+    current device, and a stream of another one is an error."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def i64_array(vals):
     vals = [int(v) for v in vals]
     return (ctypes.c_int64 * len(vals))(*vals)
@@ -173,6 +197,7 @@ KERNELS_PER_CALL.update({'motif_b200_last_error': 0, 'motif_b200_abi_version': 0
                          'motif_b200_chord_workspace_bytes': 0, 'motif_b200_chord_decode_workspace_bytes': 0,
                          'motif_b200_skinny_packed_bytes': 0, 'motif_b200_gdn_chunk_workspace_bytes': 0,
                          'motif_b200_chord_backward_workspace_bytes': 0, 'motif_b200_gdn_backward_workspace_bytes': 0,
+                         'motif_b200_rms_norm_backward_workspace_bytes': 0, 'motif_b200_rms_norm_backward': 2,
                          'motif_b200_chord_backward': 2, 'motif_b200_kv4_chord_attention': 2,
                          'motif_b200_kv4_unit_bytes': 0, 'motif_b200_kv4_attention_workspace_bytes': 0,
                          'motif_b200_wait_timeouts': 0, 'motif_b200_testing_force': 0,

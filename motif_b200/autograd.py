@@ -1,5 +1,6 @@
-"""Autograd for the three hot-path ops: their forwards run the inference kernels, their
-backwards the kernels of `csrc/backward.cu` (fp32 arithmetic on CUDA cores).
+"""Autograd for the ops.  Chord attention, the AttnRes read and the delta rule: their forwards run
+the inference kernels, their backwards the kernels of `csrc/backward.cu` (fp32 arithmetic on CUDA
+cores).  The norms and SwiGLU: `csrc/norm_grad.cu`.
 
 The reference wraps the same ops in `torch.autograd.Function`s (`_TritonChordFunction`,
 `motif/ops/chord_attention.py:1476-1554`; `_AttnResFunction`, `motif/ops/attn_res.py:367-463`;
@@ -16,6 +17,16 @@ from . import _lib
 
 def needs_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
+
+
+def first_order(backward):
+    """Refuses a backward pass that is itself recorded (`create_graph=True`): its results would
+    look like constants, and the terms of a second derivative that pass through here be dropped."""
+    def checked(ctx, *grads):
+        if torch.is_grad_enabled():
+            raise NotImplementedError('motif_b200 ops have no second derivatives (create_graph=True)')
+        return backward(ctx, *grads)
+    return checked
 
 
 def _c(t):
@@ -145,3 +156,71 @@ class GatedDeltaRuleFunction(torch.autograd.Function):
                 dv.to(v.dtype) if need[3] else None, db.to(beta.dtype) if need[4] else None,
                 dg.to(g.dtype) if need[5] else None,
                 dS0.to(S.dtype) if (S is not None and need[6]) else None)
+
+
+class RMSNormFunction(torch.autograd.Function):
+    """RMSNorm (`gated`: GatedRMSNorm) of the rows of x [M, N] ([M, 2 N]) in fp32 with one rounding
+    (`motif_b200_rms_norm_train`), with the gradients of x and the weight
+    (`motif_b200_rms_norm_backward`).  The weight keeps its own dtype, and so does its gradient."""
+
+    @staticmethod
+    def forward(ctx, x, weight, eps, gated):
+        M, N = x.shape
+        if gated:
+            N //= 2
+        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        wd = _lib.MB_F32 if weight is None else _lib.dtype_code(weight.dtype)
+        with _lib.on_device(x.device):
+            _lib.call('motif_b200_rms_norm_train', x.data_ptr(), _lib.ptr(weight), wd, y.data_ptr(), M, N, x.stride(0),
+                      N, gated, eps, _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
+        ctx.save_for_backward(x, weight)
+        ctx.eps, ctx.gated = eps, gated
+        return y
+
+    @staticmethod
+    @first_order
+    def backward(ctx, dy):
+        x, weight = ctx.saved_tensors
+        M, N = dy.shape
+        dy = _c(dy)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = ws = None
+        wd, nbytes, dc = _lib.MB_F32, 0, _lib.dtype_code(x.dtype)
+        if weight is not None:
+            wd = _lib.dtype_code(weight.dtype)
+            if ctx.needs_input_grad[1]:
+                dw = torch.empty_like(weight)
+                nbytes = _lib.load().motif_b200_rms_norm_backward_workspace_bytes(M, N, dc)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        with _lib.on_device(x.device):
+            _lib.call('motif_b200_rms_norm_backward', x.data_ptr(), _lib.ptr(weight), wd, dy.data_ptr(), dx.data_ptr(),
+                      _lib.ptr(dw), M, N, x.stride(0), dy.stride(0), dx.stride(0), ctx.gated, ctx.eps, _lib.ptr(ws),
+                      nbytes, dc, _lib.stream_ptr(x.device))
+        return dx if ctx.needs_input_grad[0] else None, dw, None, None
+
+
+class SwiGLUFunction(torch.autograd.Function):
+    """SwiGLU of the rows of x [M, 2 N] in fp32 with one rounding (`motif_b200_swiglu_train`) and its
+    gradient (`motif_b200_swiglu_backward`)."""
+
+    @staticmethod
+    def forward(ctx, x):
+        M, N = x.shape[0], x.shape[1] // 2
+        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        with _lib.on_device(x.device):
+            _lib.call('motif_b200_swiglu_train', x.data_ptr(), y.data_ptr(), M, N, x.stride(0), N,
+                      _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
+        ctx.save_for_backward(x)
+        return y
+
+    @staticmethod
+    @first_order
+    def backward(ctx, dy):
+        x, = ctx.saved_tensors
+        dy = _c(dy)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        M, N = dy.shape
+        with _lib.on_device(x.device):
+            _lib.call('motif_b200_swiglu_backward', x.data_ptr(), dy.data_ptr(), dx.data_ptr(), M, N, x.stride(0),
+                      dy.stride(0), dx.stride(0), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
+        return dx

@@ -2,11 +2,10 @@
 
 Same names, argument meanings, return values and exception types as
 `motif/ops/__init__.py:1-10` (plus `apply_block_attn_res`, `motif/ops/attn_res.py:596`),
-computed by the sm_100a kernels of `libmotif_b200.so`.  The delta rule, Chord attention and
-the attn-res read take gradients the way the reference's do (autograd Functions over the
-backward kernels, `motif_b200.autograd`); the norm / SwiGLU modules are forward-only and raise
-for inputs that require a gradient.  CPU tensors raise `ValueError`; there is no eager
-fallback.
+computed by the sm_100a kernels of `libmotif_b200.so`.  The delta rule, Chord attention, the
+attn-res read, the norms and SwiGLU take gradients the way the reference's do (autograd Functions
+over the backward kernels, `motif_b200.autograd`).  CPU tensors raise `ValueError`; there is no
+eager fallback.
 """
 
 from typing import Optional, Sequence
@@ -15,12 +14,13 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .autograd import AttnResFunction, ChordAttentionFunction, GatedDeltaRuleFunction, needs_grad
+from .autograd import (AttnResFunction, ChordAttentionFunction, GatedDeltaRuleFunction, RMSNormFunction,
+                       SwiGLUFunction, needs_grad)
 from .paged import kv4_append, kv4_chord_attention, kv4_gather, kv4_pool, paged_release, paged_reserve
 from .sampler import Sampler, make_sampler  # noqa: F401  (install targets)
 
 __all__ = [
-    'RMSNorm', 'GatedRMSNorm', 'SwiGLU', 'apply_chord_attention', 'HAS_TRITON',
+    'RMSNorm', 'GatedRMSNorm', 'SwiGLU', 'rms_norm', 'gated_rms_norm', 'swiglu', 'apply_chord_attention', 'HAS_TRITON',
     'recurrent_gated_delta_rule', 'chunk_gated_delta_rule', 'chunk_gated_delta_rule_triton',
     'attn_res_block', 'can_use_triton_attn_res', 'apply_block_attn_res', 'MAX_SRC',
     'kv4_pool', 'paged_reserve', 'paged_release', 'kv4_append', 'kv4_gather', 'kv4_chord_attention',
@@ -38,11 +38,6 @@ def _cuda(name, t):
     if not t.is_cuda:
         raise ValueError(f'{name} must live on CUDA')
     return t
-
-
-def _no_grad(*ts):
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts):
-        raise NotImplementedError('motif_b200 ops are forward-only (no autograd)')
 
 
 def _last_contig(t):
@@ -261,8 +256,82 @@ def apply_block_attn_res(cache, query: torch.Tensor, norm) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------ norms / activation
+def _rows(name, x, weight=None, dim=None):
+    """x as rows [M, N] whose elements lie next to each other, after the checks that a norm or an
+    activation makes of its tensors."""
+    _cuda('x', x)
+    if x.dim() < 1:
+        raise ValueError(f'{name}: x must have a last dimension')
+    _lib.dtype_code(x.dtype)
+    if weight is not None:
+        _cuda('weight', weight)
+        if weight.shape != (dim,):
+            raise ValueError(f'{name}: weight must be [{dim}], got {tuple(weight.shape)}')
+        if weight.device != x.device:
+            raise ValueError(f'{name}: weight is on {weight.device}, x on {x.device}')
+        _lib.dtype_code(weight.dtype)
+    return _last_contig(x.reshape(-1, x.shape[-1]))
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """`x * rsqrt(mean(x^2) + eps) * weight` over the last dimension (`motif/ops/rms_norm.py:461-486`).
+
+    Where x or the weight needs a gradient, the forward is computed in fp32 and rounded once, with a
+    weight of any dtype (fp32 next to 16-bit x); else as the eager reference does it, with the weight
+    in x's dtype and every intermediate result rounded to it."""
+    x2 = _rows('rms_norm', x, weight, x.shape[-1] if isinstance(x, torch.Tensor) and x.dim() else None)
+    M, N = x2.shape
+    if needs_grad(x, weight):
+        return RMSNormFunction.apply(x2, None if weight is None else weight.contiguous(), float(eps),
+                                     False).reshape(x.shape)
+    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+    w = None if weight is None else weight.to(x.dtype).contiguous()
+    with _lib.on_device(x.device):
+        _lib.call('motif_b200_rms_norm', _lib.ptr(x2), _lib.ptr(w), _lib.ptr(y), M, N, x2.stride(0), y.stride(0),
+                  float(eps), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
+    return y.reshape(x.shape)
+
+
+def gated_rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """`rms_norm(values) * weight * silu(gate)`, x = [values | gate] along the last dimension
+    (`motif/ops/rms_norm.py:530-553`); rounding as in `rms_norm`."""
+    _cuda('x', x)
+    if x.dim() < 1 or x.shape[-1] % 2:
+        raise ValueError(f'gated_rms_norm: x must be [..., 2 * dim], got {tuple(x.shape)}')
+    N = x.shape[-1] // 2
+    x2 = _rows('gated_rms_norm', x, weight, N)
+    if needs_grad(x, weight):
+        y = RMSNormFunction.apply(x2, None if weight is None else weight.contiguous(), float(eps), True)
+        return y.reshape(*x.shape[:-1], N)
+    y = torch.empty((x2.shape[0], N), dtype=x.dtype, device=x.device)
+    w = None if weight is None else weight.to(x.dtype).contiguous()
+    with _lib.on_device(x.device):
+        _lib.call('motif_b200_gated_rms_norm', _lib.ptr(x2), _lib.ptr(w), _lib.ptr(y), x2.shape[0], N, x2.stride(0),
+                  y.stride(0), float(eps), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
+    return y.reshape(*x.shape[:-1], N)
+
+
+def swiglu(x: torch.Tensor, dim: int = -1) -> torch.Tensor:
+    """`values * silu(gate)`, x = [values | gate] along `dim` (`motif/ops/swiglu.py:239-253`);
+    rounding as in `rms_norm`."""
+    _cuda('x', x)
+    if dim not in (-1, x.dim() - 1):
+        return swiglu(x.movedim(dim, -1)).movedim(-1, dim)
+    if x.dim() < 1 or x.shape[-1] % 2:
+        raise ValueError('SwiGLU needs an even split dimension')
+    x2 = _rows('swiglu', x)
+    M, N = x2.shape[0], x2.shape[1] // 2
+    if needs_grad(x):
+        return SwiGLUFunction.apply(x2).reshape(*x.shape[:-1], N)
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    with _lib.on_device(x.device):
+        _lib.call('motif_b200_swiglu', _lib.ptr(x2), _lib.ptr(y), M, N, x2.stride(0), y.stride(0),
+                  _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
+    return y.reshape(*x.shape[:-1], N)
+
+
 class RMSNorm(nn.Module):
-    """`RMSNorm` (`motif/ops/rms_norm.py:419-486`) on the CUDA kernel; parameter `weight`."""
+    """`RMSNorm` (`motif/ops/rms_norm.py:419-486`) on the CUDA kernels; parameter `weight`."""
 
     def __init__(self, dim, eps=1e-6, elementwise_affine=True, use_triton=True):
         super().__init__()
@@ -276,16 +345,7 @@ class RMSNorm(nn.Module):
         self.use_triton = bool(use_triton)
 
     def forward(self, x):
-        _cuda('x', x)
-        _no_grad(x, self.weight)
-        N = x.shape[-1]
-        x2 = x.reshape(-1, N)
-        x2 = _last_contig(x2)
-        y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
-        w = None if self.weight is None else self.weight.to(x.dtype).contiguous()
-        _lib.call('motif_b200_rms_norm', _lib.ptr(x2), _lib.ptr(w), _lib.ptr(y), x2.shape[0], N, x2.stride(0),
-                  y.stride(0), float(self.eps), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
-        return y.reshape(x.shape)
+        return rms_norm(x, self.weight, self.eps)
 
 
 class GatedRMSNorm(nn.Module):
@@ -304,15 +364,9 @@ class GatedRMSNorm(nn.Module):
 
     def forward(self, x):
         _cuda('x', x)
-        _no_grad(x, self.weight)
         if x.shape[-1] != 2 * self.dim:
             raise ValueError(f'GatedRMSNorm expects last dim {2 * self.dim}, got {x.shape[-1]}')
-        x2 = _last_contig(x.reshape(-1, 2 * self.dim))
-        y = torch.empty((x2.shape[0], self.dim), dtype=x.dtype, device=x.device)
-        w = None if self.weight is None else self.weight.to(x.dtype).contiguous()
-        _lib.call('motif_b200_gated_rms_norm', _lib.ptr(x2), _lib.ptr(w), _lib.ptr(y), x2.shape[0], self.dim,
-                  x2.stride(0), y.stride(0), float(self.eps), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
-        return y.reshape(*x.shape[:-1], self.dim)
+        return gated_rms_norm(x, self.weight, self.eps)
 
 
 class SwiGLU(nn.Module):
@@ -324,16 +378,4 @@ class SwiGLU(nn.Module):
         self.use_triton = bool(use_triton)
 
     def forward(self, x):
-        _cuda('x', x)
-        _no_grad(x)
-        if self.dim not in (-1, x.dim() - 1):
-            x = x.movedim(self.dim, -1)
-            return self.forward(x).movedim(-1, self.dim)
-        if x.shape[-1] % 2:
-            raise ValueError('SwiGLU needs an even split dimension')
-        n = x.shape[-1] // 2
-        x2 = _last_contig(x.reshape(-1, 2 * n))
-        y = torch.empty((x2.shape[0], n), dtype=x.dtype, device=x.device)
-        _lib.call('motif_b200_swiglu', _lib.ptr(x2), _lib.ptr(y), x2.shape[0], n, x2.stride(0), y.stride(0),
-                  _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
-        return y.reshape(*x.shape[:-1], n)
+        return swiglu(x, self.dim)
