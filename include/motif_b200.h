@@ -183,6 +183,30 @@ MB_API int motif_b200_swiglu_train(const void* x, void* y, int64_t M, int64_t N,
 MB_API int motif_b200_swiglu_backward(const void* x, const void* dy, void* dx, int64_t M, int64_t N, int64_t xs,
                                int64_t ds, int64_t os, int dtype, void* stream);
 
+/* ------------------------------------------------------------------ loss over a vocabulary
+ * Softmax cross entropy of the logits x W^T (x [N, d], rows xs apart; w [V, d], rows ws apart; elements next to
+ * each other; both of `dtype`) with int64 labels [N], without keeping the logits.  Tokens whose label
+ * is ignore_index have no loss and no gradient; a label that is neither that nor in 0 .. V - 1 makes its loss and the
+ * gradients NaN.  reduction: 0 = loss [N] (0 for ignored tokens), 1 = mean over the tokens with a loss (NaN without
+ * any), 2 = sum; fp32.  dx [N, d] and dw [V, d] are contiguous, of `dtype`; either may be NULL.
+ * grad_loss: the gradient of the loss, fp32 [N] (grad_stride apart) or one value.
+ *
+ * The forward pass leaves in `state` what the backward pass needs (the same w, ws, N, V, d, dtype and
+ * reduction); `workspace` is scratch.  Both are device memory at 256-byte boundaries;
+ * motif_b200_linear_cross_entropy_bytes writes three sizes to host memory: the state, the forward
+ * workspace and the backward workspace (the latter at most about 0.4 GB and one fp32 copy of dw).
+ * Replaces F.cross_entropy over lm_head's logits, motif/model/motif.py:184,545-630. */
+MB_API int motif_b200_linear_cross_entropy_bytes(const void* w, int64_t ws, int64_t N, int64_t V, int64_t d, int dtype,
+                                          int64_t* bytes);
+MB_API int motif_b200_linear_cross_entropy(const void* x, int64_t xs, const void* w, int64_t ws, const int64_t* labels,
+                                    int64_t ignore_index, int reduction, float* loss, int64_t N, int64_t V,
+                                    int64_t d, void* state, int64_t state_bytes, void* workspace,
+                                    int64_t workspace_bytes, int dtype, void* stream);
+MB_API int motif_b200_linear_cross_entropy_backward(const void* w, int64_t ws, const float* grad_loss,
+                                             int64_t grad_stride, int reduction, void* dx, void* dw, int64_t N,
+                                             int64_t V, int64_t d, void* state, int64_t state_bytes, void* workspace,
+                                             int64_t workspace_bytes, int dtype, void* stream);
+
 /* ------------------------------------------------------------------ fused model kernels
  * These replace sequences of reference statements inside one layer; each cites them.
  * Token-major activations: row r = b*T + t, element stride 1 within a row.

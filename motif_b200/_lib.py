@@ -47,6 +47,11 @@ SIGNATURES = {
     'motif_b200_rms_norm_backward': (_I, [_P, _P, _I, _P, _P, _P] + [_I64] * 5 + [_I, _F, _P, _I64, _I, _P]),
     'motif_b200_swiglu_train': (_I, [_P, _P] + [_I64] * 4 + [_I, _P]),
     'motif_b200_swiglu_backward': (_I, [_P, _P, _P] + [_I64] * 5 + [_I, _P]),
+    'motif_b200_linear_cross_entropy_bytes': (_I, [_P] + [_I64] * 4 + [_I, _P]),
+    'motif_b200_linear_cross_entropy': (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _P] + [_I64] * 3
+                                        + [_P, _I64, _P, _I64, _I, _P]),
+    'motif_b200_linear_cross_entropy_backward': (_I, [_P, _I64, _P, _I64, _I, _P, _P] + [_I64] * 3
+                                                 + [_P, _I64, _P, _I64, _I, _P]),
     'motif_b200_attn_res_norm': (_I, [_P, _I, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F, _F, _I, _P]),
     'motif_b200_gdn_prep': (_I, [_P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                                  _I64, _I, _P]),
@@ -197,6 +202,8 @@ KERNELS_PER_CALL.update({'motif_b200_last_error': 0, 'motif_b200_abi_version': 0
                          'motif_b200_chord_workspace_bytes': 0, 'motif_b200_chord_decode_workspace_bytes': 0,
                          'motif_b200_skinny_packed_bytes': 0, 'motif_b200_gdn_chunk_workspace_bytes': 0,
                          'motif_b200_chord_backward_workspace_bytes': 0, 'motif_b200_gdn_backward_workspace_bytes': 0,
+                         'motif_b200_linear_cross_entropy_bytes': 0, 'motif_b200_linear_cross_entropy': 3,
+                         'motif_b200_linear_cross_entropy_backward': 7,
                          'motif_b200_rms_norm_backward_workspace_bytes': 0, 'motif_b200_rms_norm_backward': 2,
                          'motif_b200_chord_backward': 2, 'motif_b200_kv4_chord_attention': 2,
                          'motif_b200_kv4_unit_bytes': 0, 'motif_b200_kv4_attention_workspace_bytes': 0,

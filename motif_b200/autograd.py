@@ -224,3 +224,52 @@ class SwiGLUFunction(torch.autograd.Function):
             _lib.call('motif_b200_swiglu_backward', x.data_ptr(), dy.data_ptr(), dx.data_ptr(), M, N, x.stride(0),
                       dy.stride(0), dx.stride(0), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
         return dx
+
+
+REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
+
+
+def cross_entropy_forward(x, weight, labels, ignore_index, reduction):
+    """Losses of the rows of x [N, d] and what the backward pass needs of them (a device buffer)."""
+    N, d = x.shape
+    V, ws, dc = weight.shape[0], weight.stride(0), _lib.dtype_code(x.dtype)
+    with _lib.on_device(x.device):
+        sizes = _lib.i64_array((0, 0, 0))
+        _lib.call('motif_b200_linear_cross_entropy_bytes', weight.data_ptr(), ws, N, V, d, dc, sizes)
+        state = torch.empty(sizes[0], dtype=torch.uint8, device=x.device)
+        work = torch.empty(sizes[1], dtype=torch.uint8, device=x.device)
+        loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=x.device)
+        _lib.call('motif_b200_linear_cross_entropy', x.data_ptr(), x.stride(0), weight.data_ptr(), ws,
+                  labels.data_ptr(), ignore_index, reduction, loss.data_ptr(), N, V, d, state.data_ptr(), sizes[0],
+                  work.data_ptr(), sizes[1], dc, _lib.stream_ptr(x.device))
+    return loss, state, sizes[2]
+
+
+class LinearCrossEntropyFunction(torch.autograd.Function):
+    """Softmax cross entropy of the logits x weight^T, which are never kept: the forward pass
+    (`motif_b200_linear_cross_entropy`) leaves the rows that have a loss, their largest logits and
+    sums, the backward pass (`motif_b200_linear_cross_entropy_backward`) computes the logits again,
+    a piece of the vocabulary for a run of rows at a time."""
+
+    @staticmethod
+    def forward(ctx, x, weight, labels, ignore_index, reduction):
+        loss, state, ctx.work_bytes = cross_entropy_forward(x, weight, labels, ignore_index, reduction)
+        ctx.save_for_backward(weight, state)
+        ctx.tokens, ctx.reduction = x.shape[0], reduction
+        return loss
+
+    @staticmethod
+    @first_order
+    def backward(ctx, up):
+        weight, state = ctx.saved_tensors
+        (V, d), N = weight.shape, ctx.tokens
+        need_x, need_w = ctx.needs_input_grad[:2]
+        dx = torch.empty((N, d), dtype=weight.dtype, device=weight.device) if need_x else None
+        dw = torch.empty((V, d), dtype=weight.dtype, device=weight.device) if need_w else None
+        work = torch.empty(ctx.work_bytes, dtype=torch.uint8, device=weight.device)
+        with _lib.on_device(weight.device):
+            _lib.call('motif_b200_linear_cross_entropy_backward', weight.data_ptr(), weight.stride(0), up.data_ptr(),
+                      up.stride(0) if ctx.reduction == 0 else 0, ctx.reduction, _lib.ptr(dx), _lib.ptr(dw), N, V, d,
+                      state.data_ptr(), state.numel(), work.data_ptr(), work.numel(), _lib.dtype_code(weight.dtype),
+                      _lib.stream_ptr(weight.device))
+        return dx, dw, None, None, None

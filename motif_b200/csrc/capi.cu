@@ -100,6 +100,21 @@ static int set_smem_attr(const void* func, int bytes) {
 
 int ensure_smem_attr(const void* func, int bytes) { return once_per_device(func, set_smem_attr, bytes); }
 
+// SMs of the current device.
+int multiprocessors() {
+  static int count[64] = {};
+  static std::mutex mu;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!count[dev]) {
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    count[dev] = n > 0 ? n : 148;
+  }
+  return count[dev];
+}
+
 // Testing hooks (motif_b200_testing_force): off unless a test turns them on.
 static std::atomic<int> g_force[MB_FORCE_COUNT];
 

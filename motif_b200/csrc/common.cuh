@@ -28,6 +28,8 @@ int encode_tile_map(CUtensorMap* map, const void* base, int elem_bytes, int rank
 int once_per_device(const void* key, int (*setup)(const void*, int), int arg);
 // Raises a kernel's dynamic shared-memory limit to `bytes` once per device (thread-safe).
 int ensure_smem_attr(const void* func, int bytes);
+// SMs of the current device (148 if it cannot be asked).
+int multiprocessors();
 // True while a test has switched testing knob `knob` on (motif_b200_testing_force).
 bool forced(int knob);
 

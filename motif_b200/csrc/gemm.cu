@@ -37,9 +37,9 @@
 // Every mbarrier wait is bounded; a role whose wait runs out counts itself
 // (motif_b200_wait_timeouts), lets its issued copies / MMAs land and leaves.
 #include <algorithm>
-#include <mutex>
 
 #include "common.cuh"
+#include "pair.cuh"
 
 namespace mb {
 
@@ -114,12 +114,6 @@ struct GemmParams {
   const void* dt_bias;   // [H] model dtype
 };
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
-  asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
-}
 
 struct TileInfo {
   int m0;     // first output row of the tile
@@ -701,54 +695,6 @@ constexpr int kHalfBBytes = (kBN / 2) * kBK * 2;   // 16 KB: this CTA's half of 
 constexpr int kStage2Bytes = kABytes + kHalfBBytes; // 32 KB
 static_assert(kStages2 * kStage2Bytes <= kStages * kStageBytes, "the pair ring fits the one-CTA ring's space");
 
-__device__ __forceinline__ uint32_t cluster_rank2() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync2() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-// shared::cluster address of `local` (a shared::cta address) in CTA `rank` of the cluster
-__device__ __forceinline__ uint32_t map_rank(uint32_t local, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(local), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(dst)), "r"(ncols)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
-}
-// X / W box into this CTA's shared memory, transaction bytes completed on the barrier at
-// shared::cluster address `bar` (the leader's)
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-      "[%4];\n" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                          uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// arrive (once) on the barrier at shared::cluster address `bar` when every MMA this thread issued has completed
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                                                                const __grid_constant__ CUtensorMap tmB2,
@@ -900,20 +846,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_pair_kernel(const __grid_con
   }
 }
 
-int sm_count() {
-  static int count[64] = {};
-  static std::mutex mu;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  std::lock_guard<std::mutex> lock(mu);
-  if (!count[dev]) {
-    int n = 0;
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    count[dev] = n > 0 ? n : 148;
-  }
-  return count[dev];
-}
-
 template <typename T>
 int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t K, GemmParams& p,
                 cudaStream_t st) {
@@ -948,7 +880,7 @@ int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t 
     if (int e = ensure_smem_attr((const void*)kern, kSmemBytes)) return e;
     p.m_tiles = (int)((M + 2 * kBM - 1) / (2 * kBM));
     const int64_t ntiles = (int64_t)p.m_tiles * p.n_tiles;
-    const int npairs = (int)std::min<int64_t>(ntiles, sm_count() / 2);
+    const int npairs = (int)std::min<int64_t>(ntiles, multiprocessors() / 2);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -968,7 +900,7 @@ int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t 
   if (int e = ensure_smem_attr((const void*)kern, kSmemBytes)) return e;
   p.m_tiles = (int)((M + kPrepRows - 1) / kPrepRows);
   const int64_t ntiles = (int64_t)p.m_tiles * p.n_tiles;
-  const int grid = (int)std::min<int64_t>(ntiles, sm_count());
+  const int grid = (int)std::min<int64_t>(ntiles, multiprocessors());
   kern<<<grid, kThreads, kSmemBytes, st>>>(tmA, tmA4, tmB, p);
   return check_launch("gemm");
 }

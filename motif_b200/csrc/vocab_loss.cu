@@ -1,0 +1,1277 @@
+// Softmax cross entropy of a linear head over a large vocabulary, without its logits.
+//
+//   s = x W^T (x [N, d], W [V, d]),  loss_n = log sum_v exp(s_nv) - s_n,t(n)
+//   G_nv = g_n (exp(s_nv) / sum - [v = t(n)]),  dx = G W,  dW = G^T x
+// (g_n: the gradient that arrives at loss_n.)  Tokens whose label is `ignore_index` are left out of all
+// of it: the rows that have a loss are packed together first, so they cost no arithmetic, and a NaN
+// or an infinity in a padded row reaches nothing.
+//
+// Everything that is a product runs on the tensor cores of CTA pairs (tcgen05 cta_group::2, tiles of
+// 256 x 256, operands by TMA, fp32 sums in TMEM):
+//   scores   a tile of s per step.  Forward: a thread owns a row and keeps its running maximum and sum
+//            of exponentials across all vocabulary tiles that its pair walks; the logits are never
+//            written.  Backward: the tile is computed again and leaves as G, in the operands' type,
+//            into a buffer that holds a piece of the vocabulary for a run of rows.
+//   product  dx += G W and dW += G^T x of that piece.  W, x and (for dW) G are read with the summed
+//            dimension along the rows (MN-major operands), so nothing is transposed.
+// Work: 2 N V d flops forward, 6 backward (the scores again, two products); the tensor cores bound it.
+//
+// Types.  16-bit operands enter as they are; G is rounded to their type once (its relative rounding,
+// 2^-9 or 2^-12, is what the last rounding of dx and dW makes as well).  G is kept between -1 and 1 (times
+// 2^15 in fp16, whose smallest normal number is 2^-14: a probability keeps its bits down to 2^-29), and
+// what g_n has beyond is multiplied in at the end.  fp32 operands are split into three bf16 parts
+// each (24 bits), and the six products of parts that matter are summed, the small ones first.
+//
+// Every wait is bounded; a CTA whose wait runs out counts itself (motif_b200_wait_timeouts), lets what
+// it issued land, and leaves NaN in the tiles that it owes.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "pair.cuh"
+
+namespace mb {
+
+__device__ unsigned int g_vocab_wait_timeouts = 0;
+
+namespace {
+
+constexpr int kTile = 256;               // rows and columns of a pair's tile
+constexpr int kBK = 64;                  // summed elements of a stage
+constexpr int kOperand = 128 * kBK * 2;  // bytes of one operand's stage in one CTA: 128 rows or columns
+constexpr int kStage = 2 * kOperand;
+constexpr int kStages = 6;
+constexpr int kThreads = 192;            // a copying warp, an issuing warp, four warps for the tile's end
+constexpr int kEnd = 4 * 4096;           // two 2 KB store buffers for each of the four
+constexpr int kSmem = kStages * kStage + kEnd + 256 + 1024;
+constexpr uint32_t kWait = 1u << 22;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kHalfScale = 32768.0f;   // of G in fp16
+
+// Which parts of the two operands a step multiplies: one part, or the six products of three parts whose
+// size is 2^-16 of the whole and more, the small ones first (each sum then rounds at its own size).
+template <int P> struct Parts;
+template <> struct Parts<1> {
+  static constexpr int n = 1;
+  __device__ static int a(int) { return 0; }
+  __device__ static int b(int) { return 0; }
+};
+template <> struct Parts<3> {
+  static constexpr int n = 6;
+  __device__ static int a(int i) { return (0x201100 >> (4 * (5 - i))) & 15; }
+  __device__ static int b(int i) { return (0x021010 >> (4 * (5 - i))) & 15; }
+};
+// The type of operands in shared memory: 16-bit tensors' own, bf16 for the parts of fp32.
+template <typename T> using Op = typename std::conditional<std::is_same<T, float>::value, __nv_bfloat16, T>::type;
+template <typename T> constexpr int kParts = std::is_same<T, float>::value ? 3 : 1;
+
+struct RowStat {
+  float top, inv;  // the largest logit; 1 / sum of exp(s - top)
+};
+
+// ------------------------------------------------------------------------------- the pair's pipeline
+struct Smem {
+  unsigned char* ring;
+  unsigned char* end;
+  uint64_t *full, *empty, *tfull, *tempty, *mdone;
+  uint32_t* tmem;
+};
+__device__ __forceinline__ Smem carve(unsigned char* raw) {
+  Smem s;
+  s.ring = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  s.end = s.ring + kStages * kStage;
+  s.full = reinterpret_cast<uint64_t*>(s.end + kEnd);
+  s.empty = s.full + kStages;
+  s.tfull = s.empty + kStages;
+  s.tempty = s.tfull + 2;
+  s.mdone = s.tempty + 2;
+  s.tmem = reinterpret_cast<uint32_t*>(s.mdone + 1);
+  return s;
+}
+__device__ __forceinline__ uint32_t pair_begin(const Smem& s) {
+  if (threadIdx.x < 32) tmem_alloc_pair(s.tmem, 512);
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.tfull[i], 1);
+      mbar_init(&s.tempty[i], 8);  // four warps of both CTAs
+    }
+    mbar_init(s.mdone, 1);
+    mbar_init_fence();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync2();  // both CTAs' barriers exist before a copy or an arrival crosses the pair
+  tc_fence_after();
+  return *s.tmem;
+}
+__device__ __forceinline__ void pair_end(uint32_t tmem) {
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync2();  // every MMA, copy and arrival of the pair is done
+  if (threadIdx.x < 32) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// The copying thread: `it` counts stages over the kernel's life.  Returns the stage's memory, or null
+// when the wait for it ran out.
+__device__ __forceinline__ unsigned char* stage_begin(const Smem& s, int it, bool leader, uint32_t& bar) {
+  const int st = it % kStages;
+  if (!mbar_wait_bounded(&s.empty[st], (uint32_t)(((it / kStages) & 1) ^ 1), kWait)) return nullptr;
+  bar = map_rank(smem_u32(&s.full[st]), 0);
+  if (leader) mbar_arrive_expect_tx(&s.full[st], 2 * kStage);
+  return s.ring + st * kStage;
+}
+__device__ __forceinline__ void copies_failed(const Smem& s, int it, bool leader) {
+  atomicAdd(&g_vocab_wait_timeouts, 1u);
+  if (leader)  // what was issued lands before the CTA leaves
+    for (int u = max(0, it - kStages); u < it; ++u)
+      mbar_wait_bounded(&s.full[u % kStages], (uint32_t)((u / kStages) & 1), kWait);
+}
+
+// The leader's issuing thread: one tile's MMAs over `steps` stages.  MN-major operands keep 64 rows of
+// the summed dimension for each block of 64 rows or columns: 2 KB further for 16 of them, 8 KB for the
+// next block.
+template <bool A_MN, bool B_MN>
+__device__ __forceinline__ bool issue_tile(const Smem& s, uint32_t d, uint32_t idesc, int steps, int& it) {
+  for (int i = 0; i < steps; ++i, ++it) {
+    const int st = it % kStages;
+    if (!mbar_wait_bounded(&s.full[st], (uint32_t)((it / kStages) & 1), kWait)) return false;
+    tc_fence_after();
+    const uint32_t a = smem_u32(s.ring + st * kStage), b = a + kOperand;
+#pragma unroll
+    for (int k = 0; k < kBK / 16; ++k)
+      umma_pair(d, A_MN ? umma_desc_sw128(a + k * 2048, 8192, 1024) : umma_desc_sw128(a + k * 32, 16, 1024),
+                B_MN ? umma_desc_sw128(b + k * 2048, 8192, 1024) : umma_desc_sw128(b + k * 32, 16, 1024), idesc,
+                (i > 0 || k > 0) ? 1u : 0u);
+    const uint32_t e = smem_u32(&s.empty[st]);
+    umma_commit_pair(e);
+    umma_commit_pair(map_rank(e, 1));
+  }
+  return true;
+}
+__device__ __forceinline__ bool tile_free(const Smem& s, int done) {
+  const bool ok = mbar_wait_bounded(&s.tempty[done & 1], (uint32_t)(((done >> 1) & 1) ^ 1), kWait);
+  tc_fence_after();
+  return ok;
+}
+__device__ __forceinline__ void tile_issued(const Smem& s, int done) {
+  const uint32_t f = smem_u32(&s.tfull[done & 1]);
+  umma_commit_pair(f);
+  umma_commit_pair(map_rank(f, 1));
+}
+__device__ __forceinline__ void issue_end(const Smem& s, bool failed) {
+  umma_commit_pair(smem_u32(s.mdone));  // every MMA issued, after a failure too
+  if (!mbar_wait_bounded(s.mdone, 0, kWait) || failed) atomicAdd(&g_vocab_wait_timeouts, 1u);
+}
+// A warp of the tile's end: the tile's sums are there (false: never; `lost` then stays set).
+__device__ __forceinline__ void tile_ready(const Smem& s, int done, bool& lost) {
+  if (lost) return;
+  const bool ok = mbar_wait_bounded(&s.tfull[done & 1], (uint32_t)((done >> 1) & 1), kWait);
+  if (__any_sync(0xffffffffu, !ok)) {
+    lost = true;
+    if ((threadIdx.x & 31) == 0) atomicAdd(&g_vocab_wait_timeouts, 1u);
+  }
+  tc_fence_after();
+}
+__device__ __forceinline__ void tile_read(const Smem& s, int done, bool lost, bool leader) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0 && !lost) {
+    if (leader)
+      mbar_arrive(&s.tempty[done & 1]);
+    else
+      mbar_arrive_remote(map_rank(smem_u32(&s.tempty[done & 1]), 0));
+  }
+}
+// 32 columns of this thread's row; NaN where the tile never came.
+__device__ __forceinline__ void read32(uint32_t taddr, bool lost, uint32_t (&r)[32]) {
+  if (!lost) {
+    tmem_ld32(taddr, r);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = 0x7fffffffu;
+}
+__device__ __forceinline__ void read32_wait(bool lost, uint32_t (&r)[32]) {
+  if (!lost) tmem_wait_ld(r);
+}
+
+// ------------------------------------------------------------------------------- packing
+struct PackArgs {
+  const void* x;           // [N, d], rows xs apart
+  const int64_t* labels;   // [N]
+  int64_t N, xs, ignore;
+  int V, d, dp;            // dp: row length of the packed operand
+  int64_t rows;            // packed rows of a part (N rounded up to a tile)
+  void* packed;            // [parts][rows][dp]
+  int* count;              // tokens that have a loss
+  int* ticket;             // zeroed here for the joining kernel
+  const int* group;        // tokens with a loss in each run of 256, or null: the labels are read instead
+  int* label;              // [rows]: of the packed rows, -1 where it is not one of V
+  int* index;              // [rows]: of the packed rows, where they came from
+  int* place;              // [N]: the packed row of a token, -1 without one
+  float* loss;             // per-token losses: 0 is written for tokens without one (null: no such output)
+};
+
+__global__ void __launch_bounds__(256) group_count_kernel(const int64_t* __restrict__ labels, int64_t N, int64_t ignore,
+                                                          int* __restrict__ group) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int n = __syncthreads_count(i < N && labels[i] != ignore);
+  if (threadIdx.x == 0) group[blockIdx.x] = n;
+}
+
+// x as the sum of three bf16 numbers (exact but for what lies below 2^-24 of x).
+__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
+  p[0] = __float2bfloat16_rn(x);
+  if (__hisinf(p[0])) {
+    p[1] = p[2] = __float2bfloat16_rn(0.f);
+    if (isinf(x)) return;  // an infinity stays one: its remainder would be a NaN
+    p[0] = __float2bfloat16_rz(x);  // beyond bf16's largest number: from below
+  }
+  const float r1 = x - __bfloat162float(p[0]);
+  p[1] = __float2bfloat16_rn(r1);
+  p[2] = __float2bfloat16_rn(r1 - __bfloat162float(p[1]));
+}
+// One row of `d` elements into its parts, zeros behind it; a warp.
+template <typename T>
+__device__ __forceinline__ void pack_row(const T* src, int d, Op<T>* dst, int dp, int64_t part, int lane) {
+  if constexpr (kParts<T> == 1) {
+    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0 && d == dp) {  // dp is a multiple of 8
+      for (int c = lane * 8; c < d; c += 256) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+    } else {
+      for (int c = lane; c < dp; c += 32) dst[c] = c < d ? src[c] : from_f<T>(0.f);
+    }
+  } else {
+    for (int c = lane; c < dp; c += 32) {
+      __nv_bfloat16 p[3];
+      split3(c < d ? src[c] : 0.f, p);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) dst[i * part + c] = p[i];
+    }
+  }
+}
+
+// A CTA packs 32 tokens: its eight warps take a token at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
+  __shared__ int part[8], before[8], place[256];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t first = (int64_t)blockIdx.x * 32, run = first / 256 * 256;
+  // tokens with a loss in the runs before this one
+  int n = 0;
+  if (a.group) {
+    for (int64_t i = tid; i < run / 256; i += 256) n += a.group[i];
+  } else {
+    for (int64_t i = tid; i < run; i += 256) n += a.labels[i] != a.ignore;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  const int64_t mine = run + tid;
+  const int64_t label = mine < a.N ? a.labels[mine] : a.ignore;
+  const bool live = label != a.ignore;
+  const unsigned vote = __ballot_sync(0xffffffffu, live);
+  if (lane == 0) {
+    before[warp] = n;
+    part[warp] = __popc(vote);
+  }
+  __syncthreads();
+  int at = 0, total = 0;
+  for (int w = 0; w < 8; ++w) {
+    at += before[w];
+    total += before[w] + part[w];
+    if (w < warp) at += part[w];
+  }
+  at += __popc(vote & ((1u << lane) - 1u));
+  place[tid] = live ? at : -1;
+  if (mine >= first && mine < first + 32 && mine < a.N) {
+    a.place[mine] = live ? at : -1;
+    if (live) {
+      a.label[at] = label >= 0 && label < a.V ? (int)label : -1;
+      a.index[at] = (int)mine;
+    } else if (a.loss) {
+      a.loss[mine] = 0.f;
+    }
+  }
+  __syncthreads();
+  const T* x = reinterpret_cast<const T*>(a.x);
+  Op<T>* out = reinterpret_cast<Op<T>*>(a.packed);
+  const int64_t plane = a.rows * a.dp;
+  for (int i = warp; i < 32; i += 8) {
+    const int64_t token = first + i;
+    if (token >= a.N) break;
+    const int to = place[token - run];
+    if (to >= 0) pack_row<T>(x + token * a.xs, a.d, out + (int64_t)to * a.dp, a.dp, plane, lane);
+  }
+  // the last CTA sees all tokens: it leaves their number and zeros up to the end of the last tile
+  if (first + 32 >= a.N) {
+    const int64_t end = min(a.rows, (int64_t)(total + kTile - 1) / kTile * kTile);
+    for (int64_t r = total + warp; r < end; r += 8)
+      for (int p = 0; p < kParts<T>; ++p)
+        for (int c = lane; c < a.dp; c += 32) out[p * plane + r * a.dp + c] = from_f<Op<T>>(0.f);
+    if (tid == 0) {
+      *a.count = total;
+      *a.ticket = 0;
+    }
+  }
+}
+
+// The weight as an operand, where it cannot be one itself: fp32, or rows that are not 16-byte aligned.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_weight_kernel(const T* __restrict__ w, int64_t ws, int V, int d, int dp,
+                                                          int64_t rows, Op<T>* __restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  const int64_t plane = rows * dp;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    if (r < V)
+      pack_row<T>(w + r * ws, d, out + r * dp, dp, plane, lane);
+    else
+      for (int p = 0; p < kParts<T>; ++p)
+        for (int c = lane; c < dp; c += 32) out[p * plane + r * dp + c] = from_f<Op<T>>(0.f);
+  }
+}
+
+// ------------------------------------------------------------------------------- scores
+struct ScoreArgs {
+  const int* count;         // tokens with a loss
+  int row0, rows;           // this call's packed rows: row0 .. row0 + rows
+  int v0, nv;               // its vocabulary: v0 .. v0 + nv
+  int kblocks;
+  int64_t x_part, w_part;   // rows from one part of an operand to the next
+  const int* label;         // [rows of the packed operand]
+  float2* seg;              // forward: (maximum, sum) of each row of a pair's run through a row tile
+  float* target;            // forward: the label's logit
+  const RowStat* stat;      // backward
+  const int* index;         // backward: packed row -> token
+  const float* up;          // backward: per-token gradients (null: 1)
+  int64_t up_stride;
+  const float* scale;       // backward: [1] = what `up` is multiplied by (a power of two)
+  int64_t g_part;           // backward: rows from one part of G to the next
+};
+
+// Pair p of np (as many as there are, or as there are tiles) walks the tiles [p T / np, (p + 1) T / np) of the
+// row tiles times nt vocabulary tiles, the vocabulary fastest.  A run through one row tile has the number
+// p + (row tile), which no other has.
+__host__ __device__ __forceinline__ int64_t range_start(int64_t p, int64_t tiles, int64_t np) { return p * tiles / np; }
+__host__ __device__ __forceinline__ int64_t range_owner(int64_t t, int64_t tiles, int64_t np) {
+  return ((t + 1) * np - 1) / tiles;
+}
+
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_constant__ CUtensorMap tmX,
+                                                             const __grid_constant__ CUtensorMap tmW,
+                                                             const __grid_constant__ CUtensorMap tmG,
+                                                             const ScoreArgs a) {
+  using O = Op<T>;
+  constexpr int P = kParts<T>;
+  extern __shared__ unsigned char raw[];
+  const Smem s = carve(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank2();
+  const bool leader = rank == 0;
+  const uint32_t tmem = pair_begin(s);
+  const int np = gridDim.x >> 1, pair = blockIdx.x >> 1;
+  const int live = min(max(*a.count - a.row0, 0), a.rows);
+  const int mt = (live + kTile - 1) / kTile, nt = (a.nv + kTile - 1) / kTile;
+  const int64_t tiles = (int64_t)mt * nt;
+  const int64_t walkers = min((int64_t)np, tiles);
+  const int64_t t0 = pair < walkers ? range_start(pair, tiles, walkers) : 0;
+  const int64_t t1 = pair < walkers ? range_start(pair + 1, tiles, walkers) : 0;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool failed = false;
+      for (int64_t t = t0; t < t1 && !failed; ++t) {
+        const int m = (int)(t / nt), n = (int)(t - (int64_t)m * nt);
+        const int xr = a.row0 + m * kTile + 128 * (int)rank, wr = a.v0 + n * kTile + 128 * (int)rank;
+        for (int p = 0; p < Parts<P>::n && !failed; ++p)
+          for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
+            uint32_t bar;
+            unsigned char* st = stage_begin(s, it, leader, bar);
+            if (!st) {
+              failed = true;
+              break;
+            }
+            tma_load_2d_pair(st, &tmX, kb * kBK, xr + (int)(Parts<P>::a(p) * a.x_part), bar);
+            tma_load_2d_pair(st + kOperand, &tmW, kb * kBK, wr + (int)(Parts<P>::b(p) * a.w_part), bar);
+          }
+      }
+      if (failed) copies_failed(s, it, leader);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      constexpr uint32_t idesc =
+          umma_idesc_f16(std::is_same<O, __nv_bfloat16>::value ? 1u : 0u, kTile, kTile, 0, 0);
+      int it = 0, done = 0;
+      bool failed = false;
+      for (int64_t t = t0; t < t1 && !failed; ++t, ++done) {
+        failed = !tile_free(s, done) ||
+                 !issue_tile<false, false>(s, tmem + (uint32_t)((done & 1) * kTile), idesc, Parts<P>::n * a.kblocks, it);
+        if (!failed) tile_issued(s, done);
+      }
+      issue_end(s, failed);
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;  // the TMEM lanes that this warp can read
+    const int in_tile = (int)rank * 128 + q * 32 + lane;
+    unsigned char* buf = s.end + (warp - 2) * 4096;
+    int slot = 0, done = 0, m_now = -1, label = -1;
+    bool lost = false;
+    float top = -INFINITY, sum = 0.f;      // forward: of the run so far
+    float neg_top = 0.f, inv = 0.f, g = 0.f;  // backward
+    bool mine = false;
+    for (int64_t t = t0; t < t1; ++t, ++done) {
+      const int m = (int)(t / nt), n = (int)(t - (int64_t)m * nt);
+      const int row = a.row0 + m * kTile + in_tile;
+      if (m != m_now) {
+        if constexpr (!GRAD) {
+          if (m_now >= 0) a.seg[(int64_t)(pair + m_now) * kTile + in_tile] = make_float2(top, sum);
+          top = -INFINITY;
+          sum = 0.f;
+        }
+        m_now = m;
+        mine = m * kTile + in_tile < live;
+        label = mine ? a.label[row] : -1;
+        if constexpr (GRAD) {
+          if (mine) {
+            const RowStat st = a.stat[row];
+            g = a.up ? a.up[a.index[row] * a.up_stride] * a.scale[1] : 1.0f;
+            if constexpr (std::is_same<T, __half>::value) g *= kHalfScale;
+            neg_top = -st.top;
+            inv = st.inv * g;
+          }
+        }
+      }
+      const int at = label - (a.v0 + n * kTile);  // the label's column, if it is in this tile
+      const int valid = a.nv - n * kTile;         // columns of the tile that are words
+      const uint32_t taddr = tmem + (uint32_t)((done & 1) * kTile) + ((uint32_t)(q * 32) << 16);
+      tile_ready(s, done, lost);
+      uint32_t r[32];
+      read32(taddr, lost, r);
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 32) {
+        read32_wait(lost, r);
+        float z[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(r[i]);
+        if (c + 32 < kTile) read32(taddr + c + 32, lost, r);  // on its way behind this chunk's arithmetic
+        const bool here = (unsigned)(at - c) < 32u;
+        if constexpr (!GRAD) {
+          if (__any_sync(0xffffffffu, here)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (at == c + i) a.target[row] = z[i];
+          }
+          if (valid < c + 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c + i >= valid) z[i] = -INFINITY;
+          }
+          float t4[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            t4[j] = fmax3(z[8 * j], z[8 * j + 1], z[8 * j + 2]);
+            t4[j] = fmax3(t4[j], z[8 * j + 3], z[8 * j + 4]);
+            t4[j] = fmax3(t4[j], z[8 * j + 5], z[8 * j + 6]);
+            t4[j] = fmaxf(t4[j], z[8 * j + 7]);
+          }
+          const float now = fmaxf(fmax3(t4[0], t4[1], t4[2]), fmaxf(t4[3], top));
+          const float ref = now == -INFINITY ? 0.f : now;
+          const float2 nref = make_float2(-ref, -ref), c2 = make_float2(kLog2e, kLog2e);
+          float2 acc = make_float2(sum * ex2f_((top - ref) * kLog2e), 0.f);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float2 e = fmul2(fadd2(make_float2(z[i], z[i + 1]), nref), c2);
+            acc = fadd2(acc, make_float2(ex2f_(e.x), ex2f_(e.y)));
+          }
+          top = now;
+          sum = acc.x + acc.y;
+        } else {
+          const float2 nref = make_float2(neg_top, neg_top), c2 = make_float2(kLog2e, kLog2e), i2 = make_float2(inv, inv);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float2 e = fmul2(fadd2(make_float2(z[i], z[i + 1]), nref), c2);
+            const float2 w = fmul2(make_float2(ex2f_(e.x), ex2f_(e.y)), i2);
+            z[i] = w.x;
+            z[i + 1] = w.y;
+          }
+          if (__any_sync(0xffffffffu, here)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (at == c + i) z[i] -= g;
+          }
+          if (!mine || valid < c + 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!mine || c + i >= valid) z[i] = 0.f;
+          }
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              w[i] = pack2<O>(z[2 * i], z[2 * i + 1]);
+              if (p + 1 < P) {
+                const float2 back = round2<O>(z[2 * i], z[2 * i + 1]);
+                z[2 * i] -= back.x;
+                z[2 * i + 1] -= back.y;
+              }
+            }
+            // two buffers of 32 rows x 64 bytes in turn, in the 64-byte swizzle of the tensor map
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
+            __syncwarp();
+            unsigned char* b = buf + slot * 2048;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              *reinterpret_cast<uint4*>(b + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) =
+                  make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
+                               reinterpret_cast<uint64_t>(&tmG)),
+                           "r"(n * kTile + c), "r"((int)(p * a.g_part) + m * kTile + (int)rank * 128 + q * 32),
+                           "r"(smem_u32(b))
+                           : "memory");
+              asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+            }
+            slot ^= 1;
+          }
+        }
+      }
+      tile_read(s, done, lost, leader);
+    }
+    if constexpr (GRAD) {
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+      __syncwarp();
+    } else {
+      if (m_now >= 0) a.seg[(int64_t)(pair + m_now) * kTile + in_tile] = make_float2(top, sum);
+    }
+  }
+  pair_end(tmem);
+}
+
+// ------------------------------------------------------------------------------- the loss
+struct JoinArgs {
+  const int* count;
+  int* ticket;
+  const float2* seg;
+  const float* target;
+  const int* label;
+  const int* index;
+  RowStat* stat;
+  float* loss;       // [N] or one value
+  double* partial;   // one a CTA
+  float* denom;      // 1 / tokens with a loss, for the backward pass
+  int nt, np;        // of the scores
+  int reduction;     // 0 none, 1 mean, 2 sum
+};
+
+__global__ void __launch_bounds__(kTile) join_kernel(const JoinArgs a) {
+  __shared__ double sums[kTile / 32];
+  __shared__ int last;
+  const int live = *a.count, m = blockIdx.x, row = m * kTile + threadIdx.x;
+  const int mt = (live + kTile - 1) / kTile;
+  if (m >= mt && m > 0) return;  // the first CTA is there for a call without tokens, too
+  double loss = 0.0;
+  if (row < live) {
+    const int64_t tiles = (int64_t)mt * a.nt, walkers = min((int64_t)a.np, tiles);
+    const int p0 = (int)range_owner((int64_t)m * a.nt, tiles, walkers);
+    const int p1 = (int)range_owner((int64_t)(m + 1) * a.nt - 1, tiles, walkers);
+    float top = -INFINITY;
+    for (int p = p0; p <= p1; ++p) top = fmaxf(top, a.seg[(int64_t)(p + m) * kTile + threadIdx.x].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int p = p0; p <= p1; ++p) {
+      const float2 v = a.seg[(int64_t)(p + m) * kTile + threadIdx.x];
+      sum += v.y * ex2f_((v.x - ref) * kLog2e);
+    }
+    const bool known = a.label[row] >= 0;
+    const float nan = __int_as_float(0x7fffffff);
+    RowStat st;
+    st.top = ref;
+    st.inv = known ? 1.0f / sum : nan;  // a label that is no word: NaN, in the gradients too
+    a.stat[row] = st;
+    const float one = known ? (ref - a.target[row]) + logf(sum) : nan;
+    if (a.reduction == 0) a.loss[a.index[row]] = one;
+    loss = one;
+  }
+  if (a.reduction == 0) return;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = loss;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    loss = 0.0;
+    for (int i = 0; i < kTile / 32; ++i) loss += sums[i];
+    a.partial[m] = loss;
+    __threadfence();
+    last = atomicAdd(a.ticket, 1) == max(mt, 1) - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  // the last CTA adds all of them, in one order whoever it is
+  __threadfence();
+  loss = 0.0;
+  for (int i = threadIdx.x; i < mt; i += kTile) loss += __ldcg(a.partial + i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = loss;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    loss = 0.0;
+    for (int i = 0; i < kTile / 32; ++i) loss += sums[i];
+    *a.loss = (float)(a.reduction == 1 ? loss / (double)live : loss);  // no tokens: 0 / 0, as it is
+    *a.denom = (float)(1.0 / (double)live);
+  }
+}
+
+// scale[0]: what dx and dW are multiplied by at the end; scale[1]: what the per-token gradients are
+// multiplied by before (a power of two that brings the largest below 1 or to it).
+__global__ void __launch_bounds__(1024) scale_kernel(const float* __restrict__ up, int64_t up_stride, int64_t N,
+                                                     const int* __restrict__ place, const int* __restrict__ count,
+                                                     int reduction, const float* __restrict__ denom, int half,
+                                                     float* __restrict__ scale) {
+  __shared__ float tops[32];
+  float fold = half ? 1.0f / kHalfScale : 1.0f;
+  if (reduction != 0) {
+    // no token has a loss: the gradients are zero, whatever 0 / 0 says
+    if (threadIdx.x == 0) scale[0] = *count > 0 ? *up * (reduction == 1 ? *denom : 1.0f) * fold : 0.0f;
+    return;
+  }
+  float top = 0.f;
+  for (int64_t i = threadIdx.x; i < N; i += 1024)
+    if (place[i] >= 0) top = fmaxf(top, fabsf(up[i * up_stride]));
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, tops[i]);
+    int e = 0;
+    if (top > 0.f && top <= 3.4e38f) frexpf(top, &e);
+    e = max(-126, min(126, e));
+    scale[0] = ldexpf(1.0f, e) * fold;
+    scale[1] = ldexpf(1.0f, -e);
+  }
+}
+
+// ------------------------------------------------------------------------------- products
+struct ProductArgs {
+  const int* count;
+  int by_rows;              // 1: dx (tile rows are tokens, the sum runs over words); 0: dW (the other way)
+  int row0, rows;           // the packed rows of this call
+  int v0, nv;               // its vocabulary
+  int d;
+  int64_t a_part, b_part;   // rows from one part of an operand to the next
+  float* slots;             // [pairs][256][256]: tiles whose sum is split
+  float* acc;               // [rows or nv][ld] fp32, or null
+  int64_t ld;
+  int first, last;          // first: acc holds nothing yet; last: the result leaves as T
+  const float* scale;
+  void* out;                // dx (rows by `index`) or dW
+  const int* index;
+};
+struct Cut {  // how a product's tiles are spread over the pairs
+  int mt, nt, kb, full, split, units;
+};
+// Whole waves of tiles keep their sum in one pair; of the rest each tile's sum is cut into as many
+// equal parts as there are pairs for it.
+__host__ __device__ __forceinline__ Cut cut_product(const ProductArgs& a, int live, int np) {
+  Cut c;
+  const int m = a.by_rows ? live : a.nv, k = a.by_rows ? (live > 0 ? a.nv : 0) : live;
+  c.mt = (m + kTile - 1) / kTile;
+  c.nt = (a.d + kTile - 1) / kTile;
+  c.kb = (k + kBK - 1) / kBK;
+  const int tiles = c.mt * c.nt, rem = tiles % np;
+  c.full = tiles - rem;
+  c.split = rem > 0 && c.kb > 1 ? min(np / rem, c.kb) : 1;
+  if (c.split <= 1) {
+    c.split = 1;
+    c.full = tiles;
+  }
+  c.units = c.full + (tiles - c.full) * c.split;
+  return c;
+}
+__device__ __forceinline__ int product_live(const ProductArgs& a) { return min(max(*a.count - a.row0, 0), a.rows); }
+struct Unit {
+  int m, n, k0, k1, slot;  // slot < 0: a whole tile
+};
+__device__ __forceinline__ Unit unit_at(const Cut& c, int u) {
+  Unit r;
+  int tile = u;
+  r.k0 = 0;
+  r.k1 = c.kb;
+  r.slot = -1;
+  if (u >= c.full) {
+    const int j = u - c.full, part = j % c.split;
+    tile = c.full + j / c.split;
+    r.k0 = (int)((int64_t)part * c.kb / c.split);
+    r.k1 = (int)((int64_t)(part + 1) * c.kb / c.split);
+    r.slot = j;
+  }
+  r.m = tile / c.nt;
+  r.n = tile - r.m * c.nt;
+  return r;
+}
+// 32 columns of a row: what earlier calls left is added; the sum stays in fp32 or leaves as T.
+template <typename T>
+__device__ __forceinline__ void finish32(const ProductArgs& a, int row, int col, float (&v)[32], float scale) {
+  const int n = min(32, a.d - col);
+  if (!a.first) {
+    const float* p = a.acc + (int64_t)row * a.ld + col;
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+      if (i < n) {  // rows are padded to fours
+        const float4 o = *reinterpret_cast<const float4*>(p + i);
+        v[i] += o.x;
+        v[i + 1] += o.y;
+        v[i + 2] += o.z;
+        v[i + 3] += o.w;
+      }
+  }
+  if (!a.last) {
+    float* p = a.acc + (int64_t)row * a.ld + col;
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+      if (i < n) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    return;
+  }
+  const int64_t to = a.by_rows ? a.index[a.row0 + row] : a.v0 + row;
+  T* p = reinterpret_cast<T*>(a.out) + to * a.d + col;
+  constexpr int E = 16 / (int)sizeof(T);
+  if (a.d % E == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < 32; i += E)
+      if (i < n) {
+        __align__(16) T o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = from_f<T>(v[i + e] * scale);
+        *reinterpret_cast<uint4*>(p + i) = *reinterpret_cast<const uint4*>(o);
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) p[i] = from_f<T>(v[i] * scale);
+  }
+}
+
+// A_MN: the left operand's summed dimension runs along its rows (dW); the right one's always does.
+template <typename T, bool A_MN>
+__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ CUtensorMap tmA,
+                                                              const __grid_constant__ CUtensorMap tmB,
+                                                              const ProductArgs a) {
+  using O = Op<T>;
+  constexpr int P = kParts<T>;
+  extern __shared__ unsigned char raw[];
+  const Smem s = carve(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank2();
+  const bool leader = rank == 0;
+  const uint32_t tmem = pair_begin(s);
+  const int np = gridDim.x >> 1, pair = blockIdx.x >> 1;
+  const int live = product_live(a);
+  const Cut c = cut_product(a, live, np);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool failed = false;
+      for (int u = pair; u < c.units && !failed; u += np) {
+        const Unit w = unit_at(c, u);
+        const int cols = (min(kTile, a.d - w.n * kTile) + 31) & ~31;
+        const int ar = w.m * kTile + 128 * (int)rank, bc = w.n * kTile + (int)rank * (cols / 2);
+        // the right operand's rows: words of this piece, or this call's tokens
+        const int br = a.by_rows ? a.v0 : a.row0;
+        for (int p = 0; p < Parts<P>::n && !failed; ++p)
+          for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
+            uint32_t bar;
+            unsigned char* st = stage_begin(s, it, leader, bar);
+            if (!st) {
+              failed = true;
+              break;
+            }
+            const int pa = (int)(Parts<P>::a(p) * a.a_part), pb = (int)(Parts<P>::b(p) * a.b_part);
+            if constexpr (A_MN) {
+              tma_load_2d_pair(st, &tmA, ar, pa + kb * kBK, bar);
+              tma_load_2d_pair(st + 8192, &tmA, ar + 64, pa + kb * kBK, bar);
+            } else {
+              tma_load_2d_pair(st, &tmA, kb * kBK, pa + ar, bar);
+            }
+            tma_load_2d_pair(st + kOperand, &tmB, bc, pb + br + kb * kBK, bar);
+            tma_load_2d_pair(st + kOperand + 8192, &tmB, bc + 64, pb + br + kb * kBK, bar);
+          }
+      }
+      if (failed) copies_failed(s, it, leader);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      int it = 0, done = 0;
+      bool failed = false;
+      for (int u = pair; u < c.units && c.kb > 0 && !failed; u += np, ++done) {
+        const Unit w = unit_at(c, u);
+        const int cols = (min(kTile, a.d - w.n * kTile) + 31) & ~31;
+        const uint32_t idesc =
+            umma_idesc_f16(std::is_same<O, __nv_bfloat16>::value ? 1u : 0u, kTile, cols, A_MN ? 1u : 0u, 1u);
+        failed = !tile_free(s, done) ||
+                 !issue_tile<A_MN, true>(s, tmem + (uint32_t)((done & 1) * kTile), idesc,
+                                         Parts<P>::n * (w.k1 - w.k0), it);
+        if (!failed) tile_issued(s, done);
+      }
+      issue_end(s, failed);
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;
+    const int in_tile = (int)rank * 128 + q * 32 + lane;
+    const float scale = a.last ? a.scale[0] : 1.0f;
+    int done = 0;
+    bool lost = false;
+    for (int u = pair; u < c.units; u += np, ++done) {
+      const Unit w = unit_at(c, u);
+      const int row = w.m * kTile + in_tile, rows = a.by_rows ? live : a.nv;
+      const uint32_t taddr = tmem + (uint32_t)((done & 1) * kTile) + ((uint32_t)(q * 32) << 16);
+      const int cols = min(kTile, a.d - w.n * kTile);
+      if (c.kb > 0) tile_ready(s, done, lost);
+#pragma unroll 1
+      for (int col = 0; col < cols; col += 32) {
+        uint32_t r[32];
+        if (c.kb > 0) {
+          read32(taddr + col, lost, r);
+          read32_wait(lost, r);
+        } else {  // nothing to sum: the result is what earlier calls left, or zero
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        }
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        if (w.slot >= 0) {
+          float* p = a.slots + ((int64_t)w.slot * kTile + in_tile) * kTile + col;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else if (row < rows) {
+          finish32<T>(a, row, w.n * kTile + col, v, scale);
+        }
+      }
+      if (c.kb > 0) tile_read(s, done, lost, leader);
+    }
+  }
+  pair_end(tmem);
+}
+
+// The tiles whose sum was split: their parts are added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_product_kernel(const ProductArgs a, int np) {
+  const int live = product_live(a);
+  const Cut c = cut_product(a, live, np);
+  const int j = blockIdx.x / 8, tile = c.full + j;  // eight CTAs a tile, 32 rows each, 32 columns a thread
+  if (tile >= c.mt * c.nt) return;
+  const int m = tile / c.nt, n = tile - m * c.nt;
+  const int in_tile = (blockIdx.x & 7) * 32 + (threadIdx.x >> 3), col = (threadIdx.x & 7) * 32;
+  const int row = m * kTile + in_tile, rows = a.by_rows ? live : a.nv;
+  if (row >= rows || n * kTile + col >= a.d) return;
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = 0.f;
+  for (int p = 0; p < c.split; ++p) {
+    const float* src = a.slots + ((int64_t)(j * c.split + p) * kTile + in_tile) * kTile + col;
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(src + i);
+      v[i] += o.x;
+      v[i + 1] += o.y;
+      v[i + 2] += o.z;
+      v[i + 3] += o.w;
+    }
+  }
+  finish32<T>(a, row, n * kTile + col, v, a.last ? a.scale[0] : 1.0f);
+}
+
+// Zeros in dx for the tokens without a loss.
+template <typename T>
+__global__ void __launch_bounds__(256) zero_rows_kernel(const int* __restrict__ place, int64_t N, int d, T* __restrict__ dx) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); n < N; n += (int64_t)gridDim.x * 8)
+    if (place[n] < 0)
+      for (int c = lane; c < d; c += 32) dx[n * d + c] = from_f<T>(0.f);
+}
+
+// ------------------------------------------------------------------------------- host
+int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// What the forward pass leaves for the backward one, and what each pass needs besides.
+struct Sizes {
+  int parts;
+  int64_t rows, dp, vrows;  // packed rows, row length, packed words
+  // offsets of the state
+  int64_t x, w, label, index, place, stat, count, ticket, denom, state_bytes;
+  // forward workspace
+  int64_t group, seg, target, partial, forward_bytes;
+  // backward: rows of a run, words of a piece, and the workspace
+  int64_t run, piece, g, slots, dx_acc, dw_acc, scale, backward_bytes;
+};
+// Elements of G that are there at once (16-bit; fp32 keeps three parts of a third as many).
+constexpr int64_t kPiece = 1LL << 27;
+constexpr int64_t kRun = 8192;
+// fp32: sums are added in fp32 after this many terms, since the tensor cores cut each partial sum off
+// (not rounding it) at 24 bits.
+constexpr int64_t kExactRun = 4096;
+
+Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) {
+  Sizes s = {};
+  s.parts = dtype == MB_F32 ? 3 : 1;
+  s.rows = up_to(std::max<int64_t>(N, 1), kTile);
+  s.dp = up_to(d, 8);
+  s.vrows = up_to(V, kTile);
+  auto take = [](int64_t& total, int64_t bytes) {
+    const int64_t at = total;
+    total = up_to(total + bytes, 256);
+    return at;
+  };
+  s.x = take(s.state_bytes, s.parts * s.rows * s.dp * 2);
+  s.w = take(s.state_bytes, pack_w ? s.parts * s.vrows * s.dp * 2 : 0);
+  s.label = take(s.state_bytes, s.rows * 4);
+  s.index = take(s.state_bytes, s.rows * 4);
+  s.place = take(s.state_bytes, N * 4);
+  s.stat = take(s.state_bytes, s.rows * (int64_t)sizeof(RowStat));
+  s.count = take(s.state_bytes, 4);
+  s.ticket = take(s.state_bytes, 4);
+  s.denom = take(s.state_bytes, 4);
+  const int64_t mt = s.rows / kTile;
+  s.group = take(s.forward_bytes, up_to(N, 256) / 256 * 4);
+  s.seg = take(s.forward_bytes, (np + mt) * kTile * (int64_t)sizeof(float2));
+  s.target = take(s.forward_bytes, s.rows * 4);
+  s.partial = take(s.forward_bytes, mt * 8);
+  // a run of rows and a piece of the vocabulary: G of both together stays below kPiece elements
+  const int64_t most = kPiece / s.parts;
+  s.run = std::min(s.rows, s.parts == 3 ? kExactRun : kRun);
+  s.piece = std::min(s.vrows, std::max<int64_t>(kTile, most / s.run / kTile * kTile));
+  if (s.parts == 3) s.piece = std::min(s.piece, kExactRun);
+  if (s.parts == 1) s.run = std::min(s.rows, std::max(s.run, most / s.piece / kTile * kTile));
+  s.g = take(s.backward_bytes, s.parts * s.run * s.piece * 2);
+  s.slots = take(s.backward_bytes, (int64_t)np * kTile * kTile * 4);
+  s.dx_acc = take(s.backward_bytes, s.piece < s.vrows ? s.run * up_to(d, 4) * 4 : 0);
+  s.dw_acc = take(s.backward_bytes, s.run < s.rows ? V * up_to(d, 4) * 4 : 0);
+  s.scale = take(s.backward_bytes, 8);
+  return s;
+}
+
+template <typename K, typename... A>
+int launch_pairs(const char* what, K kern, int np, cudaStream_t st, A... args) {
+  if (int e = ensure_smem_attr((const void*)kern, kSmem)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(2 * np));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, args...);
+  return check_launch(what);
+}
+
+struct Call {
+  const void *x, *w;
+  int64_t xs, ws;
+  const int64_t* labels;
+  int64_t ignore, N, V, d;
+  int reduction, dtype;
+  unsigned char *state, *work;
+  cudaStream_t st;
+  bool pack_w;
+  Sizes s;
+  int np;
+};
+template <typename T> T* at(unsigned char* base, int64_t off) { return reinterpret_cast<T*>(base + off); }
+
+// The weight as rows for the tensor maps: itself, or its packed copy.
+void weight_rows(const Call& c, const void** base, int64_t* rows, int64_t* stride, int64_t* cols) {
+  *base = c.pack_w ? c.state + c.s.w : c.w;
+  *rows = c.pack_w ? c.s.parts * c.s.vrows : c.V;
+  *stride = c.pack_w ? c.s.dp : c.ws;
+  *cols = c.pack_w ? c.s.dp : c.d;
+}
+
+template <typename T>
+int forward(const Call& c, float* loss) {
+  const Sizes& s = c.s;
+  int* group = nullptr;
+  if (c.N > 8192) {  // below that a CTA reads the labels before its own
+    group = at<int>(c.work, s.group);
+    group_count_kernel<<<(unsigned)((c.N + 255) / 256), 256, 0, c.st>>>(c.labels, c.N, c.ignore, group);
+    if (int e = check_launch("linear_cross_entropy (count)")) return e;
+  }
+  PackArgs p = {};
+  p.x = c.x;
+  p.labels = c.labels;
+  p.N = c.N;
+  p.xs = c.xs;
+  p.ignore = c.ignore;
+  p.V = (int)c.V;
+  p.d = (int)c.d;
+  p.dp = (int)s.dp;
+  p.rows = s.rows;
+  p.packed = c.state + s.x;
+  p.count = at<int>(c.state, s.count);
+  p.ticket = at<int>(c.state, s.ticket);
+  p.group = group;
+  p.label = at<int>(c.state, s.label);
+  p.index = at<int>(c.state, s.index);
+  p.place = at<int>(c.state, s.place);
+  p.loss = c.reduction == 0 ? loss : nullptr;
+  pack_kernel<T><<<(unsigned)std::max<int64_t>(1, (c.N + 31) / 32), 256, 0, c.st>>>(p);
+  if (int e = check_launch("linear_cross_entropy (pack)")) return e;
+  if (c.pack_w) {
+    pack_weight_kernel<T><<<(unsigned)std::min<int64_t>((s.vrows + 7) / 8, 148 * 16), 256, 0, c.st>>>(
+        (const T*)c.w, c.ws, (int)c.V, (int)c.d, (int)s.dp, s.vrows, at<Op<T>>(c.state, s.w));
+    if (int e = check_launch("linear_cross_entropy (pack weight)")) return e;
+  }
+  CUtensorMap tmX, tmW;
+  const void* wb;
+  int64_t wr, wst, wc;
+  weight_rows(c, &wb, &wr, &wst, &wc);
+  int rc = encode_tile_map_2d(&tmX, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 128, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmW, wb, 2, wc, wr, wst * 2, kBK, 128, 128);
+  if (rc) return rc;
+  ScoreArgs a = {};
+  a.count = p.count;
+  a.rows = (int)s.rows;
+  a.nv = (int)c.V;
+  a.kblocks = (int)((c.d + kBK - 1) / kBK);
+  a.x_part = s.rows;
+  a.w_part = s.vrows;
+  a.label = p.label;
+  a.seg = at<float2>(c.work, s.seg);
+  a.target = at<float>(c.work, s.target);
+  rc = launch_pairs("linear_cross_entropy (scores)", scores_kernel<T, false>, c.np, c.st, tmX, tmW, tmX, a);
+  if (rc) return rc;
+  JoinArgs j = {};
+  j.count = p.count;
+  j.ticket = p.ticket;
+  j.seg = a.seg;
+  j.target = a.target;
+  j.label = p.label;
+  j.index = p.index;
+  j.stat = at<RowStat>(c.state, s.stat);
+  j.loss = loss;
+  j.partial = at<double>(c.work, s.partial);
+  j.denom = at<float>(c.state, s.denom);
+  j.nt = (int)((c.V + kTile - 1) / kTile);
+  j.np = c.np;
+  j.reduction = c.reduction;
+  join_kernel<<<(unsigned)(s.rows / kTile), kTile, 0, c.st>>>(j);
+  return check_launch("linear_cross_entropy (join)");
+}
+
+template <typename T>
+int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* dw) {
+  const Sizes& s = c.s;
+  const int* count = at<int>(c.state, s.count);
+  const int* place = at<int>(c.state, s.place);
+  const int* index = at<int>(c.state, s.index);
+  float* scale = at<float>(c.work, s.scale);
+  scale_kernel<<<1, c.reduction == 0 ? 1024 : 32, 0, c.st>>>(up, up_stride, c.N, place, count, c.reduction,
+                                                            at<float>(c.state, s.denom),
+                                                            std::is_same<T, __half>::value, scale);
+  if (int e = check_launch("linear_cross_entropy_backward (scale)")) return e;
+  if (dx) {
+    zero_rows_kernel<T><<<(unsigned)std::min<int64_t>((c.N + 7) / 8, 148 * 8), 256, 0, c.st>>>(place, c.N, (int)c.d,
+                                                                                              (T*)dx);
+    if (int e = check_launch("linear_cross_entropy_backward (zero)")) return e;
+  }
+  const void* wb;
+  int64_t wr, wst, wc;
+  weight_rows(c, &wb, &wr, &wst, &wc);
+  CUtensorMap tmX, tmW, tmG, tmXk, tmWk, tmGa, tmGt;
+  unsigned char* g = c.work + s.g;
+  int rc = encode_tile_map_2d(&tmX, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 128, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmW, wb, 2, wc, wr, wst * 2, kBK, 128, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmXk, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, 64, kBK, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmWk, wb, 2, wc, wr, wst * 2, 64, kBK, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmG, g, 2, s.piece, s.parts * s.run, s.piece * 2, 32, 32, 64);    // stored
+  if (!rc) rc = encode_tile_map_2d(&tmGa, g, 2, s.piece, s.parts * s.run, s.piece * 2, kBK, 128, 128);  // tokens x words
+  if (!rc) rc = encode_tile_map_2d(&tmGt, g, 2, s.piece, s.parts * s.run, s.piece * 2, 64, kBK, 128);   // words x tokens
+  if (rc) return rc;
+  for (int64_t r0 = 0; r0 < s.rows; r0 += s.run)
+    for (int64_t v0 = 0; v0 < c.V; v0 += s.piece) {
+      ScoreArgs a = {};
+      a.count = count;
+      a.row0 = (int)r0;
+      a.rows = (int)std::min(s.run, s.rows - r0);
+      a.v0 = (int)v0;
+      a.nv = (int)std::min(s.piece, c.V - v0);
+      a.kblocks = (int)((c.d + kBK - 1) / kBK);
+      a.x_part = s.rows;
+      a.w_part = s.vrows;
+      a.label = at<int>(c.state, s.label);
+      a.stat = at<RowStat>(c.state, s.stat);
+      a.index = index;
+      a.up = c.reduction == 0 ? up : nullptr;
+      a.up_stride = up_stride;
+      a.scale = scale;
+      a.g_part = s.run;
+      rc = launch_pairs("linear_cross_entropy_backward (scores)", scores_kernel<T, true>, c.np, c.st, tmX, tmW, tmG, a);
+      if (rc) return rc;
+      ProductArgs p = {};
+      p.count = count;
+      p.row0 = a.row0;
+      p.rows = a.rows;
+      p.v0 = a.v0;
+      p.nv = a.nv;
+      p.d = (int)c.d;
+      p.a_part = s.run;
+      p.slots = at<float>(c.work, s.slots);
+      p.ld = up_to(c.d, 4);
+      p.scale = scale;
+      p.index = index;
+      if (dx) {
+        p.by_rows = 1;
+        p.b_part = s.vrows;
+        p.acc = at<float>(c.work, s.dx_acc);
+        p.first = v0 == 0;
+        p.last = v0 + s.piece >= c.V;
+        p.out = dx;
+        rc = launch_pairs("linear_cross_entropy_backward (dx)", product_kernel<T, false>, c.np, c.st, tmGa, tmWk, p);
+        if (rc) return rc;
+        join_product_kernel<T><<<(unsigned)(8 * c.np), 256, 0, c.st>>>(p, c.np);
+        if ((rc = check_launch("linear_cross_entropy_backward (dx join)"))) return rc;
+      }
+      if (dw) {
+        p.by_rows = 0;
+        p.b_part = s.rows;
+        p.acc = at<float>(c.work, s.dw_acc) + v0 * p.ld;
+        p.first = r0 == 0;
+        p.last = r0 + s.run >= s.rows;
+        p.out = dw;
+        rc = launch_pairs("linear_cross_entropy_backward (dw)", product_kernel<T, true>, c.np, c.st, tmGt, tmXk, p);
+        if (rc) return rc;
+        join_product_kernel<T><<<(unsigned)(8 * c.np), 256, 0, c.st>>>(p, c.np);
+        if ((rc = check_launch("linear_cross_entropy_backward (dw join)"))) return rc;
+      }
+    }
+  return MB_OK;
+}
+
+// 16-bit weights whose rows the tensor maps can describe are operands themselves.
+bool must_pack(const void* w, int64_t ws, int64_t d, int dtype) {
+  return dtype == MB_F32 || (uintptr_t)w % 16 != 0 || ws % 8 != 0 || ws < d;
+}
+
+int check_sizes(const char* what, int64_t N, int64_t V, int64_t d, int dtype) {
+  MB_REQUIRE(dtype == MB_F32 || dtype == MB_F16 || dtype == MB_BF16, MB_ERR_DTYPE, "%s: unsupported dtype code %d", what,
+             dtype);
+  MB_REQUIRE(N >= 0 && N < (1LL << 29) && V > 0 && V < (1LL << 29) && d > 0 && d < (1LL << 24), MB_ERR_SHAPE,
+             "%s: bad sizes N=%lld V=%lld d=%lld", what, (long long)N, (long long)V, (long long)d);
+  return MB_OK;
+}
+int make_call(const char* what, Call& c) {
+  if (int e = check_sizes(what, c.N, c.V, c.d, c.dtype)) return e;
+  MB_REQUIRE(c.reduction >= 0 && c.reduction <= 2, MB_ERR_ARG, "%s: unknown reduction %d", what, c.reduction);
+  MB_REQUIRE(c.w && c.state && c.work, MB_ERR_ARG, "%s: null pointer", what);
+  MB_REQUIRE(((uintptr_t)c.state | (uintptr_t)c.work) % 256 == 0, MB_ERR_ALIGN,
+             "%s: state and workspace must be 256-byte aligned", what);
+  c.np = std::max(1, multiprocessors() / 2);
+  c.pack_w = must_pack(c.w, c.ws, c.d, c.dtype);
+  c.s = sizes_of(c.N, c.V, c.d, c.pack_w, c.dtype, c.np);
+  return MB_OK;
+}
+
+}  // namespace
+
+int read_and_clear_vocab_timeouts(unsigned int* count) {
+  unsigned int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_vocab_wait_timeouts, sizeof(v)) != cudaSuccess ||
+      cudaMemcpyToSymbol(g_vocab_wait_timeouts, &zero, sizeof(zero)) != cudaSuccess)
+    return set_error(MB_ERR_CUDA, "wait_timeouts: %s", cudaGetErrorString(cudaGetLastError()));
+  *count = v;
+  return MB_OK;
+}
+
+}  // namespace mb
+
+extern "C" int motif_b200_linear_cross_entropy_bytes(const void* w, int64_t ws, int64_t N, int64_t V, int64_t d, int dtype,
+                                                     int64_t* bytes) {
+  using namespace mb;
+  MB_REQUIRE(bytes, MB_ERR_ARG, "linear_cross_entropy_bytes: null pointer");
+  if (int e = check_sizes("linear_cross_entropy_bytes", N, V, d, dtype)) return e;
+  const Sizes s = sizes_of(N, V, d, must_pack(w, ws, d, dtype), dtype, std::max(1, multiprocessors() / 2));
+  bytes[0] = s.state_bytes;
+  bytes[1] = s.forward_bytes;
+  bytes[2] = s.backward_bytes;
+  return MB_OK;
+}
+
+extern "C" int motif_b200_linear_cross_entropy(const void* x, int64_t xs, const void* w, int64_t ws, const int64_t* labels,
+                                               int64_t ignore_index, int reduction, float* loss, int64_t N, int64_t V,
+                                               int64_t d, void* state, int64_t state_bytes, void* workspace,
+                                               int64_t workspace_bytes, int dtype, void* stream) {
+  using namespace mb;
+  Call c = {};
+  c.x = x;
+  c.xs = xs;
+  c.w = w;
+  c.ws = ws;
+  c.labels = labels;
+  c.ignore = ignore_index;
+  c.reduction = reduction;
+  c.N = N;
+  c.V = V;
+  c.d = d;
+  c.dtype = dtype;
+  c.state = (unsigned char*)state;
+  c.work = (unsigned char*)workspace;
+  c.st = (cudaStream_t)stream;
+  if (int e = make_call("linear_cross_entropy", c)) return e;
+  MB_REQUIRE((N == 0 || (x && labels)) && (loss || (N == 0 && reduction == 0)), MB_ERR_ARG,
+             "linear_cross_entropy: null pointer");
+  MB_REQUIRE(state_bytes >= c.s.state_bytes && workspace_bytes >= c.s.forward_bytes, MB_ERR_ARG,
+             "linear_cross_entropy: %lld and %lld bytes of state and workspace needed, got %lld and %lld",
+             (long long)c.s.state_bytes, (long long)c.s.forward_bytes, (long long)state_bytes,
+             (long long)workspace_bytes);
+  if (dtype == MB_F32) return forward<float>(c, loss);
+  return dtype == MB_BF16 ? forward<__nv_bfloat16>(c, loss) : forward<__half>(c, loss);
+}
+
+extern "C" int motif_b200_linear_cross_entropy_backward(const void* w, int64_t ws, const float* grad_loss,
+                                                        int64_t grad_stride, int reduction, void* dx, void* dw, int64_t N,
+                                                        int64_t V, int64_t d, void* state, int64_t state_bytes,
+                                                        void* workspace, int64_t workspace_bytes, int dtype,
+                                                        void* stream) {
+  using namespace mb;
+  Call c = {};
+  c.w = w;
+  c.ws = ws;
+  c.reduction = reduction;
+  c.N = N;
+  c.V = V;
+  c.d = d;
+  c.dtype = dtype;
+  c.state = (unsigned char*)state;
+  c.work = (unsigned char*)workspace;
+  c.st = (cudaStream_t)stream;
+  if (int e = make_call("linear_cross_entropy_backward", c)) return e;
+  MB_REQUIRE(grad_loss || (N == 0 && reduction == 0), MB_ERR_ARG, "linear_cross_entropy_backward: null pointer");
+  MB_REQUIRE(state_bytes >= c.s.state_bytes && workspace_bytes >= c.s.backward_bytes, MB_ERR_ARG,
+             "linear_cross_entropy_backward: %lld and %lld bytes of state and workspace needed, got %lld and %lld",
+             (long long)c.s.state_bytes, (long long)c.s.backward_bytes, (long long)state_bytes,
+             (long long)workspace_bytes);
+  if (!dx && !dw) return MB_OK;
+  if (dtype == MB_F32) return backward<float>(c, grad_loss, grad_stride, dx, dw);
+  return dtype == MB_BF16 ? backward<__nv_bfloat16>(c, grad_loss, grad_stride, dx, dw)
+                          : backward<__half>(c, grad_loss, grad_stride, dx, dw);
+}

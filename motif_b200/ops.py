@@ -14,8 +14,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .autograd import (AttnResFunction, ChordAttentionFunction, GatedDeltaRuleFunction, RMSNormFunction,
-                       SwiGLUFunction, needs_grad)
+from .autograd import (REDUCTIONS, AttnResFunction, ChordAttentionFunction, GatedDeltaRuleFunction,
+                       LinearCrossEntropyFunction, RMSNormFunction, SwiGLUFunction, cross_entropy_forward, needs_grad)
 from .paged import kv4_append, kv4_chord_attention, kv4_gather, kv4_pool, paged_release, paged_reserve
 from .sampler import Sampler, make_sampler  # noqa: F401  (install targets)
 
@@ -23,7 +23,7 @@ __all__ = [
     'RMSNorm', 'GatedRMSNorm', 'SwiGLU', 'rms_norm', 'gated_rms_norm', 'swiglu', 'apply_chord_attention', 'HAS_TRITON',
     'recurrent_gated_delta_rule', 'chunk_gated_delta_rule', 'chunk_gated_delta_rule_triton',
     'attn_res_block', 'can_use_triton_attn_res', 'apply_block_attn_res', 'MAX_SRC',
-    'kv4_pool', 'paged_reserve', 'paged_release', 'kv4_append', 'kv4_gather', 'kv4_chord_attention',
+    'linear_cross_entropy', 'kv4_pool', 'paged_reserve', 'paged_release', 'kv4_append', 'kv4_gather', 'kv4_chord_attention',
 ]
 
 # The reference's switch for its fused-kernel path.  Here the fused path is always the
@@ -379,3 +379,43 @@ class SwiGLU(nn.Module):
 
     def forward(self, x):
         return swiglu(x, self.dim)
+
+
+# --------------------------------------------------------------------------------- loss
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = 'mean') -> torch.Tensor:
+    """`F.cross_entropy(F.linear(x, weight), labels, ignore_index=..., reduction=...)` of a linear head over
+    a vocabulary, in fp32 and without its logits (`motif/model/motif.py:545-630` computes both).
+
+    x `[..., d]`, weight `[V, d]` of the same dtype (bf16, fp16 or fp32), labels `[...]` of whole
+    numbers.  Returns an fp32 scalar, or with `reduction='none'` one loss per token (0 where the label
+    is `ignore_index`).  Such tokens cost nothing and get no gradient, whatever x holds there.
+    A label outside `0 .. V - 1` that is not `ignore_index` makes its loss, and the gradients, NaN;
+    the mean over no token is NaN and its gradients are zero.  Differentiable in x and weight; 16-bit
+    gradients are sums in fp32 over `exp(logit - log sum)` rounded once to the type.  Memory beyond
+    the results: a copy of x's rows, and at most about 0.4 GB and an fp32 copy of weight's gradient
+    during the backward pass."""
+    _cuda('x', x)
+    _cuda('weight', weight)
+    _cuda('labels', labels)
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f'x [..., d] and weight [V, d] expected, got {tuple(x.shape)} and {tuple(weight.shape)}')
+    if labels.shape != x.shape[:-1]:
+        raise ValueError(f'labels must be {tuple(x.shape[:-1])}, got {tuple(labels.shape)}')
+    if labels.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
+        raise ValueError(f'labels must be whole numbers, got {labels.dtype}')
+    _lib.dtype_code(x.dtype)
+    if weight.dtype != x.dtype:
+        raise ValueError(f'x and weight must share one dtype, got {x.dtype} and {weight.dtype}')
+    if weight.device != x.device or labels.device != x.device:
+        raise ValueError(f'x, weight and labels must share one device, got {x.device}, {weight.device} and '
+                         f'{labels.device}')
+    if weight.numel() == 0:
+        raise ValueError(f'weight must not be empty, got {tuple(weight.shape)}')
+    x2 = _last_contig(x.reshape(-1, x.shape[-1]))
+    flat = labels.reshape(-1).to(torch.int64).contiguous()
+    args = (x2, _last_contig(weight), flat, int(ignore_index), REDUCTIONS[reduction])
+    loss = LinearCrossEntropyFunction.apply(*args) if needs_grad(x, weight) else cross_entropy_forward(*args)[0]
+    return loss.reshape(labels.shape) if reduction == 'none' else loss
