@@ -163,25 +163,6 @@ def stream_ptr(device=None) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-class _Here:
-    """A context that changes nothing."""
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def on_device(device: torch.device):
-    """Context in which launches go to `device` (its index must be set): the library launches on the
-    current device, and a stream of another one is an error."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
 def i64_array(vals):
     vals = [int(v) for v in vals]
     return (ctypes.c_int64 * len(vals))(*vals)

@@ -1,6 +1,6 @@
-"""Autograd for the ops.  Chord attention, the AttnRes read and the delta rule: their forwards run
-the inference kernels, their backwards the kernels of `csrc/backward.cu` (fp32 arithmetic on CUDA
-cores).  The norms and SwiGLU: `csrc/norm_grad.cu`.
+"""Autograd for the three hot-path ops: their forwards run the inference kernels, their
+backwards the kernels of `csrc/backward.cu` (fp32 arithmetic on CUDA cores).  (The norms, SwiGLU and
+the vocabulary loss have theirs in the compiled module, `csrc/train_host.cpp`.)
 
 The reference wraps the same ops in `torch.autograd.Function`s (`_TritonChordFunction`,
 `motif/ops/chord_attention.py:1476-1554`; `_AttnResFunction`, `motif/ops/attn_res.py:367-463`;
@@ -17,16 +17,6 @@ from . import _lib
 
 def needs_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
-
-
-def first_order(backward):
-    """Refuses a backward pass that is itself recorded (`create_graph=True`): its results would
-    look like constants, and the terms of a second derivative that pass through here be dropped."""
-    def checked(ctx, *grads):
-        if torch.is_grad_enabled():
-            raise NotImplementedError('motif_b200 ops have no second derivatives (create_graph=True)')
-        return backward(ctx, *grads)
-    return checked
 
 
 def _c(t):
@@ -156,120 +146,3 @@ class GatedDeltaRuleFunction(torch.autograd.Function):
                 dv.to(v.dtype) if need[3] else None, db.to(beta.dtype) if need[4] else None,
                 dg.to(g.dtype) if need[5] else None,
                 dS0.to(S.dtype) if (S is not None and need[6]) else None)
-
-
-class RMSNormFunction(torch.autograd.Function):
-    """RMSNorm (`gated`: GatedRMSNorm) of the rows of x [M, N] ([M, 2 N]) in fp32 with one rounding
-    (`motif_b200_rms_norm_train`), with the gradients of x and the weight
-    (`motif_b200_rms_norm_backward`).  The weight keeps its own dtype, and so does its gradient."""
-
-    @staticmethod
-    def forward(ctx, x, weight, eps, gated):
-        M, N = x.shape
-        if gated:
-            N //= 2
-        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-        wd = _lib.MB_F32 if weight is None else _lib.dtype_code(weight.dtype)
-        with _lib.on_device(x.device):
-            _lib.call('motif_b200_rms_norm_train', x.data_ptr(), _lib.ptr(weight), wd, y.data_ptr(), M, N, x.stride(0),
-                      N, gated, eps, _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
-        ctx.save_for_backward(x, weight)
-        ctx.eps, ctx.gated = eps, gated
-        return y
-
-    @staticmethod
-    @first_order
-    def backward(ctx, dy):
-        x, weight = ctx.saved_tensors
-        M, N = dy.shape
-        dy = _c(dy)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = ws = None
-        wd, nbytes, dc = _lib.MB_F32, 0, _lib.dtype_code(x.dtype)
-        if weight is not None:
-            wd = _lib.dtype_code(weight.dtype)
-            if ctx.needs_input_grad[1]:
-                dw = torch.empty_like(weight)
-                nbytes = _lib.load().motif_b200_rms_norm_backward_workspace_bytes(M, N, dc)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        with _lib.on_device(x.device):
-            _lib.call('motif_b200_rms_norm_backward', x.data_ptr(), _lib.ptr(weight), wd, dy.data_ptr(), dx.data_ptr(),
-                      _lib.ptr(dw), M, N, x.stride(0), dy.stride(0), dx.stride(0), ctx.gated, ctx.eps, _lib.ptr(ws),
-                      nbytes, dc, _lib.stream_ptr(x.device))
-        return dx if ctx.needs_input_grad[0] else None, dw, None, None
-
-
-class SwiGLUFunction(torch.autograd.Function):
-    """SwiGLU of the rows of x [M, 2 N] in fp32 with one rounding (`motif_b200_swiglu_train`) and its
-    gradient (`motif_b200_swiglu_backward`)."""
-
-    @staticmethod
-    def forward(ctx, x):
-        M, N = x.shape[0], x.shape[1] // 2
-        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-        with _lib.on_device(x.device):
-            _lib.call('motif_b200_swiglu_train', x.data_ptr(), y.data_ptr(), M, N, x.stride(0), N,
-                      _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
-        ctx.save_for_backward(x)
-        return y
-
-    @staticmethod
-    @first_order
-    def backward(ctx, dy):
-        x, = ctx.saved_tensors
-        dy = _c(dy)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        M, N = dy.shape
-        with _lib.on_device(x.device):
-            _lib.call('motif_b200_swiglu_backward', x.data_ptr(), dy.data_ptr(), dx.data_ptr(), M, N, x.stride(0),
-                      dy.stride(0), dx.stride(0), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
-        return dx
-
-
-REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
-
-
-def cross_entropy_forward(x, weight, labels, ignore_index, reduction):
-    """Losses of the rows of x [N, d] and what the backward pass needs of them (a device buffer)."""
-    N, d = x.shape
-    V, ws, dc = weight.shape[0], weight.stride(0), _lib.dtype_code(x.dtype)
-    with _lib.on_device(x.device):
-        sizes = _lib.i64_array((0, 0, 0))
-        _lib.call('motif_b200_linear_cross_entropy_bytes', weight.data_ptr(), ws, N, V, d, dc, sizes)
-        state = torch.empty(sizes[0], dtype=torch.uint8, device=x.device)
-        work = torch.empty(sizes[1], dtype=torch.uint8, device=x.device)
-        loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=x.device)
-        _lib.call('motif_b200_linear_cross_entropy', x.data_ptr(), x.stride(0), weight.data_ptr(), ws,
-                  labels.data_ptr(), ignore_index, reduction, loss.data_ptr(), N, V, d, state.data_ptr(), sizes[0],
-                  work.data_ptr(), sizes[1], dc, _lib.stream_ptr(x.device))
-    return loss, state, sizes[2]
-
-
-class LinearCrossEntropyFunction(torch.autograd.Function):
-    """Softmax cross entropy of the logits x weight^T, which are never kept: the forward pass
-    (`motif_b200_linear_cross_entropy`) leaves the rows that have a loss, their largest logits and
-    sums, the backward pass (`motif_b200_linear_cross_entropy_backward`) computes the logits again,
-    a piece of the vocabulary for a run of rows at a time."""
-
-    @staticmethod
-    def forward(ctx, x, weight, labels, ignore_index, reduction):
-        loss, state, ctx.work_bytes = cross_entropy_forward(x, weight, labels, ignore_index, reduction)
-        ctx.save_for_backward(weight, state)
-        ctx.tokens, ctx.reduction = x.shape[0], reduction
-        return loss
-
-    @staticmethod
-    @first_order
-    def backward(ctx, up):
-        weight, state = ctx.saved_tensors
-        (V, d), N = weight.shape, ctx.tokens
-        need_x, need_w = ctx.needs_input_grad[:2]
-        dx = torch.empty((N, d), dtype=weight.dtype, device=weight.device) if need_x else None
-        dw = torch.empty((V, d), dtype=weight.dtype, device=weight.device) if need_w else None
-        work = torch.empty(ctx.work_bytes, dtype=torch.uint8, device=weight.device)
-        with _lib.on_device(weight.device):
-            _lib.call('motif_b200_linear_cross_entropy_backward', weight.data_ptr(), weight.stride(0), up.data_ptr(),
-                      up.stride(0) if ctx.reduction == 0 else 0, ctx.reduction, _lib.ptr(dx), _lib.ptr(dw), N, V, d,
-                      state.data_ptr(), state.numel(), work.data_ptr(), work.numel(), _lib.dtype_code(weight.dtype),
-                      _lib.stream_ptr(weight.device))
-        return dx, dw, None, None, None

@@ -3,8 +3,8 @@
 Same names, argument meanings, return values and exception types as
 `motif/ops/__init__.py:1-10` (plus `apply_block_attn_res`, `motif/ops/attn_res.py:596`),
 computed by the sm_100a kernels of `libmotif_b200.so`.  The delta rule, Chord attention, the
-attn-res read, the norms and SwiGLU take gradients the way the reference's do (autograd Functions
-over the backward kernels, `motif_b200.autograd`).  CPU tensors raise `ValueError`; there is no
+attn-res read, the norms, SwiGLU and the vocabulary loss take gradients the way the reference's do
+(autograd Functions over the backward kernels: `motif_b200.autograd` and, compiled, `_train_host`).  CPU tensors raise `ValueError`; there is no
 eager fallback.
 """
 
@@ -14,8 +14,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .autograd import (REDUCTIONS, AttnResFunction, ChordAttentionFunction, GatedDeltaRuleFunction,
-                       LinearCrossEntropyFunction, RMSNormFunction, SwiGLUFunction, cross_entropy_forward, needs_grad)
+from .autograd import AttnResFunction, ChordAttentionFunction, GatedDeltaRuleFunction, needs_grad
 from .paged import kv4_append, kv4_chord_attention, kv4_gather, kv4_pool, paged_release, paged_reserve
 from .sampler import Sampler, make_sampler  # noqa: F401  (install targets)
 
@@ -256,78 +255,51 @@ def apply_block_attn_res(cache, query: torch.Tensor, norm) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------ norms / activation
-def _rows(name, x, weight=None, dim=None):
-    """x as rows [M, N] whose elements lie next to each other, after the checks that a norm or an
-    activation makes of its tensors."""
-    _cuda('x', x)
-    if x.dim() < 1:
-        raise ValueError(f'{name}: x must have a last dimension')
-    _lib.dtype_code(x.dtype)
-    if weight is not None:
-        _cuda('weight', weight)
-        if weight.shape != (dim,):
-            raise ValueError(f'{name}: weight must be [{dim}], got {tuple(weight.shape)}')
-        if weight.device != x.device:
-            raise ValueError(f'{name}: weight is on {weight.device}, x on {x.device}')
-        _lib.dtype_code(weight.dtype)
-    return _last_contig(x.reshape(-1, x.shape[-1]))
+_host = None
+
+
+def _compiled(name, *args):
+    """One call of the compiled entry points (checks, outputs, the C ABI call and the autograd node),
+    counted and timed by a launch tracker like `_lib.call`'s."""
+    global _host
+    if _host is None:
+        _lib.load()
+        try:
+            from . import _train_host
+        except ImportError as e:
+            raise RuntimeError('motif_b200/_train_host.so is missing or was built for another torch: build it with '
+                               f'`python -m motif_b200.build` ({e})') from e
+        _host = _train_host
+    tr = _lib._tracker
+    if tr is None:
+        return getattr(_host, name)(*args)
+    ev = tr.start('motif_b200_' + name)
+    out = getattr(_host, name)(*args)
+    tr.stop('motif_b200_' + name, ev)
+    return out
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
     """`x * rsqrt(mean(x^2) + eps) * weight` over the last dimension (`motif/ops/rms_norm.py:461-486`).
 
     Where x or the weight needs a gradient, the forward is computed in fp32 and rounded once, with a
-    weight of any dtype (fp32 next to 16-bit x); else as the eager reference does it, with the weight
-    in x's dtype and every intermediate result rounded to it."""
-    x2 = _rows('rms_norm', x, weight, x.shape[-1] if isinstance(x, torch.Tensor) and x.dim() else None)
-    M, N = x2.shape
-    if needs_grad(x, weight):
-        return RMSNormFunction.apply(x2, None if weight is None else weight.contiguous(), float(eps),
-                                     False).reshape(x.shape)
-    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
-    w = None if weight is None else weight.to(x.dtype).contiguous()
-    with _lib.on_device(x.device):
-        _lib.call('motif_b200_rms_norm', _lib.ptr(x2), _lib.ptr(w), _lib.ptr(y), M, N, x2.stride(0), y.stride(0),
-                  float(eps), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
-    return y.reshape(x.shape)
+    weight of any dtype (fp32 next to 16-bit x, whose gradient is fp32 then); else as the eager
+    reference does it, with the weight in x's dtype and every intermediate result rounded to it."""
+    return _compiled('rms_norm', x, weight, eps, False)
 
 
 def gated_rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
     """`rms_norm(values) * weight * silu(gate)`, x = [values | gate] along the last dimension
     (`motif/ops/rms_norm.py:530-553`); rounding as in `rms_norm`."""
-    _cuda('x', x)
-    if x.dim() < 1 or x.shape[-1] % 2:
-        raise ValueError(f'gated_rms_norm: x must be [..., 2 * dim], got {tuple(x.shape)}')
-    N = x.shape[-1] // 2
-    x2 = _rows('gated_rms_norm', x, weight, N)
-    if needs_grad(x, weight):
-        y = RMSNormFunction.apply(x2, None if weight is None else weight.contiguous(), float(eps), True)
-        return y.reshape(*x.shape[:-1], N)
-    y = torch.empty((x2.shape[0], N), dtype=x.dtype, device=x.device)
-    w = None if weight is None else weight.to(x.dtype).contiguous()
-    with _lib.on_device(x.device):
-        _lib.call('motif_b200_gated_rms_norm', _lib.ptr(x2), _lib.ptr(w), _lib.ptr(y), x2.shape[0], N, x2.stride(0),
-                  y.stride(0), float(eps), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
-    return y.reshape(*x.shape[:-1], N)
+    return _compiled('rms_norm', x, weight, eps, True)
 
 
 def swiglu(x: torch.Tensor, dim: int = -1) -> torch.Tensor:
     """`values * silu(gate)`, x = [values | gate] along `dim` (`motif/ops/swiglu.py:239-253`);
     rounding as in `rms_norm`."""
-    _cuda('x', x)
-    if dim not in (-1, x.dim() - 1):
+    if dim != -1 and isinstance(x, torch.Tensor) and dim != x.dim() - 1:
         return swiglu(x.movedim(dim, -1)).movedim(-1, dim)
-    if x.dim() < 1 or x.shape[-1] % 2:
-        raise ValueError('SwiGLU needs an even split dimension')
-    x2 = _rows('swiglu', x)
-    M, N = x2.shape[0], x2.shape[1] // 2
-    if needs_grad(x):
-        return SwiGLUFunction.apply(x2).reshape(*x.shape[:-1], N)
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    with _lib.on_device(x.device):
-        _lib.call('motif_b200_swiglu', _lib.ptr(x2), _lib.ptr(y), M, N, x2.stride(0), y.stride(0),
-                  _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
-    return y.reshape(*x.shape[:-1], N)
+    return _compiled('swiglu', x)
 
 
 class RMSNorm(nn.Module):
@@ -382,6 +354,9 @@ class SwiGLU(nn.Module):
 
 
 # --------------------------------------------------------------------------------- loss
+_REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
+
+
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
                          reduction: str = 'mean') -> torch.Tensor:
     """`F.cross_entropy(F.linear(x, weight), labels, ignore_index=..., reduction=...)` of a linear head over
@@ -395,27 +370,6 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     gradients are sums in fp32 over `exp(logit - log sum)` rounded once to the type.  Memory beyond
     the results: a copy of x's rows, and at most about 0.4 GB and an fp32 copy of weight's gradient
     during the backward pass."""
-    _cuda('x', x)
-    _cuda('weight', weight)
-    _cuda('labels', labels)
-    if reduction not in REDUCTIONS:
+    if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
-        raise ValueError(f'x [..., d] and weight [V, d] expected, got {tuple(x.shape)} and {tuple(weight.shape)}')
-    if labels.shape != x.shape[:-1]:
-        raise ValueError(f'labels must be {tuple(x.shape[:-1])}, got {tuple(labels.shape)}')
-    if labels.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
-        raise ValueError(f'labels must be whole numbers, got {labels.dtype}')
-    _lib.dtype_code(x.dtype)
-    if weight.dtype != x.dtype:
-        raise ValueError(f'x and weight must share one dtype, got {x.dtype} and {weight.dtype}')
-    if weight.device != x.device or labels.device != x.device:
-        raise ValueError(f'x, weight and labels must share one device, got {x.device}, {weight.device} and '
-                         f'{labels.device}')
-    if weight.numel() == 0:
-        raise ValueError(f'weight must not be empty, got {tuple(weight.shape)}')
-    x2 = _last_contig(x.reshape(-1, x.shape[-1]))
-    flat = labels.reshape(-1).to(torch.int64).contiguous()
-    args = (x2, _last_contig(weight), flat, int(ignore_index), REDUCTIONS[reduction])
-    loss = LinearCrossEntropyFunction.apply(*args) if needs_grad(x, weight) else cross_entropy_forward(*args)[0]
-    return loss.reshape(labels.shape) if reduction == 'none' else loss
+    return _compiled('linear_cross_entropy', x, weight, labels, ignore_index, _REDUCTIONS[reduction])
