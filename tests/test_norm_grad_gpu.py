@@ -101,7 +101,7 @@ def check(x, w, dy, eps, kind):
 
 SHAPES = [(1, 1), (3, 7), (5, 8), (33, 64), (1025, 64), (70, 96), (17, 100), (260, 128), (50, 250), (9, 256), (31, 300),
           (12, 512), (4801, 768), (7, 1000), (6, 1024), (5, 1032), (3, 2048), (19, 4096), (700, 4104), (4, 8192), (2, 8200),
-          (3, 10001)]
+          (3, 10001), (40, 701), (11, 301), (21, 2501), (9, 5001), (900, 2048)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
