@@ -41,8 +41,9 @@ constexpr int kBK = 64;                  // summed elements of a stage
 constexpr int kOperand = 128 * kBK * 2;  // bytes of one operand's stage in one CTA: 128 rows or columns
 constexpr int kStage = 2 * kOperand;
 constexpr int kStages = 6;
-constexpr int kThreads = 192;            // a copying warp, an issuing warp, four warps for the tile's end
-constexpr int kEnd = 4 * 4096;           // two 2 KB store buffers for each of the four
+constexpr int kEnders = 8;               // warps of the tile's end: two for each quarter of the TMEM lanes
+constexpr int kThreads = 64 + 32 * kEnders;  // a copying warp, an issuing warp, and those
+constexpr int kEnd = kEnders * 4096;     // two 2 KB buffers for each
 constexpr int kSmem = kStages * kStage + kEnd + 256 + 1024;
 constexpr uint32_t kWait = 1u << 22;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -88,7 +89,11 @@ __device__ __forceinline__ Smem carve(unsigned char* raw) {
   s.tmem = reinterpret_cast<uint32_t*>(s.mdone + 1);
   return s;
 }
+// Waits for the kernel before this one in the stream (these kernels begin while it ends).
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t pair_begin(const Smem& s) {
+  allow_dependent_launch();
   if (threadIdx.x < 32) tmem_alloc_pair(s.tmem, 512);
   if (threadIdx.x == 32) {
     for (int i = 0; i < kStages; ++i) {
@@ -97,7 +102,7 @@ __device__ __forceinline__ uint32_t pair_begin(const Smem& s) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.tfull[i], 1);
-      mbar_init(&s.tempty[i], 8);  // four warps of both CTAs
+      mbar_init(&s.tempty[i], 2 * kEnders);  // both CTAs' warps
     }
     mbar_init(s.mdone, 1);
     mbar_init_fence();
@@ -106,6 +111,7 @@ __device__ __forceinline__ uint32_t pair_begin(const Smem& s) {
   __syncthreads();
   cluster_sync2();  // both CTAs' barriers exist before a copy or an arrival crosses the pair
   tc_fence_after();
+  wait_for_previous();
   return *s.tmem;
 }
 __device__ __forceinline__ void pair_end(uint32_t tmem) {
@@ -119,13 +125,24 @@ __device__ __forceinline__ void pair_end(uint32_t tmem) {
 }
 
 // The copying thread: `it` counts stages over the kernel's life.  Returns the stage's memory, or null
-// when the wait for it ran out.
-__device__ __forceinline__ unsigned char* stage_begin(const Smem& s, int it, bool leader, uint32_t& bar) {
+// when the wait for it ran out.  `bytes`: of both CTAs' copies.
+__device__ __forceinline__ unsigned char* stage_begin(const Smem& s, int it, bool leader, uint32_t bytes, uint32_t& bar) {
   const int st = it % kStages;
   if (!mbar_wait_bounded(&s.empty[st], (uint32_t)(((it / kStages) & 1) ^ 1), kWait)) return nullptr;
   bar = map_rank(smem_u32(&s.full[st]), 0);
-  if (leader) mbar_arrive_expect_tx(&s.full[st], 2 * kStage);
+  if (leader) mbar_arrive_expect_tx(&s.full[st], bytes);
   return s.ring + st * kStage;
+}
+// A left operand whose last tile is not full: boxes of 32 rows, as many as hold rows of it.  (What else lies
+// in the stage reaches only rows of the sums that nobody reads.)
+__device__ __forceinline__ int boxes_of(int rows, uint32_t rank) { return min(max((rows - 128 * (int)rank + 31) / 32, 0), 4); }
+__device__ __forceinline__ void load_rows(unsigned char* st, const CUtensorMap* whole, const CUtensorMap* box, int boxes, int x,
+                                          int y, uint32_t bar) {
+  if (boxes == 4) {
+    tma_load_2d_pair(st, whole, x, y, bar);
+  } else {
+    for (int i = 0; i < boxes; ++i) tma_load_2d_pair(st + i * 4096, box, x, y + 32 * i, bar);
+  }
 }
 __device__ __forceinline__ void copies_failed(const Smem& s, int it, bool leader) {
   atomicAdd(&g_vocab_wait_timeouts, 1u);
@@ -221,6 +238,7 @@ struct PackArgs {
 
 __global__ void __launch_bounds__(256) group_count_kernel(const int64_t* __restrict__ labels, int64_t N, int64_t ignore,
                                                           int* __restrict__ group) {
+  allow_dependent_launch();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int n = __syncthreads_count(i < N && labels[i] != ignore);
   if (threadIdx.x == 0) group[blockIdx.x] = n;
@@ -238,31 +256,69 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
   p[1] = __float2bfloat16_rn(r1);
   p[2] = __float2bfloat16_rn(r1 - __bfloat162float(p[1]));
 }
-// One row of `d` elements into its parts, zeros behind it; a warp.
-template <typename T>
-__device__ __forceinline__ void pack_row(const T* src, int d, Op<T>* dst, int dp, int64_t part, int lane) {
-  if constexpr (kParts<T> == 1) {
-    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0 && d == dp) {  // dp is a multiple of 8
-      for (int c = lane * 8; c < d; c += 256) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-    } else {
-      for (int c = lane; c < dp; c += 32) dst[c] = c < d ? src[c] : from_f<T>(0.f);
-    }
-  } else {
-    for (int c = lane; c < dp; c += 32) {
-      __nv_bfloat16 p[3];
-      split3(c < d ? src[c] : 0.f, p);
+// Eight elements from column c of a row of d, zeros behind its end.
+template <typename T> struct Eight {
+  uint4 u[sizeof(T) / 2];
+  __device__ void load(const T* src, int c, int d, bool aligned) {
+    if (aligned && c + 8 <= d) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i) dst[i * part + c] = p[i];
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(src + c)[i];
+    } else {
+      T* e = reinterpret_cast<T*>(u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = c + i < d ? src[c + i] : from_f<T>(0.f);
     }
   }
+  __device__ void store(Op<T>* dst, int c, int64_t part) const {
+    if constexpr (kParts<T> == 1) {
+      *reinterpret_cast<uint4*>(dst + c) = u[0];
+    } else {
+      const float* e = reinterpret_cast<const float*>(u);
+      __align__(16) __nv_bfloat16 o[3][8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __nv_bfloat16 p[3];
+        split3(e[i], p);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) o[k][i] = p[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(dst + k * part + c) = *reinterpret_cast<const uint4*>(o[k]);
+    }
+  }
+};
+// One row of d elements into its parts, zeros behind it up to dp (a multiple of 8); a warp, four requests at a
+// time.
+template <typename T>
+__device__ __forceinline__ void pack_row(const T* src, int d, Op<T>* dst, int dp, int64_t part, int lane) {
+  const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+  for (int c0 = lane * 8; c0 < dp; c0 += 1024) {
+    Eight<T> v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c0 + 256 * i < dp) v[i].load(src, c0 + 256 * i, d, aligned);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c0 + 256 * i < dp) v[i].store(dst, c0 + 256 * i, part);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void zero_row(Op<T>* dst, int dp, int64_t part, int lane) {
+  for (int p = 0; p < kParts<T>; ++p)
+    for (int c = lane * 8; c < dp; c += 256) *reinterpret_cast<uint4*>(dst + p * part + c) = make_uint4(0, 0, 0, 0);
 }
 
-// A CTA packs 32 tokens: its eight warps take a token at a time.
+constexpr int kPackTokens = 16;  // of a CTA: two for each of its eight warps
+
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
   __shared__ int part[8], before[8], place[256];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t first = (int64_t)blockIdx.x * 32, run = first / 256 * 256;
+  const int64_t first = (int64_t)blockIdx.x * kPackTokens, run = first / 256 * 256;
+  allow_dependent_launch();
+  wait_for_previous();
+  const int64_t mine = run + tid;
+  const int64_t label = mine < a.N ? a.labels[mine] : a.ignore;
   // tokens with a loss in the runs before this one
   int n = 0;
   if (a.group) {
@@ -272,8 +328,6 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  const int64_t mine = run + tid;
-  const int64_t label = mine < a.N ? a.labels[mine] : a.ignore;
   const bool live = label != a.ignore;
   const unsigned vote = __ballot_sync(0xffffffffu, live);
   if (lane == 0) {
@@ -289,7 +343,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
   }
   at += __popc(vote & ((1u << lane) - 1u));
   place[tid] = live ? at : -1;
-  if (mine >= first && mine < first + 32 && mine < a.N) {
+  if (mine >= first && mine < first + kPackTokens && mine < a.N) {
     a.place[mine] = live ? at : -1;
     if (live) {
       a.label[at] = label >= 0 && label < a.V ? (int)label : -1;
@@ -302,18 +356,17 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
   const T* x = reinterpret_cast<const T*>(a.x);
   Op<T>* out = reinterpret_cast<Op<T>*>(a.packed);
   const int64_t plane = a.rows * a.dp;
-  for (int i = warp; i < 32; i += 8) {
+  for (int i = warp; i < kPackTokens; i += 8) {
     const int64_t token = first + i;
     if (token >= a.N) break;
     const int to = place[token - run];
     if (to >= 0) pack_row<T>(x + token * a.xs, a.d, out + (int64_t)to * a.dp, a.dp, plane, lane);
   }
-  // the last CTA sees all tokens: it leaves their number and zeros up to the end of the last tile
-  if (first + 32 >= a.N) {
-    const int64_t end = min(a.rows, (int64_t)(total + kTile - 1) / kTile * kTile);
-    for (int64_t r = total + warp; r < end; r += 8)
-      for (int p = 0; p < kParts<T>; ++p)
-        for (int c = lane; c < a.dp; c += 32) out[p * plane + r * a.dp + c] = from_f<Op<T>>(0.f);
+  // the last CTA sees all tokens: it leaves their number, and zeros up to the end of the last 64 rows (what the
+  // products sum over together)
+  if (first + kPackTokens >= a.N) {
+    const int64_t end = min(a.rows, (int64_t)(total + kBK - 1) / kBK * kBK);
+    for (int64_t r = total + warp; r < end; r += 8) zero_row<T>(out + r * a.dp, a.dp, plane, lane);
     if (tid == 0) {
       *a.count = total;
       *a.ticket = 0;
@@ -325,14 +378,15 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(256) pack_weight_kernel(const T* __restrict__ w, int64_t ws, int V, int d, int dp,
                                                           int64_t rows, Op<T>* __restrict__ out) {
+  allow_dependent_launch();
+  wait_for_previous();
   const int lane = threadIdx.x & 31;
   const int64_t plane = rows * dp;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
     if (r < V)
       pack_row<T>(w + r * ws, d, out + r * dp, dp, plane, lane);
     else
-      for (int p = 0; p < kParts<T>; ++p)
-        for (int c = lane; c < dp; c += 32) out[p * plane + r * dp + c] = from_f<Op<T>>(0.f);
+      zero_row<T>(out + r * dp, dp, plane, lane);
   }
 }
 
@@ -344,13 +398,13 @@ struct ScoreArgs {
   int kblocks;
   int64_t x_part, w_part;   // rows from one part of an operand to the next
   const int* label;         // [rows of the packed operand]
-  float2* seg;              // forward: (maximum, sum) of each row of a pair's run through a row tile
+  float2* seg;              // forward: (maximum, sum) of each row of half a pair's run through a row tile
   float* target;            // forward: the label's logit
   const RowStat* stat;      // backward
   const int* index;         // backward: packed row -> token
   const float* up;          // backward: per-token gradients (null: 1)
   int64_t up_stride;
-  const float* scale;       // backward: [1] = what `up` is multiplied by (a power of two)
+  const float* scale;       // backward: [1] = what `up` is multiplied by (a power of two); with `up` only
   int64_t g_part;           // backward: rows from one part of G to the next
 };
 
@@ -364,6 +418,7 @@ __host__ __device__ __forceinline__ int64_t range_owner(int64_t t, int64_t tiles
 
 template <typename T, bool GRAD>
 __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_constant__ CUtensorMap tmX,
+                                                             const __grid_constant__ CUtensorMap tmX32,
                                                              const __grid_constant__ CUtensorMap tmW,
                                                              const __grid_constant__ CUtensorMap tmG,
                                                              const ScoreArgs a) {
@@ -390,15 +445,17 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       for (int64_t t = t0; t < t1 && !failed; ++t) {
         const int m = (int)(t / nt), n = (int)(t - (int64_t)m * nt);
         const int xr = a.row0 + m * kTile + 128 * (int)rank, wr = a.v0 + n * kTile + 128 * (int)rank;
+        const int rows = live - m * kTile, boxes = boxes_of(rows, rank);
+        const uint32_t bytes = 4096 * (boxes_of(rows, 0) + boxes_of(rows, 1)) + 2 * kOperand;
         for (int p = 0; p < Parts<P>::n && !failed; ++p)
           for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
             uint32_t bar;
-            unsigned char* st = stage_begin(s, it, leader, bar);
+            unsigned char* st = stage_begin(s, it, leader, bytes, bar);
             if (!st) {
               failed = true;
               break;
             }
-            tma_load_2d_pair(st, &tmX, kb * kBK, xr + (int)(Parts<P>::a(p) * a.x_part), bar);
+            load_rows(st, &tmX, &tmX32, boxes, kb * kBK, xr + (int)(Parts<P>::a(p) * a.x_part), bar);
             tma_load_2d_pair(st + kOperand, &tmW, kb * kBK, wr + (int)(Parts<P>::b(p) * a.w_part), bar);
           }
       }
@@ -420,8 +477,8 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
     }
     __syncwarp();
   } else {
-    const int q = warp & 3;  // the TMEM lanes that this warp can read
-    const int in_tile = (int)rank * 128 + q * 32 + lane;
+    const int q = warp & 3, half = (warp - 2) >> 2;  // the TMEM lanes that this warp can read; its columns
+    const int in_tile = (int)rank * 128 + q * 32 + lane, c0 = half * (kTile / 2);
     unsigned char* buf = s.end + (warp - 2) * 4096;
     int slot = 0, done = 0, m_now = -1, label = -1;
     bool lost = false;
@@ -433,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       const int row = a.row0 + m * kTile + in_tile;
       if (m != m_now) {
         if constexpr (!GRAD) {
-          if (m_now >= 0) a.seg[(int64_t)(pair + m_now) * kTile + in_tile] = make_float2(top, sum);
+          if (m_now >= 0) a.seg[((int64_t)(pair + m_now) * 2 + half) * kTile + in_tile] = make_float2(top, sum);
           top = -INFINITY;
           sum = 0.f;
         }
@@ -455,14 +512,14 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       const uint32_t taddr = tmem + (uint32_t)((done & 1) * kTile) + ((uint32_t)(q * 32) << 16);
       tile_ready(s, done, lost);
       uint32_t r[32];
-      read32(taddr, lost, r);
+      read32(taddr + c0, lost, r);
 #pragma unroll 1
-      for (int c = 0; c < kTile; c += 32) {
+      for (int c = c0; c < c0 + kTile / 2; c += 32) {
         read32_wait(lost, r);
         float z[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(r[i]);
-        if (c + 32 < kTile) read32(taddr + c + 32, lost, r);  // on its way behind this chunk's arithmetic
+        if (c + 32 < c0 + kTile / 2) read32(taddr + c + 32, lost, r);  // on its way behind this chunk's arithmetic
         const bool here = (unsigned)(at - c) < 32u;
         if constexpr (!GRAD) {
           if (__any_sync(0xffffffffu, here)) {
@@ -553,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
       __syncwarp();
     } else {
-      if (m_now >= 0) a.seg[(int64_t)(pair + m_now) * kTile + in_tile] = make_float2(top, sum);
+      if (m_now >= 0) a.seg[((int64_t)(pair + m_now) * 2 + half) * kTile + in_tile] = make_float2(top, sum);
     }
   }
   pair_end(tmem);
@@ -575,25 +632,41 @@ struct JoinArgs {
   int reduction;     // 0 none, 1 mean, 2 sum
 };
 
-__global__ void __launch_bounds__(kTile) join_kernel(const JoinArgs a) {
-  __shared__ double sums[kTile / 32];
+constexpr int kJoinRows = 32;  // of a CTA: eight threads a row share its runs
+
+__global__ void __launch_bounds__(8 * kJoinRows) join_kernel(const JoinArgs a) {
+  __shared__ double sums[kJoinRows];
   __shared__ int last;
-  const int live = *a.count, m = blockIdx.x, row = m * kTile + threadIdx.x;
-  const int mt = (live + kTile - 1) / kTile;
-  if (m >= mt && m > 0) return;  // the first CTA is there for a call without tokens, too
-  double loss = 0.0;
+  allow_dependent_launch();
+  wait_for_previous();
+  const int live = *a.count, r = threadIdx.x >> 3, j = threadIdx.x & 7, row = blockIdx.x * kJoinRows + r;
+  const int mt = (live + kTile - 1) / kTile, ctas = max((live + kJoinRows - 1) / kJoinRows, 1);
+  if (blockIdx.x >= ctas) return;  // the first CTA is there for a call without tokens, too
+  const int m = row / kTile, in_tile = row % kTile;
+  float top = -INFINITY, sum = 0.f;
   if (row < live) {
     const int64_t tiles = (int64_t)mt * a.nt, walkers = min((int64_t)a.np, tiles);
-    const int p0 = (int)range_owner((int64_t)m * a.nt, tiles, walkers);
-    const int p1 = (int)range_owner((int64_t)(m + 1) * a.nt - 1, tiles, walkers);
-    float top = -INFINITY;
-    for (int p = p0; p <= p1; ++p) top = fmaxf(top, a.seg[(int64_t)(p + m) * kTile + threadIdx.x].x);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int p = p0; p <= p1; ++p) {
-      const float2 v = a.seg[(int64_t)(p + m) * kTile + threadIdx.x];
-      sum += v.y * ex2f_((v.x - ref) * kLog2e);
+    const int s0 = 2 * ((int)range_owner((int64_t)m * a.nt, tiles, walkers) + m);
+    const int s1 = 2 * ((int)range_owner((int64_t)(m + 1) * a.nt - 1, tiles, walkers) + m) + 2;
+#pragma unroll 4
+    for (int i = s0 + j; i < s1; i += 8) {
+      const float2 v = a.seg[(int64_t)i * kTile + in_tile];
+      const float now = fmaxf(top, v.x), ref = now == -INFINITY ? 0.f : now;
+      sum = sum * ex2f_((top - ref) * kLog2e) + v.y * ex2f_((v.x - ref) * kLog2e);
+      top = now;
     }
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {  // the two sides of an exchange add in the same order
+    const float t2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
+    const float now = fmaxf(top, t2), ref = now == -INFINITY ? 0.f : now;
+    const float mine = sum * ex2f_((top - ref) * kLog2e), other = s2 * ex2f_((t2 - ref) * kLog2e);
+    sum = (j & o) ? other + mine : mine + other;
+    top = now;
+  }
+  double loss = 0.0;
+  if (row < live && j == 0) {
+    const float ref = top == -INFINITY ? 0.f : top;
     const bool known = a.label[row] >= 0;
     const float nan = __int_as_float(0x7fffffff);
     RowStat st;
@@ -605,23 +678,21 @@ __global__ void __launch_bounds__(kTile) join_kernel(const JoinArgs a) {
     loss = one;
   }
   if (a.reduction == 0) return;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = loss;
+  if (j == 0) sums[r] = loss;
   __syncthreads();
   if (threadIdx.x == 0) {
     loss = 0.0;
-    for (int i = 0; i < kTile / 32; ++i) loss += sums[i];
-    a.partial[m] = loss;
+    for (int i = 0; i < kJoinRows; ++i) loss += sums[i];
+    a.partial[blockIdx.x] = loss;
     __threadfence();
-    last = atomicAdd(a.ticket, 1) == max(mt, 1) - 1;
+    last = atomicAdd(a.ticket, 1) == ctas - 1;
   }
   __syncthreads();
   if (!last) return;
   // the last CTA adds all of them, in one order whoever it is
   __threadfence();
   loss = 0.0;
-  for (int i = threadIdx.x; i < mt; i += kTile) loss += __ldcg(a.partial + i);
+  for (int i = threadIdx.x; i < ctas; i += 8 * kJoinRows) loss += __ldcg(a.partial + i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
   __syncthreads();
@@ -629,26 +700,21 @@ __global__ void __launch_bounds__(kTile) join_kernel(const JoinArgs a) {
   __syncthreads();
   if (threadIdx.x == 0) {
     loss = 0.0;
-    for (int i = 0; i < kTile / 32; ++i) loss += sums[i];
+    for (int i = 0; i < 8; ++i) loss += sums[i];
     *a.loss = (float)(a.reduction == 1 ? loss / (double)live : loss);  // no tokens: 0 / 0, as it is
     *a.denom = (float)(1.0 / (double)live);
   }
 }
 
-// scale[0]: what dx and dW are multiplied by at the end; scale[1]: what the per-token gradients are
-// multiplied by before (a power of two that brings the largest below 1 or to it).
+// For per-token gradients.  scale[0]: what dx and dW are multiplied by at the end; scale[1]: what the
+// per-token gradients are multiplied by before (a power of two that brings the largest to 1 / 2 .. 1).
 __global__ void __launch_bounds__(1024) scale_kernel(const float* __restrict__ up, int64_t up_stride, int64_t N,
-                                                     const int* __restrict__ place, const int* __restrict__ count,
-                                                     int reduction, const float* __restrict__ denom, int half,
-                                                     float* __restrict__ scale) {
+                                                     const int* __restrict__ place, float* __restrict__ scale) {
   __shared__ float tops[32];
-  float fold = half ? 1.0f / kHalfScale : 1.0f;
-  if (reduction != 0) {
-    // no token has a loss: the gradients are zero, whatever 0 / 0 says
-    if (threadIdx.x == 0) scale[0] = *count > 0 ? *up * (reduction == 1 ? *denom : 1.0f) * fold : 0.0f;
-    return;
-  }
+  allow_dependent_launch();
+  wait_for_previous();
   float top = 0.f;
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < N; i += 1024)
     if (place[i] >= 0) top = fmaxf(top, fabsf(up[i * up_stride]));
   top = warp_max(top);
@@ -659,7 +725,7 @@ __global__ void __launch_bounds__(1024) scale_kernel(const float* __restrict__ u
     int e = 0;
     if (top > 0.f && top <= 3.4e38f) frexpf(top, &e);
     e = max(-126, min(126, e));
-    scale[0] = ldexpf(1.0f, e) * fold;
+    scale[0] = ldexpf(1.0f, e);
     scale[1] = ldexpf(1.0f, -e);
   }
 }
@@ -672,14 +738,26 @@ struct ProductArgs {
   int v0, nv;               // its vocabulary
   int d;
   int64_t a_part, b_part;   // rows from one part of an operand to the next
-  float* slots;             // [pairs][256][256]: tiles whose sum is split
+  float4* slots;            // [pairs][256 / 4][256]: tiles whose sum is split
   float* acc;               // [rows or nv][ld] fp32, or null
   int64_t ld;
   int first, last;          // first: acc holds nothing yet; last: the result leaves as T
-  const float* scale;
+  const float* scale;       // [0] (per-token gradients), or null:
+  const float* up;          // the one gradient,
+  const float* denom;       // times this (the mean's), or null
   void* out;                // dx (rows by `index`) or dW
   const int* index;
+  const int* place;         // dx, first call: [N], the tokens without a loss (-1) get zeros
+  int64_t N;
 };
+template <typename T>
+__device__ __forceinline__ float last_scale(const ProductArgs& a) {
+  if (!a.last) return 1.0f;
+  const float fold = std::is_same<T, __half>::value ? 1.0f / kHalfScale : 1.0f;
+  if (a.scale) return a.scale[0] * fold;
+  if (*a.count <= 0) return 0.0f;  // no token has a loss: the gradients are zero, whatever 0 / 0 says
+  return *a.up * (a.denom ? *a.denom : 1.0f) * fold;
+}
 struct Cut {  // how a product's tiles are spread over the pairs
   int mt, nt, kb, full, split, units;
 };
@@ -722,11 +800,17 @@ __device__ __forceinline__ Unit unit_at(const Cut& c, int u) {
   r.n = tile - r.m * c.nt;
   return r;
 }
-// 32 columns of a row: what earlier calls left is added; the sum stays in fp32 or leaves as T.
+__device__ __forceinline__ int64_t row_out(const ProductArgs& a, int row) {
+  return (a.by_rows ? (int64_t)a.index[a.row0 + row] : (int64_t)(a.v0 + row)) * a.d;
+}
+// 32 columns of each of a warp's 32 rows (a thread has a row's): what earlier calls left is added; the sum
+// stays in fp32 or leaves as T.  It goes out by way of shared memory, so that a store instruction writes whole
+// 64-byte (fp32: 128-byte) runs of rows instead of 16 bytes of each.
 template <typename T>
-__device__ __forceinline__ void finish32(const ProductArgs& a, int row, int col, float (&v)[32], float scale) {
-  const int n = min(32, a.d - col);
-  if (!a.first) {
+__device__ __forceinline__ void finish32(const ProductArgs& a, int row, int rows, int col, float (&v)[32], float scale,
+                                         unsigned char* buf) {
+  const int n = min(32, a.d - col), lane = threadIdx.x & 31;
+  if (!a.first && row < rows) {
     const float* p = a.acc + (int64_t)row * a.ld + col;
 #pragma unroll
     for (int i = 0; i < 32; i += 4)
@@ -738,35 +822,63 @@ __device__ __forceinline__ void finish32(const ProductArgs& a, int row, int col,
         v[i + 3] += o.w;
       }
   }
-  if (!a.last) {
-    float* p = a.acc + (int64_t)row * a.ld + col;
+  const bool wide = !a.last || sizeof(T) == 4;  // 128 bytes of a row, or 64
+  if (a.last) {
+    if (a.d % (16 / (int)sizeof(T)) != 0 || (reinterpret_cast<uintptr_t>(a.out) & 15) != 0) {
+      if (row < rows) {
+        T* p = reinterpret_cast<T*>(a.out) + row_out(a, row) + col;
 #pragma unroll
-    for (int i = 0; i < 32; i += 4)
-      if (i < n) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    return;
-  }
-  const int64_t to = a.by_rows ? a.index[a.row0 + row] : a.v0 + row;
-  T* p = reinterpret_cast<T*>(a.out) + to * a.d + col;
-  constexpr int E = 16 / (int)sizeof(T);
-  if (a.d % E == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
-#pragma unroll
-    for (int i = 0; i < 32; i += E)
-      if (i < n) {
-        __align__(16) T o[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = from_f<T>(v[i + e] * scale);
-        *reinterpret_cast<uint4*>(p + i) = *reinterpret_cast<const uint4*>(o);
+        for (int i = 0; i < 32; ++i)
+          if (i < n) p[i] = from_f<T>(v[i] * scale);
       }
-  } else {
+      return;
+    }
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) p[i] = from_f<T>(v[i] * scale);
+    for (int i = 0; i < 32; ++i) v[i] *= scale;
+  }
+  const int64_t mine = a.last && row < rows ? row_out(a, row) : (int64_t)row * a.ld;
+  __syncwarp();  // the chunk before has been read
+  if (wide) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      *reinterpret_cast<float4*>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) =
+          make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+  } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      *reinterpret_cast<uint4*>(buf + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(pack2<T>(v[8 * u], v[8 * u + 1]), pack2<T>(v[8 * u + 2], v[8 * u + 3]),
+                     pack2<T>(v[8 * u + 4], v[8 * u + 5]), pack2<T>(v[8 * u + 6], v[8 * u + 7]));
+  }
+  __syncwarp();
+  const int row0 = row - lane;
+  if (wide) {
+    char* out = reinterpret_cast<char*>(a.last ? reinterpret_cast<float*>(a.out) : a.acc);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3), u = lane & 7;
+      const int64_t at = __shfl_sync(0xffffffffu, mine, r);
+      if (row0 + r < rows && 4 * u < n)
+        *reinterpret_cast<float4*>(out + (at + col + 4 * u) * 4) =
+            *reinterpret_cast<const float4*>(buf + r * 128 + ((u ^ (r & 7)) << 4));
+    }
+  } else {
+    T* out = reinterpret_cast<T*>(a.out);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2), u = lane & 3;
+      const int64_t at = __shfl_sync(0xffffffffu, mine, r);
+      if (row0 + r < rows && 8 * u < n)
+        *reinterpret_cast<uint4*>(out + at + col + 8 * u) =
+            *reinterpret_cast<const uint4*>(buf + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
+    }
   }
 }
 
 // A_MN: the left operand's summed dimension runs along its rows (dW); the right one's always does.
 template <typename T, bool A_MN>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ CUtensorMap tmA,
+                                                              const __grid_constant__ CUtensorMap tmA32,
                                                               const __grid_constant__ CUtensorMap tmB,
                                                               const ProductArgs a) {
   using O = Op<T>;
@@ -789,12 +901,14 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const Unit w = unit_at(c, u);
         const int cols = (min(kTile, a.d - w.n * kTile) + 31) & ~31;
         const int ar = w.m * kTile + 128 * (int)rank, bc = w.n * kTile + (int)rank * (cols / 2);
+        const int rows = A_MN ? kTile : live - w.m * kTile, boxes = boxes_of(rows, rank);
+        const uint32_t bytes = 4096 * (boxes_of(rows, 0) + boxes_of(rows, 1)) + 2 * kOperand;
         // the right operand's rows: words of this piece, or this call's tokens
         const int br = a.by_rows ? a.v0 : a.row0;
         for (int p = 0; p < Parts<P>::n && !failed; ++p)
           for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
             uint32_t bar;
-            unsigned char* st = stage_begin(s, it, leader, bar);
+            unsigned char* st = stage_begin(s, it, leader, bytes, bar);
             if (!st) {
               failed = true;
               break;
@@ -804,7 +918,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
               tma_load_2d_pair(st, &tmA, ar, pa + kb * kBK, bar);
               tma_load_2d_pair(st + 8192, &tmA, ar + 64, pa + kb * kBK, bar);
             } else {
-              tma_load_2d_pair(st, &tmA, kb * kBK, pa + ar, bar);
+              load_rows(st, &tmA, &tmA32, boxes, kb * kBK, pa + ar, bar);
             }
             tma_load_2d_pair(st + kOperand, &tmB, bc, pb + br + kb * kBK, bar);
             tma_load_2d_pair(st + kOperand + 8192, &tmB, bc + 64, pb + br + kb * kBK, bar);
@@ -831,9 +945,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     }
     __syncwarp();
   } else {
-    const int q = warp & 3;
+    const int q = warp & 3, half = (warp - 2) >> 2;
     const int in_tile = (int)rank * 128 + q * 32 + lane;
-    const float scale = a.last ? a.scale[0] : 1.0f;
+    unsigned char* buf = s.end + (warp - 2) * 4096;
+    const float scale = last_scale<T>(a);
+    if (a.place) {  // while the first tile is on its way: zeros for the tokens without a loss
+      T* dx = reinterpret_cast<T*>(a.out);
+      for (int64_t n = (int64_t)blockIdx.x * kEnders + warp - 2; n < a.N; n += (int64_t)gridDim.x * kEnders)
+        if (a.place[n] < 0)
+          for (int c = lane; c < a.d; c += 32) dx[n * a.d + c] = from_f<T>(0.f);
+    }
     int done = 0;
     bool lost = false;
     for (int u = pair; u < c.units; u += np, ++done) {
@@ -843,7 +964,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const int cols = min(kTile, a.d - w.n * kTile);
       if (c.kb > 0) tile_ready(s, done, lost);
 #pragma unroll 1
-      for (int col = 0; col < cols; col += 32) {
+      for (int col = half * 32; col < cols; col += 64) {
         uint32_t r[32];
         if (c.kb > 0) {
           read32(taddr + col, lost, r);
@@ -855,12 +976,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if (w.slot >= 0) {
-          float* p = a.slots + ((int64_t)w.slot * kTile + in_tile) * kTile + col;
+        if (w.slot >= 0) {  // [slot][four columns][row]: the warp's rows lie next to each other
+          float4* p = a.slots + ((int64_t)w.slot * (kTile / 4) + col / 4) * kTile + in_tile;
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        } else if (row < rows) {
-          finish32<T>(a, row, w.n * kTile + col, v, scale);
+          for (int i = 0; i < 8; ++i) p[i * kTile] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+          finish32<T>(a, row, rows, w.n * kTile + col, v, scale, buf);
         }
       }
       if (c.kb > 0) tile_read(s, done, lost, leader);
@@ -869,41 +990,61 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   pair_end(tmem);
 }
 
-// The tiles whose sum was split: their parts are added in order.
+// The tiles whose sum was split: their parts are added in order.  A CTA takes 32 rows x 32 columns of a tile: a
+// warp adds four columns of the rows, then the block of sums is turned so that rows leave in runs.
 template <typename T>
 __global__ void __launch_bounds__(256) join_product_kernel(const ProductArgs a, int np) {
+  __shared__ float4 turn[32][9];
+  allow_dependent_launch();
+  wait_for_previous();
   const int live = product_live(a);
   const Cut c = cut_product(a, live, np);
-  const int j = blockIdx.x / 8, tile = c.full + j;  // eight CTAs a tile, 32 rows each, 32 columns a thread
+  const int j = blockIdx.x / 64, tile = c.full + j;
   if (tile >= c.mt * c.nt) return;
-  const int m = tile / c.nt, n = tile - m * c.nt;
-  const int in_tile = (blockIdx.x & 7) * 32 + (threadIdx.x >> 3), col = (threadIdx.x & 7) * 32;
-  const int row = m * kTile + in_tile, rows = a.by_rows ? live : a.nv;
-  if (row >= rows || n * kTile + col >= a.d) return;
-  float v[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = 0.f;
+  const int m = tile / c.nt, n = tile - m * c.nt, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r0 = (blockIdx.x >> 3 & 7) * 32, c0 = (blockIdx.x & 7) * 32;
+  const int rows = a.by_rows ? live : a.nv;
+  if (m * kTile + r0 >= rows || n * kTile + c0 >= a.d) return;
+  const float4* src = a.slots + ((int64_t)j * c.split * (kTile / 4) + c0 / 4 + warp) * kTile + r0 + lane;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
   for (int p = 0; p < c.split; ++p) {
-    const float* src = a.slots + ((int64_t)(j * c.split + p) * kTile + in_tile) * kTile + col;
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 o = *reinterpret_cast<const float4*>(src + i);
-      v[i] += o.x;
-      v[i + 1] += o.y;
-      v[i + 2] += o.z;
-      v[i + 3] += o.w;
-    }
+    const float4 o = src[(int64_t)p * (kTile / 4) * kTile];
+    v.x += o.x;
+    v.y += o.y;
+    v.z += o.z;
+    v.w += o.w;
   }
-  finish32<T>(a, row, n * kTile + col, v, a.last ? a.scale[0] : 1.0f);
-}
-
-// Zeros in dx for the tokens without a loss.
-template <typename T>
-__global__ void __launch_bounds__(256) zero_rows_kernel(const int* __restrict__ place, int64_t N, int d, T* __restrict__ dx) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); n < N; n += (int64_t)gridDim.x * 8)
-    if (place[n] < 0)
-      for (int c = lane; c < d; c += 32) dx[n * d + c] = from_f<T>(0.f);
+  turn[lane][warp] = v;
+  __syncthreads();
+  const int row = m * kTile + r0 + (threadIdx.x >> 3), col = n * kTile + c0 + 4 * (threadIdx.x & 7);
+  if (row >= rows || col >= a.d) return;
+  v = turn[threadIdx.x >> 3][threadIdx.x & 7];
+  float4* acc = reinterpret_cast<float4*>(a.acc + (int64_t)row * a.ld + col);  // rows are padded to fours
+  if (!a.first) {
+    const float4 o = *acc;
+    v.x += o.x;
+    v.y += o.y;
+    v.z += o.z;
+    v.w += o.w;
+  }
+  if (!a.last) {
+    *acc = v;
+    return;
+  }
+  const float scale = last_scale<T>(a);
+  T* p = reinterpret_cast<T*>(a.out) + row_out(a, row) + col;
+  const float e[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+  if (a.d % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<float4*>(p) = make_float4(e[0], e[1], e[2], e[3]);
+    else
+      *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < a.d) p[i] = from_f<T>(e[i]);
+  }
 }
 
 // ------------------------------------------------------------------------------- host
@@ -949,14 +1090,18 @@ Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) 
   s.denom = take(s.state_bytes, 4);
   const int64_t mt = s.rows / kTile;
   s.group = take(s.forward_bytes, up_to(N, 256) / 256 * 4);
-  s.seg = take(s.forward_bytes, (np + mt) * kTile * (int64_t)sizeof(float2));
+  s.seg = take(s.forward_bytes, (np + mt) * 2 * kTile * (int64_t)sizeof(float2));
   s.target = take(s.forward_bytes, s.rows * 4);
-  s.partial = take(s.forward_bytes, mt * 8);
+  s.partial = take(s.forward_bytes, s.rows / kJoinRows * 8);
   // a run of rows and a piece of the vocabulary: G of both together stays below kPiece elements
   const int64_t most = kPiece / s.parts;
   s.run = std::min(s.rows, s.parts == 3 ? kExactRun : kRun);
   s.piece = std::min(s.vrows, std::max<int64_t>(kTile, most / s.run / kTile * kTile));
-  if (s.parts == 3) s.piece = std::min(s.piece, kExactRun);
+  if (s.parts == 3) {
+    // dx's sums run over the words of a piece, each in as many parts as there are pairs for a tile
+    const int64_t tiles = s.run / kTile * ((d + kTile - 1) / kTile);
+    s.piece = std::min(s.piece, kExactRun * std::max<int64_t>(1, np / tiles));
+  }
   if (s.parts == 1) s.run = std::min(s.rows, std::max(s.run, most / s.piece / kTile * kTile));
   s.g = take(s.backward_bytes, s.parts * s.run * s.piece * 2);
   s.slots = take(s.backward_bytes, (int64_t)np * kTile * kTile * 4);
@@ -966,23 +1111,30 @@ Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) 
   return s;
 }
 
+// Launches that may begin while the kernel before them ends (all of these wait for it before they touch memory).
+template <typename K, typename... A>
+int launch(const char* what, K kern, int64_t grid, int threads, cudaStream_t st, int smem, int cluster, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kern, args...);
+  return check_launch(what);
+}
 template <typename K, typename... A>
 int launch_pairs(const char* what, K kern, int np, cudaStream_t st, A... args) {
   if (int e = ensure_smem_attr((const void*)kern, kSmem)) return e;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(2 * np));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = st;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kern, args...);
-  return check_launch(what);
+  return launch(what, kern, 2 * np, kThreads, st, kSmem, 2, args...);
 }
 
 struct Call {
@@ -1034,18 +1186,21 @@ int forward(const Call& c, float* loss) {
   p.index = at<int>(c.state, s.index);
   p.place = at<int>(c.state, s.place);
   p.loss = c.reduction == 0 ? loss : nullptr;
-  pack_kernel<T><<<(unsigned)std::max<int64_t>(1, (c.N + 31) / 32), 256, 0, c.st>>>(p);
-  if (int e = check_launch("linear_cross_entropy (pack)")) return e;
+  int rc = launch("linear_cross_entropy (pack)", pack_kernel<T>,
+                  std::max<int64_t>(1, (c.N + kPackTokens - 1) / kPackTokens), 256, c.st, 0, 1, p);
+  if (rc) return rc;
   if (c.pack_w) {
-    pack_weight_kernel<T><<<(unsigned)std::min<int64_t>((s.vrows + 7) / 8, 148 * 16), 256, 0, c.st>>>(
-        (const T*)c.w, c.ws, (int)c.V, (int)c.d, (int)s.dp, s.vrows, at<Op<T>>(c.state, s.w));
-    if (int e = check_launch("linear_cross_entropy (pack weight)")) return e;
+    rc = launch("linear_cross_entropy (pack weight)", pack_weight_kernel<T>,
+                std::min<int64_t>((s.vrows + 7) / 8, multiprocessors() * 16), 256, c.st, 0, 1, (const T*)c.w, c.ws,
+                (int)c.V, (int)c.d, (int)s.dp, s.vrows, at<Op<T>>(c.state, s.w));
+    if (rc) return rc;
   }
-  CUtensorMap tmX, tmW;
+  CUtensorMap tmX, tmX32, tmW;
   const void* wb;
   int64_t wr, wst, wc;
   weight_rows(c, &wb, &wr, &wst, &wc);
-  int rc = encode_tile_map_2d(&tmX, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 128, 128);
+  rc = encode_tile_map_2d(&tmX, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 128, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmX32, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 32, 128);
   if (!rc) rc = encode_tile_map_2d(&tmW, wb, 2, wc, wr, wst * 2, kBK, 128, 128);
   if (rc) return rc;
   ScoreArgs a = {};
@@ -1058,7 +1213,7 @@ int forward(const Call& c, float* loss) {
   a.label = p.label;
   a.seg = at<float2>(c.work, s.seg);
   a.target = at<float>(c.work, s.target);
-  rc = launch_pairs("linear_cross_entropy (scores)", scores_kernel<T, false>, c.np, c.st, tmX, tmW, tmX, a);
+  rc = launch_pairs("linear_cross_entropy (scores)", scores_kernel<T, false>, c.np, c.st, tmX, tmX32, tmW, tmX, a);
   if (rc) return rc;
   JoinArgs j = {};
   j.count = p.count;
@@ -1074,8 +1229,7 @@ int forward(const Call& c, float* loss) {
   j.nt = (int)((c.V + kTile - 1) / kTile);
   j.np = c.np;
   j.reduction = c.reduction;
-  join_kernel<<<(unsigned)(s.rows / kTile), kTile, 0, c.st>>>(j);
-  return check_launch("linear_cross_entropy (join)");
+  return launch("linear_cross_entropy (join)", join_kernel, s.rows / kJoinRows, 8 * kJoinRows, c.st, 0, 1, j);
 }
 
 template <typename T>
@@ -1085,26 +1239,24 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
   const int* place = at<int>(c.state, s.place);
   const int* index = at<int>(c.state, s.index);
   float* scale = at<float>(c.work, s.scale);
-  scale_kernel<<<1, c.reduction == 0 ? 1024 : 32, 0, c.st>>>(up, up_stride, c.N, place, count, c.reduction,
-                                                            at<float>(c.state, s.denom),
-                                                            std::is_same<T, __half>::value, scale);
-  if (int e = check_launch("linear_cross_entropy_backward (scale)")) return e;
-  if (dx) {
-    zero_rows_kernel<T><<<(unsigned)std::min<int64_t>((c.N + 7) / 8, 148 * 8), 256, 0, c.st>>>(place, c.N, (int)c.d,
-                                                                                              (T*)dx);
-    if (int e = check_launch("linear_cross_entropy_backward (zero)")) return e;
+  int rc = MB_OK;
+  if (c.reduction == 0) {
+    rc = launch("linear_cross_entropy_backward (scale)", scale_kernel, 1, 1024, c.st, 0, 1, up, up_stride, c.N, place, scale);
+    if (rc) return rc;
   }
   const void* wb;
   int64_t wr, wst, wc;
   weight_rows(c, &wb, &wr, &wst, &wc);
-  CUtensorMap tmX, tmW, tmG, tmXk, tmWk, tmGa, tmGt;
+  CUtensorMap tmX, tmX32, tmW, tmG, tmXk, tmWk, tmGa, tmGa32, tmGt;
   unsigned char* g = c.work + s.g;
-  int rc = encode_tile_map_2d(&tmX, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 128, 128);
+  rc = encode_tile_map_2d(&tmX, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 128, 128);
   if (!rc) rc = encode_tile_map_2d(&tmW, wb, 2, wc, wr, wst * 2, kBK, 128, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmX32, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 32, 128);
   if (!rc) rc = encode_tile_map_2d(&tmXk, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, 64, kBK, 128);
   if (!rc) rc = encode_tile_map_2d(&tmWk, wb, 2, wc, wr, wst * 2, 64, kBK, 128);
   if (!rc) rc = encode_tile_map_2d(&tmG, g, 2, s.piece, s.parts * s.run, s.piece * 2, 32, 32, 64);    // stored
   if (!rc) rc = encode_tile_map_2d(&tmGa, g, 2, s.piece, s.parts * s.run, s.piece * 2, kBK, 128, 128);  // tokens x words
+  if (!rc) rc = encode_tile_map_2d(&tmGa32, g, 2, s.piece, s.parts * s.run, s.piece * 2, kBK, 32, 128);
   if (!rc) rc = encode_tile_map_2d(&tmGt, g, 2, s.piece, s.parts * s.run, s.piece * 2, 64, kBK, 128);   // words x tokens
   if (rc) return rc;
   for (int64_t r0 = 0; r0 < s.rows; r0 += s.run)
@@ -1125,7 +1277,8 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
       a.up_stride = up_stride;
       a.scale = scale;
       a.g_part = s.run;
-      rc = launch_pairs("linear_cross_entropy_backward (scores)", scores_kernel<T, true>, c.np, c.st, tmX, tmW, tmG, a);
+      rc = launch_pairs("linear_cross_entropy_backward (scores)", scores_kernel<T, true>, c.np, c.st, tmX, tmX32,
+                        tmW, tmG, a);
       if (rc) return rc;
       ProductArgs p = {};
       p.count = count;
@@ -1135,10 +1288,13 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
       p.nv = a.nv;
       p.d = (int)c.d;
       p.a_part = s.run;
-      p.slots = at<float>(c.work, s.slots);
+      p.slots = at<float4>(c.work, s.slots);
       p.ld = up_to(c.d, 4);
-      p.scale = scale;
+      p.scale = c.reduction == 0 ? scale : nullptr;
+      p.up = up;
+      p.denom = c.reduction == 1 ? at<float>(c.state, s.denom) : nullptr;
       p.index = index;
+      p.N = c.N;
       if (dx) {
         p.by_rows = 1;
         p.b_part = s.vrows;
@@ -1146,10 +1302,14 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
         p.first = v0 == 0;
         p.last = v0 + s.piece >= c.V;
         p.out = dx;
-        rc = launch_pairs("linear_cross_entropy_backward (dx)", product_kernel<T, false>, c.np, c.st, tmGa, tmWk, p);
+        p.place = r0 == 0 && v0 == 0 ? place : nullptr;
+        rc = launch_pairs("linear_cross_entropy_backward (dx)", product_kernel<T, false>, c.np, c.st, tmGa, tmGa32, tmWk,
+                          p);
+        // how many tiles are split the device knows: at most all, and fewer than there are pairs
+        const int64_t most = std::min<int64_t>(c.np - 1, up_to(p.rows, kTile) / kTile * ((c.d + kTile - 1) / kTile));
+        if (!rc && most > 0)
+          rc = launch("linear_cross_entropy_backward (dx join)", join_product_kernel<T>, 64 * most, 256, c.st, 0, 1, p, c.np);
         if (rc) return rc;
-        join_product_kernel<T><<<(unsigned)(8 * c.np), 256, 0, c.st>>>(p, c.np);
-        if ((rc = check_launch("linear_cross_entropy_backward (dx join)"))) return rc;
       }
       if (dw) {
         p.by_rows = 0;
@@ -1158,10 +1318,12 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
         p.first = r0 == 0;
         p.last = r0 + s.run >= s.rows;
         p.out = dw;
-        rc = launch_pairs("linear_cross_entropy_backward (dw)", product_kernel<T, true>, c.np, c.st, tmGt, tmXk, p);
+        p.place = nullptr;
+        rc = launch_pairs("linear_cross_entropy_backward (dw)", product_kernel<T, true>, c.np, c.st, tmGt, tmGt, tmXk, p);
+        const int64_t rest = up_to(p.nv, kTile) / kTile * ((c.d + kTile - 1) / kTile) % c.np;
+        if (!rc && rest > 0 && c.N > kBK)  // (a sum of one stage is not split)
+          rc = launch("linear_cross_entropy_backward (dw join)", join_product_kernel<T>, 64 * rest, 256, c.st, 0, 1, p, c.np);
         if (rc) return rc;
-        join_product_kernel<T><<<(unsigned)(8 * c.np), 256, 0, c.st>>>(p, c.np);
-        if ((rc = check_launch("linear_cross_entropy_backward (dw join)"))) return rc;
       }
     }
   return MB_OK;
