@@ -207,6 +207,21 @@ MB_API int motif_b200_linear_cross_entropy_backward(const void* w, int64_t ws, c
                                              int64_t V, int64_t d, void* state, int64_t state_bytes, void* workspace,
                                              int64_t workspace_bytes, int dtype, void* stream);
 
+/* The loss (reduction 1 or 2) with the gradients that it has when the gradient arriving at it is 1, in one pass over
+ * the logits (bf16 and fp32); dx and dw as above, either may be NULL.  Workspace of
+ * motif_b200_linear_cross_entropy_train_workspace_bytes(...) bytes (-1: bad sizes) at a 256-byte boundary, at most
+ * about 0.6 GB, a copy of x (fp32: and of w, one and a half times as large) and one fp32 copy of dw. */
+MB_API int64_t motif_b200_linear_cross_entropy_train_workspace_bytes(const void* w, int64_t ws, int64_t N, int64_t V,
+                                                              int64_t d, int dtype);
+MB_API int motif_b200_linear_cross_entropy_train(const void* x, int64_t xs, const void* w, int64_t ws,
+                                          const int64_t* labels, int64_t ignore_index, int reduction, float* loss,
+                                          void* dx, void* dw, int64_t N, int64_t V, int64_t d, void* workspace,
+                                          int64_t workspace_bytes, int dtype, void* stream);
+
+/* a_out = a * scale[0], b_out = b * scale[0] (device memory; a_n and b_n elements of `dtype` at 16-byte boundaries). */
+MB_API int motif_b200_scale_gradients(const void* a, void* a_out, int64_t a_n, const void* b, void* b_out, int64_t b_n,
+                               const float* scale, int dtype, void* stream);
+
 /* ------------------------------------------------------------------ fused model kernels
  * These replace sequences of reference statements inside one layer; each cites them.
  * Token-major activations: row r = b*T + t, element stride 1 within a row.

@@ -52,6 +52,10 @@ SIGNATURES = {
                                         + [_P, _I64, _P, _I64, _I, _P]),
     'motif_b200_linear_cross_entropy_backward': (_I, [_P, _I64, _P, _I64, _I, _P, _P] + [_I64] * 3
                                                  + [_P, _I64, _P, _I64, _I, _P]),
+    'motif_b200_linear_cross_entropy_train_workspace_bytes': (_I64, [_P] + [_I64] * 4 + [_I]),
+    'motif_b200_linear_cross_entropy_train': (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _P, _P, _P] + [_I64] * 3
+                                              + [_P, _I64, _I, _P]),
+    'motif_b200_scale_gradients': (_I, [_P, _P, _I64, _P, _P, _I64, _P, _I, _P]),
     'motif_b200_attn_res_norm': (_I, [_P, _I, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F, _F, _I, _P]),
     'motif_b200_gdn_prep': (_I, [_P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                                  _I64, _I, _P]),
@@ -185,6 +189,8 @@ KERNELS_PER_CALL.update({'motif_b200_last_error': 0, 'motif_b200_abi_version': 0
                          'motif_b200_chord_backward_workspace_bytes': 0, 'motif_b200_gdn_backward_workspace_bytes': 0,
                          'motif_b200_linear_cross_entropy_bytes': 0, 'motif_b200_linear_cross_entropy': 3,
                          'motif_b200_linear_cross_entropy_backward': 7,
+                         'motif_b200_linear_cross_entropy_train_workspace_bytes': 0,
+                         'motif_b200_linear_cross_entropy_train': 8,
                          'motif_b200_rms_norm_backward_workspace_bytes': 0, 'motif_b200_rms_norm_backward': 2,
                          'motif_b200_chord_backward': 2, 'motif_b200_kv4_chord_attention': 2,
                          'motif_b200_kv4_unit_bytes': 0, 'motif_b200_kv4_attention_workspace_bytes': 0,

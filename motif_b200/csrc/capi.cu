@@ -57,9 +57,18 @@ int encode_tile_map(CUtensorMap* map, const void* base, int elem_bytes, int rank
     estr[i] = 1;
     if (i + 1 < rank) st[i] = strides_bytes[i];
   }
-  CUresult r = g_encode_tiled(map, dt, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, estr,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return g_encode_tiled(map, dt, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+    // a host thread whose first CUDA call this is (an autograd thread): the runtime makes the device's
+    // context current with its own first call that needs one, a driver call does not
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   if (r != CUDA_SUCCESS) return set_error(MB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return MB_OK;
 }

@@ -227,20 +227,59 @@ Loss loss_forward(const Tensor& x, const Tensor& weight, const Tensor& labels, i
   return out;
 }
 
+// Where one gradient arrives for all tokens, the forward pass computes the gradients as well, in one pass over
+// the logits, and the backward pass multiplies them with what arrived.  (fp16, whose range is too small for that,
+// and one gradient per token: the logits are computed again in the backward pass.)
 struct LossFunction : torch::autograd::Function<LossFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& labels, int64_t ignore,
                         int64_t reduction) {
-    Loss out = loss_forward(x, weight, labels, ignore, reduction);
-    ctx->save_for_backward({weight, out.state});
     ctx->saved_data["reduction"] = reduction;
-    ctx->saved_data["bytes"] = out.backward_bytes;
     ctx->saved_data["shape"] = x.sizes().vec();
-    return out.loss;
+    const bool again = reduction == 0 || x.scalar_type() == at::kHalf;
+    ctx->saved_data["again"] = again;
+    if (again) {
+      Loss out = loss_forward(x, weight, labels, ignore, reduction);
+      ctx->save_for_backward({weight, out.state});
+      ctx->saved_data["bytes"] = out.backward_bytes;
+      return out.loss;
+    }
+    const c10::Device dev = x.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const Tensor r = rows_of(x), w = rows_of(weight), lab = labels.to(at::kLong).contiguous();
+    const int64_t n = r.size(0), d = r.size(1), v = w.size(0);
+    const int dc = dtype_code(x.scalar_type());
+    Tensor loss = fresh({}, at::kFloat, dev), dx, dw;
+    if (x.requires_grad()) dx = fresh(x.sizes(), x.scalar_type(), dev);
+    if (weight.requires_grad()) dw = fresh({v, d}, x.scalar_type(), dev);
+    const int64_t bytes = motif_b200_linear_cross_entropy_train_workspace_bytes(w.data_ptr(), w.stride(0), n, v, d, dc);
+    check("motif_b200_linear_cross_entropy_train", bytes < 0 ? MB_ERR_SHAPE : MB_OK);
+    const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes);
+    check("motif_b200_linear_cross_entropy_train",
+          motif_b200_linear_cross_entropy_train(r.data_ptr(), r.stride(0), w.data_ptr(), w.stride(0),
+                                                lab.data_ptr<int64_t>(), ignore, (int)reduction,
+                                                loss.data_ptr<float>(), ptr(dx), ptr(dw), n, v, d, ws.get(), bytes, dc,
+                                                stream_of(dev)));
+    ctx->save_for_backward({dx, dw});
+    return loss;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order();
     const variable_list saved = ctx->get_saved_variables();
+    Tensor dx, dw;
+    if (!ctx->saved_data["again"].toBool()) {
+      const Tensor &sx = saved[0], &sw = saved[1], &any = sx.defined() ? sx : sw;
+      const c10::Device dev = any.device();
+      const c10::cuda::CUDAGuard guard(dev);
+      if (sx.defined() && ctx->needs_input_grad(0)) dx = fresh(sx.sizes(), sx.scalar_type(), dev);
+      if (sw.defined() && ctx->needs_input_grad(1)) dw = fresh(sw.sizes(), sw.scalar_type(), dev);
+      check_backward("motif_b200_scale_gradients",
+                     motif_b200_scale_gradients(dx.defined() ? sx.data_ptr() : nullptr, ptr(dx),
+                                                dx.defined() ? dx.numel() : 0, dw.defined() ? sw.data_ptr() : nullptr,
+                                                ptr(dw), dw.defined() ? dw.numel() : 0, grads[0].data_ptr<float>(),
+                                                dtype_code(any.scalar_type()), stream_of(dev)));
+      return {dx, dw, Tensor(), Tensor(), Tensor()};
+    }
     const Tensor &weight = saved[0], &state = saved[1];
     const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
     const int64_t reduction = ctx->saved_data["reduction"].toInt(), bytes = ctx->saved_data["bytes"].toInt();
@@ -250,7 +289,6 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
     const int64_t v = w.size(0), d = w.size(1);
     int64_t n = 1;
     for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
-    Tensor dx, dw;
     if (ctx->needs_input_grad(0)) dx = fresh(shape, weight.scalar_type(), dev);
     if (ctx->needs_input_grad(1)) dw = fresh({v, d}, weight.scalar_type(), dev);
     const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes);

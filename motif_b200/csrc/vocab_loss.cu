@@ -234,6 +234,11 @@ struct PackArgs {
   int* index;              // [rows]: of the packed rows, where they came from
   int* place;              // [N]: the packed row of a token, -1 without one
   float* loss;             // per-token losses: 0 is written for tokens without one (null: no such output)
+  const void* w;           // with `ref`: [V, d], rows ws apart
+  int64_t ws;
+  float* ref;              // [rows]: the label's logit of the packed rows, or null
+  int* flags;              // [runs]: zeroed here for the scores
+  int runs;
 };
 
 __global__ void __launch_bounds__(256) group_count_kernel(const int64_t* __restrict__ labels, int64_t N, int64_t ignore,
@@ -308,6 +313,30 @@ __device__ __forceinline__ void zero_row(Op<T>* dst, int dp, int64_t part, int l
     for (int c = lane * 8; c < dp; c += 256) *reinterpret_cast<uint4*>(dst + p * part + c) = make_uint4(0, 0, 0, 0);
 }
 
+// Sum of the products of two rows, in fp32; a warp.
+template <typename T>
+__device__ __forceinline__ float dot_rows(const T* x, const T* w, int d, int lane) {
+  const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, aw = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+  float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int c0 = lane * 8; c0 < d; c0 += 512) {
+    Eight<T> u[2], v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (c0 + 256 * i < d) {
+        u[i].load(x, c0 + 256 * i, d, ax);
+        v[i].load(w, c0 + 256 * i, d, aw);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (c0 + 256 * i < d) {
+        const T *p = reinterpret_cast<const T*>(u[i].u), *q = reinterpret_cast<const T*>(v[i].u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = fmaf(to_f(p[e]), to_f(q[e]), t[e]);
+      }
+  }
+  return warp_sum(((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])));
+}
+
 constexpr int kPackTokens = 16;  // of a CTA: two for each of its eight warps
 
 template <typename T>
@@ -360,7 +389,14 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
     const int64_t token = first + i;
     if (token >= a.N) break;
     const int to = place[token - run];
-    if (to >= 0) pack_row<T>(x + token * a.xs, a.d, out + (int64_t)to * a.dp, a.dp, plane, lane);
+    if (to < 0) continue;
+    pack_row<T>(x + token * a.xs, a.d, out + (int64_t)to * a.dp, a.dp, plane, lane);
+    if (a.ref) {
+      const int64_t word = a.labels[token];
+      const bool known = word >= 0 && word < a.V;
+      const float s = known ? dot_rows<T>(x + token * a.xs, reinterpret_cast<const T*>(a.w) + word * a.ws, a.d, lane) : 0.f;
+      if (lane == 0) a.ref[to] = s;
+    }
   }
   // the last CTA sees all tokens: it leaves their number, and zeros up to the end of the last 64 rows (what the
   // products sum over together)
@@ -371,6 +407,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
       *a.count = total;
       *a.ticket = 0;
     }
+    if (a.flags)
+      for (int i = tid; i < a.runs; i += 256) a.flags[i] = 0;
   }
 }
 
@@ -391,6 +429,16 @@ __global__ void __launch_bounds__(256) pack_weight_kernel(const T* __restrict__ 
 }
 
 // ------------------------------------------------------------------------------- scores
+// What becomes of a tile of logits:
+//   kLoss   nothing but its rows' maxima and sums of exponentials
+//   kAgain  G, from the rows' maxima and sums
+//   kOnce   E = exp(s - s_t) (0 at the label): the gradients' exponentials before their sum is known, with that
+//           sum.  s_t, the label's logit, is known before, and is near the largest one unless the loss is
+//           large: exp(66) fits all types here.  A row with a larger logit raises the run's flag; its sum goes
+//           on from there, and kAgain computes the run's G instead.
+enum { kLoss, kAgain, kOnce };
+constexpr float kFar = 66.0f;
+
 struct ScoreArgs {
   const int* count;         // tokens with a loss
   int row0, rows;           // this call's packed rows: row0 .. row0 + rows
@@ -398,14 +446,16 @@ struct ScoreArgs {
   int kblocks;
   int64_t x_part, w_part;   // rows from one part of an operand to the next
   const int* label;         // [rows of the packed operand]
-  float2* seg;              // forward: (maximum, sum) of each row of half a pair's run through a row tile
-  float* target;            // forward: the label's logit
-  const RowStat* stat;      // backward
-  const int* index;         // backward: packed row -> token
-  const float* up;          // backward: per-token gradients (null: 1)
+  float2* seg;              // kLoss, kOnce: (reference, sum) of each row of half a pair's run through a row tile
+  float* target;            // kLoss: the label's logit
+  const float* ref;         // kOnce: the label's logit
+  int* flag;                // kOnce: set where a logit is far above it; kAgain: works only if set (null: always)
+  const RowStat* stat;      // kAgain
+  const int* index;         // kAgain: packed row -> token
+  const float* up;          // kAgain: per-token gradients (null: 1)
   int64_t up_stride;
-  const float* scale;       // backward: [1] = what `up` is multiplied by (a power of two); with `up` only
-  int64_t g_part;           // backward: rows from one part of G to the next
+  const float* scale;       // kAgain: [1] = what `up` is multiplied by (a power of two); with `up` only
+  int64_t g_part;           // rows from one part of G or E to the next
 };
 
 // Pair p of np (as many as there are, or as there are tiles) walks the tiles [p T / np, (p + 1) T / np) of the
@@ -416,7 +466,7 @@ __host__ __device__ __forceinline__ int64_t range_owner(int64_t t, int64_t tiles
   return ((t + 1) * np - 1) / tiles;
 }
 
-template <typename T, bool GRAD>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_constant__ CUtensorMap tmX,
                                                              const __grid_constant__ CUtensorMap tmX32,
                                                              const __grid_constant__ CUtensorMap tmW,
@@ -431,7 +481,8 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
   const bool leader = rank == 0;
   const uint32_t tmem = pair_begin(s);
   const int np = gridDim.x >> 1, pair = blockIdx.x >> 1;
-  const int live = min(max(*a.count - a.row0, 0), a.rows);
+  int live = min(max(*a.count - a.row0, 0), a.rows);
+  if (MODE == kAgain && a.flag && *a.flag == 0) live = 0;
   const int mt = (live + kTile - 1) / kTile, nt = (a.nv + kTile - 1) / kTile;
   const int64_t tiles = (int64_t)mt * nt;
   const int64_t walkers = min((int64_t)np, tiles);
@@ -481,28 +532,131 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
     const int in_tile = (int)rank * 128 + q * 32 + lane, c0 = half * (kTile / 2);
     unsigned char* buf = s.end + (warp - 2) * 4096;
     int slot = 0, done = 0, m_now = -1, label = -1;
-    bool lost = false;
-    float top = -INFINITY, sum = 0.f;      // forward: of the run so far
-    float neg_top = 0.f, inv = 0.f, g = 0.f;  // backward
-    bool mine = false;
+    bool lost = false, mine = false;
+    float top = 0.f, sum = 0.f;  // kLoss, kOnce: of the run so far; kAgain: the row's largest logit
+    float inv = 0.f, g = 0.f;    // kAgain
+    // 32 columns from column c of the tile: `at` is the label's, `valid` columns are words
+    auto chunk = [&](uint32_t (&r)[32], int c, int at, int valid, int row, int x, int y) {
+      float z[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(r[i]);
+      if (MODE != kAgain && valid < c + 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (c + i >= valid) z[i] = -INFINITY;
+      }
+      if (MODE != kAgain && __any_sync(0xffffffffu, (unsigned)(at - c) < 32u)) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (at == c + i) {
+            if (MODE == kLoss)
+              a.target[row] = z[i];
+            else
+              z[i] = -INFINITY;  // its part is known
+          }
+      }
+      if constexpr (MODE != kAgain) {
+        float t4[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          t4[j] = fmax3(z[8 * j], z[8 * j + 1], z[8 * j + 2]);
+          t4[j] = fmax3(t4[j], z[8 * j + 3], z[8 * j + 4]);
+          t4[j] = fmax3(t4[j], z[8 * j + 5], z[8 * j + 6]);
+          t4[j] = fmaxf(t4[j], z[8 * j + 7]);
+        }
+        const float now = fmaxf(fmax3(t4[0], t4[1], t4[2]), t4[3]);
+        const bool raise = MODE == kLoss ? now > top : mine && now > top + kFar;  // (rows behind the last hold anything)
+        if (__any_sync(0xffffffffu, raise) && raise) {
+          sum *= ex2f_((top - now) * kLog2e);  // 0 from a reference of -inf
+          top = now;
+          if (MODE == kOnce) *a.flag = 1;
+        }
+      }
+      // (s - top) log2 e: as one multiply-add where the type's own rounding is coarser than the product top log2 e
+      const float ref = MODE == kLoss && top == -INFINITY ? 0.f : top;
+      const float2 c2 = make_float2(kLog2e, kLog2e), n2 = make_float2(-ref, -ref);
+      const float2 m2 = make_float2(-ref * kLog2e, -ref * kLog2e), i2 = make_float2(inv, inv);
+      float2 acc0 = make_float2(0.f, 0.f), acc1 = acc0;
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const float2 v = make_float2(z[i], z[i + 1]);
+        const float2 e = P == 1 ? ffma2(v, c2, m2) : fmul2(fadd2(v, n2), c2);
+        float2 w = make_float2(ex2f_(e.x), ex2f_(e.y));
+        if constexpr (MODE == kAgain) {
+          w = fmul2(w, i2);
+        } else if (i & 2) {
+          acc1 = fadd2(acc1, w);
+        } else {
+          acc0 = fadd2(acc0, w);
+        }
+        z[i] = w.x;
+        z[i + 1] = w.y;
+      }
+      if constexpr (MODE != kAgain) {
+        acc0 = fadd2(acc0, acc1);
+        sum += acc0.x + acc0.y;
+      } else if (__any_sync(0xffffffffu, (unsigned)(at - c) < 32u)) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (at == c + i) z[i] -= g;
+      }
+      if constexpr (MODE != kLoss) {
+        if (!mine || valid < c + 32) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!mine || c + i >= valid) z[i] = 0.f;
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            w[i] = pack2<O>(z[2 * i], z[2 * i + 1]);
+            if (p + 1 < P) {
+              const float2 back = round2<O>(z[2 * i], z[2 * i + 1]);
+              z[2 * i] -= back.x;
+              z[2 * i + 1] -= back.y;
+            }
+          }
+          // two buffers of 32 rows x 64 bytes in turn, in the 64-byte swizzle of the tensor map
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
+          __syncwarp();
+          unsigned char* b = buf + slot * 2048;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<uint4*>(b + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
+                             reinterpret_cast<uint64_t>(&tmG)),
+                         "r"(x + c), "r"((int)(p * a.g_part) + y), "r"(smem_u32(b))
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+          }
+          slot ^= 1;
+        }
+      }
+    };
     for (int64_t t = t0; t < t1; ++t, ++done) {
       const int m = (int)(t / nt), n = (int)(t - (int64_t)m * nt);
       const int row = a.row0 + m * kTile + in_tile;
       if (m != m_now) {
-        if constexpr (!GRAD) {
-          if (m_now >= 0) a.seg[((int64_t)(pair + m_now) * 2 + half) * kTile + in_tile] = make_float2(top, sum);
-          top = -INFINITY;
-          sum = 0.f;
-        }
+        if (MODE != kAgain && m_now >= 0)
+          a.seg[((int64_t)(pair + m_now) * 2 + half) * kTile + in_tile] = make_float2(top, sum);
         m_now = m;
         mine = m * kTile + in_tile < live;
         label = mine ? a.label[row] : -1;
-        if constexpr (GRAD) {
+        sum = 0.f;
+        if constexpr (MODE == kLoss) top = -INFINITY;
+        if constexpr (MODE == kOnce) top = mine ? a.ref[row] : 0.f;
+        if constexpr (MODE == kAgain) {
           if (mine) {
             const RowStat st = a.stat[row];
             g = a.up ? a.up[a.index[row] * a.up_stride] * a.scale[1] : 1.0f;
             if constexpr (std::is_same<T, __half>::value) g *= kHalfScale;
-            neg_top = -st.top;
+            top = st.top;
             inv = st.inv * g;
           }
         }
@@ -510,108 +664,29 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       const int at = label - (a.v0 + n * kTile);  // the label's column, if it is in this tile
       const int valid = a.nv - n * kTile;         // columns of the tile that are words
       const uint32_t taddr = tmem + (uint32_t)((done & 1) * kTile) + ((uint32_t)(q * 32) << 16);
+      const int x = n * kTile, y = m * kTile + (int)rank * 128 + q * 32;
       tile_ready(s, done, lost);
-      uint32_t r[32];
-      read32(taddr + c0, lost, r);
-#pragma unroll 1
-      for (int c = c0; c < c0 + kTile / 2; c += 32) {
-        read32_wait(lost, r);
-        float z[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(r[i]);
-        if (c + 32 < c0 + kTile / 2) read32(taddr + c + 32, lost, r);  // on its way behind this chunk's arithmetic
-        const bool here = (unsigned)(at - c) < 32u;
-        if constexpr (!GRAD) {
-          if (__any_sync(0xffffffffu, here)) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (at == c + i) a.target[row] = z[i];
-          }
-          if (valid < c + 32) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c + i >= valid) z[i] = -INFINITY;
-          }
-          float t4[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            t4[j] = fmax3(z[8 * j], z[8 * j + 1], z[8 * j + 2]);
-            t4[j] = fmax3(t4[j], z[8 * j + 3], z[8 * j + 4]);
-            t4[j] = fmax3(t4[j], z[8 * j + 5], z[8 * j + 6]);
-            t4[j] = fmaxf(t4[j], z[8 * j + 7]);
-          }
-          const float now = fmaxf(fmax3(t4[0], t4[1], t4[2]), fmaxf(t4[3], top));
-          const float ref = now == -INFINITY ? 0.f : now;
-          const float2 nref = make_float2(-ref, -ref), c2 = make_float2(kLog2e, kLog2e);
-          float2 acc = make_float2(sum * ex2f_((top - ref) * kLog2e), 0.f);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 e = fmul2(fadd2(make_float2(z[i], z[i + 1]), nref), c2);
-            acc = fadd2(acc, make_float2(ex2f_(e.x), ex2f_(e.y)));
-          }
-          top = now;
-          sum = acc.x + acc.y;
-        } else {
-          const float2 nref = make_float2(neg_top, neg_top), c2 = make_float2(kLog2e, kLog2e), i2 = make_float2(inv, inv);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 e = fmul2(fadd2(make_float2(z[i], z[i + 1]), nref), c2);
-            const float2 w = fmul2(make_float2(ex2f_(e.x), ex2f_(e.y)), i2);
-            z[i] = w.x;
-            z[i + 1] = w.y;
-          }
-          if (__any_sync(0xffffffffu, here)) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (at == c + i) z[i] -= g;
-          }
-          if (!mine || valid < c + 32) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!mine || c + i >= valid) z[i] = 0.f;
-          }
-#pragma unroll
-          for (int p = 0; p < P; ++p) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              w[i] = pack2<O>(z[2 * i], z[2 * i + 1]);
-              if (p + 1 < P) {
-                const float2 back = round2<O>(z[2 * i], z[2 * i + 1]);
-                z[2 * i] -= back.x;
-                z[2 * i + 1] -= back.y;
-              }
-            }
-            // two buffers of 32 rows x 64 bytes in turn, in the 64-byte swizzle of the tensor map
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
-            __syncwarp();
-            unsigned char* b = buf + slot * 2048;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              *reinterpret_cast<uint4*>(b + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
-                               reinterpret_cast<uint64_t>(&tmG)),
-                           "r"(n * kTile + c), "r"((int)(p * a.g_part) + m * kTile + (int)rank * 128 + q * 32),
-                           "r"(smem_u32(b))
-                           : "memory");
-              asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
-            }
-            slot ^= 1;
-          }
-        }
-      }
-      tile_read(s, done, lost, leader);
+      uint32_t ra[32], rb[32];  // a chunk is on its way while the one before is computed
+      read32(taddr + c0, lost, ra);
+      read32_wait(lost, ra);
+      read32(taddr + c0 + 32, lost, rb);
+      chunk(ra, c0, at, valid, row, x, y);
+      read32_wait(lost, rb);
+      read32(taddr + c0 + 64, lost, ra);
+      chunk(rb, c0 + 32, at, valid, row, x, y);
+      read32_wait(lost, ra);
+      read32(taddr + c0 + 96, lost, rb);
+      chunk(ra, c0 + 64, at, valid, row, x, y);
+      read32_wait(lost, rb);
+      tile_read(s, done, lost, leader);  // the tile is in registers: the next one may come
+      chunk(rb, c0 + 96, at, valid, row, x, y);
     }
-    if constexpr (GRAD) {
+    if constexpr (MODE != kLoss) {
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
       __syncwarp();
-    } else {
-      if (m_now >= 0) a.seg[((int64_t)(pair + m_now) * 2 + half) * kTile + in_tile] = make_float2(top, sum);
     }
+    if (MODE != kAgain && m_now >= 0)
+      a.seg[((int64_t)(pair + m_now) * 2 + half) * kTile + in_tile] = make_float2(top, sum);
   }
   pair_end(tmem);
 }
@@ -627,16 +702,43 @@ struct JoinArgs {
   RowStat* stat;
   float* loss;       // [N] or one value
   double* partial;   // one a CTA
-  float* denom;      // 1 / tokens with a loss, for the backward pass
   int nt, np;        // of the scores
   int reduction;     // 0 none, 1 mean, 2 sum
 };
+
+// The sum of a CTA's losses to partial[cta]; the last CTA of all adds those, in one order whoever it is.
+template <int N>
+__device__ __forceinline__ void add_losses(double* sums, int cta, int ctas, double* partial, int* ticket, bool mean, int live,
+                                           float* out) {
+  __shared__ int last;
+  __shared__ double warps[8];
+  double loss = 0.0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < N; ++i) loss += sums[i];
+    partial[cta] = loss;
+    __threadfence();
+    last = atomicAdd(ticket, 1) == ctas - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  loss = 0.0;
+  for (int i = threadIdx.x; i < ctas; i += 256) loss += __ldcg(partial + i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = loss;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    loss = 0.0;
+    for (int i = 0; i < 8; ++i) loss += warps[i];
+    *out = (float)(mean ? loss / (double)live : loss);  // no tokens: 0 / 0, as it is
+  }
+}
 
 constexpr int kJoinRows = 32;  // of a CTA: eight threads a row share its runs
 
 __global__ void __launch_bounds__(8 * kJoinRows) join_kernel(const JoinArgs a) {
   __shared__ double sums[kJoinRows];
-  __shared__ int last;
   allow_dependent_launch();
   wait_for_previous();
   const int live = *a.count, r = threadIdx.x >> 3, j = threadIdx.x & 7, row = blockIdx.x * kJoinRows + r;
@@ -680,29 +782,139 @@ __global__ void __launch_bounds__(8 * kJoinRows) join_kernel(const JoinArgs a) {
   if (a.reduction == 0) return;
   if (j == 0) sums[r] = loss;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    loss = 0.0;
-    for (int i = 0; i < kJoinRows; ++i) loss += sums[i];
-    a.partial[blockIdx.x] = loss;
-    __threadfence();
-    last = atomicAdd(a.ticket, 1) == ctas - 1;
-  }
-  __syncthreads();
-  if (!last) return;
-  // the last CTA adds all of them, in one order whoever it is
-  __threadfence();
-  loss = 0.0;
-  for (int i = threadIdx.x; i < ctas; i += 8 * kJoinRows) loss += __ldcg(a.partial + i);
+  add_losses<kJoinRows>(sums, blockIdx.x, ctas, a.partial, a.ticket, a.reduction == 1, live, a.loss);
+}
+
+// kOnce's rows: their loss, and what turns exponentials into gradients.  G L = E - L [v = t] with L the whole
+// sum, so the label's place gets 1 - L = -(the sum of the others), which loses nothing however near to 1 its
+// probability is; dx's rows are divided by L at the end, and dW sums E times x / L.  A warp a row.
+struct SettleArgs {
+  const int* count;
+  int* ticket;
+  const float2* seg;
+  const float* ref;
+  const int* label;
+  RowStat* stat;
+  const int* flag;       // the run's exponentials are G (kAgain computes them next): nothing is left to divide
+  float* row_scale;      // [rows of the run]
+  float* loss;
+  double* partial;
+  int nt, np, mean;
+  int row0, rows;        // the run
+  const void* x;         // [parts][x_part][dp]
+  int64_t x_part;
+  void* weighed;         // [parts][w_part][dp]: x / L of the run's rows, zeros up to the end of 64
+  int64_t w_part;
+  int dp;
+  void* e;               // [parts][w_part][ld]
+  int64_t ld;
+};
+constexpr int kSettleRows = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kSettleRows) settle_kernel(const SettleArgs a) {
+  using O = Op<T>;
+  constexpr int P = kParts<T>;
+  __shared__ double sums[kSettleRows];
+  allow_dependent_launch();
+  wait_for_previous();
+  const int all = *a.count, live = min(max(all - a.row0, 0), a.rows), flagged = *a.flag;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x * kSettleRows + warp, row = a.row0 + r;
+  const int cta = a.row0 / kSettleRows + blockIdx.x, ctas = max((all + kSettleRows - 1) / kSettleRows, 1);
+  O* weighed = reinterpret_cast<O*>(a.weighed) + (int64_t)r * a.dp;
+  const int64_t w_plane = a.w_part * a.dp, x_plane = a.x_part * a.dp;
+  double loss = 0.0;
+  if (r < live) {
+    const int mt = (live + kTile - 1) / kTile, m = r / kTile, in_tile = r % kTile;
+    const int64_t tiles = (int64_t)mt * a.nt, walkers = min((int64_t)a.np, tiles);
+    const int s0 = 2 * ((int)range_owner((int64_t)m * a.nt, tiles, walkers) + m);
+    const int s1 = 2 * ((int)range_owner((int64_t)(m + 1) * a.nt - 1, tiles, walkers) + m) + 2;
+    const float ref = a.ref[row];
+    float top = ref, sum = 0.f;
+    for (int i = s0 + lane; i < s1; i += 32) {
+      const float2 v = a.seg[(int64_t)i * kTile + in_tile];
+      const float now = fmaxf(top, v.x);
+      sum = sum * ex2f_((top - now) * kLog2e) + v.y * ex2f_((v.x - now) * kLog2e);
+      top = now;
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+    for (int o = 1; o < 32; o <<= 1) {
+      const float t2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
+      const float now = fmaxf(top, t2);
+      const float mine = sum * ex2f_((top - now) * kLog2e), other = s2 * ex2f_((t2 - now) * kLog2e);
+      sum = (lane & o) ? other + mine : mine + other;
+      top = now;
+    }
+    const int label = a.label[row];
+    const float nan = __int_as_float(0x7fffffff), own = ex2f_((ref - top) * kLog2e);  // 1 but for far logits
+    const float inv = label >= 0 ? 1.0f / (sum + own) : nan;  // a label that is no word: NaN, in the gradients too
+    loss = label < 0 ? nan : top == ref ? log1pf(sum) : (top - ref) + logf(sum + own);
+    const float scale = flagged && label >= 0 ? 1.0f : inv;
+    if (lane == 0) {
+      RowStat st;
+      st.top = top;
+      st.inv = inv;
+      a.stat[row] = st;
+      a.row_scale[r] = scale;
+      if (!flagged && label >= 0) {
+        O* e = reinterpret_cast<O*>(a.e) + (int64_t)r * a.ld + label;
+        if constexpr (P == 1) {
+          *e = from_f<O>(-sum);
+        } else {
+          __nv_bfloat16 p[3];
+          split3(-sum, p);
+          for (int i = 0; i < 3; ++i) e[i * a.w_part * a.ld] = p[i];
+        }
+      }
+    }
+    const O* x = reinterpret_cast<const O*>(a.x) + (int64_t)row * a.dp;
+    for (int c = lane * 8; c < a.dp; c += 256) {
+      Eight<T> v;
+      T* o = reinterpret_cast<T*>(v.u);
+      float f[8];
+      uint4 u[P];
+#pragma unroll
+      for (int p = 0; p < P; ++p) u[p] = *reinterpret_cast<const uint4*>(x + p * x_plane + c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[i] = to_f(reinterpret_cast<const O*>(&u[P - 1])[i]);
+        for (int p = P - 2; p >= 0; --p) f[i] += to_f(reinterpret_cast<const O*>(&u[p])[i]);
+        o[i] = from_f<T>(f[i] * scale);
+      }
+      v.store(weighed, c, w_plane);
+    }
+  } else if (r < (live + kBK - 1) / kBK * kBK) {
+    zero_row<T>(weighed, a.dp, w_plane, lane);
+  }
+  if (cta >= ctas || (r - warp >= live && cta > 0)) return;  // (the first CTA is there for a call without tokens, too)
+  if (lane == 0) sums[warp] = loss;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = loss;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    loss = 0.0;
-    for (int i = 0; i < 8; ++i) loss += sums[i];
-    *a.loss = (float)(a.reduction == 1 ? loss / (double)live : loss);  // no tokens: 0 / 0, as it is
-    *a.denom = (float)(1.0 / (double)live);
+  add_losses<kSettleRows>(sums, cta, ctas, a.partial, a.ticket, a.mean, all, a.loss);
+}
+
+// dst = src * *scale, for up to two arrays: the gradients of a loss that another one follows.
+template <typename T>
+__global__ void __launch_bounds__(256) scale_out_kernel(const T* __restrict__ a, T* __restrict__ ao, int64_t na,
+                                                        const T* __restrict__ b, T* __restrict__ bo, int64_t nb,
+                                                        const float* __restrict__ scale) {
+  const float s = *scale;
+  const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const T* src = which ? b : a;
+    T* dst = which ? bo : ao;
+    const int64_t n = which ? nb : na, vecs = n / E;
+#pragma unroll 4
+    for (int64_t i = first; i < vecs; i += step) {
+      const uint4 u = reinterpret_cast<const uint4*>(src)[i];
+      const T* e = reinterpret_cast<const T*>(&u);
+      __align__(16) T o[E];
+#pragma unroll
+      for (int k = 0; k < E; ++k) o[k] = from_f<T>(to_f(e[k]) * s);
+      reinterpret_cast<uint4*>(dst)[i] = *reinterpret_cast<const uint4*>(o);
+    }
+    for (int64_t i = vecs * E + first; i < n; i += step) dst[i] = from_f<T>(to_f(src[i]) * s);
   }
 }
 
@@ -738,13 +950,16 @@ struct ProductArgs {
   int v0, nv;               // its vocabulary
   int d;
   int64_t a_part, b_part;   // rows from one part of an operand to the next
-  float4* slots;            // [pairs][256 / 4][256]: tiles whose sum is split
+  float4* slots;            // [2 pairs][256 / 4][256]: tiles whose sum is split
   float* acc;               // [rows or nv][ld] fp32, or null
   int64_t ld;
   int first, last;          // first: acc holds nothing yet; last: the result leaves as T
+  int g0;                   // column of G where the piece begins
+  int b_row0;               // dW: the right operand's first row
+  const float* row_scale;   // dx: [rows], or null
   const float* scale;       // [0] (per-token gradients), or null:
-  const float* up;          // the one gradient,
-  const float* denom;       // times this (the mean's), or null
+  const float* up;          // the one gradient (null: 1),
+  int mean;                 // over the tokens with a loss
   void* out;                // dx (rows by `index`) or dW
   const int* index;
   const int* place;         // dx, first call: [N], the tokens without a loss (-1) get zeros
@@ -756,13 +971,12 @@ __device__ __forceinline__ float last_scale(const ProductArgs& a) {
   const float fold = std::is_same<T, __half>::value ? 1.0f / kHalfScale : 1.0f;
   if (a.scale) return a.scale[0] * fold;
   if (*a.count <= 0) return 0.0f;  // no token has a loss: the gradients are zero, whatever 0 / 0 says
-  return *a.up * (a.denom ? *a.denom : 1.0f) * fold;
+  return (a.up ? *a.up : 1.0f) * (a.mean ? 1.0f / (float)*a.count : 1.0f) * fold;
 }
 struct Cut {  // how a product's tiles are spread over the pairs
   int mt, nt, kb, full, split, units;
 };
-// Whole waves of tiles keep their sum in one pair; of the rest each tile's sum is cut into as many
-// equal parts as there are pairs for it.
+// Whole waves of tiles keep their sum in one pair; of the rest each tile's sum is cut into equal parts.
 __host__ __device__ __forceinline__ Cut cut_product(const ProductArgs& a, int live, int np) {
   Cut c;
   const int m = a.by_rows ? live : a.nv, k = a.by_rows ? (live > 0 ? a.nv : 0) : live;
@@ -771,7 +985,11 @@ __host__ __device__ __forceinline__ Cut cut_product(const ProductArgs& a, int li
   c.kb = (k + kBK - 1) / kBK;
   const int tiles = c.mt * c.nt, rem = tiles % np;
   c.full = tiles - rem;
-  c.split = rem > 0 && c.kb > 1 ? min(np / rem, c.kb) : 1;
+  // one wave of parts, or two where that ends more than a tenth sooner (48 tiles on 74 pairs: 3 parts each)
+  c.split = rem > 0 ? np / rem : 1;
+  const int two = rem > 0 ? 2 * np / rem : 1;
+  if (c.split * 18 < two * 10) c.split = two;
+  c.split = min(c.split, c.kb);
   if (c.split <= 1) {
     c.split = 1;
     c.full = tiles;
@@ -904,7 +1122,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const int rows = A_MN ? kTile : live - w.m * kTile, boxes = boxes_of(rows, rank);
         const uint32_t bytes = 4096 * (boxes_of(rows, 0) + boxes_of(rows, 1)) + 2 * kOperand;
         // the right operand's rows: words of this piece, or this call's tokens
-        const int br = a.by_rows ? a.v0 : a.row0;
+        const int br = a.by_rows ? a.v0 : a.b_row0;
         for (int p = 0; p < Parts<P>::n && !failed; ++p)
           for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
             uint32_t bar;
@@ -915,10 +1133,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             }
             const int pa = (int)(Parts<P>::a(p) * a.a_part), pb = (int)(Parts<P>::b(p) * a.b_part);
             if constexpr (A_MN) {
-              tma_load_2d_pair(st, &tmA, ar, pa + kb * kBK, bar);
-              tma_load_2d_pair(st + 8192, &tmA, ar + 64, pa + kb * kBK, bar);
+              tma_load_2d_pair(st, &tmA, a.g0 + ar, pa + kb * kBK, bar);
+              tma_load_2d_pair(st + 8192, &tmA, a.g0 + ar + 64, pa + kb * kBK, bar);
             } else {
-              load_rows(st, &tmA, &tmA32, boxes, kb * kBK, pa + ar, bar);
+              load_rows(st, &tmA, &tmA32, boxes, a.g0 + kb * kBK, pa + ar, bar);
             }
             tma_load_2d_pair(st + kOperand, &tmB, bc, pb + br + kb * kBK, bar);
             tma_load_2d_pair(st + kOperand + 8192, &tmB, bc + 64, pb + br + kb * kBK, bar);
@@ -981,7 +1199,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 #pragma unroll
           for (int i = 0; i < 8; ++i) p[i * kTile] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         } else {
-          finish32<T>(a, row, rows, w.n * kTile + col, v, scale, buf);
+          const float own = a.last && a.row_scale && row < rows ? scale * a.row_scale[row] : scale;
+          finish32<T>(a, row, rows, w.n * kTile + col, v, own, buf);
         }
       }
       if (c.kb > 0) tile_read(s, done, lost, leader);
@@ -1032,7 +1251,7 @@ __global__ void __launch_bounds__(256) join_product_kernel(const ProductArgs a, 
     *acc = v;
     return;
   }
-  const float scale = last_scale<T>(a);
+  const float scale = last_scale<T>(a) * (a.row_scale ? a.row_scale[row] : 1.0f);
   T* p = reinterpret_cast<T*>(a.out) + row_out(a, row) + col;
   const float e[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
   if (a.d % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
@@ -1055,7 +1274,7 @@ struct Sizes {
   int parts;
   int64_t rows, dp, vrows;  // packed rows, row length, packed words
   // offsets of the state
-  int64_t x, w, label, index, place, stat, count, ticket, denom, state_bytes;
+  int64_t x, w, label, index, place, stat, count, ticket, state_bytes;
   // forward workspace
   int64_t group, seg, target, partial, forward_bytes;
   // backward: rows of a run, words of a piece, and the workspace
@@ -1087,7 +1306,6 @@ Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) 
   s.stat = take(s.state_bytes, s.rows * (int64_t)sizeof(RowStat));
   s.count = take(s.state_bytes, 4);
   s.ticket = take(s.state_bytes, 4);
-  s.denom = take(s.state_bytes, 4);
   const int64_t mt = s.rows / kTile;
   s.group = take(s.forward_bytes, up_to(N, 256) / 256 * 4);
   s.seg = take(s.forward_bytes, (np + mt) * 2 * kTile * (int64_t)sizeof(float2));
@@ -1104,10 +1322,64 @@ Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) 
   }
   if (s.parts == 1) s.run = std::min(s.rows, std::max(s.run, most / s.piece / kTile * kTile));
   s.g = take(s.backward_bytes, s.parts * s.run * s.piece * 2);
-  s.slots = take(s.backward_bytes, (int64_t)np * kTile * kTile * 4);
+  s.slots = take(s.backward_bytes, 2LL * np * kTile * kTile * 4);
   s.dx_acc = take(s.backward_bytes, s.piece < s.vrows ? s.run * up_to(d, 4) * 4 : 0);
   s.dw_acc = take(s.backward_bytes, s.run < s.rows ? V * up_to(d, 4) * 4 : 0);
   s.scale = take(s.backward_bytes, 8);
+  return s;
+}
+
+// The loss and its gradients at once: everything lies in the workspace.
+struct OnceSizes {
+  int parts;
+  int64_t rows, dp, vrows, run, runs, piece;
+  int64_t x, w, label, index, place, stat, ref, row_scale, count, ticket, flags, group, seg, partial;
+  int64_t e, weighed, slots, dx_acc, dw_acc, bytes;
+};
+// Elements of E that are there at once: a run of rows with the whole vocabulary (fp32: three parts of a third
+// as many).
+constexpr int64_t kOnceElements = 1LL << 28;
+// 16-bit: terms that are added within the tensor cores, which cut each partial sum off at 24 bits (2^16 / 16
+// of them: 2^-12 of the result at most, half a unit of bf16 being 2^-9).
+constexpr int64_t kLongRun = 1LL << 16;
+
+OnceSizes once_sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) {
+  OnceSizes s = {};
+  s.parts = dtype == MB_F32 ? 3 : 1;
+  s.rows = up_to(std::max<int64_t>(N, 1), kTile);
+  s.dp = up_to(d, 8);
+  s.vrows = up_to(V, kTile);
+  s.run = std::min(s.rows, std::max<int64_t>(kTile, kOnceElements / s.parts / s.vrows / kTile * kTile));
+  if (s.parts == 3) s.run = std::min(s.run, kExactRun);
+  s.run = std::min(s.run, kLongRun);
+  s.runs = (s.rows + s.run - 1) / s.run;
+  // dx's sums run over the words of a piece; fp32: each in as many parts as there are pairs for a tile
+  const int64_t tiles = s.run / kTile * ((d + kTile - 1) / kTile);
+  s.piece = std::min(s.vrows, s.parts == 3 ? kExactRun * std::max<int64_t>(1, np / tiles) : kLongRun);
+  auto take = [&](int64_t bytes) {
+    const int64_t at = s.bytes;
+    s.bytes = up_to(s.bytes + bytes, 256);
+    return at;
+  };
+  s.x = take(s.parts * s.rows * s.dp * 2);
+  s.w = take(pack_w ? s.parts * s.vrows * s.dp * 2 : 0);
+  s.label = take(s.rows * 4);
+  s.index = take(s.rows * 4);
+  s.place = take(N * 4);
+  s.stat = take(s.rows * (int64_t)sizeof(RowStat));
+  s.ref = take(s.rows * 4);
+  s.row_scale = take(s.run * 4);
+  s.count = take(4);
+  s.ticket = take(4);
+  s.flags = take(s.runs * 4);
+  s.group = take(up_to(N, 256) / 256 * 4);
+  s.seg = take((np + s.run / kTile) * 2 * kTile * (int64_t)sizeof(float2));
+  s.partial = take(s.rows / kSettleRows * 8);
+  s.e = take(s.parts * s.run * s.vrows * 2);
+  s.weighed = take(s.parts * s.run * s.dp * 2);
+  s.slots = take(2LL * np * kTile * kTile * 4);
+  s.dx_acc = take(s.piece < s.vrows ? s.run * up_to(d, 4) * 4 : 0);
+  s.dw_acc = take(s.runs > 1 ? V * up_to(d, 4) * 4 : 0);
   return s;
 }
 
@@ -1159,16 +1431,14 @@ void weight_rows(const Call& c, const void** base, int64_t* rows, int64_t* strid
   *cols = c.pack_w ? c.s.dp : c.d;
 }
 
+// The rows that have a loss, packed, and the weight where it has to be.
 template <typename T>
-int forward(const Call& c, float* loss) {
-  const Sizes& s = c.s;
-  int* group = nullptr;
+int pack(const Call& c, PackArgs& p, int* group, void* packed_w, int64_t vrows) {
   if (c.N > 8192) {  // below that a CTA reads the labels before its own
-    group = at<int>(c.work, s.group);
     group_count_kernel<<<(unsigned)((c.N + 255) / 256), 256, 0, c.st>>>(c.labels, c.N, c.ignore, group);
     if (int e = check_launch("linear_cross_entropy (count)")) return e;
+    p.group = group;
   }
-  PackArgs p = {};
   p.x = c.x;
   p.labels = c.labels;
   p.N = c.N;
@@ -1176,25 +1446,30 @@ int forward(const Call& c, float* loss) {
   p.ignore = c.ignore;
   p.V = (int)c.V;
   p.d = (int)c.d;
+  int rc = launch("linear_cross_entropy (pack)", pack_kernel<T>,
+                  std::max<int64_t>(1, (c.N + kPackTokens - 1) / kPackTokens), 256, c.st, 0, 1, p);
+  if (!rc && c.pack_w)
+    rc = launch("linear_cross_entropy (pack weight)", pack_weight_kernel<T>,
+                std::min<int64_t>((vrows + 7) / 8, multiprocessors() * 16), 256, c.st, 0, 1, (const T*)c.w, c.ws,
+                (int)c.V, (int)c.d, p.dp, vrows, (Op<T>*)packed_w);
+  return rc;
+}
+
+template <typename T>
+int forward(const Call& c, float* loss) {
+  const Sizes& s = c.s;
+  PackArgs p = {};
   p.dp = (int)s.dp;
   p.rows = s.rows;
   p.packed = c.state + s.x;
   p.count = at<int>(c.state, s.count);
   p.ticket = at<int>(c.state, s.ticket);
-  p.group = group;
   p.label = at<int>(c.state, s.label);
   p.index = at<int>(c.state, s.index);
   p.place = at<int>(c.state, s.place);
   p.loss = c.reduction == 0 ? loss : nullptr;
-  int rc = launch("linear_cross_entropy (pack)", pack_kernel<T>,
-                  std::max<int64_t>(1, (c.N + kPackTokens - 1) / kPackTokens), 256, c.st, 0, 1, p);
+  int rc = pack<T>(c, p, at<int>(c.work, s.group), c.state + s.w, s.vrows);
   if (rc) return rc;
-  if (c.pack_w) {
-    rc = launch("linear_cross_entropy (pack weight)", pack_weight_kernel<T>,
-                std::min<int64_t>((s.vrows + 7) / 8, multiprocessors() * 16), 256, c.st, 0, 1, (const T*)c.w, c.ws,
-                (int)c.V, (int)c.d, (int)s.dp, s.vrows, at<Op<T>>(c.state, s.w));
-    if (rc) return rc;
-  }
   CUtensorMap tmX, tmX32, tmW;
   const void* wb;
   int64_t wr, wst, wc;
@@ -1213,7 +1488,7 @@ int forward(const Call& c, float* loss) {
   a.label = p.label;
   a.seg = at<float2>(c.work, s.seg);
   a.target = at<float>(c.work, s.target);
-  rc = launch_pairs("linear_cross_entropy (scores)", scores_kernel<T, false>, c.np, c.st, tmX, tmX32, tmW, tmX, a);
+  rc = launch_pairs("linear_cross_entropy (scores)", scores_kernel<T, kLoss>, c.np, c.st, tmX, tmX32, tmW, tmX, a);
   if (rc) return rc;
   JoinArgs j = {};
   j.count = p.count;
@@ -1225,7 +1500,6 @@ int forward(const Call& c, float* loss) {
   j.stat = at<RowStat>(c.state, s.stat);
   j.loss = loss;
   j.partial = at<double>(c.work, s.partial);
-  j.denom = at<float>(c.state, s.denom);
   j.nt = (int)((c.V + kTile - 1) / kTile);
   j.np = c.np;
   j.reduction = c.reduction;
@@ -1277,7 +1551,7 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
       a.up_stride = up_stride;
       a.scale = scale;
       a.g_part = s.run;
-      rc = launch_pairs("linear_cross_entropy_backward (scores)", scores_kernel<T, true>, c.np, c.st, tmX, tmX32,
+      rc = launch_pairs("linear_cross_entropy_backward (scores)", scores_kernel<T, kAgain>, c.np, c.st, tmX, tmX32,
                         tmW, tmG, a);
       if (rc) return rc;
       ProductArgs p = {};
@@ -1292,7 +1566,8 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
       p.ld = up_to(c.d, 4);
       p.scale = c.reduction == 0 ? scale : nullptr;
       p.up = up;
-      p.denom = c.reduction == 1 ? at<float>(c.state, s.denom) : nullptr;
+      p.mean = c.reduction == 1;
+      p.b_row0 = p.row0;
       p.index = index;
       p.N = c.N;
       if (dx) {
@@ -1326,6 +1601,139 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
         if (rc) return rc;
       }
     }
+  return MB_OK;
+}
+
+// Loss and gradients, run by run: E, its rows' sums, then both products.
+template <typename T>
+int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
+  unsigned char* ws = c.work;
+  PackArgs p = {};
+  p.dp = (int)s.dp;
+  p.rows = s.rows;
+  p.packed = ws + s.x;
+  p.count = at<int>(ws, s.count);
+  p.ticket = at<int>(ws, s.ticket);
+  p.label = at<int>(ws, s.label);
+  p.index = at<int>(ws, s.index);
+  p.place = at<int>(ws, s.place);
+  p.w = c.w;
+  p.ws = c.ws;
+  p.ref = at<float>(ws, s.ref);
+  p.flags = at<int>(ws, s.flags);
+  p.runs = (int)s.runs;
+  int rc = pack<T>(c, p, at<int>(ws, s.group), ws + s.w, s.vrows);
+  if (rc) return rc;
+  const void* wb = c.pack_w ? ws + s.w : c.w;
+  const int64_t wr = c.pack_w ? s.parts * s.vrows : c.V, wst = c.pack_w ? s.dp : c.ws, wc = c.pack_w ? s.dp : c.d;
+  CUtensorMap tmX, tmX32, tmW, tmWk, tmE, tmEa, tmEa32, tmEt, tmXk;
+  unsigned char* e = ws + s.e;
+  rc = encode_tile_map_2d(&tmX, ws + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 128, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmX32, ws + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 32, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmW, wb, 2, wc, wr, wst * 2, kBK, 128, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmWk, wb, 2, wc, wr, wst * 2, 64, kBK, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmXk, ws + s.weighed, 2, s.dp, s.parts * s.run, s.dp * 2, 64, kBK, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmE, e, 2, s.vrows, s.parts * s.run, s.vrows * 2, 32, 32, 64);       // stored
+  if (!rc) rc = encode_tile_map_2d(&tmEa, e, 2, s.vrows, s.parts * s.run, s.vrows * 2, kBK, 128, 128);   // tokens x words
+  if (!rc) rc = encode_tile_map_2d(&tmEa32, e, 2, s.vrows, s.parts * s.run, s.vrows * 2, kBK, 32, 128);
+  if (!rc) rc = encode_tile_map_2d(&tmEt, e, 2, s.vrows, s.parts * s.run, s.vrows * 2, 64, kBK, 128);    // words x tokens
+  if (rc) return rc;
+  for (int64_t i = 0; i < s.runs; ++i) {
+    ScoreArgs a = {};
+    a.count = p.count;
+    a.row0 = (int)(i * s.run);
+    a.rows = (int)std::min(s.run, s.rows - i * s.run);
+    a.nv = (int)c.V;
+    a.kblocks = (int)((c.d + kBK - 1) / kBK);
+    a.x_part = s.rows;
+    a.w_part = s.vrows;
+    a.label = p.label;
+    a.seg = at<float2>(ws, s.seg);
+    a.ref = p.ref;
+    a.flag = p.flags + i;
+    a.stat = at<RowStat>(ws, s.stat);
+    a.index = p.index;
+    a.g_part = s.run;
+    rc = launch_pairs("linear_cross_entropy_train (scores)", scores_kernel<T, kOnce>, c.np, c.st, tmX, tmX32, tmW, tmE, a);
+    if (rc) return rc;
+    SettleArgs b = {};
+    b.count = p.count;
+    b.ticket = p.ticket;
+    b.seg = a.seg;
+    b.ref = p.ref;
+    b.label = p.label;
+    b.stat = at<RowStat>(ws, s.stat);
+    b.flag = a.flag;
+    b.row_scale = at<float>(ws, s.row_scale);
+    b.loss = loss;
+    b.partial = at<double>(ws, s.partial);
+    b.nt = (int)((c.V + kTile - 1) / kTile);
+    b.np = c.np;
+    b.mean = c.reduction == 1;
+    b.row0 = a.row0;
+    b.rows = a.rows;
+    b.x = ws + s.x;
+    b.x_part = s.rows;
+    b.weighed = ws + s.weighed;
+    b.w_part = s.run;
+    b.dp = (int)s.dp;
+    b.e = e;
+    b.ld = s.vrows;
+    rc = launch("linear_cross_entropy_train (settle)", settle_kernel<T>, a.rows / kSettleRows, 32 * kSettleRows, c.st, 0, 1, b);
+    if (!rc)
+      rc = launch_pairs("linear_cross_entropy_train (again)", scores_kernel<T, kAgain>, c.np, c.st, tmX, tmX32, tmW, tmE, a);
+    if (rc) return rc;
+    ProductArgs q = {};
+    q.count = p.count;
+    q.row0 = a.row0;
+    q.rows = a.rows;
+    q.d = (int)c.d;
+    q.a_part = s.run;
+    q.slots = at<float4>(ws, s.slots);
+    q.ld = up_to(c.d, 4);
+    q.mean = c.reduction == 1;
+    q.index = p.index;
+    q.N = c.N;
+    const int64_t nt = (c.d + kTile - 1) / kTile;
+    for (int64_t v0 = 0; dx && v0 < c.V; v0 += s.piece) {
+      q.by_rows = 1;
+      q.v0 = (int)v0;
+      q.g0 = (int)v0;
+      q.nv = (int)std::min(s.piece, c.V - v0);
+      q.b_part = s.vrows;
+      q.acc = at<float>(ws, s.dx_acc);
+      q.row_scale = b.row_scale;
+      q.first = v0 == 0;
+      q.last = v0 + s.piece >= c.V;
+      q.out = dx;
+      q.place = i == 0 && v0 == 0 ? p.place : nullptr;
+      rc = launch_pairs("linear_cross_entropy_train (dx)", product_kernel<T, false>, c.np, c.st, tmEa, tmEa32, tmWk, q);
+      // how many tiles are split the device knows: at most all, and fewer than there are pairs
+      const int64_t most = std::min<int64_t>(c.np - 1, a.rows / kTile * nt);
+      if (!rc && most > 0)
+        rc = launch("linear_cross_entropy_train (dx join)", join_product_kernel<T>, 64 * most, 256, c.st, 0, 1, q, c.np);
+      if (rc) return rc;
+    }
+    if (dw) {
+      q.by_rows = 0;
+      q.v0 = 0;
+      q.g0 = 0;
+      q.nv = (int)c.V;
+      q.b_part = s.run;
+      q.b_row0 = 0;
+      q.acc = at<float>(ws, s.dw_acc);
+      q.row_scale = nullptr;
+      q.first = i == 0;
+      q.last = i + 1 == s.runs;
+      q.out = dw;
+      q.place = nullptr;
+      rc = launch_pairs("linear_cross_entropy_train (dw)", product_kernel<T, true>, c.np, c.st, tmEt, tmEt, tmXk, q);
+      const int64_t rest = s.vrows / kTile * nt % c.np;
+      if (!rc && rest > 0 && c.N > kBK)  // (a sum of one stage is not split)
+        rc = launch("linear_cross_entropy_train (dw join)", join_product_kernel<T>, 64 * rest, 256, c.st, 0, 1, q, c.np);
+      if (rc) return rc;
+    }
+  }
   return MB_OK;
 }
 
@@ -1436,4 +1844,63 @@ extern "C" int motif_b200_linear_cross_entropy_backward(const void* w, int64_t w
   if (dtype == MB_F32) return backward<float>(c, grad_loss, grad_stride, dx, dw);
   return dtype == MB_BF16 ? backward<__nv_bfloat16>(c, grad_loss, grad_stride, dx, dw)
                           : backward<__half>(c, grad_loss, grad_stride, dx, dw);
+}
+
+extern "C" int64_t motif_b200_linear_cross_entropy_train_workspace_bytes(const void* w, int64_t ws, int64_t N, int64_t V,
+                                                                         int64_t d, int dtype) {
+  using namespace mb;
+  if (check_sizes("linear_cross_entropy_train_workspace_bytes", N, V, d, dtype)) return -1;
+  return once_sizes_of(N, V, d, must_pack(w, ws, d, dtype), dtype, std::max(1, multiprocessors() / 2)).bytes;
+}
+
+extern "C" int motif_b200_linear_cross_entropy_train(const void* x, int64_t xs, const void* w, int64_t ws,
+                                                     const int64_t* labels, int64_t ignore_index, int reduction,
+                                                     float* loss, void* dx, void* dw, int64_t N, int64_t V, int64_t d,
+                                                     void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+  using namespace mb;
+  Call c = {};
+  c.x = x;
+  c.xs = xs;
+  c.w = w;
+  c.ws = ws;
+  c.labels = labels;
+  c.ignore = ignore_index;
+  c.reduction = reduction;
+  c.N = N;
+  c.V = V;
+  c.d = d;
+  c.dtype = dtype;
+  c.state = c.work = (unsigned char*)workspace;
+  c.st = (cudaStream_t)stream;
+  if (int e = make_call("linear_cross_entropy_train", c)) return e;
+  MB_REQUIRE(dtype != MB_F16, MB_ERR_UNSUPPORTED,
+             "linear_cross_entropy_train: fp16 has too small a range for exponentials without their sum");
+  MB_REQUIRE(reduction == 1 || reduction == 2, MB_ERR_ARG, "linear_cross_entropy_train: reduction must be 1 or 2, got %d",
+             reduction);
+  MB_REQUIRE((N == 0 || (x && labels)) && loss, MB_ERR_ARG, "linear_cross_entropy_train: null pointer");
+  const OnceSizes s = once_sizes_of(N, V, d, c.pack_w, dtype, c.np);
+  MB_REQUIRE(workspace_bytes >= s.bytes, MB_ERR_ARG, "linear_cross_entropy_train: %lld bytes of workspace needed, got %lld",
+             (long long)s.bytes, (long long)workspace_bytes);
+  return dtype == MB_F32 ? once<float>(c, s, loss, dx, dw) : once<__nv_bfloat16>(c, s, loss, dx, dw);
+}
+
+extern "C" int motif_b200_scale_gradients(const void* a, void* a_out, int64_t a_n, const void* b, void* b_out, int64_t b_n,
+                                          const float* scale, int dtype, void* stream) {
+  using namespace mb;
+  MB_REQUIRE(scale && a_n >= 0 && b_n >= 0 && (a_n == 0 || (a && a_out)) && (b_n == 0 || (b && b_out)), MB_ERR_ARG,
+             "scale_gradients: null pointer or bad size");
+  MB_REQUIRE(((uintptr_t)a | (uintptr_t)a_out | (uintptr_t)b | (uintptr_t)b_out) % 16 == 0, MB_ERR_ALIGN,
+             "scale_gradients: arrays must be 16-byte aligned");
+  MB_REQUIRE(dtype == MB_F32 || dtype == MB_F16 || dtype == MB_BF16, MB_ERR_DTYPE,
+             "scale_gradients: unsupported dtype code %d", dtype);
+  if (a_n + b_n == 0) return MB_OK;
+  const int64_t most = std::max(a_n, b_n) / 8 / 256 + 1;
+  const unsigned grid = (unsigned)std::min<int64_t>(most, multiprocessors() * 8);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    scale_out_kernel<T><<<grid, 256, 0, (cudaStream_t)stream>>>((const T*)a, (T*)a_out, a_n, (const T*)b, (T*)b_out, b_n,
+                                                               scale);
+    return check_launch("scale_gradients");
+  };
+  return dtype == MB_F32 ? go(0.f) : dtype == MB_BF16 ? go(__nv_bfloat16{}) : go(__half{});
 }

@@ -12,7 +12,12 @@ Tolerances.  With u the half step of the tensors' type (`eps / 2`) and e = 2^-24
            (in fp16 also its smallest step, 2^-24 / 2^15; in fp32 three parts: 4 e instead of u)
   dx, dW   the errors of G times the other operand, summed as magnitudes; 2 e (terms / 16 + 8) of the sum of
            magnitudes for the summation; u of the result for the last rounding
+  in one pass (mean and sum, bf16 and fp32): what is rounded is exp(s - s_t), relative to which G's error is the
+           same; dW's other operand is x / sum rounded to the type (u of |G| |x|); and the result is rounded once
+           more when it is multiplied with the gradient that arrives (u)
 """
+
+import threading
 
 import pytest
 import torch
@@ -89,6 +94,9 @@ def reference(x, w, label, reduction, up, ignore=-100):
     dw = G.t() @ xl
     bdw = dG.t() @ xl.abs() + 2 * E * (N / 16 + 8) * (G.abs().t() @ xl.abs())
     tiny = TINY[dtype]
+    if reduction != 'none' and dtype != torch.float16:  # in one pass
+        bdw = bdw + (u + 4 * E) * (G.abs().t() @ xl.abs())
+        u = 2 * u
     return (loss, dx, dw), (bound, bdx + (u + 4 * E) * dx.abs() + tiny, bdw + (u + 4 * E) * dw.abs() + tiny)
 
 
@@ -118,7 +126,7 @@ def check(x, w, label, reduction, up=None, ignore=-100):
     for name, a, b, c in zip(('loss', 'dx', 'dw'), got, want, bound):
         near(name, a, b, c)
     with torch.no_grad():
-        assert torch.equal(ops.linear_cross_entropy(x, w, label, ignore, reduction), got[0])
+        near('loss alone', ops.linear_cross_entropy(x, w, label, ignore, reduction), want[0], bound[0])
     return got
 
 
@@ -323,7 +331,7 @@ def test_a_large_vocabulary_and_what_it_takes():
     base = torch.cuda.memory_allocated()
     run(x, w, label, 'mean', upstream(4100, 'mean'))
     peak = torch.cuda.max_memory_allocated() - base
-    assert peak < 0.45e9 < 4100 * 131072 * 2, peak
+    assert peak < 0.75e9 < 4100 * 131072 * 2, peak
 
 
 def test_refusals():
@@ -340,11 +348,69 @@ def test_refusals():
     with pytest.raises(NotImplementedError, match='second derivatives'):
         torch.autograd.grad(ops.linear_cross_entropy(xl, w, label), xl, create_graph=True)
     wl = w.clone().requires_grad_()
-    loss = ops.linear_cross_entropy(x, wl, label)
+    loss, each = ops.linear_cross_entropy(x, wl, label), ops.linear_cross_entropy(x, wl, label, reduction='none')
+    want = torch.autograd.grad(ops.linear_cross_entropy(x, wl, label), wl)[0]
     with torch.no_grad():
         wl.mul_(2)
+    assert torch.equal(torch.autograd.grad(loss, wl)[0], want)  # computed with the loss
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
-        loss.backward()
+        each.sum().backward()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_far_logits_in_some_runs_of_rows(dtype):
+    """Labels whose logits are more than 66 below the largest one: their run of rows is computed again, with
+    the others' results as they are.  (Runs are of 2^28 / 33024 words = 7936 rows, fp32 2560; no token is
+    ignored, so that the far rows are the second's, the fourth's.)"""
+    x, w, label = inputs(9000, 64, 33000, dtype, 12)
+    alone = run(x, w, label, 'mean', upstream(9000, 'mean'))
+    x[8500:8600] = (x[8500:8600].float() * 40).to(dtype)
+    far = x[8500:8600].double() @ w.double().t()
+    assert (far.amax(1) - far[torch.arange(100), label[8500:8600].clamp_min(0)]).max() > 100
+    got = check(x, w, label, 'mean')
+    assert torch.equal(got[1][:7680], alone[1][:7680])  # whole runs before them in both types
+
+
+def test_gradients_are_used_twice():
+    x, w, label = (t.clone() for t in inputs(300, 64, 500, torch.bfloat16, 4))
+    x.requires_grad_(), w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, label)
+    one = torch.autograd.grad(loss, (x, w), retain_graph=True)
+    for t in one:
+        t.zero_()  # what a caller does with its gradients changes nothing
+    two = torch.autograd.grad(loss, (x, w), torch.tensor(2.0, device='cuda'))
+    want = run(x, w, label, 'mean', torch.tensor(2.0, device='cuda'))
+    assert torch.equal(two[0], want[1]) and torch.equal(two[1], want[2])
+
+
+def test_first_call_of_a_host_thread():
+    """A thread without a CUDA context of its own (an autograd thread's first call): the tensor maps are made all
+    the same."""
+    x, w, label = inputs(70, 64, 300, torch.bfloat16, 3)
+    want = run(x, w, label, 'none', upstream(70, 'none'))
+    sizes = _lib.i64_array((0, 0, 0))
+    _lib.call('motif_b200_linear_cross_entropy_bytes', w.data_ptr(), 64, 70, 300, 64, _lib.MB_BF16, sizes)
+    state, work = (torch.empty(n, dtype=torch.uint8, device='cuda') for n in (sizes[0], sizes[1]))
+    loss, st = torch.empty(70, device='cuda'), torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    errors = []
+
+    def call():
+        try:
+            _lib.call('motif_b200_linear_cross_entropy', x.data_ptr(), 64, w.data_ptr(), 64, label.data_ptr(), -100, 0,
+                      loss.data_ptr(), 70, 300, 64, state.data_ptr(), sizes[0], work.data_ptr(), sizes[1], _lib.MB_BF16, st)
+            _lib.call('motif_b200_gemm', x.data_ptr(), 64, w.data_ptr(), 64, out.data_ptr(), 304, 70, 300, 64, _lib.MB_BF16,
+                      st)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    out = torch.empty(70, 304, dtype=torch.bfloat16, device='cuda')
+    t = threading.Thread(target=call)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert torch.equal(loss, want[0])
 
 
 def test_entry_points_refuse_short_buffers():
@@ -357,6 +423,15 @@ def test_entry_points_refuse_short_buffers():
     with pytest.raises(ValueError, match='256-byte aligned'):
         _lib.call('motif_b200_linear_cross_entropy', x.data_ptr(), 64, w.data_ptr(), 64, label.data_ptr(), -100, 1, *common,
                   buf.data_ptr() + 16, 1 << 19, buf.data_ptr(), buf.numel(), _lib.MB_BF16, None)
+    with pytest.raises(ValueError, match='bytes of workspace needed'):
+        _lib.call('motif_b200_linear_cross_entropy_train', x.data_ptr(), 64, w.data_ptr(), 64, label.data_ptr(), -100, 1,
+                  loss.data_ptr(), None, None, 10, 100, 64, buf.data_ptr(), buf.numel(), _lib.MB_BF16, None)
+    with pytest.raises(NotImplementedError, match='fp16'):
+        _lib.call('motif_b200_linear_cross_entropy_train', x.data_ptr(), 64, w.data_ptr(), 64, label.data_ptr(), -100, 1,
+                  loss.data_ptr(), None, None, 10, 100, 64, buf.data_ptr(), buf.numel(), _lib.MB_F16, None)
+    with pytest.raises(ValueError, match='reduction must be 1 or 2'):
+        _lib.call('motif_b200_linear_cross_entropy_train', x.data_ptr(), 64, w.data_ptr(), 64, label.data_ptr(), -100, 0,
+                  loss.data_ptr(), None, None, 10, 100, 64, buf.data_ptr(), buf.numel(), _lib.MB_BF16, None)
     with pytest.raises(ValueError, match='unknown reduction'):
         _lib.call('motif_b200_linear_cross_entropy_backward', w.data_ptr(), 64, loss.data_ptr(), 0, 3, None, None, 10, 100, 64,
                   buf.data_ptr(), buf.numel(), buf.data_ptr(), buf.numel(), _lib.MB_BF16, None)
