@@ -218,7 +218,8 @@ MB_API int motif_b200_linear_cross_entropy_train(const void* x, int64_t xs, cons
                                           void* dx, void* dw, int64_t N, int64_t V, int64_t d, void* workspace,
                                           int64_t workspace_bytes, int dtype, void* stream);
 
-/* a_out = a * scale[0], b_out = b * scale[0] (device memory; a_n and b_n elements of `dtype` at 16-byte boundaries). */
+/* a_out = a * scale[0], b_out = b * scale[0] (device memory; a_n and b_n elements of `dtype` at 16-byte boundaries; an
+ * output may be its input, and then is not touched where scale[0] is 1). */
 MB_API int motif_b200_scale_gradients(const void* a, void* a_out, int64_t a_n, const void* b, void* b_out, int64_t b_n,
                                const float* scale, int dtype, void* stream);
 

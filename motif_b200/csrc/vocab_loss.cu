@@ -43,7 +43,7 @@ constexpr int kStage = 2 * kOperand;
 constexpr int kStages = 6;
 constexpr int kEnders = 8;               // warps of the tile's end: two for each quarter of the TMEM lanes
 constexpr int kThreads = 64 + 32 * kEnders;  // a copying warp, an issuing warp, and those
-constexpr int kEnd = kEnders * 4096;     // two 2 KB buffers for each
+constexpr int kEnd = kEnders * 4096;     // a buffer for each
 constexpr int kSmem = kStages * kStage + kEnd + 256 + 1024;
 constexpr uint32_t kWait = 1u << 22;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -479,10 +479,14 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank2();
   const bool leader = rank == 0;
+  if (MODE == kAgain && a.flag) {
+    allow_dependent_launch();
+    wait_for_previous();
+    if (*a.flag == 0) return;  // both CTAs of a pair read the same
+  }
   const uint32_t tmem = pair_begin(s);
   const int np = gridDim.x >> 1, pair = blockIdx.x >> 1;
-  int live = min(max(*a.count - a.row0, 0), a.rows);
-  if (MODE == kAgain && a.flag && *a.flag == 0) live = 0;
+  const int live = min(max(*a.count - a.row0, 0), a.rows);
   const int mt = (live + kTile - 1) / kTile, nt = (a.nv + kTile - 1) / kTile;
   const int64_t tiles = (int64_t)mt * nt;
   const int64_t walkers = min((int64_t)np, tiles);
@@ -531,40 +535,45 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
     const int q = warp & 3, half = (warp - 2) >> 2;  // the TMEM lanes that this warp can read; its columns
     const int in_tile = (int)rank * 128 + q * 32 + lane, c0 = half * (kTile / 2);
     unsigned char* buf = s.end + (warp - 2) * 4096;
-    int slot = 0, done = 0, m_now = -1, label = -1;
+    int done = 0, m_now = -1, label = -1;
     bool lost = false, mine = false;
     float top = 0.f, sum = 0.f;  // kLoss, kOnce: of the run so far; kAgain: the row's largest logit
     float inv = 0.f, g = 0.f;    // kAgain
-    // 32 columns from column c of the tile: `at` is the label's, `valid` columns are words
-    auto chunk = [&](uint32_t (&r)[32], int c, int at, int valid, int row, int x, int y) {
-      float z[32];
+    // 64 columns from column c of the tile: `at` is the label's, `valid` columns are words.  64 at a time, so that
+    // each of the few warps has enough independent work (32 at a time took twice as long a tile).
+    auto block = [&](uint32_t (&r0)[32], uint32_t (&r1)[32], int c, int at, int valid, int row, int x, int y) {
+      float z[64];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(r[i]);
-      if (MODE != kAgain && valid < c + 32) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (c + i >= valid) z[i] = -INFINITY;
+      for (int i = 0; i < 32; ++i) {
+        z[i] = __uint_as_float(r0[i]);
+        z[32 + i] = __uint_as_float(r1[i]);
       }
-      if (MODE != kAgain && __any_sync(0xffffffffu, (unsigned)(at - c) < 32u)) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (at == c + i) {
-            if (MODE == kLoss)
-              a.target[row] = z[i];
-            else
-              z[i] = -INFINITY;  // its part is known
-          }
-      }
+      const bool here = __any_sync(0xffffffffu, (unsigned)(at - c) < 64u);
       if constexpr (MODE != kAgain) {
-        float t4[4];
+        if (valid < c + 64) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          t4[j] = fmax3(z[8 * j], z[8 * j + 1], z[8 * j + 2]);
-          t4[j] = fmax3(t4[j], z[8 * j + 3], z[8 * j + 4]);
-          t4[j] = fmax3(t4[j], z[8 * j + 5], z[8 * j + 6]);
-          t4[j] = fmaxf(t4[j], z[8 * j + 7]);
+          for (int i = 0; i < 64; ++i)
+            if (c + i >= valid) z[i] = -INFINITY;
         }
-        const float now = fmaxf(fmax3(t4[0], t4[1], t4[2]), t4[3]);
+        if (here) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (at == c + i) {
+              if (MODE == kLoss)
+                a.target[row] = z[i];
+              else
+                z[i] = -INFINITY;  // its part is known
+            }
+        }
+        float t8[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          t8[j] = fmax3(z[8 * j], z[8 * j + 1], z[8 * j + 2]);
+          t8[j] = fmax3(t8[j], z[8 * j + 3], z[8 * j + 4]);
+          t8[j] = fmax3(t8[j], z[8 * j + 5], z[8 * j + 6]);
+          t8[j] = fmaxf(t8[j], z[8 * j + 7]);
+        }
+        const float now = fmax3(fmax3(t8[0], t8[1], t8[2]), fmax3(t8[3], t8[4], t8[5]), fmaxf(t8[6], t8[7]));
         const bool raise = MODE == kLoss ? now > top : mine && now > top + kFar;  // (rows behind the last hold anything)
         if (__any_sync(0xffffffffu, raise) && raise) {
           sum *= ex2f_((top - now) * kLog2e);  // 0 from a reference of -inf
@@ -576,41 +585,38 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       const float ref = MODE == kLoss && top == -INFINITY ? 0.f : top;
       const float2 c2 = make_float2(kLog2e, kLog2e), n2 = make_float2(-ref, -ref);
       const float2 m2 = make_float2(-ref * kLog2e, -ref * kLog2e), i2 = make_float2(inv, inv);
-      float2 acc0 = make_float2(0.f, 0.f), acc1 = acc0;
+      float2 acc[4] = {};
 #pragma unroll
-      for (int i = 0; i < 32; i += 2) {
+      for (int i = 0; i < 64; i += 2) {
         const float2 v = make_float2(z[i], z[i + 1]);
         const float2 e = P == 1 ? ffma2(v, c2, m2) : fmul2(fadd2(v, n2), c2);
         float2 w = make_float2(ex2f_(e.x), ex2f_(e.y));
-        if constexpr (MODE == kAgain) {
+        if constexpr (MODE == kAgain)
           w = fmul2(w, i2);
-        } else if (i & 2) {
-          acc1 = fadd2(acc1, w);
-        } else {
-          acc0 = fadd2(acc0, w);
-        }
+        else
+          acc[i / 2 % 4] = fadd2(acc[i / 2 % 4], w);
         z[i] = w.x;
         z[i + 1] = w.y;
       }
       if constexpr (MODE != kAgain) {
-        acc0 = fadd2(acc0, acc1);
-        sum += acc0.x + acc0.y;
-      } else if (__any_sync(0xffffffffu, (unsigned)(at - c) < 32u)) {
+        const float2 all = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
+        sum += all.x + all.y;
+      } else if (here) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < 64; ++i)
           if (at == c + i) z[i] -= g;
       }
       if constexpr (MODE != kLoss) {
-        if (!mine || valid < c + 32) {
+        if (!mine || valid < c + 64) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int i = 0; i < 64; ++i)
             if (!mine || c + i >= valid) z[i] = 0.f;
         }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          uint32_t w[16];
+          uint32_t w[32];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 32; ++i) {
             w[i] = pack2<O>(z[2 * i], z[2 * i + 1]);
             if (p + 1 < P) {
               const float2 back = round2<O>(z[2 * i], z[2 * i + 1]);
@@ -618,24 +624,22 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
               z[2 * i + 1] -= back.y;
             }
           }
-          // two buffers of 32 rows x 64 bytes in turn, in the 64-byte swizzle of the tensor map
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
+          // 32 rows x 128 bytes in the 128-byte swizzle of the tensor map, once the block before has left
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
           __syncwarp();
-          unsigned char* b = buf + slot * 2048;
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            *reinterpret_cast<uint4*>(b + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) =
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) =
                 make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
             asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
                              reinterpret_cast<uint64_t>(&tmG)),
-                         "r"(x + c), "r"((int)(p * a.g_part) + y), "r"(smem_u32(b))
+                         "r"(x + c), "r"((int)(p * a.g_part) + y), "r"(smem_u32(buf))
                          : "memory");
             asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
           }
-          slot ^= 1;
         }
       }
     };
@@ -666,20 +670,16 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       const uint32_t taddr = tmem + (uint32_t)((done & 1) * kTile) + ((uint32_t)(q * 32) << 16);
       const int x = n * kTile, y = m * kTile + (int)rank * 128 + q * 32;
       tile_ready(s, done, lost);
-      uint32_t ra[32], rb[32];  // a chunk is on its way while the one before is computed
-      read32(taddr + c0, lost, ra);
-      read32_wait(lost, ra);
-      read32(taddr + c0 + 32, lost, rb);
-      chunk(ra, c0, at, valid, row, x, y);
-      read32_wait(lost, rb);
-      read32(taddr + c0 + 64, lost, ra);
-      chunk(rb, c0 + 32, at, valid, row, x, y);
-      read32_wait(lost, ra);
-      read32(taddr + c0 + 96, lost, rb);
-      chunk(ra, c0 + 64, at, valid, row, x, y);
-      read32_wait(lost, rb);
-      tile_read(s, done, lost, leader);  // the tile is in registers: the next one may come
-      chunk(rb, c0 + 96, at, valid, row, x, y);
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        uint32_t r0[32], r1[32];
+        read32(taddr + c0 + 64 * h, lost, r0);
+        read32(taddr + c0 + 64 * h + 32, lost, r1);
+        read32_wait(lost, r0);
+        read32_wait(lost, r1);
+        if (h == 1) tile_read(s, done, lost, leader);  // the tile is in registers: the next one may come
+        block(r0, r1, c0 + 64 * h, at, valid, row, x, y);
+      }
     }
     if constexpr (MODE != kLoss) {
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
@@ -892,10 +892,10 @@ __global__ void __launch_bounds__(32 * kSettleRows) settle_kernel(const SettleAr
   add_losses<kSettleRows>(sums, cta, ctas, a.partial, a.ticket, a.mean, all, a.loss);
 }
 
-// dst = src * *scale, for up to two arrays: the gradients of a loss that another one follows.
+// dst = src * *scale, for up to two arrays: the gradients of a loss that another one follows.  In place there is nothing
+// to do where that is 1.
 template <typename T>
-__global__ void __launch_bounds__(256) scale_out_kernel(const T* __restrict__ a, T* __restrict__ ao, int64_t na,
-                                                        const T* __restrict__ b, T* __restrict__ bo, int64_t nb,
+__global__ void __launch_bounds__(256) scale_out_kernel(const T* a, T* ao, int64_t na, const T* b, T* bo, int64_t nb,
                                                         const float* __restrict__ scale) {
   const float s = *scale;
   const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -905,6 +905,7 @@ __global__ void __launch_bounds__(256) scale_out_kernel(const T* __restrict__ a,
     const T* src = which ? b : a;
     T* dst = which ? bo : ao;
     const int64_t n = which ? nb : na, vecs = n / E;
+    if (src == dst && s == 1.0f) continue;
 #pragma unroll 4
     for (int64_t i = first; i < vecs; i += step) {
       const uint4 u = reinterpret_cast<const uint4*>(src)[i];
@@ -943,14 +944,17 @@ __global__ void __launch_bounds__(1024) scale_kernel(const float* __restrict__ u
 }
 
 // ------------------------------------------------------------------------------- products
+constexpr int kMostWaves = 3;
+
 struct ProductArgs {
   const int* count;
   int by_rows;              // 1: dx (tile rows are tokens, the sum runs over words); 0: dW (the other way)
   int row0, rows;           // the packed rows of this call
   int v0, nv;               // its vocabulary
   int d;
+  int steps;                // products of parts a stage of the sum takes
   int64_t a_part, b_part;   // rows from one part of an operand to the next
-  float4* slots;            // [2 pairs][256 / 4][256]: tiles whose sum is split
+  float4* slots;            // [kMostWaves pairs][256 / 4][256]: tiles whose sum is split
   float* acc;               // [rows or nv][ld] fp32, or null
   int64_t ld;
   int first, last;          // first: acc holds nothing yet; last: the result leaves as T
@@ -974,21 +978,27 @@ __device__ __forceinline__ float last_scale(const ProductArgs& a) {
   return (a.up ? *a.up : 1.0f) * (a.mean ? 1.0f / (float)*a.count : 1.0f) * fold;
 }
 struct Cut {  // how a product's tiles are spread over the pairs
-  int mt, nt, kb, full, split, units;
+  int mt, nt, width, kb, full, split, units;  // width: columns of a tile
 };
-// Whole waves of tiles keep their sum in one pair; of the rest each tile's sum is cut into equal parts.
+// Columns are cut evenly, in steps of 32.  Whole waves of tiles keep their sum in one pair; of the rest each
+// tile's sum is cut into equal parts: one wave of them, or, where the sums are long, two or three waves if that ends
+// more than a tenth sooner (48 tiles on 74 pairs: three parts each, two waves of a third).
 __host__ __device__ __forceinline__ Cut cut_product(const ProductArgs& a, int live, int np) {
   Cut c;
   const int m = a.by_rows ? live : a.nv, k = a.by_rows ? (live > 0 ? a.nv : 0) : live;
   c.mt = (m + kTile - 1) / kTile;
   c.nt = (a.d + kTile - 1) / kTile;
+  c.width = ((a.d + c.nt - 1) / c.nt + 31) & ~31;
   c.kb = (k + kBK - 1) / kBK;
   const int tiles = c.mt * c.nt, rem = tiles % np;
   c.full = tiles - rem;
-  // one wave of parts, or two where that ends more than a tenth sooner (48 tiles on 74 pairs: 3 parts each)
   c.split = rem > 0 ? np / rem : 1;
-  const int two = rem > 0 ? 2 * np / rem : 1;
-  if (c.split * 18 < two * 10) c.split = two;
+  if (rem > 0 && c.kb * a.steps >= 128)
+    for (int waves = 2, best = 1; waves <= kMostWaves; ++waves)
+      if (waves * np / rem * 9 * best > c.split * 10 * waves) {
+        c.split = waves * np / rem;
+        best = waves;
+      }
   c.split = min(c.split, c.kb);
   if (c.split <= 1) {
     c.split = 1;
@@ -1025,9 +1035,9 @@ __device__ __forceinline__ int64_t row_out(const ProductArgs& a, int row) {
 // stays in fp32 or leaves as T.  It goes out by way of shared memory, so that a store instruction writes whole
 // 64-byte (fp32: 128-byte) runs of rows instead of 16 bytes of each.
 template <typename T>
-__device__ __forceinline__ void finish32(const ProductArgs& a, int row, int rows, int col, float (&v)[32], float scale,
-                                         unsigned char* buf) {
-  const int n = min(32, a.d - col), lane = threadIdx.x & 31;
+__device__ __forceinline__ void finish32(const ProductArgs& a, int row, int rows, int col, int end, float (&v)[32],
+                                         float scale, unsigned char* buf) {
+  const int n = min(32, end - col), lane = threadIdx.x & 31;
   if (!a.first && row < rows) {
     const float* p = a.acc + (int64_t)row * a.ld + col;
 #pragma unroll
@@ -1117,8 +1127,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       bool failed = false;
       for (int u = pair; u < c.units && !failed; u += np) {
         const Unit w = unit_at(c, u);
-        const int cols = (min(kTile, a.d - w.n * kTile) + 31) & ~31;
-        const int ar = w.m * kTile + 128 * (int)rank, bc = w.n * kTile + (int)rank * (cols / 2);
+        const int cols = (min(c.width, a.d - w.n * c.width) + 31) & ~31;
+        const int ar = w.m * kTile + 128 * (int)rank, bc = w.n * c.width + (int)rank * (cols / 2);
         const int rows = A_MN ? kTile : live - w.m * kTile, boxes = boxes_of(rows, rank);
         const uint32_t bytes = 4096 * (boxes_of(rows, 0) + boxes_of(rows, 1)) + 2 * kOperand;
         // the right operand's rows: words of this piece, or this call's tokens
@@ -1151,7 +1161,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       bool failed = false;
       for (int u = pair; u < c.units && c.kb > 0 && !failed; u += np, ++done) {
         const Unit w = unit_at(c, u);
-        const int cols = (min(kTile, a.d - w.n * kTile) + 31) & ~31;
+        const int cols = (min(c.width, a.d - w.n * c.width) + 31) & ~31;
         const uint32_t idesc =
             umma_idesc_f16(std::is_same<O, __nv_bfloat16>::value ? 1u : 0u, kTile, cols, A_MN ? 1u : 0u, 1u);
         failed = !tile_free(s, done) ||
@@ -1179,7 +1189,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const Unit w = unit_at(c, u);
       const int row = w.m * kTile + in_tile, rows = a.by_rows ? live : a.nv;
       const uint32_t taddr = tmem + (uint32_t)((done & 1) * kTile) + ((uint32_t)(q * 32) << 16);
-      const int cols = min(kTile, a.d - w.n * kTile);
+      const int cols = min(c.width, a.d - w.n * c.width);
       if (c.kb > 0) tile_ready(s, done, lost);
 #pragma unroll 1
       for (int col = half * 32; col < cols; col += 64) {
@@ -1200,7 +1210,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           for (int i = 0; i < 8; ++i) p[i * kTile] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         } else {
           const float own = a.last && a.row_scale && row < rows ? scale * a.row_scale[row] : scale;
-          finish32<T>(a, row, rows, w.n * kTile + col, v, own, buf);
+          finish32<T>(a, row, rows, w.n * c.width + col, w.n * c.width + cols, v, own, buf);
         }
       }
       if (c.kb > 0) tile_read(s, done, lost, leader);
@@ -1223,7 +1233,8 @@ __global__ void __launch_bounds__(256) join_product_kernel(const ProductArgs a, 
   const int m = tile / c.nt, n = tile - m * c.nt, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r0 = (blockIdx.x >> 3 & 7) * 32, c0 = (blockIdx.x & 7) * 32;
   const int rows = a.by_rows ? live : a.nv;
-  if (m * kTile + r0 >= rows || n * kTile + c0 >= a.d) return;
+  const int end = min(a.d, (n + 1) * c.width);
+  if (m * kTile + r0 >= rows || n * c.width + c0 >= end) return;
   const float4* src = a.slots + ((int64_t)j * c.split * (kTile / 4) + c0 / 4 + warp) * kTile + r0 + lane;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
@@ -1236,8 +1247,8 @@ __global__ void __launch_bounds__(256) join_product_kernel(const ProductArgs a, 
   }
   turn[lane][warp] = v;
   __syncthreads();
-  const int row = m * kTile + r0 + (threadIdx.x >> 3), col = n * kTile + c0 + 4 * (threadIdx.x & 7);
-  if (row >= rows || col >= a.d) return;
+  const int row = m * kTile + r0 + (threadIdx.x >> 3), col = n * c.width + c0 + 4 * (threadIdx.x & 7);
+  if (row >= rows || col >= end) return;
   v = turn[threadIdx.x >> 3][threadIdx.x & 7];
   float4* acc = reinterpret_cast<float4*>(a.acc + (int64_t)row * a.ld + col);  // rows are padded to fours
   if (!a.first) {
@@ -1262,7 +1273,7 @@ __global__ void __launch_bounds__(256) join_product_kernel(const ProductArgs a, 
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (col + i < a.d) p[i] = from_f<T>(e[i]);
+      if (col + i < end) p[i] = from_f<T>(e[i]);
   }
 }
 
@@ -1322,7 +1333,7 @@ Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) 
   }
   if (s.parts == 1) s.run = std::min(s.rows, std::max(s.run, most / s.piece / kTile * kTile));
   s.g = take(s.backward_bytes, s.parts * s.run * s.piece * 2);
-  s.slots = take(s.backward_bytes, 2LL * np * kTile * kTile * 4);
+  s.slots = take(s.backward_bytes, (int64_t)kMostWaves * np * kTile * kTile * 4);
   s.dx_acc = take(s.backward_bytes, s.piece < s.vrows ? s.run * up_to(d, 4) * 4 : 0);
   s.dw_acc = take(s.backward_bytes, s.run < s.rows ? V * up_to(d, 4) * 4 : 0);
   s.scale = take(s.backward_bytes, 8);
@@ -1377,7 +1388,7 @@ OnceSizes once_sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype,
   s.partial = take(s.rows / kSettleRows * 8);
   s.e = take(s.parts * s.run * s.vrows * 2);
   s.weighed = take(s.parts * s.run * s.dp * 2);
-  s.slots = take(2LL * np * kTile * kTile * 4);
+  s.slots = take((int64_t)kMostWaves * np * kTile * kTile * 4);
   s.dx_acc = take(s.piece < s.vrows ? s.run * up_to(d, 4) * 4 : 0);
   s.dw_acc = take(s.runs > 1 ? V * up_to(d, 4) * 4 : 0);
   return s;
@@ -1528,7 +1539,7 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
   if (!rc) rc = encode_tile_map_2d(&tmX32, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, kBK, 32, 128);
   if (!rc) rc = encode_tile_map_2d(&tmXk, c.state + s.x, 2, s.dp, s.parts * s.rows, s.dp * 2, 64, kBK, 128);
   if (!rc) rc = encode_tile_map_2d(&tmWk, wb, 2, wc, wr, wst * 2, 64, kBK, 128);
-  if (!rc) rc = encode_tile_map_2d(&tmG, g, 2, s.piece, s.parts * s.run, s.piece * 2, 32, 32, 64);    // stored
+  if (!rc) rc = encode_tile_map_2d(&tmG, g, 2, s.piece, s.parts * s.run, s.piece * 2, 64, 32, 128);   // stored
   if (!rc) rc = encode_tile_map_2d(&tmGa, g, 2, s.piece, s.parts * s.run, s.piece * 2, kBK, 128, 128);  // tokens x words
   if (!rc) rc = encode_tile_map_2d(&tmGa32, g, 2, s.piece, s.parts * s.run, s.piece * 2, kBK, 32, 128);
   if (!rc) rc = encode_tile_map_2d(&tmGt, g, 2, s.piece, s.parts * s.run, s.piece * 2, 64, kBK, 128);   // words x tokens
@@ -1555,6 +1566,7 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
                         tmW, tmG, a);
       if (rc) return rc;
       ProductArgs p = {};
+      p.steps = Parts<kParts<T>>::n;
       p.count = count;
       p.row0 = a.row0;
       p.rows = a.rows;
@@ -1633,7 +1645,7 @@ int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
   if (!rc) rc = encode_tile_map_2d(&tmW, wb, 2, wc, wr, wst * 2, kBK, 128, 128);
   if (!rc) rc = encode_tile_map_2d(&tmWk, wb, 2, wc, wr, wst * 2, 64, kBK, 128);
   if (!rc) rc = encode_tile_map_2d(&tmXk, ws + s.weighed, 2, s.dp, s.parts * s.run, s.dp * 2, 64, kBK, 128);
-  if (!rc) rc = encode_tile_map_2d(&tmE, e, 2, s.vrows, s.parts * s.run, s.vrows * 2, 32, 32, 64);       // stored
+  if (!rc) rc = encode_tile_map_2d(&tmE, e, 2, s.vrows, s.parts * s.run, s.vrows * 2, 64, 32, 128);      // stored
   if (!rc) rc = encode_tile_map_2d(&tmEa, e, 2, s.vrows, s.parts * s.run, s.vrows * 2, kBK, 128, 128);   // tokens x words
   if (!rc) rc = encode_tile_map_2d(&tmEa32, e, 2, s.vrows, s.parts * s.run, s.vrows * 2, kBK, 32, 128);
   if (!rc) rc = encode_tile_map_2d(&tmEt, e, 2, s.vrows, s.parts * s.run, s.vrows * 2, 64, kBK, 128);    // words x tokens
@@ -1684,6 +1696,7 @@ int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
       rc = launch_pairs("linear_cross_entropy_train (again)", scores_kernel<T, kAgain>, c.np, c.st, tmX, tmX32, tmW, tmE, a);
     if (rc) return rc;
     ProductArgs q = {};
+    q.steps = Parts<kParts<T>>::n;
     q.count = p.count;
     q.row0 = a.row0;
     q.rows = a.rows;
