@@ -447,8 +447,8 @@ struct ScoreArgs {
   int64_t x_part, w_part;   // rows from one part of an operand to the next
   const int* label;         // [rows of the packed operand]
   float2* seg;              // kLoss, kOnce: (reference, sum) of each row of half a pair's run through a row tile
-  float* target;            // kLoss: the label's logit
-  const float* ref;         // kOnce: the label's logit
+  float* target;            // kLoss, kOnce: the label's logit
+  const float* ref;         // kOnce: the label's logit, known before (to a rounding or two)
   int* flag;                // kOnce: set where a logit is far above it; kAgain: works only if set (null: always)
   const RowStat* stat;      // kAgain
   const int* index;         // kAgain: packed row -> token
@@ -559,10 +559,8 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             if (at == c + i) {
-              if (MODE == kLoss)
-                a.target[row] = z[i];
-              else
-                z[i] = -INFINITY;  // its part is known
+              a.target[row] = z[i];
+              if (MODE == kOnce) z[i] = -INFINITY;  // its part is added when the row is settled
             }
         }
         float t8[8];
@@ -786,13 +784,17 @@ __global__ void __launch_bounds__(8 * kJoinRows) join_kernel(const JoinArgs a) {
 }
 
 // kOnce's rows: their loss, and what turns exponentials into gradients.  G L = E - L [v = t] with L the whole
-// sum, so the label's place gets 1 - L = -(the sum of the others), which loses nothing however near to 1 its
-// probability is; dx's rows are divided by L at the end, and dW sums E times x / L.  A warp a row.
+// sum, so the label's place gets -(the sum of the others), which loses nothing however near to 1 its
+// probability is; dx's rows are divided by L at the end, and dW sums E times x / L.  The label's part of L comes
+// from the tiles, like the others' (the tensor cores cut sums off, which moves large logits by 4e-7 of
+// themselves; between logits of one size it cancels).  In bf16 the divisor also takes back the rounding of the
+// label's place, the largest part of G: without that, the error of dx was 1.4 times as large.  A warp a row.
 struct SettleArgs {
   const int* count;
   int* ticket;
   const float2* seg;
   const float* ref;
+  const float* target;
   const int* label;
   RowStat* stat;
   const int* flag;       // the run's exponentials are G (kAgain computes them next): nothing is left to divide
@@ -846,10 +848,13 @@ __global__ void __launch_bounds__(32 * kSettleRows) settle_kernel(const SettleAr
       top = now;
     }
     const int label = a.label[row];
-    const float nan = __int_as_float(0x7fffffff), own = ex2f_((ref - top) * kLog2e);  // 1 but for far logits
-    const float inv = label >= 0 ? 1.0f / (sum + own) : nan;  // a label that is no word: NaN, in the gradients too
-    loss = label < 0 ? nan : top == ref ? log1pf(sum) : (top - ref) + logf(sum + own);
-    const float scale = flagged && label >= 0 ? 1.0f : inv;
+    const float nan = __int_as_float(0x7fffffff);
+    const float target = label >= 0 ? a.target[row] : nan;  // a label that is no word: NaN, in the gradients too
+    const float own = ex2f_((target - top) * kLog2e);       // 1 to a rounding but for far logits
+    const float inv = 1.0f / (sum + own);
+    loss = own > 0.5f ? log1pf(sum / own) : (top - target) + logf(sum + own);
+    float scale = flagged && label >= 0 ? 1.0f : inv;
+    if (P == 1 && !flagged && sum > 1e-30f && sum < 1e30f) scale *= sum / to_f(from_f<O>(sum));
     if (lane == 0) {
       RowStat st;
       st.top = top;
@@ -1344,7 +1349,7 @@ Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) 
 struct OnceSizes {
   int parts;
   int64_t rows, dp, vrows, run, runs, piece;
-  int64_t x, w, label, index, place, stat, ref, row_scale, count, ticket, flags, group, seg, partial;
+  int64_t x, w, label, index, place, stat, ref, target, row_scale, count, ticket, flags, group, seg, partial;
   int64_t e, weighed, slots, dx_acc, dw_acc, bytes;
 };
 // Elements of E that are there at once: a run of rows with the whole vocabulary (fp32: three parts of a third
@@ -1379,6 +1384,7 @@ OnceSizes once_sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype,
   s.place = take(N * 4);
   s.stat = take(s.rows * (int64_t)sizeof(RowStat));
   s.ref = take(s.rows * 4);
+  s.target = take(s.rows * 4);
   s.row_scale = take(s.run * 4);
   s.count = take(4);
   s.ticket = take(4);
@@ -1662,6 +1668,7 @@ int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
     a.label = p.label;
     a.seg = at<float2>(ws, s.seg);
     a.ref = p.ref;
+    a.target = at<float>(ws, s.target);
     a.flag = p.flags + i;
     a.stat = at<RowStat>(ws, s.stat);
     a.index = p.index;
@@ -1673,6 +1680,7 @@ int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
     b.ticket = p.ticket;
     b.seg = a.seg;
     b.ref = p.ref;
+    b.target = a.target;
     b.label = p.label;
     b.stat = at<RowStat>(ws, s.stat);
     b.flag = a.flag;
