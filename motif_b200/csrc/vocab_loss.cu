@@ -172,13 +172,16 @@ __device__ __forceinline__ bool issue_tile(const Smem& s, uint32_t d, uint32_t i
   }
   return true;
 }
+// BUFS: tiles of TMEM that take turns.
+template <int BUFS>
 __device__ __forceinline__ bool tile_free(const Smem& s, int done) {
-  const bool ok = mbar_wait_bounded(&s.tempty[done & 1], (uint32_t)(((done >> 1) & 1) ^ 1), kWait);
+  const bool ok = mbar_wait_bounded(&s.tempty[done % BUFS], (uint32_t)(((done / BUFS) & 1) ^ 1), kWait);
   tc_fence_after();
   return ok;
 }
+template <int BUFS>
 __device__ __forceinline__ void tile_issued(const Smem& s, int done) {
-  const uint32_t f = smem_u32(&s.tfull[done & 1]);
+  const uint32_t f = smem_u32(&s.tfull[done % BUFS]);
   umma_commit_pair(f);
   umma_commit_pair(map_rank(f, 1));
 }
@@ -187,23 +190,25 @@ __device__ __forceinline__ void issue_end(const Smem& s, bool failed) {
   if (!mbar_wait_bounded(s.mdone, 0, kWait) || failed) atomicAdd(&g_vocab_wait_timeouts, 1u);
 }
 // A warp of the tile's end: the tile's sums are there (false: never; `lost` then stays set).
+template <int BUFS>
 __device__ __forceinline__ void tile_ready(const Smem& s, int done, bool& lost) {
   if (lost) return;
-  const bool ok = mbar_wait_bounded(&s.tfull[done & 1], (uint32_t)((done >> 1) & 1), kWait);
+  const bool ok = mbar_wait_bounded(&s.tfull[done % BUFS], (uint32_t)((done / BUFS) & 1), kWait);
   if (__any_sync(0xffffffffu, !ok)) {
     lost = true;
     if ((threadIdx.x & 31) == 0) atomicAdd(&g_vocab_wait_timeouts, 1u);
   }
   tc_fence_after();
 }
+template <int BUFS>
 __device__ __forceinline__ void tile_read(const Smem& s, int done, bool lost, bool leader) {
   tc_fence_before();
   __syncwarp();
   if ((threadIdx.x & 31) == 0 && !lost) {
     if (leader)
-      mbar_arrive(&s.tempty[done & 1]);
+      mbar_arrive(&s.tempty[done % BUFS]);
     else
-      mbar_arrive_remote(map_rank(smem_u32(&s.tempty[done & 1]), 0));
+      mbar_arrive_remote(map_rank(smem_u32(&s.tempty[done % BUFS]), 0));
   }
 }
 // 32 columns of this thread's row; NaN where the tile never came.
@@ -524,9 +529,9 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       int it = 0, done = 0;
       bool failed = false;
       for (int64_t t = t0; t < t1 && !failed; ++t, ++done) {
-        failed = !tile_free(s, done) ||
+        failed = !tile_free<2>(s, done) ||
                  !issue_tile<false, false>(s, tmem + (uint32_t)((done & 1) * kTile), idesc, Parts<P>::n * a.kblocks, it);
-        if (!failed) tile_issued(s, done);
+        if (!failed) tile_issued<2>(s, done);
       }
       issue_end(s, failed);
     }
@@ -556,12 +561,14 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
             if (c + i >= valid) z[i] = -INFINITY;
         }
         if (here) {
+          float own = 0.f;
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (at == c + i) {
-              a.target[row] = z[i];
-              if (MODE == kOnce) z[i] = -INFINITY;  // its part is added when the row is settled
-            }
+          for (int i = 0; i < 64; ++i) {
+            const bool it = at == c + i;
+            own = it ? z[i] : own;
+            if (MODE == kOnce) z[i] = it ? -INFINITY : z[i];  // its part is added when the row is settled
+          }
+          if ((unsigned)(at - c) < 64u) a.target[row] = own;
         }
         float t8[8];
 #pragma unroll
@@ -667,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       const int valid = a.nv - n * kTile;         // columns of the tile that are words
       const uint32_t taddr = tmem + (uint32_t)((done & 1) * kTile) + ((uint32_t)(q * 32) << 16);
       const int x = n * kTile, y = m * kTile + (int)rank * 128 + q * 32;
-      tile_ready(s, done, lost);
+      tile_ready<2>(s, done, lost);
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         uint32_t r0[32], r1[32];
@@ -675,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
         read32(taddr + c0 + 64 * h + 32, lost, r1);
         read32_wait(lost, r0);
         read32_wait(lost, r1);
-        if (h == 1) tile_read(s, done, lost, leader);  // the tile is in registers: the next one may come
+        if (h == 1) tile_read<2>(s, done, lost, leader);  // the tile is in registers: the next one may come
         block(r0, r1, c0 + 64 * h, at, valid, row, x, y);
       }
     }
@@ -1108,6 +1115,22 @@ __device__ __forceinline__ void finish32(const ProductArgs& a, int row, int rows
   }
 }
 
+// fp32: a sum leaves the tensor cores every 512 terms, since they cut each partial sum off at 24 bits; what has left
+// adds up in the other half of the TMEM (dx of 512 tokens, 1024 features and 32000 words: error 4.4e-6 with 3556 terms
+// at a time, 6.8e-7).
+constexpr int kFlush = 8;  // stages
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
 // A_MN: the left operand's summed dimension runs along its rows (dW); the right one's always does.
 template <typename T, bool A_MN>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ CUtensorMap tmA,
@@ -1116,6 +1139,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                                                               const ProductArgs a) {
   using O = Op<T>;
   constexpr int P = kParts<T>;
+  constexpr int kBufs = P == 1 ? 2 : 1, kTake = P == 1 ? 1 << 30 : kFlush;
   extern __shared__ unsigned char raw[];
   const Smem s = carve(raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1138,8 +1162,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const uint32_t bytes = 4096 * (boxes_of(rows, 0) + boxes_of(rows, 1)) + 2 * kOperand;
         // the right operand's rows: words of this piece, or this call's tokens
         const int br = a.by_rows ? a.v0 : a.b_row0;
+        for (int k0 = w.k0; k0 < w.k1 && !failed; k0 += kTake)
         for (int p = 0; p < Parts<P>::n && !failed; ++p)
-          for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
+          for (int kb = k0; kb < min(w.k1, k0 + kTake); ++kb, ++it) {
             uint32_t bar;
             unsigned char* st = stage_begin(s, it, leader, bytes, bar);
             if (!st) {
@@ -1164,15 +1189,17 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     if (lane == 0 && leader) {
       int it = 0, done = 0;
       bool failed = false;
-      for (int u = pair; u < c.units && c.kb > 0 && !failed; u += np, ++done) {
+      for (int u = pair; u < c.units && c.kb > 0 && !failed; u += np) {
         const Unit w = unit_at(c, u);
         const int cols = (min(c.width, a.d - w.n * c.width) + 31) & ~31;
         const uint32_t idesc =
             umma_idesc_f16(std::is_same<O, __nv_bfloat16>::value ? 1u : 0u, kTile, cols, A_MN ? 1u : 0u, 1u);
-        failed = !tile_free(s, done) ||
-                 !issue_tile<A_MN, true>(s, tmem + (uint32_t)((done & 1) * kTile), idesc,
-                                         Parts<P>::n * (w.k1 - w.k0), it);
-        if (!failed) tile_issued(s, done);
+        for (int k0 = w.k0; k0 < w.k1 && !failed; k0 += kTake, ++done) {
+          failed = !tile_free<kBufs>(s, done) ||
+                   !issue_tile<A_MN, true>(s, tmem + (uint32_t)(done % kBufs * kTile), idesc,
+                                           Parts<P>::n * min(kTake, w.k1 - k0), it);
+          if (!failed) tile_issued<kBufs>(s, done);
+        }
       }
       issue_end(s, failed);
     }
@@ -1193,9 +1220,30 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     for (int u = pair; u < c.units; u += np, ++done) {
       const Unit w = unit_at(c, u);
       const int row = w.m * kTile + in_tile, rows = a.by_rows ? live : a.nv;
-      const uint32_t taddr = tmem + (uint32_t)((done & 1) * kTile) + ((uint32_t)(q * 32) << 16);
       const int cols = min(c.width, a.d - w.n * c.width);
-      if (c.kb > 0) tile_ready(s, done, lost);
+      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+      bool more = false;  // parts of this sum have left before
+      if constexpr (P > 1)
+        for (int k0 = w.k0; k0 + kTake < w.k1; k0 += kTake, ++done) {
+          tile_ready<kBufs>(s, done, lost);
+#pragma unroll 1
+          for (int col = half * 32; col < cols; col += 64) {
+            uint32_t r[32], o[32];
+            read32(lanes + col, lost, r);
+            if (more) read32(lanes + kTile + col, lost, o);
+            read32_wait(lost, r);
+            if (more) read32_wait(lost, o);
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) + (more ? __uint_as_float(o[i]) : 0.f);
+            if (!lost) tmem_st32(lanes + kTile + col, v);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+          more = true;
+          tile_read<kBufs>(s, done, lost, leader);
+        }
+      const uint32_t taddr = lanes + (uint32_t)(done % kBufs * kTile);
+      if (c.kb > 0) tile_ready<kBufs>(s, done, lost);
 #pragma unroll 1
       for (int col = half * 32; col < cols; col += 64) {
         uint32_t r[32];
@@ -1209,6 +1257,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        if (P > 1 && more) {
+          read32(lanes + kTile + col, lost, r);
+          read32_wait(lost, r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(r[i]);
+        }
         if (w.slot >= 0) {  // [slot][four columns][row]: the warp's rows lie next to each other
           float4* p = a.slots + ((int64_t)w.slot * (kTile / 4) + col / 4) * kTile + in_tile;
 #pragma unroll
@@ -1218,7 +1272,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           finish32<T>(a, row, rows, w.n * c.width + col, w.n * c.width + cols, v, own, buf);
         }
       }
-      if (c.kb > 0) tile_read(s, done, lost, leader);
+      if (c.kb > 0) tile_read<kBufs>(s, done, lost, leader);
     }
   }
   pair_end(tmem);
@@ -1299,10 +1353,6 @@ struct Sizes {
 // Elements of G that are there at once (16-bit; fp32 keeps three parts of a third as many).
 constexpr int64_t kPiece = 1LL << 27;
 constexpr int64_t kRun = 8192;
-// fp32: sums are added in fp32 after this many terms, since the tensor cores cut each partial sum off
-// (not rounding it) at 24 bits.
-constexpr int64_t kExactRun = 4096;
-
 Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) {
   Sizes s = {};
   s.parts = dtype == MB_F32 ? 3 : 1;
@@ -1329,14 +1379,9 @@ Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) 
   s.partial = take(s.forward_bytes, s.rows / kJoinRows * 8);
   // a run of rows and a piece of the vocabulary: G of both together stays below kPiece elements
   const int64_t most = kPiece / s.parts;
-  s.run = std::min(s.rows, s.parts == 3 ? kExactRun : kRun);
+  s.run = std::min(s.rows, s.parts == 3 ? kRun / 2 : kRun);
   s.piece = std::min(s.vrows, std::max<int64_t>(kTile, most / s.run / kTile * kTile));
-  if (s.parts == 3) {
-    // dx's sums run over the words of a piece, each in as many parts as there are pairs for a tile
-    const int64_t tiles = s.run / kTile * ((d + kTile - 1) / kTile);
-    s.piece = std::min(s.piece, kExactRun * std::max<int64_t>(1, np / tiles));
-  }
-  if (s.parts == 1) s.run = std::min(s.rows, std::max(s.run, most / s.piece / kTile * kTile));
+  s.run = std::min(s.rows, std::max(s.run, most / s.piece / kTile * kTile));
   s.g = take(s.backward_bytes, s.parts * s.run * s.piece * 2);
   s.slots = take(s.backward_bytes, (int64_t)kMostWaves * np * kTile * kTile * 4);
   s.dx_acc = take(s.backward_bytes, s.piece < s.vrows ? s.run * up_to(d, 4) * 4 : 0);
@@ -1366,12 +1411,9 @@ OnceSizes once_sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype,
   s.dp = up_to(d, 8);
   s.vrows = up_to(V, kTile);
   s.run = std::min(s.rows, std::max<int64_t>(kTile, kOnceElements / s.parts / s.vrows / kTile * kTile));
-  if (s.parts == 3) s.run = std::min(s.run, kExactRun);
   s.run = std::min(s.run, kLongRun);
   s.runs = (s.rows + s.run - 1) / s.run;
-  // dx's sums run over the words of a piece; fp32: each in as many parts as there are pairs for a tile
-  const int64_t tiles = s.run / kTile * ((d + kTile - 1) / kTile);
-  s.piece = std::min(s.vrows, s.parts == 3 ? kExactRun * std::max<int64_t>(1, np / tiles) : kLongRun);
+  s.piece = std::min(s.vrows, s.parts == 1 ? kLongRun : s.vrows);  // dx's sums run over the words of a piece
   auto take = [&](int64_t bytes) {
     const int64_t at = s.bytes;
     s.bytes = up_to(s.bytes + bytes, 256);
