@@ -994,7 +994,10 @@ struct Cut {  // how a product's tiles are spread over the pairs
 };
 // Columns are cut evenly, in steps of 32.  Whole waves of tiles keep their sum in one pair; of the rest each
 // tile's sum is cut into equal parts: one wave of them, or, where the sums are long, two or three waves if that ends
-// more than a tenth sooner (48 tiles on 74 pairs: three parts each, two waves of a third).
+// more than a tenth sooner (48 tiles on 74 pairs: three parts each, two waves of a third).  (Dealing the rest's stages
+// out evenly instead, so that a pair works on two neighbouring tiles, balances better but lets the pairs read
+// different rows of W at a time: 16384 x 768 x 32000 1883 -> 1920 us, 3277 rows 442 -> 466.)  Not so where it saves less
+// than the parts' way through memory costs (6 us; a stage of a tile is 0.28 us).
 __host__ __device__ __forceinline__ Cut cut_product(const ProductArgs& a, int live, int np) {
   Cut c;
   const int m = a.by_rows ? live : a.nv, k = a.by_rows ? (live > 0 ? a.nv : 0) : live;
@@ -1012,7 +1015,7 @@ __host__ __device__ __forceinline__ Cut cut_product(const ProductArgs& a, int li
         best = waves;
       }
   c.split = min(c.split, c.kb);
-  if (c.split <= 1) {
+  if (c.split <= 1 || c.kb * a.steps * (c.split - 1) < 20 * c.split) {
     c.split = 1;
     c.full = tiles;
   }
