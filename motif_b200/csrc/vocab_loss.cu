@@ -740,36 +740,42 @@ __device__ __forceinline__ void add_losses(double* sums, int cta, int ctas, doub
   }
 }
 
-constexpr int kJoinRows = 32;  // of a CTA: eight threads a row share its runs
+constexpr int kJoinRows = 8;  // of a CTA: a warp a row
 
-__global__ void __launch_bounds__(8 * kJoinRows) join_kernel(const JoinArgs a) {
-  __shared__ double sums[kJoinRows];
-  allow_dependent_launch();
-  wait_for_previous();
-  const int live = *a.count, r = threadIdx.x >> 3, j = threadIdx.x & 7, row = blockIdx.x * kJoinRows + r;
-  const int mt = (live + kTile - 1) / kTile, ctas = max((live + kJoinRows - 1) / kJoinRows, 1);
-  if (blockIdx.x >= ctas) return;  // the first CTA is there for a call without tokens, too
-  const int m = row / kTile, in_tile = row % kTile;
-  float top = -INFINITY, sum = 0.f;
-  if (row < live) {
-    const int64_t tiles = (int64_t)mt * a.nt, walkers = min((int64_t)a.np, tiles);
-    const int s0 = 2 * ((int)range_owner((int64_t)m * a.nt, tiles, walkers) + m);
-    const int s1 = 2 * ((int)range_owner((int64_t)(m + 1) * a.nt - 1, tiles, walkers) + m) + 2;
+// (reference, sum) pairs of a row's runs s0 .. s1, joined over a warp: exponentials relative to the largest reference.
+__device__ __forceinline__ void join_runs(const float2* seg, int s0, int s1, int in_tile, float& top, float& sum) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll 4
-    for (int i = s0 + j; i < s1; i += 8) {
-      const float2 v = a.seg[(int64_t)i * kTile + in_tile];
-      const float now = fmaxf(top, v.x), ref = now == -INFINITY ? 0.f : now;
-      sum = sum * ex2f_((top - ref) * kLog2e) + v.y * ex2f_((v.x - ref) * kLog2e);
-      top = now;
-    }
+  for (int i = s0 + lane; i < s1; i += 32) {
+    const float2 v = seg[(int64_t)i * kTile + in_tile];
+    const float now = fmaxf(top, v.x), ref = now == -INFINITY ? 0.f : now;
+    sum = sum * ex2f_((top - ref) * kLog2e) + v.y * ex2f_((v.x - ref) * kLog2e);
+    top = now;
   }
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {  // the two sides of an exchange add in the same order
+  for (int o = 1; o < 32; o <<= 1) {  // the two sides of an exchange add in the same order
     const float t2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
     const float now = fmaxf(top, t2), ref = now == -INFINITY ? 0.f : now;
     const float mine = sum * ex2f_((top - ref) * kLog2e), other = s2 * ex2f_((t2 - ref) * kLog2e);
-    sum = (j & o) ? other + mine : mine + other;
+    sum = (lane & o) ? other + mine : mine + other;
     top = now;
+  }
+}
+
+__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const JoinArgs a) {
+  __shared__ double sums[kJoinRows];
+  allow_dependent_launch();
+  wait_for_previous();
+  const int live = *a.count, r = threadIdx.x >> 5, j = threadIdx.x & 31, row = blockIdx.x * kJoinRows + r;
+  const int mt = (live + kTile - 1) / kTile, ctas = max((live + kJoinRows - 1) / kJoinRows, 1);
+  if (blockIdx.x >= ctas) return;  // the first CTA is there for a call without tokens, too
+  float top = -INFINITY, sum = 0.f;
+  if (row < live) {
+    const int m = row / kTile;
+    const int64_t tiles = (int64_t)mt * a.nt, walkers = min((int64_t)a.np, tiles);
+    const int s0 = 2 * ((int)range_owner((int64_t)m * a.nt, tiles, walkers) + m);
+    const int s1 = 2 * ((int)range_owner((int64_t)(m + 1) * a.nt - 1, tiles, walkers) + m) + 2;
+    join_runs(a.seg, s0, s1, row % kTile, top, sum);
   }
   double loss = 0.0;
   if (row < live && j == 0) {
@@ -840,20 +846,7 @@ __global__ void __launch_bounds__(32 * kSettleRows) settle_kernel(const SettleAr
     const int s1 = 2 * ((int)range_owner((int64_t)(m + 1) * a.nt - 1, tiles, walkers) + m) + 2;
     const float ref = a.ref[row];
     float top = ref, sum = 0.f;
-    for (int i = s0 + lane; i < s1; i += 32) {
-      const float2 v = a.seg[(int64_t)i * kTile + in_tile];
-      const float now = fmaxf(top, v.x);
-      sum = sum * ex2f_((top - now) * kLog2e) + v.y * ex2f_((v.x - now) * kLog2e);
-      top = now;
-    }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float t2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-      const float now = fmaxf(top, t2);
-      const float mine = sum * ex2f_((top - now) * kLog2e), other = s2 * ex2f_((t2 - now) * kLog2e);
-      sum = (lane & o) ? other + mine : mine + other;
-      top = now;
-    }
+    join_runs(a.seg, s0, s1, in_tile, top, sum);
     const int label = a.label[row];
     const float nan = __int_as_float(0x7fffffff);
     const float target = label >= 0 ? a.target[row] : nan;  // a label that is no word: NaN, in the gradients too
@@ -1565,7 +1558,7 @@ int forward(const Call& c, float* loss) {
   j.nt = (int)((c.V + kTile - 1) / kTile);
   j.np = c.np;
   j.reduction = c.reduction;
-  return launch("linear_cross_entropy (join)", join_kernel, s.rows / kJoinRows, 8 * kJoinRows, c.st, 0, 1, j);
+  return launch("linear_cross_entropy (join)", join_kernel, s.rows / kJoinRows, 32 * kJoinRows, c.st, 0, 1, j);
 }
 
 template <typename T>
