@@ -540,6 +540,9 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
     const int q = warp & 3, half = (warp - 2) >> 2;  // the TMEM lanes that this warp can read; its columns
     const int in_tile = (int)rank * 128 + q * 32 + lane, c0 = half * (kTile / 2);
     unsigned char* buf = s.end + (warp - 2) * 4096;
+    // what leaves is larger than the L2 and read next by another kernel: it should not push the weight out
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(policy));
     int done = 0, m_now = -1, label = -1;
     bool lost = false, mine = false;
     float top = 0.f, sum = 0.f;  // kLoss, kOnce: of the run so far; kAgain: the row's largest logit
@@ -639,9 +642,9 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%1, %2}], [%3], %4;\n" ::"l"(
                              reinterpret_cast<uint64_t>(&tmG)),
-                         "r"(x + c), "r"((int)(p * a.g_part) + y), "r"(smem_u32(buf))
+                         "r"(x + c), "r"((int)(p * a.g_part) + y), "r"(smem_u32(buf)), "l"(policy)
                          : "memory");
             asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
           }
@@ -973,6 +976,7 @@ struct ProductArgs {
   const int* index;
   const int* place;         // dx, first call: [N], the tokens without a loss (-1) get zeros
   int64_t N;
+  struct Cut* cut;          // left here for the join: dividing again in each of its threads took most of its time
 };
 template <typename T>
 __device__ __forceinline__ float last_scale(const ProductArgs& a) {
@@ -1145,6 +1149,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   const int np = gridDim.x >> 1, pair = blockIdx.x >> 1;
   const int live = product_live(a);
   const Cut c = cut_product(a, live, np);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.cut = c;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -1277,13 +1282,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 // The tiles whose sum was split: their parts are added in order.  A CTA takes 32 rows x 32 columns of a tile: a
 // warp adds four columns of the rows, then the block of sums is turned so that rows leave in runs.
 template <typename T>
-__global__ void __launch_bounds__(256) join_product_kernel(const ProductArgs a, int np) {
+__global__ void __launch_bounds__(256) join_product_kernel(const ProductArgs a) {
   __shared__ float4 turn[32][9];
   allow_dependent_launch();
   wait_for_previous();
-  const int live = product_live(a);
-  const Cut c = cut_product(a, live, np);
-  const int j = blockIdx.x / 64, tile = c.full + j;
+  const Cut c = *a.cut;
+  const int live = product_live(a), j = blockIdx.x / 64, tile = c.full + j;
   if (tile >= c.mt * c.nt) return;
   const int m = tile / c.nt, n = tile - m * c.nt, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r0 = (blockIdx.x >> 3 & 7) * 32, c0 = (blockIdx.x & 7) * 32;
@@ -1344,7 +1348,7 @@ struct Sizes {
   // forward workspace
   int64_t group, seg, target, partial, forward_bytes;
   // backward: rows of a run, words of a piece, and the workspace
-  int64_t run, piece, g, slots, dx_acc, dw_acc, scale, backward_bytes;
+  int64_t run, piece, g, slots, dx_acc, dw_acc, scale, cut, backward_bytes;
 };
 // Elements of G that are there at once (16-bit; fp32 keeps three parts of a third as many).
 constexpr int64_t kPiece = 1LL << 27;
@@ -1383,6 +1387,7 @@ Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) 
   s.dx_acc = take(s.backward_bytes, s.piece < s.vrows ? s.run * up_to(d, 4) * 4 : 0);
   s.dw_acc = take(s.backward_bytes, s.run < s.rows ? V * up_to(d, 4) * 4 : 0);
   s.scale = take(s.backward_bytes, 8);
+  s.cut = take(s.backward_bytes, sizeof(Cut));
   return s;
 }
 
@@ -1391,7 +1396,7 @@ struct OnceSizes {
   int parts;
   int64_t rows, dp, vrows, run, runs, piece;
   int64_t x, w, label, index, place, stat, ref, target, row_scale, count, ticket, flags, group, seg, partial;
-  int64_t e, weighed, slots, dx_acc, dw_acc, bytes;
+  int64_t e, weighed, slots, dx_acc, dw_acc, cut, bytes;
 };
 // Elements of E that are there at once: a run of rows with the whole vocabulary (fp32: three parts of a third
 // as many).
@@ -1435,6 +1440,7 @@ OnceSizes once_sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype,
   s.slots = take((int64_t)kMostWaves * np * kTile * kTile * 4);
   s.dx_acc = take(s.piece < s.vrows ? s.run * up_to(d, 4) * 4 : 0);
   s.dw_acc = take(s.runs > 1 ? V * up_to(d, 4) * 4 : 0);
+  s.cut = take(sizeof(Cut));
   return s;
 }
 
@@ -1620,6 +1626,7 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
       p.a_part = s.run;
       p.slots = at<float4>(c.work, s.slots);
       p.ld = up_to(c.d, 4);
+      p.cut = at<Cut>(c.work, s.cut);
       p.scale = c.reduction == 0 ? scale : nullptr;
       p.up = up;
       p.mean = c.reduction == 1;
@@ -1639,7 +1646,7 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
         // how many tiles are split the device knows: at most all, and fewer than there are pairs
         const int64_t most = std::min<int64_t>(c.np - 1, up_to(p.rows, kTile) / kTile * ((c.d + kTile - 1) / kTile));
         if (!rc && most > 0)
-          rc = launch("linear_cross_entropy_backward (dx join)", join_product_kernel<T>, 64 * most, 256, c.st, 0, 1, p, c.np);
+          rc = launch("linear_cross_entropy_backward (dx join)", join_product_kernel<T>, 64 * most, 256, c.st, 0, 1, p);
         if (rc) return rc;
       }
       if (dw) {
@@ -1653,7 +1660,7 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
         rc = launch_pairs("linear_cross_entropy_backward (dw)", product_kernel<T, true>, c.np, c.st, tmGt, tmGt, tmXk, p);
         const int64_t rest = up_to(p.nv, kTile) / kTile * ((c.d + kTile - 1) / kTile) % c.np;
         if (!rc && rest > 0 && c.N > kBK)  // (a sum of one stage is not split)
-          rc = launch("linear_cross_entropy_backward (dw join)", join_product_kernel<T>, 64 * rest, 256, c.st, 0, 1, p, c.np);
+          rc = launch("linear_cross_entropy_backward (dw join)", join_product_kernel<T>, 64 * rest, 256, c.st, 0, 1, p);
         if (rc) return rc;
       }
     }
@@ -1750,6 +1757,7 @@ int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
     q.a_part = s.run;
     q.slots = at<float4>(ws, s.slots);
     q.ld = up_to(c.d, 4);
+    q.cut = at<Cut>(ws, s.cut);
     q.mean = c.reduction == 1;
     q.index = p.index;
     q.N = c.N;
@@ -1770,7 +1778,7 @@ int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
       // how many tiles are split the device knows: at most all, and fewer than there are pairs
       const int64_t most = std::min<int64_t>(c.np - 1, a.rows / kTile * nt);
       if (!rc && most > 0)
-        rc = launch("linear_cross_entropy_train (dx join)", join_product_kernel<T>, 64 * most, 256, c.st, 0, 1, q, c.np);
+        rc = launch("linear_cross_entropy_train (dx join)", join_product_kernel<T>, 64 * most, 256, c.st, 0, 1, q);
       if (rc) return rc;
     }
     if (dw) {
@@ -1789,7 +1797,7 @@ int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
       rc = launch_pairs("linear_cross_entropy_train (dw)", product_kernel<T, true>, c.np, c.st, tmEt, tmEt, tmXk, q);
       const int64_t rest = s.vrows / kTile * nt % c.np;
       if (!rc && rest > 0 && c.N > kBK)  // (a sum of one stage is not split)
-        rc = launch("linear_cross_entropy_train (dw join)", join_product_kernel<T>, 64 * rest, 256, c.st, 0, 1, q, c.np);
+        rc = launch("linear_cross_entropy_train (dw join)", join_product_kernel<T>, 64 * rest, 256, c.st, 0, 1, q);
       if (rc) return rc;
     }
   }
