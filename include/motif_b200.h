@@ -194,7 +194,7 @@ MB_API int motif_b200_swiglu_backward(const void* x, const void* dy, void* dx, i
  * The forward pass leaves in `state` what the backward pass needs (the same w, ws, N, V, d, dtype and
  * reduction); `workspace` is scratch.  Both are device memory at 256-byte boundaries;
  * motif_b200_linear_cross_entropy_bytes writes three sizes to host memory: the state, the forward
- * workspace and the backward workspace (the latter at most about 0.4 GB and one fp32 copy of dw).
+ * workspace and the backward workspace (the latter at most about 0.35 GB and one fp32 copy of dw).
  * Replaces F.cross_entropy over lm_head's logits, motif/model/motif.py:184,545-630. */
 MB_API int motif_b200_linear_cross_entropy_bytes(const void* w, int64_t ws, int64_t N, int64_t V, int64_t d, int dtype,
                                           int64_t* bytes);

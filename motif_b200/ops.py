@@ -366,10 +366,14 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     numbers.  Returns an fp32 scalar, or with `reduction='none'` one loss per token (0 where the label
     is `ignore_index`).  Such tokens cost nothing and get no gradient, whatever x holds there.
     A label outside `0 .. V - 1` that is not `ignore_index` makes its loss, and the gradients, NaN;
-    the mean over no token is NaN and its gradients are zero.  Differentiable in x and weight; 16-bit
-    gradients are sums in fp32 over `exp(logit - log sum)` rounded once to the type.  Memory beyond
-    the results: a copy of x's rows, and at most about 0.4 GB and an fp32 copy of weight's gradient
-    during the backward pass."""
+    the mean over no token is NaN and its gradients are zero.  Differentiable in x and weight.
+
+    With `mean` and `sum` in bf16 and fp32 the gradients are computed together with the loss, in one
+    pass over the logits; a call whose loss is not differentiated belongs under `torch.no_grad()`,
+    where it computes the loss alone.  With `none`, and in fp16, the backward pass computes the logits
+    again.  16-bit gradients are sums in fp32 over probabilities rounded to the type (and, for
+    the weight's, rows of x divided by their sums and rounded).  Memory beyond the results: a copy of
+    x's rows, and during a pass that computes gradients 0.6 GB at most and an fp32 copy of the weight's."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
     return _compiled('linear_cross_entropy', x, weight, labels, ignore_index, _REDUCTIONS[reduction])
