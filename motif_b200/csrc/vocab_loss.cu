@@ -40,6 +40,7 @@
 
 #include "common.cuh"
 #include "pair.cuh"
+#include "vocab_few.cuh"
 
 namespace mb {
 
@@ -1836,7 +1837,26 @@ int make_call(const char* what, Call& c) {
   c.np = std::max(1, multiprocessors() / 2);
   c.pack_w = must_pack(c.w, c.ws, c.d, c.dtype);
   c.s = sizes_of(c.N, c.V, c.d, c.pack_w, c.dtype, c.np);
+  if (few_tokens(c.N, c.d, c.dtype)) few_sizes(c.N, c.V, c.d, &c.s.state_bytes, &c.s.forward_bytes, &c.s.backward_bytes);
   return MB_OK;
+}
+// The call as the kernels of a few fp32 tokens take it.
+FewCall few_call(const Call& c) {
+  FewCall f = {};
+  f.x = (const float*)c.x;
+  f.w = (const float*)c.w;
+  f.xs = c.xs;
+  f.ws = c.ws;
+  f.labels = c.labels;
+  f.ignore = c.ignore;
+  f.N = c.N;
+  f.V = c.V;
+  f.d = c.d;
+  f.reduction = c.reduction;
+  f.state = c.state;
+  f.work = c.work;
+  f.st = c.st;
+  return f;
 }
 
 }  // namespace
@@ -1857,6 +1877,10 @@ extern "C" int motif_b200_linear_cross_entropy_bytes(const void* w, int64_t ws, 
   using namespace mb;
   MB_REQUIRE(bytes, MB_ERR_ARG, "linear_cross_entropy_bytes: null pointer");
   if (int e = check_sizes("linear_cross_entropy_bytes", N, V, d, dtype)) return e;
+  if (few_tokens(N, d, dtype)) {
+    few_sizes(N, V, d, bytes, bytes + 1, bytes + 2);
+    return MB_OK;
+  }
   const Sizes s = sizes_of(N, V, d, must_pack(w, ws, d, dtype), dtype, std::max(1, multiprocessors() / 2));
   bytes[0] = s.state_bytes;
   bytes[1] = s.forward_bytes;
@@ -1891,6 +1915,11 @@ extern "C" int motif_b200_linear_cross_entropy(const void* x, int64_t xs, const 
              "linear_cross_entropy: %lld and %lld bytes of state and workspace needed, got %lld and %lld",
              (long long)c.s.state_bytes, (long long)c.s.forward_bytes, (long long)state_bytes,
              (long long)workspace_bytes);
+  if (few_tokens(N, d, dtype)) {
+    FewCall f = few_call(c);
+    f.loss = loss;
+    return few_forward(f);
+  }
   if (dtype == MB_F32) return forward<float>(c, loss);
   return dtype == MB_BF16 ? forward<__nv_bfloat16>(c, loss) : forward<__half>(c, loss);
 }
@@ -1919,6 +1948,14 @@ extern "C" int motif_b200_linear_cross_entropy_backward(const void* w, int64_t w
              (long long)c.s.state_bytes, (long long)c.s.backward_bytes, (long long)state_bytes,
              (long long)workspace_bytes);
   if (!dx && !dw) return MB_OK;
+  if (few_tokens(N, d, dtype)) {
+    FewCall f = few_call(c);
+    f.up = grad_loss;
+    f.up_stride = grad_stride;
+    f.dx = (float*)dx;
+    f.dw = (float*)dw;
+    return few_backward(f);
+  }
   if (dtype == MB_F32) return backward<float>(c, grad_loss, grad_stride, dx, dw);
   return dtype == MB_BF16 ? backward<__nv_bfloat16>(c, grad_loss, grad_stride, dx, dw)
                           : backward<__half>(c, grad_loss, grad_stride, dx, dw);
@@ -1928,6 +1965,11 @@ extern "C" int64_t motif_b200_linear_cross_entropy_train_workspace_bytes(const v
                                                                          int64_t d, int dtype) {
   using namespace mb;
   if (check_sizes("linear_cross_entropy_train_workspace_bytes", N, V, d, dtype)) return -1;
+  if (few_tokens(N, d, dtype)) {
+    int64_t state, forward_bytes, backward_bytes;
+    few_sizes(N, V, d, &state, &forward_bytes, &backward_bytes);
+    return state + std::max(forward_bytes, backward_bytes);
+  }
   return once_sizes_of(N, V, d, must_pack(w, ws, d, dtype), dtype, std::max(1, multiprocessors() / 2)).bytes;
 }
 
@@ -1956,6 +1998,18 @@ extern "C" int motif_b200_linear_cross_entropy_train(const void* x, int64_t xs, 
   MB_REQUIRE(reduction == 1 || reduction == 2, MB_ERR_ARG, "linear_cross_entropy_train: reduction must be 1 or 2, got %d",
              reduction);
   MB_REQUIRE((N == 0 || (x && labels)) && loss, MB_ERR_ARG, "linear_cross_entropy_train: null pointer");
+  if (few_tokens(N, d, dtype)) {
+    MB_REQUIRE(workspace_bytes >= c.s.state_bytes + std::max(c.s.forward_bytes, c.s.backward_bytes), MB_ERR_ARG,
+               "linear_cross_entropy_train: %lld bytes of workspace needed, got %lld",
+               (long long)(c.s.state_bytes + std::max(c.s.forward_bytes, c.s.backward_bytes)), (long long)workspace_bytes);
+    FewCall f = few_call(c);
+    f.loss = loss;
+    f.dx = (float*)dx;
+    f.dw = (float*)dw;
+    f.work = c.work + c.s.state_bytes;
+    if (int e = few_forward(f)) return e;
+    return dx || dw ? few_backward(f) : MB_OK;
+  }
   const OnceSizes s = once_sizes_of(N, V, d, c.pack_w, dtype, c.np);
   MB_REQUIRE(workspace_bytes >= s.bytes, MB_ERR_ARG, "linear_cross_entropy_train: %lld bytes of workspace needed, got %lld",
              (long long)s.bytes, (long long)workspace_bytes);
