@@ -3,6 +3,7 @@
 // backward pass that needs no Python.  As Python autograd functions over ctypes a forward and backward pass
 // of a small norm took 130 us of host time, more than its elementary operations; here it takes 61 to 69, as torch.neg
 // does (67): the autograd engine's own.  A loss alone takes 12.
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/engine.h>
 #include <torch/csrc/autograd/graph_task.h>
@@ -274,8 +275,10 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
       const Tensor &sx = saved[0], &sw = saved[1], &any = sx.defined() ? sx : sw;
       const c10::Device dev = any.device();
       const c10::cuda::CUDAGuard guard(dev);
-      // a graph that is not kept has no other use for them: they are multiplied where they are
-      const bool keep = torch::autograd::get_current_graph_task_keep_graph();
+      // a graph that is not kept has no other use for them: they are multiplied where they are (not while a CUDA
+      // graph captures this pass, which may run again by itself)
+      const bool keep = torch::autograd::get_current_graph_task_keep_graph() ||
+                        c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
       if (sx.defined() && ctx->needs_input_grad(0)) dx = keep ? fresh(sx.sizes(), sx.scalar_type(), dev) : sx;
       if (sw.defined() && ctx->needs_input_grad(1)) dw = keep ? fresh(sw.sizes(), sw.scalar_type(), dev) : sw;
       check_backward("motif_b200_scale_gradients",

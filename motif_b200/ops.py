@@ -4,8 +4,8 @@ Same names, argument meanings, return values and exception types as
 `motif/ops/__init__.py:1-10` (plus `apply_block_attn_res`, `motif/ops/attn_res.py:596`),
 computed by the sm_100a kernels of `libmotif_b200.so`.  The delta rule, Chord attention, the
 attn-res read, the norms, SwiGLU and the vocabulary loss take gradients the way the reference's do
-(autograd Functions over the backward kernels: `motif_b200.autograd` and, compiled, `_train_host`).  CPU tensors raise `ValueError`; there is no
-eager fallback.
+(autograd Functions over the backward kernels: `motif_b200.autograd` and, compiled, `_train_host`).
+CPU tensors raise `ValueError`; there is no eager fallback.
 """
 
 from typing import Optional, Sequence
@@ -373,7 +373,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     where it computes the loss alone.  With `none`, and in fp16, the backward pass computes the logits
     again.  16-bit gradients are sums in fp32 over probabilities rounded to the type (and, for
     the weight's, rows of x divided by their sums and rounded).  Memory beyond the results: a copy of
-    x's rows, and during a pass that computes gradients 0.6 GB at most and an fp32 copy of the weight's."""
+    x's rows, and during a pass that computes gradients 0.6 GB at most and an fp32 copy of the weight's;
+    in fp32 also x and weight as three bf16 parts (6 bytes a value), or for 16 tokens or less the logits.
+
+    Both passes may be captured into CUDA graphs, on leaves that no living eager graph holds.  There are
+    no second derivatives."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
     return _compiled('linear_cross_entropy', x, weight, labels, ignore_index, _REDUCTIONS[reduction])

@@ -469,3 +469,25 @@ def test_few_fp32_tokens_strides_and_labels():
     label[0], label[1] = 701, -5
     loss, dx, dw = run(x, w, label, 'none', upstream(11, 'none'))
     assert loss[:2].isnan().all() and dx[:2].isnan().all() and not loss[2:].isnan().any() and not dx[2:].isnan().any()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_a_captured_backward_pass_runs_twice(dtype):
+    """Forward and backward passes in graphs of their own: each run of the second gives the same gradients."""
+    x, w, label = inputs(300, 96, 700, dtype, 4, 0.2)
+    up = torch.tensor(1.5, device='cuda')
+    want = run(x, w, label, 'mean', up)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    ahead, back = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        xl, wl = x.detach().requires_grad_(), w.detach().requires_grad_()
+        with torch.cuda.graph(ahead, stream=stream):
+            loss = ops.linear_cross_entropy(xl, wl, label)
+        with torch.cuda.graph(back, stream=stream, pool=ahead.pool()):
+            grads = torch.autograd.grad(loss, (xl, wl), up)
+    torch.cuda.current_stream().wait_stream(stream)
+    ahead.replay()
+    for _ in range(3):
+        back.replay()
+        assert all(torch.equal(a, b) for a, b in zip((loss, *grads), want))
