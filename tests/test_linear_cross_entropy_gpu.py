@@ -14,7 +14,11 @@ Tolerances.  With u the half step of the tensors' type (`eps / 2`) and e = 2^-24
            magnitudes for the summation; u of the result for the last rounding
   in one pass (mean and sum, bf16 and fp32): what is rounded is exp(s - s_t), relative to which G's error is the
            same; dW's other operand is x / sum rounded to the type (u of |G| |x|); and the result is rounded once
-           more when it is multiplied with the gradient that arrives (u)
+           more when it is multiplied with the gradient that arrives (u).  In bf16 a row's divisor takes back the
+           rounding of its label's place, so the others carry that one as well (u p), and three roundings in a row
+           are (1 + u)^3 - 1 < 3.03 u
+  tiny     an exponential below 2^-126 is 0, so G may be off by that and by as much where it is multiplied:
+           2^-125 |g|, times the other operand
   16 fp32 tokens or less, without the tensor cores: a lane adds d / 8 + 4 products one after another and the warp
            five times (ds holds); dx adds up to 64 words one after another (e each) where V / 16 is less
 """
@@ -87,6 +91,11 @@ def reference(x, w, label, reduction, up, ignore=-100):
     dG = p * (3 * dmax[:, None] + (V / 32 + 64 + (top - s).abs()) * E) + ru * G.abs() + 4 * E * hit
     if dtype == torch.float16:
         dG = dG + 2.0 ** -40
+    once = reduction != 'none' and dtype != torch.float16
+    if once and dtype == torch.bfloat16:
+        dG = 1.01 * (dG + u * p)
+    if dtype != torch.float16:
+        dG = dG + 2.0 ** -125
     ga = g.abs()[:, None]
     G, dG = G * g[:, None], dG * ga + 4 * E * G.abs() * ga
     if reduction == 'none' and dtype == torch.float16 and n:  # G is kept relative to the largest gradient
@@ -97,7 +106,7 @@ def reference(x, w, label, reduction, up, ignore=-100):
     dw = G.t() @ xl
     bdw = dG.t() @ xl.abs() + 2 * E * (N / 16 + 8) * (G.abs().t() @ xl.abs())
     tiny = TINY[dtype]
-    if reduction != 'none' and dtype != torch.float16:  # in one pass
+    if once:
         bdw = bdw + (u + 4 * E) * (G.abs().t() @ xl.abs())
         u = 2 * u
     return (loss, dx, dw), (bound, bdx + (u + 4 * E) * dx.abs() + tiny, bdw + (u + 4 * E) * dw.abs() + tiny)
