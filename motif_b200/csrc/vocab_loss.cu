@@ -32,6 +32,7 @@
 // fp16, whose smallest normal number is 2^-14: a probability keeps its bits down to 2^-29), and what g_n has beyond
 // is multiplied in at the end.  fp32 operands are split into three bf16 parts each (24 bits), and the six products
 // of parts that matter are summed, the small ones first: the rate of these is a sixth, still three times plain fp32's.
+// 16 fp32 tokens or less are bound by W's bytes instead and go to vocab_few.cu.
 //
 // Every wait is bounded; a CTA whose wait runs out counts itself (motif_b200_wait_timeouts), lets what
 // it issued land, and leaves NaN in the tiles that it owes.
