@@ -191,10 +191,14 @@ MB_API int motif_b200_swiglu_backward(const void* x, const void* dy, void* dx, i
  * any), 2 = sum; fp32.  dx [N, d] and dw [V, d] are contiguous, of `dtype`; either may be NULL.
  * grad_loss: the gradient of the loss, fp32 [N] (grad_stride apart) or one value.
  *
- * The forward pass leaves in `state` what the backward pass needs (the same w, ws, N, V, d, dtype and
+ * The forward pass leaves in `state` what the backward pass needs (the same values of w, N, V, d, dtype and
  * reduction); `workspace` is scratch.  Both are device memory at 256-byte boundaries;
  * motif_b200_linear_cross_entropy_bytes writes three sizes to host memory: the state, the forward
  * workspace and the backward workspace (the latter at most about 0.35 GB and one fp32 copy of dw).
+ * A 16-bit weight whose rows do not begin at 16-byte boundaries is copied into the state by the forward pass, and the
+ * backward pass reads that copy.  The state's size says so: hand the backward pass, as state_bytes, exactly what was
+ * asked for the forward pass's w and ws (another size is refused).  Where there is no copy, w may lie elsewhere by then
+ * and have other strides, but its rows must begin at 16-byte boundaries.
  * Replaces F.cross_entropy over lm_head's logits, motif/model/motif.py:184,545-630. */
 MB_API int motif_b200_linear_cross_entropy_bytes(const void* w, int64_t ws, int64_t N, int64_t V, int64_t d, int dtype,
                                           int64_t* bytes);

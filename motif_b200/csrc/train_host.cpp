@@ -231,6 +231,19 @@ Loss loss_forward(const Tensor& x, const Tensor& weight, const Tensor& labels, i
   return out;
 }
 
+// What saved-tensor hooks (offloading, packing) give back may lie elsewhere, with other strides: `t` as plain memory
+// at a boundary of `bytes`.
+Tensor plain(const Tensor& t, uintptr_t bytes) {
+  return t.is_contiguous() && (uintptr_t)t.data_ptr() % bytes == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+// w [V, d] with rows that begin at 16-byte boundaries.
+Tensor aligned_rows(const Tensor& w) {
+  const int64_t step = 16 / w.element_size();
+  if ((uintptr_t)w.data_ptr() % 16 == 0 && w.stride(0) % step == 0 && w.stride(0) >= w.size(1)) return w;
+  Tensor out = at::empty({w.size(0), (w.size(1) + step - 1) / step * step}, w.options()).narrow(1, 0, w.size(1));
+  return out.copy_(w);
+}
+
 // Where one gradient arrives for all tokens, the forward pass computes the gradients as well, in one pass over
 // the logits, and the backward pass multiplies them with what arrived.  (fp16, whose range is too small for that,
 // and one gradient per token: the logits are computed again in the backward pass.)
@@ -245,6 +258,9 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
       Loss out = loss_forward(x, weight, labels, ignore, reduction);
       ctx->save_for_backward({weight, out.state});
       ctx->saved_data["bytes"] = out.backward_bytes;
+      ctx->saved_data["state"] = out.state.numel();
+      ctx->saved_data["words"] = weight.size(0);
+      ctx->saved_data["dtype"] = (int64_t)weight.scalar_type();
       return out.loss;
     }
     const c10::Device dev = x.device();
@@ -288,23 +304,36 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
                                                 dtype_code(any.scalar_type()), stream_of(dev)));
       return {dx, dw, Tensor(), Tensor(), Tensor()};
     }
-    const Tensor &weight = saved[0], &state = saved[1];
+    const Tensor& weight = saved[0];
     const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
     const int64_t reduction = ctx->saved_data["reduction"].toInt(), bytes = ctx->saved_data["bytes"].toInt();
-    const c10::Device dev = weight.device();
+    const int64_t v = ctx->saved_data["words"].toInt(), d = shape.back();
+    const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+    const int dc = dtype_code(dtype);
+    const c10::Device dev = grads[0].device();
+    // the kernels index memory with what they find in the state
+    TORCH_CHECK(saved[1].device() == dev && saved[1].scalar_type() == at::kByte &&
+                    saved[1].numel() == ctx->saved_data["state"].toInt() && weight.device() == dev &&
+                    weight.scalar_type() == dtype && weight.sizes() == at::IntArrayRef({v, d}),
+                "linear_cross_entropy: the tensors saved by its forward pass came back as others");
     const c10::cuda::CUDAGuard guard(dev);
-    const Tensor w = rows_of(weight), up = reduction == 0 ? grads[0].reshape({-1}) : grads[0];
-    const int64_t v = w.size(0), d = w.size(1);
+    const Tensor state = plain(saved[1], 256), up = reduction == 0 ? grads[0].reshape({-1}) : grads[0];
+    Tensor w = rows_of(weight);
     int64_t n = 1;
     for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
-    if (ctx->needs_input_grad(0)) dx = fresh(shape, weight.scalar_type(), dev);
-    if (ctx->needs_input_grad(1)) dw = fresh({v, d}, weight.scalar_type(), dev);
+    // a weight that the forward pass read where it was and that came back with other strides
+    int64_t now[3];
+    check_backward("motif_b200_linear_cross_entropy_bytes",
+                   motif_b200_linear_cross_entropy_bytes(w.data_ptr(), w.stride(0), n, v, d, dc, now));
+    if (now[0] > state.numel()) w = aligned_rows(w);
+    if (ctx->needs_input_grad(0)) dx = fresh(shape, dtype, dev);
+    if (ctx->needs_input_grad(1)) dw = fresh({v, d}, dtype, dev);
     const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes);
     check_backward("motif_b200_linear_cross_entropy_backward",
                    motif_b200_linear_cross_entropy_backward(
                        w.data_ptr(), w.stride(0), up.data_ptr<float>(), reduction == 0 ? up.stride(0) : 0,
                        (int)reduction, ptr(dx), ptr(dw), n, v, d, state.data_ptr(), state.numel(), ws.get(), bytes,
-                       dtype_code(weight.scalar_type()), stream_of(dev)));
+                       dc, stream_of(dev)));
     return {dx, dw, Tensor(), Tensor(), Tensor()};
   }
 };

@@ -1380,13 +1380,13 @@ Sizes sizes_of(int64_t N, int64_t V, int64_t d, bool pack_w, int dtype, int np) 
     return at;
   };
   s.x = take(s.state_bytes, s.parts * s.rows * s.dp * 2);
-  s.w = take(s.state_bytes, pack_w ? s.parts * s.vrows * s.dp * 2 : 0);
   s.label = take(s.state_bytes, s.rows * 4);
   s.index = take(s.state_bytes, s.rows * 4);
   s.place = take(s.state_bytes, N * 4);
   s.stat = take(s.state_bytes, s.rows * (int64_t)sizeof(RowStat));
   s.count = take(s.state_bytes, 4);
   s.ticket = take(s.state_bytes, 4);
+  s.w = take(s.state_bytes, pack_w ? s.parts * s.vrows * s.dp * 2 : 0);  // last: nothing's place depends on it
   const int64_t mt = s.rows / kTile;
   s.group = take(s.forward_bytes, up_to(N, 256) / 256 * 4);
   s.seg = take(s.forward_bytes, (np + mt) * 2 * kTile * (int64_t)sizeof(float2));
@@ -1833,7 +1833,9 @@ int check_sizes(const char* what, int64_t N, int64_t V, int64_t d, int dtype) {
              "%s: bad sizes N=%lld V=%lld d=%lld", what, (long long)N, (long long)V, (long long)d);
   return MB_OK;
 }
-int make_call(const char* what, Call& c) {
+// `state_bytes`: the backward pass's, which is laid out as the forward pass chose (0: this is that pass).  Where the
+// weight lies and how its rows are strided may have changed in between, so neither tells: the state's size does.
+int make_call(const char* what, Call& c, int64_t state_bytes = 0) {
   if (int e = check_sizes(what, c.N, c.V, c.d, c.dtype)) return e;
   MB_REQUIRE(c.reduction >= 0 && c.reduction <= 2, MB_ERR_ARG, "%s: unknown reduction %d", what, c.reduction);
   MB_REQUIRE(c.w && c.state && c.work, MB_ERR_ARG, "%s: null pointer", what);
@@ -1842,7 +1844,21 @@ int make_call(const char* what, Call& c) {
   c.np = std::max(1, multiprocessors() / 2);
   c.pack_w = must_pack(c.w, c.ws, c.d, c.dtype);
   c.s = sizes_of(c.N, c.V, c.d, c.pack_w, c.dtype, c.np);
-  if (few_tokens(c.N, c.d, c.dtype)) few_sizes(c.N, c.V, c.d, &c.s.state_bytes, &c.s.forward_bytes, &c.s.backward_bytes);
+  if (few_tokens(c.N, c.d, c.dtype)) {
+    few_sizes(c.N, c.V, c.d, &c.s.state_bytes, &c.s.forward_bytes, &c.s.backward_bytes);
+  } else if (state_bytes && c.dtype != MB_F32) {  // (fp32 weights are always packed)
+    const Sizes other = sizes_of(c.N, c.V, c.d, !c.pack_w, c.dtype, c.np);
+    if (state_bytes == other.state_bytes) {
+      MB_REQUIRE(!c.pack_w, MB_ERR_ALIGN,
+                 "%s: the forward pass read the weight where it was, so its rows must begin at 16-byte boundaries here, too",
+                 what);
+      c.pack_w = true;
+      c.s = other;
+    }
+    MB_REQUIRE(state_bytes == c.s.state_bytes, MB_ERR_ARG,
+               "%s: a state of %lld bytes is none that a forward pass of these sizes left (%lld or %lld)", what,
+               (long long)state_bytes, (long long)c.s.state_bytes, (long long)other.state_bytes);
+  }
   return MB_OK;
 }
 // The call as the kernels of a few fp32 tokens take it.
@@ -1946,7 +1962,7 @@ extern "C" int motif_b200_linear_cross_entropy_backward(const void* w, int64_t w
   c.state = (unsigned char*)state;
   c.work = (unsigned char*)workspace;
   c.st = (cudaStream_t)stream;
-  if (int e = make_call("linear_cross_entropy_backward", c)) return e;
+  if (int e = make_call("linear_cross_entropy_backward", c, std::max<int64_t>(1, state_bytes))) return e;
   MB_REQUIRE(grad_loss || (N == 0 && reduction == 0), MB_ERR_ARG, "linear_cross_entropy_backward: null pointer");
   MB_REQUIRE(state_bytes >= c.s.state_bytes && workspace_bytes >= c.s.backward_bytes, MB_ERR_ARG,
              "linear_cross_entropy_backward: %lld and %lld bytes of state and workspace needed, got %lld and %lld",
