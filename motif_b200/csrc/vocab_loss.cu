@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
         }
       }
       // (s - top) log2 e: as one multiply-add where the type's own rounding is coarser than the product top log2 e
-      const float ref = MODE == kLoss && top == -INFINITY ? 0.f : top;
+      const float ref = MODE != kAgain && top == -INFINITY ? 0.f : top;  // (kOnce: the label's logit may be -inf)
       const float2 c2 = make_float2(kLog2e, kLog2e), n2 = make_float2(-ref, -ref);
       const float2 m2 = make_float2(-ref * kLog2e, -ref * kLog2e), i2 = make_float2(inv, inv);
       float2 acc[4] = {};

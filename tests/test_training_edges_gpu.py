@@ -1,0 +1,58 @@
+"""Edges of the training operators: labels infinitely far away, logits far from zero, long sums, weights of other
+types, calls under torch's transforms, tensors past 2^31 elements, and what a launch tracker sees."""
+
+import pytest
+import torch
+
+from motif_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    _lib.wait_timeouts()
+    yield
+    assert _lib.wait_timeouts() == 0
+
+
+def gradients(x, w, label, reduction='mean', up=None):
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, label, reduction=reduction)
+    up = torch.ones_like(loss) if up is None else up
+    return (loss.detach(), *torch.autograd.grad(loss, (x, w), up))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize('N,V', [(40, 300), (40, 257), (9, 300)])
+def test_a_label_whose_logit_is_minus_infinity(dtype, N, V):
+    """Its loss is infinite and its gradients are those of a label that is only far away: the label's own probability is
+    0 in both.  (The last tile's columns behind the words are -inf as well.)"""
+    g = torch.Generator(device='cuda').manual_seed(V)
+    x = torch.randn(N, 64, device='cuda', generator=g)
+    x[:, 0] = 16
+    x = x.to(dtype)
+    w = torch.randn(V, 64, device='cuda', generator=g) * 0.2
+    w[:, 0] = 0
+    far, label = V - 1, torch.randint(0, V - 1, (N,), device='cuda', generator=g)
+    label[::3] = far
+    w = w.to(dtype)
+    w[far, 0] = -100
+    want = gradients(x, w, label)
+    # 16 times the type's lowest number is -inf in fp32; fp16's own infinity
+    w[far, 0] = float('-inf') if dtype == torch.float16 else torch.finfo(dtype).min
+    assert want[0].isfinite() and want[1].isfinite().all() and want[2].isfinite().all()
+    for reduction in ('mean', 'sum', 'none'):
+        with torch.no_grad():
+            alone = ops.linear_cross_entropy(x, w, label, reduction=reduction)
+        got = gradients(x, w, label, reduction)
+        assert torch.equal(got[0], alone) and not got[0].isnan().any() and got[0].isinf().any()
+        if reduction == 'none':
+            assert torch.equal(got[0].isinf(), label == far)
+        assert got[2].isfinite().all()
+        if reduction == 'mean':
+            assert torch.equal(got[2], want[2])
+            if dtype != torch.float16:  # (0 times fp16's infinity)
+                assert torch.equal(got[1][:, 1:], want[1][:, 1:])
