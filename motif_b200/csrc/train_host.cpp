@@ -252,6 +252,8 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
                         int64_t reduction) {
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["words"] = weight.size(0);
+    ctx->saved_data["dtype"] = (int64_t)weight.scalar_type();
     const bool again = reduction == 0 || x.scalar_type() == at::kHalf;
     ctx->saved_data["again"] = again;
     if (again) {
@@ -259,8 +261,6 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
       ctx->save_for_backward({weight, out.state});
       ctx->saved_data["bytes"] = out.backward_bytes;
       ctx->saved_data["state"] = out.state.numel();
-      ctx->saved_data["words"] = weight.size(0);
-      ctx->saved_data["dtype"] = (int64_t)weight.scalar_type();
       return out.loss;
     }
     const c10::Device dev = x.device();
@@ -279,6 +279,8 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
                                                 lab.data_ptr<int64_t>(), ignore, (int)reduction,
                                                 loss.data_ptr<float>(), ptr(dx), ptr(dw), n, v, d, ws.get(), bytes, dc,
                                                 stream_of(dev)));
+    // saved-tensor hooks may keep what they are handed: then the backward pass writes elsewhere
+    ctx->saved_data["own"] = !at::SavedTensorDefaultHooks::get_hooks().has_value();
     ctx->save_for_backward({dx, dw});
     return loss;
   }
@@ -286,39 +288,47 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order();
     const variable_list saved = ctx->get_saved_variables();
-    Tensor dx, dw;
-    if (!ctx->saved_data["again"].toBool()) {
-      const Tensor &sx = saved[0], &sw = saved[1], &any = sx.defined() ? sx : sw;
-      const c10::Device dev = any.device();
-      const c10::cuda::CUDAGuard guard(dev);
-      // a graph that is not kept has no other use for them: they are multiplied where they are (not while a CUDA
-      // graph captures this pass, which may run again by itself)
-      const bool keep = torch::autograd::get_current_graph_task_keep_graph() ||
-                        c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
-      if (sx.defined() && ctx->needs_input_grad(0)) dx = keep ? fresh(sx.sizes(), sx.scalar_type(), dev) : sx;
-      if (sw.defined() && ctx->needs_input_grad(1)) dw = keep ? fresh(sw.sizes(), sw.scalar_type(), dev) : sw;
-      check_backward("motif_b200_scale_gradients",
-                     motif_b200_scale_gradients(dx.defined() ? sx.data_ptr() : nullptr, ptr(dx),
-                                                dx.defined() ? dx.numel() : 0, dw.defined() ? sw.data_ptr() : nullptr,
-                                                ptr(dw), dw.defined() ? dw.numel() : 0, grads[0].data_ptr<float>(),
-                                                dtype_code(any.scalar_type()), stream_of(dev)));
-      return {dx, dw, Tensor(), Tensor(), Tensor()};
-    }
-    const Tensor& weight = saved[0];
     const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
-    const int64_t reduction = ctx->saved_data["reduction"].toInt(), bytes = ctx->saved_data["bytes"].toInt();
+    const int64_t reduction = ctx->saved_data["reduction"].toInt();
     const int64_t v = ctx->saved_data["words"].toInt(), d = shape.back();
     const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
     const int dc = dtype_code(dtype);
     const c10::Device dev = grads[0].device();
-    // the kernels index memory with what they find in the state
-    TORCH_CHECK(saved[1].device() == dev && saved[1].scalar_type() == at::kByte &&
-                    saved[1].numel() == ctx->saved_data["state"].toInt() && weight.device() == dev &&
-                    weight.scalar_type() == dtype && weight.sizes() == at::IntArrayRef({v, d}),
-                "linear_cross_entropy: the tensors saved by its forward pass came back as others");
     const c10::cuda::CUDAGuard guard(dev);
+    // what hooks hand back is read as what was saved (and memory is indexed with what lies in the state)
+    auto came_back = [&](const Tensor& t, at::ScalarType type, at::IntArrayRef sizes) {
+      TORCH_CHECK(t.device() == dev && t.scalar_type() == type && t.sizes() == sizes,
+                  "linear_cross_entropy: the tensors saved by its forward pass came back as others");
+    };
+    Tensor dx, dw;
+    if (!ctx->saved_data["again"].toBool()) {
+      Tensor sx = saved[0], sw = saved[1];
+      if (sx.defined()) {
+        came_back(sx, dtype, shape);
+        sx = plain(sx, 16);
+      }
+      if (sw.defined()) {
+        came_back(sw, dtype, {v, d});
+        sw = plain(sw, 16);
+      }
+      // a graph that is not kept has no other use for them: they are multiplied where they are (not while a CUDA
+      // graph captures this pass, which may run again by itself)
+      const bool keep = !ctx->saved_data["own"].toBool() || torch::autograd::get_current_graph_task_keep_graph() ||
+                        c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+      if (sx.defined() && ctx->needs_input_grad(0)) dx = keep ? fresh(shape, dtype, dev) : sx;
+      if (sw.defined() && ctx->needs_input_grad(1)) dw = keep ? fresh({v, d}, dtype, dev) : sw;
+      check_backward("motif_b200_scale_gradients",
+                     motif_b200_scale_gradients(dx.defined() ? sx.data_ptr() : nullptr, ptr(dx),
+                                                dx.defined() ? dx.numel() : 0, dw.defined() ? sw.data_ptr() : nullptr,
+                                                ptr(dw), dw.defined() ? dw.numel() : 0, grads[0].data_ptr<float>(), dc,
+                                                stream_of(dev)));
+      return {dx, dw, Tensor(), Tensor(), Tensor()};
+    }
+    came_back(saved[0], dtype, {v, d});
+    came_back(saved[1], at::kByte, {ctx->saved_data["state"].toInt()});
+    const int64_t bytes = ctx->saved_data["bytes"].toInt();
     const Tensor state = plain(saved[1], 256), up = reduction == 0 ? grads[0].reshape({-1}) : grads[0];
-    Tensor w = rows_of(weight);
+    Tensor w = rows_of(saved[0]);
     int64_t n = 1;
     for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
     // a weight that the forward pass read where it was and that came back with other strides

@@ -107,3 +107,47 @@ def test_other_tensors_than_were_saved_are_refused():
             loss = ops.linear_cross_entropy(x, w, label)
         with pytest.raises(RuntimeError, match='came back as others'):
             loss.backward()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('hook', HOOKS)
+@pytest.mark.parametrize('N,d,V', [(70, 96, 700), (33, 97, 300), (9, 33, 130)])
+def test_gradients_that_were_computed_with_the_loss(hook, dtype, N, d, V):
+    g = torch.Generator(device='cuda').manual_seed(N)
+    x = torch.randn(N, d, device='cuda', generator=g).to(dtype).requires_grad_()
+    w = (torch.randn(V, d, device='cuda', generator=g) * 0.2).to(dtype).requires_grad_()
+    label = torch.randint(0, V, (N,), device='cuda', generator=g)
+    up = torch.tensor(1.5, device='cuda')
+    want = torch.autograd.grad(ops.linear_cross_entropy(x, w, label), (x, w), up)
+    with HOOKS[hook]():
+        loss = ops.linear_cross_entropy(x, w, label)
+    for keep in (True, False):
+        got = torch.autograd.grad(loss, (x, w), up, retain_graph=keep)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_what_a_hook_keeps_is_not_written_to(dtype):
+    x = torch.randn(40, 64, device='cuda').to(dtype).requires_grad_()
+    w = torch.randn(300, 64, device='cuda').to(dtype).requires_grad_()
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        loss = ops.linear_cross_entropy(x, w, torch.arange(40, device='cuda'))
+    before = [t.clone() for t in kept]
+    got = torch.autograd.grad(loss, (x, w), torch.tensor(3.0, device='cuda'))
+    assert kept and all(torch.equal(a, b) for a, b in zip(kept, before))
+    for t in got:
+        t.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(kept, before))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('N', [50, 9])
+def test_other_gradients_than_were_saved_are_refused(dtype, N):
+    x = torch.randn(N, 64, device='cuda').to(dtype).requires_grad_()
+    w = (torch.randn(300, 64, device='cuda') * 0.2).to(dtype).requires_grad_()
+    for change in (lambda t: t[:-1], lambda t: t.double(), lambda t: t.half(), lambda t: t.cpu(), lambda t: t.flatten()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            loss = ops.linear_cross_entropy(x, w, torch.arange(N, device='cuda'))
+        with pytest.raises(RuntimeError, match='came back as others'):
+            loss.backward()
