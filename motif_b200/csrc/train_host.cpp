@@ -70,6 +70,13 @@ std::vector<int64_t> shape_with(const Tensor& x, int64_t last) {
 Tensor flat(const Tensor& w) { return !w.defined() || w.is_contiguous() ? w : w.contiguous(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// What a backward pass finds saved may be other than what its forward pass saved (a hook's mistake, an exchanged
+// .data): the kernels go by the sizes of dy, so x has to be of them, `last` in its last dimension.
+void came_back(const char* op, const Tensor& x, const Tensor& dy, int64_t last) {
+  TORCH_CHECK(x.device() == dy.device() && x.scalar_type() == dy.scalar_type() && x.sizes().vec() == shape_with(dy, last), op,
+              ": the input saved by its forward pass came back as another");
+}
+
 // ------------------------------------------------------------------ norms
 struct NormFunction : torch::autograd::Function<NormFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, double eps, bool gated) {
@@ -85,6 +92,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     ctx->save_for_backward({x, weight ? *weight : Tensor()});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["gated"] = gated;
+    ctx->saved_data["weight"] = (int64_t)(weight ? weight->scalar_type() : at::ScalarType::Undefined);
     return y;
   }
 
@@ -94,10 +102,16 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     const Tensor &x = saved[0], &weight = saved[1];
     const bool gated = ctx->saved_data["gated"].toBool();
     const float eps = (float)ctx->saved_data["eps"].toDouble();
-    const c10::Device dev = x.device();
+    const c10::Device dev = grads[0].device();
     const c10::cuda::CUDAGuard guard(dev);
+    const int64_t n = grads[0].size(-1);
+    came_back("rms_norm", x, grads[0], gated ? 2 * n : n);
+    TORCH_CHECK(ctx->saved_data["weight"].toInt() ==
+                        (weight.defined() ? (int64_t)weight.scalar_type() : (int64_t)at::ScalarType::Undefined) &&
+                    (!weight.defined() || (weight.device() == dev && weight.sizes() == at::IntArrayRef({n}))),
+                "rms_norm: the weight saved by its forward pass came back as another");
     const Tensor r = rows_of(x), dy = rows_of(grads[0]), w = flat(weight);
-    const int64_t m = r.size(0), n = dy.size(1);
+    const int64_t m = r.size(0);
     Tensor dx = fresh(x.sizes(), x.scalar_type(), dev), dw;
     const int wd = w.defined() ? dtype_code(w.scalar_type()) : MB_F32, dc = dtype_code(x.scalar_type());
     int64_t bytes = 0;
@@ -167,8 +181,9 @@ struct SwiGLUFunction : torch::autograd::Function<SwiGLUFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order();
     const Tensor x = ctx->get_saved_variables()[0];
-    const c10::Device dev = x.device();
+    const c10::Device dev = grads[0].device();
     const c10::cuda::CUDAGuard guard(dev);
+    came_back("swiglu", x, grads[0], 2 * grads[0].size(-1));
     const Tensor r = rows_of(x), dy = rows_of(grads[0]);
     Tensor dx = fresh(x.sizes(), x.scalar_type(), dev);
     check_backward("motif_b200_swiglu_backward",

@@ -151,3 +151,49 @@ def test_other_gradients_than_were_saved_are_refused(dtype, N):
             loss = ops.linear_cross_entropy(x, w, torch.arange(N, device='cuda'))
         with pytest.raises(RuntimeError, match='came back as others'):
             loss.backward()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('hook', HOOKS)
+@pytest.mark.parametrize('kind', ['rms', 'gated', 'swiglu'])
+def test_norms(kind, hook, dtype):
+    """Dense copies give the same bits.  Rows that vectors take and that come back as ones that they do not: the same but
+    for the order of the sums, N / 32 + 40 steps of 2^-24 for a row's and 33 more for dW's, of magnitudes below
+    |dy w r| (|x r| + 1) (|g| + 1) < 4 x 3 x 1.3 x 5 x 2 = 156 at these sizes."""
+    g = torch.Generator(device='cuda').manual_seed(1)
+    for N in (64, 250, 1032):
+        x = torch.randn(3, 11, N if kind == 'rms' else 2 * N, device='cuda', generator=g).to(dtype)
+        w = torch.randn(N, device='cuda', generator=g).to(dtype)
+        dy = torch.randn(3, 11, N, device='cuda', generator=g).to(dtype)
+        f = {'rms': ops.rms_norm, 'gated': ops.gated_rms_norm, 'swiglu': lambda x, w: ops.swiglu(x)}[kind]
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        leaves = (xl, wl)[:1 if kind == 'swiglu' else 2]
+        want = torch.autograd.grad(f(xl, wl), leaves, dy)
+        with HOOKS[hook]():
+            y = f(xl, wl)
+        got = torch.autograd.grad(y, leaves, dy)
+        for a, b in zip(got, want):
+            if hook in ('dense', 'host'):
+                assert torch.equal(a, b)
+            tol = 2.02 * torch.finfo(dtype).eps / 2 * b.double().abs() + 2 * (N / 32 + 73) * 2.0 ** -24 * 156
+            assert ((a.double() - b.double()).abs() <= tol).all()
+
+
+def test_other_rows_than_were_saved_are_refused():
+    x, w = torch.randn(20, 64, device='cuda').requires_grad_(), torch.ones(64, device='cuda').requires_grad_()
+    half = torch.ones(32, device='cuda').requires_grad_()
+    calls = (lambda: ops.rms_norm(x, w), lambda: ops.gated_rms_norm(x, half), lambda: ops.swiglu(x), lambda: ops.rms_norm(x))
+    for f in calls:
+        for change in (lambda t: t[:-1], lambda t: t.double(), lambda t: t.half(), lambda t: t.cpu(), lambda t: t[..., :-2],
+                       lambda t: torch.cat([t, t])):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+                y = f()
+            with pytest.raises(RuntimeError, match='came back as another'):
+                y.sum().backward()
+    # the weight alone, exchanged for a shorter one or one of another type
+    for other in (torch.ones(32, device='cuda'), torch.ones(64, device='cuda', dtype=torch.float64)):
+        p = torch.nn.Parameter(torch.ones(64, device='cuda'))
+        y = ops.rms_norm(x, p)
+        p.data = other
+        with pytest.raises(RuntimeError, match='came back as another'):
+            y.sum().backward()
