@@ -302,6 +302,13 @@ def swiglu(x: torch.Tensor, dim: int = -1) -> torch.Tensor:
     return _compiled('swiglu', x)
 
 
+def _readable(weight, x):
+    """A module's weight in a type that the kernels read: its own, or else x's (its gradient goes back the same way)."""
+    if weight is None or weight.dtype in (torch.float32, torch.bfloat16, torch.float16):
+        return weight
+    return weight.to(x.dtype)
+
+
 class RMSNorm(nn.Module):
     """`RMSNorm` (`motif/ops/rms_norm.py:419-486`) on the CUDA kernels; parameter `weight`."""
 
@@ -317,7 +324,7 @@ class RMSNorm(nn.Module):
         self.use_triton = bool(use_triton)
 
     def forward(self, x):
-        return rms_norm(x, self.weight, self.eps)
+        return rms_norm(x, _readable(self.weight, x), float(self.eps))
 
 
 class GatedRMSNorm(nn.Module):
@@ -338,7 +345,7 @@ class GatedRMSNorm(nn.Module):
         _cuda('x', x)
         if x.shape[-1] != 2 * self.dim:
             raise ValueError(f'GatedRMSNorm expects last dim {2 * self.dim}, got {x.shape[-1]}')
-        return gated_rms_norm(x, self.weight, self.eps)
+        return gated_rms_norm(x, _readable(self.weight, x), float(self.eps))
 
 
 class SwiGLU(nn.Module):

@@ -56,3 +56,24 @@ def test_a_label_whose_logit_is_minus_infinity(dtype, N, V):
             assert torch.equal(got[2], want[2])
             if dtype != torch.float16:  # (0 times fp16's infinity)
                 assert torch.equal(got[1][:, 1:], want[1][:, 1:])
+
+
+@pytest.mark.parametrize('kind', [torch.float64, torch.int32, torch.bool])
+def test_norm_modules_take_weights_of_any_type(kind):
+    """As they did before they took gradients: a weight in a type that no kernel reads is converted to the input's."""
+    g = torch.Generator(device='cuda').manual_seed(1)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        x = torch.randn(5, 64, device='cuda', generator=g).to(dtype)
+        for module, n in ((ops.RMSNorm, 64), (ops.GatedRMSNorm, 32)):
+            w = (2 * torch.randn(n, device='cuda', generator=g)).to(kind)
+            m, same = module(n, eps='1e-5').cuda(), module(n, eps=1e-5).cuda()  # (what float() reads will do, too)
+            m.weight = torch.nn.Parameter(w, requires_grad=kind == torch.float64)
+            same.weight = torch.nn.Parameter(w.to(dtype))
+            with torch.no_grad():
+                assert torch.equal(m(x), same(x))
+            xl, xs = x.clone().requires_grad_(), x.clone().requires_grad_()
+            y, z = m(xl), same(xs)
+            y.sum().backward(), z.sum().backward()
+            assert torch.equal(y, z) and torch.equal(xl.grad, xs.grad)
+            if kind == torch.float64:
+                assert m.weight.grad.dtype == kind and torch.equal(m.weight.grad, same.weight.grad.double())
