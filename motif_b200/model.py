@@ -537,8 +537,11 @@ class MotifChordModel(nn.Module):
             position = int(position.reshape(-1)[0])
         if cache is None:
             cache = self.create_cache()
-        if labels is not None and not return_logits and labels.shape != input_ids.shape:
-            raise ValueError(f'labels {tuple(labels.shape)} do not match input_ids {tuple(input_ids.shape)}')
+        if labels is not None and not return_logits:  # before any layer has advanced its cache
+            if labels.shape != input_ids.shape:
+                raise ValueError(f'labels {tuple(labels.shape)} do not match input_ids {tuple(input_ids.shape)}')
+            if labels.dtype == torch.bool or labels.is_floating_point() or labels.is_complex():
+                raise ValueError(f'labels must be whole numbers, got {labels.dtype}')
         with torch.no_grad():
             logits, x_final, hn = _forward(self, input_ids.to(self.embed.weight.device), cache, position or 0,
                                            key_bias if mask is not None else None, return_logits)

@@ -5,6 +5,8 @@ import pytest
 import torch
 
 from motif_b200 import _lib, ops
+from motif_b200.config import MotifChordConfig
+from motif_b200.model import MotifChordModel
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +79,17 @@ def test_norm_modules_take_weights_of_any_type(kind):
             assert torch.equal(y, z) and torch.equal(xl.grad, xs.grad)
             if kind == torch.float64:
                 assert m.weight.grad.dtype == kind and torch.equal(m.weight.grad, same.weight.grad.double())
+
+
+def test_labels_are_refused_before_the_cache_moves():
+    torch.manual_seed(0)
+    cfg = MotifChordConfig(vocab_size=500, model_dim=256, num_heads=4, num_kv_heads=2, head_k_dim=64, block_n=1)
+    m = MotifChordModel(cfg).cuda().eval()
+    ids = torch.randint(0, 500, (2, 20), device='cuda')
+    with torch.no_grad():
+        want = m(ids).logits
+        cache = m.create_cache()
+        for bad in (ids.float(), ids.bool(), ids[:, 1:]):
+            with pytest.raises(ValueError, match='labels'):
+                m(ids, cache=cache, labels=bad, return_logits=False)
+        assert torch.equal(m(ids, cache=cache).logits, want)
