@@ -41,8 +41,11 @@ void first_order() {
                               "motif_b200 ops have no second derivatives (create_graph=True)");
 }
 
+// The values that t stands for as they lie in memory (a copy of a view that is negated lazily).
+Tensor resolved(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 // t as rows of its last dimension whose elements lie next to each other (a copy where they do not).
-Tensor rows_of(const Tensor& t) {
+Tensor rows_of(const Tensor& lazy) {
+  const Tensor t = resolved(lazy);
   Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / std::max<int64_t>(t.size(-1), 1), t.size(-1)});
   return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
 }
@@ -67,7 +70,7 @@ std::vector<int64_t> shape_with(const Tensor& x, int64_t last) {
   return s;
 }
 // Plain [n] memory of a weight.
-Tensor flat(const Tensor& w) { return !w.defined() || w.is_contiguous() ? w : w.contiguous(); }
+Tensor flat(const Tensor& w) { return w.defined() ? resolved(w).contiguous() : w; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // What a backward pass finds saved may be other than what its forward pass saved (a hook's mistake, an exchanged
@@ -228,7 +231,7 @@ struct Loss {
 Loss loss_forward(const Tensor& x, const Tensor& weight, const Tensor& labels, int64_t ignore, int64_t reduction) {
   const c10::Device dev = x.device();
   const c10::cuda::CUDAGuard guard(dev);
-  const Tensor r = rows_of(x), w = rows_of(weight), lab = labels.to(at::kLong).contiguous();
+  const Tensor r = rows_of(x), w = rows_of(weight), lab = resolved(labels).to(at::kLong).contiguous();
   const int64_t n = r.size(0), d = r.size(1), v = w.size(0);
   const int dc = dtype_code(x.scalar_type());
   int64_t bytes[3];
@@ -249,7 +252,8 @@ Loss loss_forward(const Tensor& x, const Tensor& weight, const Tensor& labels, i
 // What saved-tensor hooks (offloading, packing) give back may lie elsewhere, with other strides: `t` as plain memory
 // at a boundary of `bytes`.
 Tensor plain(const Tensor& t, uintptr_t bytes) {
-  return t.is_contiguous() && (uintptr_t)t.data_ptr() % bytes == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+  if (t.is_contiguous() && !t.is_neg() && (uintptr_t)t.data_ptr() % bytes == 0) return t;
+  return resolved(t).clone(at::MemoryFormat::Contiguous);
 }
 // w [V, d] with rows that begin at 16-byte boundaries.
 Tensor aligned_rows(const Tensor& w) {
@@ -280,7 +284,7 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
     }
     const c10::Device dev = x.device();
     const c10::cuda::CUDAGuard guard(dev);
-    const Tensor r = rows_of(x), w = rows_of(weight), lab = labels.to(at::kLong).contiguous();
+    const Tensor r = rows_of(x), w = rows_of(weight), lab = resolved(labels).to(at::kLong).contiguous();
     const int64_t n = r.size(0), d = r.size(1), v = w.size(0);
     const int dc = dtype_code(x.scalar_type());
     Tensor loss = fresh({}, at::kFloat, dev), dx, dw;
@@ -335,14 +339,14 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
       check_backward("motif_b200_scale_gradients",
                      motif_b200_scale_gradients(dx.defined() ? sx.data_ptr() : nullptr, ptr(dx),
                                                 dx.defined() ? dx.numel() : 0, dw.defined() ? sw.data_ptr() : nullptr,
-                                                ptr(dw), dw.defined() ? dw.numel() : 0, grads[0].data_ptr<float>(), dc,
-                                                stream_of(dev)));
+                                                ptr(dw), dw.defined() ? dw.numel() : 0,
+                                                resolved(grads[0]).data_ptr<float>(), dc, stream_of(dev)));
       return {dx, dw, Tensor(), Tensor(), Tensor()};
     }
     came_back(saved[0], dtype, {v, d});
     came_back(saved[1], at::kByte, {ctx->saved_data["state"].toInt()});
     const int64_t bytes = ctx->saved_data["bytes"].toInt();
-    const Tensor state = plain(saved[1], 256), up = reduction == 0 ? grads[0].reshape({-1}) : grads[0];
+    const Tensor state = plain(saved[1], 256), up = reduction == 0 ? resolved(grads[0]).reshape({-1}) : resolved(grads[0]);
     Tensor w = rows_of(saved[0]);
     int64_t n = 1;
     for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];

@@ -93,3 +93,33 @@ def test_labels_are_refused_before_the_cache_moves():
             with pytest.raises(ValueError, match='labels'):
                 m(ids, cache=cache, labels=bad, return_logits=False)
         assert torch.equal(m(ids, cache=cache).logits, want)
+
+
+def test_views_that_are_negated_lazily():
+    g = torch.Generator(device='cuda').manual_seed(5)
+    x, w = torch.randn(40, 64, device='cuda', generator=g), torch.randn(64, device='cuda', generator=g)
+    head = torch.randn(300, 64, device='cuda', generator=g) * 0.2
+    label = torch.randint(0, 300, (40,), device='cuda', generator=g)
+    up = torch.randn(40, 64, device='cuda', generator=g)
+    neg = torch._neg_view
+    for f in (lambda x, w: ops.rms_norm(x, w), lambda x, w: ops.gated_rms_norm(x, w[:32]), lambda x, w: ops.swiglu(x)):
+        for grad in (False, True):
+            a, b = neg(x).requires_grad_(grad), neg(w).requires_grad_(grad)
+            c, d = (-x).requires_grad_(grad), (-w).requires_grad_(grad)
+            y, z = f(a, b), f(c, d)
+            assert torch.equal(y, z)
+            if grad:
+                dy = up[:, :y.shape[1]].contiguous()
+                for p, q in zip(torch.autograd.grad(y, (a, b), neg(dy), allow_unused=True),
+                                torch.autograd.grad(z, (c, d), -dy, allow_unused=True)):
+                    assert (p is None and q is None) or torch.equal(p, q)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        for n in (40, 9):
+            for reduction in ('none', 'mean'):
+                a, b = x[:n].to(dtype), head.to(dtype)
+                u = up[:n, 0].contiguous() if reduction == 'none' else torch.tensor(1.5, device='cuda')
+                want = gradients(-a, -b, label[:n], reduction, -u)
+                a, b = neg(a).requires_grad_(), neg(b).requires_grad_()
+                loss = ops.linear_cross_entropy(a, b, neg(-label[:n]), reduction=reduction)
+                got = (loss, *torch.autograd.grad(loss, (a, b), neg(u)))
+                assert all(torch.equal(p, q) for p, q in zip(got, want))
