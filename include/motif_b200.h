@@ -47,6 +47,8 @@ enum { MB_F32 = 0, MB_F16 = 1, MB_BF16 = 2 };
 MB_API const char* motif_b200_last_error(void);
 /* ABI version of this library (bumped on any signature change). */
 MB_API int motif_b200_abi_version(void);
+/* Kernels that this host thread has launched through the library so far. */
+MB_API int64_t motif_b200_launches(void);
 
 /* ------------------------------------------------------------------ gated delta rule
  * Layout of `strides` (elements), [18]:

@@ -9,6 +9,7 @@ dtype / alignment errors, `NotImplementedError` for shapes this build has no ker
 
 import ctypes
 import os
+import sys
 import threading
 
 import torch
@@ -30,6 +31,7 @@ _F = ctypes.c_float
 # name -> (restype, argtypes); must match include/motif_b200.h
 SIGNATURES = {
     'motif_b200_last_error': (ctypes.c_char_p, []),
+    'motif_b200_launches': (_I64, []),
     'motif_b200_abi_version': (_I, []),
     'motif_b200_gdn_recurrent': (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I, _P]),
     'motif_b200_gdn_chunk': (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I, _P]),
@@ -181,17 +183,18 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-# Kernels each entry point launches (for launch accounting); 0 = host-only query.
+# Kernels each entry point launches (for launch accounting); 0 = host-only query, None = as many as the call's
+# sizes ask for: the library's own count says.
 KERNELS_PER_CALL = {n: 1 for n in SIGNATURES}
-KERNELS_PER_CALL.update({'motif_b200_last_error': 0, 'motif_b200_abi_version': 0,
+KERNELS_PER_CALL.update({'motif_b200_last_error': 0, 'motif_b200_abi_version': 0, 'motif_b200_launches': 0,
                          'motif_b200_chord_workspace_bytes': 0, 'motif_b200_chord_decode_workspace_bytes': 0,
                          'motif_b200_skinny_packed_bytes': 0, 'motif_b200_gdn_chunk_workspace_bytes': 0,
                          'motif_b200_chord_backward_workspace_bytes': 0, 'motif_b200_gdn_backward_workspace_bytes': 0,
-                         'motif_b200_linear_cross_entropy_bytes': 0, 'motif_b200_linear_cross_entropy': 3,
-                         'motif_b200_linear_cross_entropy_backward': 7,
+                         'motif_b200_linear_cross_entropy_bytes': 0, 'motif_b200_linear_cross_entropy': None,
+                         'motif_b200_linear_cross_entropy_backward': None,
                          'motif_b200_linear_cross_entropy_train_workspace_bytes': 0,
-                         'motif_b200_linear_cross_entropy_train': 8,
-                         'motif_b200_rms_norm_backward_workspace_bytes': 0, 'motif_b200_rms_norm_backward': 2,
+                         'motif_b200_linear_cross_entropy_train': None,
+                         'motif_b200_rms_norm_backward_workspace_bytes': 0, 'motif_b200_rms_norm_backward': None,
                          'motif_b200_chord_backward': 2, 'motif_b200_kv4_chord_attention': 2,
                          'motif_b200_kv4_unit_bytes': 0, 'motif_b200_kv4_attention_workspace_bytes': 0,
                          'motif_b200_wait_timeouts': 0, 'motif_b200_testing_force': 0,
@@ -202,10 +205,15 @@ KERNELS_PER_CALL.update({'motif_b200_last_error': 0, 'motif_b200_abi_version': 0
 
 class Tracker:
     """Counts kernel launches and (optionally) times calls with CUDA events on the
-    current stream.  `timed` names the entry points to bracket with events (None = all)."""
+    current stream.  `timed` names the entry points to bracket with events (None = all).
+
+    The compiled operators (norms, SwiGLU, vocabulary loss) are timed under their own name, whichever of
+    their entry points a call takes; their backward passes are counted while the tracker is installed, not timed."""
 
     def __init__(self, timed=None, events=True):
-        self.launches = 0
+        self._calls = 0      # launched by calls
+        self._backward = 0   # by backward passes while installed, up to the last removal
+        self._since = None   # the backward passes' count when it was installed last
         self.timed = timed
         self.events = events
         self.records = []  # (name, start_event, end_event)
@@ -217,8 +225,20 @@ class Tracker:
             return ev
         return None
 
-    def stop(self, name, ev):
-        self.launches += KERNELS_PER_CALL.get(name, 1)
+    @property
+    def launches(self):
+        now = 0 if self._since is None else _backward_launches() - self._since
+        return self._calls + self._backward + now
+
+    def _install(self, on):
+        if on:
+            self._since = _backward_launches()
+        elif self._since is not None:
+            self._backward += _backward_launches() - self._since
+            self._since = None
+
+    def stop(self, name, ev, kernels=None):
+        self._calls += KERNELS_PER_CALL.get(name, 1) if kernels is None else kernels
         if ev is not None:
             end = torch.cuda.Event(enable_timing=True)
             end.record()
@@ -236,10 +256,20 @@ class Tracker:
 _tracker = None
 
 
+def _backward_launches():
+    """Kernels that the compiled operators' backward passes have launched (0 before the first of their calls)."""
+    host = sys.modules.get(__package__ + '._train_host')
+    return 0 if host is None else host.backward_launches()
+
+
 def set_tracker(tr):
     """Install (or remove with None) the launch tracker; returns the previous one."""
     global _tracker
     prev, _tracker = _tracker, tr
+    if prev is not None:
+        prev._install(False)
+    if tr is not None:
+        tr._install(True)
     return prev
 
 
@@ -247,10 +277,12 @@ def call(name: str, *args) -> None:
     """Call one entry point and raise on a nonzero status."""
     lib = load()
     tr = _tracker
-    ev = tr.start(name) if tr is not None else None
+    if tr is not None:
+        ev, before = tr.start(name), lib.motif_b200_launches()
     rc = getattr(lib, name)(*args)
     if tr is not None and rc == MB_OK:
-        tr.stop(name, ev)
+        kernels = lib.motif_b200_launches() - before if KERNELS_PER_CALL.get(name, 1) is None else None
+        tr.stop(name, ev, kernels)
     if rc != MB_OK:
         msg = lib.motif_b200_last_error().decode(errors='replace')
         if rc in (MB_ERR_ARG, MB_ERR_SHAPE, MB_ERR_DTYPE, MB_ERR_ALIGN):

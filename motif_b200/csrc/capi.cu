@@ -22,9 +22,13 @@ int set_error(int code, const char* fmt, ...) {
   return code;
 }
 
+// Kernels that this host thread has launched through the library.
+static thread_local int64_t g_launches = 0;
+
 int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(MB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  ++g_launches;
   g_last_error[0] = '\0';
   return MB_OK;
 }
@@ -139,3 +143,4 @@ extern "C" int motif_b200_testing_force(int knob, int value) {
 
 extern "C" const char* motif_b200_last_error(void) { return mb::g_last_error; }
 extern "C" int motif_b200_abi_version(void) { return 1; }
+extern "C" int64_t motif_b200_launches(void) { return mb::g_launches; }

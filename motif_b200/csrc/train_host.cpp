@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/engine.h>
 #include <torch/csrc/autograd/graph_task.h>
 
+#include <atomic>
 #include <string>
 
 #include "host.hpp"
@@ -19,6 +20,13 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
+
+// Kernels that backward passes have launched (on the autograd engine's threads), for launch trackers.
+std::atomic<int64_t> backward_kernels{0};
+struct Counted {
+  const int64_t before = motif_b200_launches();
+  ~Counted() { backward_kernels += motif_b200_launches() - before; }
+};
 
 bool grad_needed(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // A forward-mode tangent is refused, not dropped.
@@ -101,6 +109,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order();
+    const Counted counted;
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1];
     const bool gated = ctx->saved_data["gated"].toBool();
@@ -183,6 +192,7 @@ struct SwiGLUFunction : torch::autograd::Function<SwiGLUFunction> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order();
+    const Counted counted;
     const Tensor x = ctx->get_saved_variables()[0];
     const c10::Device dev = grads[0].device();
     const c10::cuda::CUDAGuard guard(dev);
@@ -306,6 +316,7 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order();
+    const Counted counted;
     const variable_list saved = ctx->get_saved_variables();
     const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
     const int64_t reduction = ctx->saved_data["reduction"].toInt();
@@ -397,8 +408,12 @@ PyObject* loss(PyObject* const* a) {
   return wrap(out);
 }
 
+// Kernels launched by backward passes so far.
+PyObject* backward_launches(PyObject* const*) { return PyLong_FromLongLong(backward_kernels.load()); }
+
 PyMethodDef methods[] = {method<norm, 4>("rms_norm"), method<swiglu, 1>("swiglu"),
-                         method<loss, 5>("linear_cross_entropy"), {nullptr, nullptr, 0, nullptr}};
+                         method<loss, 5>("linear_cross_entropy"), method<backward_launches, 0>("backward_launches"),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_train_host", nullptr, -1, methods};
 
 }  // namespace

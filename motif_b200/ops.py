@@ -260,7 +260,8 @@ _host = None
 
 def _compiled(name, *args):
     """One call of the compiled entry points (checks, outputs, the C ABI call and the autograd node),
-    counted and timed by a launch tracker like `_lib.call`'s."""
+    counted and timed by a launch tracker like `_lib.call`'s (what it launches depends on its sizes and on what
+    needs a gradient: the library's own count)."""
     global _host
     if _host is None:
         _lib.load()
@@ -273,9 +274,10 @@ def _compiled(name, *args):
     tr = _lib._tracker
     if tr is None:
         return getattr(_host, name)(*args)
-    ev = tr.start('motif_b200_' + name)
+    launches = _lib.load().motif_b200_launches
+    ev, before = tr.start('motif_b200_' + name), launches()
     out = getattr(_host, name)(*args)
-    tr.stop('motif_b200_' + name, ev)
+    tr.stop('motif_b200_' + name, ev, launches() - before)
     return out
 
 

@@ -123,3 +123,55 @@ def test_views_that_are_negated_lazily():
                 loss = ops.linear_cross_entropy(a, b, neg(-label[:n]), reduction=reduction)
                 got = (loss, *torch.autograd.grad(loss, (a, b), neg(u)))
                 assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def launched(f):
+    tr = _lib.Tracker(events=False)
+    before = _lib.set_tracker(tr)
+    try:
+        f()
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_tracker(before)
+    count = tr.launches
+    f()  # not counted any more
+    assert tr.launches == count
+    return count
+
+
+def test_a_tracker_counts_the_kernels_that_ran():
+    """bf16 loss: packed rows, scores, join; with gradients scores, settled rows, their second form, and for dx and dW a
+    product and a join of split sums each, for every run of rows.  fp16 and `none`: the backward pass computes scores."""
+    g = torch.Generator(device='cuda').manual_seed(1)
+
+    def loss(N, V, dtype, reduction, grads, d=64, shift=0):
+        x = torch.randn(N, d, device='cuda', generator=g).to(dtype).requires_grad_('x' in grads)
+        w = torch.randn(V, d + shift, device='cuda', generator=g).to(dtype)[:, shift:].requires_grad_('w' in grads)
+        label = torch.randint(0, V, (N,), device='cuda', generator=g)
+
+        def run():
+            out = ops.linear_cross_entropy(x, w, label, reduction=reduction)
+            if 'b' in grads:
+                out.sum().backward()
+        return launched(run)
+
+    bf16, fp32 = torch.bfloat16, torch.float32
+    assert loss(300, 1000, bf16, 'none', '') == loss(300, 1000, bf16, 'mean', '') == 3
+    assert loss(300, 1000, bf16, 'mean', '', shift=1) == 4    # the weight is packed
+    assert loss(9000, 1000, bf16, 'mean', '') == 4            # the labels are counted first
+    assert loss(300, 1000, bf16, 'mean', 'xw') == 8
+    assert loss(300, 1000, bf16, 'mean', 'x') == loss(300, 1000, bf16, 'mean', 'w') == 6
+    assert loss(9000, 33000, bf16, 'mean', 'xw') == 2 + 2 * 7  # two runs of 7936 rows
+    assert loss(300, 1000, bf16, 'mean', 'xwb') == 8 + 1       # and the product with what arrives
+    assert loss(300, 1000, bf16, 'none', 'xwb') == 3 + 6
+    assert loss(300, 1000, fp32, 'mean', 'xwb') == 9 + 1
+    assert loss(9, 1000, fp32, 'mean', 'xwb') == 3 + 3 + 1
+
+    x = torch.randn(50, 128, device='cuda', generator=g)
+    w = torch.ones(128, device='cuda', requires_grad=True)
+    xl = x.clone().requires_grad_()
+    assert launched(lambda: ops.rms_norm(x, w.detach())) == 1
+    assert launched(lambda: ops.rms_norm(xl, w)) == 1
+    assert launched(lambda: ops.rms_norm(xl, w).sum().backward()) == 1 + 2
+    assert launched(lambda: ops.rms_norm(xl, w.detach()).sum().backward()) == 1 + 1
+    assert launched(lambda: ops.swiglu(xl).sum().backward()) == 1 + 1
