@@ -631,9 +631,12 @@ int launch_norm(const NormArgs& a, const Plan& p, cudaStream_t st) {
   integral_constant<int, 4> n4;
   if (p.way == kByRows)
     norm_long_kernel<T, GATED, BWD><<<p.grid, kThreads, 0, st>>>(a);
-  else if (p.way == kByElements)
-    rc = p.g == 32 ? (p.n == 8 ? some(c32, c8) : p.n == 16 ? some(c32, c16) : some(c32, c32))
-                   : (p.n == 8 ? some(all, c8) : p.n == 16 ? some(all, c16) : some(all, c32));
+  else if (p.way == kByElements && p.g == 32)
+    rc = p.n == 8 ? some(c32, c8) : p.n == 16 ? some(c32, c16) : some(c32, c32);
+  else if (p.way == kByElements) {
+    if constexpr (BWD)  // (longer rows go forward a CTA at a time)
+      rc = p.n == 8 ? some(all, c8) : p.n == 16 ? some(all, c16) : some(all, c32);
+  }
   else if (p.g == 8)
     rc = rows(c8, n1);
   else if (p.g == 16)
