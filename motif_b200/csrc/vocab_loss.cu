@@ -483,6 +483,14 @@ __host__ __device__ __forceinline__ int64_t range_owner(int64_t t, int64_t tiles
   return ((t + 1) * np - 1) / tiles;
 }
 
+// 16-bit operands' exponentials are 2^(s log2 e - m), one multiply-add each, with m = top log2 e rounded: what that
+// rounding takes off is the same for a whole row, and is put back where the row's sum or divisor leaves.  (Left out, a
+// loss is off by half a unit of m: 4e-5 for logits near 1000.)
+__device__ __forceinline__ float lost_of(float top) {
+  const float m = __fmul_rn(top, kLog2e);
+  return fabsf(m) < INFINITY ? fmaf(top, kLog2e, -m) : 0.f;
+}
+
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_constant__ CUtensorMap tmX,
                                                              const __grid_constant__ CUtensorMap tmX32,
@@ -596,12 +604,13 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
         const float now = fmax3(fmax3(t8[0], t8[1], t8[2]), fmax3(t8[3], t8[4], t8[5]), fmaxf(t8[6], t8[7]));
         const bool raise = MODE == kLoss ? now > top : mine && now > top + kFar;  // (rows behind the last hold anything)
         if (__any_sync(0xffffffffu, raise) && raise) {
-          sum *= ex2f_((top - now) * kLog2e);  // 0 from a reference of -inf
+          // (0 from a reference of -inf)
+          sum *= ex2f_(P == 1 ? __fsub_rn(__fmul_rn(top, kLog2e), __fmul_rn(now, kLog2e)) : (top - now) * kLog2e);
           top = now;
           if (MODE == kOnce) *a.flag = 1;
         }
       }
-      // (s - top) log2 e: as one multiply-add where the type's own rounding is coarser than the product top log2 e
+      // (s - top) log2 e: for 16-bit operands as one multiply-add (`lost_of`)
       const float ref = MODE != kAgain && top == -INFINITY ? 0.f : top;  // (kOnce: the label's logit may be -inf)
       const float2 c2 = make_float2(kLog2e, kLog2e), n2 = make_float2(-ref, -ref);
       const float2 m2 = make_float2(-ref * kLog2e, -ref * kLog2e), i2 = make_float2(inv, inv);
@@ -663,12 +672,15 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
         }
       }
     };
+    auto run_ends = [&] {
+      a.seg[((int64_t)(pair + m_now) * 2 + half) * kTile + in_tile] =
+          make_float2(top, P == 1 ? sum * ex2f_(-lost_of(top)) : sum);
+    };
     for (int64_t t = t0; t < t1; ++t, ++done) {
       const int m = (int)(t / nt), n = (int)(t - (int64_t)m * nt);
       const int row = a.row0 + m * kTile + in_tile;
       if (m != m_now) {
-        if (MODE != kAgain && m_now >= 0)
-          a.seg[((int64_t)(pair + m_now) * 2 + half) * kTile + in_tile] = make_float2(top, sum);
+        if (MODE != kAgain && m_now >= 0) run_ends();
         m_now = m;
         mine = m * kTile + in_tile < live;
         label = mine ? a.label[row] : -1;
@@ -681,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
             g = a.up ? a.up[a.index[row] * a.up_stride] * a.scale[1] : 1.0f;
             if constexpr (std::is_same<T, __half>::value) g *= kHalfScale;
             top = st.top;
-            inv = st.inv * g;
+            inv = P == 1 ? st.inv * g * ex2f_(-lost_of(top)) : st.inv * g;
           }
         }
       }
@@ -705,8 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
       __syncwarp();
     }
-    if (MODE != kAgain && m_now >= 0)
-      a.seg[((int64_t)(pair + m_now) * 2 + half) * kTile + in_tile] = make_float2(top, sum);
+    if (MODE != kAgain && m_now >= 0) run_ends();
   }
   pair_end(tmem);
 }
@@ -869,7 +880,13 @@ __global__ void __launch_bounds__(32 * kSettleRows) settle_kernel(const SettleAr
     const float inv = 1.0f / (sum + own);
     loss = own > 0.5f ? log1pf(sum / own) : (top - target) + logf(sum + own);
     float scale = flagged && label >= 0 ? 1.0f : inv;
-    if (P == 1 && !flagged && sum > 1e-30f && sum < 1e30f) scale *= sum / to_f(from_f<O>(sum));
+    float others = sum;  // as E holds them
+    if (P == 1 && !flagged) {
+      const float lost = lost_of(ref);
+      others *= ex2f_(lost);
+      scale *= ex2f_(-lost);
+      if (sum > 1e-30f && sum < 1e30f) scale *= others / to_f(from_f<O>(others));
+    }
     if (lane == 0) {
       RowStat st;
       st.top = top;
@@ -879,10 +896,10 @@ __global__ void __launch_bounds__(32 * kSettleRows) settle_kernel(const SettleAr
       if (!flagged && label >= 0) {
         O* e = reinterpret_cast<O*>(a.e) + (int64_t)r * a.ld + label;
         if constexpr (P == 1) {
-          *e = from_f<O>(-sum);
+          *e = from_f<O>(-others);
         } else {
           __nv_bfloat16 p[3];
-          split3(-sum, p);
+          split3(-others, p);
           for (int i = 0; i < 3; ++i) e[i * a.w_part * a.ld] = p[i];
         }
       }

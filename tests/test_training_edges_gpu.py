@@ -175,3 +175,26 @@ def test_a_tracker_counts_the_kernels_that_ran():
     assert launched(lambda: ops.rms_norm(xl, w).sum().backward()) == 1 + 2
     assert launched(lambda: ops.rms_norm(xl, w.detach()).sum().backward()) == 1 + 1
     assert launched(lambda: ops.swiglu(xl).sum().backward()) == 1 + 1
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_losses_of_logits_far_from_zero(dtype):
+    """Logits z + w_v with z of 500 to 1000 and w_v multiples of 1 / 16 below 8: products and sums are exact in fp32, and z
+    cancels.  What is left, in units e of the loss (|z + w - top| < 16, 24 in powers of two): the exponent's rounding 24
+    ln 2 e, log2 e's own 4 e, ex2's 4 e, the sum's V / 32 + 64 e, the logarithm's and the last two sums' 16 e each."""
+    V, N = 300, 90
+    g = torch.Generator(device='cuda').manual_seed(3)
+    z = 500 + 4 * torch.randint(0, 126, (N,), device='cuda', generator=g)
+    own = torch.randint(-127, 128, (V,), device='cuda', generator=g) / 16
+    x, w = torch.zeros(N, 8, device='cuda'), torch.zeros(V, 8, device='cuda')
+    x[:, 0], x[:, 1], w[:, 0], w[:, 1] = z, 1, 1, own
+    x, w = x.to(dtype), w.to(dtype)
+    assert torch.equal(x[:, 0].float(), z.float()) and torch.equal(w[:, 1].float(), own)
+    label = torch.randint(0, V, (N,), device='cuda', generator=g)
+    want = own.double().logsumexp(0) - own.double()[label]
+    bound = (17 + 4 + 4 + V / 32 + 64 + 48) * E
+    with torch.no_grad():
+        got = ops.linear_cross_entropy(x, w, label, reduction='none')
+    assert (got.double() - want).abs().max() <= bound, (got.double() - want).abs().max() / E
+    each = torch.stack([gradients(x[i:i + 1], w, label[i:i + 1], 'sum')[0] for i in range(N)])
+    assert (each.double() - want).abs().max() <= bound, (each.double() - want).abs().max() / E
