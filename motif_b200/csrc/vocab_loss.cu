@@ -237,6 +237,51 @@ __device__ __forceinline__ void read32_wait(bool lost, uint32_t (&r)[32]) {
   if (!lost) tmem_wait_ld(r);
 }
 
+// fp32: a sum leaves the tensor cores every 512 terms, since they cut each partial sum off at 24 bits; what has left
+// adds up in the other half of the TMEM (dx of 512 tokens, 1024 features and 32000 words: error 4.4e-6 with 3556 terms
+// at a time, 6.8e-7; a logit of 16384 positive products: 6.8e-5 of it all at once, 4.6e-7).
+constexpr int kFlush = 8;  // stages
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// A warp of the tile's end: a part of the sum that is not its last, for the columns first, first + step, .. < end (32 at
+// a time) of the warp's lanes.  `more`: parts have left before.
+__device__ __forceinline__ void keep_part(const Smem& s, int done, bool& lost, bool leader, uint32_t lanes, int first, int end,
+                                          int step, bool more) {
+  tile_ready<1>(s, done, lost);
+#pragma unroll 1
+  for (int col = first; col < end; col += step) {
+    uint32_t r[32], o[32];
+    read32(lanes + col, lost, r);
+    if (more) read32(lanes + kTile + col, lost, o);
+    read32_wait(lost, r);
+    if (more) read32_wait(lost, o);
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) + (more ? __uint_as_float(o[i]) : 0.f);
+    if (!lost) tmem_st32(lanes + kTile + col, v);
+  }
+  asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+  tile_read<1>(s, done, lost, leader);
+}
+// 32 columns of the last part with what has left before.
+__device__ __forceinline__ void add_parts(uint32_t lanes, int col, bool lost, uint32_t (&r)[32]) {
+  uint32_t o[32];
+  read32(lanes + kTile + col, lost, o);
+  read32_wait(lost, o);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(o[i]));
+}
+
 // ------------------------------------------------------------------------------- packing
 struct PackArgs {
   const void* x;           // [N, d], rows xs apart
@@ -491,7 +536,10 @@ __device__ __forceinline__ float lost_of(float top) {
   return fabsf(m) < INFINITY ? fmaf(top, kLog2e, -m) : 0.f;
 }
 
-template <typename T, int MODE>
+// LONG (fp32, more than 512 features): the sums leave the tensor cores in parts, so one tile has all of the TMEM and the
+// next one waits for its end (4096 x 768 x 32000, loss 914 -> 964 us, with gradients 2905 -> 2973; the losses' error 3.7e-7 ->
+// 2.0e-7, at 4096 features 2.3e-6 -> 2.3e-7).
+template <typename T, int MODE, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_constant__ CUtensorMap tmX,
                                                              const __grid_constant__ CUtensorMap tmX32,
                                                              const __grid_constant__ CUtensorMap tmW,
@@ -499,6 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
                                                              const ScoreArgs a) {
   using O = Op<T>;
   constexpr int P = kParts<T>;
+  static_assert(!LONG || P > 1, "16-bit operands' sums stay in the tensor cores");
+  constexpr int kBufs = LONG ? 1 : 2, kTake = LONG ? kFlush : 1 << 30;
   extern __shared__ unsigned char raw[];
   const Smem s = carve(raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -527,8 +577,9 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
         const int xr = a.row0 + m * kTile + 128 * (int)rank, wr = a.v0 + n * kTile + 128 * (int)rank;
         const int rows = live - m * kTile, boxes = boxes_of(rows, rank);
         const uint32_t bytes = 4096 * (boxes_of(rows, 0) + boxes_of(rows, 1)) + 2 * kOperand;
+        for (int k0 = 0; k0 < a.kblocks && !failed; k0 += kTake)
         for (int p = 0; p < Parts<P>::n && !failed; ++p)
-          for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
+          for (int kb = k0; kb < min(a.kblocks, k0 + kTake); ++kb, ++it) {
             uint32_t bar;
             unsigned char* st = stage_begin(s, it, leader, bytes, bar);
             if (!st) {
@@ -548,11 +599,13 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
           umma_idesc_f16(std::is_same<O, __nv_bfloat16>::value ? 1u : 0u, kTile, kTile, 0, 0);
       int it = 0, done = 0;
       bool failed = false;
-      for (int64_t t = t0; t < t1 && !failed; ++t, ++done) {
-        failed = !tile_free<2>(s, done) ||
-                 !issue_tile<false, false>(s, tmem + (uint32_t)((done & 1) * kTile), idesc, Parts<P>::n * a.kblocks, it);
-        if (!failed) tile_issued<2>(s, done);
-      }
+      for (int64_t t = t0; t < t1 && !failed; ++t)
+        for (int k0 = 0; k0 < a.kblocks && !failed; k0 += kTake, ++done) {
+          failed = !tile_free<kBufs>(s, done) ||
+                   !issue_tile<false, false>(s, tmem + (uint32_t)(done % kBufs * kTile), idesc,
+                                             Parts<P>::n * min(kTake, a.kblocks - k0), it);
+          if (!failed) tile_issued<kBufs>(s, done);
+        }
       issue_end(s, failed);
     }
     __syncwarp();
@@ -699,9 +752,13 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
       }
       const int at = label - (a.v0 + n * kTile);  // the label's column, if it is in this tile
       const int valid = a.nv - n * kTile;         // columns of the tile that are words
-      const uint32_t taddr = tmem + (uint32_t)((done & 1) * kTile) + ((uint32_t)(q * 32) << 16);
       const int x = n * kTile, y = m * kTile + (int)rank * 128 + q * 32;
-      tile_ready<2>(s, done, lost);
+      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+      if constexpr (LONG)
+        for (int k0 = 0; k0 + kTake < a.kblocks; k0 += kTake, ++done)
+          keep_part(s, done, lost, leader, lanes, c0, c0 + kTile / 2, 32, k0 > 0);
+      const uint32_t taddr = lanes + (uint32_t)(done % kBufs * kTile);
+      tile_ready<kBufs>(s, done, lost);
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         uint32_t r0[32], r1[32];
@@ -709,7 +766,11 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
         read32(taddr + c0 + 64 * h + 32, lost, r1);
         read32_wait(lost, r0);
         read32_wait(lost, r1);
-        if (h == 1) tile_read<2>(s, done, lost, leader);  // the tile is in registers: the next one may come
+        if constexpr (LONG) {  // (there has been a part before: more features than one holds)
+          add_parts(lanes, c0 + 64 * h, lost, r0);
+          add_parts(lanes, c0 + 64 * h + 32, lost, r1);
+        }
+        if (h == 1) tile_read<kBufs>(s, done, lost, leader);  // the tile is in registers: the next one may come
         block(r0, r1, c0 + 64 * h, at, valid, row, x, y);
       }
     }
@@ -1147,22 +1208,6 @@ __device__ __forceinline__ void finish32(const ProductArgs& a, int row, int rows
   }
 }
 
-// fp32: a sum leaves the tensor cores every 512 terms, since they cut each partial sum off at 24 bits; what has left
-// adds up in the other half of the TMEM (dx of 512 tokens, 1024 features and 32000 words: error 4.4e-6 with 3556 terms
-// at a time, 6.8e-7).
-constexpr int kFlush = 8;  // stages
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
-  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-
 // A_MN: the left operand's summed dimension runs along its rows (dW); the right one's always does.
 template <typename T, bool A_MN>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ CUtensorMap tmA,
@@ -1258,22 +1303,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       bool more = false;  // parts of this sum have left before
       if constexpr (P > 1)
         for (int k0 = w.k0; k0 + kTake < w.k1; k0 += kTake, ++done) {
-          tile_ready<kBufs>(s, done, lost);
-#pragma unroll 1
-          for (int col = half * 32; col < cols; col += 64) {
-            uint32_t r[32], o[32];
-            read32(lanes + col, lost, r);
-            if (more) read32(lanes + kTile + col, lost, o);
-            read32_wait(lost, r);
-            if (more) read32_wait(lost, o);
-            float v[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) + (more ? __uint_as_float(o[i]) : 0.f);
-            if (!lost) tmem_st32(lanes + kTile + col, v);
-          }
-          asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+          keep_part(s, done, lost, leader, lanes, half * 32, cols, 64, more);
           more = true;
-          tile_read<kBufs>(s, done, lost, leader);
         }
       const uint32_t taddr = lanes + (uint32_t)(done % kBufs * kTile);
       if (c.kb > 0) tile_ready<kBufs>(s, done, lost);
@@ -1287,15 +1318,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 #pragma unroll
           for (int i = 0; i < 32; ++i) r[i] = 0u;
         }
+        if (P > 1 && more) add_parts(lanes, col, lost, r);
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if (P > 1 && more) {
-          read32(lanes + kTile + col, lost, r);
-          read32_wait(lost, r);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(r[i]);
-        }
         if (w.slot >= 0) {  // [slot][four columns][row]: the warp's rows lie next to each other
           float4* p = a.slots + ((int64_t)w.slot * (kTile / 4) + col / 4) * kTile + in_tile;
 #pragma unroll
@@ -1516,6 +1542,15 @@ struct Call {
 };
 template <typename T> T* at(unsigned char* base, int64_t off) { return reinterpret_cast<T*>(base + off); }
 
+// The scores' kernel of a call.
+template <typename T, int MODE>
+int launch_scores(const char* what, int np, cudaStream_t st, const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& w,
+                  const CUtensorMap& g, const ScoreArgs& a) {
+  if constexpr (kParts<T> > 1)
+    if (a.kblocks > kFlush) return launch_pairs(what, scores_kernel<T, MODE, true>, np, st, x, x32, w, g, a);
+  return launch_pairs(what, scores_kernel<T, MODE, false>, np, st, x, x32, w, g, a);
+}
+
 // The weight as rows for the tensor maps: itself, or its packed copy.
 void weight_rows(const Call& c, const void** base, int64_t* rows, int64_t* stride, int64_t* cols) {
   *base = c.pack_w ? c.state + c.s.w : c.w;
@@ -1583,7 +1618,7 @@ int forward(const Call& c, float* loss) {
   a.label = p.label;
   a.seg = at<float2>(c.work, s.seg);
   a.target = at<float>(c.work, s.target);
-  rc = launch_pairs("linear_cross_entropy (scores)", scores_kernel<T, kLoss>, c.np, c.st, tmX, tmX32, tmW, tmX, a);
+  rc = launch_scores<T, kLoss>("linear_cross_entropy (scores)", c.np, c.st, tmX, tmX32, tmW, tmX, a);
   if (rc) return rc;
   JoinArgs j = {};
   j.count = p.count;
@@ -1646,8 +1681,7 @@ int backward(const Call& c, const float* up, int64_t up_stride, void* dx, void* 
       a.up_stride = up_stride;
       a.scale = scale;
       a.g_part = s.run;
-      rc = launch_pairs("linear_cross_entropy_backward (scores)", scores_kernel<T, kAgain>, c.np, c.st, tmX, tmX32,
-                        tmW, tmG, a);
+      rc = launch_scores<T, kAgain>("linear_cross_entropy_backward (scores)", c.np, c.st, tmX, tmX32, tmW, tmG, a);
       if (rc) return rc;
       ProductArgs p = {};
       p.steps = Parts<kParts<T>>::n;
@@ -1752,7 +1786,7 @@ int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
     a.stat = at<RowStat>(ws, s.stat);
     a.index = p.index;
     a.g_part = s.run;
-    rc = launch_pairs("linear_cross_entropy_train (scores)", scores_kernel<T, kOnce>, c.np, c.st, tmX, tmX32, tmW, tmE, a);
+    rc = launch_scores<T, kOnce>("linear_cross_entropy_train (scores)", c.np, c.st, tmX, tmX32, tmW, tmE, a);
     if (rc) return rc;
     SettleArgs b = {};
     b.count = p.count;
@@ -1780,7 +1814,7 @@ int once(const Call& c, const OnceSizes& s, float* loss, void* dx, void* dw) {
     b.ld = s.vrows;
     rc = launch("linear_cross_entropy_train (settle)", settle_kernel<T>, a.rows / kSettleRows, 32 * kSettleRows, c.st, 0, 1, b);
     if (!rc)
-      rc = launch_pairs("linear_cross_entropy_train (again)", scores_kernel<T, kAgain>, c.np, c.st, tmX, tmX32, tmW, tmE, a);
+      rc = launch_scores<T, kAgain>("linear_cross_entropy_train (again)", c.np, c.st, tmX, tmX32, tmW, tmE, a);
     if (rc) return rc;
     ProductArgs q = {};
     q.steps = Parts<kParts<T>>::n;

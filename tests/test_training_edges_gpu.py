@@ -198,3 +198,26 @@ def test_losses_of_logits_far_from_zero(dtype):
     assert (got.double() - want).abs().max() <= bound, (got.double() - want).abs().max() / E
     each = torch.stack([gradients(x[i:i + 1], w, label[i:i + 1], 'sum')[0] for i in range(N)])
     assert (each.double() - want).abs().max() <= bound, (each.double() - want).abs().max() / E
+
+
+@pytest.mark.parametrize('N', [20, 300])
+def test_fp32_scores_of_many_features(N):
+    """One word's logit is a sum of 16384 positive products, the others' are 0: the loss is that sum.  512 terms at a time
+    are cut off at 24 bits (2 e) once for 16 of them, the six products of parts add 4 such ends and lose 4 e; then 32 sums
+    are added with a rounding each, and the loss is rounded."""
+    d, V = 16384, 300
+    g = torch.Generator(device='cuda').manual_seed(N)
+    x = 0.5 + torch.rand(N, d, device='cuda', generator=g)
+    w = torch.zeros(V, d, device='cuda')
+    w[0] = 0.03 + 0.06 * torch.rand(d, device='cuda', generator=g)
+    label = torch.randint(1, V, (N,), device='cuda', generator=g)
+    want = x.double() @ w[0].double()
+    bound = (2 * (512 / 16 + 4) + 4 + 32 + 4) * E * want
+    with torch.no_grad():
+        got = ops.linear_cross_entropy(x, w, label, reduction='none')
+    assert ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() / want).max() / E
+    loss = gradients(x, w, label, 'sum')[0]
+    assert abs(loss.item() - want.sum().item()) <= (bound.sum() + 2 * E * want.sum()).item()
+    got = gradients(x, w, label, 'none')  # G is -1 at the label and 1 at word 0: dW's row there is the sum of x
+    total = x.double().sum(0)
+    assert ((got[2][0].double() - total).abs() <= (2 * (N / 16 + 8) + 8) * E * total).all()
