@@ -221,3 +221,76 @@ def test_fp32_scores_of_many_features(N):
     got = gradients(x, w, label, 'none')  # G is -1 at the label and 1 at word 0: dW's row there is the sum of x
     total = x.double().sum(0)
     assert ((got[2][0].double() - total).abs() <= (2 * (N / 16 + 8) + 8) * E * total).all()
+
+
+def test_transforms_are_refused():
+    """Forward-mode tangents, vmap, torch.func's gradients and batched upstream gradients: an error, never a number."""
+    from torch.autograd import forward_ad as fw
+
+    x = torch.randn(6, 64, device='cuda')
+    w, half = torch.ones(64, device='cuda'), torch.ones(32, device='cuda')
+    head, label = torch.randn(100, 64, device='cuda') * 0.2, torch.arange(6, device='cuda')
+    calls = [lambda x: ops.rms_norm(x, w), lambda x: ops.gated_rms_norm(x, half), ops.swiglu,
+             lambda x: ops.linear_cross_entropy(x, head, label[:x.shape[0]]),
+             lambda x: ops.linear_cross_entropy(x, head, label[:x.shape[0]], reduction='none')]
+    for f in calls:
+        for grad in (False, True):
+            with fw.dual_level(), pytest.raises(NotImplementedError, match='forward-mode'):
+                f(fw.make_dual(x.clone().requires_grad_(grad), torch.ones_like(x)))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x.expand(3, 6, 64).clone())
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).sum())(x)
+        xl = x.clone().requires_grad_()
+        y = f(xl)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, xl, torch.ones(2, *y.shape, device='cuda'), is_grads_batched=True)
+    for f, t in ((lambda w: ops.rms_norm(x, w), w), (lambda w: ops.linear_cross_entropy(x, w, label), head)):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).sum())(t)
+        with fw.dual_level(), pytest.raises(NotImplementedError, match='forward-mode'):
+            f(fw.make_dual(t, torch.ones_like(t)))
+    assert ops.rms_norm(x, w).isfinite().all()  # and the calls after those are as ever
+
+
+def test_weight_gradients_past_32_bits():
+    """Only the first and the last rows, the latter past 2^31 elements, have a gradient: dW is that of those rows alone,
+    but for the order of its sums (a bound of fp32's: terms one after another, on the sum of magnitudes)."""
+    rows, dim = (1 << 31) // 768 + 1000, 768
+    x = torch.empty(rows, dim, dtype=torch.bfloat16, device='cuda').normal_(generator=torch.Generator('cuda').manual_seed(1))
+    w = torch.ones(dim, device='cuda').requires_grad_()
+    dy = torch.zeros(rows, dim, dtype=torch.bfloat16, device='cuda')
+    some = torch.cat([torch.arange(40), torch.arange(rows - 900, rows)]).cuda()
+    assert (rows - 900) * dim > 1 << 31
+    dy[some] = torch.randn(940, dim, device='cuda', generator=torch.Generator('cuda').manual_seed(2)).to(dy.dtype)
+    dw, = torch.autograd.grad(ops.rms_norm(x, w), w, dy)
+    xs, ds = x[some].double(), dy[some].double()
+    terms = ds * xs * torch.rsqrt(xs.square().mean(1, keepdim=True) + 1e-6)
+    # r and the products (dim / 32 + 40) e each as in the norms' own tests, up to 940 terms in a row
+    assert ((dw.double() - terms.sum(0)).abs() <= (dim / 32 + 40 + 940) * E * terms.abs().sum(0)).all()
+    del x, dy, dw
+
+    tokens, dim, vocab = (1 << 31) // 1024 + 700, 1024, 100
+    x = torch.empty(tokens, dim, dtype=torch.bfloat16, device='cuda').normal_(generator=torch.Generator('cuda').manual_seed(3))
+    w = (0.05 * torch.randn(vocab, dim, device='cuda')).to(torch.bfloat16).requires_grad_()
+    label = torch.randint(0, vocab, (tokens,), device='cuda')
+    up = torch.zeros(tokens, device='cuda')
+    some = torch.cat([torch.arange(30), torch.arange(tokens - 600, tokens)]).cuda()
+    assert (tokens - 600) * dim > 1 << 31
+    up[some] = 1
+    # all tokens have a loss: packed rows past 2^31 elements
+    dw, = torch.autograd.grad(ops.linear_cross_entropy(x, w, label, reduction='none'), w, up)
+    want, = torch.autograd.grad(ops.linear_cross_entropy(x[some], w, label[some], reduction='none'), w, up[some])
+    xs = x[some].double()
+    G = torch.softmax(xs @ w.double().t(), 1)
+    G[torch.arange(630), label[some]] -= 1
+    size = G.abs().t() @ xs.abs()
+    # the same roundings of the same G (its logits' sums are those of one tile either way); sums cut off once for 16
+    # terms; and each of the two results is within half a step of its sum, 2^-8 of that, so they are 2 x 2^-8 apart
+    bound = 2.02 * 2.0 ** -8 * want.double().abs() + 4 * E * (630 / 16 + 8 + 2) * size
+    assert ((dw.double() - want.double()).abs() <= bound).all()
+    # and all others ignored: the last rows are packed to the front
+    label[:tokens - 600] = -100
+    dw, = torch.autograd.grad(ops.linear_cross_entropy(x, w, label, reduction='sum'), w)
+    want, = torch.autograd.grad(ops.linear_cross_entropy(x[-600:], w, label[-600:], reduction='sum'), w)
+    assert torch.equal(dw, want)
