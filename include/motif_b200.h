@@ -195,8 +195,9 @@ MB_API int motif_b200_swiglu_backward(const void* x, const void* dy, void* dx, i
  *
  * The forward pass leaves in `state` what the backward pass needs (the same values of w, N, V, d, dtype and
  * reduction); `workspace` is scratch.  Both are device memory at 256-byte boundaries;
- * motif_b200_linear_cross_entropy_bytes writes three sizes to host memory: the state, the forward
- * workspace and the backward workspace (the latter at most about 0.35 GB and one fp32 copy of dw).
+ * motif_b200_linear_cross_entropy_bytes writes three sizes to host memory: the state, the forward workspace and the
+ * backward workspace.  The latter is at most 0.34 GB, an fp32 copy of dw where N is more than 8192 (fp32: 4096), and
+ * fp32 sums of dx, of 8192 (fp32: 4096) rows at most, where V is more than 16384 (fp32: 10752).
  * A 16-bit weight whose rows do not begin at 16-byte boundaries is copied into the state by the forward pass, and the
  * backward pass reads that copy.  The state's size says so: hand the backward pass, as state_bytes, exactly what was
  * asked for the forward pass's w and ws (another size is refused).  Where there is no copy, w may lie elsewhere by then
@@ -215,8 +216,12 @@ MB_API int motif_b200_linear_cross_entropy_backward(const void* w, int64_t ws, c
 
 /* The loss (reduction 1 or 2) with the gradients that it has when the gradient arriving at it is 1, in one pass over
  * the logits (bf16 and fp32); dx and dw as above, either may be NULL.  Workspace of
- * motif_b200_linear_cross_entropy_train_workspace_bytes(...) bytes (-1: bad sizes) at a 256-byte boundary, at most
- * about 0.6 GB, a copy of x (fp32: and of w, one and a half times as large) and one fp32 copy of dw. */
+ * motif_b200_linear_cross_entropy_train_workspace_bytes(...) bytes (-1: bad sizes) at a 256-byte boundary: a copy of x and
+ * its rows' statistics (64 bytes each), a copy of w in fp32 and where its rows do not begin at 16-byte boundaries (fp32
+ * copies are one and a half times as large), and for r = min(N, 65536, 2^28 / V) rows at a time (fp32: a third of
+ * 2^28 / V; never less than 256) their V exponentials, 0.54 GB up to a million words (fp32: 349000), and
+ * a second copy of those rows of x; 0.06 GB of partial sums; an fp32 copy of dw where N is more than r; and fp32 sums of dx
+ * for r rows where a 16-bit type has more than 65536 words. */
 MB_API int64_t motif_b200_linear_cross_entropy_train_workspace_bytes(const void* w, int64_t ws, int64_t N, int64_t V,
                                                               int64_t d, int dtype);
 MB_API int motif_b200_linear_cross_entropy_train(const void* x, int64_t xs, const void* w, int64_t ws,

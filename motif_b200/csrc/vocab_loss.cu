@@ -1457,7 +1457,7 @@ struct OnceSizes {
   int64_t e, weighed, slots, dx_acc, dw_acc, cut, bytes;
 };
 // Elements of E that are there at once: a run of rows with the whole vocabulary (fp32: three parts of a third
-// as many).
+// as many), or 256 rows of a vocabulary so large that they have more.
 constexpr int64_t kOnceElements = 1LL << 28;
 // 16-bit: terms that are added within the tensor cores, which cut each partial sum off at 24 bits (2^16 / 16
 // of them: 2^-12 of the result at most, half a unit of bf16 being 2^-9).

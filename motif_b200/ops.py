@@ -381,9 +381,15 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     pass over the logits; a call whose loss is not differentiated belongs under `torch.no_grad()`,
     where it computes the loss alone.  With `none`, and in fp16, the backward pass computes the logits
     again.  16-bit gradients are sums in fp32 over probabilities rounded to the type (and, for
-    the weight's, rows of x divided by their sums and rounded).  Memory beyond the results: a copy of
-    x's rows, and during a pass that computes gradients 0.6 GB at most and an fp32 copy of the weight's;
-    in fp32 also x and weight as three bf16 parts (6 bytes a value), or for 16 tokens or less the logits.
+    the weight's, rows of x divided by their sums and rounded).  Where the gradients are computed with the
+    loss they are rounded to x's dtype as for a loss that is differentiated itself, and once more when they are
+    multiplied with a gradient other than 1 that arrives.
+
+    Memory beyond the results: a copy of x's rows (in fp32 of x and weight, as three bf16 parts, 6 bytes a value; of
+    16-bit weights only if their rows do not begin at 16-byte boundaries), kept for the backward pass where that
+    computes the logits again.  During a pass that computes gradients 0.6 GB at most up to a million words (fp32: 349000),
+    an fp32 copy of the weight's gradient, and with the loss a second copy of the rows of x that are worked on at a time
+    (2^28 / V and 65536 at most).  For 16 fp32 tokens or less: the logits.
 
     Both passes may be captured into CUDA graphs, on leaves that no living eager graph holds.  There are
     no second derivatives."""
