@@ -16,8 +16,8 @@
 // backward pass from values that are there anyway instead of stored (4 bytes a row each way: 3 % of
 // the traffic of rows of 64).  The weight's gradient is a sum over all rows: each thread keeps its
 // columns' sums in registers over the rows that its group walks, the CTA adds its groups in order
-// and leaves one row of partial sums, and a second kernel adds those in order: no atomics, the same
-// bits every time.
+// and leaves one row of partial sums, and a second kernel adds those in order (both in 64 bits): no
+// atomics, the same bits every time.
 #include <algorithm>
 #include <type_traits>
 
@@ -81,7 +81,7 @@ __device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float v)
     reinterpret_cast<__half*>(p)[i] = from_f<__half>(v);
 }
 
-// sig(g) with the MUFU exponential and reciprocal (relative error a few 1e-7)
+// sig(g) with the MUFU exponential and reciprocal: a few units of 2^-23, and |g| of 2^-24 from the rounded exponent
 __device__ __forceinline__ float sig_(float g) { return rcpf_(1.0f + ex2f_(g * kNegLog2e)); }
 
 struct NormArgs {
@@ -296,10 +296,10 @@ __global__ void __launch_bounds__(kThreads, resident<NV, GATED, BWD>()) norm_row
         for (int e = 0; e < E; ++e) acc[group * W + (v * G + lane) * E + e] = e % 2 ? dw[v][e / 2].y : dw[v][e / 2].x;
       __syncthreads();
       for (int c = threadIdx.x; c < N; c += kThreads) {
-        float t = 0.f;
+        double t = 0.0;
 #pragma unroll 4
         for (int i = 0; i < kGroups; ++i) t += acc[i * W + c];
-        pr[c] = t;
+        pr[c] = (float)t;
       }
     }
   }
@@ -420,10 +420,10 @@ __global__ void __launch_bounds__(kThreads) norm_some_kernel(const NormArgs a) {
     if constexpr (kGroups > 1) {
       __syncthreads();
       for (int c = threadIdx.x; c < N; c += kThreads) {
-        float t = 0.f;
+        double t = 0.0;
 #pragma unroll
         for (int i = 0; i < kGroups; ++i) t += sums[i * N + c];
-        pr[c] = t;
+        pr[c] = (float)t;
       }
     }
   }
@@ -481,24 +481,26 @@ __global__ void __launch_bounds__(kThreads) norm_long_kernel(const NormArgs a) {
   }
 }
 
-// dw[c] = the sum of part[0 .. parts)[c], in that order within each of 32 runs, the runs in order.
+// dw[c] = the sum of part[0 .. parts)[c], in that order within each of 32 runs, the runs in order; in 64 bits, as where a
+// CTA's groups are added: a sum of a few hundred rows is off by its terms' roundings and its own alone (512 x 256 in
+// fp32: 6.8e-8, 1.3e-7 with 32).
 __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* __restrict__ part, int parts, int N,
                                                        void* __restrict__ dw, int w_dtype) {
-  __shared__ float sums[32][33];
+  __shared__ double sums[32][33];
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int cx = threadIdx.x & 31, py = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
   const int run = (parts + 31) / 32, p1 = min(parts, (py + 1) * run);
-  float t = 0.f;
+  double t = 0.0;
   if (c < N)
 #pragma unroll 8
     for (int p = py * run; p < p1; ++p) t += part[(int64_t)p * N + c];
   sums[py][cx] = t;
   __syncthreads();
   if (py == 0 && c < N) {
-    t = 0.f;
+    t = 0.0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) t += sums[i][cx];
-    store_as(dw, w_dtype, c, t);
+    store_as(dw, w_dtype, c, (float)t);
   }
 }
 
