@@ -530,10 +530,12 @@ __host__ __device__ __forceinline__ int64_t range_owner(int64_t t, int64_t tiles
 
 // 16-bit operands' exponentials are 2^(s log2 e - m), one multiply-add each, with m = top log2 e rounded: what that
 // rounding takes off is the same for a whole row, and is put back where the row's sum or divisor leaves.  (Left out, a
-// loss is off by half a unit of m: 4e-5 for logits near 1000.)
+// loss is off by half a unit of m: 4e-5 for logits near 1000.)  From 2^29 on (a label masked with the type's lowest value),
+// where m loses more than 32 or is not finite, neighbouring numbers are 64 apart: next to the largest logit nothing
+// counts, in any base, and in base 2 the exponent s - top is exact.
+constexpr float kFarTop = 536870912.0f;
 __device__ __forceinline__ float lost_of(float top) {
-  const float m = __fmul_rn(top, kLog2e);
-  return fabsf(m) < INFINITY ? fmaf(top, kLog2e, -m) : 0.f;
+  return fabsf(top) < kFarTop ? fmaf(top, kLog2e, -__fmul_rn(top, kLog2e)) : 0.f;
 }
 
 // LONG (fp32, more than 512 features): the sums leave the tensor cores in parts, so one tile has all of the TMEM and the
@@ -655,18 +657,20 @@ __global__ void __launch_bounds__(kThreads, 1) scores_kernel(const __grid_consta
           t8[j] = fmaxf(t8[j], z[8 * j + 7]);
         }
         const float now = fmax3(fmax3(t8[0], t8[1], t8[2]), fmax3(t8[3], t8[4], t8[5]), fmaxf(t8[6], t8[7]));
-        const bool raise = MODE == kLoss ? now > top : mine && now > top + kFar;  // (rows behind the last hold anything)
+        // (from a million on m loses bits that exponentials of 66 have no room for)
+        const float reach = P == 1 && fabsf(top) >= 1048576.0f ? 0.f : kFar;
+        const bool raise = MODE == kLoss ? now > top : mine && now > top + reach;  // (rows behind the last hold anything)
         if (__any_sync(0xffffffffu, raise) && raise) {
-          // (0 from a reference of -inf)
-          sum *= ex2f_(P == 1 ? __fsub_rn(__fmul_rn(top, kLog2e), __fmul_rn(now, kLog2e)) : (top - now) * kLog2e);
+          sum *= ex2f_((top - now) * kLog2e + (P == 1 ? lost_of(now) - lost_of(top) : 0.f));  // 0 from -inf
           top = now;
           if (MODE == kOnce) *a.flag = 1;
         }
       }
       // (s - top) log2 e: for 16-bit operands as one multiply-add (`lost_of`)
       const float ref = MODE != kAgain && top == -INFINITY ? 0.f : top;  // (kOnce: the label's logit may be -inf)
-      const float2 c2 = make_float2(kLog2e, kLog2e), n2 = make_float2(-ref, -ref);
-      const float2 m2 = make_float2(-ref * kLog2e, -ref * kLog2e), i2 = make_float2(inv, inv);
+      const float c1 = P == 1 && fabsf(ref) >= kFarTop ? 1.f : kLog2e, m = -ref * c1;
+      const float2 c2 = make_float2(c1, c1), n2 = make_float2(-ref, -ref);
+      const float2 m2 = make_float2(m, m), i2 = make_float2(inv, inv);
       float2 acc[4] = {};
 #pragma unroll
       for (int i = 0; i < 64; i += 2) {

@@ -294,3 +294,60 @@ def test_weight_gradients_past_32_bits():
     dw, = torch.autograd.grad(ops.linear_cross_entropy(x, w, label, reduction='sum'), w)
     want, = torch.autograd.grad(ops.linear_cross_entropy(x[-600:], w, label[-600:], reduction='sum'), w)
     assert torch.equal(dw, want)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize('N,V', [(40, 300), (40, 257), (9, 300)])
+@pytest.mark.parametrize('low', [-2.0e3, -6.0e4, -1e8, -1e10, -1e20, None])
+def test_a_label_that_is_masked_with_a_low_value(dtype, N, V, low):
+    """Its loss is what it is below the others, to the rounding of that number, with or without gradients; these are those
+    of a label 100 below."""
+    low = torch.finfo(dtype).min if low is None else low
+    if abs(low) > torch.finfo(dtype).max:
+        pytest.skip('not a number of this type')
+    g = torch.Generator(device='cuda').manual_seed(V)
+    x = torch.randn(N, 64, device='cuda', generator=g)
+    x[:, 0] = 1
+    x = x.to(dtype)
+    w = torch.randn(V, 64, device='cuda', generator=g) * 0.2
+    w[:, 0] = 0
+    far, label = V - 1, torch.randint(0, V - 1, (N,), device='cuda', generator=g)
+    label[::3] = far
+    w = w.to(dtype)
+    w[far, 0] = -1000
+    want = gradients(x, w, label)
+    w[far, 0] = low
+    s = x.double() @ w.double().t()
+    exact = s.logsumexp(1) - s[torch.arange(N), label]
+    for reduction in ('none', 'sum', 'mean'):
+        with torch.no_grad():
+            alone = ops.linear_cross_entropy(x, w, label, reduction=reduction)
+        got = gradients(x, w, label, reduction)
+        there = {'none': exact, 'sum': exact.sum(), 'mean': exact.mean()}[reduction]
+        over = there.abs() > torch.finfo(torch.float32).max
+        for loss in (alone, got[0]):
+            assert torch.equal(loss.isinf(), over) and not loss.isnan().any()
+            # sums of 64 products (the one of the label's is as it is) and of V exponentials: far below 1e-5
+            assert ((loss.double() - there).abs() <= 1e-5 + 1e-6 * there.abs())[~over].all()
+        assert all(t.isfinite().all() for t in got[1:])
+        if reduction == 'mean':
+            assert torch.equal(got[2], want[2]) and torch.equal(got[1][:, 1:], want[1][:, 1:])
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('size', [1e5, 2e6, 1e9, 1e12, 1e30])
+def test_logits_of_any_size(dtype, size):
+    """One word in eight is far above the others, by the same amount for all of them: their logits are equal, so a loss is
+    the logarithm of their number for their own labels."""
+    for N in (40, 9):
+        x = torch.zeros(N, 64, device='cuda', dtype=dtype)
+        w = torch.zeros(304, 64, device='cuda', dtype=dtype)
+        x[:, 0], w[::8, 0] = 1, size
+        label = torch.arange(N, device='cuda') * 8 % 304
+        for reduction in ('none', 'mean'):
+            loss, dx, dw = gradients(x, w, label, reduction)
+            with torch.no_grad():
+                alone = ops.linear_cross_entropy(x, w, label, reduction=reduction)
+            want = torch.full_like(loss, 38).log()
+            assert ((loss - want).abs() <= 1e-5).all() and ((alone - want).abs() <= 1e-5).all(), (loss, alone)
+            assert dx.isfinite().all() and dw.isfinite().all()
