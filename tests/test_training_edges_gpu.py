@@ -296,15 +296,15 @@ def test_weight_gradients_past_32_bits():
     assert torch.equal(dw, want)
 
 
-@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
+LOW = [(dtype, low) for dtype in (torch.bfloat16, torch.float16, torch.float32)
+       for low in (-2.0e3, -6.0e4, -1e8, -1e10, -1e20, torch.finfo(dtype).min) if low >= torch.finfo(dtype).min]
+
+
+@pytest.mark.parametrize('dtype,low', LOW)
 @pytest.mark.parametrize('N,V', [(40, 300), (40, 257), (9, 300)])
-@pytest.mark.parametrize('low', [-2.0e3, -6.0e4, -1e8, -1e10, -1e20, None])
 def test_a_label_that_is_masked_with_a_low_value(dtype, N, V, low):
     """Its loss is what it is below the others, to the rounding of that number, with or without gradients; these are those
     of a label 100 below."""
-    low = torch.finfo(dtype).min if low is None else low
-    if abs(low) > torch.finfo(dtype).max:
-        pytest.skip('not a number of this type')
     g = torch.Generator(device='cuda').manual_seed(V)
     x = torch.randn(N, 64, device='cuda', generator=g)
     x[:, 0] = 1
