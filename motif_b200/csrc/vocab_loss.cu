@@ -893,7 +893,7 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const JoinArgs a) 
 // from the tiles, like the others' (the tensor cores cut sums off, which moves large logits by 4e-7 of
 // themselves; between logits of one size it cancels).  In bf16 the divisor also takes back the rounding of the
 // label's place, the largest part of G: without that, the error of dx was 1.4 times as large.  (The row's other words, which
-are as much together but less each, carry it instead, on top of the rounding of their own.)  A warp a row.
+// are as much together but less each, carry it instead, on top of the rounding of their own.)  A warp a row.
 struct SettleArgs {
   const int* count;
   int* ticket;
